@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <chrono>
 #include <thread>
 
@@ -44,19 +45,37 @@ g4a_status g4a_check_launch(const char* what) {
   return G4A_OK;
 }
 
+g4a_device_guard::g4a_device_guard(const g4a_ctx* ctx) {
+  int cur = -1;
+  cudaError_t e = cudaGetDevice(&cur);
+  if (e == cudaSuccess && cur != ctx->device) {
+    e = cudaSetDevice(ctx->device);
+    if (e == cudaSuccess) prev = cur;
+  }
+  if (e != cudaSuccess) status = g4a_cuda_fail(e, "making the context's device current");
+}
+
+g4a_device_guard::~g4a_device_guard() {
+  if (prev >= 0) cudaSetDevice(prev);
+}
+
 g4a_status g4a_ensure_workspace(g4a_ctx* ctx, size_t bytes) {
   if (bytes <= ctx->workspace_bytes) return G4A_OK;
-  // Growing must not free memory that queued kernels still read.
-  G4A_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-  if (ctx->workspace) {
-    cudaFree(ctx->workspace);
-    ctx->workspace = nullptr;
-    ctx->workspace_bytes = 0;
-  }
-  size_t want = bytes < (size_t)(1u << 20) ? (size_t)(1u << 20) : bytes;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  G4A_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &capturing));
+  if (capturing != cudaStreamCaptureStatusNone)
+    return g4a_fail(G4A_EINVAL,
+                    "the workspace has to grow to %zu bytes, which a stream capture does not allow: make one call of "
+                    "this shape before capturing",
+                    bytes);
+  // The old workspace is kept until the context goes: queued kernels, and graphs captured from
+  // earlier calls, still use it.  Each growth at least doubles it, so what is kept stays below
+  // the size of the last one.
+  const size_t want = std::max({bytes, (size_t)1 << 20, 2 * ctx->workspace_bytes});
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, want);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaMalloc(workspace)");
+  if (ctx->workspace) ctx->old_workspaces.push_back(ctx->workspace);
   ctx->workspace = p;
   ctx->workspace_bytes = want;
   return G4A_OK;
@@ -64,7 +83,8 @@ g4a_status g4a_ensure_workspace(g4a_ctx* ctx, size_t bytes) {
 
 const char* const g4a_prof_names[G4A_PROF_NUM_LABELS] = {
     "norm_rope", "rms_norm_no_weight", "kv_store", "decode_prep", "decode_splitkv",
-    "decode_merge", "decode_generic", "lse_merge", "prefill_prep", "prefill_attn", "matmul"};
+    "decode_merge", "decode_generic", "lse_merge", "prefill_prep", "prefill_attn", "matmul",
+    "rope_table", "paged_prep", "paged_compact", "tree_attn", "tree_merge", "token_logprobs"};
 
 static cudaEvent_t prof_event(g4a_ctx* ctx) {
   if (!ctx->prof_free.empty()) {
@@ -202,6 +222,7 @@ g4a_status g4a_destroy(g4a_ctx* ctx) {
   }
   for (auto e : ctx->prof_free) cudaEventDestroy(e);
   if (ctx->workspace) cudaFree(ctx->workspace);
+  for (void* w : ctx->old_workspaces) cudaFree(w);
   if (ctx->seq_lens) cudaFree(ctx->seq_lens);
   if (ctx->sync_event) cudaEventDestroy(ctx->sync_event);
   if (ctx->dev_err_host) cudaFreeHost((void*)ctx->dev_err_host);
@@ -247,6 +268,9 @@ g4a_status g4a_sync(g4a_ctx* ctx, uint32_t timeout_ms) {
     return g4a_fail(G4A_ETIMEOUT, "g4a_sync: a kernel reported device error code %d (%s)", derr,
                     derr == G4A_DEVERR_PAGE        ? "page id out of range, row skipped"
                     : derr == G4A_DEVERR_KVLEN     ? "kv_len beyond page-table capacity, capped"
+                    : derr == G4A_DEVERR_SLOT      ? "sequence index, slot or path entry out of range, skipped"
+                    : derr == G4A_DEVERR_TREE      ? "q_indptr and kv_lens of a sequence do not fit, sequence skipped"
+                    : derr == G4A_DEVERR_TOKEN     ? "token id beyond the vocabulary, NaN written"
                     : derr == G4A_DEVERR_WAIT_PEER ? "a peer's split-KV partial did not arrive, output zeroed"
                                                    : "bounded wait gave up");
   }

@@ -25,6 +25,12 @@ enum g4a_prof_label : int {
   G4A_PROF_PREFILL_PREP,
   G4A_PROF_PREFILL_ATTN,
   G4A_PROF_MATMUL,
+  G4A_PROF_ROPE_TABLE,
+  G4A_PROF_PAGED_PREP,
+  G4A_PROF_PAGED_COMPACT,
+  G4A_PROF_TREE_ATTN,
+  G4A_PROF_TREE_MERGE,
+  G4A_PROF_TOKEN_LOGPROBS,
   G4A_PROF_NUM_LABELS
 };
 extern const char* const g4a_prof_names[G4A_PROF_NUM_LABELS];
@@ -46,6 +52,7 @@ struct g4a_ctx {
   // ranges.  Grown on demand by the decode entry points (or once by g4a_reserve_workspace).
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
+  std::vector<void*> old_workspaces;  // outgrown ones, which captured graphs may still use
   // Per-token kv lengths of a prefill that runs through the decode kernels (grown on demand).
   int* seq_lens = nullptr;
   size_t seq_lens_cap = 0;
@@ -78,6 +85,14 @@ struct g4a_prof_scope {
   cudaEvent_t end = nullptr;
   g4a_prof_scope(g4a_ctx* c, int l);
   ~g4a_prof_scope();
+};
+
+// Makes the context's device current for the length of a call and puts the caller's back.
+struct g4a_device_guard {
+  int prev = -1;
+  g4a_status status = G4A_OK;
+  explicit g4a_device_guard(const g4a_ctx* ctx);
+  ~g4a_device_guard();
 };
 
 // Per-thread last-error message (set by every failing entry point).
@@ -116,6 +131,9 @@ enum : int {
   G4A_DEVERR_WAIT_PEER = 5,   // a peer's exchange flag did not arrive in time
   G4A_DEVERR_KVLEN = 16,      // kv_lens[b] exceeded the page table's capacity (capped)
   G4A_DEVERR_PAGE = 17,       // page id out of [0, num_pages) (row skipped)
+  G4A_DEVERR_SLOT = 18,       // a sequence index, slot or path entry out of range (skipped)
+  G4A_DEVERR_TREE = 19,       // q_indptr / kv_lens of a sequence do not fit together (sequence skipped)
+  G4A_DEVERR_TOKEN = 20,      // a token id beyond the vocabulary (NaN written)
 };
 
 // ----------------------------------------------------------------------------- device side

@@ -1,0 +1,387 @@
+// Log probabilities, entropy and top alternatives of logit rows (no reference counterpart: the
+// reference samples on the host from the logits it reads back).
+//
+// Over one row, y = c tanh(x / c) (or x), m = max y, S = sum e^(y - m), T = sum (y - m) e^(y - m):
+//   log p(t) = y_t - m - ln S,   H = ln S - T / S.
+// All three fold over parts of the row: a part's S and T are rescaled to a larger m by
+// S' = w S, T' = w (T + (m - m') S), w = e^(m - m').  So one pass over the logits is enough, split
+// over as many CTAs as the batch leaves free; a second kernel joins the parts of a row.
+//
+// Top k.  Values are ranked by 64-bit keys (order-preserving bits of x above the complement of the
+// id), so no two are equal and ties go to the lower id.  Each CTA keeps its k largest in shared
+// memory, sorted.  A tile of the row can only add values above the k-th of them, which after the
+// first tiles is rare (k ln n expected over n values); one compare per thread and tile (its
+// maximum, which the softmax needs anyway) and one block-wide count tell.  When more than k threads
+// hold such a value, the k-th largest of the 256 thread maxima is a second lower bound: k values
+// at least that large exist.  Then at most k threads append, so the list is bounded by
+// k + k * (values per thread) for any input, equal values included.
+#include "g4a_internal.cuh"
+
+namespace {
+
+constexpr int kThreadsL = 256;
+constexpr int kMaxTop = G4A_MAX_TOP_K;
+constexpr int kEpt = 16;                                   // values per thread and tile
+constexpr int kTile = kThreadsL * kEpt;
+constexpr int kList = kMaxTop + kMaxTop * kEpt;            // appended values of a tile + the kept ones
+constexpr int kMaxSplit = kThreadsL;                       // parts of a row: one thread each in the join
+constexpr float kLog2eL = 1.4426950408889634f;
+constexpr float kLn2L = 0.6931471805599453f;
+
+struct LogprobParams {
+  const void* logits;
+  const int* tokens;
+  size_t row_stride;
+  uint32_t rows, vocab, split, part;  // part: values of a row per CTA (a multiple of kTile)
+  int tokens_per_row, top_k;
+  float cap, inv_cap2;  // inv_cap2 = 2 log2(e) / cap
+  float4* stats;        // [rows, split] (m, S, T)
+  uint64_t* keys;       // [rows, split, top_k], sorted, 0 = none
+  float *logprob, *entropy, *top_logprob;
+  int* top_ids;
+  int* err;
+};
+
+// Order-preserving bits: larger floats give larger words, -0 = +0, NaN below everything.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return x != x ? 0u : b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t o) {
+  if (o == 0u) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t id) {
+  return ((uint64_t)ordered(x) << 32) | (0xffffffffu - id);
+}
+
+// c tanh(x / c) = c (1 - 2 / (e^(2x/c) + 1)); the exponential's overflow and underflow give +-c.
+// The absolute error is a few ulp of c, a few 1e-6 at c = 30: the size of a logit's own rounding.
+// -inf (a banned token, and the filler of values outside the row) stays -inf.
+__device__ __forceinline__ float capped(float x, float cap, float inv_cap2) {
+  const float e = g4a::fast_exp2(x * inv_cap2);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
+  const float y = fmaf(-2.0f * cap, r, cap);
+  return x == -INFINITY ? -INFINITY : y;
+}
+
+struct Stat {
+  float m, s, t;  // t in log2 units: sum (y - m) log2(e) e^(y - m)
+};
+__device__ __forceinline__ Stat join(const Stat a, const Stat b) {
+  const float m = fmaxf(a.m, b.m);
+  Stat r = {m, 0.f, 0.f};
+  // a part with nothing in it (m = -inf) has s = t = 0 unless it met a NaN, which has to stay
+  const float da = a.m == -INFINITY ? 0.f : (a.m - m) * kLog2eL, db = b.m == -INFINITY ? 0.f : (b.m - m) * kLog2eL;
+  const float wa = exp2f(da), wb = exp2f(db);
+  r.s = wa * a.s + wb * b.s;
+  r.t = (wa > 0.f ? wa * (a.t + da * a.s) : 0.f) + (wb > 0.f ? wb * (b.t + db * b.s) : 0.f);
+  return r;
+}
+__device__ __forceinline__ Stat block_join(Stat x, Stat* red) {
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    const Stat y = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.s, o),
+                    __shfl_xor_sync(0xffffffffu, x.t, o)};
+    x = join(x, y);
+  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = red[0];
+#pragma unroll
+  for (int w = 1; w < kThreadsL / 32; w++) x = join(x, red[w]);
+  return x;
+}
+
+// Sorts the n keys of `list` by rank (they are distinct) and leaves the k largest, sorted, in
+// `out` (0 where there are fewer).  All threads; n <= 1024 or so.
+__device__ __forceinline__ void keep_top(const uint64_t* list, int n, int k, uint64_t* out) {
+  for (int i = threadIdx.x; i < n; i += kThreadsL) {
+    const uint64_t x = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += list[j] > x;
+    if (rank < k) out[rank] = x;
+  }
+  if (n < k)
+    for (int i = n + threadIdx.x; i < k; i += kThreadsL) out[i] = 0;
+}
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[4]) {
+    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = g4a::h2_to_f2(w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+};
+
+// One part of one row: CTA (row, part).  A tile is 256 threads x 16 values in 16-byte loads from
+// the aligned address at or before the row's start; a load that reaches over either end of the
+// part is made value by value, so nothing outside the row is read.
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
+  constexpr int VN = Vec<T>::N, NV = kEpt / VN;
+  __shared__ Stat red[kThreadsL / 32];
+  __shared__ uint64_t list[kList], kept[kMaxTop], tops[kThreadsL];
+  __shared__ uint64_t bound;
+  __shared__ int count;
+  const uint32_t row = blockIdx.x / p.split, part = blockIdx.x - row * p.split;
+  const int k = p.top_k, tid = threadIdx.x;
+  g4a::pdl_wait_primary();
+  g4a::pdl_launch_dependents();
+  const T* x0 = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride;
+  // ids are counted from the aligned address; ids below `head` lie before the row
+  const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(x0) & 15u) / sizeof(T));
+  const T* base = x0 - head;
+  const uint32_t lo = max(part * p.part, head);
+  const uint32_t hi = min(part * p.part + p.part, p.vocab + head);
+  if (tid < kMaxTop) kept[tid] = 0;
+  if (tid == 0) count = 0;
+  Stat st = {-INFINITY, 0.f, 0.f};
+  int have = 0;            // kept values (uniform)
+  uint64_t thr = 0;        // the k-th of them
+  __syncthreads();
+  for (uint32_t t0 = part * p.part; t0 < hi; t0 += kTile) {
+    float x[kEpt];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      const uint32_t i0 = t0 + (uint32_t)(j * kThreadsL + tid) * VN;
+      float v[VN];
+      if (i0 >= lo && i0 + VN <= hi) {
+        Vec<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(base + i0)), v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VN; e++)
+          v[e] = (i0 + e >= lo && i0 + e < hi) ? Vec<T>::one(base + i0 + e) : -INFINITY;
+      }
+#pragma unroll
+      for (int e = 0; e < VN; e++) x[j * VN + e] = v[e];
+    }
+    float top = x[0];
+#pragma unroll
+    for (int e = 1; e < kEpt; e++) top = fmaxf(top, x[e]);  // NaN is passed over
+    const float ym = CAP ? capped(top, p.cap, p.inv_cap2) : top;
+    const float m = fmaxf(st.m, ym);
+    const float ml = (m == -INFINITY ? 0.f : m) * kLog2eL;
+    if (m > st.m) {
+      const float d = st.m == -INFINITY ? 0.f : (st.m - m) * kLog2eL, w = g4a::fast_exp2(d);
+      st.t = w * (st.t + d * st.s);
+      st.s *= w;
+      st.m = m;
+    }
+#pragma unroll
+    for (int e = 0; e < kEpt; e++) {
+      const float y = CAP ? capped(x[e], p.cap, p.inv_cap2) : x[e];
+      const float d = fmaf(y, kLog2eL, -ml);
+      const float w = g4a::fast_exp2(d);
+      st.s += w;
+      st.t = fmaf(fmaxf(d, -1000.f), w, st.t);  // -inf: -1000 * 0
+    }
+    if (k == 0) continue;
+    // which threads hold values above the k-th kept one
+    auto id_of = [&](int e) { return t0 + (uint32_t)((e / VN) * kThreadsL + tid) * VN + (uint32_t)(e % VN); };
+    auto valid = [&](int e) { const uint32_t i = id_of(e); return i >= lo && i < hi; };
+    uint64_t best = 0;
+    const uint32_t thr_hi = (uint32_t)(thr >> 32);
+    // below a full list every value counts, NaN (ordered 0) included
+    if (have < k || ordered(top) >= thr_hi) {
+#pragma unroll
+      for (int e = 0; e < kEpt; e++)
+        if (valid(e)) {
+          const uint64_t key = make_key(x[e], id_of(e) - head);
+          if (key > best) best = key;
+        }
+      if (have >= k && best <= thr) best = 0;
+    }
+    const int n_hold = __syncthreads_count(best != 0);
+    if (n_hold == 0) continue;
+    uint64_t lim = have < k ? 1 : thr + 1;
+    if (n_hold > k) {
+      tops[tid] = best;
+      __syncthreads();
+      if (best != 0) {
+        int rank = 0;
+        for (int j = 0; j < kThreadsL; j++) rank += tops[j] > best;
+        if (rank == k - 1) bound = best;
+      }
+      __syncthreads();
+      lim = max(lim, bound);
+    }
+    if (best >= lim && best != 0) {
+#pragma unroll
+      for (int e = 0; e < kEpt; e++)
+        if (valid(e)) {
+          const uint64_t key = make_key(x[e], id_of(e) - head);
+          if (key >= lim) list[atomicAdd(&count, 1)] = key;
+        }
+    }
+    if (tid < have) list[kList - 1 - tid] = kept[tid];  // the kept ones at the other end
+    __syncthreads();
+    const int n = count;
+    // gather both ends into one run (positions n .. n + have - 1)
+    uint64_t mine = tid < have ? list[kList - 1 - tid] : 0;
+    __syncthreads();
+    if (tid < have) list[n + tid] = mine;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    keep_top(list, n + have, k, kept);
+    __syncthreads();
+    have = min(n + have, k);
+    thr = kept[k - 1];
+  }
+  st = block_join(st, red);
+  const size_t slot = (size_t)row * p.split + part;
+  if (tid == 0) p.stats[slot] = make_float4(st.m, st.s, st.t, 0.f);
+  if (tid < k) p.keys[slot * k + tid] = kept[tid];
+}
+
+// Joins the parts of one row (at most one per thread).  The k-th largest of the parts' maxima
+// bounds the row's k-th value from below, so at most k parts, k values each, are candidates.
+template <typename T>
+__global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobParams p) {
+  __shared__ Stat red[kThreadsL / 32];
+  __shared__ uint64_t list[kMaxTop * kMaxTop], tops[kThreadsL], kept[kMaxTop];
+  __shared__ uint64_t bound;
+  __shared__ int count;
+  const uint32_t row = blockIdx.x;
+  const int tid = threadIdx.x, k = p.top_k, ns = (int)p.split;
+  g4a::pdl_wait_primary();
+  g4a::pdl_launch_dependents();
+  Stat st = {-INFINITY, 0.f, 0.f};
+  if (tid < ns) {
+    const float4 f = p.stats[(size_t)row * ns + tid];
+    st = {f.x, f.y, f.z};
+  }
+  const uint64_t* keys = p.keys + (size_t)row * ns * k;
+  if (k) {
+    tops[tid] = tid < ns ? keys[(size_t)tid * k] : 0;
+    if (tid == 0) count = 0, bound = 0;
+  }
+  st = block_join(st, red);  // (a barrier inside)
+  const float ln_s = logf(st.s);
+  const float cap = p.cap;
+  if (p.entropy && tid == 0) p.entropy[row] = ln_s - kLn2L * st.t / st.s;
+  for (int j = tid; j < p.tokens_per_row; j += kThreadsL) {
+    const int tok = p.tokens[(size_t)row * p.tokens_per_row + j];
+    float lp = 0.f;
+    if (tok >= 0 && (uint32_t)tok < p.vocab) {
+      const float x = Vec<T>::one(reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride + tok);
+      lp = (cap > 0.f ? capped(x, cap, p.inv_cap2) : x) - st.m - ln_s;
+    } else if (tok != -1) {
+      lp = __uint_as_float(0x7fc00000u);
+      atomicExch(p.err, G4A_DEVERR_TOKEN);
+    }
+    p.logprob[(size_t)row * p.tokens_per_row + j] = lp;
+  }
+  if (k == 0) return;
+  if (ns > k) {
+    const uint64_t mine = tops[tid];
+    if (mine != 0) {
+      int rank = 0;
+      for (int j = 0; j < ns; j++) rank += tops[j] > mine;
+      if (rank == k - 1) bound = mine;
+    }
+    __syncthreads();
+  }
+  const uint64_t lim = max(bound, (uint64_t)1);
+  if (tid < ns && tops[tid] >= lim)
+    for (int j = 0; j < k; j++) {
+      const uint64_t key = keys[(size_t)tid * k + j];
+      if (key < lim) break;
+      list[atomicAdd(&count, 1)] = key;
+    }
+  __syncthreads();
+  keep_top(list, count, k, kept);
+  __syncthreads();
+  if (tid < k) {
+    const uint64_t key = kept[tid];
+    const float x = from_ordered((uint32_t)(key >> 32));
+    p.top_ids[(size_t)row * k + tid] = (int)(0xffffffffu - (uint32_t)key);
+    p.top_logprob[(size_t)row * k + tid] = (cap > 0.f ? capped(x, cap, p.inv_cap2) : x) - st.m - ln_s;
+  }
+}
+
+template <typename T>
+g4a_status launch_logprobs(g4a_ctx* ctx, LogprobParams& p) {
+  // parts of a row: enough CTAs to fill the SMs several times over, whole tiles each
+  const uint32_t tiles = (p.vocab + 8 + kTile - 1) / kTile;  // + the values before an unaligned row
+  const uint32_t want = (uint32_t)(ctx->num_sms * 16);
+  uint32_t split = (want + p.rows - 1) / p.rows;
+  split = split < 1 ? 1 : split > tiles ? tiles : split;
+  if (split > (uint32_t)kMaxSplit) split = kMaxSplit;
+  const uint32_t per = (tiles + split - 1) / split;
+  p.split = (tiles + per - 1) / per;
+  p.part = per * kTile;
+  if ((uint64_t)p.rows * p.split > 0x7fffffffull)
+    return g4a_fail(G4A_EINVAL, "g4a_token_logprobs: rows %u too many", p.rows);
+  const size_t parts = (size_t)p.rows * p.split;
+  if (g4a_status s = g4a_ensure_workspace(ctx, parts * (sizeof(float4) + (size_t)p.top_k * sizeof(uint64_t)))) return s;
+  p.stats = static_cast<float4*>(ctx->workspace);
+  p.keys = reinterpret_cast<uint64_t*>(p.stats + parts);
+  g4a_prof_scope ps(ctx, G4A_PROF_TOKEN_LOGPROBS);
+  cudaError_t e = g4a_launch(p.cap > 0.f ? logprob_part_kernel<T, true> : logprob_part_kernel<T, false>,
+                             dim3((unsigned)parts), dim3(kThreadsL), 0, ctx->stream, true, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch logprob_part_kernel");
+  e = g4a_launch(logprob_join_kernel<T>, dim3(p.rows), dim3(kThreadsL), 0, ctx->stream, true, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch logprob_join_kernel");
+  return G4A_OK;
+}
+
+}  // namespace
+
+extern "C" g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint32_t format, const int32_t* tokens,
+                                         uint32_t rows, uint32_t vocab, uint64_t row_stride, uint32_t tokens_per_row,
+                                         uint32_t top_k, float softcap, float* logprob, float* entropy,
+                                         float* top_logprob, int32_t* top_ids) {
+  G4A_CHECK_CTX(ctx);
+  const char* fn = "g4a_token_logprobs";
+  if (format != G4A_ACT_F32 && format != G4A_ACT_F16) return g4a_fail(G4A_EINVAL, "%s: unknown format %u", fn, format);
+  if (rows == 0) return G4A_OK;
+  if (!logits) return g4a_fail(G4A_EINVAL, "%s: null logits", fn);
+  if (rows > 0x7fffffffu) return g4a_fail(G4A_EINVAL, "%s: rows %u too many", fn, rows);
+  if (vocab == 0 || vocab > 0x7ffff000u) return g4a_fail(G4A_EINVAL, "%s: vocab %u out of range", fn, vocab);
+  if (row_stride == 0) row_stride = vocab;
+  if (row_stride < vocab) return g4a_fail(G4A_EINVAL, "%s: row_stride below vocab %u", fn, vocab);
+  if ((uintptr_t)logits & (format == G4A_ACT_F32 ? 3u : 1u)) return g4a_fail(G4A_EINVAL, "%s: unaligned logits", fn);
+  if (top_k > (uint32_t)kMaxTop || top_k > vocab)
+    return g4a_fail(G4A_EINVAL, "%s: top_k %u exceeds %d or vocab %u", fn, top_k, kMaxTop, vocab);
+  if (tokens_per_row > 0x7fffffffu) return g4a_fail(G4A_EINVAL, "%s: tokens_per_row out of range", fn);
+  if (tokens_per_row && (!tokens || !logprob)) return g4a_fail(G4A_EINVAL, "%s: null tokens or logprob", fn);
+  if (top_k && (!top_logprob || !top_ids)) return g4a_fail(G4A_EINVAL, "%s: null top_logprob or top_ids", fn);
+  if (!(softcap >= 0.f) || softcap > 1e30f) return g4a_fail(G4A_EINVAL, "%s: softcap must be >= 0 and finite", fn);
+  if (tokens_per_row == 0 && !entropy && top_k == 0) return G4A_OK;
+  g4a_device_guard dev(ctx);
+  if (dev.status != G4A_OK) return dev.status;
+  LogprobParams p = {};
+  p.logits = logits;
+  p.tokens = tokens;
+  p.row_stride = row_stride;
+  p.rows = rows;
+  p.vocab = vocab;
+  p.tokens_per_row = (int)tokens_per_row;
+  p.top_k = (int)top_k;
+  p.cap = softcap;
+  p.inv_cap2 = softcap > 0.f ? 2.0f * kLog2eL / softcap : 0.f;
+  p.logprob = logprob;
+  p.entropy = entropy;
+  p.top_logprob = top_logprob;
+  p.top_ids = top_ids;
+  p.err = ctx->dev_err_dev;
+  return format == G4A_ACT_F16 ? launch_logprobs<__half>(ctx, p) : launch_logprobs<float>(ctx, p);
+}

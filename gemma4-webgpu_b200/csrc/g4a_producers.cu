@@ -311,6 +311,28 @@ __global__ void __launch_bounds__(1024) prefill_prep_kernel(const float* q, cons
   g4a::pdl_launch_dependents();
 }
 
+// cos and sin of every token's RoPE angles, with the arithmetic of norm_rope_head: row i holds the
+// cosines of its hd/2 pairs, then their sines.  A forward pass calls it once per (theta, divisor)
+// and every layer of that kind reads the rows, so the double-precision sincos are not repeated per
+// layer and head.  A negative position (padding) gives the row of position 0.
+__global__ void __launch_bounds__(kWG) rope_table_kernel(const int* positions, const __half* rope_freqs,
+                                                          float* cos_sin, int hd,
+                                                          const __grid_constant__ RopePow tab, uint32_t apply_div) {
+  g4a::pdl_wait_primary();
+  g4a::pdl_launch_dependents();
+  const int half_dim = hd / 2;
+  const int pos = positions[blockIdx.x];
+  const float posf = __uint2float_rn((uint32_t)(pos < 0 ? 0 : pos));
+  float* row = cos_sin + (size_t)blockIdx.x * hd;
+  for (int p = threadIdx.x; p < half_dim; p += blockDim.x) {
+    const float angle = __fmul_rn(posf, rope_freq(p, tab, rope_freqs, apply_div));
+    double s, c;
+    sincos((double)angle, &s, &c);
+    row[p] = __double2float_rn(c);
+    row[half_dim + p] = __double2float_rn(s);
+  }
+}
+
 g4a_status check_head_dim(const char* fn, uint32_t hd, bool need_even) {
   if (hd == 0 || hd > (uint32_t)kMaxHeadDim)
     return g4a_fail(G4A_EINVAL, "%s: head_dim %u not in [1, %d]", fn, hd, kMaxHeadDim);
@@ -360,6 +382,26 @@ g4a_status g4a_kv_store(g4a_ctx* ctx, const float* k, float* v, uint16_t* k_cach
   kv_store_kernel<<<num_kv_heads, kWG, 0, ctx->stream>>>(k, v, (__half*)k_cache, (__half*)v_cache, (int)num_kv_heads,
                                                          (int)head_dim, slot, eps, fuse_v_norm ? 1 : 0);
   return g4a_check_launch("kv_store_kernel");
+}
+
+g4a_status g4a_rope_table(g4a_ctx* ctx, const int32_t* positions, const uint16_t* rope_freqs, float* cos_sin,
+                          uint32_t num_tokens, uint32_t head_dim, float theta, uint32_t apply_divisor) {
+  G4A_CHECK_CTX(ctx);
+  if (g4a_status s = check_head_dim(__func__, head_dim, true)) return s;
+  if (num_tokens == 0) return G4A_OK;
+  if (num_tokens > 0x7fffffffu) return g4a_fail(G4A_EINVAL, "g4a_rope_table: num_tokens %u too large", num_tokens);
+  if (!positions || !cos_sin) return g4a_fail(G4A_EINVAL, "g4a_rope_table: null positions or cos_sin");
+  if (apply_divisor && !rope_freqs)
+    return g4a_fail(G4A_EINVAL, "g4a_rope_table: apply_divisor set but rope_freqs is null");
+  g4a_device_guard dev(ctx);
+  if (dev.status != G4A_OK) return dev.status;
+  g4a_prof_scope ps(ctx, G4A_PROF_ROPE_TABLE);
+  const uint32_t threads = head_dim / 2 <= 64 ? 64u : head_dim / 2 <= 128 ? 128u : (uint32_t)kWG;
+  const cudaError_t e = g4a_launch(rope_table_kernel, dim3(num_tokens), dim3(threads), 0, ctx->stream, true, positions,
+                                   (const __half*)rope_freqs, cos_sin, (int)head_dim, make_rope_pow(theta, head_dim),
+                                   apply_divisor);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch rope_table_kernel");
+  return G4A_OK;
 }
 
 g4a_status g4a_prefill_qkv_prep(g4a_ctx* ctx, const float* q, const float* k, const float* v,

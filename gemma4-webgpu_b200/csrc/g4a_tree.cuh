@@ -1,0 +1,146 @@
+// What the kernels of g4a_tree_attn_paged share: the work partition and the visibility rules.
+#pragma once
+
+#include "g4a_internal.cuh"
+
+namespace g4a_tree {
+
+constexpr int kMaxTokens = 64;  // drafted tokens of a sequence (bits of a tree mask)
+constexpr float kLog2eT = 1.4426950408889634f;
+
+struct TreeParams {
+  const void* q;  // [tokens, nqh, hd] f32 or f16
+  void* out;
+  const __half *k, *v;  // page pools [num_pages, page_size, nkh, hd]
+  const int *page_table, *kv_lens, *q_indptr;
+  const unsigned long long* mask;  // per token, or null (chain)
+  int tokens, batch, max_tokens;
+  int page_size, max_pages, num_pages;
+  int nqh, nkh, group, hd;  // group = nqh / nkh
+  float scale_log2;         // scale * log2(e)
+  uint32_t window;
+  int rows, kps;  // query rows of a tile, keys of a stage (of the launched kernel)
+  int grid;       // CTAs of the launched kernel
+  float* part;    // [2 * grid] partial rows: o [rows, hd_pad] | m [rows] | l [rows]
+  int hd_pad;
+  int* err;
+};
+
+// One sequence: T drafted tokens (rows row0 .. of q), base older rows, keys [lo, L) to be read.
+// T = 0: nothing to do (also for a sequence that does not fit together, which is reported).
+struct Seq {
+  int row0, T, base, L, lo;
+  int tiles;   // query tiles of one kv head
+  int stages;  // key stages of one tile
+};
+
+__device__ __forceinline__ Seq seq_of(const TreeParams& p, int b) {
+  Seq s = {};
+  const int r0 = p.q_indptr[b], r1 = p.q_indptr[b + 1], L = p.kv_lens[b];
+  const long long cap = (long long)p.max_pages * p.page_size;
+  if (r0 < 0 || r1 < r0 || r1 > p.tokens || r1 - r0 > p.max_tokens || L < r1 - r0 || L > cap) {
+    atomicExch(p.err, G4A_DEVERR_TREE);
+    return s;
+  }
+  s.row0 = r0;
+  s.T = r1 - r0;
+  s.L = L;
+  s.base = L - s.T;
+  // the earliest key any token's window can reach (a token that sees itself alone: base + 1 - W;
+  // one whose mask is empty: base - W)
+  s.lo = (p.window != 0u && (uint32_t)s.base > p.window) ? s.base - (int)p.window : 0;
+  s.tiles = (s.T * p.group + p.rows - 1) / p.rows;
+  s.stages = s.tiles > 0 ? (L - s.lo + p.kps - 1) / p.kps : 0;
+  return s;
+}
+
+__device__ __forceinline__ long long stages_of(const TreeParams& p, const Seq& s) {
+  return (long long)p.nkh * s.tiles * s.stages;
+}
+
+// The flattened list of (sequence, kv head, tile, stage) is cut into equal runs, one per CTA;
+// only the first min(grid, total) CTAs have work.
+struct Split {
+  long long total, active, each, extra;
+  __device__ __forceinline__ void of(long long t, int grid) {
+    total = t;
+    active = grid < t ? grid : t;
+    each = active ? t / active : 0;
+    extra = active ? t % active : 0;
+  }
+  __device__ __forceinline__ long long begin(long long c) const { return c * each + (c < extra ? c : extra); }
+  // the CTA whose run holds stage s
+  __device__ __forceinline__ long long owner(long long s) const {
+    const long long cut = extra * (each + 1);
+    return s < cut ? s / (each + 1) : extra + (s - cut) / each;
+  }
+};
+
+// Total stages over the batch, by one full warp (every lane returns it).
+__device__ __forceinline__ long long total_stages(const TreeParams& p) {
+  long long n = 0;
+  for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += stages_of(p, seq_of(p, b));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+
+// The sequence that holds flattened stage s (s < total) and the first stage of that sequence; one
+// full warp, every lane returns them.
+__device__ __forceinline__ int find_seq(const TreeParams& p, long long s, long long& first) {
+  const int lane = threadIdx.x & 31;
+  long long acc = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const long long n = b < p.batch ? stages_of(p, seq_of(p, b)) : 0;
+    long long incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const long long start = acc + incl - n;
+    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && s >= start && s < start + n);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      first = __shfl_sync(0xffffffffu, start, src);
+      return b0 + src;
+    }
+    acc += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  first = acc;
+  return p.batch;
+}
+
+// What query row r of a tile's sequence sees: prefix rows [kmin, base) and the drafted rows of
+// `bits`.  Of the base + popcount(mask) rows in its list only the last W stay.
+struct Sees {
+  int kmin;
+  unsigned long long bits;
+};
+__device__ __forceinline__ Sees sees_of(const TreeParams& p, const Seq& s, int token) {
+  const unsigned long long all = s.T >= 64 ? ~0ull : (1ull << s.T) - 1ull;
+  unsigned long long m = p.mask ? p.mask[s.row0 + token] & all : (token >= 63 ? ~0ull : (2ull << token) - 1ull);
+  Sees v = {0, m};
+  if (p.window != 0u) {
+    const int n = s.base + __popcll(m);
+    int drop = (uint32_t)n > p.window ? n - (int)p.window : 0;  // of the list's first rows
+    v.kmin = drop < s.base ? drop : s.base;
+    for (drop -= v.kmin; drop > 0; drop--) m &= m - 1;
+    v.bits = m;
+  }
+  return v;
+}
+
+// Element offset of cache row `key` of sequence b and kv head kvh, or -1 for a bad page id.
+__device__ __forceinline__ long long row_offset(const TreeParams& p, int b, int kvh, int key) {
+  const int j = key / p.page_size;
+  const int page = p.page_table[(size_t)b * p.max_pages + j];
+  if (page < 0 || page >= p.num_pages) {
+    atomicExch(p.err, G4A_DEVERR_PAGE);
+    return -1;
+  }
+  return (((long long)page * p.page_size + (key - j * p.page_size)) * p.nkh + kvh) * p.hd;
+}
+
+}  // namespace g4a_tree

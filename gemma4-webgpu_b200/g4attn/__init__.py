@@ -64,6 +64,42 @@ def _check(t, name, dtype, numel=None, device=None):
         raise ValueError(f"{name} is on cuda:{t.device.index}, context is on cuda:{device}")
 
 
+def _fmt(t, name) -> int:
+    import torch
+
+    if t.dtype == torch.float32:
+        return _lib.ACT_F32
+    if t.dtype == torch.float16:
+        return _lib.ACT_F16
+    raise TypeError(f"{name} must be torch.float32 or torch.float16, got {t.dtype}")
+
+
+def _check_rows(t, name, dtype, width, device) -> tuple[int, int]:
+    """(rows, row stride in elements) of a tensor whose rows are `width` packed elements."""
+    import torch
+
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, context is on cuda:{device}")
+    if t.dim() == 2:
+        rows, n, packed = t.shape[0], t.shape[1], t.stride(1) == 1 or t.shape[1] <= 1
+    elif t.dim() == 3:
+        rows, n = t.shape[0], t.shape[1] * t.shape[2]
+        packed = (t.stride(2) == 1 or t.shape[2] <= 1) and (t.stride(1) == t.shape[2] or t.shape[1] <= 1)
+    else:
+        raise ValueError(f"{name} must be [rows, width] or [rows, heads, head_dim]")
+    if n != width or not packed:
+        raise ValueError(f"{name} must have rows of {width} packed elements, got shape {tuple(t.shape)} with strides "
+                         f"{t.stride()}")
+    stride = t.stride(0) if rows > 1 else width
+    if stride < width:
+        raise ValueError(f"{name} has overlapping rows (stride {stride})")
+    return rows, stride
+
+
 class Context:
     """One libg4attn context: a CUDA device, a stream and the split-KV workspace.
 
@@ -257,6 +293,140 @@ class Context:
              _ptr(v_cache), num_q_heads, num_kv_heads, head_dim, float(eps), int(position), int(slot), int(kv_len),
              int(max_seq_len), float(theta), int(apply_divisor), float(scale), int(sliding_window),
              int(is_producer))
+
+    # ---------------------------------------------------------------- speculative step, paged cache
+    def rope_table(self, positions, rope_freqs, cos_sin, *, head_dim, theta, apply_divisor=0) -> None:
+        """cos and sin of the tokens' RoPE angles (g4a_rope_table), once per step for all layers."""
+        import torch
+
+        n = positions.numel()
+        _check(positions, "positions", torch.int32, None, self.device)
+        _check(cos_sin, "cos_sin", torch.float32, n * head_dim, self.device)
+        if apply_divisor:
+            _check(rope_freqs, "rope_freqs", torch.float16, head_dim // 2, self.device)
+        call("g4a_rope_table", self._h, _ptr(positions), _ptr(rope_freqs), _ptr(cos_sin), n, head_dim, float(theta),
+             int(apply_divisor))
+
+    def _pages(self, k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size):
+        """Checks a page pool and its table; returns (batch, max_pages_per_seq, num_pages)."""
+        import torch
+
+        _check(k_pages, "k_pages", torch.float16, None, self.device)
+        _check(v_pages, "v_pages", torch.float16, k_pages.numel(), self.device)
+        _check(page_table, "page_table", torch.int32, None, self.device)
+        if page_table.dim() != 2:
+            raise ValueError("page_table must be [batch, max_pages_per_seq]")
+        per_page = page_size * num_kv_heads * head_dim
+        if per_page <= 0 or k_pages.numel() < per_page:
+            raise ValueError(f"k_pages has {k_pages.numel()} elements, one page takes {per_page}")
+        return page_table.shape[0], page_table.shape[1], k_pages.numel() // per_page
+
+    def paged_qkv_prep(self, q, k, v, q_norm_w, k_norm_w, cos_sin, q_out, k_pages, v_pages, page_table, token_seq,
+                       slots, *, num_q_heads, num_kv_heads, head_dim, page_size, eps) -> None:
+        """New tokens of a batch: q / k norm + RoPE, v norm, append to the paged cache
+        (g4a_paged_qkv_prep).  q, k and v may be row-strided (columns of one projection's output);
+        k = v = None computes q alone."""
+        import torch
+
+        n = token_seq.numel()
+        _check(token_seq, "token_seq", torch.int32, None, self.device)
+        _check(cos_sin, "cos_sin", torch.float32, n * head_dim, self.device)
+        qs = ks = fmt = 0
+        if num_q_heads:
+            rows, qs = _check_rows(q, "q", torch.float32, num_q_heads * head_dim, self.device)
+            if rows < n:
+                raise ValueError(f"q has {rows} rows, needs {n}")
+            _check(q_norm_w, "q_norm_w", torch.float16, head_dim, self.device)
+            fmt = _fmt(q_out, "q_out")
+            _check(q_out, "q_out", q_out.dtype, n * num_q_heads * head_dim, self.device)
+        batch = max_pages = num_pages = 0
+        if page_table is not None:
+            batch, max_pages = page_table.shape[0], page_table.shape[-1]
+        if k is not None or v is not None:
+            rows, ks = _check_rows(k, "k", torch.float32, num_kv_heads * head_dim, self.device)
+            vrows, vs = _check_rows(v, "v", torch.float32, num_kv_heads * head_dim, self.device)
+            if min(rows, vrows) < n:
+                raise ValueError(f"k and v have {rows} and {vrows} rows, need {n}")
+            if ks != vs and n > 1:
+                raise ValueError(f"k and v must have one row stride, got {ks} and {vs}")
+            _check(k_norm_w, "k_norm_w", torch.float16, head_dim, self.device)
+            _check(slots, "slots", torch.int32, n, self.device)
+            batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
+        call("g4a_paged_qkv_prep", self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos_sin),
+             _ptr(q_out), fmt, _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(token_seq), _ptr(slots), n, batch,
+             page_size, max_pages, num_pages, num_q_heads, num_kv_heads, head_dim, qs, ks, float(eps))
+
+    def tree_attn_paged(self, q, k_pages, v_pages, page_table, kv_lens, q_indptr, tree_mask, out, *, num_q_heads,
+                        num_kv_heads, head_dim, page_size, max_tokens, scale=1.0, sliding_window=0,
+                        host_kv_lens=None) -> None:
+        """Attention of drafted tokens (a tree per sequence, or a chain with tree_mask None) over the
+        paged cache (g4a_tree_attn_paged).  tree_mask is int64, one word of ancestor bits per token."""
+        import numpy as np
+        import torch
+
+        batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
+        fmt = _fmt(q, "q")
+        _check(q, "q", q.dtype, None, self.device)
+        n = q.shape[0]
+        if q.numel() != n * num_q_heads * head_dim:
+            raise ValueError(f"q must be [tokens, {num_q_heads}, {head_dim}], got {tuple(q.shape)}")
+        _check(out, "out", q.dtype, q.numel(), self.device)
+        _check(kv_lens, "kv_lens", torch.int32, batch, self.device)
+        _check(q_indptr, "q_indptr", torch.int32, batch + 1, self.device)
+        if tree_mask is not None:
+            _check(tree_mask, "tree_mask", torch.int64, n, self.device)
+        hl = c_void_p(None)
+        if host_kv_lens is not None:
+            arr = np.ascontiguousarray(np.asarray(host_kv_lens, dtype=np.int32))
+            if arr.size != batch:
+                raise ValueError("host_kv_lens must have one entry per sequence")
+            hl = c_void_p(arr.ctypes.data)
+        call("g4a_tree_attn_paged", self._h, _ptr(q), fmt, _ptr(k_pages), _ptr(v_pages), _ptr(page_table),
+             _ptr(kv_lens), hl, _ptr(q_indptr), _ptr(tree_mask), n, batch, int(max_tokens), page_size, max_pages,
+             num_pages, num_q_heads, num_kv_heads, head_dim, float(scale), int(sliding_window), _ptr(out))
+
+    def token_logprobs(self, logits, tokens, logprob, entropy=None, top_logprob=None, top_ids=None, *,
+                       softcap=0.0) -> None:
+        """Log probabilities of given tokens, entropy and top alternatives of rows of logits
+        (g4a_token_logprobs).  logits [rows, vocab] f32 or f16, row-strided; tokens and logprob
+        [rows, n] (both None: left out); top_logprob and top_ids [rows, k]."""
+        import torch
+
+        if logits.dim() != 2:
+            raise ValueError("logits must be [rows, vocab]")
+        fmt = _fmt(logits, "logits")
+        rows, stride = _check_rows(logits, "logits", logits.dtype, logits.shape[1], self.device)
+        per_row = top_k = 0
+        if tokens is not None:
+            if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+                raise ValueError(f"tokens must be [{rows}] or [{rows}, n]")
+            per_row = tokens.shape[1] if tokens.dim() == 2 else 1
+            _check(tokens, "tokens", torch.int32, None, self.device)
+            _check(logprob, "logprob", torch.float32, rows * per_row, self.device)
+        if entropy is not None:
+            _check(entropy, "entropy", torch.float32, rows, self.device)
+        if top_ids is not None or top_logprob is not None:
+            if top_ids is None or top_ids.dim() != 2 or top_ids.shape[0] != rows:
+                raise ValueError(f"top_ids must be [{rows}, k]")
+            top_k = top_ids.shape[1]
+            _check(top_ids, "top_ids", torch.int32, None, self.device)
+            _check(top_logprob, "top_logprob", torch.float32, rows * top_k, self.device)
+        call("g4a_token_logprobs", self._h, _ptr(logits), fmt, _ptr(tokens), rows, logits.shape[1], stride, per_row,
+             top_k, float(softcap), _ptr(logprob), _ptr(entropy), _ptr(top_logprob), _ptr(top_ids))
+
+    def paged_kv_compact(self, k_pages, v_pages, page_table, base_lens, path, path_lens, *, num_kv_heads, head_dim,
+                         page_size) -> None:
+        """Rows base + path[i] of each sequence become rows base + i (g4a_paged_kv_compact)."""
+        import torch
+
+        batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
+        _check(base_lens, "base_lens", torch.int32, batch, self.device)
+        _check(path_lens, "path_lens", torch.int32, batch, self.device)
+        _check(path, "path", torch.int32, None, self.device)
+        if path.dim() != 2 or path.shape[0] != batch:
+            raise ValueError(f"path must be [{batch}, max_path]")
+        call("g4a_paged_kv_compact", self._h, _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(base_lens),
+             _ptr(path), _ptr(path_lens), batch, path.shape[1], page_size, max_pages, num_pages, num_kv_heads, head_dim)
 
     # ---------------------------------------------------------------- memory and IPC
     def alloc(self, nbytes: int) -> int:

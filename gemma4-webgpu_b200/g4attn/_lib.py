@@ -35,6 +35,8 @@ class G4AError(RuntimeError):
         super().__init__(f"{func}: {self.status_name}: {message}")
 
 
+ACT_F32, ACT_F16 = 0, 1  # G4A_ACT_*: formats of queries, outputs and logits
+MAX_TOP_K = 32  # G4A_MAX_TOP_K
 WEIGHT_F16, WEIGHT_Q8, WEIGHT_Q4K = 0, 1, 2  # G4A_WEIGHT_* of g4a_matmul
 MATMUL_MAX_JOBS = 4
 DIST_ID_BYTES = 128  # G4A_DIST_ID_BYTES
@@ -48,6 +50,7 @@ class MatmulJob(ctypes.Structure):
 
 # (name, argtypes) for every g4a_status entry point.
 _u32 = c_uint32
+_u64 = c_size_t  # uint64_t
 _f = c_float
 _p = c_void_p
 SIGNATURES: dict[str, list] = {
@@ -80,6 +83,11 @@ SIGNATURES: dict[str, list] = {
     "g4a_prefill_qkv_prep": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _u32, _f, _f,
                              _u32],
     "g4a_prefill_attn": [_p, _p, _p, _p, _p, _u32, _u32, _u32, _u32, _u32, _f, _u32],
+    "g4a_rope_table": [_p, _p, _p, _p, _u32, _u32, _f, _u32],
+    "g4a_paged_qkv_prep": [_p] * 8 + [_u32] + [_p] * 5 + [_u32] * 10 + [_f],
+    "g4a_tree_attn_paged": [_p, _p, _u32] + [_p] * 7 + [_u32] * 9 + [_f, _u32, _p],
+    "g4a_token_logprobs": [_p, _p, _u32, _p, _u32, _u32, _u64, _u32, _u32, _f, _p, _p, _p, _p],
+    "g4a_paged_kv_compact": [_p] * 7 + [_u32] * 7,
     "g4a_ipc_get_handle": [_p, _p, _p],
     "g4a_ipc_open_handle": [_p, _p, POINTER(c_void_p)],
     "g4a_ipc_close_handle": [_p, _p],

@@ -97,7 +97,8 @@ g4a_status g4a_reserve_workspace(g4a_ctx* ctx, uint32_t max_batch, uint32_t head
 /* Per-kernel profiler: when enabled, every kernel launch is bracketed by CUDA events and its
  * device time is summed per label ("norm_rope", "rms_norm_no_weight", "kv_store",
  * "decode_prep", "decode_splitkv", "decode_merge", "decode_generic", "lse_merge",
- * "prefill_prep", "prefill_attn", "matmul").  Counterpart of the reference's per-pass timestamp
+ * "prefill_prep", "prefill_attn", "matmul", "rope_table", "paged_prep", "paged_compact",
+ * "tree_attn", "tree_merge", "token_logprobs").  Counterpart of the reference's per-pass timestamp
  * queries (src/engine.ts:3208-3285, src/diagnostics/profile.ts:48-132).  Reading waits for
  * the context's stream.  Leave it off for timing whole steps: the events serialise launches. */
 g4a_status g4a_profile_enable(g4a_ctx* ctx, int enable);
@@ -378,6 +379,108 @@ typedef struct {
 } g4a_matmul_job;
 g4a_status g4a_matmul_group(g4a_ctx* ctx, uint32_t weight_format, const float* input, uint32_t N,
                             const g4a_matmul_job* jobs, uint32_t num_jobs);
+
+/* ------------------------------------------------------------------ speculative step, paged cache */
+
+/* One step of speculative decoding over the paged cache of g4a_decode_attn_paged (no reference
+ * counterpart: the reference decodes one token of one sequence).  A draft proposes a tree of up
+ * to 64 tokens per sequence; the target model then runs all of them at once:
+ *   once per step   g4a_rope_table        the tokens' rotation angles, for every layer
+ *   per layer       g4a_paged_qkv_prep    norms, rotation, k and v appended to the pages
+ *                   g4a_tree_attn_paged   every token over the prefix and its own ancestors
+ *   after lm-head   g4a_token_logprobs    what the target thinks of the proposed tokens
+ *   per cache       g4a_paged_kv_compact  the accepted path's rows moved together
+ * Formats of activations (queries, outputs, logits): */
+#define G4A_ACT_F32 0u
+#define G4A_ACT_F16 1u
+
+/* cos and sin of the RoPE angles of num_tokens tokens: row i of cos_sin (f32 [num_tokens,
+ * head_dim]) holds cos of the head_dim/2 pairs at positions[i], then their sin.  The values are
+ * those that g4a_norm_rope turns its pairs by, to the bit (theta, rope_freqs and apply_divisor as
+ * there), so rows cached by either can be mixed.  A negative position counts as 0. */
+g4a_status g4a_rope_table(g4a_ctx* ctx, const int32_t* positions, const uint16_t* rope_freqs,
+                          float* cos_sin, uint32_t num_tokens, uint32_t head_dim, float theta,
+                          uint32_t apply_divisor);
+
+/* New tokens of a batch into the paged cache: q and k heads get RMSNorm with their f16 weight and
+ * the rotation, v heads the weightless RMSNorm; k and v are rounded to f16 and stored.  Decode
+ * steps (one token per sequence), trees and prompt chunks of unequal length are all just tokens.
+ * q is f32 [num_tokens, num_q_heads, head_dim] with q_row_stride elements from token to token, k
+ * and v f32 [num_tokens, num_kv_heads, head_dim] with kv_row_stride (0: packed), so the three may
+ * be columns of one projection's output; they are left as they are.  q_out is packed, f32 or f16
+ * (q_out_format).  Token i belongs to sequence token_seq[i] in [0, batch) and is stored in row
+ * slots[i] of it: page page_table[token_seq[i]*max_pages_per_seq + slots[i]/page_size], row
+ * slots[i]%page_size.  token_seq[i] < 0 is padding: nothing of the token is read or written.
+ * slots[i] < 0 stores nothing but computes q.  The (sequence, slot) pairs of one call must be
+ * distinct.  A sequence index, slot or page id out of range is not stored and g4a_sync reports
+ * it.  k = v = NULL (a layer that reads another layer's cache) computes q alone; num_q_heads = 0
+ * stores k and v alone.  cos_sin as from g4a_rope_table.  head_dim a multiple of 8, <= 512. */
+g4a_status g4a_paged_qkv_prep(g4a_ctx* ctx, const float* q, const float* k, const float* v,
+                              const uint16_t* q_norm_w, const uint16_t* k_norm_w, const float* cos_sin,
+                              void* q_out, uint32_t q_out_format, uint16_t* k_pages, uint16_t* v_pages,
+                              const int32_t* page_table, const int32_t* token_seq, const int32_t* slots,
+                              uint32_t num_tokens, uint32_t batch, uint32_t page_size,
+                              uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_q_heads,
+                              uint32_t num_kv_heads, uint32_t head_dim, uint32_t q_row_stride,
+                              uint32_t kv_row_stride, float eps);
+
+/* Attention of drafted tokens over the paged cache.  Sequence b's tokens are rows q_indptr[b] ..
+ * q_indptr[b+1]-1 of q and out ([num_tokens, num_q_heads, head_dim], both f32 or both f16 as
+ * `format` says), T of them; its cache holds kv_lens[b] rows, the last T of which are these
+ * tokens' own (stored before the call, token j in row base + j, base = kv_lens[b] - T).  Token i
+ * attends to rows [0, base) and to the drafted tokens j whose bit is set in tree_mask[q_indptr[b]
+ * + i] (bit j, 64-bit words, one per token: its ancestors and itself); tree_mask NULL is a chain,
+ * every token seeing the earlier ones and itself.  sliding_window W > 0 keeps the last W of these
+ * rows in the order of the row index, which is g4a_decode_attn's window for a token at
+ * position base + (ancestors).  A token that sees nothing gets zeros.  f32 queries keep f32
+ * accuracy (as g4a_decode_attn); f16 queries round the softmax weights to f16.
+ * kv head of q head h is h*num_kv_heads/num_q_heads; num_q_heads must be a multiple of
+ * num_kv_heads.  max_tokens (1..64) bounds T for every sequence.  q_indptr, kv_lens, page_table
+ * and tree_mask are device arrays; host_kv_lens (may be NULL) is an optional host copy used only
+ * to size the launch.  A sequence whose q_indptr is not increasing within [0, num_tokens], with T
+ * > max_tokens, kv_lens[b] < T or kv_lens[b] beyond max_pages_per_seq*page_size is skipped (its
+ * rows of out stay as they were) and g4a_sync reports it; so do page ids out of range, whose rows
+ * count as not there.  Rows of out behind the last sequence stay as they were.  A value that is
+ * not finite in a row of the cache reaches only the tokens that attend to that row.  The partial
+ * results live in the context's workspace: before capturing the call into a graph, make one of
+ * the same shape, and do not let graphs captured from one context run at the same time. */
+g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t format, const uint16_t* k_pages,
+                               const uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                               const int32_t* host_kv_lens, const int32_t* q_indptr,
+                               const uint64_t* tree_mask, uint32_t num_tokens, uint32_t batch,
+                               uint32_t max_tokens, uint32_t page_size, uint32_t max_pages_per_seq,
+                               uint32_t num_pages, uint32_t num_q_heads, uint32_t num_kv_heads,
+                               uint32_t head_dim, float scale, uint32_t sliding_window, void* out);
+
+/* Log probabilities under rows of logits ([rows, vocab] f32 or f16, row_stride elements from row
+ * to row, 0: packed).  softcap c > 0 first caps every logit, y = c tanh(x / c) (Gemma's final
+ * logit cap; -inf stays -inf); 0 leaves y = x.  With Z = sum exp(y):
+ *   logprob [rows, tokens_per_row]  y[tokens[r, j]] - log Z of tokens (int32, same shape); token
+ *                                   -1 (none) gives 0, another id beyond the vocabulary NaN, which
+ *                                   g4a_sync reports
+ *   entropy [rows]                  log Z - sum y exp(y) / Z (a logit of -inf adds nothing)
+ *   top_logprob, top_ids [rows, top_k]  the largest logits in falling order, the lower id first
+ *                                   among equal ones, top_k <= 32 and <= vocab
+ * logprob / tokens (tokens_per_row 0), entropy (NULL) and the top arrays (top_k 0) may each be
+ * left out.  A row with a NaN or +inf, or with no finite logit, has NaN probabilities; a NaN ranks
+ * below -inf.  Sums are held in f32.  One call per row count before capturing it into a graph
+ * (the partial sums live in the context's workspace). */
+#define G4A_MAX_TOP_K 32
+g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint32_t format, const int32_t* tokens,
+                              uint32_t rows, uint32_t vocab, uint64_t row_stride,
+                              uint32_t tokens_per_row, uint32_t top_k, float softcap, float* logprob,
+                              float* entropy, float* top_logprob, int32_t* top_ids);
+
+/* Moves the cache rows of an accepted path together: for each sequence b and i < path_lens[b],
+ * row base_lens[b] + path[b*max_path + i] becomes row base_lens[b] + i of k_pages and v_pages, as
+ * if all rows were read before any is written.  path (device, int32 [batch, max_path]) holds
+ * indices of drafted tokens, max_path <= 64.  Entries out of range are skipped and reported by
+ * g4a_sync, as are sequences with path_lens[b] > max_path or a negative base. */
+g4a_status g4a_paged_kv_compact(g4a_ctx* ctx, uint16_t* k_pages, uint16_t* v_pages,
+                                const int32_t* page_table, const int32_t* base_lens, const int32_t* path,
+                                const int32_t* path_lens, uint32_t batch, uint32_t max_path,
+                                uint32_t page_size, uint32_t max_pages_per_seq, uint32_t num_pages,
+                                uint32_t num_kv_heads, uint32_t head_dim);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop
