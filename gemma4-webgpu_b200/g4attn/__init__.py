@@ -64,40 +64,72 @@ def _check(t, name, dtype, numel=None, device=None):
         raise ValueError(f"{name} is on cuda:{t.device.index}, context is on cuda:{device}")
 
 
+def _addr(t, name, dtype, numel, device) -> int:
+    """The address of a contiguous CUDA tensor of at least `numel` elements on the context's device.
+    One comparison of four properties on the way that every call takes (a small step's calls cost
+    their host time); _check then says what is wrong."""
+    try:
+        if t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= numel:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _check(t, name, dtype, numel, device)
+    return t.data_ptr()
+
+
 def _fmt(t, name) -> int:
-    import torch
-
-    if t.dtype == torch.float32:
-        return _lib.ACT_F32
-    if t.dtype == torch.float16:
-        return _lib.ACT_F16
-    raise TypeError(f"{name} must be torch.float32 or torch.float16, got {t.dtype}")
+    f = _formats().get(getattr(t, "dtype", None))
+    if f is None:
+        raise TypeError(f"{name} must be a torch.float32 or torch.float16 tensor")
+    return f
 
 
-def _check_rows(t, name, dtype, width, device) -> tuple[int, int]:
-    """(rows, row stride in elements) of a tensor whose rows are `width` packed elements."""
+_formats_of: dict = {}
+
+
+def _formats() -> dict:
+    if not _formats_of:
+        import torch
+
+        _formats_of.update({torch.float32: _lib.ACT_F32, torch.float16: _lib.ACT_F16})
+    return _formats_of
+
+
+def _rows_addr(t, name, dtype, width, device) -> tuple[int, int, int]:
+    """(address, rows, row stride in elements) of a tensor whose rows are `width` packed elements."""
     import torch
 
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_cuda or t.device.index != device:
+    if t.get_device() != device:
         raise ValueError(f"{name} is on {t.device}, context is on cuda:{device}")
-    if t.dim() == 2:
-        rows, n, packed = t.shape[0], t.shape[1], t.stride(1) == 1 or t.shape[1] <= 1
-    elif t.dim() == 3:
-        rows, n = t.shape[0], t.shape[1] * t.shape[2]
-        packed = (t.stride(2) == 1 or t.shape[2] <= 1) and (t.stride(1) == t.shape[2] or t.shape[1] <= 1)
+    shape, st = t.shape, t.stride()
+    if len(shape) == 2:
+        n, packed = shape[1], st[1] == 1 or shape[1] <= 1
+    elif len(shape) == 3:
+        n = shape[1] * shape[2]
+        packed = (st[2] == 1 or shape[2] <= 1) and (st[1] == shape[2] or shape[1] <= 1)
     else:
         raise ValueError(f"{name} must be [rows, width] or [rows, heads, head_dim]")
     if n != width or not packed:
-        raise ValueError(f"{name} must have rows of {width} packed elements, got shape {tuple(t.shape)} with strides "
-                         f"{t.stride()}")
-    stride = t.stride(0) if rows > 1 else width
+        raise ValueError(f"{name} must have rows of {width} packed elements, got shape {tuple(shape)} with strides {st}")
+    stride = st[0] if shape[0] > 1 else width
     if stride < width:
         raise ValueError(f"{name} has overlapping rows (stride {stride})")
-    return rows, stride
+    return t.data_ptr(), shape[0], stride
+
+
+def _host_lens(lens, batch):
+    import numpy as np
+
+    arr = lens
+    if not (isinstance(arr, np.ndarray) and arr.dtype == np.int32 and arr.flags.c_contiguous):
+        arr = np.ascontiguousarray(np.asarray(arr, dtype=np.int32))
+    if arr.size != batch:
+        raise ValueError("host_kv_lens must have one entry per sequence")
+    return arr
 
 
 class Context:
@@ -299,91 +331,84 @@ class Context:
         """cos and sin of the tokens' RoPE angles (g4a_rope_table), once per step for all layers."""
         import torch
 
-        n = positions.numel()
-        _check(positions, "positions", torch.int32, None, self.device)
-        _check(cos_sin, "cos_sin", torch.float32, n * head_dim, self.device)
-        if apply_divisor:
-            _check(rope_freqs, "rope_freqs", torch.float16, head_dim // 2, self.device)
-        call("g4a_rope_table", self._h, _ptr(positions), _ptr(rope_freqs), _ptr(cos_sin), n, head_dim, float(theta),
-             int(apply_divisor))
+        dev, n = self.device, positions.numel()
+        rf = _addr(rope_freqs, "rope_freqs", torch.float16, head_dim // 2, dev) if apply_divisor else None
+        call("g4a_rope_table", self._h, _addr(positions, "positions", torch.int32, 0, dev), rf,
+             _addr(cos_sin, "cos_sin", torch.float32, n * head_dim, dev), n, head_dim, theta, apply_divisor)
 
     def _pages(self, k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size):
-        """Checks a page pool and its table; returns (batch, max_pages_per_seq, num_pages)."""
+        """Checks a page pool and its table; returns their addresses and (batch, max_pages_per_seq, num_pages)."""
         import torch
 
-        _check(k_pages, "k_pages", torch.float16, None, self.device)
-        _check(v_pages, "v_pages", torch.float16, k_pages.numel(), self.device)
-        _check(page_table, "page_table", torch.int32, None, self.device)
-        if page_table.dim() != 2:
+        dev, size = self.device, k_pages.numel()
+        k = _addr(k_pages, "k_pages", torch.float16, 0, dev)
+        v = _addr(v_pages, "v_pages", torch.float16, size, dev)
+        t = _addr(page_table, "page_table", torch.int32, 0, dev)
+        shape = page_table.shape
+        if len(shape) != 2:
             raise ValueError("page_table must be [batch, max_pages_per_seq]")
         per_page = page_size * num_kv_heads * head_dim
-        if per_page <= 0 or k_pages.numel() < per_page:
-            raise ValueError(f"k_pages has {k_pages.numel()} elements, one page takes {per_page}")
-        return page_table.shape[0], page_table.shape[1], k_pages.numel() // per_page
+        if per_page <= 0 or size < per_page:
+            raise ValueError(f"k_pages has {size} elements, one page takes {per_page}")
+        return k, v, t, shape[0], shape[1], size // per_page
 
     def paged_qkv_prep(self, q, k, v, q_norm_w, k_norm_w, cos_sin, q_out, k_pages, v_pages, page_table, token_seq,
                        slots, *, num_q_heads, num_kv_heads, head_dim, page_size, eps) -> None:
         """New tokens of a batch: q / k norm + RoPE, v norm, append to the paged cache
         (g4a_paged_qkv_prep).  q, k and v may be row-strided (columns of one projection's output);
-        k = v = None computes q alone."""
+        k = v = None computes q alone, num_q_heads = 0 stores k and v alone."""
         import torch
 
-        n = token_seq.numel()
-        _check(token_seq, "token_seq", torch.int32, None, self.device)
-        _check(cos_sin, "cos_sin", torch.float32, n * head_dim, self.device)
-        qs = ks = fmt = 0
+        dev, n, f16, f32 = self.device, token_seq.numel(), torch.float16, torch.float32
+        seq = _addr(token_seq, "token_seq", torch.int32, 0, dev)
+        cs = _addr(cos_sin, "cos_sin", f32, n * head_dim, dev)
+        qp = qw = qo = kp = vp = kw = kpool = vpool = table = sl = None
+        qs = ks = fmt = batch = max_pages = num_pages = 0
         if num_q_heads:
-            rows, qs = _check_rows(q, "q", torch.float32, num_q_heads * head_dim, self.device)
+            qp, rows, qs = _rows_addr(q, "q", f32, num_q_heads * head_dim, dev)
             if rows < n:
                 raise ValueError(f"q has {rows} rows, needs {n}")
-            _check(q_norm_w, "q_norm_w", torch.float16, head_dim, self.device)
+            qw = _addr(q_norm_w, "q_norm_w", f16, head_dim, dev)
             fmt = _fmt(q_out, "q_out")
-            _check(q_out, "q_out", q_out.dtype, n * num_q_heads * head_dim, self.device)
-        batch = max_pages = num_pages = 0
-        if page_table is not None:
-            batch, max_pages = page_table.shape[0], page_table.shape[-1]
+            qo = _addr(q_out, "q_out", q_out.dtype, n * num_q_heads * head_dim, dev)
         if k is not None or v is not None:
-            rows, ks = _check_rows(k, "k", torch.float32, num_kv_heads * head_dim, self.device)
-            vrows, vs = _check_rows(v, "v", torch.float32, num_kv_heads * head_dim, self.device)
-            if min(rows, vrows) < n:
+            kp, rows, ks = _rows_addr(k, "k", f32, num_kv_heads * head_dim, dev)
+            vp, vrows, vs = _rows_addr(v, "v", f32, num_kv_heads * head_dim, dev)
+            if rows < n or vrows < n:
                 raise ValueError(f"k and v have {rows} and {vrows} rows, need {n}")
             if ks != vs and n > 1:
                 raise ValueError(f"k and v must have one row stride, got {ks} and {vs}")
-            _check(k_norm_w, "k_norm_w", torch.float16, head_dim, self.device)
-            _check(slots, "slots", torch.int32, n, self.device)
-            batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
-        call("g4a_paged_qkv_prep", self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos_sin),
-             _ptr(q_out), fmt, _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(token_seq), _ptr(slots), n, batch,
-             page_size, max_pages, num_pages, num_q_heads, num_kv_heads, head_dim, qs, ks, float(eps))
+            kw = _addr(k_norm_w, "k_norm_w", f16, head_dim, dev)
+            sl = _addr(slots, "slots", torch.int32, n, dev)
+            kpool, vpool, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads,
+                                                                           head_dim, page_size)
+        elif page_table is not None:
+            batch = page_table.shape[0]
+        else:
+            batch = 0x7fffffff  # q alone: any sequence index
+        call("g4a_paged_qkv_prep", self._h, qp, kp, vp, qw, kw, cs, qo, fmt, kpool, vpool, table, seq, sl, n, batch,
+             page_size, max_pages, num_pages, num_q_heads, num_kv_heads, head_dim, qs, ks, eps)
 
     def tree_attn_paged(self, q, k_pages, v_pages, page_table, kv_lens, q_indptr, tree_mask, out, *, num_q_heads,
                         num_kv_heads, head_dim, page_size, max_tokens, scale=1.0, sliding_window=0,
                         host_kv_lens=None) -> None:
         """Attention of drafted tokens (a tree per sequence, or a chain with tree_mask None) over the
         paged cache (g4a_tree_attn_paged).  tree_mask is int64, one word of ancestor bits per token."""
-        import numpy as np
         import torch
 
-        batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
-        fmt = _fmt(q, "q")
-        _check(q, "q", q.dtype, None, self.device)
-        n = q.shape[0]
-        if q.numel() != n * num_q_heads * head_dim:
+        dev, i32 = self.device, torch.int32
+        kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
+                                                                 page_size)
+        fmt, n, size = _fmt(q, "q"), q.shape[0], q.numel()
+        if size != n * num_q_heads * head_dim:
             raise ValueError(f"q must be [tokens, {num_q_heads}, {head_dim}], got {tuple(q.shape)}")
-        _check(out, "out", q.dtype, q.numel(), self.device)
-        _check(kv_lens, "kv_lens", torch.int32, batch, self.device)
-        _check(q_indptr, "q_indptr", torch.int32, batch + 1, self.device)
-        if tree_mask is not None:
-            _check(tree_mask, "tree_mask", torch.int64, n, self.device)
-        hl = c_void_p(None)
-        if host_kv_lens is not None:
-            arr = np.ascontiguousarray(np.asarray(host_kv_lens, dtype=np.int32))
-            if arr.size != batch:
-                raise ValueError("host_kv_lens must have one entry per sequence")
-            hl = c_void_p(arr.ctypes.data)
-        call("g4a_tree_attn_paged", self._h, _ptr(q), fmt, _ptr(k_pages), _ptr(v_pages), _ptr(page_table),
-             _ptr(kv_lens), hl, _ptr(q_indptr), _ptr(tree_mask), n, batch, int(max_tokens), page_size, max_pages,
-             num_pages, num_q_heads, num_kv_heads, head_dim, float(scale), int(sliding_window), _ptr(out))
+        mask = None if tree_mask is None else _addr(tree_mask, "tree_mask", torch.int64, n, dev)
+        lens = None if host_kv_lens is None else _host_lens(host_kv_lens, batch)
+        call("g4a_tree_attn_paged", self._h, _addr(q, "q", q.dtype, 0, dev), fmt, kp, vp, table,
+             _addr(kv_lens, "kv_lens", i32, batch, dev), None if lens is None else lens.ctypes.data,
+             _addr(q_indptr, "q_indptr", i32, batch + 1, dev), mask, n, batch, max_tokens, page_size, max_pages,
+             num_pages, num_q_heads, num_kv_heads, head_dim, scale, sliding_window,
+             _addr(out, "out", q.dtype, size, dev))
 
     def token_logprobs(self, logits, tokens, logprob, entropy=None, top_logprob=None, top_ids=None, *,
                        softcap=0.0) -> None:
@@ -392,41 +417,45 @@ class Context:
         [rows, n] (both None: left out); top_logprob and top_ids [rows, k]."""
         import torch
 
+        dev, f32 = self.device, torch.float32
+        fmt = _fmt(logits, "logits")
         if logits.dim() != 2:
             raise ValueError("logits must be [rows, vocab]")
-        fmt = _fmt(logits, "logits")
-        rows, stride = _check_rows(logits, "logits", logits.dtype, logits.shape[1], self.device)
+        vocab = logits.shape[1]
+        x, rows, stride = _rows_addr(logits, "logits", logits.dtype, vocab, dev)
         per_row = top_k = 0
+        tok = lp = ent = tv = ti = None
         if tokens is not None:
-            if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+            shape = tokens.shape
+            if len(shape) not in (1, 2) or shape[0] != rows:
                 raise ValueError(f"tokens must be [{rows}] or [{rows}, n]")
-            per_row = tokens.shape[1] if tokens.dim() == 2 else 1
-            _check(tokens, "tokens", torch.int32, None, self.device)
-            _check(logprob, "logprob", torch.float32, rows * per_row, self.device)
+            per_row = shape[1] if len(shape) == 2 else 1
+            tok = _addr(tokens, "tokens", torch.int32, 0, dev)
+            lp = _addr(logprob, "logprob", f32, rows * per_row, dev)
         if entropy is not None:
-            _check(entropy, "entropy", torch.float32, rows, self.device)
+            ent = _addr(entropy, "entropy", f32, rows, dev)
         if top_ids is not None or top_logprob is not None:
             if top_ids is None or top_ids.dim() != 2 or top_ids.shape[0] != rows:
                 raise ValueError(f"top_ids must be [{rows}, k]")
             top_k = top_ids.shape[1]
-            _check(top_ids, "top_ids", torch.int32, None, self.device)
-            _check(top_logprob, "top_logprob", torch.float32, rows * top_k, self.device)
-        call("g4a_token_logprobs", self._h, _ptr(logits), fmt, _ptr(tokens), rows, logits.shape[1], stride, per_row,
-             top_k, float(softcap), _ptr(logprob), _ptr(entropy), _ptr(top_logprob), _ptr(top_ids))
+            ti = _addr(top_ids, "top_ids", torch.int32, 0, dev)
+            tv = _addr(top_logprob, "top_logprob", f32, rows * top_k, dev)
+        call("g4a_token_logprobs", self._h, x, fmt, tok, rows, vocab, stride, per_row, top_k, softcap, lp, ent, tv, ti)
 
     def paged_kv_compact(self, k_pages, v_pages, page_table, base_lens, path, path_lens, *, num_kv_heads, head_dim,
                          page_size) -> None:
         """Rows base + path[i] of each sequence become rows base + i (g4a_paged_kv_compact)."""
         import torch
 
-        batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size)
-        _check(base_lens, "base_lens", torch.int32, batch, self.device)
-        _check(path_lens, "path_lens", torch.int32, batch, self.device)
-        _check(path, "path", torch.int32, None, self.device)
-        if path.dim() != 2 or path.shape[0] != batch:
+        dev, i32 = self.device, torch.int32
+        kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
+                                                                 page_size)
+        shape = path.shape
+        if len(shape) != 2 or shape[0] != batch:
             raise ValueError(f"path must be [{batch}, max_path]")
-        call("g4a_paged_kv_compact", self._h, _ptr(k_pages), _ptr(v_pages), _ptr(page_table), _ptr(base_lens),
-             _ptr(path), _ptr(path_lens), batch, path.shape[1], page_size, max_pages, num_pages, num_kv_heads, head_dim)
+        call("g4a_paged_kv_compact", self._h, kp, vp, table, _addr(base_lens, "base_lens", i32, batch, dev),
+             _addr(path, "path", i32, 0, dev), _addr(path_lens, "path_lens", i32, batch, dev), batch, shape[1], page_size,
+             max_pages, num_pages, num_kv_heads, head_dim)
 
     # ---------------------------------------------------------------- memory and IPC
     def alloc(self, nbytes: int) -> int:

@@ -102,22 +102,22 @@ def test_binding_checks_without_a_gpu():
     """The Python checks that need no device: dtypes, shapes and strides of row-strided tensors."""
     import torch
 
-    from g4attn import _check_rows
+    from g4attn import _rows_addr
 
     class Cuda(torch.Tensor):  # a CPU tensor that says it lives on cuda:0
-        is_cuda = True
-        device = torch.device("cuda", 0)
+        def get_device(self):
+            return 0
 
     def t(*shape, dtype=torch.float32):
         return torch.zeros(shape, dtype=dtype).as_subclass(Cuda)
 
-    assert _check_rows(t(3, 8), "x", torch.float32, 8, 0) == (3, 8)
-    assert _check_rows(t(3, 20)[:, 4:12], "x", torch.float32, 8, 0) == (3, 20)
-    assert _check_rows(t(3, 2, 4), "x", torch.float32, 8, 0) == (3, 8)
+    assert _rows_addr(t(3, 8), "x", torch.float32, 8, 0)[1:] == (3, 8)
+    assert _rows_addr(t(3, 20)[:, 4:12], "x", torch.float32, 8, 0)[1:] == (3, 20)
+    assert _rows_addr(t(3, 2, 4), "x", torch.float32, 8, 0)[1:] == (3, 8)
     for bad in (t(3, 9), t(8, 3).t(), t(3, 4, 4)[:, :2, ::2], t(1, 8).expand(3, 8)):
         with pytest.raises(ValueError):
-            _check_rows(bad, "x", torch.float32, 8, 0)
+            _rows_addr(bad, "x", torch.float32, 8, 0)
     with pytest.raises(TypeError):
-        _check_rows(t(3, 8, dtype=torch.float16), "x", torch.float32, 8, 0)
+        _rows_addr(t(3, 8, dtype=torch.float16), "x", torch.float32, 8, 0)
     with pytest.raises(ValueError):
-        _check_rows(torch.zeros(3, 8), "x", torch.float32, 8, 0)
+        _rows_addr(torch.zeros(3, 8), "x", torch.float32, 8, 0)
