@@ -23,7 +23,18 @@ struct TreeParams {
   int grid;       // CTAs of the launched kernel
   float* part;    // [2 * grid] partial rows: o [rows, hd_pad] | m [rows] | l [rows]
   int hd_pad;
+  struct Cut* cuts;  // [grid]
   int* err;
+};
+
+// A tile whose keys were cut between CTAs, written by the CTA c that has its first stages; its
+// parts are in slot `slot` (2 c or 2 c + 1) and then in slots 2 (c + 1), 2 (c + 2), ...
+struct Cut {
+  int parts;  // 0: CTA c began no such tile
+  int slot;
+  int rows;         // query rows of the tile that exist
+  int row0;         // the sequence's first row of q
+  int kvh, first;   // kv head; the tile's first row in units of (token, head of the group)
 };
 
 // One sequence: T drafted tokens (rows row0 .. of q), base older rows, keys [lo, L) to be read.

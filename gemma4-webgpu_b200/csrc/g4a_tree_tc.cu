@@ -1,0 +1,858 @@
+// The tensor-core kernel of g4a_tree_attn_paged (tcgen05 / TMEM), and why it is turned round.
+//
+// A tcgen05 MMA computes 128 x N with N from 16 up.  Here the plentiful dimension is the keys and
+// the head dims, and the query rows are few (8 to a few hundred), so the products are transposed:
+//   S^T [128 keys x N] = K [128 x hd] Q^T          A = K tile, B = the tile's queries
+//   O^T [hd x N]      += V^T [hd x 128] P^T        A = V tile (MN-major), B = P (MN-major)
+// The 128 side is always full, the work grows with the rows that exist, and at head_dim 512 the
+// accumulator of 64 rows takes 4 x 64 TMEM columns where [rows x 512] would take all 512.  TMEM
+// lane = key (scores) or head dim (output), column = query row.
+//   f16 queries: N columns are N query rows.
+//   f32 queries: N columns are N / 2 rows, first their high, then their low f16 terms (of Q and of
+//   P), so one MMA of N columns multiplies both; a thread adds a row's two columns itself.
+//
+// Bound.  An MMA of M 128, N 64, K 16 takes 48 cycles from shared memory (6 KB of operands at 128
+// B / cycle), so 64 columns over 128 keys at head_dim 512 take 3,072 cycles, while bringing those
+// keys' 256 KB at an SM's share of the HBM rate (about 23 B / cycle) takes 11,000: memory-bound up
+// to 3 tiles (192 columns) per kv head, tensor-bound beyond.
+//
+// Shared memory: Q [64-dim chunk][N][128 B], P [64-column chunk][128 keys][128 B], and a ring of
+// 32 KB units, each 128 keys x 128 dims of K or V as two [128 keys][128 B] chunks, all with the
+// 128-byte swizzle (16-byte piece k of row r at k ^ (r & 7)).
+// Warps (16, of which the last three have nothing to do):
+//   0-7    softmax: warp w has TMEM lanes 32 (w % 4) .. + 31 (keys) and the rows of half w / 4.
+//          A thread holds one key's scores for its rows.  The running maximum of a row is raised
+//          only when a score passes it by 2^8 (p = 2^(s - m + 7) <= 2^15 stays in f16): whether
+//          any does is one block-wide vote per stage; finding the maxima (a transposing reduction
+//          over the lanes and the four warps) and rescaling O in TMEM happens only then.
+//   8-11   loads: row addresses through the page table (any page size), cp.async into the ring
+//          with zero fill for rows that are not there, and the tile's queries.
+//   12     one thread issues the MMAs: S of stage i, then O of stage i - 1, so the softmax of a
+//          stage runs under the next stage's score product.
+// Every wait is bounded; a thread that gives up sets the abort flag and the error word, all waits
+// then end at once, and the CTA frees its TMEM and leaves.
+#include <algorithm>
+#include <atomic>
+
+#include "g4a_tcgen05.cuh"
+#include "g4a_tree.cuh"
+
+namespace {
+
+using namespace g4a;
+using namespace g4a_tree;
+
+constexpr int kKeysT = 128;
+constexpr int kMaxGrid = 256;        // (the join looks at one cut per thread)
+constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one with the MMA warp
+// Registers: 512 threads start with 128 each (65,536); the softmax warpgroups, which hold a row
+// block of scores and sums, take 168, the others give theirs: 256 * 168 + 128 * 96 + 128 * 72 = 64,512.
+constexpr int kRegsSoftmax = 168, kRegsLoad = 96, kRegsMma = 72;
+constexpr int kUnit = 32768;         // 128 keys x 128 dims f16
+constexpr float kPUp = 7.0f;         // p = 2^(s - m + 7)
+constexpr float kRaise = 8.0f;       // a score this far above m raises it
+constexpr float kUnseen = -1e30f;    // m of a row that has seen nothing yet (any score raises it)
+
+template <int HD, int N, bool F32>
+struct Tc {
+  static constexpr int MB = HD / 128;                 // 128-dim blocks = ring units of a K or V tile
+  static constexpr int ROWS = F32 ? N / 2 : N;        // query rows of a tile
+  static constexpr int RH = ROWS / 2;                 // rows of a softmax half
+  static constexpr int W = RH < 32 ? RH : 32;         // rows a thread works on at a time
+  static constexpr int G = RH / W;
+  static constexpr int Q_BYTES = N * HD * 2;
+  static constexpr int P_BYTES = kKeysT * N * 2;
+  static constexpr int FIT2 = (216 * 1024 - 2 * Q_BYTES - P_BYTES) / kUnit;
+  static constexpr int NQ = FIT2 >= 4 ? 2 : 1;        // query buffers
+  static constexpr int FIT = (216 * 1024 - NQ * Q_BYTES - P_BYTES) / kUnit;
+  static constexpr int UNITS = FIT > 5 ? 5 : FIT;
+  static constexpr int LAG = UNITS - 1 > 3 ? 3 : UNITS - 1;  // units in flight before the oldest is waited for
+  static constexpr int OFF_P = NQ * Q_BYTES;
+  static constexpr int OFF_RING = OFF_P + P_BYTES;
+  static constexpr int OFF_SEES = OFF_RING + UNITS * kUnit;   // [4][ROWS] Sees
+  static constexpr int OFF_SCALE = OFF_SEES + 4 * ROWS * 16;  // [4][ROWS]
+  static constexpr int OFF_U = OFF_SCALE + 4 * ROWS * 4;      // [8 warps][RH] m - 7 of its rows
+  static constexpr int OFF_F = OFF_U + 8 * RH * 4;            // [8 warps][RH] rescale factors
+  static constexpr int OFF_MAX = OFF_F + 8 * RH * 4;          // [2 halves][4 quarters][RH]
+  static constexpr int OFF_OK = OFF_MAX + 8 * RH * 4;         // [8 stages][4] which rows are there
+  static constexpr int OFF_BAD = OFF_OK + 128;                // [8] tile + 1 that had a V value that is not finite
+  static constexpr int OFF_BAR = OFF_BAD + 32;
+  static constexpr int NBARS = 2 * UNITS + 4 + 2 + 2 + 2 + 5;
+  static constexpr int OFF_END = OFF_BAR + NBARS * 8;
+  static constexpr size_t SMEM = 1024 + OFF_END + 16;
+  static constexpr uint32_t COL_O = 0, COL_S = MB * N;
+  static constexpr uint32_t TMEM_COLS = COL_S + 2 * N <= 256 ? 256u : 512u;
+  static_assert(COL_S + 2 * N <= 512 && UNITS >= 3 && UNITS >= MB && SMEM <= 232448, "tile fits");
+};
+
+template <int R>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// `count` consecutive TMEM columns of this warp's 32 lanes (count 16 or 32).
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+
+// Whether any of `count` threads (whole warps) says so; a barrier among them.
+__device__ __forceinline__ bool any_of(uint32_t id, uint32_t count, bool pred) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(count), "r"(pred ? 1u : 0u)
+      : "memory");
+  return r != 0;
+}
+
+// Reduces W values per lane over the warp's lanes, value n's result in lane n (W = 16: also in lane
+// n + 16).  Each step hands half of the values to the lane at distance o and keeps the other half.
+template <int W, typename Op>
+__device__ __forceinline__ float transpose_reduce(const float (&x)[W], Op op) {
+  const int lane = threadIdx.x & 31;
+  float v[W];
+#pragma unroll
+  for (int n = 0; n < W; n++) v[n] = x[n];
+  if constexpr (W == 16) {
+#pragma unroll
+    for (int n = 0; n < 16; n++) v[n] = op(v[n], __shfl_xor_sync(0xffffffffu, v[n], 16));
+  }
+#pragma unroll
+  for (int o = W / 2; o >= 1; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int n = 0; n < o; n++) {
+      const float give = up ? v[n] : v[n + o], keep = up ? v[n + o] : v[n];
+      v[n] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+  return v[0];
+}
+
+// Where a role stands in the CTA's run of stages.
+struct Walk {
+  Seq s;
+  int b, item, j;  // item = kv head * tiles + tile
+  __device__ __forceinline__ void next(const TreeParams& p) {
+    if (++j < s.stages) return;
+    j = 0;
+    item++;
+    while (b < p.batch && (s.stages == 0 || item == p.nkh * s.tiles)) {
+      item = 0;
+      if (++b < p.batch) s = seq_of(p, b);
+    }
+  }
+  // the first key from which every row sees all of the prefix
+  __device__ __forceinline__ int kfull(const TreeParams& p) const {
+    const long long k = p.window ? (long long)s.base + s.T - (long long)p.window : 0;
+    return k < 0 ? 0 : k > s.base ? s.base : (int)k;
+  }
+  __device__ __forceinline__ int key0() const { return s.lo + j * kKeysT; }
+  __device__ __forceinline__ bool clean(const TreeParams& p) const {
+    return key0() >= kfull(p) && key0() + kKeysT <= s.base;
+  }
+};
+
+template <int HD, int N, bool F32>
+__global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams p) {
+  using C = Tc<HD, N, F32>;
+  constexpr int MB = C::MB, ROWS = C::ROWS, RH = C::RH, W = C::W, G = C::G, UNITS = C::UNITS, NQ = C::NQ;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Sees* sees = reinterpret_cast<Sees*>(smem + C::OFF_SEES);
+  float* scales = reinterpret_cast<float*>(smem + C::OFF_SCALE);
+  uint32_t* okw = reinterpret_cast<uint32_t*>(smem + C::OFF_OK);
+  volatile int* badv = reinterpret_cast<volatile int*>(smem + C::OFF_BAD);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* full = bars;                // [UNITS] 4 loading warps
+  uint64_t* empty = full + UNITS;       // [UNITS] MMA commit
+  uint64_t* qfull = empty + UNITS;      // [4] tile & 3: 4 loading warps
+  uint64_t* qempty = qfull + 4;         // [2] MMA commit
+  uint64_t* sfull = qempty + 2;         // [2] MMA commit
+  uint64_t* sfree = sfull + 2;          // [2] 8 softmax warps
+  uint64_t* pfull = sfree + 2;          // 8 softmax warps
+  uint64_t* pvdone = pfull + 1;         // MMA commit
+  uint64_t* ofree = pvdone + 1;         // 8 softmax warps
+  uint64_t* mend = ofree + 1;           // MMA commit
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+
+  // ---- this CTA's run of stages
+  Split split;
+  split.of(total_stages(p), (int)gridDim.x);
+  const long long cta = blockIdx.x;
+  if (cta >= split.active) {
+    if (tid == 0) p.cuts[cta].parts = 0;
+    return;
+  }
+  const long long s0 = split.begin(cta);
+  const int n_stages = (int)(split.begin(cta + 1) - s0);
+  Walk at;
+  {
+    long long first = 0;
+    at.b = find_seq(p, s0, first);
+    at.s = seq_of(p, at.b);
+    at.item = (int)((s0 - first) / at.s.stages);
+    at.j = (int)((s0 - first) % at.s.stages);
+  }
+
+  if (tid == 0) {
+    // the tile that this CTA begins and others go on with, if there is one: its last
+    Walk w = at;
+    Cut c = {};
+    int begun = 0;  // stage of this CTA's run at which the last tile begins
+    for (int i = 0; i < n_stages;) {
+      begun = i;
+      i += w.s.stages - w.j;
+      if (i >= n_stages) break;
+      w.j = w.s.stages - 1;
+      w.next(p);
+    }
+    const long long end = s0 + begun - w.j + w.s.stages;  // the tile's end in the list
+    if (w.j == 0 && end > s0 + n_stages) {
+      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+      c.parts = (int)(split.owner(end - 1) - cta) + 1;
+      c.slot = (int)(2 * cta) + (begun > 0 ? 1 : 0);
+      c.rows = min(ROWS, w.s.T * p.group - tile * ROWS);
+      c.row0 = w.s.row0;
+      c.kvh = kvh;
+      c.first = tile * ROWS;
+    }
+    p.cuts[cta] = c;
+    for (int u = 0; u < UNITS; u++) {
+      mbar_init(&full[u], 4);
+      mbar_init(&empty[u], 1);
+    }
+    for (int u = 0; u < 4; u++) mbar_init(&qfull[u], 4);
+    for (int u = 0; u < 2; u++) {
+      mbar_init(&qempty[u], 1);
+      mbar_init(&sfull[u], 1);
+      mbar_init(&sfree[u], 8);
+    }
+    mbar_init(pfull, 8);
+    mbar_init(pvdone, 1);
+    mbar_init(ofree, 8);
+    mbar_init(mend, 1);
+    *abort_flag = 0;
+    for (int u = 0; u < 8; u++) badv[u] = 0;
+    fence_mbar_init();
+  }
+  if (warp == 12) {  // one CTA per SM (shared memory), so the allocation never waits
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t sbase = smem_u32(smem);
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    return wait_or_abort(bar, parity & 1u, abort_flag, p.err, code);
+  };
+
+  if (warp >= 8 && warp < 12) {
+    // ------------------------------------------------------------------------------ loads
+    regs_down<kRegsLoad>();
+    const int pw = warp - 8;
+    int issued = 0, signalled = 0;   // units
+    uint32_t scan = 0;               // bit k: unit signalled + k is a V unit whose rows see different keys
+    unsigned long long scan_tiles = 0;  // 16 bits per unit from `signalled` on: tile + 1 of those
+    auto signal = [&]() {            // the oldest unit in flight has landed (this thread's copies)
+      if (scan & 1u) {
+        // p = 0 times an infinite or NaN V would reach rows that do not see the key: such values
+        // become 0 here, and the epilogue adds them to the rows that do
+        bool bad = false;
+        unsigned char* u = smem + C::OFF_RING + (signalled % UNITS) * kUnit;
+        for (int it = 0; it < 8; it++)
+          for (int ch = 0; ch < 2; ch++) {
+            const int r = pw * 32 + it * 4 + lane / 8, k = lane % 8;
+            __half* x = reinterpret_cast<__half*>(u + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4));
+            for (int e = 0; e < 8; e++)
+              if ((__half_as_ushort(x[e]) & 0x7c00u) == 0x7c00u) {
+                x[e] = __ushort_as_half(0);
+                bad = true;
+              }
+          }
+        const int t = (int)(scan_tiles & 0xffffu);
+        if (bad) badv[t & 7] = t;
+      }
+      scan >>= 1;
+      scan_tiles >>= 16;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[signalled % UNITS]);
+      signalled++;
+    };
+    auto load_unit = [&](const __half* pool, long long off, int block, bool scan_it, int tile) {
+      const int slot = issued % UNITS;
+      if (issued >= UNITS) {
+        const uint32_t ph = (uint32_t)(issued / UNITS - 1) & 1u;
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&empty[slot], ph))) {
+          // nothing to issue now: hand over everything that is in flight
+          if (signalled < issued) {
+            cp_wait<0>();
+            while (signalled < issued) signal();
+          }
+          (void)wait(&empty[slot], ph, G4A_DEVERR_WAIT_EMPTY);
+          __syncwarp();
+        }
+      }
+      const uint32_t dst = sbase + C::OFF_RING + slot * kUnit;
+#pragma unroll
+      for (int it = 0; it < 8; it++) {
+        const int r = pw * 32 + it * 4 + lane / 8, k = lane % 8;
+        const long long o = __shfl_sync(0xffffffffu, off, it * 4 + lane / 8);
+#pragma unroll
+        for (int ch = 0; ch < 2; ch++) {
+          const int d = block * 128 + ch * 64 + k * 8;
+          const bool ok = o >= 0 && d < p.hd;
+          cp16(dst + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4), pool + (ok ? o + d : 0), ok);
+        }
+      }
+      cp_commit();
+      if (scan_it) {
+        scan |= 1u << (issued - signalled);
+        scan_tiles |= (unsigned long long)((tile + 1) & 0xffff) << (16 * (issued - signalled));
+      }
+      issued++;
+      if (issued - signalled > C::LAG) {
+        cp_wait<C::LAG>();
+        signal();
+      }
+    };
+    Walk w = at;
+    long long off = -1, off_prev = -1;
+    bool scan_prev = false;
+    int tile_no = -1, tile_prev = 0;  // tiles this CTA has begun
+    for (int i = 0; i <= n_stages; i++) {
+      bool scan_now = false;
+      if (i < n_stages) {
+        const bool first = i == 0 || w.j == 0;
+        if (first) tile_no++;
+        const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+        off = -1;
+        const int key = w.key0() + pw * 32 + lane;
+        if (key < w.s.L) off = row_offset(p, w.b, kvh, key);
+        scan_now = !w.clean(p);
+        const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
+        for (int u = 0; u < MB; u++) {
+          load_unit(p.k, off, u, false, 0);
+          // (written once K's first unit has a slot: the softmax is then done with stage i - 8)
+          if (u == 0 && lane == 0) okw[(i & 7) * 4 + pw] = there;
+        }
+        if (first) {
+          // ---- the tile's queries, what its rows see
+          const int qb = tile_no % NQ, sb = tile_no & 3;
+          if (tile_no >= NQ) {
+            if (signalled < issued) {
+              cp_wait<0>();
+              while (signalled < issued) signal();
+            }
+            (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
+            __syncwarp();
+          }
+          const int live = min(ROWS, w.s.T * p.group - tile * ROWS);
+          unsigned char* qs = smem + qb * C::Q_BYTES;
+          for (int r = pw * 32 + lane; r < ROWS; r += 128) {
+            Sees v = {0, ~0ull};  // rows past the last one: their results are not written
+            if (r < live) v = sees_of(p, w.s, (tile * ROWS + r) / p.group);
+            sees[sb * ROWS + r] = v;
+          }
+          auto row_of = [&](int r) {
+            const int gr = tile * ROWS + r, t = gr / p.group;
+            return ((size_t)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
+          };
+          if constexpr (F32) {
+            constexpr int V4 = HD / 128;
+#pragma unroll 1
+            for (int r0 = pw; r0 < ROWS; r0 += 16) {  // four rows of a warp at a time
+              float4 x[4][V4];
+#pragma unroll
+              for (int q = 0; q < 4; q++) {
+                const int r = r0 + 4 * q;
+                const float* src = reinterpret_cast<const float*>(p.q) + (r < live ? row_of(r) : 0);
+#pragma unroll
+                for (int u = 0; u < V4; u++) {
+                  const int d = u * 128 + lane * 4;
+                  x[q][u] = (r < live && d < p.hd) ? *reinterpret_cast<const float4*>(src + d)
+                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 4; q++) {
+                const int r = r0 + 4 * q;
+                if (r >= ROWS) continue;
+                float big = 0.f;
+#pragma unroll
+                for (int u = 0; u < V4; u++)
+                  big = fmaxf(big, fmaxf(fmaxf(fabsf(x[q][u].x), fabsf(x[q][u].y)),
+                                         fmaxf(fabsf(x[q][u].z), fabsf(x[q][u].w))));
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                int e = 0;
+                if (big > 0.f && big < INFINITY) e = max(-120, min(120, 10 - ilogbf(big)));
+                const float up = __int_as_float((127 + e) << 23);
+                if (lane == 0) scales[sb * ROWS + r] = ldexpf(p.scale_log2, -e);
+#pragma unroll
+                for (int u = 0; u < V4; u++) {
+                  const float v[4] = {x[q][u].x * up, x[q][u].y * up, x[q][u].z * up, x[q][u].w * up};
+                  float lo[4];
+#pragma unroll
+                  for (int k = 0; k < 4; k++) lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
+                  // dims u * 128 + 4 lane: chunk 2 u + lane / 16, half of 16-byte piece (lane / 2) % 8
+                  const int ch = 2 * u + (lane >> 4), k = (lane >> 1) & 7;
+#pragma unroll
+                  for (int term = 0; term < 2; term++) {
+                    const int n = r + term * ROWS;
+                    const float* y = term ? lo : v;
+                    *reinterpret_cast<uint2*>(qs + ch * (N * 128) + n * 128 + ((k ^ (n & 7)) << 4) + (lane & 1) * 8) =
+                        make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+                  }
+                }
+              }
+            }
+          } else {
+            constexpr int PC = HD / 8;  // 16-byte pieces of a row
+#pragma unroll 4
+            for (int e = pw * 32 + lane; e < ROWS * PC; e += 128) {
+              const int r = e / PC, k = e % PC;
+              uint4 v = make_uint4(0u, 0u, 0u, 0u);
+              if (r < live && k * 8 < p.hd)
+                v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + row_of(r) + k * 8);
+              *reinterpret_cast<uint4*>(qs + (k >> 3) * (N * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4)) = v;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&qfull[sb]);
+        }
+      }
+      if (i > 0)
+        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u, scan_prev, tile_prev);
+      off_prev = off;
+      scan_prev = scan_now;
+      tile_prev = tile_no;
+      if (i + 1 < n_stages) w.next(p);
+    }
+    cp_wait<0>();
+    while (signalled < issued) signal();
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------------------ MMAs
+    regs_down<kRegsMma>();
+    if (warp == 12 && lane == 0) {
+      constexpr uint32_t idesc_s = f16_idesc(N, false), idesc_o = f16_idesc(N, true, true);
+      Walk w = at;
+      int unit = 0, tile_no = -1, tile_o = -1;
+      bool first_prev = false, ok = true;
+      for (int i = 0; ok && i <= n_stages; i++) {
+        bool first = false;
+        if (i < n_stages) {
+          const int b = i & 1;
+          first = i == 0 || w.j == 0;
+          if (first) {
+            tile_no++;
+            ok = wait(&qfull[tile_no & 3], (uint32_t)(tile_no >> 2), G4A_DEVERR_WAIT_FULL);
+          }
+          if (ok && i >= 2) ok = wait(&sfree[b], (uint32_t)(i / 2 - 1), G4A_DEVERR_WAIT_MMA);
+          const uint64_t dq = sw128_desc(sbase + (tile_no % NQ) * C::Q_BYTES, 16, 1024);
+          for (int u = 0; ok && u < MB; u++, unit++) {
+            const int slot = unit % UNITS;
+            ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+              umma_f16_ss(tmem + C::COL_S + (uint32_t)(b * N), dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                          dq + (uint64_t)(((2 * u + (kk >> 2)) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
+                          (u > 0 || kk > 0) ? 1u : 0u);
+            umma_commit(&empty[slot]);
+          }
+          if (!ok) break;
+          umma_commit(&sfull[b]);
+          if (i + 1 == n_stages || w.j + 1 == w.s.stages) umma_commit(&qempty[tile_no % NQ]);
+        }
+        if (i > 0) {  // O of stage i - 1
+          if (first_prev) {
+            tile_o++;
+            if (tile_o > 0) ok = wait(ofree, (uint32_t)(tile_o - 1), G4A_DEVERR_WAIT_MMA);
+          }
+          if (ok) ok = wait(pfull, (uint32_t)(i - 1), G4A_DEVERR_WAIT_MMA);
+          const uint64_t dp = sw128_desc(sbase + C::OFF_P, 16384, 1024);
+          for (int u = 0; ok && u < MB; u++, unit++) {
+            const int slot = unit % UNITS;
+            ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dv = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16384, 1024);
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+              umma_f16_ss(tmem + C::COL_O + (uint32_t)(u * N), dv + (uint64_t)((kk * 2048) >> 4),
+                          dp + (uint64_t)((kk * 2048) >> 4), idesc_o, (!first_prev || kk > 0) ? 1u : 0u);
+            umma_commit(&empty[slot]);
+          }
+          if (!ok) break;
+          umma_commit(pvdone);
+        }
+        first_prev = first;
+        if (i + 1 < n_stages) w.next(p);
+      }
+      // no MMA may still be running when TMEM is freed, also after an abort
+      umma_commit(mend);
+      (void)mbar_wait_bounded(mend, 0, p.err, G4A_DEVERR_WAIT_MMA);
+    }
+  } else {
+    // ------------------------------------------------------------------------------ softmax
+    regs_up<kRegsSoftmax>();
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    float* su = reinterpret_cast<float*>(smem + C::OFF_U) + warp * RH;
+    float* sf = reinterpret_cast<float*>(smem + C::OFF_F) + warp * RH;
+    float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX) + half * 4 * RH;
+    const uint32_t bar_id = 1 + half;
+    const int key_in = quarter * 32 + lane;  // this thread's key of a stage
+    unsigned char* prow = smem + C::OFF_P + key_in * 128;
+    Walk w = at;
+    int tile_no = -1, j_first = 0;
+    float m[G];     // lane n: running maximum of row g * W + n of this half
+    float l[G][W];  // this thread's keys' share of the row sums
+    for (int i = 0; i < n_stages; i++) {
+      const int b = i & 1;
+      const bool first = i == 0 || w.j == 0;
+      const bool last = i + 1 == n_stages || w.j + 1 == w.s.stages;
+      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+      const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - half * RH;  // rows of this half
+      if (first) {
+        tile_no++;
+        j_first = w.j;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          m[g] = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < W; n++) l[g][n] = 0.f;
+        }
+        __syncwarp();
+        for (int n = lane; n < RH; n += 32) su[n] = kUnseen;
+        __syncwarp();
+      }
+      (void)warp_wait(&sfull[b], (uint32_t)(i >> 1) & 1u, abort_flag, p.err);
+      tc_fence_after();
+      if (live > 0) {
+        const int key0 = w.key0(), key = key0 + key_in;
+        const uint4 ok4 = *reinterpret_cast<const uint4*>(okw + (i & 7) * 4);
+        const bool clean = w.clean(p) && (ok4.x & ok4.y & ok4.z & ok4.w) == ~0u;
+        const uint32_t okq = quarter == 0 ? ok4.x : quarter == 1 ? ok4.y : quarter == 2 ? ok4.z : ok4.w;
+        const bool there = (okq >> lane) & 1u;
+        const Sees* see = sees + (tile_no & 3) * ROWS + half * RH;
+        const float* sc = scales + (tile_no & 3) * ROWS + half * RH;
+        bool pv_waited = i == 0;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          // ---- scores in powers of two
+          float x[W];
+          {
+            uint32_t r[W];
+            const uint32_t col = lanes + C::COL_S + (uint32_t)(b * N + half * RH + g * W);
+            tmem_load(col, r);
+#pragma unroll
+            for (int n = 0; n < W; n++) x[n] = __uint_as_float(r[n]);
+            if constexpr (F32) {
+              tmem_load(col + ROWS, r);
+#pragma unroll
+              for (int n = 0; n < W; n++) x[n] = (x[n] + __uint_as_float(r[n])) * sc[g * W + n];
+            } else {
+#pragma unroll
+              for (int n = 0; n < W; n++) x[n] *= p.scale_log2;
+            }
+          }
+          if (!clean) {
+            if (!there) {
+#pragma unroll
+              for (int n = 0; n < W; n++) x[n] = -INFINITY;
+            } else {
+#pragma unroll
+              for (int n = 0; n < W; n++) {
+                const Sees v = see[g * W + n];
+                const bool in = key < w.s.base ? key >= v.kmin : ((v.bits >> (key - w.s.base)) & 1) != 0;
+                if (!in) x[n] = -INFINITY;
+              }
+            }
+          }
+          if (g == G - 1) {  // every score of this buffer is in registers
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sfree[b]);
+          }
+          // ---- does a score pass its row's maximum by 2^8?
+          bool over = false;
+          const float4* u4 = reinterpret_cast<const float4*>(su + g * W);
+#pragma unroll
+          for (int n = 0; n < W; n += 4) {
+            const float4 u = u4[n / 4];
+            over |= x[n] - u.x > kPUp + kRaise;
+            over |= x[n + 1] - u.y > kPUp + kRaise;
+            over |= x[n + 2] - u.z > kPUp + kRaise;
+            over |= x[n + 3] - u.w > kPUp + kRaise;
+          }
+          if (any_of(bar_id, 128, over)) {
+            const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
+            if (lane < W) smax[quarter * RH + g * W + lane] = mine;
+            named_bar_sync(bar_id, 128);
+            const int n_of = g * W + (lane % W);
+            const float mx = fmaxf(fmaxf(smax[n_of], smax[RH + n_of]), fmaxf(smax[2 * RH + n_of], smax[3 * RH + n_of]));
+            const bool raise = mx > m[g] + kRaise;
+            const float f = !raise ? 1.f : m[g] == -INFINITY ? 0.f : fast_exp2(m[g] - mx);
+            if (raise) m[g] = mx;
+            if (lane < W) {
+              su[n_of] = m[g] == -INFINITY ? kUnseen : m[g] - kPUp;
+              sf[n_of] = f;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < W; n++) l[g][n] *= sf[g * W + n];
+            if (__any_sync(0xffffffffu, f != 1.f) && !first) {  // the same in the half's four warps
+              if (!pv_waited) {
+                (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
+                pv_waited = true;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int k = 0; k < MB * (F32 ? 2 : 1); k++) {  // M blocks (x terms)
+                const uint32_t col = lanes + C::COL_O + (uint32_t)((k % MB) * N + (k / MB) * ROWS + half * RH + g * W);
+                uint32_t r[W];
+                tmem_load(col, r);
+#pragma unroll
+                for (int n = 0; n < W; n++) r[n] = __float_as_uint(__uint_as_float(r[n]) * sf[g * W + n]);
+                tmem_store(col, r);
+              }
+              tmem_wait_st();
+            }
+          }
+          // ---- p = 2^(s - m + 7)
+          uint32_t hi[W / 2], lo[F32 ? W / 2 : 1];
+#pragma unroll
+          for (int n = 0; n < W; n += 4) {
+            const float4 u = u4[n / 4];
+            const float p0 = fast_exp2(x[n] - u.x), p1 = fast_exp2(x[n + 1] - u.y);
+            const float p2 = fast_exp2(x[n + 2] - u.z), p3 = fast_exp2(x[n + 3] - u.w);
+            l[g][n] += p0;
+            l[g][n + 1] += p1;
+            l[g][n + 2] += p2;
+            l[g][n + 3] += p3;
+            hi[n / 2] = pack2(p0, p1);
+            hi[n / 2 + 1] = pack2(p2, p3);
+            if constexpr (F32) {
+              const float2 h0 = h2_to_f2(hi[n / 2]), h1 = h2_to_f2(hi[n / 2 + 1]);
+              lo[n / 2] = pack2(p0 - h0.x, p1 - h0.y);
+              lo[n / 2 + 1] = pack2(p2 - h1.x, p3 - h1.y);
+            }
+          }
+          if (!pv_waited) {  // the previous stage's product has read P
+            (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
+            pv_waited = true;
+          }
+#pragma unroll
+          for (int term = 0; term < (F32 ? 2 : 1); term++) {
+            const int n0 = term * ROWS + half * RH + g * W;  // first column of this thread's run
+#pragma unroll
+            for (int k = 0; k < W / 8; k++) {
+              const int piece = n0 / 8 + k;
+              const uint32_t* v = (term ? lo : hi) + 4 * k;
+              *reinterpret_cast<uint4*>(prow + (piece >> 3) * 16384 + (((piece & 7) ^ (key_in & 7)) << 4)) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      } else {
+        // no rows of the tile in this half: its columns' P is never looked at
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sfree[b]);
+        if (i > 0) (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
+      }
+      fence_proxy_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(pfull);
+
+      if (last) {
+        // ---- row sums, then O / l (or the part of a tile that other CTAs share)
+        (void)warp_wait(pvdone, (uint32_t)i & 1u, abort_flag, p.err);
+        tc_fence_after();
+        if (live > 0) {
+          const bool whole = j_first == 0 && w.j + 1 == w.s.stages;
+          const bool later = i - (w.j - j_first) > 0;  // not the tile this CTA's run begins with
+          float* part = p.part + (size_t)(2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
+          float lt[G];
+          named_bar_sync(bar_id, 128);  // smax is free
+#pragma unroll
+          for (int g = 0; g < G; g++) {
+            const float mine = transpose_reduce<W>(l[g], [](float a, float c) { return a + c; });
+            if (lane < W) smax[quarter * RH + g * W + lane] = mine;
+          }
+          named_bar_sync(bar_id, 128);
+#pragma unroll
+          for (int g = 0; g < G; g++) {
+            const int n_of = g * W + (lane % W);
+            lt[g] = (smax[n_of] + smax[RH + n_of]) + (smax[2 * RH + n_of] + smax[3 * RH + n_of]);
+            if (lane < W) sf[n_of] = !whole ? 1.f : lt[g] == 0.f ? 0.f : 1.f / lt[g];
+            if (!whole && quarter == 0 && lane < W) {
+              part[(size_t)ROWS * HD + half * RH + n_of] = m[g];
+              part[(size_t)ROWS * HD + ROWS + half * RH + n_of] = lt[g];
+            }
+          }
+          __syncwarp();
+          const bool bad = badv[(tile_no + 1) & 7] == ((tile_no + 1) & 0xffff);
+#pragma unroll 1
+          for (int k = 0; k < MB * G; k++) {
+            const int mb = k / G, g = k % G;
+            const int d = mb * 128 + key_in;
+            const uint32_t col = lanes + C::COL_O + (uint32_t)(mb * N + half * RH + g * W);
+            float o[W];
+            {
+              uint32_t r[W];
+              tmem_load(col, r);
+#pragma unroll
+              for (int n = 0; n < W; n++) o[n] = __uint_as_float(r[n]);
+              if constexpr (F32) {
+                tmem_load(col + ROWS, r);
+#pragma unroll
+                for (int n = 0; n < W; n++) o[n] += __uint_as_float(r[n]);
+              }
+            }
+            if (bad && d < p.hd) {  // what the loads took out: infinities and NaN, for the rows that see them
+              for (int j = j_first; j <= w.j; j++) {
+                Walk t = w;
+                t.j = j;
+                if (t.clean(p)) continue;
+                for (int kk = t.key0(); kk < min(t.key0() + kKeysT, w.s.L); kk++) {
+                  const long long off = row_offset(p, w.b, kvh, kk);
+                  if (off < 0) continue;
+                  const float v = __half2float(p.v[off + d]);
+                  if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+                  for (int n = 0; n < W; n++)
+                    if (g * W + n < live) {
+                      const Sees q = sees_of(p, w.s, (tile * ROWS + half * RH + g * W + n) / p.group);
+                      if (kk < w.s.base ? kk >= q.kmin : ((q.bits >> (kk - w.s.base)) & 1) != 0) o[n] += v;
+                    }
+                }
+              }
+            }
+            const int nl = min(W, live - g * W);
+            if (whole) {
+              const int gr0 = tile * ROWS + half * RH + g * W;
+              long long row = 0;
+              if (lane < nl) {
+                const int gr = gr0 + lane, t = gr / p.group;
+                row = ((long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
+              }
+#pragma unroll
+              for (int n = 0; n < W; n++) {
+                const long long a = __shfl_sync(0xffffffffu, row, n);
+                if (n < nl && d < p.hd) {
+                  const float y = o[n] * sf[g * W + n];
+                  if constexpr (F32) reinterpret_cast<float*>(p.out)[a + d] = y;
+                  else reinterpret_cast<__half*>(p.out)[a + d] = __float2half_rn(y);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int n = 0; n < W; n++)
+                if (n < nl) part[(size_t)(half * RH + g * W + n) * HD + d] = o[n];
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ofree);
+      }
+      if (i + 1 < n_stages) w.next(p);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 12)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
+}
+
+template <int HD, int N, bool F32>
+g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long tokens_rows) {
+  using C = Tc<HD, N, F32>;
+  static std::atomic<bool> done[64];
+  if (ctx->device >= 64 || !done[ctx->device].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<HD, N, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)C::SMEM);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(tree_tc_kernel)");
+    if (ctx->device < 64) done[ctx->device].store(true, std::memory_order_release);
+  }
+  p.rows = C::ROWS;
+  p.kps = kKeysT;
+  p.hd_pad = HD;
+  const long long tiles = (tokens_rows + C::ROWS - 1) / C::ROWS;
+  const long long stages = (keys / kKeysT + p.batch) * tiles * p.nkh;
+  p.grid = (int)std::max<long long>(1, std::min<long long>(stages, std::min(ctx->num_sms, kMaxGrid)));
+  const size_t parts = (size_t)2 * p.grid * C::ROWS * (HD + 2) * sizeof(float);
+  if (g4a_status s = g4a_ensure_workspace(ctx, parts + (size_t)p.grid * sizeof(Cut))) return s;
+  p.part = static_cast<float*>(ctx->workspace);
+  p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(ctx->workspace) + parts);
+  g4a_prof_scope ps(ctx, G4A_PROF_TREE_ATTN);
+  const cudaError_t e =
+      g4a_launch(tree_tc_kernel<HD, N, F32>, dim3(p.grid), dim3(kThreadsTc), C::SMEM, ctx->stream, true, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch tree_tc_kernel");
+  return G4A_OK;
+}
+
+}  // namespace
+
+g4a_status g4a_tree_tc_launch(g4a_ctx* ctx, g4a_tree::TreeParams& p, bool f32, long long keys) {
+  const int rows = p.max_tokens * p.group;
+  if (p.hd > 256) return f32 ? launch_tc<512, 64, true>(ctx, p, keys, rows) : launch_tc<512, 64, false>(ctx, p, keys, rows);
+  if (p.hd > 128) {
+    if (f32) return rows <= 32 ? launch_tc<256, 64, true>(ctx, p, keys, rows) : launch_tc<256, 128, true>(ctx, p, keys, rows);
+    return rows <= 64 ? launch_tc<256, 64, false>(ctx, p, keys, rows) : launch_tc<256, 128, false>(ctx, p, keys, rows);
+  }
+  if (f32) return rows <= 32 ? launch_tc<128, 64, true>(ctx, p, keys, rows) : launch_tc<128, 128, true>(ctx, p, keys, rows);
+  return rows <= 64 ? launch_tc<128, 64, false>(ctx, p, keys, rows) : launch_tc<128, 128, false>(ctx, p, keys, rows);
+}
