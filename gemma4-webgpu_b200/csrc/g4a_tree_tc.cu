@@ -66,7 +66,6 @@ struct Tc {
   static constexpr int NQ = FIT2 >= 4 ? 2 : 1;        // query buffers
   static constexpr int FIT = (216 * 1024 - NQ * Q_BYTES - P_BYTES) / kUnit;
   static constexpr int UNITS = FIT > 5 ? 5 : FIT;
-  static constexpr int LAG = UNITS - 1 > 3 ? 3 : UNITS - 1;  // units in flight before the oldest is waited for
   static constexpr int OFF_P = NQ * Q_BYTES;
   static constexpr int OFF_RING = OFF_P + P_BYTES;
   static constexpr int OFF_SEES = OFF_RING + UNITS * kUnit;   // [4][ROWS] Sees
@@ -96,10 +95,18 @@ __device__ __forceinline__ void regs_down() {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Arrives on `bar` (one of its expected count) when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Sets infinite and NaN halves of a pair to 0; whether there was one.
+__device__ __forceinline__ bool clear_non_finite(uint32_t& w) {
+  uint32_t keep = 0xffffffffu;
+  if ((w & 0x7c00u) == 0x7c00u) keep &= 0xffff0000u;
+  if ((w & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
+  w &= keep;
+  return keep != 0xffffffffu;
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -195,7 +202,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
   uint32_t* okw = reinterpret_cast<uint32_t*>(smem + C::OFF_OK);
   volatile int* badv = reinterpret_cast<volatile int*>(smem + C::OFF_BAD);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* full = bars;                // [UNITS] 4 loading warps
+  uint64_t* full = bars;                // [UNITS] 128 loading threads
   uint64_t* empty = full + UNITS;       // [UNITS] MMA commit
   uint64_t* qfull = empty + UNITS;      // [4] tile & 3: 4 loading warps
   uint64_t* qempty = qfull + 4;         // [2] MMA commit
@@ -255,7 +262,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
     }
     p.cuts[cta] = c;
     for (int u = 0; u < UNITS; u++) {
-      mbar_init(&full[u], 4);
+      mbar_init(&full[u], 128);
       mbar_init(&empty[u], 1);
     }
     for (int u = 0; u < 4; u++) mbar_init(&qfull[u], 4);
@@ -293,48 +300,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
     // ------------------------------------------------------------------------------ loads
     regs_down<kRegsLoad>();
     const int pw = warp - 8;
-    int issued = 0, signalled = 0;   // units
-    uint32_t scan = 0;               // bit k: unit signalled + k is a V unit whose rows see different keys
-    unsigned long long scan_tiles = 0;  // 16 bits per unit from `signalled` on: tile + 1 of those
-    auto signal = [&]() {            // the oldest unit in flight has landed (this thread's copies)
-      if (scan & 1u) {
-        // p = 0 times an infinite or NaN V would reach rows that do not see the key: such values
-        // become 0 here, and the epilogue adds them to the rows that do
-        bool bad = false;
-        unsigned char* u = smem + C::OFF_RING + (signalled % UNITS) * kUnit;
-        for (int it = 0; it < 8; it++)
-          for (int ch = 0; ch < 2; ch++) {
-            const int r = pw * 32 + it * 4 + lane / 8, k = lane % 8;
-            __half* x = reinterpret_cast<__half*>(u + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4));
-            for (int e = 0; e < 8; e++)
-              if ((__half_as_ushort(x[e]) & 0x7c00u) == 0x7c00u) {
-                x[e] = __ushort_as_half(0);
-                bad = true;
-              }
-          }
-        const int t = (int)(scan_tiles & 0xffffu);
-        if (bad) badv[t & 7] = t;
-      }
-      scan >>= 1;
-      scan_tiles >>= 16;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&full[signalled % UNITS]);
-      signalled++;
-    };
-    auto load_unit = [&](const __half* pool, long long off, int block, bool scan_it, int tile) {
+    int issued = 0;  // units
+    auto load_unit = [&](const __half* pool, long long off, int block, bool hold) {
       const int slot = issued % UNITS;
       if (issued >= UNITS) {
-        const uint32_t ph = (uint32_t)(issued / UNITS - 1) & 1u;
-        if (!__all_sync(0xffffffffu, mbar_try_wait(&empty[slot], ph))) {
-          // nothing to issue now: hand over everything that is in flight
-          if (signalled < issued) {
-            cp_wait<0>();
-            while (signalled < issued) signal();
-          }
-          (void)wait(&empty[slot], ph, G4A_DEVERR_WAIT_EMPTY);
-          __syncwarp();
-        }
+        (void)wait(&empty[slot], (uint32_t)(issued / UNITS - 1), G4A_DEVERR_WAIT_EMPTY);
+        __syncwarp();
       }
       const uint32_t dst = sbase + C::OFF_RING + slot * kUnit;
 #pragma unroll
@@ -348,16 +319,31 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
           cp16(dst + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4), pool + (ok ? o + d : 0), ok);
         }
       }
-      cp_commit();
-      if (scan_it) {
-        scan |= 1u << (issued - signalled);
-        scan_tiles |= (unsigned long long)((tile + 1) & 0xffff) << (16 * (issued - signalled));
-      }
+      // arrives when this thread's copies have landed; the MMA thread's proxy fence follows its wait
+      if (!hold) cp_arrive(&full[slot]);
       issued++;
-      if (issued - signalled > C::LAG) {
-        cp_wait<C::LAG>();
-        signal();
+    };
+    // V of a stage whose rows see different keys: p = 0 times an infinite or NaN V would reach rows
+    // that do not see the key.  Such values become 0 here, and the epilogue adds them to the rows
+    // that do.  (The ring holds all units of a stage: no slot is waited for in between.)
+    auto scan_units = [&](int tile) {
+      cp_wait_all();
+      bool bad = false;
+      for (int q = issued - MB; q < issued; q++) {
+        unsigned char* u = smem + C::OFF_RING + (q % UNITS) * kUnit;
+#pragma unroll 1
+        for (int it = 0; it < 16; it++) {
+          const int r = pw * 32 + (it >> 1) * 4 + lane / 8, k = lane % 8;
+          uint4* x = reinterpret_cast<uint4*>(u + (it & 1) * 16384 + r * 128 + ((k ^ (r & 7)) << 4));
+          uint4 v = *x;
+          if (clear_non_finite(v.x) | clear_non_finite(v.y) | clear_non_finite(v.z) | clear_non_finite(v.w)) {
+            *x = v;
+            bad = true;
+          }
+        }
+        mbar_arrive(&full[q % UNITS]);
       }
+      if (bad) badv[(tile + 1) & 7] = (tile + 1) & 0xffff;
     };
     Walk w = at;
     long long off = -1, off_prev = -1;
@@ -374,19 +360,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
         if (key < w.s.L) off = row_offset(p, w.b, kvh, key);
         scan_now = !w.clean(p);
         const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
-        for (int u = 0; u < MB; u++) {
-          load_unit(p.k, off, u, false, 0);
-          // (written once K's first unit has a slot: the softmax is then done with stage i - 8)
-          if (u == 0 && lane == 0) okw[(i & 7) * 4 + pw] = there;
-        }
+        // (the ring holds at most five units, so the loads are at most five stages ahead of the softmax)
+        if (lane == 0) okw[(i & 7) * 4 + pw] = there;
+        for (int u = 0; u < MB; u++) load_unit(p.k, off, u, false);
         if (first) {
           // ---- the tile's queries, what its rows see
           const int qb = tile_no % NQ, sb = tile_no & 3;
           if (tile_no >= NQ) {
-            if (signalled < issued) {
-              cp_wait<0>();
-              while (signalled < issued) signal();
-            }
             (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
             __syncwarp();
           }
@@ -466,15 +446,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
           if (lane == 0) mbar_arrive(&qfull[sb]);
         }
       }
-      if (i > 0)
-        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u, scan_prev, tile_prev);
+      if (i > 0) {
+        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u, scan_prev);
+        if (scan_prev) scan_units(tile_prev);
+      }
       off_prev = off;
       scan_prev = scan_now;
       tile_prev = tile_no;
       if (i + 1 < n_stages) w.next(p);
     }
-    cp_wait<0>();
-    while (signalled < issued) signal();
+    cp_wait_all();
   } else if (warp >= 12) {
     // ------------------------------------------------------------------------------ MMAs
     regs_down<kRegsMma>();
@@ -498,6 +479,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
             const int slot = unit % UNITS;
             ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
             if (!ok) break;
+            fence_proxy_async_smem();  // the copies were made by the generic proxy
             tc_fence_after();
             const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
 #pragma unroll
@@ -522,6 +504,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
             const int slot = unit % UNITS;
             ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
             if (!ok) break;
+            fence_proxy_async_smem();
             tc_fence_after();
             const uint64_t dv = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16384, 1024);
 #pragma unroll
