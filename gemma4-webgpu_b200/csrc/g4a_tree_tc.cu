@@ -19,7 +19,7 @@
 // Shared memory: Q [64-dim chunk][N][128 B], P [64-column chunk][128 keys][128 B], and a ring of
 // 32 KB units, each 128 keys x 128 dims of K or V as two [128 keys][128 B] chunks, all with the
 // 128-byte swizzle (16-byte piece k of row r at k ^ (r & 7)).
-// Warps (16, of which the last three have nothing to do):
+// Warps (16):
 //   0-7    softmax: warp w has TMEM lanes 32 (w % 4) .. + 31 (keys) and the rows of half w / 4.
 //          A thread holds one key's scores for its rows.  The running maximum of a row is raised
 //          only when a score passes it by 2^8 (p = 2^(s - m + 7) <= 2^15 stays in f16): whether
@@ -29,6 +29,7 @@
 //          with zero fill for rows that are not there, and the tile's queries.
 //   12     one thread issues the MMAs: S of stage i, then O of stage i - 1, so the softmax of a
 //          stage runs under the next stage's score product.
+//   13-15  hand landed units over to the MMA thread (proxy fence), V values checked on the way.
 // Every wait is bounded; a thread that gives up sets the abort flag and the error word, all waits
 // then end at once, and the CTA frees its TMEM and leaves.
 #include <algorithm>
@@ -44,7 +45,7 @@ using namespace g4a_tree;
 
 constexpr int kKeysT = 128;
 constexpr int kMaxGrid = 256;        // (the join looks at one cut per thread)
-constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one with the MMA warp
+constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one MMA and handing over
 // Registers: 512 threads start with 128 each (65,536); the softmax warpgroups, which hold a row
 // block of scores and sums, take 168, the others give theirs: 256 * 168 + 128 * 96 + 128 * 72 = 64,512.
 constexpr int kRegsSoftmax = 168, kRegsLoad = 96, kRegsMma = 72;
@@ -76,7 +77,7 @@ struct Tc {
   static constexpr int OFF_OK = OFF_MAX + 8 * RH * 4;         // [8 stages][4] which rows are there
   static constexpr int OFF_BAD = OFF_OK + 128;                // [8] tile + 1 that had a V value that is not finite
   static constexpr int OFF_BAR = OFF_BAD + 32;
-  static constexpr int NBARS = 2 * UNITS + 4 + 2 + 2 + 2 + 5;
+  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5;
   static constexpr int OFF_END = OFF_BAR + NBARS * 8;
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
@@ -190,8 +191,40 @@ struct Walk {
   }
 };
 
+// Head dim d of `rows` query rows (from row gr0 of the kv head): adds the infinities and NaN of the V
+// values that were taken out of the tile's stages from key0 on, for the rows that see their keys, to
+// what this thread has just stored (in `part`, pitch floats from row to row, or in the output).
+template <bool F32>
+__device__ __noinline__ void add_non_finite(const TreeParams& p, Seq s, int b, int kvh, int key0, int k_end, int kfull,
+                                            int d, int gr0, int rows, float* part, int pitch) {
+  for (int key = key0; key < k_end; key++) {
+    if (key >= kfull && key < s.base) {
+      key = s.base - 1;
+      continue;
+    }
+    const long long off = row_offset(p, b, kvh, key);
+    if (off < 0) continue;
+    const float v = __half2float(p.v[off + d]);
+    if (fabsf(v) < INFINITY) continue;
+    for (int n = 0; n < rows; n++) {
+      const int gr = gr0 + n, t = gr / p.group;
+      const Sees q = sees_of(p, s, t);
+      if (!(key < s.base ? key >= q.kmin : ((q.bits >> (key - s.base)) & 1) != 0)) continue;
+      const size_t at = ((size_t)(s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd + d;
+      if (part != nullptr) {
+        part[(size_t)n * pitch + d] += v;
+      } else if constexpr (F32) {
+        reinterpret_cast<float*>(p.out)[at] += v;
+      } else {
+        __half* o = reinterpret_cast<__half*>(p.out) + at;
+        *o = __float2half_rn(__half2float(*o) + v);
+      }
+    }
+  }
+}
+
 template <int HD, int N, bool F32>
-__global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams p) {
+__global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_constant__ TreeParams p) {
   using C = Tc<HD, N, F32>;
   constexpr int MB = C::MB, ROWS = C::ROWS, RH = C::RH, W = C::W, G = C::G, UNITS = C::UNITS, NQ = C::NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -202,9 +235,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
   uint32_t* okw = reinterpret_cast<uint32_t*>(smem + C::OFF_OK);
   volatile int* badv = reinterpret_cast<volatile int*>(smem + C::OFF_BAD);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* full = bars;                // [UNITS] 128 loading threads
+  uint64_t* landed = bars;              // [UNITS] 128 loading threads
+  uint64_t* full = landed + UNITS;      // [UNITS] 3 handing-over warps
   uint64_t* empty = full + UNITS;       // [UNITS] MMA commit
-  uint64_t* qfull = empty + UNITS;      // [4] tile & 3: 4 loading warps
+  uint64_t* qlanded = empty + UNITS;    // [4] tile & 3: 128 loading threads
+  uint64_t* qfull = qlanded + 4;        // [4] 3 handing-over warps
   uint64_t* qempty = qfull + 4;         // [2] MMA commit
   uint64_t* sfull = qempty + 2;         // [2] MMA commit
   uint64_t* sfree = sfull + 2;          // [2] 8 softmax warps
@@ -262,10 +297,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
     }
     p.cuts[cta] = c;
     for (int u = 0; u < UNITS; u++) {
-      mbar_init(&full[u], 128);
+      mbar_init(&landed[u], 128);
+      mbar_init(&full[u], 3);
       mbar_init(&empty[u], 1);
     }
-    for (int u = 0; u < 4; u++) mbar_init(&qfull[u], 4);
+    for (int u = 0; u < 4; u++) {
+      mbar_init(&qlanded[u], 128);
+      mbar_init(&qfull[u], 3);
+    }
     for (int u = 0; u < 2; u++) {
       mbar_init(&qempty[u], 1);
       mbar_init(&sfull[u], 1);
@@ -301,7 +340,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
     regs_down<kRegsLoad>();
     const int pw = warp - 8;
     int issued = 0;  // units
-    auto load_unit = [&](const __half* pool, long long off, int block, bool hold) {
+    auto load_unit = [&](const __half* pool, long long off, int block) {
       const int slot = issued % UNITS;
       if (issued >= UNITS) {
         (void)wait(&empty[slot], (uint32_t)(issued / UNITS - 1), G4A_DEVERR_WAIT_EMPTY);
@@ -319,38 +358,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
           cp16(dst + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4), pool + (ok ? o + d : 0), ok);
         }
       }
-      // arrives when this thread's copies have landed; the MMA thread's proxy fence follows its wait
-      if (!hold) cp_arrive(&full[slot]);
+      cp_arrive(&landed[slot]);  // when this thread's copies have landed
       issued++;
-    };
-    // V of a stage whose rows see different keys: p = 0 times an infinite or NaN V would reach rows
-    // that do not see the key.  Such values become 0 here, and the epilogue adds them to the rows
-    // that do.  (The ring holds all units of a stage: no slot is waited for in between.)
-    auto scan_units = [&](int tile) {
-      cp_wait_all();
-      bool bad = false;
-      for (int q = issued - MB; q < issued; q++) {
-        unsigned char* u = smem + C::OFF_RING + (q % UNITS) * kUnit;
-#pragma unroll 1
-        for (int it = 0; it < 16; it++) {
-          const int r = pw * 32 + (it >> 1) * 4 + lane / 8, k = lane % 8;
-          uint4* x = reinterpret_cast<uint4*>(u + (it & 1) * 16384 + r * 128 + ((k ^ (r & 7)) << 4));
-          uint4 v = *x;
-          if (clear_non_finite(v.x) | clear_non_finite(v.y) | clear_non_finite(v.z) | clear_non_finite(v.w)) {
-            *x = v;
-            bad = true;
-          }
-        }
-        mbar_arrive(&full[q % UNITS]);
-      }
-      if (bad) badv[(tile + 1) & 7] = (tile + 1) & 0xffff;
     };
     Walk w = at;
     long long off = -1, off_prev = -1;
-    bool scan_prev = false;
-    int tile_no = -1, tile_prev = 0;  // tiles this CTA has begun
+    int tile_no = -1;  // tiles this CTA has begun
     for (int i = 0; i <= n_stages; i++) {
-      bool scan_now = false;
       if (i < n_stages) {
         const bool first = i == 0 || w.j == 0;
         if (first) tile_no++;
@@ -358,11 +372,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
         off = -1;
         const int key = w.key0() + pw * 32 + lane;
         if (key < w.s.L) off = row_offset(p, w.b, kvh, key);
-        scan_now = !w.clean(p);
         const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
         // (the ring holds at most five units, so the loads are at most five stages ahead of the softmax)
         if (lane == 0) okw[(i & 7) * 4 + pw] = there;
-        for (int u = 0; u < MB; u++) load_unit(p.k, off, u, false);
+        for (int u = 0; u < MB; u++) load_unit(p.k, off, u);
         if (first) {
           // ---- the tile's queries, what its rows see
           const int qb = tile_no % NQ, sb = tile_no & 3;
@@ -372,35 +385,37 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
           }
           const int live = min(ROWS, w.s.T * p.group - tile * ROWS);
           unsigned char* qs = smem + qb * C::Q_BYTES;
-          for (int r = pw * 32 + lane; r < ROWS; r += 128) {
+          // lane k looks up row pw + 4 k of the tile: where its query is, and what it sees
+          constexpr int RW = ROWS / 4;
+          long long mine = -1;
+          if (lane < RW) {
+            const int r = pw + 4 * lane, gr = tile * ROWS + r, t = gr / p.group;
             Sees v = {0, ~0ull};  // rows past the last one: their results are not written
-            if (r < live) v = sees_of(p, w.s, (tile * ROWS + r) / p.group);
+            if (r < live) {
+              mine = ((long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
+              v = sees_of(p, w.s, t);
+            }
             sees[sb * ROWS + r] = v;
           }
-          auto row_of = [&](int r) {
-            const int gr = tile * ROWS + r, t = gr / p.group;
-            return ((size_t)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
-          };
           if constexpr (F32) {
-            constexpr int V4 = HD / 128;
+            constexpr int V4 = HD / 128, RB = 16 / V4 < RW ? 16 / V4 : RW;  // rows in flight (64 registers)
 #pragma unroll 1
-            for (int r0 = pw; r0 < ROWS; r0 += 16) {  // four rows of a warp at a time
-              float4 x[4][V4];
+            for (int k0 = 0; k0 < RW; k0 += RB) {
+              float4 x[RB][V4];
 #pragma unroll
-              for (int q = 0; q < 4; q++) {
-                const int r = r0 + 4 * q;
-                const float* src = reinterpret_cast<const float*>(p.q) + (r < live ? row_of(r) : 0);
+              for (int q = 0; q < RB; q++) {
+                const long long o = __shfl_sync(0xffffffffu, mine, k0 + q);
+                const float* src = reinterpret_cast<const float*>(p.q) + o;
 #pragma unroll
                 for (int u = 0; u < V4; u++) {
                   const int d = u * 128 + lane * 4;
-                  x[q][u] = (r < live && d < p.hd) ? *reinterpret_cast<const float4*>(src + d)
-                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+                  x[q][u] = (o >= 0 && d < p.hd) ? __ldg(reinterpret_cast<const float4*>(src + d))
+                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
               }
 #pragma unroll
-              for (int q = 0; q < 4; q++) {
-                const int r = r0 + 4 * q;
-                if (r >= ROWS) continue;
+              for (int q = 0; q < RB; q++) {
+                const int r = pw + 4 * (k0 + q);
                 float big = 0.f;
 #pragma unroll
                 for (int u = 0; u < V4; u++)
@@ -408,8 +423,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
                                          fmaxf(fabsf(x[q][u].z), fabsf(x[q][u].w))));
 #pragma unroll
                 for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                // 2^e brings the largest element to [2^10, 2^11); its exponent is read from the bits
                 int e = 0;
-                if (big > 0.f && big < INFINITY) e = max(-120, min(120, 10 - ilogbf(big)));
+                if (big > 0.f && big < INFINITY) e = max(-120, min(120, 137 - (int)(__float_as_uint(big) >> 23)));
                 const float up = __int_as_float((127 + e) << 23);
                 if (lane == 0) scales[sb * ROWS + r] = ldexpf(p.scale_log2, -e);
 #pragma unroll
@@ -430,29 +446,30 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
                 }
               }
             }
+            mbar_arrive(&qlanded[sb]);
           } else {
-            constexpr int PC = HD / 8;  // 16-byte pieces of a row
+            constexpr int PC = HD / 8;                     // 16-byte pieces of a row
+            constexpr int PER = PC < 32 ? 32 / PC : 1;     // rows per copy instruction
+            const uint32_t qa = smem_u32(qs);
 #pragma unroll 4
-            for (int e = pw * 32 + lane; e < ROWS * PC; e += 128) {
-              const int r = e / PC, k = e % PC;
-              uint4 v = make_uint4(0u, 0u, 0u, 0u);
-              if (r < live && k * 8 < p.hd)
-                v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __half*>(p.q) + row_of(r) + k * 8);
-              *reinterpret_cast<uint4*>(qs + (k >> 3) * (N * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4)) = v;
+            for (int k0 = 0; k0 < RW; k0 += PER) {
+              const int kr = k0 + (PC < 32 ? lane / PC : 0), r = pw + 4 * kr;
+              const long long o = __shfl_sync(0xffffffffu, mine, kr);
+#pragma unroll
+              for (int u = 0; u < (PC > 32 ? PC / 32 : 1); u++) {
+                const int k = (PC < 32 ? lane % PC : lane + 32 * u);
+                const bool ok = o >= 0 && k * 8 < p.hd;
+                cp16(qa + (k >> 3) * (N * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4),
+                     reinterpret_cast<const __half*>(p.q) + (ok ? o + k * 8 : 0), ok);
+              }
             }
+            cp_arrive(&qlanded[sb]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&qfull[sb]);
         }
       }
-      if (i > 0) {
-        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u, scan_prev);
-        if (scan_prev) scan_units(tile_prev);
-      }
+      if (i > 0)
+        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u);
       off_prev = off;
-      scan_prev = scan_now;
-      tile_prev = tile_no;
       if (i + 1 < n_stages) w.next(p);
     }
     cp_wait_all();
@@ -479,7 +496,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
             const int slot = unit % UNITS;
             ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
             if (!ok) break;
-            fence_proxy_async_smem();  // the copies were made by the generic proxy
             tc_fence_after();
             const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
 #pragma unroll
@@ -504,7 +520,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
             const int slot = unit % UNITS;
             ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
             if (!ok) break;
-            fence_proxy_async_smem();
             tc_fence_after();
             const uint64_t dv = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16384, 1024);
 #pragma unroll
@@ -522,6 +537,58 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
       // no MMA may still be running when TMEM is freed, also after an abort
       umma_commit(mend);
       (void)mbar_wait_bounded(mend, 0, p.err, G4A_DEVERR_WAIT_MMA);
+    }
+    if (warp > 12) {
+      // ---------------------------------------------------------------------------- handing over
+      // Takes the units in the order of their loads: waits until one has landed, makes the copies
+      // (generic proxy) visible to the tensor core (async proxy), passes it on.  (The same fence
+      // in the MMA thread held every unit up by several hundred cycles.)
+      // V of keys that not every row sees: p = 0 times an infinite or NaN V would reach the rows
+      // that do not.  Such values become 0 here, and the epilogue adds them to the rows that do.
+      const int hw = warp - 13;
+      Walk w = at, before = at;
+      int unit = 0, tile_no = -1, tile_before = 0;
+      auto pass = [&](uint64_t* from, uint64_t* to, uint32_t parity) {
+        (void)warp_wait(from, parity & 1u, abort_flag, p.err);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(to);
+      };
+      for (int i = 0; i <= n_stages; i++) {
+        if (i < n_stages) {
+          const bool first = i == 0 || w.j == 0;
+          if (first) tile_no++;
+          for (int u = 0; u < MB; u++, unit++)
+            pass(&landed[unit % UNITS], &full[unit % UNITS], (uint32_t)(unit / UNITS));
+          if (first) pass(&qlanded[tile_no & 3], &qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+        }
+        if (i > 0) {
+          const bool mixed = !before.clean(p);
+          for (int u = 0; u < MB; u++, unit++) {
+            if (mixed) {
+              (void)warp_wait(&landed[unit % UNITS], (uint32_t)(unit / UNITS) & 1u, abort_flag, p.err);
+              const int k0 = before.key0(), a1 = before.kfull(p) - k0, b0 = before.s.base - k0, b1 = before.s.L - k0;
+              unsigned char* x0 = smem + C::OFF_RING + (unit % UNITS) * kUnit;
+              bool bad = false;
+              for (int e = hw * 32 + lane; e < kKeysT * 16; e += 96) {
+                const int r = e >> 4;
+                if (!(r < a1 || (r >= b0 && r < b1))) continue;
+                uint4* x = reinterpret_cast<uint4*>(x0 + ((e >> 3) & 1) * 16384 + r * 128 + ((e & 7) << 4));
+                uint4 v = *x;
+                if (clear_non_finite(v.x) | clear_non_finite(v.y) | clear_non_finite(v.z) | clear_non_finite(v.w)) {
+                  *x = v;
+                  bad = true;
+                }
+              }
+              if (bad) badv[(tile_before + 1) & 7] = (tile_before + 1) & 0xffff;
+            }
+            pass(&landed[unit % UNITS], &full[unit % UNITS], (uint32_t)(unit / UNITS));
+          }
+        }
+        before = w;
+        tile_before = tile_no;
+        if (i + 1 < n_stages) w.next(p);
+      }
     }
   } else {
     // ------------------------------------------------------------------------------ softmax
@@ -742,25 +809,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
                 for (int n = 0; n < W; n++) o[n] += __uint_as_float(r[n]);
               }
             }
-            if (bad && d < p.hd) {  // what the loads took out: infinities and NaN, for the rows that see them
-              for (int j = j_first; j <= w.j; j++) {
-                Walk t = w;
-                t.j = j;
-                if (t.clean(p)) continue;
-                for (int kk = t.key0(); kk < min(t.key0() + kKeysT, w.s.L); kk++) {
-                  const long long off = row_offset(p, w.b, kvh, kk);
-                  if (off < 0) continue;
-                  const float v = __half2float(p.v[off + d]);
-                  if (fabsf(v) < INFINITY) continue;
-#pragma unroll
-                  for (int n = 0; n < W; n++)
-                    if (g * W + n < live) {
-                      const Sees q = sees_of(p, w.s, (tile * ROWS + half * RH + g * W + n) / p.group);
-                      if (kk < w.s.base ? kk >= q.kmin : ((q.bits >> (kk - w.s.base)) & 1) != 0) o[n] += v;
-                    }
-                }
-              }
-            }
             const int nl = min(W, live - g * W);
             if (whole) {
               const int gr0 = tile * ROWS + half * RH + g * W;
@@ -783,6 +831,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const TreeParams
               for (int n = 0; n < W; n++)
                 if (n < nl) part[(size_t)(half * RH + g * W + n) * HD + d] = o[n];
             }
+            if (bad && d < p.hd)
+              add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0() + kKeysT, w.s.L), w.kfull(p),
+                                  d, tile * ROWS + half * RH + g * W, nl,
+                                  whole ? nullptr : part + (size_t)(half * RH + g * W) * HD, HD);
           }
         }
         tc_fence_before();
