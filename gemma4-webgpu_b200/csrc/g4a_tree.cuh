@@ -24,6 +24,8 @@ struct TreeParams {
   float* part;    // [2 * grid] partial rows: o [rows, hd_pad] | m [rows] | l [rows]
   int hd_pad;
   struct Cut* cuts;  // [grid]
+  const __half* q_terms;  // f32 queries: [tokens, nqh][2][hd_pad], high and low f16 terms
+  const float* q_scale;   // and [tokens, nqh] scale * log2(e) over the power of two in them
   int* err;
 };
 

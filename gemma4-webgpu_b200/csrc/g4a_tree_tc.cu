@@ -26,7 +26,8 @@
 //          any does is one block-wide vote per stage; finding the maxima (a transposing reduction
 //          over the lanes and the four warps) and rescaling O in TMEM happens only then.
 //   8-11   loads: row addresses through the page table (any page size), cp.async into the ring
-//          with zero fill for rows that are not there, and the tile's queries.
+//          with zero fill for rows that are not there, and the tile's queries (f32 queries as the
+//          terms that a small kernel before this one has split them into).
 //   12     one thread issues the MMAs: S of stage i, then O of stage i - 1, so the softmax of a
 //          stage runs under the next stage's score product.
 //   13-15  hand landed units over to the MMA thread (proxy fence), V values checked on the way.
@@ -128,6 +129,17 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { t
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
+
+// True in one lane of a converged warp (always the same one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 
 // Whether any of `count` threads (whole warps) says so; a barrier among them.
 __device__ __forceinline__ bool any_of(uint32_t id, uint32_t count, bool pred) {
@@ -250,52 +262,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_wait_primary();
-  pdl_launch_dependents();
-
-  // ---- this CTA's run of stages
-  Split split;
-  split.of(total_stages(p), (int)gridDim.x);
-  const long long cta = blockIdx.x;
-  if (cta >= split.active) {
-    if (tid == 0) p.cuts[cta].parts = 0;
-    return;
-  }
-  const long long s0 = split.begin(cta);
-  const int n_stages = (int)(split.begin(cta + 1) - s0);
-  Walk at;
-  {
-    long long first = 0;
-    at.b = find_seq(p, s0, first);
-    at.s = seq_of(p, at.b);
-    at.item = (int)((s0 - first) / at.s.stages);
-    at.j = (int)((s0 - first) % at.s.stages);
-  }
-
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // ---- barriers and TMEM, before the wait for the preceding kernel
   if (tid == 0) {
-    // the tile that this CTA begins and others go on with, if there is one: its last
-    Walk w = at;
-    Cut c = {};
-    int begun = 0;  // stage of this CTA's run at which the last tile begins
-    for (int i = 0; i < n_stages;) {
-      begun = i;
-      i += w.s.stages - w.j;
-      if (i >= n_stages) break;
-      w.j = w.s.stages - 1;
-      w.next(p);
-    }
-    const long long end = s0 + begun - w.j + w.s.stages;  // the tile's end in the list
-    if (w.j == 0 && end > s0 + n_stages) {
-      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
-      c.parts = (int)(split.owner(end - 1) - cta) + 1;
-      c.slot = (int)(2 * cta) + (begun > 0 ? 1 : 0);
-      c.rows = min(ROWS, w.s.T * p.group - tile * ROWS);
-      c.row0 = w.s.row0;
-      c.kvh = kvh;
-      c.first = tile * ROWS;
-    }
-    p.cuts[cta] = c;
     for (int u = 0; u < UNITS; u++) {
       mbar_init(&landed[u], 128);
       mbar_init(&full[u], 3);
@@ -329,6 +298,50 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait_primary();
+  pdl_launch_dependents();
+
+  // ---- this CTA's run of stages
+  Split split;
+  split.of(total_stages(p), (int)gridDim.x);
+  const long long cta = blockIdx.x;
+  // (a CTA without work goes through the roles with 0 stages and frees its TMEM like the others)
+  const long long s0 = cta < split.active ? split.begin(cta) : 0;
+  const int n_stages = cta < split.active ? (int)(split.begin(cta + 1) - s0) : 0;
+  Walk at = {};
+  if (n_stages > 0) {
+    long long first = 0;
+    at.b = find_seq(p, s0, first);
+    at.s = seq_of(p, at.b);
+    at.item = (int)((s0 - first) / at.s.stages);
+    at.j = (int)((s0 - first) % at.s.stages);
+  }
+
+  if (tid == 0) {
+    // the tile that this CTA begins and others go on with, if there is one: its last
+    Walk w = at;
+    Cut c = {};
+    int begun = 0;  // stage of this CTA's run at which the last tile begins
+    for (int i = 0; i < n_stages;) {
+      begun = i;
+      i += w.s.stages - w.j;
+      if (i >= n_stages) break;
+      w.j = w.s.stages - 1;
+      w.next(p);
+    }
+    const long long end = s0 + begun - w.j + w.s.stages;  // the tile's end in the list
+    if (n_stages > 0 && w.j == 0 && end > s0 + n_stages) {
+      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+      c.parts = (int)(split.owner(end - 1) - cta) + 1;
+      c.slot = (int)(2 * cta) + (begun > 0 ? 1 : 0);
+      c.rows = min(ROWS, w.s.T * p.group - tile * ROWS);
+      c.row0 = w.s.row0;
+      c.kvh = kvh;
+      c.first = tile * ROWS;
+    }
+    p.cuts[cta] = c;
+  }
+  __syncwarp();
   const uint32_t tmem = *tmem_slot;
   const uint32_t sbase = smem_u32(smem);
   auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
@@ -340,202 +353,191 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     regs_down<kRegsLoad>();
     const int pw = warp - 8;
     int issued = 0;  // units
-    auto load_unit = [&](const __half* pool, long long off, int block) {
-      const int slot = issued % UNITS;
-      if (issued >= UNITS) {
-        (void)wait(&empty[slot], (uint32_t)(issued / UNITS - 1), G4A_DEVERR_WAIT_EMPTY);
-        __syncwarp();
-      }
-      const uint32_t dst = sbase + C::OFF_RING + slot * kUnit;
+    // A lane copies the 16-byte pieces k = lane % 8 of rows 32 pw + 4 it + lane / 8, it = 0..7; what it
+    // needs of a stage's rows is looked up once and kept for all units of K and, later, of V.
+    struct Rows {
+      size_t at[8];  // the row's piece, in elements from the pool's start
+      uint32_t ok;   // bit it: the row is there
+    };
+    const int k8 = (lane & 7) * 8;
+    const uint32_t lane_dst = (uint32_t)(pw * 4096 + (lane >> 3) * 128);
+    const uint32_t sw0 = (uint32_t)(((lane & 7) ^ (lane >> 3)) << 4), sw1 = sw0 ^ 64u;  // it even, odd
+    auto load_units = [&](const Rows& rows, const __half* pool) {
 #pragma unroll
-      for (int it = 0; it < 8; it++) {
-        const int r = pw * 32 + it * 4 + lane / 8, k = lane % 8;
-        const long long o = __shfl_sync(0xffffffffu, off, it * 4 + lane / 8);
-#pragma unroll
-        for (int ch = 0; ch < 2; ch++) {
-          const int d = block * 128 + ch * 64 + k * 8;
-          const bool ok = o >= 0 && d < p.hd;
-          cp16(dst + ch * 16384 + r * 128 + ((k ^ (r & 7)) << 4), pool + (ok ? o + d : 0), ok);
+      for (int u = 0; u < MB; u++) {
+        const int slot = issued % UNITS;
+        if (issued >= UNITS) {
+          (void)wait(&empty[slot], (uint32_t)(issued / UNITS - 1), G4A_DEVERR_WAIT_EMPTY);
+          __syncwarp();
         }
+        const uint32_t dst = sbase + C::OFF_RING + slot * kUnit + lane_dst;
+        const bool in0 = u * 128 + k8 < p.hd, in1 = u * 128 + 64 + k8 < p.hd;
+#pragma unroll
+        for (int it = 0; it < 8; it++) {
+          const uint32_t to = dst + it * 512 + (it & 1 ? sw1 : sw0);
+          const bool ok = (rows.ok >> it) & 1u;
+          const __half* from = pool + rows.at[it];
+          cp16(to, from + (in0 ? u * 128 : 0), ok && in0);
+          cp16(to + 16384, from + (in1 ? u * 128 + 64 : 0), ok && in1);
+        }
+        cp_arrive(&landed[slot]);  // when this thread's copies have landed
+        issued++;
       }
-      cp_arrive(&landed[slot]);  // when this thread's copies have landed
-      issued++;
     };
     Walk w = at;
-    long long off = -1, off_prev = -1;
+    Rows rows = {}, rows_before = {};
     int tile_no = -1;  // tiles this CTA has begun
+    // The tile's queries into Q buffer tile_no % NQ, and what its rows see.  Lane k looks up row
+    // pw + 4 k of the tile.
+    auto load_queries = [&]() {
+      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+      const int qb = tile_no % NQ, sb = tile_no & 3;
+      if (tile_no >= NQ) {
+        (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
+        __syncwarp();
+      }
+      const int live = min(ROWS, w.s.T * p.group - tile * ROWS);
+      constexpr int RW = ROWS / 4;
+      const int r_mine = pw + 4 * lane, gr = tile * ROWS + r_mine, t = gr / p.group;
+      long long mine = -1;  // its row of q, in heads
+      if (lane < RW && r_mine < live)
+        mine = (long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group);
+      constexpr int PC = HD / 8;                  // 16-byte pieces of a row
+      constexpr int PER = PC < 32 ? 32 / PC : 1;  // rows per copy instruction
+      const uint32_t qa = sbase + qb * C::Q_BYTES;
+#pragma unroll 4
+      for (int k0 = 0; k0 < RW; k0 += PER) {
+        const int kr = k0 + (PC < 32 ? lane / PC : 0), r = pw + 4 * kr;
+        const long long o = __shfl_sync(0xffffffffu, mine, kr);
+#pragma unroll
+        for (int term = 0; term < (F32 ? 2 : 1); term++)
+#pragma unroll
+          for (int u = 0; u < (PC > 32 ? PC / 32 : 1); u++) {
+            const int k = (PC < 32 ? lane % PC : lane + 32 * u), n = r + term * ROWS;
+            // f32: the row's two f16 terms, [token, head][2][HD], from tree_split_kernel
+            const bool ok = o >= 0 && (F32 || k * 8 < p.hd);
+            const __half* src = F32 ? p.q_terms + ((size_t)(ok ? o : 0) * 2 + term) * HD
+                                    : reinterpret_cast<const __half*>(p.q) + (size_t)(ok ? o : 0) * p.hd;
+            cp16(qa + (k >> 3) * (N * 128) + n * 128 + (((k & 7) ^ (n & 7)) << 4), src + (ok ? k * 8 : 0), ok);
+          }
+      }
+      if (lane < RW) {
+        Sees v = {0, ~0ull};  // rows past the last one: their results are not written
+        if (mine >= 0) v = sees_of(p, w.s, t);
+        sees[sb * ROWS + r_mine] = v;
+        if constexpr (F32) scales[sb * ROWS + r_mine] = mine >= 0 ? p.q_scale[mine] : 0.f;
+      }
+      cp_arrive(&qlanded[sb]);
+    };
     for (int i = 0; i <= n_stages; i++) {
       if (i < n_stages) {
         const bool first = i == 0 || w.j == 0;
         if (first) tile_no++;
-        const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
-        off = -1;
+        if (i == 0) load_queries();  // nothing to wait for: all in flight before the first keys
+        long long off = -1;
         const int key = w.key0() + pw * 32 + lane;
-        if (key < w.s.L) off = row_offset(p, w.b, kvh, key);
+        if (key < w.s.L) off = row_offset(p, w.b, w.item / w.s.tiles, key);
         const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
         // (the ring holds at most five units, so the loads are at most five stages ahead of the softmax)
         if (lane == 0) okw[(i & 7) * 4 + pw] = there;
-        for (int u = 0; u < MB; u++) load_unit(p.k, off, u);
-        if (first) {
-          // ---- the tile's queries, what its rows see
-          const int qb = tile_no % NQ, sb = tile_no & 3;
-          if (tile_no >= NQ) {
-            (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
-            __syncwarp();
-          }
-          const int live = min(ROWS, w.s.T * p.group - tile * ROWS);
-          unsigned char* qs = smem + qb * C::Q_BYTES;
-          // lane k looks up row pw + 4 k of the tile: where its query is, and what it sees
-          constexpr int RW = ROWS / 4;
-          long long mine = -1;
-          if (lane < RW) {
-            const int r = pw + 4 * lane, gr = tile * ROWS + r, t = gr / p.group;
-            Sees v = {0, ~0ull};  // rows past the last one: their results are not written
-            if (r < live) {
-              mine = ((long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
-              v = sees_of(p, w.s, t);
-            }
-            sees[sb * ROWS + r] = v;
-          }
-          if constexpr (F32) {
-            constexpr int V4 = HD / 128, RB = 16 / V4 < RW ? 16 / V4 : RW;  // rows in flight (64 registers)
-#pragma unroll 1
-            for (int k0 = 0; k0 < RW; k0 += RB) {
-              float4 x[RB][V4];
+        rows.ok = 0;
 #pragma unroll
-              for (int q = 0; q < RB; q++) {
-                const long long o = __shfl_sync(0xffffffffu, mine, k0 + q);
-                const float* src = reinterpret_cast<const float*>(p.q) + o;
-#pragma unroll
-                for (int u = 0; u < V4; u++) {
-                  const int d = u * 128 + lane * 4;
-                  x[q][u] = (o >= 0 && d < p.hd) ? __ldg(reinterpret_cast<const float4*>(src + d))
-                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-              }
-#pragma unroll
-              for (int q = 0; q < RB; q++) {
-                const int r = pw + 4 * (k0 + q);
-                float big = 0.f;
-#pragma unroll
-                for (int u = 0; u < V4; u++)
-                  big = fmaxf(big, fmaxf(fmaxf(fabsf(x[q][u].x), fabsf(x[q][u].y)),
-                                         fmaxf(fabsf(x[q][u].z), fabsf(x[q][u].w))));
-#pragma unroll
-                for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                // 2^e brings the largest element to [2^10, 2^11); its exponent is read from the bits
-                int e = 0;
-                if (big > 0.f && big < INFINITY) e = max(-120, min(120, 137 - (int)(__float_as_uint(big) >> 23)));
-                const float up = __int_as_float((127 + e) << 23);
-                if (lane == 0) scales[sb * ROWS + r] = ldexpf(p.scale_log2, -e);
-#pragma unroll
-                for (int u = 0; u < V4; u++) {
-                  const float v[4] = {x[q][u].x * up, x[q][u].y * up, x[q][u].z * up, x[q][u].w * up};
-                  float lo[4];
-#pragma unroll
-                  for (int k = 0; k < 4; k++) lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
-                  // dims u * 128 + 4 lane: chunk 2 u + lane / 16, half of 16-byte piece (lane / 2) % 8
-                  const int ch = 2 * u + (lane >> 4), k = (lane >> 1) & 7;
-#pragma unroll
-                  for (int term = 0; term < 2; term++) {
-                    const int n = r + term * ROWS;
-                    const float* y = term ? lo : v;
-                    *reinterpret_cast<uint2*>(qs + ch * (N * 128) + n * 128 + ((k ^ (n & 7)) << 4) + (lane & 1) * 8) =
-                        make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
-                  }
-                }
-              }
-            }
-            mbar_arrive(&qlanded[sb]);
-          } else {
-            constexpr int PC = HD / 8;                     // 16-byte pieces of a row
-            constexpr int PER = PC < 32 ? 32 / PC : 1;     // rows per copy instruction
-            const uint32_t qa = smem_u32(qs);
-#pragma unroll 4
-            for (int k0 = 0; k0 < RW; k0 += PER) {
-              const int kr = k0 + (PC < 32 ? lane / PC : 0), r = pw + 4 * kr;
-              const long long o = __shfl_sync(0xffffffffu, mine, kr);
-#pragma unroll
-              for (int u = 0; u < (PC > 32 ? PC / 32 : 1); u++) {
-                const int k = (PC < 32 ? lane % PC : lane + 32 * u);
-                const bool ok = o >= 0 && k * 8 < p.hd;
-                cp16(qa + (k >> 3) * (N * 128) + r * 128 + (((k & 7) ^ (r & 7)) << 4),
-                     reinterpret_cast<const __half*>(p.q) + (ok ? o + k * 8 : 0), ok);
-              }
-            }
-            cp_arrive(&qlanded[sb]);
-          }
+        for (int it = 0; it < 8; it++) {
+          const int r = it * 4 + (lane >> 3);
+          const long long o = __shfl_sync(0xffffffffu, off, r);
+          rows.at[it] = o >= 0 ? (size_t)(o + k8) : 0;
+          rows.ok |= (o >= 0 ? 1u : 0u) << it;
         }
+        load_units(rows, p.k);
+        if (first && i > 0) load_queries();
       }
-      if (i > 0)
-        for (int u = 0; u < MB; u++) load_unit(p.v, off_prev, u);
-      off_prev = off;
+      if (i > 0) load_units(rows_before, p.v);
+      rows_before = rows;
       if (i + 1 < n_stages) w.next(p);
     }
     cp_wait_all();
   } else if (warp >= 12) {
     // ------------------------------------------------------------------------------ MMAs
     regs_down<kRegsMma>();
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
+      // The whole warp runs the loop and one elected lane issues: descriptors and column addresses are
+      // then uniform values the MMAs take as they are.  (From a loop that only lane 0 entered every
+      // MMA was issued 2.5 times slower than it ran: 128 against 54 cycles at N = 64.)
       constexpr uint32_t idesc_s = f16_idesc(N, false), idesc_o = f16_idesc(N, true, true);
+      auto ready = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity & 1u, abort_flag, p.err); };
+      const uint64_t dp = sw128_desc(sbase + C::OFF_P, 16384, 1024);
       Walk w = at;
-      int unit = 0, tile_no = -1, tile_o = -1;
+      int slot = 0, tile_no = -1, tile_o = -1;
+      uint32_t round = 0;  // of the ring
       bool first_prev = false, ok = true;
       for (int i = 0; ok && i <= n_stages; i++) {
         bool first = false;
         if (i < n_stages) {
           const int b = i & 1;
           first = i == 0 || w.j == 0;
+          const bool last = i + 1 == n_stages || w.j + 1 == w.s.stages;
           if (first) {
             tile_no++;
-            ok = wait(&qfull[tile_no & 3], (uint32_t)(tile_no >> 2), G4A_DEVERR_WAIT_FULL);
+            ok = ready(&qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
           }
-          if (ok && i >= 2) ok = wait(&sfree[b], (uint32_t)(i / 2 - 1), G4A_DEVERR_WAIT_MMA);
+          if (ok && i >= 2) ok = ready(&sfree[b], (uint32_t)(i / 2 - 1));
           const uint64_t dq = sw128_desc(sbase + (tile_no % NQ) * C::Q_BYTES, 16, 1024);
-          for (int u = 0; ok && u < MB; u++, unit++) {
-            const int slot = unit % UNITS;
-            ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
+          const uint32_t d = tmem + C::COL_S + (uint32_t)(b * N);
+#pragma unroll
+          for (int u = 0; u < MB; u++) {
+            if (ok) ok = ready(&full[slot], round);
             if (!ok) break;
             tc_fence_after();
             const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-              umma_f16_ss(tmem + C::COL_S + (uint32_t)(b * N), dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
-                          dq + (uint64_t)(((2 * u + (kk >> 2)) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
-                          (u > 0 || kk > 0) ? 1u : 0u);
-            umma_commit(&empty[slot]);
+              for (int kk = 0; kk < 8; kk++)
+                umma_f16_ss(d, dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                            dq + (uint64_t)(((2 * u + (kk >> 2)) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
+                            (u > 0 || kk > 0) ? 1u : 0u);
+              umma_commit(&empty[slot]);
+              if (u == MB - 1) {
+                umma_commit(&sfull[b]);
+                if (last) umma_commit(&qempty[tile_no % NQ]);
+              }
+            }
+            __syncwarp();
+            if (++slot == UNITS) slot = 0, round++;
           }
           if (!ok) break;
-          umma_commit(&sfull[b]);
-          if (i + 1 == n_stages || w.j + 1 == w.s.stages) umma_commit(&qempty[tile_no % NQ]);
         }
         if (i > 0) {  // O of stage i - 1
           if (first_prev) {
             tile_o++;
-            if (tile_o > 0) ok = wait(ofree, (uint32_t)(tile_o - 1), G4A_DEVERR_WAIT_MMA);
+            if (tile_o > 0) ok = ready(ofree, (uint32_t)(tile_o - 1));
           }
-          if (ok) ok = wait(pfull, (uint32_t)(i - 1), G4A_DEVERR_WAIT_MMA);
-          const uint64_t dp = sw128_desc(sbase + C::OFF_P, 16384, 1024);
-          for (int u = 0; ok && u < MB; u++, unit++) {
-            const int slot = unit % UNITS;
-            ok = wait(&full[slot], (uint32_t)(unit / UNITS), G4A_DEVERR_WAIT_FULL);
+          if (ok) ok = ready(pfull, (uint32_t)(i - 1));
+          const uint32_t go_on = first_prev ? 0u : 1u;
+#pragma unroll
+          for (int u = 0; u < MB; u++) {
+            if (ok) ok = ready(&full[slot], round);
             if (!ok) break;
             tc_fence_after();
             const uint64_t dv = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16384, 1024);
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-              umma_f16_ss(tmem + C::COL_O + (uint32_t)(u * N), dv + (uint64_t)((kk * 2048) >> 4),
-                          dp + (uint64_t)((kk * 2048) >> 4), idesc_o, (!first_prev || kk > 0) ? 1u : 0u);
-            umma_commit(&empty[slot]);
+              for (int kk = 0; kk < 8; kk++)
+                umma_f16_ss(tmem + C::COL_O + (uint32_t)(u * N), dv + (uint64_t)((kk * 2048) >> 4),
+                            dp + (uint64_t)((kk * 2048) >> 4), idesc_o, kk > 0 ? 1u : go_on);
+              umma_commit(&empty[slot]);
+              if (u == MB - 1) umma_commit(pvdone);
+            }
+            __syncwarp();
+            if (++slot == UNITS) slot = 0, round++;
           }
           if (!ok) break;
-          umma_commit(pvdone);
         }
         first_prev = first;
         if (i + 1 < n_stages) w.next(p);
       }
       // no MMA may still be running when TMEM is freed, also after an abort
-      umma_commit(mend);
+      if (elect_one()) umma_commit(mend);
+      __syncwarp();
       (void)mbar_wait_bounded(mend, 0, p.err, G4A_DEVERR_WAIT_MMA);
     }
     if (warp > 12) {
@@ -852,6 +854,46 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
 }
 
+// f32 queries as two f16 terms and a scale, one warp per (token, head): x 2^e = hi + lo with the
+// largest element brought to [2^10, 2^11), so that the low terms of every element that counts stay
+// above f16's smallest step.  terms [token, head][2][hd_pad], zero beyond head_dim; scale = scale
+// log2(e) 2^-e.  Once per call: inside the attention kernel every CTA of a long context would split
+// the same rows again (10 us of its start at 64 rows).
+__global__ void __launch_bounds__(256) tree_split_kernel(const float* q, __half* terms, float* scales, long long rows,
+                                                         int hd, int hd_pad, float scale_log2) {
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (row >= rows) return;
+  float4 x[4];
+  float big = 0.f;
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int d = u * 128 + lane * 4;
+    x[u] = d < hd ? *reinterpret_cast<const float4*>(q + row * hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    big = fmaxf(big, fmaxf(fmaxf(fabsf(x[u].x), fabsf(x[u].y)), fmaxf(fabsf(x[u].z), fabsf(x[u].w))));
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  int e = 0;
+  if (big > 0.f && big < INFINITY) e = max(-120, min(120, 137 - (int)(__float_as_uint(big) >> 23)));
+  const float up = __int_as_float((127 + e) << 23);
+  if (lane == 0) scales[row] = ldexpf(scale_log2, -e);
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int d = u * 128 + lane * 4;
+    if (d >= hd_pad) continue;
+    const float v[4] = {x[u].x * up, x[u].y * up, x[u].z * up, x[u].w * up};
+    float lo[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) lo[k] = v[k] - __half2float(__float2half_rn(v[k]));
+    __half* to = terms + row * 2 * hd_pad + d;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+    *reinterpret_cast<uint2*>(to + hd_pad) = make_uint2(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]));
+  }
+}
+
 template <int HD, int N, bool F32>
 g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long tokens_rows) {
   using C = Tc<HD, N, F32>;
@@ -869,10 +911,26 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
   const long long stages = (keys / kKeysT + p.batch) * tiles * p.nkh;
   p.grid = (int)std::max<long long>(1, std::min<long long>(stages, std::min(ctx->num_sms, kMaxGrid)));
   const size_t parts = (size_t)2 * p.grid * C::ROWS * (HD + 2) * sizeof(float);
-  if (g4a_status s = g4a_ensure_workspace(ctx, parts + (size_t)p.grid * sizeof(Cut))) return s;
-  p.part = static_cast<float*>(ctx->workspace);
-  p.cuts = reinterpret_cast<Cut*>(static_cast<char*>(ctx->workspace) + parts);
+  // workspace: the parts of cut tiles, the cuts, the queries' terms and scales (16-byte pieces)
+  const size_t cuts = ((size_t)p.grid * sizeof(Cut) + 15) & ~size_t(15);
+  const size_t rows = F32 ? (size_t)p.tokens * p.nqh : 0, terms = rows * 2 * HD * sizeof(__half);
+  const size_t need = parts + cuts + terms + rows * sizeof(float);
+  if (g4a_status s = g4a_ensure_workspace(ctx, need)) return s;
+  char* ws = static_cast<char*>(ctx->workspace);
+  p.part = reinterpret_cast<float*>(ws);
+  p.cuts = reinterpret_cast<Cut*>(ws + parts);
   g4a_prof_scope ps(ctx, G4A_PROF_TREE_ATTN);
+  if constexpr (F32) {
+    __half* q_terms = reinterpret_cast<__half*>(ws + parts + cuts);
+    float* q_scale = reinterpret_cast<float*>(ws + parts + cuts + terms);
+    p.q_terms = q_terms;
+    p.q_scale = q_scale;
+    if ((rows + 7) / 8 > 0x7fffffffull) return g4a_fail(G4A_EINVAL, "g4a_tree_attn_paged: num_tokens * num_q_heads too large");
+    const cudaError_t e = g4a_launch(tree_split_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, ctx->stream, true,
+                                     static_cast<const float*>(p.q), q_terms, q_scale, (long long)rows, p.hd, HD,
+                                     p.scale_log2);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "launch tree_split_kernel");
+  }
   const cudaError_t e =
       g4a_launch(tree_tc_kernel<HD, N, F32>, dim3(p.grid), dim3(kThreadsTc), C::SMEM, ctx->stream, true, p);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch tree_tc_kernel");
