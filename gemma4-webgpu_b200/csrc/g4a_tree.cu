@@ -34,13 +34,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // dims of 1 to 4 rows of a tile, spread over all CTAs: 256 threads = 32 float4 columns x 8, which
 // are lanes over the parts of a row (a long context has one tile with a part in every CTA) or rows
 // (a batch of short ones has many tiles of two parts).  A lane folds its parts one by one with a
-// running maximum, four loads ahead; the lanes of a row meet in shared memory.
+// running maximum, several loads ahead; the lanes of a row meet in shared memory.
 constexpr int kMergeThreads = 256;
-constexpr int kMaxCuts = 256;  // CTAs of the attention kernel
+constexpr int kMaxCuts = 512;  // two for each CTA of the attention kernel
 
 template <bool F32>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeParams p) {
-  __shared__ int ends[kMaxCuts];  // running count of units after cut c
+  __shared__ int ends[kMaxCuts];  // running count of units up to and with cut c
   __shared__ int warp_sum[kMergeThreads / 32];
   __shared__ float sm[8][2];
   __shared__ float4 so[8][32];
@@ -50,15 +50,21 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
   pdl_launch_dependents();
   auto lanes_of = [](int parts) { return parts > 4 ? 8 : parts > 2 ? 4 : 2; };
   {
-    int n = 0;
-    if (tid < p.grid) {
-      const int parts = p.cuts[tid].parts;
-      if (parts > 0) {
-        const int rows_per = 8 / lanes_of(parts);
-        n = (p.cuts[tid].rows + rows_per - 1) / rows_per * blocks;
+    int n[2], incl = 0;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const int c = 2 * tid + k;
+      n[k] = 0;
+      if (c < 2 * p.grid) {
+        const int parts = p.cuts[c].parts;
+        if (parts > 0) {
+          const int rows_per = 8 / lanes_of(parts);
+          n[k] = (p.cuts[c].rows + rows_per - 1) / rows_per * blocks;
+        }
       }
+      incl += n[k];
     }
-    int incl = n;
+    const int both = incl;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
@@ -67,13 +73,14 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     if (lane == 31) warp_sum[sub] = incl;
     __syncthreads();
     for (int w = 0; w < sub; w++) incl += warp_sum[w];
-    ends[tid] = incl;
+    ends[2 * tid] = incl - both + n[0];
+    ends[2 * tid + 1] = incl;
     __syncthreads();
   }
-  const int total = ends[kMergeThreads - 1];
+  const int total = ends[kMaxCuts - 1];
   const size_t stride = (size_t)p.rows * (p.hd_pad + 2);
   for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
-    int lo = 0, hi = kMergeThreads - 1;  // the first cut whose end is above the unit
+    int lo = 0, hi = kMaxCuts - 1;  // the first cut whose end is above the unit
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (ends[mid] > unit) hi = mid;
@@ -87,9 +94,11 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < cut.rows) {
-#pragma unroll 4
-      for (int i = part0; i < cut.parts; i += pl) {
-        const float* base = p.part + (i == 0 ? (size_t)cut.slot : (size_t)2 * (lo + i)) * stride;
+      Split split;
+      split.each = cut.each;
+      split.extra = cut.extra;
+      auto fold = [&](size_t slot) {
+        const float* base = p.part + slot * stride;
         const float mi = __ldcg(base + (size_t)p.rows * p.hd_pad + r);
         const float li = __ldcg(base + (size_t)p.rows * p.hd_pad + p.rows + r);
         const float4 x = __ldcg(reinterpret_cast<const float4*>(base + (size_t)r * p.hd_pad + d));
@@ -102,6 +111,18 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
         o.y = wo * o.y + wi * x.y;
         o.z = wo * o.z + wi * x.z;
         o.w = wo * o.w + wi * x.w;
+      };
+      if (cut.chunks == 1) {
+        // the piece that begins the tile is in slot lo, the others begin their CTAs' runs
+#pragma unroll 4
+        for (int i = part0; i < cut.parts; i += pl) fold(i == 0 ? (size_t)lo : (size_t)2 * (lo / 2 + i));
+      } else {
+        for (int c = part0; c < cut.chunks; c += pl) {
+          const int j0 = chunk_at(cut.stages, cut.chunks, c), j1 = chunk_at(cut.stages, cut.chunks, c + 1);
+          const long long s0 = cut.base + (long long)cut.tiles * j0 + (long long)cut.tile * (j1 - j0);
+          const long long c0 = split.owner(s0), c1 = split.owner(s0 + (j1 - j0) - 1);
+          for (long long k = c0; k <= c1; k++) fold((size_t)(2 * k + (k == c0 && s0 > split.begin(k) ? 1 : 0)));
+        }
       }
     }
     if (lane == 0) sm[sub][0] = m, sm[sub][1] = l;
@@ -169,6 +190,9 @@ extern "C" g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t 
     return g4a_fail(G4A_EINVAL, "%s: page_size, max_pages_per_seq or num_pages out of range", fn);
   if ((uint64_t)page_size * max_pages_per_seq > 0x7fff0000ull)
     return g4a_fail(G4A_EINVAL, "%s: page_size * max_pages_per_seq exceeds 2^31", fn);
+  // (rows are addressed in 16-byte units of 32 bits)
+  if ((uint64_t)num_pages * page_size * num_kv_heads > 0xffffffffull / (head_dim / 8))
+    return g4a_fail(G4A_EINVAL, "%s: a page pool of more than 64 GiB", fn);
   g4a_device_guard dev(ctx);
   if (dev.status != G4A_OK) return dev.status;
   TreeParams p = {};

@@ -23,20 +23,22 @@ struct TreeParams {
   int grid;       // CTAs of the launched kernel
   float* part;    // [2 * grid] partial rows: o [rows, hd_pad] | m [rows] | l [rows]
   int hd_pad;
-  struct Cut* cuts;  // [grid]
+  struct Cut* cuts;  // [2 * grid]
   const __half* q_terms;  // f32 queries: [tokens, nqh][2][hd_pad], high and low f16 terms
   const float* q_scale;   // and [tokens, nqh] scale * log2(e) over the power of two in them
   int* err;
 };
 
-// A tile whose keys were cut between CTAs, written by the CTA c that has its first stages; its
-// parts are in slot `slot` (2 c or 2 c + 1) and then in slots 2 (c + 1), 2 (c + 2), ...
+// A tile whose keys were not all done by one CTA, written by the CTA that has its first piece, at the
+// index of that piece's slot.
 struct Cut {
-  int parts;  // 0: CTA c began no such tile
-  int slot;
-  int rows;         // query rows of the tile that exist
-  int row0;         // the sequence's first row of q
-  int kvh, first;   // kv head; the tile's first row in units of (token, head of the group)
+  int parts;             // pieces (chunks == 1) or chunks to be joined; 0: nothing
+  int rows;              // query rows of the tile that exist
+  int row0;              // the sequence's first row of q
+  int kvh, first;        // kv head; the tile's first row in units of (token, head of the group)
+  int stages, chunks, tiles, tile;
+  int each, extra;       // the split of the list over the CTAs
+  long long base;        // stage of the list at which the (sequence, kv head) begins
 };
 
 // One sequence: T drafted tokens (rows row0 .. of q), base older rows, keys [lo, L) to be read.
@@ -71,8 +73,13 @@ __device__ __forceinline__ long long stages_of(const TreeParams& p, const Seq& s
   return (long long)p.nkh * s.tiles * s.stages;
 }
 
-// The flattened list of (sequence, kv head, tile, stage) is cut into equal runs, one per CTA;
-// only the first min(grid, total) CTAs have work.
+// The list of all stages is cut into equal runs, one per CTA; only the first min(grid, total) CTAs
+// have work.  Order: sequence, kv head, chunk of keys, tile, stage.  The tiles of a kv head read the
+// same keys, so its keys are cut into chunks about as long as a run and a chunk's tiles follow one
+// another: their CTAs read the same rows at the same time, and only the first reads them from HBM.
+// (Tile after tile, the six tiles of a 131,000-key context came past each row 90 MB apart and the L2
+// had lost it.)  A chunk is at least as long as a run, so a run holds at most two pieces of tiles
+// that are not whole: one that begins before or with it and one that goes on after it.
 struct Split {
   long long total, active, each, extra;
   __device__ __forceinline__ void of(long long t, int grid) {
@@ -86,6 +93,72 @@ struct Split {
   __device__ __forceinline__ long long owner(long long s) const {
     const long long cut = extra * (each + 1);
     return s < cut ? s / (each + 1) : extra + (s - cut) / each;
+  }
+};
+
+// First stage of chunk c of n stages in `chunks`.
+__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)((long long)n * c / chunks); }
+
+// Where a role stands in the CTA's run of stages.
+struct Walk {
+  Seq s;
+  int b, kvh, tile;
+  int chunks, chunk, j, j_end;  // stage of the tile; end of the chunk
+
+  __device__ __forceinline__ void chunk_of(const Split& split) {
+    chunks = s.tiles > 1 ? max(1, (int)min((long long)s.stages, s.stages / max(1ll, split.each))) : 1;
+  }
+  // stage `local` of sequence b's list
+  __device__ __forceinline__ void seek(const TreeParams& p, const Split& split, int seq, long long local) {
+    b = seq;
+    s = seq_of(p, b);
+    chunk_of(split);
+    const long long per_head = (long long)s.tiles * s.stages;
+    kvh = (int)(local / per_head);
+    local -= kvh * per_head;
+    chunk = (int)(local / s.tiles * chunks / s.stages);
+    while (chunk > 0 && local < (long long)s.tiles * chunk_at(s.stages, chunks, chunk)) chunk--;
+    while (local >= (long long)s.tiles * chunk_at(s.stages, chunks, chunk + 1)) chunk++;
+    const int j0 = chunk_at(s.stages, chunks, chunk);
+    j_end = chunk_at(s.stages, chunks, chunk + 1);
+    local -= (long long)s.tiles * j0;
+    tile = (int)(local / (j_end - j0));
+    j = j0 + (int)(local - (long long)tile * (j_end - j0));
+  }
+  // past the end of a tile's chunk
+  __device__ __forceinline__ void next_piece(const TreeParams& p, const Split& split) {
+    if (++tile == s.tiles) {
+      tile = 0;
+      if (++chunk == chunks) {
+        chunk = 0;
+        if (++kvh == p.nkh) {
+          kvh = 0;
+          do {
+            if (++b >= p.batch) {
+              s.stages = 0;
+              return;
+            }
+            s = seq_of(p, b);
+          } while (s.stages == 0);
+          chunk_of(split);
+        }
+      }
+    }
+    j = chunk_at(s.stages, chunks, chunk);
+    j_end = chunk_at(s.stages, chunks, chunk + 1);
+  }
+  __device__ __forceinline__ void next(const TreeParams& p, const Split& split) {
+    if (++j == j_end) next_piece(p, split);
+  }
+  __device__ __forceinline__ bool begins() const { return j == chunk_at(s.stages, chunks, chunk); }
+  // the first key from which every row sees all of the prefix
+  __device__ __forceinline__ int kfull(const TreeParams& p) const {
+    const long long k = p.window ? (long long)s.base + s.T - (long long)p.window : 0;
+    return k < 0 ? 0 : k > s.base ? s.base : (int)k;
+  }
+  __device__ __forceinline__ int key0(const TreeParams& p) const { return s.lo + j * p.kps; }
+  __device__ __forceinline__ bool clean(const TreeParams& p) const {
+    return key0(p) >= kfull(p) && key0(p) + p.kps <= s.base;
   }
 };
 

@@ -47,9 +47,6 @@ using namespace g4a_tree;
 constexpr int kKeysT = 128;
 constexpr int kMaxGrid = 256;        // (the join looks at one cut per thread)
 constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one MMA and handing over
-// Registers: 512 threads start with 128 each (65,536); the softmax warpgroups, which hold a row
-// block of scores and sums, take 168, the others give theirs: 256 * 168 + 128 * 96 + 128 * 72 = 64,512.
-constexpr int kRegsSoftmax = 168, kRegsLoad = 96, kRegsMma = 72;
 constexpr int kUnit = 32768;         // 128 keys x 128 dims f16
 constexpr float kPUp = 7.0f;         // p = 2^(s - m + 7)
 constexpr float kRaise = 8.0f;       // a score this far above m raises it
@@ -62,6 +59,12 @@ struct Tc {
   static constexpr int RH = ROWS / 2;                 // rows of a softmax half
   static constexpr int W = RH < 32 ? RH : 32;         // rows a thread works on at a time
   static constexpr int G = RH / W;
+  // Registers: 512 threads start with 128 each (65,536).  The softmax warpgroups, which hold a block
+  // of scores and row sums, take more and the others give theirs.  (Spills are dear here: shared
+  // memory leaves the L1 almost nothing, so local memory is in the L2.)
+  static constexpr int REGS_SOFTMAX = G > 1 ? 184 : N > 64 ? 168 : 160;
+  static constexpr int REGS_LOAD = G > 1 ? 80 : N > 64 ? 96 : 112, REGS_MMA = G > 1 ? 64 : 80;
+  static_assert(256 * REGS_SOFTMAX + 128 * REGS_LOAD + 128 * REGS_MMA <= 65536, "register file");
   static constexpr int Q_BYTES = N * HD * 2;
   static constexpr int P_BYTES = kKeysT * N * 2;
   static constexpr int FIT2 = (216 * 1024 - 2 * Q_BYTES - P_BYTES) / kUnit;
@@ -77,8 +80,10 @@ struct Tc {
   static constexpr int OFF_MAX = OFF_F + 8 * RH * 4;          // [2 halves][4 quarters][RH]
   static constexpr int OFF_OK = OFF_MAX + 8 * RH * 4;         // [8 stages][4] which rows are there
   static constexpr int OFF_BAD = OFF_OK + 128;                // [8] tile + 1 that had a V value that is not finite
-  static constexpr int OFF_BAR = OFF_BAD + 32;
-  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5;
+  static constexpr int OFF_VOTE = OFF_BAD + 32;               // [2 halves][2][4 quarters]
+  static constexpr int OFF_INFO = OFF_VOTE + 64;               // [4] Walk of a piece's begin
+  static constexpr int OFF_BAR = OFF_INFO + 4 * 64;
+  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5 + 2;
   static constexpr int OFF_END = OFF_BAR + NBARS * 8;
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
@@ -141,20 +146,6 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-// Whether any of `count` threads (whole warps) says so; a barrier among them.
-__device__ __forceinline__ bool any_of(uint32_t id, uint32_t count, bool pred) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.u32 p, %3, 0;\n\t"
-      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(id), "r"(count), "r"(pred ? 1u : 0u)
-      : "memory");
-  return r != 0;
-}
-
 // Reduces W values per lane over the warp's lanes, value n's result in lane n (W = 16: also in lane
 // n + 16).  Each step hands half of the values to the lane at distance o and keeps the other half.
 template <int W, typename Op>
@@ -178,30 +169,6 @@ __device__ __forceinline__ float transpose_reduce(const float (&x)[W], Op op) {
   }
   return v[0];
 }
-
-// Where a role stands in the CTA's run of stages.
-struct Walk {
-  Seq s;
-  int b, item, j;  // item = kv head * tiles + tile
-  __device__ __forceinline__ void next(const TreeParams& p) {
-    if (++j < s.stages) return;
-    j = 0;
-    item++;
-    while (b < p.batch && (s.stages == 0 || item == p.nkh * s.tiles)) {
-      item = 0;
-      if (++b < p.batch) s = seq_of(p, b);
-    }
-  }
-  // the first key from which every row sees all of the prefix
-  __device__ __forceinline__ int kfull(const TreeParams& p) const {
-    const long long k = p.window ? (long long)s.base + s.T - (long long)p.window : 0;
-    return k < 0 ? 0 : k > s.base ? s.base : (int)k;
-  }
-  __device__ __forceinline__ int key0() const { return s.lo + j * kKeysT; }
-  __device__ __forceinline__ bool clean(const TreeParams& p) const {
-    return key0() >= kfull(p) && key0() + kKeysT <= s.base;
-  }
-};
 
 // Head dim d of `rows` query rows (from row gr0 of the kv head): adds the infinities and NaN of the V
 // values that were taken out of the tile's stages from key0 on, for the rows that see their keys, to
@@ -245,6 +212,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   Sees* sees = reinterpret_cast<Sees*>(smem + C::OFF_SEES);
   float* scales = reinterpret_cast<float*>(smem + C::OFF_SCALE);
   uint32_t* okw = reinterpret_cast<uint32_t*>(smem + C::OFF_OK);
+  // Only the loads walk through the list; the other roles read where a piece lies from here.
+  Walk* pieces = reinterpret_cast<Walk*>(smem + C::OFF_INFO);
+  static_assert(sizeof(Walk) <= 64, "piece ring");
   volatile int* badv = reinterpret_cast<volatile int*>(smem + C::OFF_BAD);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* landed = bars;              // [UNITS] 128 loading threads
@@ -259,6 +229,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   uint64_t* pvdone = pfull + 1;         // MMA commit
   uint64_t* ofree = pvdone + 1;         // 8 softmax warps
   uint64_t* mend = ofree + 1;           // MMA commit
+  uint64_t* meet_bar = mend + 1;        // [2 halves] its 4 softmax warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
 
@@ -283,8 +254,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     mbar_init(pvdone, 1);
     mbar_init(ofree, 8);
     mbar_init(mend, 1);
+    mbar_init(&meet_bar[0], 4);
+    mbar_init(&meet_bar[1], 4);
     *abort_flag = 0;
     for (int u = 0; u < 8; u++) badv[u] = 0;
+    for (int u = 0; u < 4; u++) pieces[u] = Walk{};  // (what a role reads that had to give up a wait)
     fence_mbar_init();
   }
   if (warp == 12) {  // one CTA per SM (shared memory), so the allocation never waits
@@ -309,37 +283,44 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   const long long s0 = cta < split.active ? split.begin(cta) : 0;
   const int n_stages = cta < split.active ? (int)(split.begin(cta + 1) - s0) : 0;
   Walk at = {};
-  if (n_stages > 0) {
+  if (n_stages > 0 && (warp == 15 || (warp >= 8 && warp < 12))) {
     long long first = 0;
-    at.b = find_seq(p, s0, first);
-    at.s = seq_of(p, at.b);
-    at.item = (int)((s0 - first) / at.s.stages);
-    at.j = (int)((s0 - first) % at.s.stages);
-  }
-
-  if (tid == 0) {
-    // the tile that this CTA begins and others go on with, if there is one: its last
-    Walk w = at;
-    Cut c = {};
-    int begun = 0;  // stage of this CTA's run at which the last tile begins
-    for (int i = 0; i < n_stages;) {
-      begun = i;
-      i += w.s.stages - w.j;
-      if (i >= n_stages) break;
-      w.j = w.s.stages - 1;
-      w.next(p);
+    const int b = find_seq(p, s0, first);
+    at.seek(p, split, b, s0 - first);
+    if (warp == 15) {
+      // the tiles that are not whole and whose first pieces lie here: one at the run's begin, one at its end
+      Walk w = at;
+      long long s = s0;  // where piece w begins in this run
+      bool end_too = true;
+      for (int piece = 0; piece < 2; piece++) {
+        Cut c = {};
+        const long long s1 = min(s + (w.j_end - w.j), s0 + n_stages);
+        const bool whole = w.chunks == 1 && s1 - s == w.s.stages;
+        if ((piece == 0 || end_too) && w.j == 0 && !whole) {
+          c.base = s - (long long)w.tile * w.j_end;
+          c.stages = w.s.stages;
+          c.chunks = w.chunks;
+          c.tiles = w.s.tiles;
+          c.tile = w.tile;
+          c.each = (int)split.each;
+          c.extra = (int)split.extra;
+          c.parts = w.chunks > 1 ? w.chunks : (int)(split.owner(s + w.s.stages - 1) - cta) + 1;
+          c.rows = min(ROWS, w.s.T * p.group - w.tile * ROWS);
+          c.row0 = w.s.row0;
+          c.kvh = w.kvh;
+          c.first = w.tile * ROWS;
+        }
+        if (lane == 0) p.cuts[2 * cta + piece] = c;
+        // to the run's last piece
+        end_too = s1 < s0 + n_stages;
+        while (s + (w.j_end - w.j) < s0 + n_stages) {
+          s += w.j_end - w.j;
+          w.next_piece(p, split);
+        }
+      }
     }
-    const long long end = s0 + begun - w.j + w.s.stages;  // the tile's end in the list
-    if (n_stages > 0 && w.j == 0 && end > s0 + n_stages) {
-      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
-      c.parts = (int)(split.owner(end - 1) - cta) + 1;
-      c.slot = (int)(2 * cta) + (begun > 0 ? 1 : 0);
-      c.rows = min(ROWS, w.s.T * p.group - tile * ROWS);
-      c.row0 = w.s.row0;
-      c.kvh = kvh;
-      c.first = tile * ROWS;
-    }
-    p.cuts[cta] = c;
+  } else if (n_stages == 0 && warp == 15 && lane == 0) {
+    p.cuts[2 * cta].parts = p.cuts[2 * cta + 1].parts = 0;
   }
   __syncwarp();
   const uint32_t tmem = *tmem_slot;
@@ -350,20 +331,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
 
   if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------------------------ loads
-    regs_down<kRegsLoad>();
+    regs_down<C::REGS_LOAD>();
     const int pw = warp - 8;
     int issued = 0;  // units
     // A lane copies the 16-byte pieces k = lane % 8 of rows 32 pw + 4 it + lane / 8, it = 0..7; what it
     // needs of a stage's rows is looked up once and kept for all units of K and, later, of V.
     struct Rows {
-      size_t at[8];  // the row's piece, in elements from the pool's start
-      uint32_t ok;   // bit it: the row is there
+      uint32_t at[8];  // the row's piece, in 16-byte units from the pool's start
+      uint32_t ok;     // bit it: the row is there
     };
     const int k8 = (lane & 7) * 8;
     const uint32_t lane_dst = (uint32_t)(pw * 4096 + (lane >> 3) * 128);
     const uint32_t sw0 = (uint32_t)(((lane & 7) ^ (lane >> 3)) << 4), sw1 = sw0 ^ 64u;  // it even, odd
     auto load_units = [&](const Rows& rows, const __half* pool) {
-#pragma unroll
+#pragma unroll 1
       for (int u = 0; u < MB; u++) {
         const int slot = issued % UNITS;
         if (issued >= UNITS) {
@@ -376,7 +357,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         for (int it = 0; it < 8; it++) {
           const uint32_t to = dst + it * 512 + (it & 1 ? sw1 : sw0);
           const bool ok = (rows.ok >> it) & 1u;
-          const __half* from = pool + rows.at[it];
+          const __half* from = pool + (size_t)rows.at[it] * 8;
           cp16(to, from + (in0 ? u * 128 : 0), ok && in0);
           cp16(to + 16384, from + (in1 ? u * 128 + 64 : 0), ok && in1);
         }
@@ -390,7 +371,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     // The tile's queries into Q buffer tile_no % NQ, and what its rows see.  Lane k looks up row
     // pw + 4 k of the tile.
     auto load_queries = [&]() {
-      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
+      const int kvh = w.kvh, tile = w.tile;
       const int qb = tile_no % NQ, sb = tile_no & 3;
       if (tile_no >= NQ) {
         (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
@@ -421,6 +402,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             cp16(qa + (k >> 3) * (N * 128) + n * 128 + (((k & 7) ^ (n & 7)) << 4), src + (ok ? k * 8 : 0), ok);
           }
       }
+      if (pw == 0 && lane == 0) pieces[sb] = w;
       if (lane < RW) {
         Sees v = {0, ~0ull};  // rows past the last one: their results are not written
         if (mine >= 0) v = sees_of(p, w.s, t);
@@ -431,12 +413,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     };
     for (int i = 0; i <= n_stages; i++) {
       if (i < n_stages) {
-        const bool first = i == 0 || w.j == 0;
+        const bool first = i == 0 || w.begins();
         if (first) tile_no++;
         if (i == 0) load_queries();  // nothing to wait for: all in flight before the first keys
         long long off = -1;
-        const int key = w.key0() + pw * 32 + lane;
-        if (key < w.s.L) off = row_offset(p, w.b, w.item / w.s.tiles, key);
+        const int key = w.key0(p) + pw * 32 + lane;
+        if (key < w.s.L) off = row_offset(p, w.b, w.kvh, key);
         const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
         // (the ring holds at most five units, so the loads are at most five stages ahead of the softmax)
         if (lane == 0) okw[(i & 7) * 4 + pw] = there;
@@ -445,7 +427,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         for (int it = 0; it < 8; it++) {
           const int r = it * 4 + (lane >> 3);
           const long long o = __shfl_sync(0xffffffffu, off, r);
-          rows.at[it] = o >= 0 ? (size_t)(o + k8) : 0;
+          rows.at[it] = o >= 0 ? (uint32_t)((o + k8) >> 3) : 0u;
           rows.ok |= (o >= 0 ? 1u : 0u) << it;
         }
         load_units(rows, p.k);
@@ -453,12 +435,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       }
       if (i > 0) load_units(rows_before, p.v);
       rows_before = rows;
-      if (i + 1 < n_stages) w.next(p);
+      if (i + 1 < n_stages) w.next(p, split);
     }
     cp_wait_all();
   } else if (warp >= 12) {
     // ------------------------------------------------------------------------------ MMAs
-    regs_down<kRegsMma>();
+    regs_down<C::REGS_MMA>();
     if (warp == 12) {
       // The whole warp runs the loop and one elected lane issues: descriptors and column addresses are
       // then uniform values the MMAs take as they are.  (From a loop that only lane 0 entered every
@@ -466,35 +448,37 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       constexpr uint32_t idesc_s = f16_idesc(N, false), idesc_o = f16_idesc(N, true, true);
       auto ready = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity & 1u, abort_flag, p.err); };
       const uint64_t dp = sw128_desc(sbase + C::OFF_P, 16384, 1024);
-      Walk w = at;
-      int slot = 0, tile_no = -1, tile_o = -1;
+      int slot = 0, tile_no = -1, tile_o = -1, j = 0, j_end = 0;
       uint32_t round = 0;  // of the ring
       bool first_prev = false, ok = true;
       for (int i = 0; ok && i <= n_stages; i++) {
         bool first = false;
         if (i < n_stages) {
           const int b = i & 1;
-          first = i == 0 || w.j == 0;
-          const bool last = i + 1 == n_stages || w.j + 1 == w.s.stages;
+          first = j == j_end;
           if (first) {
             tile_no++;
             ok = ready(&qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+            j = pieces[tile_no & 3].j;
+            j_end = pieces[tile_no & 3].j_end;
           }
+          const bool last = i + 1 == n_stages || ++j == j_end;
           if (ok && i >= 2) ok = ready(&sfree[b], (uint32_t)(i / 2 - 1));
           const uint64_t dq = sw128_desc(sbase + (tile_no % NQ) * C::Q_BYTES, 16, 1024);
           const uint32_t d = tmem + C::COL_S + (uint32_t)(b * N);
-#pragma unroll
+#pragma unroll 1
           for (int u = 0; u < MB; u++) {
             if (ok) ok = ready(&full[slot], round);
             if (!ok) break;
             tc_fence_after();
             const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
+            const uint64_t dqu = dq + (uint64_t)((u * 2 * N * 128) >> 4);
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < 8; kk++)
                 umma_f16_ss(d, dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
-                            dq + (uint64_t)(((2 * u + (kk >> 2)) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
-                            (u > 0 || kk > 0) ? 1u : 0u);
+                            dqu + (uint64_t)(((kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
+                            kk > 0 ? 1u : u > 0 ? 1u : 0u);
               umma_commit(&empty[slot]);
               if (u == MB - 1) {
                 umma_commit(&sfull[b]);
@@ -513,7 +497,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           }
           if (ok) ok = ready(pfull, (uint32_t)(i - 1));
           const uint32_t go_on = first_prev ? 0u : 1u;
-#pragma unroll
+#pragma unroll 1
           for (int u = 0; u < MB; u++) {
             if (ok) ok = ready(&full[slot], round);
             if (!ok) break;
@@ -533,7 +517,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           if (!ok) break;
         }
         first_prev = first;
-        if (i + 1 < n_stages) w.next(p);
       }
       // no MMA may still be running when TMEM is freed, also after an abort
       if (elect_one()) umma_commit(mend);
@@ -548,7 +531,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       // V of keys that not every row sees: p = 0 times an infinite or NaN V would reach the rows
       // that do not.  Such values become 0 here, and the epilogue adds them to the rows that do.
       const int hw = warp - 13;
-      Walk w = at, before = at;
+      Walk w = {}, before = {};
       int unit = 0, tile_no = -1, tile_before = 0;
       auto pass = [&](uint64_t* from, uint64_t* to, uint32_t parity) {
         (void)warp_wait(from, parity & 1u, abort_flag, p.err);
@@ -558,18 +541,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       };
       for (int i = 0; i <= n_stages; i++) {
         if (i < n_stages) {
-          const bool first = i == 0 || w.j == 0;
-          if (first) tile_no++;
           for (int u = 0; u < MB; u++, unit++)
             pass(&landed[unit % UNITS], &full[unit % UNITS], (uint32_t)(unit / UNITS));
-          if (first) pass(&qlanded[tile_no & 3], &qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+          if (w.j == w.j_end) {
+            tile_no++;
+            pass(&qlanded[tile_no & 3], &qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+            w = pieces[tile_no & 3];
+          }
         }
         if (i > 0) {
           const bool mixed = !before.clean(p);
           for (int u = 0; u < MB; u++, unit++) {
             if (mixed) {
               (void)warp_wait(&landed[unit % UNITS], (uint32_t)(unit / UNITS) & 1u, abort_flag, p.err);
-              const int k0 = before.key0(), a1 = before.kfull(p) - k0, b0 = before.s.base - k0, b1 = before.s.L - k0;
+              const int k0 = before.key0(p), a1 = before.kfull(p) - k0, b0 = before.s.base - k0, b1 = before.s.L - k0;
               unsigned char* x0 = smem + C::OFF_RING + (unit % UNITS) * kUnit;
               bool bad = false;
               for (int e = hw * 32 + lane; e < kKeysT * 16; e += 96) {
@@ -589,47 +574,68 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         }
         before = w;
         tile_before = tile_no;
-        if (i + 1 < n_stages) w.next(p);
+        w.j++;
       }
     }
   } else {
     // ------------------------------------------------------------------------------ softmax
-    regs_up<kRegsSoftmax>();
+    regs_up<C::REGS_SOFTMAX>();
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     float* su = reinterpret_cast<float*>(smem + C::OFF_U) + warp * RH;
     float* sf = reinterpret_cast<float*>(smem + C::OFF_F) + warp * RH;
     float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX) + half * 4 * RH;
-    const uint32_t bar_id = 1 + half;
+    int* votes = reinterpret_cast<int*>(smem + C::OFF_VOTE) + half * 8;
+    // The half's four warps meet (a bounded wait like every other); what they wrote before is visible
+    // after.  `votes` alternates between two sets, so that nobody writes what another still reads.
+    uint32_t met = 0;
+    auto meet = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&meet_bar[half]);
+      (void)warp_wait(&meet_bar[half], met & 1u, abort_flag, p.err);
+      met++;
+    };
+    auto any_of = [&](bool pred) {
+      const bool mine = __any_sync(0xffffffffu, pred);
+      int* v = votes + (met & 1) * 4;
+      if (lane == 0) v[quarter] = mine ? 1 : 0;
+      meet();
+      const int4 all = *reinterpret_cast<const int4*>(v);
+      return (all.x | all.y | all.z | all.w) != 0;
+    };
     const int key_in = quarter * 32 + lane;  // this thread's key of a stage
     unsigned char* prow = smem + C::OFF_P + key_in * 128;
-    Walk w = at;
+    Walk w = {};
     int tile_no = -1, j_first = 0;
     float m[G];     // lane n: running maximum of row g * W + n of this half
     float l[G][W];  // this thread's keys' share of the row sums
+    auto reset = [&]() {
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        m[g] = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < W; n++) l[g][n] = 0.f;
+      }
+      __syncwarp();
+      for (int n = lane; n < RH; n += 32) su[n] = kUnseen;
+      __syncwarp();
+    };
+    reset();
     for (int i = 0; i < n_stages; i++) {
       const int b = i & 1;
-      const bool first = i == 0 || w.j == 0;
-      const bool last = i + 1 == n_stages || w.j + 1 == w.s.stages;
-      const int kvh = w.item / w.s.tiles, tile = w.item - kvh * w.s.tiles;
-      const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - half * RH;  // rows of this half
-      if (first) {
-        tile_no++;
-        j_first = w.j;
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          m[g] = -INFINITY;
-#pragma unroll
-          for (int n = 0; n < W; n++) l[g][n] = 0.f;
-        }
-        __syncwarp();
-        for (int n = lane; n < RH; n += 32) su[n] = kUnseen;
-        __syncwarp();
-      }
+      const bool first = w.j == w.j_end;
       (void)warp_wait(&sfull[b], (uint32_t)(i >> 1) & 1u, abort_flag, p.err);
       tc_fence_after();
+      if (first) {
+        tile_no++;
+        w = pieces[tile_no & 3];
+        j_first = w.j;
+      }
+      const bool last = i + 1 == n_stages || w.j + 1 == w.j_end;
+      const int kvh = w.kvh, tile = w.tile;
+      const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - half * RH;  // rows of this half
       if (live > 0) {
-        const int key0 = w.key0(), key = key0 + key_in;
+        const int key0 = w.key0(p), key = key0 + key_in;
         const uint4 ok4 = *reinterpret_cast<const uint4*>(okw + (i & 7) * 4);
         const bool clean = w.clean(p) && (ok4.x & ok4.y & ok4.z & ok4.w) == ~0u;
         const uint32_t okq = quarter == 0 ? ok4.x : quarter == 1 ? ok4.y : quarter == 2 ? ok4.z : ok4.w;
@@ -685,10 +691,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             over |= x[n + 2] - u.z > kPUp + kRaise;
             over |= x[n + 3] - u.w > kPUp + kRaise;
           }
-          if (any_of(bar_id, 128, over)) {
+          if (any_of(over)) {
             const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
             if (lane < W) smax[quarter * RH + g * W + lane] = mine;
-            named_bar_sync(bar_id, 128);
+            meet();
             const int n_of = g * W + (lane % W);
             const float mx = fmaxf(fmaxf(smax[n_of], smax[RH + n_of]), fmaxf(smax[2 * RH + n_of], smax[3 * RH + n_of]));
             const bool raise = mx > m[g] + kRaise;
@@ -771,17 +777,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         (void)warp_wait(pvdone, (uint32_t)i & 1u, abort_flag, p.err);
         tc_fence_after();
         if (live > 0) {
-          const bool whole = j_first == 0 && w.j + 1 == w.s.stages;
-          const bool later = i - (w.j - j_first) > 0;  // not the tile this CTA's run begins with
+          const bool whole = w.chunks == 1 && j_first == 0 && w.j + 1 == w.s.stages;
+          const bool later = i - (w.j - j_first) > 0;  // not the piece this CTA's run begins with
           float* part = p.part + (size_t)(2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
           float lt[G];
-          named_bar_sync(bar_id, 128);  // smax is free
+          meet();  // smax is free
 #pragma unroll
           for (int g = 0; g < G; g++) {
             const float mine = transpose_reduce<W>(l[g], [](float a, float c) { return a + c; });
             if (lane < W) smax[quarter * RH + g * W + lane] = mine;
           }
-          named_bar_sync(bar_id, 128);
+          meet();
 #pragma unroll
           for (int g = 0; g < G; g++) {
             const int n_of = g * W + (lane % W);
@@ -834,7 +840,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
                 if (n < nl) part[(size_t)(half * RH + g * W + n) * HD + d] = o[n];
             }
             if (bad && d < p.hd)
-              add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0() + kKeysT, w.s.L), w.kfull(p),
+              add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0(p) + kKeysT, w.s.L), w.kfull(p),
                                   d, tile * ROWS + half * RH + g * W, nl,
                                   whole ? nullptr : part + (size_t)(half * RH + g * W) * HD, HD);
           }
@@ -842,8 +848,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ofree);
+        reset();
       }
-      if (i + 1 < n_stages) w.next(p);
+      w.j++;
     }
   }
   __syncwarp();
@@ -912,7 +919,7 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
   p.grid = (int)std::max<long long>(1, std::min<long long>(stages, std::min(ctx->num_sms, kMaxGrid)));
   const size_t parts = (size_t)2 * p.grid * C::ROWS * (HD + 2) * sizeof(float);
   // workspace: the parts of cut tiles, the cuts, the queries' terms and scales (16-byte pieces)
-  const size_t cuts = ((size_t)p.grid * sizeof(Cut) + 15) & ~size_t(15);
+  const size_t cuts = ((size_t)2 * p.grid * sizeof(Cut) + 15) & ~size_t(15);
   const size_t rows = F32 ? (size_t)p.tokens * p.nqh : 0, terms = rows * 2 * HD * sizeof(__half);
   const size_t need = parts + cuts + terms + rows * sizeof(float);
   if (g4a_status s = g4a_ensure_workspace(ctx, need)) return s;

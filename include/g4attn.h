@@ -441,7 +441,8 @@ g4a_status g4a_paged_qkv_prep(g4a_ctx* ctx, const float* q, const float* k, cons
  * > max_tokens, kv_lens[b] < T or kv_lens[b] beyond max_pages_per_seq*page_size is skipped (its
  * rows of out stay as they were) and g4a_sync reports it; so do page ids out of range, whose rows
  * count as not there.  Rows of out behind the last sequence stay as they were.  A value that is
- * not finite in a row of the cache reaches only the tokens that attend to that row.  The partial
+ * not finite in a row of the cache reaches only the tokens that attend to that row.  A page pool
+ * holds at most 64 GiB.  The partial
  * results live in the context's workspace: before capturing the call into a graph, make one of
  * the same shape, and do not let graphs captured from one context run at the same time. */
 g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t format, const uint16_t* k_pages,
