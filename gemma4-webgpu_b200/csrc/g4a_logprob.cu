@@ -8,23 +8,30 @@
 // over as many CTAs as the batch leaves free; a second kernel joins the parts of a row.
 //
 // Top k.  Values are ranked by 64-bit keys (order-preserving bits of x above the complement of the
-// id), so no two are equal and ties go to the lower id.  Each CTA keeps its k largest in shared
-// memory, sorted.  A tile of the row can only add values above the k-th of them, which after the
-// first tiles is rare (k ln n expected over n values); one compare per thread and tile (its
-// maximum, which the softmax needs anyway) and one block-wide count tell.  When more than k threads
-// hold such a value, the k-th largest of the 256 thread maxima is a second lower bound: k values
-// at least that large exist.  Then at most k threads append, so the list is bounded by
-// k + k * (values per thread) for any input, equal values included.
+// id), so no two are equal and ties go to the lower id.  The pass over the logits only keeps the
+// largest value of every segment of 512 consecutive ids (a warp's share of a tile; 1/512 of the
+// row).  The join then takes the k + 2 largest segments, by (largest value, lower segment first),
+// and looks for the k largest values in those alone: a value outside has k segments before its own
+// whose largest values all rank above it.  (Two more than k because the first and the last segment
+// of a row may be filled up with -inf.)
+//
+// Both selections are the same block-wide routine: tiles of 4,096 values against a sorted list of the
+// best so far.  When more threads than wanted hold a value above the list's last, the k-th largest
+// of the 256 thread maxima is a second lower bound (k values at least that large exist), so at most
+// k threads append their 16 values and the list stays within k + 16 k for any input, equal values
+// included.
 #include "g4a_internal.cuh"
 
 namespace {
 
 constexpr int kThreadsL = 256;
 constexpr int kMaxTop = G4A_MAX_TOP_K;
-constexpr int kEpt = 16;                                   // values per thread and tile
+constexpr int kEpt = 16;                          // values per thread and tile
 constexpr int kTile = kThreadsL * kEpt;
-constexpr int kList = kMaxTop + kMaxTop * kEpt;            // appended values of a tile + the kept ones
-constexpr int kMaxSplit = kThreadsL;                       // parts of a row: one thread each in the join
+constexpr int kSeg = 32 * kEpt;                   // values of a segment
+constexpr int kMaxPick = kMaxTop + 2;             // segments looked at
+constexpr int kList = kMaxPick + kMaxPick * kEpt; // the kept values and those a tile appends
+constexpr int kMaxSplit = kThreadsL;              // parts of a row: one thread each in the join
 constexpr float kLog2eL = 1.4426950408889634f;
 constexpr float kLn2L = 0.6931471805599453f;
 
@@ -34,9 +41,10 @@ struct LogprobParams {
   size_t row_stride;
   uint32_t rows, vocab, split, part;  // part: values of a row per CTA (a multiple of kTile)
   int tokens_per_row, top_k;
-  float cap, inv_cap2;  // inv_cap2 = 2 log2(e) / cap
-  float4* stats;        // [rows, split] (m, S, T)
-  uint64_t* keys;       // [rows, split, top_k], sorted, 0 = none
+  float cap, inv_cap, inv_cap2;  // inv_cap2 = 2 log2(e) / cap
+  float4* stats;                 // [rows, split] (m, S, T)
+  float* seg_max;                // [rows, segs]
+  uint32_t segs;
   float *logprob, *entropy, *top_logprob;
   int* top_ids;
   int* err;
@@ -64,6 +72,24 @@ __device__ __forceinline__ float capped(float x, float cap, float inv_cap2) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
   const float y = fmaf(-2.0f * cap, r, cap);
   return x == -INFINITY ? -INFINITY : y;
+}
+
+// The same for |x| <= 0.9 c as x times a polynomial in (x / c)^2, a least-maximum fit of tanh(z) / z on
+// [0, 0.9] (relative error 1.4e-8): nine multiply-adds where the form above takes two special-
+// function operations, of which an SM makes 16 a cycle against 128 of the former.
+constexpr float kCapRange = 0.9f;
+constexpr float kT0 = 0.99999998584f, kT1 = -0.33333160193f, kT2 = 0.13329835261f, kT3 = -0.05369905191f,
+                kT4 = 0.02085770253f, kT5 = -0.00681405711f, kT6 = 0.00128645157f;
+__device__ __forceinline__ float capped_small(float x, float inv_cap) {
+  const float z = x * inv_cap, u = z * z;
+  float q = kT6;
+  q = fmaf(q, u, kT5);
+  q = fmaf(q, u, kT4);
+  q = fmaf(q, u, kT3);
+  q = fmaf(q, u, kT2);
+  q = fmaf(q, u, kT1);
+  q = fmaf(q, u, kT0);
+  return x * q;
 }
 
 struct Stat {
@@ -94,17 +120,70 @@ __device__ __forceinline__ Stat block_join(Stat x, Stat* red) {
   return x;
 }
 
-// Sorts the n keys of `list` by rank (they are distinct) and leaves the k largest, sorted, in
-// `out` (0 where there are fewer).  All threads; n <= 1024 or so.
-__device__ __forceinline__ void keep_top(const uint64_t* list, int n, int k, uint64_t* out) {
-  for (int i = threadIdx.x; i < n; i += kThreadsL) {
-    const uint64_t x = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; j++) rank += list[j] > x;
-    if (rank < k) out[rank] = x;
+// The k largest of n keys into kept[0, k), sorted, 0 where there are fewer; key(i) gives the i-th (0:
+// none).  All 256 threads; `low`: values below this key are known not to be among them.
+struct alignas(16) TopShared {
+  uint64_t list[kList], kept[kMaxPick], tops[kThreadsL];
+  uint64_t bound;
+  int count;
+};
+template <typename Key>
+__device__ __forceinline__ void block_top(uint64_t n, int k, uint64_t low, TopShared& sh, Key key) {
+  const int tid = threadIdx.x;
+  if (tid < kMaxPick) sh.kept[tid] = 0;
+  if (tid == 0) sh.count = 0;
+  int have = 0;
+  uint64_t lim0 = low > 1 ? low : 1;
+  __syncthreads();
+  for (uint64_t t0 = 0; t0 < n; t0 += kTile) {
+    uint64_t x[kEpt], best = 0;
+#pragma unroll
+    for (int e = 0; e < kEpt; e++) {
+      const uint64_t i = t0 + (uint32_t)(e * kThreadsL + tid);
+      x[e] = i < n ? key(i) : 0;
+    }
+#pragma unroll
+    for (int e = 0; e < kEpt; e++) best = x[e] > best ? x[e] : best;
+    const bool holds = best >= lim0;
+    const int n_hold = __syncthreads_count(holds);
+    if (n_hold == 0) continue;
+    uint64_t lim = lim0;
+    if (n_hold > k) {
+      sh.tops[tid] = holds ? best : 0;
+      __syncthreads();
+      if (holds) {
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < kThreadsL; j += 2) {
+          const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(&sh.tops[j]);
+          rank += (o.x > best) + (o.y > best);
+        }
+        if (rank == k - 1) sh.bound = best;
+      }
+      __syncthreads();
+      lim = max(lim, sh.bound);
+    }
+    if (best >= lim) {
+#pragma unroll
+      for (int e = 0; e < kEpt; e++)
+        if (x[e] >= lim) sh.list[atomicAdd(&sh.count, 1)] = x[e];
+    }
+    const uint64_t old = tid < have ? sh.kept[tid] : 0;
+    __syncthreads();
+    const int added = sh.count, all = added + have;
+    if (tid < have) sh.list[added + tid] = old;
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    for (int i = tid; i < all; i += kThreadsL) {
+      const uint64_t mine = sh.list[i];
+      int rank = 0;
+      for (int j = 0; j < all; j++) rank += sh.list[j] > mine;
+      if (rank < k) sh.kept[rank] = mine;
+    }
+    __syncthreads();
+    have = min(all, k);
+    if (have == k) lim0 = max(lim0, sh.kept[k - 1] + 1);
   }
-  if (n < k)
-    for (int i = n + threadIdx.x; i < k; i += kThreadsL) out[i] = 0;
 }
 
 template <typename T>
@@ -131,18 +210,16 @@ struct Vec<__half> {
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
 };
 
-// One part of one row: CTA (row, part).  A tile is 256 threads x 16 values in 16-byte loads from
-// the aligned address at or before the row's start; a load that reaches over either end of the
-// part is made value by value, so nothing outside the row is read.
+// One part of one row: CTA (row, part).  A tile is 8 warps x 512 consecutive values (16 a thread), in
+// 16-byte loads from the aligned address at or before the row's start; a load that reaches over
+// either end of the part is made value by value, so nothing outside the row is read.  No thread
+// waits for another before the end of the part.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
   constexpr int VN = Vec<T>::N, NV = kEpt / VN;
   __shared__ Stat red[kThreadsL / 32];
-  __shared__ uint64_t list[kList], kept[kMaxTop], tops[kThreadsL];
-  __shared__ uint64_t bound;
-  __shared__ int count;
   const uint32_t row = blockIdx.x / p.split, part = blockIdx.x - row * p.split;
-  const int k = p.top_k, tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   g4a::pdl_wait_primary();
   g4a::pdl_launch_dependents();
   const T* x0 = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride;
@@ -151,17 +228,14 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
   const T* base = x0 - head;
   const uint32_t lo = max(part * p.part, head);
   const uint32_t hi = min(part * p.part + p.part, p.vocab + head);
-  if (tid < kMaxTop) kept[tid] = 0;
-  if (tid == 0) count = 0;
+  float* seg_max = p.top_k ? p.seg_max + (size_t)row * p.segs : nullptr;
+  const float small = CAP ? kCapRange * p.cap : 3.0e38f;
   Stat st = {-INFINITY, 0.f, 0.f};
-  int have = 0;            // kept values (uniform)
-  uint64_t thr = 0;        // the k-th of them
-  __syncthreads();
-  for (uint32_t t0 = part * p.part; t0 < hi; t0 += kTile) {
+  for (uint32_t t0 = part * p.part + warp * kSeg; t0 < hi; t0 += kTile) {
     float x[kEpt];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-      const uint32_t i0 = t0 + (uint32_t)(j * kThreadsL + tid) * VN;
+      const uint32_t i0 = t0 + (uint32_t)(j * 32 + lane) * VN;
       float v[VN];
       if (i0 >= lo && i0 + VN <= hi) {
         Vec<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(base + i0)), v);
@@ -173,116 +247,82 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
 #pragma unroll
       for (int e = 0; e < VN; e++) x[j * VN + e] = v[e];
     }
-    float top = x[0];
+    float top = x[0], low = x[0];
 #pragma unroll
-    for (int e = 1; e < kEpt; e++) top = fmaxf(top, x[e]);  // NaN is passed over
+    for (int e = 1; e < kEpt; e++) top = fmaxf(top, x[e]), low = fminf(low, x[e]);  // NaN is passed over
+    if (seg_max != nullptr) {
+      float s = top;
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+      if (lane == 0) seg_max[t0 / kSeg] = s;
+    }
     const float ym = CAP ? capped(top, p.cap, p.inv_cap2) : top;
     const float m = fmaxf(st.m, ym);
-    const float ml = (m == -INFINITY ? 0.f : m) * kLog2eL;
     if (m > st.m) {
       const float d = st.m == -INFINITY ? 0.f : (st.m - m) * kLog2eL, w = g4a::fast_exp2(d);
       st.t = w * (st.t + d * st.s);
       st.s *= w;
       st.m = m;
     }
+    const float ml = (m == -INFINITY ? 0.f : m) * kLog2eL;
+    float s = 0.f, t = 0.f;
+    if (top <= small && low >= -small) {  // finite, and within the polynomial's range
 #pragma unroll
-    for (int e = 0; e < kEpt; e++) {
-      const float y = CAP ? capped(x[e], p.cap, p.inv_cap2) : x[e];
-      const float d = fmaf(y, kLog2eL, -ml);
-      const float w = g4a::fast_exp2(d);
-      st.s += w;
-      st.t = fmaf(fmaxf(d, -1000.f), w, st.t);  // -inf: -1000 * 0
-    }
-    if (k == 0) continue;
-    // which threads hold values above the k-th kept one
-    auto id_of = [&](int e) { return t0 + (uint32_t)((e / VN) * kThreadsL + tid) * VN + (uint32_t)(e % VN); };
-    auto valid = [&](int e) { const uint32_t i = id_of(e); return i >= lo && i < hi; };
-    uint64_t best = 0;
-    const uint32_t thr_hi = (uint32_t)(thr >> 32);
-    // below a full list every value counts, NaN (ordered 0) included
-    if (have < k || ordered(top) >= thr_hi) {
-#pragma unroll
-      for (int e = 0; e < kEpt; e++)
-        if (valid(e)) {
-          const uint64_t key = make_key(x[e], id_of(e) - head);
-          if (key > best) best = key;
-        }
-      if (have >= k && best <= thr) best = 0;
-    }
-    const int n_hold = __syncthreads_count(best != 0);
-    if (n_hold == 0) continue;
-    uint64_t lim = have < k ? 1 : thr + 1;
-    if (n_hold > k) {
-      tops[tid] = best;
-      __syncthreads();
-      if (best != 0) {
-        int rank = 0;
-        for (int j = 0; j < kThreadsL; j++) rank += tops[j] > best;
-        if (rank == k - 1) bound = best;
+      for (int e = 0; e < kEpt; e++) {
+        const float y = CAP ? capped_small(x[e], p.inv_cap) : x[e];
+        const float d = fmaf(y, kLog2eL, -ml);
+        const float w = g4a::fast_exp2(d);
+        s += w;
+        t = fmaf(d, w, t);
       }
-      __syncthreads();
-      lim = max(lim, bound);
-    }
-    if (best >= lim && best != 0) {
+    } else {
 #pragma unroll
-      for (int e = 0; e < kEpt; e++)
-        if (valid(e)) {
-          const uint64_t key = make_key(x[e], id_of(e) - head);
-          if (key >= lim) list[atomicAdd(&count, 1)] = key;
-        }
+      for (int e = 0; e < kEpt; e++) {
+        const float y = CAP ? capped(x[e], p.cap, p.inv_cap2) : x[e];
+        const float d = fmaf(y, kLog2eL, -ml);
+        const float w = g4a::fast_exp2(d);
+        s += w;
+        t = fmaf(fmaxf(d, -1000.f), w, t);  // -inf: -1000 * 0
+      }
     }
-    if (tid < have) list[kList - 1 - tid] = kept[tid];  // the kept ones at the other end
-    __syncthreads();
-    const int n = count;
-    // gather both ends into one run (positions n .. n + have - 1)
-    uint64_t mine = tid < have ? list[kList - 1 - tid] : 0;
-    __syncthreads();
-    if (tid < have) list[n + tid] = mine;
-    if (tid == 0) count = 0;
-    __syncthreads();
-    keep_top(list, n + have, k, kept);
-    __syncthreads();
-    have = min(n + have, k);
-    thr = kept[k - 1];
+    st.s += s;
+    st.t += t;
   }
   st = block_join(st, red);
-  const size_t slot = (size_t)row * p.split + part;
-  if (tid == 0) p.stats[slot] = make_float4(st.m, st.s, st.t, 0.f);
-  if (tid < k) p.keys[slot * k + tid] = kept[tid];
+  if (tid == 0) p.stats[(size_t)row * p.split + part] = make_float4(st.m, st.s, st.t, 0.f);
 }
 
-// Joins the parts of one row (at most one per thread).  The k-th largest of the parts' maxima
-// bounds the row's k-th value from below, so at most k parts, k values each, are candidates.
+// Joins the parts of one row (at most one per thread) and picks its largest values.
 template <typename T>
 __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobParams p) {
   __shared__ Stat red[kThreadsL / 32];
-  __shared__ uint64_t list[kMaxTop * kMaxTop], tops[kThreadsL], kept[kMaxTop];
-  __shared__ uint64_t bound;
-  __shared__ int count;
+  __shared__ TopShared sh;
+  __shared__ uint32_t picked[kMaxPick];
   const uint32_t row = blockIdx.x;
   const int tid = threadIdx.x, k = p.top_k, ns = (int)p.split;
   g4a::pdl_wait_primary();
   g4a::pdl_launch_dependents();
+  const T* x0 = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride;
   Stat st = {-INFINITY, 0.f, 0.f};
   if (tid < ns) {
     const float4 f = p.stats[(size_t)row * ns + tid];
     st = {f.x, f.y, f.z};
   }
-  const uint64_t* keys = p.keys + (size_t)row * ns * k;
-  if (k) {
-    tops[tid] = tid < ns ? keys[(size_t)tid * k] : 0;
-    if (tid == 0) count = 0, bound = 0;
-  }
   st = block_join(st, red);  // (a barrier inside)
   const float ln_s = logf(st.s);
   const float cap = p.cap;
+  auto value = [&](float x) {  // log probability of a logit
+    const float y = !(cap > 0.f)                      ? x
+                    : fabsf(x) <= kCapRange * cap ? capped_small(x, p.inv_cap)
+                                                  : capped(x, cap, p.inv_cap2);
+    return y - st.m - ln_s;
+  };
   if (p.entropy && tid == 0) p.entropy[row] = ln_s - kLn2L * st.t / st.s;
   for (int j = tid; j < p.tokens_per_row; j += kThreadsL) {
     const int tok = p.tokens[(size_t)row * p.tokens_per_row + j];
     float lp = 0.f;
     if (tok >= 0 && (uint32_t)tok < p.vocab) {
-      const float x = Vec<T>::one(reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride + tok);
-      lp = (cap > 0.f ? capped(x, cap, p.inv_cap2) : x) - st.m - ln_s;
+      lp = value(Vec<T>::one(x0 + tok));
     } else if (tok != -1) {
       lp = __uint_as_float(0x7fc00000u);
       atomicExch(p.err, G4A_DEVERR_TOKEN);
@@ -290,30 +330,23 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
     p.logprob[(size_t)row * p.tokens_per_row + j] = lp;
   }
   if (k == 0) return;
-  if (ns > k) {
-    const uint64_t mine = tops[tid];
-    if (mine != 0) {
-      int rank = 0;
-      for (int j = 0; j < ns; j++) rank += tops[j] > mine;
-      if (rank == k - 1) bound = mine;
-    }
-    __syncthreads();
-  }
-  const uint64_t lim = max(bound, (uint64_t)1);
-  if (tid < ns && tops[tid] >= lim)
-    for (int j = 0; j < k; j++) {
-      const uint64_t key = keys[(size_t)tid * k + j];
-      if (key < lim) break;
-      list[atomicAdd(&count, 1)] = key;
-    }
+  const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(x0) & 15u) / sizeof(T));
+  const uint32_t segs = (p.vocab + head + kSeg - 1) / kSeg;
+  const float* seg_max = p.seg_max + (size_t)row * p.segs;
+  const int pick = (int)min(segs, (uint32_t)k + 2);
+  block_top(segs, pick, 0, sh, [&](uint64_t i) { return make_key(seg_max[i], (uint32_t)i); });
+  if (tid < pick) picked[tid] = 0xffffffffu - (uint32_t)sh.kept[tid];
+  // the k-th segment's largest value bounds the k-th value from below (its id is not known here)
+  const uint64_t low = pick == k + 2 ? (sh.kept[k + 1] >> 32) << 32 : 0;
   __syncthreads();
-  keep_top(list, count, k, kept);
-  __syncthreads();
+  block_top((uint64_t)pick * kSeg, k, low, sh, [&](uint64_t i) -> uint64_t {
+    const long long id = (long long)picked[i / kSeg] * kSeg + (long long)(i % kSeg) - head;
+    return id >= 0 && id < (long long)p.vocab ? make_key(Vec<T>::one(x0 + id), (uint32_t)id) : 0;
+  });
   if (tid < k) {
-    const uint64_t key = kept[tid];
-    const float x = from_ordered((uint32_t)(key >> 32));
+    const uint64_t key = sh.kept[tid];
     p.top_ids[(size_t)row * k + tid] = (int)(0xffffffffu - (uint32_t)key);
-    p.top_logprob[(size_t)row * k + tid] = (cap > 0.f ? capped(x, cap, p.inv_cap2) : x) - st.m - ln_s;
+    p.top_logprob[(size_t)row * k + tid] = value(from_ordered((uint32_t)(key >> 32)));
   }
 }
 
@@ -331,9 +364,11 @@ g4a_status launch_logprobs(g4a_ctx* ctx, LogprobParams& p) {
   if ((uint64_t)p.rows * p.split > 0x7fffffffull)
     return g4a_fail(G4A_EINVAL, "g4a_token_logprobs: rows %u too many", p.rows);
   const size_t parts = (size_t)p.rows * p.split;
-  if (g4a_status s = g4a_ensure_workspace(ctx, parts * (sizeof(float4) + (size_t)p.top_k * sizeof(uint64_t)))) return s;
+  p.segs = tiles * (kTile / kSeg);
+  const size_t segs = p.top_k ? (size_t)p.rows * p.segs : 0;
+  if (g4a_status s = g4a_ensure_workspace(ctx, parts * sizeof(float4) + segs * sizeof(float))) return s;
   p.stats = static_cast<float4*>(ctx->workspace);
-  p.keys = reinterpret_cast<uint64_t*>(p.stats + parts);
+  p.seg_max = reinterpret_cast<float*>(p.stats + parts);
   g4a_prof_scope ps(ctx, G4A_PROF_TOKEN_LOGPROBS);
   cudaError_t e = g4a_launch(p.cap > 0.f ? logprob_part_kernel<T, true> : logprob_part_kernel<T, false>,
                              dim3((unsigned)parts), dim3(kThreadsL), 0, ctx->stream, true, p);
@@ -377,6 +412,7 @@ extern "C" g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint3
   p.tokens_per_row = (int)tokens_per_row;
   p.top_k = (int)top_k;
   p.cap = softcap;
+  p.inv_cap = softcap > 0.f ? 1.0f / softcap : 0.f;
   p.inv_cap2 = softcap > 0.f ? 2.0f * kLog2eL / softcap : 0.f;
   p.logprob = logprob;
   p.entropy = entropy;
