@@ -20,6 +20,8 @@
 // of the 256 thread maxima is a second lower bound (k values at least that large exist), so at most
 // k threads append their 16 values and the list stays within k + 16 k for any input, equal values
 // included.
+#include <string.h>
+
 #include "g4a_internal.cuh"
 
 namespace {
@@ -100,7 +102,7 @@ __device__ __forceinline__ Stat join(const Stat a, const Stat b) {
   Stat r = {m, 0.f, 0.f};
   // a part with nothing in it (m = -inf) has s = t = 0 unless it met a NaN, which has to stay
   const float da = a.m == -INFINITY ? 0.f : (a.m - m) * kLog2eL, db = b.m == -INFINITY ? 0.f : (b.m - m) * kLog2eL;
-  const float wa = exp2f(da), wb = exp2f(db);
+  const float wa = g4a::fast_exp2(da), wb = g4a::fast_exp2(db);
   r.s = wa * a.s + wb * b.s;
   r.t = (wa > 0.f ? wa * (a.t + da * a.s) : 0.f) + (wb > 0.f ? wb * (b.t + db * b.s) : 0.f);
   return r;
@@ -114,9 +116,13 @@ __device__ __forceinline__ Stat block_join(Stat x, Stat* red) {
   }
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
   __syncthreads();
-  x = red[0];
+  x = red[threadIdx.x & (kThreadsL / 32 - 1)];
 #pragma unroll
-  for (int w = 1; w < kThreadsL / 32; w++) x = join(x, red[w]);
+  for (int o = kThreadsL / 64; o >= 1; o >>= 1) {
+    const Stat y = {__shfl_xor_sync(0xffffffffu, x.m, o), __shfl_xor_sync(0xffffffffu, x.s, o),
+                    __shfl_xor_sync(0xffffffffu, x.t, o)};
+    x = join(x, y);
+  }
   return x;
 }
 
@@ -211,8 +217,8 @@ struct Vec<__half> {
 };
 
 // One part of one row: CTA (row, part).  A tile is 8 warps x 512 consecutive values (16 a thread), in
-// 16-byte loads from the aligned address at or before the row's start; a load that reaches over
-// either end of the part is made value by value, so nothing outside the row is read.  No thread
+// 16-byte loads from the aligned address at or before the row's start; a segment that reaches over
+// either end of the row is read value by value, so nothing outside the row is read.  No thread
 // waits for another before the end of the part.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
@@ -231,22 +237,34 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
   float* seg_max = p.top_k ? p.seg_max + (size_t)row * p.segs : nullptr;
   const float small = CAP ? kCapRange * p.cap : 3.0e38f;
   Stat st = {-INFINITY, 0.f, 0.f};
-  for (uint32_t t0 = part * p.part + warp * kSeg; t0 < hi; t0 += kTile) {
-    float x[kEpt];
+  // the next segment's values are on their way while this one's are summed
+  uint4 raw[NV];
+  auto fetch = [&](uint32_t t0) {
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       const uint32_t i0 = t0 + (uint32_t)(j * 32 + lane) * VN;
-      float v[VN];
       if (i0 >= lo && i0 + VN <= hi) {
-        Vec<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(base + i0)), v);
-      } else {
+        raw[j] = __ldcs(reinterpret_cast<const uint4*>(base + i0));
+      } else {  // over an end of the row: value by value, -inf outside
+        T v[VN];
 #pragma unroll
-        for (int e = 0; e < VN; e++)
-          v[e] = (i0 + e >= lo && i0 + e < hi) ? Vec<T>::one(base + i0 + e) : -INFINITY;
+        for (int e = 0; e < VN; e++) v[e] = i0 + e >= lo && i0 + e < hi ? base[i0 + e] : (T)(-INFINITY);
+        memcpy(&raw[j], v, 16);
       }
+    }
+  };
+  const uint32_t first = part * p.part + warp * kSeg;
+  if (first < hi) fetch(first);
+  for (uint32_t t0 = first; t0 < hi; t0 += kTile) {
+    float x[kEpt];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      float v[VN];
+      Vec<T>::unpack(raw[j], v);
 #pragma unroll
       for (int e = 0; e < VN; e++) x[j * VN + e] = v[e];
     }
+    if (t0 + kTile < hi) fetch(t0 + kTile);
     float top = x[0], low = x[0];
 #pragma unroll
     for (int e = 1; e < kEpt; e++) top = fmaxf(top, x[e]), low = fminf(low, x[e]);  // NaN is passed over
@@ -303,11 +321,21 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
   g4a::pdl_wait_primary();
   g4a::pdl_launch_dependents();
   const T* x0 = reinterpret_cast<const T*>(p.logits) + (size_t)row * p.row_stride;
+  const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(x0) & 15u) / sizeof(T));
+  const uint32_t segs = k ? (p.vocab + head + kSeg - 1) / kSeg : 0;
+  const float* seg_max = p.seg_max + (size_t)row * p.segs;
+  // every load that needs nothing else first
+  constexpr int kNear = 4;  // segments per thread of a row of up to 1024
+  float near[kNear];
+#pragma unroll
+  for (int e = 0; e < kNear; e++) near[e] = (uint32_t)(e * kThreadsL + tid) < segs ? seg_max[e * kThreadsL + tid] : 0.f;
+  const int my_tok = tid < p.tokens_per_row ? p.tokens[(size_t)row * p.tokens_per_row + tid] : -1;
   Stat st = {-INFINITY, 0.f, 0.f};
   if (tid < ns) {
     const float4 f = p.stats[(size_t)row * ns + tid];
     st = {f.x, f.y, f.z};
   }
+  const float my_x = my_tok >= 0 && (uint32_t)my_tok < p.vocab ? Vec<T>::one(x0 + my_tok) : 0.f;
   st = block_join(st, red);  // (a barrier inside)
   const float ln_s = logf(st.s);
   const float cap = p.cap;
@@ -319,10 +347,10 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
   };
   if (p.entropy && tid == 0) p.entropy[row] = ln_s - kLn2L * st.t / st.s;
   for (int j = tid; j < p.tokens_per_row; j += kThreadsL) {
-    const int tok = p.tokens[(size_t)row * p.tokens_per_row + j];
+    const int tok = j == tid ? my_tok : p.tokens[(size_t)row * p.tokens_per_row + j];
     float lp = 0.f;
     if (tok >= 0 && (uint32_t)tok < p.vocab) {
-      lp = value(Vec<T>::one(x0 + tok));
+      lp = value(j == tid ? my_x : Vec<T>::one(x0 + tok));
     } else if (tok != -1) {
       lp = __uint_as_float(0x7fc00000u);
       atomicExch(p.err, G4A_DEVERR_TOKEN);
@@ -330,19 +358,86 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
     p.logprob[(size_t)row * p.tokens_per_row + j] = lp;
   }
   if (k == 0) return;
-  const uint32_t head = (uint32_t)((reinterpret_cast<uintptr_t>(x0) & 15u) / sizeof(T));
-  const uint32_t segs = (p.vocab + head + kSeg - 1) / kSeg;
-  const float* seg_max = p.seg_max + (size_t)row * p.segs;
   const int pick = (int)min(segs, (uint32_t)k + 2);
-  block_top(segs, pick, 0, sh, [&](uint64_t i) { return make_key(seg_max[i], (uint32_t)i); });
+  auto rank_list = [&](int all, int want) {  // the list's `want` largest into kept
+    for (int i = tid; i < all; i += kThreadsL) {
+      const uint64_t mine = sh.list[i];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < all; j++) rank += sh.list[j] > mine;
+      if (rank < want) sh.kept[rank] = mine;
+    }
+    __syncthreads();
+  };
+  // ---- the segments.  A row of up to 1024 of them: the pick-th largest of the thread maxima bounds
+  // the pick-th segment from below; what reaches it is listed and ranked.
+  bool have_segs = false;
+  if (segs <= kNear * kThreadsL) {
+    uint32_t o[kNear], best = 0;
+#pragma unroll
+    for (int e = 0; e < kNear; e++) {
+      o[e] = (uint32_t)(e * kThreadsL + tid) < segs ? ordered(near[e]) : 0u;
+      best = max(best, o[e]);
+    }
+    uint32_t* tops = reinterpret_cast<uint32_t*>(sh.tops);
+    tops[tid] = best;
+    if (tid == 0) sh.bound = 0, sh.count = 0;
+    __syncthreads();
+    int above = 0, equal = 0;
+#pragma unroll 8
+    for (int j = 0; j < kThreadsL / 4; j++) {
+      const uint4 v = reinterpret_cast<const uint4*>(tops)[j];
+      above += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
+      equal += (v.x == best) + (v.y == best) + (v.z == best) + (v.w == best);
+    }
+    if (above < pick && pick <= above + equal) sh.bound = best;
+    __syncthreads();
+    const uint32_t bound = (uint32_t)sh.bound;
+#pragma unroll
+    for (int e = 0; e < kNear; e++)
+      if ((uint32_t)(e * kThreadsL + tid) < segs && o[e] >= bound) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kList) sh.list[at] = ((uint64_t)o[e] << 32) | (0xffffffffu - (uint32_t)(e * kThreadsL + tid));
+      }
+    __syncthreads();
+    const int all = sh.count;
+    have_segs = all <= kList;
+    if (have_segs) rank_list(all, pick);
+  }
+  if (!have_segs) block_top(segs, pick, 0, sh, [&](uint64_t i) { return make_key(seg_max[i], (uint32_t)i); });
   if (tid < pick) picked[tid] = 0xffffffffu - (uint32_t)sh.kept[tid];
   // the k-th segment's largest value bounds the k-th value from below (its id is not known here)
   const uint64_t low = pick == k + 2 ? (sh.kept[k + 1] >> 32) << 32 : 0;
   __syncthreads();
-  block_top((uint64_t)pick * kSeg, k, low, sh, [&](uint64_t i) -> uint64_t {
-    const long long id = (long long)picked[i / kSeg] * kSeg + (long long)(i % kSeg) - head;
-    return id >= 0 && id < (long long)p.vocab ? make_key(Vec<T>::one(x0 + id), (uint32_t)id) : 0;
-  });
+  const uint32_t n = (uint32_t)pick * kSeg;
+  auto id_of = [&](uint32_t i) { return (long long)picked[i / kSeg] * kSeg + (long long)(i % kSeg) - head; };
+  // Few values of the picked segments reach the bound (k and a handful): all of them are loaded at
+  // once, those that do are listed and ranked.  If they do not fit (equal values), or there is no
+  // bound (a short row), the general selection does it.
+  bool listed = false;
+  if (low != 0) {
+    const float bound = from_ordered((uint32_t)(low >> 32));
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (uint32_t i = tid; i < n; i += kThreadsL) {
+      const long long id = id_of(i);
+      const float x = id >= 0 && id < (long long)p.vocab ? Vec<T>::one(x0 + id) : -INFINITY;
+      if (x >= bound && id >= 0 && id < (long long)p.vocab) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kList) sh.list[at] = make_key(x, (uint32_t)id);
+      }
+    }
+    __syncthreads();
+    const int all = sh.count;
+    listed = all <= kList;
+    if (listed) rank_list(all, k);
+  }
+  if (!listed)
+    block_top(n, k, low, sh, [&](uint64_t i) -> uint64_t {
+      const long long id = id_of((uint32_t)i);
+      return id >= 0 && id < (long long)p.vocab ? make_key(Vec<T>::one(x0 + id), (uint32_t)id) : 0;
+    });
   if (tid < k) {
     const uint64_t key = sh.kept[tid];
     p.top_ids[(size_t)row * k + tid] = (int)(0xffffffffu - (uint32_t)key);
