@@ -94,6 +94,44 @@ __device__ __forceinline__ float capped_small(float x, float inv_cap) {
   return x * q;
 }
 
+// Two floats in one 64-bit register: the packed multiply-add does both in one issue slot, and the
+// pass over capped logits is bound by issue slots.
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void apart(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// capped_small of two values
+__device__ __forceinline__ uint64_t capped_small2(uint64_t x, uint64_t inv_cap) {
+  const uint64_t z = mul2(x, inv_cap), u = mul2(z, z);
+  uint64_t q = two(kT6, kT6);
+  q = fma2(q, u, two(kT5, kT5));
+  q = fma2(q, u, two(kT4, kT4));
+  q = fma2(q, u, two(kT3, kT3));
+  q = fma2(q, u, two(kT2, kT2));
+  q = fma2(q, u, two(kT1, kT1));
+  q = fma2(q, u, two(kT0, kT0));
+  return mul2(x, q);
+}
+
 struct Stat {
   float m, s, t;  // t in log2 units: sum (y - m) log2(e) e^(y - m)
 };
@@ -285,14 +323,23 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
     const float ml = (m == -INFINITY ? 0.f : m) * kLog2eL;
     float s = 0.f, t = 0.f;
     if (top <= small && low >= -small) {  // finite, and within the polynomial's range
+      uint64_t s2 = 0, t2 = 0;
+      const uint64_t ic = two(p.inv_cap, p.inv_cap), l2 = two(kLog2eL, kLog2eL), off = two(-ml, -ml);
 #pragma unroll
-      for (int e = 0; e < kEpt; e++) {
-        const float y = CAP ? capped_small(x[e], p.inv_cap) : x[e];
-        const float d = fmaf(y, kLog2eL, -ml);
-        const float w = g4a::fast_exp2(d);
-        s += w;
-        t = fmaf(d, w, t);
+      for (int e = 0; e < kEpt; e += 2) {
+        const uint64_t x2 = two(x[e], x[e + 1]);
+        const uint64_t d2 = fma2(CAP ? capped_small2(x2, ic) : x2, l2, off);
+        float d0, d1;
+        apart(d2, d0, d1);
+        const uint64_t w2 = two(g4a::fast_exp2(d0), g4a::fast_exp2(d1));
+        s2 = add2(s2, w2);
+        t2 = fma2(d2, w2, t2);
       }
+      float a, b;
+      apart(s2, a, b);
+      s = a + b;
+      apart(t2, a, b);
+      t = a + b;
     } else {
 #pragma unroll
       for (int e = 0; e < kEpt; e++) {
@@ -419,13 +466,39 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
     const float bound = from_ordered((uint32_t)(low >> 32));
     if (tid == 0) sh.count = 0;
     __syncthreads();
-#pragma unroll 8
-    for (uint32_t i = tid; i < n; i += kThreadsL) {
-      const long long id = id_of(i);
-      const float x = id >= 0 && id < (long long)p.vocab ? Vec<T>::one(x0 + id) : -INFINITY;
-      if (x >= bound && id >= 0 && id < (long long)p.vocab) {
-        const int at = atomicAdd(&sh.count, 1);
-        if (at < kList) sh.list[at] = make_key(x, (uint32_t)id);
+    constexpr int VN = Vec<T>::N, kFly = 6;  // 16-byte loads of a thread in flight
+    constexpr uint32_t per_seg = kSeg / VN;
+    const T* base = x0 - head;
+    for (uint32_t v0 = tid; v0 < (uint32_t)pick * per_seg; v0 += kFly * kThreadsL) {
+      uint4 raw[kFly];
+      uint32_t first[kFly];  // its first id, from the aligned address
+#pragma unroll
+      for (int f = 0; f < kFly; f++) {
+        const uint32_t v = v0 + f * kThreadsL;
+        first[f] = 0xffffffffu;
+        if (v >= (uint32_t)pick * per_seg) continue;
+        first[f] = picked[v / per_seg] * kSeg + v % per_seg * VN;
+        if (first[f] >= head && first[f] + VN <= p.vocab + head) {
+          raw[f] = *reinterpret_cast<const uint4*>(base + first[f]);
+        } else {
+          T x[VN];
+#pragma unroll
+          for (int e = 0; e < VN; e++)
+            x[e] = first[f] + e >= head && first[f] + e < p.vocab + head ? base[first[f] + e] : (T)(-INFINITY);
+          memcpy(&raw[f], x, 16);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < kFly; f++) {
+        if (first[f] == 0xffffffffu) continue;
+        float x[VN];
+        Vec<T>::unpack(raw[f], x);
+#pragma unroll
+        for (int e = 0; e < VN; e++)
+          if (x[e] >= bound && first[f] + e >= head && first[f] + e < p.vocab + head) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kList) sh.list[at] = make_key(x[e], first[f] + e - head);
+          }
       }
     }
     __syncthreads();
