@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
       };
       if (cut.chunks == 1) {
         // the piece that begins the tile is in slot lo, the others begin their CTAs' runs
-#pragma unroll 4
+#pragma unroll 8
         for (int i = part0; i < cut.parts; i += pl) fold(i == 0 ? (size_t)lo : (size_t)2 * (lo / 2 + i));
       } else {
         for (int c = part0; c < cut.chunks; c += pl) {

@@ -80,24 +80,31 @@ __device__ __forceinline__ long long stages_of(const TreeParams& p, const Seq& s
 // (Tile after tile, the six tiles of a 131,000-key context came past each row 90 MB apart and the L2
 // had lost it.)  A chunk is at least as long as a run, so a run holds at most two pieces of tiles
 // that are not whole: one that begins before or with it and one that goes on after it.
+// Division of non-negative numbers that are nearly always below 2^32 (the 64-bit one is a long
+// sequence, and the walk starts with several of them).
+__device__ __forceinline__ long long quot(long long a, long long b) {
+  if ((((unsigned long long)a | (unsigned long long)b) >> 32) == 0) return (long long)((uint32_t)a / (uint32_t)b);
+  return a / b;
+}
+
 struct Split {
   long long total, active, each, extra;
   __device__ __forceinline__ void of(long long t, int grid) {
     total = t;
     active = grid < t ? grid : t;
-    each = active ? t / active : 0;
-    extra = active ? t % active : 0;
+    each = active ? quot(t, active) : 0;
+    extra = t - each * active;
   }
   __device__ __forceinline__ long long begin(long long c) const { return c * each + (c < extra ? c : extra); }
   // the CTA whose run holds stage s
   __device__ __forceinline__ long long owner(long long s) const {
     const long long cut = extra * (each + 1);
-    return s < cut ? s / (each + 1) : extra + (s - cut) / each;
+    return s < cut ? quot(s, each + 1) : extra + quot(s - cut, each);
   }
 };
 
 // First stage of chunk c of n stages in `chunks`.
-__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)((long long)n * c / chunks); }
+__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)quot((long long)n * c, chunks); }
 
 // Where a role stands in the CTA's run of stages.
 struct Walk {
@@ -106,7 +113,7 @@ struct Walk {
   int chunks, chunk, j, j_end;  // stage of the tile; end of the chunk
 
   __device__ __forceinline__ void chunk_of(const Split& split) {
-    chunks = s.tiles > 1 ? max(1, (int)min((long long)s.stages, s.stages / max(1ll, split.each))) : 1;
+    chunks = s.tiles > 1 ? max(1, (int)quot(s.stages, max(1ll, split.each))) : 1;
   }
   // stage `local` of sequence b's list
   __device__ __forceinline__ void seek(const TreeParams& p, const Split& split, int seq, long long local) {
@@ -114,15 +121,15 @@ struct Walk {
     s = seq_of(p, b);
     chunk_of(split);
     const long long per_head = (long long)s.tiles * s.stages;
-    kvh = (int)(local / per_head);
+    kvh = (int)quot(local, per_head);
     local -= kvh * per_head;
-    chunk = (int)(local / s.tiles * chunks / s.stages);
+    chunk = (int)quot(quot(local, s.tiles) * chunks, s.stages);
     while (chunk > 0 && local < (long long)s.tiles * chunk_at(s.stages, chunks, chunk)) chunk--;
     while (local >= (long long)s.tiles * chunk_at(s.stages, chunks, chunk + 1)) chunk++;
     const int j0 = chunk_at(s.stages, chunks, chunk);
     j_end = chunk_at(s.stages, chunks, chunk + 1);
     local -= (long long)s.tiles * j0;
-    tile = (int)(local / (j_end - j0));
+    tile = (int)quot(local, j_end - j0);
     j = j0 + (int)(local - (long long)tile * (j_end - j0));
   }
   // past the end of a tile's chunk

@@ -119,19 +119,42 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// `count` consecutive TMEM columns of this warp's 32 lanes (count 16 or 32).
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+// 16 or 32 consecutive TMEM columns of this warp's 32 lanes; the registers may be used after
+// tmem_landed() has named them.
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) { tmem_ld16(taddr, r); }
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// (volatile statements keep their order: no use of the registers can move before the wait)
+template <int W>
+__device__ __forceinline__ void tmem_landed(uint32_t (&r)[W]) {
+#pragma unroll
+  for (int n = 0; n < W; n++) asm volatile("" : "+r"(r[n]));
+}
+template <int W>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
+  tmem_get(taddr, r);
+  tmem_wait_ld();
+  tmem_landed(r);
+}
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 
@@ -368,11 +391,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     Walk w = at;
     Rows rows = {}, rows_before = {};
     int tile_no = -1;  // tiles this CTA has begun
-    // The tile's queries into Q buffer tile_no % NQ, and what its rows see.  Lane k looks up row
-    // pw + 4 k of the tile.
+    // The tile's queries into Q buffer tile_no % NQ (copies under way when it returns), and after the
+    // tile's first keys are under way too, what its rows see.  Lane k looks up row pw + 4 k of the tile.
+    long long mine = -1;  // that row of q, in heads
     auto load_queries = [&]() {
       const int kvh = w.kvh, tile = w.tile;
-      const int qb = tile_no % NQ, sb = tile_no & 3;
+      const int qb = tile_no % NQ;
       if (tile_no >= NQ) {
         (void)wait(&qempty[qb], (uint32_t)(tile_no / NQ - 1), G4A_DEVERR_WAIT_EMPTY);
         __syncwarp();
@@ -380,7 +404,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       const int live = min(ROWS, w.s.T * p.group - tile * ROWS);
       constexpr int RW = ROWS / 4;
       const int r_mine = pw + 4 * lane, gr = tile * ROWS + r_mine, t = gr / p.group;
-      long long mine = -1;  // its row of q, in heads
+      mine = -1;
       if (lane < RW && r_mine < live)
         mine = (long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group);
       constexpr int PC = HD / 8;                  // 16-byte pieces of a row
@@ -402,10 +426,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             cp16(qa + (k >> 3) * (N * 128) + n * 128 + (((k & 7) ^ (n & 7)) << 4), src + (ok ? k * 8 : 0), ok);
           }
       }
+    };
+    auto finish_queries = [&]() {
+      constexpr int RW = ROWS / 4;
+      const int sb = tile_no & 3, r_mine = pw + 4 * lane;
       if (pw == 0 && lane == 0) pieces[sb] = w;
       if (lane < RW) {
         Sees v = {0, ~0ull};  // rows past the last one: their results are not written
-        if (mine >= 0) v = sees_of(p, w.s, t);
+        if (mine >= 0) v = sees_of(p, w.s, (w.tile * ROWS + r_mine) / p.group);
         sees[sb * ROWS + r_mine] = v;
         if constexpr (F32) scales[sb * ROWS + r_mine] = mine >= 0 ? p.q_scale[mine] : 0.f;
       }
@@ -415,7 +443,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       if (i < n_stages) {
         const bool first = i == 0 || w.begins();
         if (first) tile_no++;
-        if (i == 0) load_queries();  // nothing to wait for: all in flight before the first keys
+        if (first) load_queries();
         long long off = -1;
         const int key = w.key0(p) + pw * 32 + lane;
         if (key < w.s.L) off = row_offset(p, w.b, w.kvh, key);
@@ -431,7 +459,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           rows.ok |= (o >= 0 ? 1u : 0u) << it;
         }
         load_units(rows, p.k);
-        if (first && i > 0) load_queries();
+        if (first) finish_queries();
       }
       if (i > 0) load_units(rows_before, p.v);
       rows_before = rows;
@@ -650,16 +678,25 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           {
             uint32_t r[W];
             const uint32_t col = lanes + C::COL_S + (uint32_t)(b * N + half * RH + g * W);
-            tmem_load(col, r);
-#pragma unroll
-            for (int n = 0; n < W; n++) x[n] = __uint_as_float(r[n]);
             if constexpr (F32) {
-              tmem_load(col + ROWS, r);
+              uint32_t r2[W];
+              tmem_get(col, r);
+              tmem_get(col + ROWS, r2);
+              tmem_wait_ld();
+              tmem_landed(r);
+              tmem_landed(r2);
 #pragma unroll
-              for (int n = 0; n < W; n++) x[n] = (x[n] + __uint_as_float(r[n])) * sc[g * W + n];
+              for (int n = 0; n < W; n += 4) {
+                const float4 c4 = *reinterpret_cast<const float4*>(sc + g * W + n);
+                const float cs[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                  x[n + e] = (__uint_as_float(r[n + e]) + __uint_as_float(r2[n + e])) * cs[e];
+              }
             } else {
+              tmem_load(col, r);
 #pragma unroll
-              for (int n = 0; n < W; n++) x[n] *= p.scale_log2;
+              for (int n = 0; n < W; n++) x[n] = __uint_as_float(r[n]) * p.scale_log2;
             }
           }
           if (!clean) {
@@ -681,17 +718,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             if (lane == 0) mbar_arrive(&sfree[b]);
           }
           // ---- does a score pass its row's maximum by 2^8?
-          bool over = false;
-          const float4* u4 = reinterpret_cast<const float4*>(su + g * W);
+          float far = -INFINITY;
+          const float4* u4 = reinterpret_cast<const float4*>(su + g * W);  // m - 7 of the rows
 #pragma unroll
           for (int n = 0; n < W; n += 4) {
             const float4 u = u4[n / 4];
-            over |= x[n] - u.x > kPUp + kRaise;
-            over |= x[n + 1] - u.y > kPUp + kRaise;
-            over |= x[n + 2] - u.z > kPUp + kRaise;
-            over |= x[n + 3] - u.w > kPUp + kRaise;
+            far = fmaxf(far, fmaxf(fmaxf(x[n] - u.x, x[n + 1] - u.y), fmaxf(x[n + 2] - u.z, x[n + 3] - u.w)));
           }
-          if (any_of(over)) {
+          if (any_of(far > kPUp + kRaise)) {
             const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
             if (lane < W) smax[quarter * RH + g * W + lane] = mine;
             meet();
@@ -951,8 +985,8 @@ g4a_status g4a_tree_tc_launch(g4a_ctx* ctx, g4a_tree::TreeParams& p, bool f32, l
   if (p.hd > 256) return f32 ? launch_tc<512, 64, true>(ctx, p, keys, rows) : launch_tc<512, 64, false>(ctx, p, keys, rows);
   if (p.hd > 128) {
     if (f32) return rows <= 32 ? launch_tc<256, 64, true>(ctx, p, keys, rows) : launch_tc<256, 128, true>(ctx, p, keys, rows);
-    return rows <= 64 ? launch_tc<256, 64, false>(ctx, p, keys, rows) : launch_tc<256, 128, false>(ctx, p, keys, rows);
+    return launch_tc<256, 64, false>(ctx, p, keys, rows);
   }
   if (f32) return rows <= 32 ? launch_tc<128, 64, true>(ctx, p, keys, rows) : launch_tc<128, 128, true>(ctx, p, keys, rows);
-  return rows <= 64 ? launch_tc<128, 64, false>(ctx, p, keys, rows) : launch_tc<128, 128, false>(ctx, p, keys, rows);
+  return launch_tc<128, 64, false>(ctx, p, keys, rows);
 }
