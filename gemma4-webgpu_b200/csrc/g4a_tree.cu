@@ -36,6 +36,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // (a batch of short ones has many tiles of two parts).  A lane folds its parts one by one with a
 // running maximum, several loads ahead; the lanes of a row meet in shared memory.
 constexpr int kMergeThreads = 256;
+constexpr int kMergeFly = 10;  // parts of a lane in flight
 constexpr int kMaxCuts = 512;  // two for each CTA of the attention kernel
 
 template <bool F32>
@@ -78,7 +79,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     __syncthreads();
   }
   const int total = ends[kMaxCuts - 1];
-  const size_t stride = (size_t)p.rows * (p.hd_pad + 2);
+  const int tile_rows = 1 << p.rows_log2;
+  const size_t stride = (size_t)tile_rows * (p.hd_pad + 2);
   for (int unit = blockIdx.x; unit < total; unit += gridDim.x) {
     int lo = 0, hi = kMaxCuts - 1;  // the first cut whose end is above the unit
     while (lo < hi) {
@@ -94,34 +96,35 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < cut.rows) {
-      Split split;
-      split.each = cut.each;
-      split.extra = cut.extra;
-      auto fold = [&](size_t slot) {
-        const float* base = p.part + slot * stride;
-        const float mi = __ldcg(base + (size_t)p.rows * p.hd_pad + r);
-        const float li = __ldcg(base + (size_t)p.rows * p.hd_pad + p.rows + r);
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(base + (size_t)r * p.hd_pad + d));
-        const float mn = fmaxf(m, mi);
-        // a part that saw nothing has weight 0 and sums of 0 (or the NaN of a NaN score, which stays)
-        const float wo = m == mn ? 1.f : fast_exp2(m - mn), wi = mi == mn ? 1.f : fast_exp2(mi - mn);
+      for (int i0 = part0; i0 < cut.parts; i0 += kMergeFly * pl) {
+        float mi[kMergeFly], li[kMergeFly];
+        float4 x[kMergeFly];
+#pragma unroll
+        for (int f = 0; f < kMergeFly; f++) {
+          const int i = i0 + f * pl;
+          mi[f] = -INFINITY, li[f] = 0.f, x[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i >= cut.parts) continue;
+          const float* base = p.part + (size_t)(i == 0 ? lo : (lo & ~1) + i * cut.stride) * stride;
+          mi[f] = __ldcg(base + (size_t)tile_rows * p.hd_pad + r);
+          li[f] = __ldcg(base + (size_t)tile_rows * p.hd_pad + tile_rows + r);
+          x[f] = __ldcg(reinterpret_cast<const float4*>(base + (size_t)r * p.hd_pad + d));
+        }
+        float mn = m;
+#pragma unroll
+        for (int f = 0; f < kMergeFly; f++) mn = fmaxf(mn, mi[f]);
+        const float wo = m == mn ? 1.f : fast_exp2(m - mn);
         m = mn;
-        l = wo * l + wi * li;
-        o.x = wo * o.x + wi * x.x;
-        o.y = wo * o.y + wi * x.y;
-        o.z = wo * o.z + wi * x.z;
-        o.w = wo * o.w + wi * x.w;
-      };
-      if (cut.chunks == 1) {
-        // the piece that begins the tile is in slot lo, the others begin their CTAs' runs
-#pragma unroll 8
-        for (int i = part0; i < cut.parts; i += pl) fold(i == 0 ? (size_t)lo : (size_t)2 * (lo / 2 + i));
-      } else {
-        for (int c = part0; c < cut.chunks; c += pl) {
-          const int j0 = chunk_at(cut.stages, cut.chunks, c), j1 = chunk_at(cut.stages, cut.chunks, c + 1);
-          const long long s0 = cut.base + (long long)cut.tiles * j0 + (long long)cut.tile * (j1 - j0);
-          const long long c0 = split.owner(s0), c1 = split.owner(s0 + (j1 - j0) - 1);
-          for (long long k = c0; k <= c1; k++) fold((size_t)(2 * k + (k == c0 && s0 > split.begin(k) ? 1 : 0)));
+        l *= wo;
+        o.x *= wo, o.y *= wo, o.z *= wo, o.w *= wo;
+#pragma unroll
+        for (int f = 0; f < kMergeFly; f++) {
+          // a part that saw nothing has weight 0 and sums of 0 (or the NaN of a NaN score, which stays)
+          const float w = mi[f] == mn ? 1.f : fast_exp2(mi[f] - mn);
+          l = fmaf(w, li[f], l);
+          o.x = fmaf(w, x[f].x, o.x);
+          o.y = fmaf(w, x[f].y, o.y);
+          o.z = fmaf(w, x[f].z, o.z);
+          o.w = fmaf(w, x[f].w, o.w);
         }
       }
     }

@@ -19,7 +19,7 @@ struct TreeParams {
   int nqh, nkh, group, hd;  // group = nqh / nkh
   float scale_log2;         // scale * log2(e)
   uint32_t window;
-  int rows, kps;  // query rows of a tile, keys of a stage (of the launched kernel)
+  int rows_log2;  // query rows of a tile of the launched kernel, 2^rows_log2
   int grid;       // CTAs of the launched kernel
   float* part;    // [2 * grid] partial rows: o [rows, hd_pad] | m [rows] | l [rows]
   int hd_pad;
@@ -29,16 +29,16 @@ struct TreeParams {
   int* err;
 };
 
+constexpr int kStageLog2 = 7;  // keys of a stage: 128
+
 // A tile whose keys were not all done by one CTA, written by the CTA that has its first piece, at the
-// index of that piece's slot.
+// index of that piece's slot k; the other pieces are in slots (k & ~1) + i * stride.
 struct Cut {
-  int parts;             // pieces (chunks == 1) or chunks to be joined; 0: nothing
-  int rows;              // query rows of the tile that exist
-  int row0;              // the sequence's first row of q
-  int kvh, first;        // kv head; the tile's first row in units of (token, head of the group)
-  int stages, chunks, tiles, tile;
-  int each, extra;       // the split of the list over the CTAs
-  long long base;        // stage of the list at which the (sequence, kv head) begins
+  int parts;       // pieces; 0: nothing
+  int stride;
+  int rows;        // query rows of the tile that exist
+  int row0;        // the sequence's first row of q
+  int kvh, first;  // kv head; the tile's first row in units of (token, head of the group)
 };
 
 // One sequence: T drafted tokens (rows row0 .. of q), base older rows, keys [lo, L) to be read.
@@ -64,8 +64,8 @@ __device__ __forceinline__ Seq seq_of(const TreeParams& p, int b) {
   // the earliest key any token's window can reach (a token that sees itself alone: base + 1 - W;
   // one whose mask is empty: base - W)
   s.lo = (p.window != 0u && (uint32_t)s.base > p.window) ? s.base - (int)p.window : 0;
-  s.tiles = (s.T * p.group + p.rows - 1) / p.rows;
-  s.stages = s.tiles > 0 ? (L - s.lo + p.kps - 1) / p.kps : 0;
+  s.tiles = (s.T * p.group + (1 << p.rows_log2) - 1) >> p.rows_log2;
+  s.stages = s.tiles > 0 ? (L - s.lo + (1 << kStageLog2) - 1) >> kStageLog2 : 0;
   return s;
 }
 
@@ -73,28 +73,29 @@ __device__ __forceinline__ long long stages_of(const TreeParams& p, const Seq& s
   return (long long)p.nkh * s.tiles * s.stages;
 }
 
-// The list of all stages is cut into equal runs, one per CTA; only the first min(grid, total) CTAs
-// have work.  Order: sequence, kv head, chunk of keys, tile, stage.  The tiles of a kv head read the
-// same keys, so its keys are cut into chunks about as long as a run and a chunk's tiles follow one
-// another: their CTAs read the same rows at the same time, and only the first reads them from HBM.
-// (Tile after tile, the six tiles of a 131,000-key context came past each row 90 MB apart and the L2
-// had lost it.)  A chunk is at least as long as a run, so a run holds at most two pieces of tiles
-// that are not whole: one that begins before or with it and one that goes on after it.
 // Division of non-negative numbers that are nearly always below 2^32 (the 64-bit one is a long
-// sequence, and the walk starts with several of them).
+// sequence of instructions).
 __device__ __forceinline__ long long quot(long long a, long long b) {
   if ((((unsigned long long)a | (unsigned long long)b) >> 32) == 0) return (long long)((uint32_t)a / (uint32_t)b);
   return a / b;
 }
 
-struct Split {
-  long long total, active, each, extra;
-  __device__ __forceinline__ void of(long long t, int grid) {
-    total = t;
-    active = grid < t ? grid : t;
-    each = active ? quot(t, active) : 0;
-    extra = t - each * active;
-  }
+// First stage of chunk c of n stages in `chunks`.
+__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)quot((long long)n * c, chunks); }
+
+// How the tiles' stages are dealt to the CTAs, found by every warp for itself from the lengths on the
+// device.
+//  - At most one tile per CTA (`run` > 0): each kv head's keys are cut into the fewest chunks of at
+//    most `run` stages, run the smallest length found for which the pieces (chunk, tile) are no more
+//    than the CTAs, and CTA c does piece c, in the order sequence, kv head, chunk, tile.  A chunk's
+//    tiles are neighbours and read the same rows at the same time, so only one of them goes to HBM.
+//    (Tile after tile, the six tiles of a 131,000-key context came past each row 90 MB apart and the
+//    L2 had lost it.)
+//  - More tiles than CTAs: the list of all stages (sequence, kv head, tile, stage) is cut into equal
+//    runs.  A run holds whole tiles, and at most two pieces: one at its begin, one at its end.
+struct Plan {
+  int run;
+  long long active, each, extra;
   __device__ __forceinline__ long long begin(long long c) const { return c * each + (c < extra ? c : extra); }
   // the CTA whose run holds stage s
   __device__ __forceinline__ long long owner(long long s) const {
@@ -103,106 +104,148 @@ struct Split {
   }
 };
 
-// First stage of chunk c of n stages in `chunks`.
-__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)quot((long long)n * c, chunks); }
-
-// Where a role stands in the CTA's run of stages.
+// Where a role stands in the CTA's stages.
 struct Walk {
   Seq s;
   int b, kvh, tile;
   int chunks, chunk, j, j_end;  // stage of the tile; end of the chunk
 
-  __device__ __forceinline__ void chunk_of(const Split& split) {
-    chunks = s.tiles > 1 ? max(1, (int)quot(s.stages, max(1ll, split.each))) : 1;
-  }
-  // stage `local` of sequence b's list
-  __device__ __forceinline__ void seek(const TreeParams& p, const Split& split, int seq, long long local) {
-    b = seq;
-    s = seq_of(p, b);
-    chunk_of(split);
-    const long long per_head = (long long)s.tiles * s.stages;
-    kvh = (int)quot(local, per_head);
-    local -= kvh * per_head;
-    chunk = (int)quot(quot(local, s.tiles) * chunks, s.stages);
-    while (chunk > 0 && local < (long long)s.tiles * chunk_at(s.stages, chunks, chunk)) chunk--;
-    while (local >= (long long)s.tiles * chunk_at(s.stages, chunks, chunk + 1)) chunk++;
-    const int j0 = chunk_at(s.stages, chunks, chunk);
-    j_end = chunk_at(s.stages, chunks, chunk + 1);
-    local -= (long long)s.tiles * j0;
-    tile = (int)quot(local, j_end - j0);
-    j = j0 + (int)(local - (long long)tile * (j_end - j0));
-  }
-  // past the end of a tile's chunk
-  __device__ __forceinline__ void next_piece(const TreeParams& p, const Split& split) {
-    if (++tile == s.tiles) {
-      tile = 0;
-      if (++chunk == chunks) {
-        chunk = 0;
-        if (++kvh == p.nkh) {
-          kvh = 0;
-          do {
-            if (++b >= p.batch) {
-              s.stages = 0;
-              return;
-            }
-            s = seq_of(p, b);
-          } while (s.stages == 0);
-          chunk_of(split);
-        }
+  // past the last stage of a tile (more tiles than CTAs: one chunk)
+  __device__ __forceinline__ void next_tile(const TreeParams& p) {
+    j = 0;
+    if (++tile < s.tiles) return;
+    tile = 0;
+    if (++kvh < p.nkh) return;
+    kvh = 0;
+    do {
+      if (++b >= p.batch) {
+        s.stages = j_end = 0;
+        return;
       }
-    }
-    j = chunk_at(s.stages, chunks, chunk);
-    j_end = chunk_at(s.stages, chunks, chunk + 1);
+      s = seq_of(p, b);
+    } while (s.stages == 0);
+    j_end = s.stages;
   }
-  __device__ __forceinline__ void next(const TreeParams& p, const Split& split) {
-    if (++j == j_end) next_piece(p, split);
-  }
-  __device__ __forceinline__ bool begins() const { return j == chunk_at(s.stages, chunks, chunk); }
   // the first key from which every row sees all of the prefix
   __device__ __forceinline__ int kfull(const TreeParams& p) const {
     const long long k = p.window ? (long long)s.base + s.T - (long long)p.window : 0;
     return k < 0 ? 0 : k > s.base ? s.base : (int)k;
   }
-  __device__ __forceinline__ int key0(const TreeParams& p) const { return s.lo + j * p.kps; }
+  __device__ __forceinline__ int key0() const { return s.lo + (j << kStageLog2); }
   __device__ __forceinline__ bool clean(const TreeParams& p) const {
-    return key0(p) >= kfull(p) && key0(p) + p.kps <= s.base;
+    return key0() >= kfull(p) && key0() + (1 << kStageLog2) <= s.base;
   }
 };
 
-// Total stages over the batch, by one full warp (every lane returns it).
-__device__ __forceinline__ long long total_stages(const TreeParams& p) {
-  long long n = 0;
-  for (int b = threadIdx.x & 31; b < p.batch; b += 32) n += stages_of(p, seq_of(p, b));
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
-
-// The sequence that holds flattened stage s (s < total) and the first stage of that sequence; one
-// full warp, every lane returns them.
-__device__ __forceinline__ int find_seq(const TreeParams& p, long long s, long long& first) {
+// One full warp: the plan, and CTA `cta`'s first stage and their number (0: no work).
+__device__ __forceinline__ int deal(const TreeParams& p, int cta, int grid, Plan& plan, Walk& at) {
   const int lane = threadIdx.x & 31;
-  long long acc = 0;
+  // up to 32 sequences: lane b keeps sequence b
+  const bool kept = p.batch <= 32;
+  Seq mine = {};
+  if (kept && lane < p.batch) mine = seq_of(p, lane);
+  auto each_of = [&](auto f) {  // the lane's share of a sum over the batch
+    if (kept) return f(mine);
+    decltype(f(mine)) n = 0;
+    for (int b = lane; b < p.batch; b += 32) n += f(seq_of(p, b));
+    return n;
+  };
+  auto sum32 = [&](auto f) { return __reduce_add_sync(0xffffffffu, each_of(f)); };
+  constexpr int kMany = 1 << 16;  // (keeps sums of pieces below 2^31 for any batch)
+  const int tiles = sum32([&](const Seq& s) { return (int)min((long long)kMany, (long long)p.nkh * s.tiles); });
+  long long total = each_of([&](const Seq& s) { return (long long)p.nkh * s.tiles * s.stages; });
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  plan.run = 0;
+  plan.active = plan.each = plan.extra = 0;
+  if (total == 0) return 0;
+  int n_stages = 0;
+  if (tiles <= grid) {
+    int most = mine.stages;
+    if (!kept)
+      for (int b = lane; b < p.batch; b += 32) most = max(most, seq_of(p, b).stages);
+    const int longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+    auto pieces_at = [&](int run) {
+      return sum32([&](const Seq& s) { return (int)min((long long)kMany, (long long)p.nkh * s.tiles * ((s.stages + run - 1) / run)); });
+    };
+    int run = (int)min((long long)longest, quot(total + grid - 1, grid));
+    int pieces = pieces_at(run);
+    for (int k = 0; k < 12 && pieces > grid; k++) {
+      run = min(longest, max(run + 1, (int)quot((long long)run * pieces + grid - 1, grid)));
+      pieces = pieces_at(run);
+    }
+    if (pieces > grid) run = longest, pieces = tiles;
+    plan.run = run;
+    plan.active = pieces;
+    if (cta >= pieces) return 0;
+    int before = 0, hit = -1, local = 0;
+    Seq s = {};
+    for (int b0 = 0; b0 < p.batch && hit < 0; b0 += 32) {
+      if (!kept) mine = b0 + lane < p.batch ? seq_of(p, b0 + lane) : Seq{};
+      const int n = p.nkh * mine.tiles * ((mine.stages + run - 1) / run);
+      int incl = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      const int start = before + incl - n;
+      const unsigned found = __ballot_sync(0xffffffffu, n > 0 && cta >= start && cta < start + n);
+      if (found) {
+        const int src = __ffs(found) - 1;
+        hit = b0 + src;
+        local = cta - __shfl_sync(0xffffffffu, start, src);
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (hit < 0) return 0;
+    s = seq_of(p, hit);
+    at.s = s;
+    at.b = hit;
+    at.chunks = (s.stages + run - 1) / run;
+    const int q = local / s.tiles;
+    at.tile = local - q * s.tiles;
+    at.kvh = q / at.chunks;
+    at.chunk = q - at.kvh * at.chunks;
+    at.j = chunk_at(s.stages, at.chunks, at.chunk);
+    at.j_end = chunk_at(s.stages, at.chunks, at.chunk + 1);
+    return at.j_end - at.j;
+  }
+  plan.active = grid < total ? grid : total;
+  plan.each = quot(total, plan.active);
+  plan.extra = total - plan.each * plan.active;
+  if (cta >= plan.active) return 0;
+  const long long s0 = plan.begin(cta);
+  n_stages = (int)(plan.begin(cta + 1) - s0);
+  long long before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int b = b0 + lane;
-    const long long n = b < p.batch ? stages_of(p, seq_of(p, b)) : 0;
+    if (!kept) mine = b0 + lane < p.batch ? seq_of(p, b0 + lane) : Seq{};
+    const long long n = (long long)p.nkh * mine.tiles * mine.stages;
     long long incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    const long long start = acc + incl - n;
-    const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && s >= start && s < start + n);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      first = __shfl_sync(0xffffffffu, start, src);
-      return b0 + src;
+    const long long start = before + incl - n;
+    const unsigned found = __ballot_sync(0xffffffffu, n > 0 && s0 >= start && s0 < start + n);
+    if (found) {
+      const int src = __ffs(found) - 1;
+      const long long local = s0 - __shfl_sync(0xffffffffu, start, src);
+      at.b = b0 + src;
+      at.s = seq_of(p, at.b);
+      const long long item = quot(local, at.s.stages);
+      at.j = (int)(local - item * at.s.stages);
+      at.j_end = at.s.stages;
+      at.kvh = (int)quot(item, at.s.tiles);
+      at.tile = (int)(item - (long long)at.kvh * at.s.tiles);
+      at.chunks = 1;
+      at.chunk = 0;
+      return n_stages;
     }
-    acc += __shfl_sync(0xffffffffu, incl, 31);
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  first = acc;
-  return p.batch;
+  return 0;
 }
 
 // What query row r of a tile's sequence sees: prefix rows [kmin, base) and the drafted rows of

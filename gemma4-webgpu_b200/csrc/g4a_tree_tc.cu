@@ -44,7 +44,7 @@ namespace {
 using namespace g4a;
 using namespace g4a_tree;
 
-constexpr int kKeysT = 128;
+constexpr int kKeysT = 1 << kStageLog2;
 constexpr int kMaxGrid = 256;        // (the join looks at one cut per thread)
 constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one MMA and handing over
 constexpr int kUnit = 32768;         // 128 keys x 128 dims f16
@@ -298,52 +298,40 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   pdl_wait_primary();
   pdl_launch_dependents();
 
-  // ---- this CTA's run of stages
-  Split split;
-  split.of(total_stages(p), (int)gridDim.x);
-  const long long cta = blockIdx.x;
-  // (a CTA without work goes through the roles with 0 stages and frees its TMEM like the others)
-  const long long s0 = cta < split.active ? split.begin(cta) : 0;
-  const int n_stages = cta < split.active ? (int)(split.begin(cta + 1) - s0) : 0;
+  // ---- this CTA's stages.  (One without work goes through the roles with none and frees its TMEM
+  // like the others.)
+  Plan plan;
   Walk at = {};
-  if (n_stages > 0 && (warp == 15 || (warp >= 8 && warp < 12))) {
-    long long first = 0;
-    const int b = find_seq(p, s0, first);
-    at.seek(p, split, b, s0 - first);
-    if (warp == 15) {
-      // the tiles that are not whole and whose first pieces lie here: one at the run's begin, one at its end
-      Walk w = at;
-      long long s = s0;  // where piece w begins in this run
-      bool end_too = true;
-      for (int piece = 0; piece < 2; piece++) {
-        Cut c = {};
-        const long long s1 = min(s + (w.j_end - w.j), s0 + n_stages);
-        const bool whole = w.chunks == 1 && s1 - s == w.s.stages;
-        if ((piece == 0 || end_too) && w.j == 0 && !whole) {
-          c.base = s - (long long)w.tile * w.j_end;
-          c.stages = w.s.stages;
-          c.chunks = w.chunks;
-          c.tiles = w.s.tiles;
-          c.tile = w.tile;
-          c.each = (int)split.each;
-          c.extra = (int)split.extra;
-          c.parts = w.chunks > 1 ? w.chunks : (int)(split.owner(s + w.s.stages - 1) - cta) + 1;
-          c.rows = min(ROWS, w.s.T * p.group - w.tile * ROWS);
-          c.row0 = w.s.row0;
-          c.kvh = w.kvh;
-          c.first = w.tile * ROWS;
-        }
-        if (lane == 0) p.cuts[2 * cta + piece] = c;
-        // to the run's last piece
-        end_too = s1 < s0 + n_stages;
-        while (s + (w.j_end - w.j) < s0 + n_stages) {
-          s += w.j_end - w.j;
-          w.next_piece(p, split);
-        }
+  const int cta = (int)blockIdx.x;
+  const int n_stages = deal(p, cta, (int)gridDim.x, plan, at);
+  if (warp == 15) {
+    // the tiles whose first pieces lie here and that others go on with: one that begins with this
+    // CTA's stages, one at their end
+    Walk w = at;
+    int done = 0;  // stages before tile w
+    for (int piece = 0; piece < 2; piece++) {
+      Cut c = {};
+      const int here = min(w.s.stages - w.j, n_stages - done);
+      if (n_stages > 0 && w.j == 0 && here < w.s.stages && (piece == 0 || done > 0)) {
+        c.parts = plan.run > 0 ? w.chunks : (int)(plan.owner(plan.begin(cta) + done + w.s.stages - 1) - cta) + 1;
+        c.stride = plan.run > 0 ? 2 * w.s.tiles : 2;
+        c.rows = min(ROWS, w.s.T * p.group - w.tile * ROWS);
+        c.row0 = w.s.row0;
+        c.kvh = w.kvh;
+        c.first = w.tile * ROWS;
+      }
+      if (plan.run > 0 && w.chunks == 1) c.parts = 0;
+      if (lane == 0) p.cuts[2 * cta + piece] = c;
+      if (plan.run > 0) {
+        done = 0;
+        w.j = 1;  // (no second piece)
+        continue;
+      }
+      while (done + (w.j_end - w.j) < n_stages) {
+        done += w.j_end - w.j;
+        w.next_tile(p);
       }
     }
-  } else if (n_stages == 0 && warp == 15 && lane == 0) {
-    p.cuts[2 * cta].parts = p.cuts[2 * cta + 1].parts = 0;
   }
   __syncwarp();
   const uint32_t tmem = *tmem_slot;
@@ -441,11 +429,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     };
     for (int i = 0; i <= n_stages; i++) {
       if (i < n_stages) {
-        const bool first = i == 0 || w.begins();
+        const bool first = i == 0 || w.j == 0;
         if (first) tile_no++;
         if (first) load_queries();
         long long off = -1;
-        const int key = w.key0(p) + pw * 32 + lane;
+        const int key = w.key0() + pw * 32 + lane;
         if (key < w.s.L) off = row_offset(p, w.b, w.kvh, key);
         const uint32_t there = __ballot_sync(0xffffffffu, off >= 0);
         // (the ring holds at most five units, so the loads are at most five stages ahead of the softmax)
@@ -463,7 +451,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       }
       if (i > 0) load_units(rows_before, p.v);
       rows_before = rows;
-      if (i + 1 < n_stages) w.next(p, split);
+      if (++w.j == w.j_end && i + 1 < n_stages) w.next_tile(p);
     }
     cp_wait_all();
   } else if (warp >= 12) {
@@ -582,7 +570,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           for (int u = 0; u < MB; u++, unit++) {
             if (mixed) {
               (void)warp_wait(&landed[unit % UNITS], (uint32_t)(unit / UNITS) & 1u, abort_flag, p.err);
-              const int k0 = before.key0(p), a1 = before.kfull(p) - k0, b0 = before.s.base - k0, b1 = before.s.L - k0;
+              const int k0 = before.key0(), a1 = before.kfull(p) - k0, b0 = before.s.base - k0, b1 = before.s.L - k0;
               unsigned char* x0 = smem + C::OFF_RING + (unit % UNITS) * kUnit;
               bool bad = false;
               for (int e = hw * 32 + lane; e < kKeysT * 16; e += 96) {
@@ -663,7 +651,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       const int kvh = w.kvh, tile = w.tile;
       const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - half * RH;  // rows of this half
       if (live > 0) {
-        const int key0 = w.key0(p), key = key0 + key_in;
+        const int key0 = w.key0(), key = key0 + key_in;
         const uint4 ok4 = *reinterpret_cast<const uint4*>(okw + (i & 7) * 4);
         const bool clean = w.clean(p) && (ok4.x & ok4.y & ok4.z & ok4.w) == ~0u;
         const uint32_t okq = quarter == 0 ? ok4.x : quarter == 1 ? ok4.y : quarter == 2 ? ok4.z : ok4.w;
@@ -725,7 +713,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             const float4 u = u4[n / 4];
             far = fmaxf(far, fmaxf(fmaxf(x[n] - u.x, x[n + 1] - u.y), fmaxf(x[n + 2] - u.z, x[n + 3] - u.w)));
           }
-          if (any_of(far > kPUp + kRaise)) {
+          if (first || any_of(far > kPUp + kRaise)) {
             const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
             if (lane < W) smax[quarter * RH + g * W + lane] = mine;
             meet();
@@ -813,7 +801,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         if (live > 0) {
           const bool whole = w.chunks == 1 && j_first == 0 && w.j + 1 == w.s.stages;
           const bool later = i - (w.j - j_first) > 0;  // not the piece this CTA's run begins with
-          float* part = p.part + (size_t)(2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
+          float* part = p.part + ((size_t)2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
           float lt[G];
           meet();  // smax is free
 #pragma unroll
@@ -874,7 +862,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
                 if (n < nl) part[(size_t)(half * RH + g * W + n) * HD + d] = o[n];
             }
             if (bad && d < p.hd)
-              add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0(p) + kKeysT, w.s.L), w.kfull(p),
+              add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0() + kKeysT, w.s.L), w.kfull(p),
                                   d, tile * ROWS + half * RH + g * W, nl,
                                   whole ? nullptr : part + (size_t)(half * RH + g * W) * HD, HD);
           }
@@ -945,8 +933,8 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
     if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(tree_tc_kernel)");
     if (ctx->device < 64) done[ctx->device].store(true, std::memory_order_release);
   }
-  p.rows = C::ROWS;
-  p.kps = kKeysT;
+  p.rows_log2 = C::ROWS == 64 ? 6 : 5;
+  static_assert(C::ROWS == 64 || C::ROWS == 32, "tile rows");
   p.hd_pad = HD;
   const long long tiles = (tokens_rows + C::ROWS - 1) / C::ROWS;
   const long long stages = (keys / kKeysT + p.batch) * tiles * p.nkh;
