@@ -30,26 +30,28 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Joins the parts of the tiles that were cut between CTAs.  The work is cut into units of 128 head
-// dims of 1 to 4 rows of a tile, spread over all CTAs: 256 threads = 32 float4 columns x 8, which
-// are lanes over the parts of a row (a long context has one tile with a part in every CTA) or rows
-// (a batch of short ones has many tiles of two parts).  A lane folds its parts one by one with a
-// running maximum, several loads ahead; the lanes of a row meet in shared memory.
+// Joins the parts of the tiles that were cut between CTAs.  The work is cut into units spread over all
+// CTAs.  A thread is a float4 column of a row and a lane over its parts: 32 columns x 8 where a tile
+// has few parts (lanes over the parts, or over 2 or 4 rows), 8 columns x 32 where it has many (one long
+// context: a part in every CTA; 148 parts one after another by eight lanes took 9 us).  A lane folds
+// its parts four at a time with a running maximum; the lanes of a row meet in shared memory.
 constexpr int kMergeThreads = 256;
-constexpr int kMergeFly = 10;  // parts of a lane in flight
+constexpr int kMergeFly = 4;   // parts of a lane in flight
 constexpr int kMaxCuts = 512;  // two for each CTA of the attention kernel
 
 template <bool F32>
 __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreeParams p) {
   __shared__ int ends[kMaxCuts];  // running count of units up to and with cut c
   __shared__ int warp_sum[kMergeThreads / 32];
-  __shared__ float sm[8][2];
-  __shared__ float4 so[8][32];
-  const int tid = threadIdx.x, lane = tid & 31, sub = tid >> 5;
-  const int blocks = p.hd_pad / 128;
+  __shared__ float sm[32][2];
+  __shared__ float4 so[kMergeThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait_primary();
   pdl_launch_dependents();
-  auto lanes_of = [](int parts) { return parts > 4 ? 8 : parts > 2 ? 4 : 2; };
+  auto columns_of = [](int parts) { return parts > 32 ? 8 : 32; };
+  auto lanes_of = [](int parts) { return parts > 32 ? 32 : parts > 4 ? 8 : parts > 2 ? 4 : 2; };  // over parts
+  auto rows_of = [&](int parts) { return kMergeThreads / columns_of(parts) / lanes_of(parts); };  // of a unit
+  auto blocks_of = [&](int parts) { return p.hd_pad / 4 / columns_of(parts); };                   // units of a row
   {
     int n[2], incl = 0;
 #pragma unroll
@@ -59,8 +61,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
       if (c < 2 * p.grid) {
         const int parts = p.cuts[c].parts;
         if (parts > 0) {
-          const int rows_per = 8 / lanes_of(parts);
-          n[k] = (p.cuts[c].rows + rows_per - 1) / rows_per * blocks;
+          const int rows_per = rows_of(parts);
+          n[k] = (p.cuts[c].rows + rows_per - 1) / rows_per * blocks_of(parts);
         }
       }
       incl += n[k];
@@ -71,9 +73,9 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    if (lane == 31) warp_sum[sub] = incl;
+    if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    for (int w = 0; w < sub; w++) incl += warp_sum[w];
+    for (int w = 0; w < warp; w++) incl += warp_sum[w];
     ends[2 * tid] = incl - both + n[0];
     ends[2 * tid + 1] = incl;
     __syncthreads();
@@ -90,9 +92,10 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
     }
     const Cut cut = p.cuts[lo];
     const int at = unit - (lo ? ends[lo - 1] : 0);
-    const int pl = lanes_of(cut.parts), block = at % blocks;
-    const int r = at / blocks * (8 / pl) + sub / pl, part0 = sub % pl;
-    const int d = block * 128 + lane * 4;
+    const int cols = columns_of(cut.parts), pl = lanes_of(cut.parts), blocks = blocks_of(cut.parts);
+    const int col = tid & (cols - 1), sub = tid / cols, block = at % blocks;
+    const int r = at / blocks * rows_of(cut.parts) + sub / pl, part0 = sub & (pl - 1);
+    const int d = (block * cols + col) * 4;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < cut.rows) {
@@ -128,8 +131,8 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
         }
       }
     }
-    if (lane == 0) sm[sub][0] = m, sm[sub][1] = l;
-    so[sub][lane] = o;
+    if (col == 0) sm[sub][0] = m, sm[sub][1] = l;
+    so[tid] = o;
     __syncthreads();
     if (part0 == 0 && r < cut.rows && d < p.hd) {
       float mx = m;
@@ -138,7 +141,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
       o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int i = 0; i < pl; i++) {
         const float w = sm[sub + i][0] == mx ? 1.f : fast_exp2(sm[sub + i][0] - mx);
-        const float4 x = so[sub + i][lane];
+        const float4 x = so[tid + i * cols];
         lt += w * sm[sub + i][1];
         o.x += w * x.x;
         o.y += w * x.y;

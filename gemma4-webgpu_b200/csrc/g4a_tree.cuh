@@ -80,19 +80,24 @@ __device__ __forceinline__ long long quot(long long a, long long b) {
   return a / b;
 }
 
-// First stage of chunk c of n stages in `chunks`.
-__device__ __forceinline__ int chunk_at(int n, int chunks, int c) { return (int)quot((long long)n * c, chunks); }
+// First stage of chunk c of n stages in `chunks`; the first n % chunks have one more.
+__device__ __forceinline__ int chunk_at(int n, int chunks, int c) {
+  const uint32_t part = (uint32_t)n / (uint32_t)chunks, rest = (uint32_t)n - part * (uint32_t)chunks;
+  return (int)(part * (uint32_t)c + min((uint32_t)c, rest));
+}
 
 // How the tiles' stages are dealt to the CTAs, found by every warp for itself from the lengths on the
 // device.
-//  - At most one tile per CTA (`run` > 0): each kv head's keys are cut into the fewest chunks of at
-//    most `run` stages, run the smallest length found for which the pieces (chunk, tile) are no more
-//    than the CTAs, and CTA c does piece c, in the order sequence, kv head, chunk, tile.  A chunk's
-//    tiles are neighbours and read the same rows at the same time, so only one of them goes to HBM.
-//    (Tile after tile, the six tiles of a 131,000-key context came past each row 90 MB apart and the
-//    L2 had lost it.)
-//  - More tiles than CTAs: the list of all stages (sequence, kv head, tile, stage) is cut into equal
-//    runs.  A run holds whole tiles, and at most two pieces: one at its begin, one at its end.
+//  - One piece per CTA (`run` > 0), where that costs little balance: each kv head's keys are cut into
+//    the fewest chunks of at most `run` stages, run the smallest length found for which the pieces
+//    (chunk, tile) are no more than the CTAs, and CTA c does piece c, in the order sequence, kv head,
+//    chunk, tile.  A chunk's tiles are neighbours and read the same rows at the same time, so only
+//    one of them goes to HBM.  (Tile after tile, the six tiles of a 131,000-key context came past
+//    each row 90 MB apart and the L2 had lost it: 321 us instead of 221.)  A piece's start and end
+//    cost as much as two to four stages, so one longer piece beats two (64 tokens over 32k keys: 78
+//    -> 64 us) unless the longest is more than a quarter (and a stage) above the mean.
+//  - Else the list of all stages (sequence, kv head, tile, stage) is cut into equal runs.  A run holds
+//    whole tiles, and at most two pieces: one at its begin, one at its end.
 struct Plan {
   int run;
   long long active, each, extra;
@@ -137,90 +142,83 @@ struct Walk {
   }
 };
 
-// One full warp: the plan, and CTA `cta`'s first stage and their number (0: no work).
-__device__ __forceinline__ int deal(const TreeParams& p, int cta, int grid, Plan& plan, Walk& at) {
+__device__ __forceinline__ void seek_piece(const TreeParams& p, int run, int b, const Seq& s, uint32_t local, Walk& at) {
+  at.s = s;
+  at.b = b;
+  at.chunks = (int)((uint32_t)(s.stages + run - 1) / (uint32_t)run);
+  const uint32_t q = local / (uint32_t)s.tiles;
+  at.tile = (int)(local - q * (uint32_t)s.tiles);
+  at.kvh = (int)(q / (uint32_t)at.chunks);
+  at.chunk = (int)(q - (uint32_t)at.kvh * (uint32_t)at.chunks);
+  at.j = chunk_at(s.stages, at.chunks, at.chunk);
+  at.j_end = chunk_at(s.stages, at.chunks, at.chunk + 1);
+}
+__device__ __forceinline__ void seek_stage(const TreeParams& p, int b, const Seq& s, long long local, Walk& at) {
+  at.s = s;
+  at.b = b;
+  const long long item = quot(local, s.stages);
+  at.j = (int)(local - item * s.stages);
+  at.j_end = s.stages;
+  at.kvh = (int)quot(item, s.tiles);
+  at.tile = (int)(item - (long long)at.kvh * s.tiles);
+  at.chunks = 1;
+  at.chunk = 0;
+}
+// Whether pieces of `run` stages are worth it where equal runs have `mean`.
+__device__ __forceinline__ bool run_fits(long long run, long long mean) { return run <= mean + mean / 4 + 1; }
+
+// The general case of deal(): any batch, totals beyond 32 bits.
+static __device__ __noinline__ int deal_any(const TreeParams& p, int cta, int grid, Plan& plan, Walk& at) {
   const int lane = threadIdx.x & 31;
-  // up to 32 sequences: lane b keeps sequence b
-  const bool kept = p.batch <= 32;
-  Seq mine = {};
-  if (kept && lane < p.batch) mine = seq_of(p, lane);
-  auto each_of = [&](auto f) {  // the lane's share of a sum over the batch
-    if (kept) return f(mine);
-    decltype(f(mine)) n = 0;
-    for (int b = lane; b < p.batch; b += 32) n += f(seq_of(p, b));
+  auto warp_sum = [](long long n) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
   };
-  auto sum32 = [&](auto f) { return __reduce_add_sync(0xffffffffu, each_of(f)); };
-  constexpr int kMany = 1 << 16;  // (keeps sums of pieces below 2^31 for any batch)
-  const int tiles = sum32([&](const Seq& s) { return (int)min((long long)kMany, (long long)p.nkh * s.tiles); });
-  long long total = each_of([&](const Seq& s) { return (long long)p.nkh * s.tiles * s.stages; });
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  long long tiles = 0, total = 0;
+  int longest = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const Seq s = seq_of(p, b);
+    tiles += (long long)p.nkh * s.tiles;
+    total += (long long)p.nkh * s.tiles * s.stages;
+    longest = max(longest, s.stages);
+  }
+  tiles = warp_sum(tiles);
+  total = warp_sum(total);
+  longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
   plan.run = 0;
   plan.active = plan.each = plan.extra = 0;
   if (total == 0) return 0;
-  int n_stages = 0;
+  const long long mean = quot(total + grid - 1, grid);
   if (tiles <= grid) {
-    int most = mine.stages;
-    if (!kept)
-      for (int b = lane; b < p.batch; b += 32) most = max(most, seq_of(p, b).stages);
-    const int longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
-    auto pieces_at = [&](int run) {
-      return sum32([&](const Seq& s) { return (int)min((long long)kMany, (long long)p.nkh * s.tiles * ((s.stages + run - 1) / run)); });
-    };
-    int run = (int)min((long long)longest, quot(total + grid - 1, grid));
-    int pieces = pieces_at(run);
-    for (int k = 0; k < 12 && pieces > grid; k++) {
-      run = min(longest, max(run + 1, (int)quot((long long)run * pieces + grid - 1, grid)));
-      pieces = pieces_at(run);
-    }
-    if (pieces > grid) run = longest, pieces = tiles;
-    plan.run = run;
-    plan.active = pieces;
-    if (cta >= pieces) return 0;
-    int before = 0, hit = -1, local = 0;
-    Seq s = {};
-    for (int b0 = 0; b0 < p.batch && hit < 0; b0 += 32) {
-      if (!kept) mine = b0 + lane < p.batch ? seq_of(p, b0 + lane) : Seq{};
-      const int n = p.nkh * mine.tiles * ((mine.stages + run - 1) / run);
-      int incl = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
+    long long run = min((long long)longest, mean), pieces = 0;
+    for (int k = 0; k < 12; k++) {
+      pieces = 0;
+      for (int b = lane; b < p.batch; b += 32) {
+        const Seq s = seq_of(p, b);
+        pieces += (long long)p.nkh * s.tiles * quot(s.stages + run - 1, run);
       }
-      const int start = before + incl - n;
-      const unsigned found = __ballot_sync(0xffffffffu, n > 0 && cta >= start && cta < start + n);
-      if (found) {
-        const int src = __ffs(found) - 1;
-        hit = b0 + src;
-        local = cta - __shfl_sync(0xffffffffu, start, src);
-      }
-      before += __shfl_sync(0xffffffffu, incl, 31);
+      pieces = warp_sum(pieces);
+      if (pieces <= grid || !run_fits(run, mean)) break;
+      run = min((long long)longest, max(run + 1, quot(run * pieces + grid - 1, grid)));
     }
-    if (hit < 0) return 0;
-    s = seq_of(p, hit);
-    at.s = s;
-    at.b = hit;
-    at.chunks = (s.stages + run - 1) / run;
-    const int q = local / s.tiles;
-    at.tile = local - q * s.tiles;
-    at.kvh = q / at.chunks;
-    at.chunk = q - at.kvh * at.chunks;
-    at.j = chunk_at(s.stages, at.chunks, at.chunk);
-    at.j_end = chunk_at(s.stages, at.chunks, at.chunk + 1);
-    return at.j_end - at.j;
+    if (pieces <= grid && run_fits(run, mean)) {
+      plan.run = (int)run;
+      plan.active = pieces;
+    }
   }
-  plan.active = grid < total ? grid : total;
-  plan.each = quot(total, plan.active);
-  plan.extra = total - plan.each * plan.active;
+  if (plan.run == 0) {
+    plan.active = grid < total ? grid : total;
+    plan.each = quot(total, plan.active);
+    plan.extra = total - plan.each * plan.active;
+  }
   if (cta >= plan.active) return 0;
-  const long long s0 = plan.begin(cta);
-  n_stages = (int)(plan.begin(cta + 1) - s0);
+  const long long want = plan.run > 0 ? cta : plan.begin(cta);
   long long before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    if (!kept) mine = b0 + lane < p.batch ? seq_of(p, b0 + lane) : Seq{};
-    const long long n = (long long)p.nkh * mine.tiles * mine.stages;
+    const Seq s = b0 + lane < p.batch ? seq_of(p, b0 + lane) : Seq{};
+    const long long n =
+        (long long)p.nkh * s.tiles * (plan.run > 0 ? quot(s.stages + plan.run - 1, plan.run) : (long long)s.stages);
     long long incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -228,20 +226,98 @@ __device__ __forceinline__ int deal(const TreeParams& p, int cta, int grid, Plan
       if (lane >= o) incl += t;
     }
     const long long start = before + incl - n;
-    const unsigned found = __ballot_sync(0xffffffffu, n > 0 && s0 >= start && s0 < start + n);
+    const unsigned found = __ballot_sync(0xffffffffu, n > 0 && want >= start && want < start + n);
     if (found) {
       const int src = __ffs(found) - 1;
-      const long long local = s0 - __shfl_sync(0xffffffffu, start, src);
-      at.b = b0 + src;
-      at.s = seq_of(p, at.b);
-      const long long item = quot(local, at.s.stages);
-      at.j = (int)(local - item * at.s.stages);
-      at.j_end = at.s.stages;
-      at.kvh = (int)quot(item, at.s.tiles);
-      at.tile = (int)(item - (long long)at.kvh * at.s.tiles);
-      at.chunks = 1;
-      at.chunk = 0;
-      return n_stages;
+      const long long local = want - __shfl_sync(0xffffffffu, start, src);
+      const Seq hit = seq_of(p, b0 + src);
+      if (plan.run > 0) {
+        seek_piece(p, plan.run, b0 + src, hit, (uint32_t)local, at);
+        return at.j_end - at.j;
+      }
+      seek_stage(p, b0 + src, hit, local, at);
+      return (int)(plan.begin(cta + 1) - want);
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return 0;
+}
+
+constexpr int kTable = 512;  // sequences that deal() keeps in shared memory
+
+// The table's entry of sequence b: tiles of all kv heads, stages of a tile.
+__device__ __forceinline__ int2 table_entry(const TreeParams& p, int b) {
+  const Seq s = seq_of(p, b);
+  return make_int2(p.nkh * s.tiles, s.stages);
+}
+
+// One full warp: the plan, CTA `cta`'s first stage, and their number (0: no work).  Up to kTable
+// sequences are dealt from `table` (filled by the whole CTA: one round of loads) in 32 bits and little
+// code: the kernels start cold, and every line of code on this path is fetched before the first key is.
+__device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int cta, int grid, Plan& plan, Walk& at) {
+  const int lane = threadIdx.x & 31;
+  int tiles = 0, total = 0;
+  bool large = p.batch > kTable;
+  for (int b = lane; b < p.batch && !large; b += 32) {
+    const int2 e = table[b];
+    const long long n = (long long)e.x * e.y;
+    large = n > 0x3fffff || total > 0x3ffffff;
+    tiles += e.x;
+    total += (int)n;
+  }
+  if (__any_sync(0xffffffffu, large)) return deal_any(p, cta, grid, plan, at);
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
+  total = __reduce_add_sync(0xffffffffu, total);
+  plan.run = 0;
+  plan.active = plan.each = plan.extra = 0;
+  if (total == 0) return 0;
+  const int mean = (int)((uint32_t)(total + grid - 1) / (uint32_t)grid);
+  if (tiles <= grid) {
+    int run = mean;
+    do {
+      int pieces = 0;
+      for (int b = lane; b < p.batch; b += 32) {
+        const int2 e = table[b];
+        pieces += e.x * (int)((uint32_t)(e.y + run - 1) / (uint32_t)run);
+      }
+      pieces = __reduce_add_sync(0xffffffffu, pieces);
+      if (pieces <= grid) {
+        plan.run = run;
+        plan.active = pieces;
+        break;
+      }
+      run = max(run + 1, (int)quot((long long)run * pieces, grid));
+    } while (run_fits(run, mean));
+  }
+  if (plan.run == 0) {
+    plan.active = min(grid, total);
+    plan.each = (uint32_t)total / (uint32_t)plan.active;
+    plan.extra = total - plan.each * plan.active;
+  }
+  if (cta >= plan.active) return 0;
+  const int want = plan.run > 0 ? cta : (int)plan.begin(cta);
+  int before = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int2 e = b0 + lane < p.batch ? table[b0 + lane] : make_int2(0, 0);
+    const int n = e.x * (plan.run > 0 ? (int)((uint32_t)(e.y + plan.run - 1) / (uint32_t)plan.run) : e.y);
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const int start = before + incl - n;
+    const unsigned found = __ballot_sync(0xffffffffu, want >= start && want < start + n);
+    if (found) {
+      const int src = __ffs(found) - 1;
+      const int local = want - __shfl_sync(0xffffffffu, start, src);
+      const Seq hit = seq_of(p, b0 + src);
+      if (plan.run > 0) {
+        seek_piece(p, plan.run, b0 + src, hit, (uint32_t)local, at);
+        return at.j_end - at.j;
+      }
+      seek_stage(p, b0 + src, hit, local, at);
+      return (int)plan.begin(cta + 1) - want;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
   }

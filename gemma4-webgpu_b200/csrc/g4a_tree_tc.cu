@@ -303,7 +303,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   Plan plan;
   Walk at = {};
   const int cta = (int)blockIdx.x;
-  const int n_stages = deal(p, cta, (int)gridDim.x, plan, at);
+  // (the table lies where P will: P is written after every warp has read it)
+  int2* table = reinterpret_cast<int2*>(smem + C::OFF_P);
+  static_assert(C::P_BYTES >= kTable * (int)sizeof(int2), "table of sequences");
+  if (p.batch <= kTable) {
+    for (int b = tid; b < p.batch; b += kThreadsTc) table[b] = table_entry(p, b);
+    __syncthreads();
+  }
+  const int n_stages = deal(p, table, cta, (int)gridDim.x, plan, at);
   if (warp == 15) {
     // the tiles whose first pieces lie here and that others go on with: one that begins with this
     // CTA's stages, one at their end
