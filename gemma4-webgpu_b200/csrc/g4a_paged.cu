@@ -24,9 +24,8 @@ struct PrepParams {
   int* err;
 };
 
-// The cache row (in units of nkh * hd elements) of token i, or -1 when it is not to be stored.
-__device__ __forceinline__ long long cache_row(const PrepParams& p, uint32_t i, int seq) {
-  const int slot = p.slots[i];
+// The cache row (in units of nkh * hd elements) of a slot, or -1 when it is not to be stored.
+__device__ __forceinline__ long long cache_row(const PrepParams& p, int slot, int seq) {
   if (slot < 0) return -1;
   const int j = slot / p.page_size;
   if (j >= p.max_pages) {
@@ -92,9 +91,12 @@ __device__ __forceinline__ float warp_sum(float x) {
 }
 
 // y = x w / sqrt(mean(x^2) + eps), then the pairs (p, p + hd/2) turned by the token's angles:
-// (a, b) -> (a cos - b sin, a sin + b cos).  v heads are divided only.  One warp per head of a
-// token; the heads of a token are neighbours, so its cos / sin row comes from L1 after the first.
-// Everything is in f32; q leaves in f32 or rounded once to f16, k and v rounded once to f16.
+// (a, b) -> (a cos - b sin, a sin + b cos).  v heads are divided only.  Everything is in f32; q leaves
+// in f32 or rounded once to f16, k and v rounded once to f16.
+// Bound by HBM for many tokens and by latency for few, so a warp takes two neighbouring heads of a
+// token, reads its cos / sin row once for both, and issues every load that needs no other one (both
+// heads, angles, sequence, slot) before it waits for the first; only the page id has to follow.
+// (One head per warp that first looked at the token's sequence: 36 us for 9,005 tokens of 10 heads.)
 // VEC > 0: hd = 64 VEC, a lane holds VEC consecutive elements of each half, in vector loads and
 // stores (16 bytes at hd >= 256).  VEC = 0: any even hd <= 512 and any alignment, elements
 // strided by 32 lanes.
@@ -102,103 +104,119 @@ template <int VEC, typename QOut>
 __global__ void __launch_bounds__(kPrepWarps * 32) paged_prep_kernel(const PrepParams p) {
   constexpr int N = VEC > 0 ? VEC : 8;  // elements of each half per lane
   const int lane = threadIdx.x & 31;
+  const uint32_t pairs = (uint32_t)(p.heads + 1) / 2;
   const uint64_t w = (uint64_t)blockIdx.x * kPrepWarps + (threadIdx.x >> 5);
-  const uint32_t tok = (uint32_t)(w / (uint32_t)p.heads);
-  const int head = (int)(w - (uint64_t)tok * (uint32_t)p.heads);
+  const uint32_t tok = (uint32_t)(w / pairs);
+  const int head0 = 2 * (int)(w - (uint64_t)tok * pairs);
   const int hd = p.hd, half = hd / 2;
   g4a::pdl_wait_primary();
   g4a::pdl_launch_dependents();
   if (tok >= p.tokens) return;
-  const int seq = p.token_seq[tok];
-  if (seq < 0) return;  // padding: nothing of this token is read or written
-  if (seq >= p.batch) {
-    if (lane == 0) atomicExch(p.err, G4A_DEVERR_SLOT);
-    return;
-  }
-  const bool is_q = head < p.nqh, is_k = !is_q && head < p.nqh + p.nkh;
-  const int kvh = is_q ? 0 : is_k ? head - p.nqh : head - p.nqh - p.nkh;
-  long long row = 0;
-  if (!is_q) {
-    row = cache_row(p, tok, seq);
-    if (row < 0) return;
-  }
-  const float* src = is_q   ? p.q + (size_t)tok * p.q_stride + (size_t)head * hd
-                     : is_k ? p.k + (size_t)tok * p.kv_stride + (size_t)kvh * hd
-                            : p.v + (size_t)tok * p.kv_stride + (size_t)kvh * hd;
-  __half* kv = (is_k ? p.k_pages : p.v_pages) + ((size_t)row * p.nkh + kvh) * hd;
-  QOut* qo = reinterpret_cast<QOut*>(p.q_out) + ((size_t)tok * p.nqh + head) * hd;
-  float a[N], b[N], c[N], s[N];
   // a pair's index of element e of this lane
   auto at = [&](int e) { return VEC > 0 ? lane * N + e : lane + 32 * e; };
-  if constexpr (VEC > 0) {
-    load_f32<N>(src + lane * N, a);
-    load_f32<N>(src + half + lane * N, b);
-    if (is_q || is_k) {
-      const float* cs = p.cos_sin + (size_t)tok * hd;
-      load_f32<N>(cs + lane * N, c);
-      load_f32<N>(cs + half + lane * N, s);
-    }
-  } else {
+  const bool turns = head0 < p.nqh + p.nkh;      // a q or k head among the two
+  const bool stores = head0 + 1 >= p.nqh && p.k;  // a k or v head among them (or past the last)
+  const int seq = p.token_seq[tok];
+  const int slot = stores ? p.slots[tok] : -1;
+  float a[2][N], b[2][N], c[N], s[N];
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      const bool in = at(e) < half;
-      a[e] = in ? src[at(e)] : 0.f;
-      b[e] = in ? src[half + at(e)] : 0.f;
-      if (is_q || is_k) {
-        c[e] = in ? p.cos_sin[(size_t)tok * hd + at(e)] : 0.f;
-        s[e] = in ? p.cos_sin[(size_t)tok * hd + half + at(e)] : 0.f;
-      }
-    }
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < N; e++) ss += a[e] * a[e] + b[e] * b[e];
-  const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)hd + p.eps);
-  if (is_q || is_k) {
-    const __half* wt = is_q ? p.qw : p.kw;
-    float wa[N], wb[N];
+  for (int u = 0; u < 2; u++) {
+    const int head = min(head0 + u, p.heads - 1);
+    const float* src = head < p.nqh           ? p.q + (size_t)tok * p.q_stride + (size_t)head * hd
+                       : head < p.nqh + p.nkh ? p.k + (size_t)tok * p.kv_stride + (size_t)(head - p.nqh) * hd
+                                              : p.v + (size_t)tok * p.kv_stride + (size_t)(head - p.nqh - p.nkh) * hd;
     if constexpr (VEC > 0) {
-      load_f16<N>(wt + lane * N, wa);
-      load_f16<N>(wt + half + lane * N, wb);
+      load_f32<N>(src + lane * N, a[u]);
+      load_f32<N>(src + half + lane * N, b[u]);
     } else {
 #pragma unroll
       for (int e = 0; e < N; e++) {
         const bool in = at(e) < half;
-        wa[e] = in ? __half2float(wt[at(e)]) : 0.f;
-        wb[e] = in ? __half2float(wt[half + at(e)]) : 0.f;
+        a[u][e] = in ? src[at(e)] : 0.f;
+        b[u][e] = in ? src[half + at(e)] : 0.f;
       }
     }
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      const float x = a[e] * wa[e] * inv, y = b[e] * wb[e] * inv;
-      a[e] = x * c[e] - y * s[e];
-      b[e] = x * s[e] + y * c[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; e++) a[e] *= inv, b[e] *= inv;
   }
-  if constexpr (VEC > 0) {
-    if (!is_q) {
-      store_f16<N>(kv + lane * N, a);
-      store_f16<N>(kv + half + lane * N, b);
-    } else if constexpr (sizeof(QOut) == 4) {
-      store_f32<N>(qo + lane * N, a);
-      store_f32<N>(qo + half + lane * N, b);
+  if (turns) {
+    const float* cs = p.cos_sin + (size_t)tok * hd;
+    if constexpr (VEC > 0) {
+      load_f32<N>(cs + lane * N, c);
+      load_f32<N>(cs + half + lane * N, s);
     } else {
-      store_f16<N>(qo + lane * N, a);
-      store_f16<N>(qo + half + lane * N, b);
-    }
-  } else {
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      if (at(e) >= half) continue;
-      if (!is_q) {
-        kv[at(e)] = __float2half_rn(a[e]);
-        kv[half + at(e)] = __float2half_rn(b[e]);
+      for (int e = 0; e < N; e++) {
+        const bool in = at(e) < half;
+        c[e] = in ? cs[at(e)] : 0.f;
+        s[e] = in ? cs[half + at(e)] : 0.f;
+      }
+    }
+  }
+  if (seq < 0) return;  // padding: nothing of this token is written
+  if (seq >= p.batch) {
+    if (lane == 0) atomicExch(p.err, G4A_DEVERR_SLOT);
+    return;
+  }
+  const long long row = stores ? cache_row(p, slot, seq) : -1;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int head = head0 + u;
+    if (head >= p.heads) break;
+    const bool is_q = head < p.nqh, is_k = !is_q && head < p.nqh + p.nkh;
+    if (!is_q && row < 0) continue;
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; e++) ss += a[u][e] * a[u][e] + b[u][e] * b[u][e];
+    const float inv = 1.0f / sqrtf(warp_sum(ss) / (float)hd + p.eps);
+    float y0[N], y1[N];
+    if (is_q || is_k) {
+      const __half* wt = is_q ? p.qw : p.kw;
+      float wa[N], wb[N];
+      if constexpr (VEC > 0) {
+        load_f16<N>(wt + lane * N, wa);
+        load_f16<N>(wt + half + lane * N, wb);
       } else {
-        qo[at(e)] = (QOut)a[e];
-        qo[half + at(e)] = (QOut)b[e];
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          const bool in = at(e) < half;
+          wa[e] = in ? __half2float(wt[at(e)]) : 0.f;
+          wb[e] = in ? __half2float(wt[half + at(e)]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const float x = a[u][e] * wa[e] * inv, y = b[u][e] * wb[e] * inv;
+        y0[e] = x * c[e] - y * s[e];
+        y1[e] = x * s[e] + y * c[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++) y0[e] = a[u][e] * inv, y1[e] = b[u][e] * inv;
+    }
+    const int kvh = is_q ? 0 : is_k ? head - p.nqh : head - p.nqh - p.nkh;
+    __half* kv = (is_k ? p.k_pages : p.v_pages) + ((size_t)(is_q ? 0 : row) * p.nkh + kvh) * hd;
+    QOut* qo = reinterpret_cast<QOut*>(p.q_out) + ((size_t)tok * p.nqh + head) * hd;
+    if constexpr (VEC > 0) {
+      if (!is_q) {
+        store_f16<N>(kv + lane * N, y0);
+        store_f16<N>(kv + half + lane * N, y1);
+      } else if constexpr (sizeof(QOut) == 4) {
+        store_f32<N>(qo + lane * N, y0);
+        store_f32<N>(qo + half + lane * N, y1);
+      } else {
+        store_f16<N>(qo + lane * N, y0);
+        store_f16<N>(qo + half + lane * N, y1);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        if (at(e) >= half) continue;
+        if (!is_q) {
+          kv[at(e)] = __float2half_rn(y0[e]);
+          kv[half + at(e)] = __float2half_rn(y1[e]);
+        } else {
+          qo[at(e)] = (QOut)y0[e];
+          qo[half + at(e)] = (QOut)y1[e];
+        }
       }
     }
   }
@@ -356,7 +374,7 @@ g4a_status g4a_paged_qkv_prep(g4a_ctx* ctx, const float* q, const float* k, cons
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_norm_w | (uintptr_t)k_norm_w |
                          (uintptr_t)cos_sin | (uintptr_t)q_out;
   const bool vec = (ptrs & 15u) == 0 && ((q_row_stride | kv_row_stride) & 3u) == 0;
-  const uint64_t warps = (uint64_t)num_tokens * (uint32_t)p.heads;
+  const uint64_t warps = (uint64_t)num_tokens * ((uint32_t)(p.heads + 1) / 2);
   const uint64_t blocks = (warps + kPrepWarps - 1) / kPrepWarps;
   if (blocks > 0x7fffffffull) return g4a_fail(G4A_EINVAL, "%s: num_tokens * heads too large", fn);
   g4a_prof_scope ps(ctx, G4A_PROF_PAGED_PREP);

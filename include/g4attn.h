@@ -410,7 +410,7 @@ g4a_status g4a_rope_table(g4a_ctx* ctx, const int32_t* positions, const uint16_t
  * be columns of one projection's output; they are left as they are.  q_out is packed, f32 or f16
  * (q_out_format).  Token i belongs to sequence token_seq[i] in [0, batch) and is stored in row
  * slots[i] of it: page page_table[token_seq[i]*max_pages_per_seq + slots[i]/page_size], row
- * slots[i]%page_size.  token_seq[i] < 0 is padding: nothing of the token is read or written.
+ * slots[i]%page_size.  token_seq[i] < 0 is padding: nothing of the token is written.
  * slots[i] < 0 stores nothing but computes q.  The (sequence, slot) pairs of one call must be
  * distinct.  A sequence index, slot or page id out of range is not stored and g4a_sync reports
  * it.  k = v = NULL (a layer that reads another layer's cache) computes q alone; num_q_heads = 0
