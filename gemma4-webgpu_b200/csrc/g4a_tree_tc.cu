@@ -46,7 +46,10 @@ using namespace g4a_tree;
 
 constexpr int kKeysT = 1 << kStageLog2;
 constexpr int kMaxGrid = 256;        // (the join looks at one cut per thread)
-constexpr int kThreadsTc = 16 * 32;  // four warpgroups: two softmax, one loading, one MMA and handing over
+constexpr int kSoftWarps = 8;        // two for each lane quarter: the rows in two shares
+constexpr int kLoadWarp = kSoftWarps, kMmaWarp = kLoadWarp + 4;
+constexpr int kThreadsTc = (kMmaWarp + 4) * 32;  // softmax, loading, MMA and handing over
+constexpr int kShares = kSoftWarps / 4;
 constexpr int kUnit = 32768;         // 128 keys x 128 dims f16
 constexpr float kPUp = 7.0f;         // p = 2^(s - m + 7)
 constexpr float kRaise = 8.0f;       // a score this far above m raises it
@@ -56,15 +59,12 @@ template <int HD, int N, bool F32>
 struct Tc {
   static constexpr int MB = HD / 128;                 // 128-dim blocks = ring units of a K or V tile
   static constexpr int ROWS = F32 ? N / 2 : N;        // query rows of a tile
-  static constexpr int RH = ROWS / 2;                 // rows of a softmax half
-  static constexpr int W = RH < 32 ? RH : 32;         // rows a thread works on at a time
-  static constexpr int G = RH / W;
-  // Registers: 512 threads start with 128 each (65,536).  The softmax warpgroups, which hold a block
-  // of scores and row sums, take more and the others give theirs.  (Spills are dear here: shared
-  // memory leaves the L1 almost nothing, so local memory is in the L2.)
-  static constexpr int REGS_SOFTMAX = G > 1 ? 184 : N > 64 ? 168 : 160;
-  static constexpr int REGS_LOAD = G > 1 ? 80 : N > 64 ? 96 : 112, REGS_MMA = G > 1 ? 64 : 80;
-  static_assert(256 * REGS_SOFTMAX + 128 * REGS_LOAD + 128 * REGS_MMA <= 65536, "register file");
+  static constexpr int W = ROWS / kShares;            // rows of a softmax warp (its share)
+  // Registers: 512 threads start with 128 each (65,536); the softmax warps, which hold a block of
+  // scores and the row sums, take some from the others.  (Spills are dear here: shared memory leaves
+  // the L1 almost nothing, so local memory is in the L2.)
+  static constexpr int REGS_SOFT = 160, REGS_LOAD = 112, REGS_MMA = 80;
+  static_assert(kSoftWarps * 32 * REGS_SOFT + 128 * REGS_LOAD + 128 * REGS_MMA <= kThreadsTc * 128, "register file");
   static constexpr int Q_BYTES = N * HD * 2;
   static constexpr int P_BYTES = kKeysT * N * 2;
   static constexpr int FIT2 = (216 * 1024 - 2 * Q_BYTES - P_BYTES) / kUnit;
@@ -75,15 +75,15 @@ struct Tc {
   static constexpr int OFF_RING = OFF_P + P_BYTES;
   static constexpr int OFF_SEES = OFF_RING + UNITS * kUnit;   // [4][ROWS] Sees
   static constexpr int OFF_SCALE = OFF_SEES + 4 * ROWS * 16;  // [4][ROWS]
-  static constexpr int OFF_U = OFF_SCALE + 4 * ROWS * 4;      // [8 warps][RH] m - 7 of its rows
-  static constexpr int OFF_F = OFF_U + 8 * RH * 4;            // [8 warps][RH] rescale factors
-  static constexpr int OFF_MAX = OFF_F + 8 * RH * 4;          // [2 halves][4 quarters][RH]
-  static constexpr int OFF_OK = OFF_MAX + 8 * RH * 4;         // [8 stages][4] which rows are there
+  static constexpr int OFF_U = OFF_SCALE + 4 * ROWS * 4;      // [softmax warps][W] m - 7 of its rows
+  static constexpr int OFF_F = OFF_U + kSoftWarps * W * 4;    // [softmax warps][W] rescale factors
+  static constexpr int OFF_MAX = OFF_F + kSoftWarps * W * 4;  // [shares][4 quarters][W]
+  static constexpr int OFF_OK = OFF_MAX + kSoftWarps * W * 4; // [8 stages][4] which rows are there
   static constexpr int OFF_BAD = OFF_OK + 128;                // [8] tile + 1 that had a V value that is not finite
-  static constexpr int OFF_VOTE = OFF_BAD + 32;               // [2 halves][2][4 quarters]
-  static constexpr int OFF_INFO = OFF_VOTE + 64;               // [4] Walk of a piece's begin
+  static constexpr int OFF_VOTE = OFF_BAD + 32;               // [shares][2][4 quarters]
+  static constexpr int OFF_INFO = OFF_VOTE + kShares * 32;               // [4] Walk of a piece's begin
   static constexpr int OFF_BAR = OFF_INFO + 4 * 64;
-  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5 + 2;
+  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5 + kShares;
   static constexpr int OFF_END = OFF_BAR + NBARS * 8;
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
@@ -158,29 +158,49 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[W]) {
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[32]) { tmem_st32(taddr, r); }
 __device__ __forceinline__ void tmem_store(uint32_t taddr, const uint32_t (&r)[16]) { tmem_st16(taddr, r); }
 
-// True in one lane of a converged warp (always the same one).
-__device__ __forceinline__ bool elect_one() {
+// 1 in one lane of a converged warp (always the same one), 0 in the others.
+__device__ __forceinline__ uint32_t elect_one() {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(r));
-  return r != 0;
+  return r;
+}
+// D (+)= A B^T and the commit, by the lane for which `on` is not 0.  The instructions are predicated, not
+// branched to, so that the warp's control flow stays uniform and the descriptors in uniform registers.
+__device__ __forceinline__ void umma_if(uint32_t on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t on, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(on)
+      : "memory");
 }
 
-// Reduces W values per lane over the warp's lanes, value n's result in lane n (W = 16: also in lane
-// n + 16).  Each step hands half of the values to the lane at distance o and keeps the other half.
+// Reduces W (16 or 32) values per lane over the warp's lanes; value n's result in the lanes n % W.  Each
+// step of the second loop hands half of the values to the lane at distance o and keeps the others.
 template <int W, typename Op>
 __device__ __forceinline__ float transpose_reduce(const float (&x)[W], Op op) {
   const int lane = threadIdx.x & 31;
   float v[W];
 #pragma unroll
   for (int n = 0; n < W; n++) v[n] = x[n];
-  if constexpr (W == 16) {
 #pragma unroll
-    for (int n = 0; n < 16; n++) v[n] = op(v[n], __shfl_xor_sync(0xffffffffu, v[n], 16));
-  }
+  for (int o = 16; o >= W; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < W; n++) v[n] = op(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
 #pragma unroll
   for (int o = W / 2; o >= 1; o >>= 1) {
     const bool up = (lane & o) != 0;
@@ -228,7 +248,7 @@ __device__ __noinline__ void add_non_finite(const TreeParams& p, Seq s, int b, i
 template <int HD, int N, bool F32>
 __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_constant__ TreeParams p) {
   using C = Tc<HD, N, F32>;
-  constexpr int MB = C::MB, ROWS = C::ROWS, RH = C::RH, W = C::W, G = C::G, UNITS = C::UNITS, NQ = C::NQ;
+  constexpr int MB = C::MB, ROWS = C::ROWS, W = C::W, UNITS = C::UNITS, NQ = C::NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -247,12 +267,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   uint64_t* qfull = qlanded + 4;        // [4] 3 handing-over warps
   uint64_t* qempty = qfull + 4;         // [2] MMA commit
   uint64_t* sfull = qempty + 2;         // [2] MMA commit
-  uint64_t* sfree = sfull + 2;          // [2] 8 softmax warps
-  uint64_t* pfull = sfree + 2;          // 8 softmax warps
+  uint64_t* sfree = sfull + 2;          // [2] softmax warps
+  uint64_t* pfull = sfree + 2;          // softmax warps
   uint64_t* pvdone = pfull + 1;         // MMA commit
-  uint64_t* ofree = pvdone + 1;         // 8 softmax warps
+  uint64_t* ofree = pvdone + 1;         // softmax warps
   uint64_t* mend = ofree + 1;           // MMA commit
-  uint64_t* meet_bar = mend + 1;        // [2 halves] its 4 softmax warps
+  uint64_t* meet_bar = mend + 1;        // [shares] its 4 softmax warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
 
@@ -271,20 +291,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     for (int u = 0; u < 2; u++) {
       mbar_init(&qempty[u], 1);
       mbar_init(&sfull[u], 1);
-      mbar_init(&sfree[u], 8);
+      mbar_init(&sfree[u], kSoftWarps);
     }
-    mbar_init(pfull, 8);
+    mbar_init(pfull, kSoftWarps);
     mbar_init(pvdone, 1);
-    mbar_init(ofree, 8);
+    mbar_init(ofree, kSoftWarps);
     mbar_init(mend, 1);
-    mbar_init(&meet_bar[0], 4);
-    mbar_init(&meet_bar[1], 4);
+    for (int u = 0; u < kShares; u++) mbar_init(&meet_bar[u], 4);
     *abort_flag = 0;
     for (int u = 0; u < 8; u++) badv[u] = 0;
     for (int u = 0; u < 4; u++) pieces[u] = Walk{};  // (what a role reads that had to give up a wait)
     fence_mbar_init();
   }
-  if (warp == 12) {  // one CTA per SM (shared memory), so the allocation never waits
+  if (warp == kMmaWarp) {  // one CTA per SM (shared memory), so the allocation never waits
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(C::TMEM_COLS)
@@ -311,7 +330,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     __syncthreads();
   }
   const int n_stages = deal(p, table, cta, (int)gridDim.x, plan, at);
-  if (warp == 15) {
+  if (warp == kMmaWarp + 3) {
     // the tiles whose first pieces lie here and that others go on with: one that begins with this
     // CTA's stages, one at their end
     Walk w = at;
@@ -347,10 +366,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     return wait_or_abort(bar, parity & 1u, abort_flag, p.err, code);
   };
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= kLoadWarp && warp < kMmaWarp) {
     // ------------------------------------------------------------------------------ loads
     regs_down<C::REGS_LOAD>();
-    const int pw = warp - 8;
+    const int pw = warp - kLoadWarp;
     int issued = 0;  // units
     // A lane copies the 16-byte pieces k = lane % 8 of rows 32 pw + 4 it + lane / 8, it = 0..7; what it
     // needs of a stage's rows is looked up once and kept for all units of K and, later, of V.
@@ -461,13 +480,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       if (++w.j == w.j_end && i + 1 < n_stages) w.next_tile(p);
     }
     cp_wait_all();
-  } else if (warp >= 12) {
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------------------ MMAs
     regs_down<C::REGS_MMA>();
-    if (warp == 12) {
-      // The whole warp runs the loop and one elected lane issues: descriptors and column addresses are
-      // then uniform values the MMAs take as they are.  (From a loop that only lane 0 entered every
-      // MMA was issued 2.5 times slower than it ran: 128 against 54 cycles at N = 64.)
+    if (warp == kMmaWarp) {
+      // The whole warp runs the loop and one elected lane's MMAs are predicated on: the control flow is
+      // uniform, so descriptors stay in uniform registers.  With a loop that only lane 0 entered, or a
+      // branch around the MMAs, the other warps' work slowed their issue to 110-130 cycles each; so
+      // issued they run at 48 (N = 64), whatever the loads and the softmax do.
+      const uint32_t on = elect_one();
       constexpr uint32_t idesc_s = f16_idesc(N, false), idesc_o = f16_idesc(N, true, true);
       auto ready = [&](uint64_t* bar, uint32_t parity) { return warp_wait(bar, parity & 1u, abort_flag, p.err); };
       const uint64_t dp = sw128_desc(sbase + C::OFF_P, 16384, 1024);
@@ -496,19 +517,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             tc_fence_after();
             const uint64_t dk = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16, 1024);
             const uint64_t dqu = dq + (uint64_t)((u * 2 * N * 128) >> 4);
-            if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < 8; kk++)
-                umma_f16_ss(d, dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+            for (int kk = 0; kk < 8; kk++)
+              umma_if(on, d, dk + (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
                             dqu + (uint64_t)(((kk >> 2) * (N * 128) + (kk & 3) * 32) >> 4), idesc_s,
                             kk > 0 ? 1u : u > 0 ? 1u : 0u);
-              umma_commit(&empty[slot]);
-              if (u == MB - 1) {
-                umma_commit(&sfull[b]);
-                if (last) umma_commit(&qempty[tile_no % NQ]);
-              }
+            commit_if(on, &empty[slot]);
+            if (u == MB - 1) {
+              commit_if(on, &sfull[b]);
+              if (last) commit_if(on, &qempty[tile_no % NQ]);
             }
-            __syncwarp();
             if (++slot == UNITS) slot = 0, round++;
           }
           if (!ok) break;
@@ -526,15 +544,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             if (!ok) break;
             tc_fence_after();
             const uint64_t dv = sw128_desc(sbase + C::OFF_RING + slot * kUnit, 16384, 1024);
-            if (elect_one()) {
 #pragma unroll
-              for (int kk = 0; kk < 8; kk++)
-                umma_f16_ss(tmem + C::COL_O + (uint32_t)(u * N), dv + (uint64_t)((kk * 2048) >> 4),
+            for (int kk = 0; kk < 8; kk++)
+              umma_if(on, tmem + C::COL_O + (uint32_t)(u * N), dv + (uint64_t)((kk * 2048) >> 4),
                             dp + (uint64_t)((kk * 2048) >> 4), idesc_o, kk > 0 ? 1u : go_on);
-              umma_commit(&empty[slot]);
-              if (u == MB - 1) umma_commit(pvdone);
-            }
-            __syncwarp();
+            commit_if(on, &empty[slot]);
+            if (u == MB - 1) commit_if(on, pvdone);
             if (++slot == UNITS) slot = 0, round++;
           }
           if (!ok) break;
@@ -542,18 +557,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         first_prev = first;
       }
       // no MMA may still be running when TMEM is freed, also after an abort
-      if (elect_one()) umma_commit(mend);
-      __syncwarp();
+      commit_if(on, mend);
       (void)mbar_wait_bounded(mend, 0, p.err, G4A_DEVERR_WAIT_MMA);
     }
-    if (warp > 12) {
+    if (warp > kMmaWarp) {
       // ---------------------------------------------------------------------------- handing over
       // Takes the units in the order of their loads: waits until one has landed, makes the copies
       // (generic proxy) visible to the tensor core (async proxy), passes it on.  (The same fence
       // in the MMA thread held every unit up by several hundred cycles.)
       // V of keys that not every row sees: p = 0 times an infinite or NaN V would reach the rows
       // that do not.  Such values become 0 here, and the epilogue adds them to the rows that do.
-      const int hw = warp - 13;
+      const int hw = warp - kMmaWarp - 1;
       Walk w = {}, before = {};
       int unit = 0, tile_no = -1, tile_before = 0;
       auto pass = [&](uint64_t* from, uint64_t* to, uint32_t parity) {
@@ -602,20 +616,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     }
   } else {
     // ------------------------------------------------------------------------------ softmax
-    regs_up<C::REGS_SOFTMAX>();
-    const int quarter = warp & 3, half = warp >> 2;
+    regs_up<C::REGS_SOFT>();
+    const int quarter = warp & 3, share = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    float* su = reinterpret_cast<float*>(smem + C::OFF_U) + warp * RH;
-    float* sf = reinterpret_cast<float*>(smem + C::OFF_F) + warp * RH;
-    float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX) + half * 4 * RH;
-    int* votes = reinterpret_cast<int*>(smem + C::OFF_VOTE) + half * 8;
-    // The half's four warps meet (a bounded wait like every other); what they wrote before is visible
+    float* su = reinterpret_cast<float*>(smem + C::OFF_U) + warp * W;
+    float* sf = reinterpret_cast<float*>(smem + C::OFF_F) + warp * W;
+    float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX) + share * 4 * W;
+    int* votes = reinterpret_cast<int*>(smem + C::OFF_VOTE) + share * 8;
+    // The share's four warps meet (a bounded wait like every other); what they wrote before is visible
     // after.  `votes` alternates between two sets, so that nobody writes what another still reads.
     uint32_t met = 0;
     auto meet = [&]() {
       __syncwarp();
-      if (lane == 0) mbar_arrive(&meet_bar[half]);
-      (void)warp_wait(&meet_bar[half], met & 1u, abort_flag, p.err);
+      if (lane == 0) mbar_arrive(&meet_bar[share]);
+      (void)warp_wait(&meet_bar[share], met & 1u, abort_flag, p.err);
       met++;
     };
     auto any_of = [&](bool pred) {
@@ -627,20 +641,18 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       return (all.x | all.y | all.z | all.w) != 0;
     };
     const int key_in = quarter * 32 + lane;  // this thread's key of a stage
+    const int n_of = lane % W;               // the row whose maximum and sum this lane keeps
     unsigned char* prow = smem + C::OFF_P + key_in * 128;
     Walk w = {};
     int tile_no = -1, j_first = 0;
-    float m[G];     // lane n: running maximum of row g * W + n of this half
-    float l[G][W];  // this thread's keys' share of the row sums
+    float m;     // running maximum of row n_of of the share
+    float l[W];  // this thread's keys' part of the row sums
     auto reset = [&]() {
+      m = -INFINITY;
 #pragma unroll
-      for (int g = 0; g < G; g++) {
-        m[g] = -INFINITY;
-#pragma unroll
-        for (int n = 0; n < W; n++) l[g][n] = 0.f;
-      }
+      for (int n = 0; n < W; n++) l[n] = 0.f;
       __syncwarp();
-      for (int n = lane; n < RH; n += 32) su[n] = kUnseen;
+      if (lane < W) su[lane] = kUnseen;
       __syncwarp();
     };
     reset();
@@ -656,141 +668,127 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       }
       const bool last = i + 1 == n_stages || w.j + 1 == w.j_end;
       const int kvh = w.kvh, tile = w.tile;
-      const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - half * RH;  // rows of this half
+      const int live = min(ROWS, w.s.T * p.group - tile * ROWS) - share * W;  // rows of this share
       if (live > 0) {
         const int key0 = w.key0(), key = key0 + key_in;
         const uint4 ok4 = *reinterpret_cast<const uint4*>(okw + (i & 7) * 4);
         const bool clean = w.clean(p) && (ok4.x & ok4.y & ok4.z & ok4.w) == ~0u;
-        const uint32_t okq = quarter == 0 ? ok4.x : quarter == 1 ? ok4.y : quarter == 2 ? ok4.z : ok4.w;
-        const bool there = (okq >> lane) & 1u;
-        const Sees* see = sees + (tile_no & 3) * ROWS + half * RH;
-        const float* sc = scales + (tile_no & 3) * ROWS + half * RH;
+        // ---- scores in powers of two
+        float x[W];
+        {
+          uint32_t r[W];
+          const uint32_t col = lanes + C::COL_S + (uint32_t)(b * N + share * W);
+          if constexpr (F32) {
+            const float* sc = scales + (tile_no & 3) * ROWS + share * W;
+            uint32_t r2[W];
+            tmem_get(col, r);
+            tmem_get(col + ROWS, r2);
+            tmem_wait_ld();
+            tmem_landed(r);
+            tmem_landed(r2);
+#pragma unroll
+            for (int n = 0; n < W; n += 4) {
+              const float4 c4 = *reinterpret_cast<const float4*>(sc + n);
+              const float cs[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                x[n + e] = (__uint_as_float(r[n + e]) + __uint_as_float(r2[n + e])) * cs[e];
+            }
+          } else {
+            tmem_load(col, r);
+#pragma unroll
+            for (int n = 0; n < W; n++) x[n] = __uint_as_float(r[n]) * p.scale_log2;
+          }
+        }
+        if (!clean) {
+          const uint32_t okq = quarter == 0 ? ok4.x : quarter == 1 ? ok4.y : quarter == 2 ? ok4.z : ok4.w;
+          const bool there = (okq >> lane) & 1u;
+          const Sees* see = sees + (tile_no & 3) * ROWS + share * W;
+#pragma unroll
+          for (int n = 0; n < W; n++) {
+            const Sees v = see[n];
+            const bool in = key < w.s.base ? key >= v.kmin : ((v.bits >> (key - w.s.base)) & 1) != 0;
+            if (!there || !in) x[n] = -INFINITY;
+          }
+        }
+        // every score of this buffer is in registers
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sfree[b]);
+        // ---- does a score pass its row's maximum by 2^8?
+        float far = -INFINITY;
+        const float4* u4 = reinterpret_cast<const float4*>(su);  // m - 7 of the rows
+#pragma unroll
+        for (int n = 0; n < W; n += 4) {
+          const float4 u = u4[n / 4];
+          far = fmaxf(far, fmaxf(fmaxf(x[n] - u.x, x[n + 1] - u.y), fmaxf(x[n + 2] - u.z, x[n + 3] - u.w)));
+        }
         bool pv_waited = i == 0;
-#pragma unroll
-        for (int g = 0; g < G; g++) {
-          // ---- scores in powers of two
-          float x[W];
-          {
-            uint32_t r[W];
-            const uint32_t col = lanes + C::COL_S + (uint32_t)(b * N + half * RH + g * W);
-            if constexpr (F32) {
-              uint32_t r2[W];
-              tmem_get(col, r);
-              tmem_get(col + ROWS, r2);
-              tmem_wait_ld();
-              tmem_landed(r);
-              tmem_landed(r2);
-#pragma unroll
-              for (int n = 0; n < W; n += 4) {
-                const float4 c4 = *reinterpret_cast<const float4*>(sc + g * W + n);
-                const float cs[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                  x[n + e] = (__uint_as_float(r[n + e]) + __uint_as_float(r2[n + e])) * cs[e];
-              }
-            } else {
-              tmem_load(col, r);
-#pragma unroll
-              for (int n = 0; n < W; n++) x[n] = __uint_as_float(r[n]) * p.scale_log2;
-            }
+        if (first || any_of(far > kPUp + kRaise)) {
+          const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
+          if (lane < W) smax[quarter * W + lane] = mine;
+          meet();
+          const float mx = fmaxf(fmaxf(smax[n_of], smax[W + n_of]), fmaxf(smax[2 * W + n_of], smax[3 * W + n_of]));
+          const bool raise = mx > m + kRaise;
+          const float f = !raise ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - mx);
+          if (raise) m = mx;
+          if (lane < W) {
+            su[lane] = m == -INFINITY ? kUnseen : m - kPUp;
+            sf[lane] = f;
           }
-          if (!clean) {
-            if (!there) {
+          __syncwarp();
 #pragma unroll
-              for (int n = 0; n < W; n++) x[n] = -INFINITY;
-            } else {
-#pragma unroll
-              for (int n = 0; n < W; n++) {
-                const Sees v = see[g * W + n];
-                const bool in = key < w.s.base ? key >= v.kmin : ((v.bits >> (key - w.s.base)) & 1) != 0;
-                if (!in) x[n] = -INFINITY;
-              }
-            }
-          }
-          if (g == G - 1) {  // every score of this buffer is in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sfree[b]);
-          }
-          // ---- does a score pass its row's maximum by 2^8?
-          float far = -INFINITY;
-          const float4* u4 = reinterpret_cast<const float4*>(su + g * W);  // m - 7 of the rows
-#pragma unroll
-          for (int n = 0; n < W; n += 4) {
-            const float4 u = u4[n / 4];
-            far = fmaxf(far, fmaxf(fmaxf(x[n] - u.x, x[n + 1] - u.y), fmaxf(x[n + 2] - u.z, x[n + 3] - u.w)));
-          }
-          if (first || any_of(far > kPUp + kRaise)) {
-            const float mine = transpose_reduce<W>(x, [](float a, float c) { return fmaxf(a, c); });
-            if (lane < W) smax[quarter * RH + g * W + lane] = mine;
-            meet();
-            const int n_of = g * W + (lane % W);
-            const float mx = fmaxf(fmaxf(smax[n_of], smax[RH + n_of]), fmaxf(smax[2 * RH + n_of], smax[3 * RH + n_of]));
-            const bool raise = mx > m[g] + kRaise;
-            const float f = !raise ? 1.f : m[g] == -INFINITY ? 0.f : fast_exp2(m[g] - mx);
-            if (raise) m[g] = mx;
-            if (lane < W) {
-              su[n_of] = m[g] == -INFINITY ? kUnseen : m[g] - kPUp;
-              sf[n_of] = f;
-            }
-            __syncwarp();
-#pragma unroll
-            for (int n = 0; n < W; n++) l[g][n] *= sf[g * W + n];
-            if (__any_sync(0xffffffffu, f != 1.f) && !first) {  // the same in the half's four warps
-              if (!pv_waited) {
-                (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
-                pv_waited = true;
-              }
-              tc_fence_after();
-#pragma unroll 1
-              for (int k = 0; k < MB * (F32 ? 2 : 1); k++) {  // M blocks (x terms)
-                const uint32_t col = lanes + C::COL_O + (uint32_t)((k % MB) * N + (k / MB) * ROWS + half * RH + g * W);
-                uint32_t r[W];
-                tmem_load(col, r);
-#pragma unroll
-                for (int n = 0; n < W; n++) r[n] = __float_as_uint(__uint_as_float(r[n]) * sf[g * W + n]);
-                tmem_store(col, r);
-              }
-              tmem_wait_st();
-            }
-          }
-          // ---- p = 2^(s - m + 7)
-          uint32_t hi[W / 2], lo[F32 ? W / 2 : 1];
-#pragma unroll
-          for (int n = 0; n < W; n += 4) {
-            const float4 u = u4[n / 4];
-            const float p0 = fast_exp2(x[n] - u.x), p1 = fast_exp2(x[n + 1] - u.y);
-            const float p2 = fast_exp2(x[n + 2] - u.z), p3 = fast_exp2(x[n + 3] - u.w);
-            l[g][n] += p0;
-            l[g][n + 1] += p1;
-            l[g][n + 2] += p2;
-            l[g][n + 3] += p3;
-            hi[n / 2] = pack2(p0, p1);
-            hi[n / 2 + 1] = pack2(p2, p3);
-            if constexpr (F32) {
-              const float2 h0 = h2_to_f2(hi[n / 2]), h1 = h2_to_f2(hi[n / 2 + 1]);
-              lo[n / 2] = pack2(p0 - h0.x, p1 - h0.y);
-              lo[n / 2 + 1] = pack2(p2 - h1.x, p3 - h1.y);
-            }
-          }
-          if (!pv_waited) {  // the previous stage's product has read P
+          for (int n = 0; n < W; n++) l[n] *= sf[n];
+          if (!first && __any_sync(0xffffffffu, f != 1.f)) {  // the same in the share's four warps
             (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
             pv_waited = true;
-          }
+            tc_fence_after();
+#pragma unroll 1
+            for (int k = 0; k < MB * (F32 ? 2 : 1); k++) {  // M blocks (x terms)
+              const uint32_t col = lanes + C::COL_O + (uint32_t)((k % MB) * N + (k / MB) * ROWS + share * W);
+              uint32_t r[W];
+              tmem_load(col, r);
 #pragma unroll
-          for (int term = 0; term < (F32 ? 2 : 1); term++) {
-            const int n0 = term * ROWS + half * RH + g * W;  // first column of this thread's run
-#pragma unroll
-            for (int k = 0; k < W / 8; k++) {
-              const int piece = n0 / 8 + k;
-              const uint32_t* v = (term ? lo : hi) + 4 * k;
-              *reinterpret_cast<uint4*>(prow + (piece >> 3) * 16384 + (((piece & 7) ^ (key_in & 7)) << 4)) =
-                  make_uint4(v[0], v[1], v[2], v[3]);
+              for (int n = 0; n < W; n++) r[n] = __float_as_uint(__uint_as_float(r[n]) * sf[n]);
+              tmem_store(col, r);
             }
+            tmem_wait_st();
+          }
+        }
+        // ---- p = 2^(s - m + 7)
+        uint32_t hi[W / 2], lo[F32 ? W / 2 : 1];
+#pragma unroll
+        for (int n = 0; n < W; n += 4) {
+          const float4 u = u4[n / 4];
+          const float p0 = fast_exp2(x[n] - u.x), p1 = fast_exp2(x[n + 1] - u.y);
+          const float p2 = fast_exp2(x[n + 2] - u.z), p3 = fast_exp2(x[n + 3] - u.w);
+          l[n] += p0;
+          l[n + 1] += p1;
+          l[n + 2] += p2;
+          l[n + 3] += p3;
+          hi[n / 2] = pack2(p0, p1);
+          hi[n / 2 + 1] = pack2(p2, p3);
+          if constexpr (F32) {
+            const float2 h0 = h2_to_f2(hi[n / 2]), h1 = h2_to_f2(hi[n / 2 + 1]);
+            lo[n / 2] = pack2(p0 - h0.x, p1 - h0.y);
+            lo[n / 2 + 1] = pack2(p2 - h1.x, p3 - h1.y);
+          }
+        }
+        // the previous stage's product has read P
+        if (!pv_waited) (void)warp_wait(pvdone, (uint32_t)(i - 1) & 1u, abort_flag, p.err);
+#pragma unroll
+        for (int term = 0; term < (F32 ? 2 : 1); term++) {
+          const int n0 = term * ROWS + share * W;  // first column of this thread's run
+#pragma unroll
+          for (int k = 0; k < W / 8; k++) {
+            const int piece = n0 / 8 + k;
+            const uint32_t* v = (term ? lo : hi) + 4 * k;
+            *reinterpret_cast<uint4*>(prow + (piece >> 3) * 16384 + (((piece & 7) ^ (key_in & 7)) << 4)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
       } else {
-        // no rows of the tile in this half: its columns' P is never looked at
+        // no rows of the tile in this share: its columns' P is never looked at
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sfree[b]);
@@ -803,62 +801,60 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
 
       if (last) {
         // ---- row sums, then O / l (or the part of a tile that other CTAs share)
+        const bool whole = w.chunks == 1 && j_first == 0 && w.j + 1 == w.s.stages;
+        const bool later = i - (w.j - j_first) > 0;  // not the piece this CTA's stages begin with
+        float* part = p.part + ((size_t)2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
+        if (live > 0) {
+          meet();  // smax is free
+          const float mine = transpose_reduce<W>(l, [](float a, float c) { return a + c; });
+          if (lane < W) smax[quarter * W + lane] = mine;
+          meet();
+          const float lt = (smax[n_of] + smax[W + n_of]) + (smax[2 * W + n_of] + smax[3 * W + n_of]);
+          if (lane < W) sf[lane] = !whole ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
+          if (!whole && quarter == 0 && lane < W) {
+            part[(size_t)ROWS * HD + share * W + lane] = m;
+            part[(size_t)ROWS * HD + ROWS + share * W + lane] = lt;
+          }
+          __syncwarp();
+        }
         (void)warp_wait(pvdone, (uint32_t)i & 1u, abort_flag, p.err);
         tc_fence_after();
         if (live > 0) {
-          const bool whole = w.chunks == 1 && j_first == 0 && w.j + 1 == w.s.stages;
-          const bool later = i - (w.j - j_first) > 0;  // not the piece this CTA's run begins with
-          float* part = p.part + ((size_t)2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
-          float lt[G];
-          meet();  // smax is free
-#pragma unroll
-          for (int g = 0; g < G; g++) {
-            const float mine = transpose_reduce<W>(l[g], [](float a, float c) { return a + c; });
-            if (lane < W) smax[quarter * RH + g * W + lane] = mine;
-          }
-          meet();
-#pragma unroll
-          for (int g = 0; g < G; g++) {
-            const int n_of = g * W + (lane % W);
-            lt[g] = (smax[n_of] + smax[RH + n_of]) + (smax[2 * RH + n_of] + smax[3 * RH + n_of]);
-            if (lane < W) sf[n_of] = !whole ? 1.f : lt[g] == 0.f ? 0.f : 1.f / lt[g];
-            if (!whole && quarter == 0 && lane < W) {
-              part[(size_t)ROWS * HD + half * RH + n_of] = m[g];
-              part[(size_t)ROWS * HD + ROWS + half * RH + n_of] = lt[g];
-            }
-          }
-          __syncwarp();
           const bool bad = badv[(tile_no + 1) & 7] == ((tile_no + 1) & 0xffff);
+          const int nl = min(W, live);
+          long long row = 0;  // lane n: where row n of the share lies in the output
+          if (lane < nl) {
+            const int gr = tile * ROWS + share * W + lane, t = gr / p.group;
+            row = ((long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
+          }
 #pragma unroll 1
-          for (int k = 0; k < MB * G; k++) {
-            const int mb = k / G, g = k % G;
+          for (int mb = 0; mb < MB; mb++) {
             const int d = mb * 128 + key_in;
-            const uint32_t col = lanes + C::COL_O + (uint32_t)(mb * N + half * RH + g * W);
+            const uint32_t col = lanes + C::COL_O + (uint32_t)(mb * N + share * W);
             float o[W];
             {
               uint32_t r[W];
-              tmem_load(col, r);
-#pragma unroll
-              for (int n = 0; n < W; n++) o[n] = __uint_as_float(r[n]);
               if constexpr (F32) {
-                tmem_load(col + ROWS, r);
+                uint32_t r2[W];
+                tmem_get(col, r);
+                tmem_get(col + ROWS, r2);
+                tmem_wait_ld();
+                tmem_landed(r);
+                tmem_landed(r2);
 #pragma unroll
-                for (int n = 0; n < W; n++) o[n] += __uint_as_float(r[n]);
+                for (int n = 0; n < W; n++) o[n] = __uint_as_float(r[n]) + __uint_as_float(r2[n]);
+              } else {
+                tmem_load(col, r);
+#pragma unroll
+                for (int n = 0; n < W; n++) o[n] = __uint_as_float(r[n]);
               }
             }
-            const int nl = min(W, live - g * W);
             if (whole) {
-              const int gr0 = tile * ROWS + half * RH + g * W;
-              long long row = 0;
-              if (lane < nl) {
-                const int gr = gr0 + lane, t = gr / p.group;
-                row = ((long long)(w.s.row0 + t) * p.nqh + kvh * p.group + (gr - t * p.group)) * p.hd;
-              }
 #pragma unroll
               for (int n = 0; n < W; n++) {
                 const long long a = __shfl_sync(0xffffffffu, row, n);
                 if (n < nl && d < p.hd) {
-                  const float y = o[n] * sf[g * W + n];
+                  const float y = o[n] * sf[n];
                   if constexpr (F32) reinterpret_cast<float*>(p.out)[a + d] = y;
                   else reinterpret_cast<__half*>(p.out)[a + d] = __float2half_rn(y);
                 }
@@ -866,12 +862,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             } else {
 #pragma unroll
               for (int n = 0; n < W; n++)
-                if (n < nl) part[(size_t)(half * RH + g * W + n) * HD + d] = o[n];
+                if (n < nl) part[(size_t)(share * W + n) * HD + d] = o[n];
             }
             if (bad && d < p.hd)
               add_non_finite<F32>(p, w.s, w.b, kvh, w.s.lo + j_first * kKeysT, min(w.key0() + kKeysT, w.s.L), w.kfull(p),
-                                  d, tile * ROWS + half * RH + g * W, nl,
-                                  whole ? nullptr : part + (size_t)(half * RH + g * W) * HD, HD);
+                                  d, tile * ROWS + share * W, nl, whole ? nullptr : part + (size_t)share * W * HD, HD);
           }
         }
         tc_fence_before();
@@ -886,7 +881,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 12)
+  if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS));
 }
 
