@@ -31,10 +31,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // Joins the parts of the tiles that were cut between CTAs.  The work is cut into units spread over all
-// CTAs.  A thread is a float4 column of a row and a lane over its parts: 32 columns x 8 where a tile
-// has few parts (lanes over the parts, or over 2 or 4 rows), 8 columns x 32 where it has many (one long
-// context: a part in every CTA; 148 parts one after another by eight lanes took 9 us).  A lane folds
-// its parts four at a time with a running maximum; the lanes of a row meet in shared memory.
+// CTAs.  A thread is a float4 column of a row and a lane over its parts, which it loads four at a time and
+// folds with a running maximum; the lanes of a row, if there are several, meet in shared memory.  What
+// bounds it is the latency of a unit, cut -> parts -> output, 1 to 2 us cold, not the 5 to 20 MB of parts,
+// which lie in the L2: so as many rows to a unit as there are threads for (six parts of 24 tiles with eight
+// lanes to a row: five units for each CTA one after another, 16 us; with two lanes 7), and many lanes only
+// where there are many parts (148 parts of one long context with eight lanes: 9 us, with 32: 4.5).
 constexpr int kMergeThreads = 256;
 constexpr int kMergeFly = 4;   // parts of a lane in flight
 constexpr int kMaxCuts = 512;  // two for each CTA of the attention kernel
@@ -49,7 +51,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
   pdl_wait_primary();
   pdl_launch_dependents();
   auto columns_of = [](int parts) { return parts > 32 ? 8 : 32; };
-  auto lanes_of = [](int parts) { return parts > 32 ? 32 : parts > 4 ? 8 : parts > 2 ? 4 : 2; };  // over parts
+  auto lanes_of = [](int parts) { return parts > 32 ? 32 : parts > 8 ? 8 : parts > 4 ? 2 : 1; };  // over parts
   auto rows_of = [&](int parts) { return kMergeThreads / columns_of(parts) / lanes_of(parts); };  // of a unit
   auto blocks_of = [&](int parts) { return p.hd_pad / 4 / columns_of(parts); };                   // units of a row
   {
@@ -131,22 +133,27 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
         }
       }
     }
-    if (col == 0) sm[sub][0] = m, sm[sub][1] = l;
-    so[tid] = o;
-    __syncthreads();
+    if (pl > 1) {  // (the same for the whole unit)
+      if (col == 0) sm[sub][0] = m, sm[sub][1] = l;
+      so[tid] = o;
+      __syncthreads();
+    }
     if (part0 == 0 && r < cut.rows && d < p.hd) {
-      float mx = m;
-      for (int i = 1; i < pl; i++) mx = fmaxf(mx, sm[sub + i][0]);
-      float lt = 0.f;
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < pl; i++) {
-        const float w = sm[sub + i][0] == mx ? 1.f : fast_exp2(sm[sub + i][0] - mx);
-        const float4 x = so[tid + i * cols];
-        lt += w * sm[sub + i][1];
-        o.x += w * x.x;
-        o.y += w * x.y;
-        o.z += w * x.z;
-        o.w += w * x.w;
+      float lt = l;
+      if (pl > 1) {
+        float mx = m;
+        for (int i = 1; i < pl; i++) mx = fmaxf(mx, sm[sub + i][0]);
+        lt = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < pl; i++) {
+          const float w = sm[sub + i][0] == mx ? 1.f : fast_exp2(sm[sub + i][0] - mx);
+          const float4 x = so[tid + i * cols];
+          lt += w * sm[sub + i][1];
+          o.x += w * x.x;
+          o.y += w * x.y;
+          o.z += w * x.z;
+          o.w += w * x.w;
+        }
       }
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
       const int gr = cut.first + r, t = gr / p.group;
@@ -158,7 +165,7 @@ __global__ void __launch_bounds__(kMergeThreads) tree_merge_kernel(const TreePar
         *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(p.out) + a) =
             make_uint2(pack2(o.x * inv, o.y * inv), pack2(o.z * inv, o.w * inv));
     }
-    __syncthreads();
+    if (pl > 1) __syncthreads();
   }
 }
 

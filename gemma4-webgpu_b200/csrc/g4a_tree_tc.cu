@@ -970,13 +970,19 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
 
 }  // namespace
 
+// Tile widths.  f16 queries and head_dim above 256 have 64 columns.  f32 queries up to 256 dims: 64
+// columns (32 rows) where that makes at most two stages for each SM, since a CTA's softmax and epilogue
+// are then half as long (24 tokens x 8 heads of 256 dims: 1,024 keys 16.9 us against 20.1 with 128 columns,
+// 6,000 keys 20.7 / 28.7), and 128 beyond, which read and load each key for twice the rows (8 tokens over
+// 32k keys, 3.5 stages: both 27; 64 tokens over 32k: 85 / 71).
 g4a_status g4a_tree_tc_launch(g4a_ctx* ctx, g4a_tree::TreeParams& p, bool f32, long long keys) {
-  const int rows = p.max_tokens * p.group;
+  const long long rows = (long long)p.max_tokens * p.group;
+  const bool narrow = rows <= 32 || (keys / kKeysT + p.batch) * ((rows + 31) / 32) * p.nkh <= 2 * ctx->num_sms;
   if (p.hd > 256) return f32 ? launch_tc<512, 64, true>(ctx, p, keys, rows) : launch_tc<512, 64, false>(ctx, p, keys, rows);
   if (p.hd > 128) {
-    if (f32) return rows <= 32 ? launch_tc<256, 64, true>(ctx, p, keys, rows) : launch_tc<256, 128, true>(ctx, p, keys, rows);
+    if (f32) return narrow ? launch_tc<256, 64, true>(ctx, p, keys, rows) : launch_tc<256, 128, true>(ctx, p, keys, rows);
     return launch_tc<256, 64, false>(ctx, p, keys, rows);
   }
-  if (f32) return rows <= 32 ? launch_tc<128, 64, true>(ctx, p, keys, rows) : launch_tc<128, 128, true>(ctx, p, keys, rows);
+  if (f32) return narrow ? launch_tc<128, 64, true>(ctx, p, keys, rows) : launch_tc<128, 128, true>(ctx, p, keys, rows);
   return launch_tc<128, 64, false>(ctx, p, keys, rows);
 }
