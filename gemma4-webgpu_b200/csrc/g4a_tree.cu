@@ -35,8 +35,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // folds with a running maximum; the lanes of a row, if there are several, meet in shared memory.  What
 // bounds it is the latency of a unit, cut -> parts -> output, 1 to 2 us cold, not the 5 to 20 MB of parts,
 // which lie in the L2: so as many rows to a unit as there are threads for (six parts of 24 tiles with eight
-// lanes to a row: five units for each CTA one after another, 16 us; with two lanes 7), and many lanes only
-// where there are many parts (148 parts of one long context with eight lanes: 9 us, with 32: 4.5).
+// lanes to a row: five units for each CTA one after another, 18 us; with two lanes 8.5), and many lanes only
+// where there are many parts (148 parts of one long context with eight lanes: 9 us, with 32: 5).
 constexpr int kMergeThreads = 256;
 constexpr int kMergeFly = 4;   // parts of a lane in flight
 constexpr int kMaxCuts = 512;  // two for each CTA of the attention kernel

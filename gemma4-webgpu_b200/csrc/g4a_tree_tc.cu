@@ -55,10 +55,10 @@ constexpr float kPUp = 7.0f;         // p = 2^(s - m + 7)
 constexpr float kRaise = 8.0f;       // a score this far above m raises it
 constexpr float kUnseen = -1e30f;    // m of a row that has seen nothing yet (any score raises it)
 
-template <int HD, int N, bool F32>
+template <int HD, int N, bool F32, int R>
 struct Tc {
   static constexpr int MB = HD / 128;                 // 128-dim blocks = ring units of a K or V tile
-  static constexpr int ROWS = F32 ? N / 2 : N;        // query rows of a tile
+  static constexpr int ROWS = R;                      // query rows of a tile
   static constexpr int W = ROWS / kShares;            // rows of a softmax warp (its share)
   // Registers: 512 threads start with 128 each (65,536); the softmax warps, which hold a block of
   // scores and the row sums, take some from the others.  (Spills are dear here: shared memory leaves
@@ -245,9 +245,9 @@ __device__ __noinline__ void add_non_finite(const TreeParams& p, Seq s, int b, i
   }
 }
 
-template <int HD, int N, bool F32>
+template <int HD, int N, bool F32, int R>
 __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_constant__ TreeParams p) {
-  using C = Tc<HD, N, F32>;
+  using C = Tc<HD, N, F32, R>;
   constexpr int MB = C::MB, ROWS = C::ROWS, W = C::W, UNITS = C::UNITS, NQ = C::NQ;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
@@ -925,18 +925,19 @@ __global__ void __launch_bounds__(256) tree_split_kernel(const float* q, __half*
   }
 }
 
-template <int HD, int N, bool F32>
+template <int HD, int N, bool F32, int R>
 g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long tokens_rows) {
-  using C = Tc<HD, N, F32>;
+  using C = Tc<HD, N, F32, R>;
   static std::atomic<bool> done[64];
   if (ctx->device >= 64 || !done[ctx->device].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<HD, N, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    const cudaError_t e = cudaFuncSetAttribute(tree_tc_kernel<HD, N, F32, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                (int)C::SMEM);
     if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(tree_tc_kernel)");
     if (ctx->device < 64) done[ctx->device].store(true, std::memory_order_release);
   }
   p.rows_log2 = C::ROWS == 64 ? 6 : 5;
   static_assert(C::ROWS == 64 || C::ROWS == 32, "tile rows");
+  static_assert(C::ROWS * (F32 ? 2 : 1) <= N, "columns");
   p.hd_pad = HD;
   const long long tiles = (tokens_rows + C::ROWS - 1) / C::ROWS;
   const long long stages = (keys / kKeysT + p.batch) * tiles * p.nkh;
@@ -963,26 +964,33 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
     if (e != cudaSuccess) return g4a_cuda_fail(e, "launch tree_split_kernel");
   }
   const cudaError_t e =
-      g4a_launch(tree_tc_kernel<HD, N, F32>, dim3(p.grid), dim3(kThreadsTc), C::SMEM, ctx->stream, true, p);
+      g4a_launch(tree_tc_kernel<HD, N, F32, R>, dim3(p.grid), dim3(kThreadsTc), C::SMEM, ctx->stream, true, p);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch tree_tc_kernel");
   return G4A_OK;
 }
 
 }  // namespace
 
-// Tile widths.  f16 queries and head_dim above 256 have 64 columns.  f32 queries up to 256 dims: 64
-// columns (32 rows) where that makes at most two stages for each SM, since a CTA's softmax and epilogue
-// are then half as long (24 tokens x 8 heads of 256 dims: 1,024 keys 16.9 us against 20.1 with 128 columns,
-// 6,000 keys 20.7 / 28.7), and 128 beyond, which read and load each key for twice the rows (8 tokens over
-// 32k keys, 3.5 stages: both 27; 64 tokens over 32k: 85 / 71).
+// Tile heights.  32 rows (64 columns; f16 queries leave half of them idle) where a sequence has no more or
+// where that makes at most two stages for each SM: a softmax warp then has 16 rows instead of 32, and a
+// CTA's softmax and epilogue are half as long.  64 rows beyond (f32 queries of up to 256 dims: 128 columns),
+// which read and load each key for twice the rows.  Both sides measured, 32 / 64 rows: f32, 24 tokens x 8
+// heads of 256 dims, 1,024 keys 16.9 / 20.1 us, 6,000 keys 20.7 / 28.7; 8 tokens over 32k keys (3.5 stages) 27
+// / 27; 64 tokens over 32k 85 / 71.  f16, 7 tokens x 3 heads, 32 sequences 44 / 56; 24 tokens x 8 heads, 3,000
+// keys 16.4 / 18.0.  (A head of more than 256 dims has room for 64 columns only, so f32 has 32 rows.)
 g4a_status g4a_tree_tc_launch(g4a_ctx* ctx, g4a_tree::TreeParams& p, bool f32, long long keys) {
   const long long rows = (long long)p.max_tokens * p.group;
   const bool narrow = rows <= 32 || (keys / kKeysT + p.batch) * ((rows + 31) / 32) * p.nkh <= 2 * ctx->num_sms;
-  if (p.hd > 256) return f32 ? launch_tc<512, 64, true>(ctx, p, keys, rows) : launch_tc<512, 64, false>(ctx, p, keys, rows);
-  if (p.hd > 128) {
-    if (f32) return narrow ? launch_tc<256, 64, true>(ctx, p, keys, rows) : launch_tc<256, 128, true>(ctx, p, keys, rows);
-    return launch_tc<256, 64, false>(ctx, p, keys, rows);
+  if (p.hd > 256) {
+    if (f32) return launch_tc<512, 64, true, 32>(ctx, p, keys, rows);
+    return narrow ? launch_tc<512, 64, false, 32>(ctx, p, keys, rows) : launch_tc<512, 64, false, 64>(ctx, p, keys, rows);
   }
-  if (f32) return narrow ? launch_tc<128, 64, true>(ctx, p, keys, rows) : launch_tc<128, 128, true>(ctx, p, keys, rows);
-  return launch_tc<128, 64, false>(ctx, p, keys, rows);
+  if (p.hd > 128) {
+    if (f32)
+      return narrow ? launch_tc<256, 64, true, 32>(ctx, p, keys, rows) : launch_tc<256, 128, true, 64>(ctx, p, keys, rows);
+    return narrow ? launch_tc<256, 64, false, 32>(ctx, p, keys, rows) : launch_tc<256, 64, false, 64>(ctx, p, keys, rows);
+  }
+  if (f32)
+    return narrow ? launch_tc<128, 64, true, 32>(ctx, p, keys, rows) : launch_tc<128, 128, true, 64>(ctx, p, keys, rows);
+  return narrow ? launch_tc<128, 64, false, 32>(ctx, p, keys, rows) : launch_tc<128, 64, false, 64>(ctx, p, keys, rows);
 }
