@@ -283,6 +283,43 @@ def test_tree_attn_long_cache_split_over_all_sms(ctx):
     _check_tree(out, case, q, words)
 
 
+@pytest.mark.parametrize("hd,nqh,nkh,fmt,T,n", [(256, 8, 1, torch.float32, 48, 9001), (512, 8, 1, torch.float16, 40, 6007),
+                                                (128, 12, 4, torch.float32, 64, 5000), (256, 8, 1, torch.float16, 64, 4100),
+                                                (512, 4, 1, torch.float32, 20, 3001)])
+def test_tree_attn_several_tiles_over_a_long_cache(ctx, hd, nqh, nkh, fmt, T, n):
+    """Every tile's keys are cut into several pieces, and the pieces of several tiles are joined."""
+    case = Paged(n, [n], [T], nkh=nkh, hd=hd, page=64)
+    words = tree_masks([T], random.Random(n))
+    q = (torch.randn((T, nqh, hd), generator=torch.Generator().manual_seed(n)) * 2).to(fmt).cuda()
+    for window in (0, n // 2):
+        out = _run_tree(ctx, case, q, words, window=window)
+        ctx.sync()
+        _check_tree(out, case, q, words, window=window)
+
+
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("batch,longest,nkh,group,most", [
+    (60, 900, 4, 2, 8),   # more tiles than SMs: tiles cut at any stage, two pieces to a CTA
+    (9, 6000, 2, 8, 24),  # short sequences beside one that is far longer than the rest
+    (33, 500, 1, 8, 5),   # just past 32 sequences
+    (600, 90, 1, 4, 3),   # more sequences than the table in shared memory holds
+])
+def test_tree_attn_partitions(ctx, fmt, batch, longest, nkh, group, most):
+    rnd = random.Random(batch)
+    counts = [rnd.randint(0, most) for _ in range(batch)]
+    counts[0], counts[-1] = most, max(counts[-1], 1)
+    lens = [c + (rnd.randint(0, longest) if batch != 9 or b == 4 else rnd.randint(0, 60)) for b, c in enumerate(counts)]
+    lens[batch // 2] = longest
+    case = Paged(batch, lens, counts, nkh=nkh, hd=64, page=16)
+    words = tree_masks(counts, rnd)
+    g = torch.Generator().manual_seed(batch)
+    q = (torch.randn((sum(counts) + 1, nkh * group, 64), generator=g) * 2).to(fmt).cuda()
+    for host, window in ((True, 0), (False, 0), (True, 200)):
+        out = _run_tree(ctx, case, q, words, window=window, host=host, extra=1)
+        ctx.sync()
+        _check_tree(out, case, q, words, window=window)
+
+
 @pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
 def test_tree_attn_empty_masks_give_zeros(ctx, fmt):
     """A word without bits sees the prefix alone; without a prefix it sees nothing and gives zeros."""
