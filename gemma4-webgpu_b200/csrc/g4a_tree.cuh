@@ -96,11 +96,13 @@ __device__ __forceinline__ int chunk_at(int n, int chunks, int c) {
 //    each row 90 MB apart and the L2 had lost it: 321 us instead of 221.)  A piece's start and end
 //    cost as much as two to four stages, so one longer piece beats two (64 tokens over 32k keys: 78
 //    -> 64 us) unless the longest is more than a quarter (and a stage) above the mean.
-//  - Else the list of all stages (sequence, kv head, tile, stage) is cut into equal runs.  A run holds
-//    whole tiles, and at most two pieces: one at its begin, one at its end.
+//  - Else the list of all stages (sequence, kv head, tile, stage) is cut into equal runs, where a tile
+//    counts `lead` stages more than it has, in front: its queries, join and epilogue.  A run holds whole
+//    tiles, and at most two pieces: one at its begin, one at its end.
 struct Plan {
-  int run;
+  int run, lead;
   long long active, each, extra;
+  long long origin;  // where the tile begins in which this CTA's run begins, in the list with the leads
   __device__ __forceinline__ long long begin(long long c) const { return c * each + (c < extra ? c : extra); }
   // the CTA whose run holds stage s
   __device__ __forceinline__ long long owner(long long s) const {
@@ -186,8 +188,8 @@ static __device__ __noinline__ int deal_any(const TreeParams& p, int cta, int gr
   tiles = warp_sum(tiles);
   total = warp_sum(total);
   longest = (int)__reduce_max_sync(0xffffffffu, (unsigned)longest);
-  plan.run = 0;
-  plan.active = plan.each = plan.extra = 0;
+  plan.run = plan.lead = 0;
+  plan.active = plan.each = plan.extra = plan.origin = 0;
   if (total == 0) return 0;
   const long long mean = quot(total + grid - 1, grid);
   if (tiles <= grid) {
@@ -236,6 +238,7 @@ static __device__ __noinline__ int deal_any(const TreeParams& p, int cta, int gr
         return at.j_end - at.j;
       }
       seek_stage(p, b0 + src, hit, local, at);
+      plan.origin = want - at.j;
       return (int)(plan.begin(cta + 1) - want);
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
@@ -244,6 +247,9 @@ static __device__ __noinline__ int deal_any(const TreeParams& p, int cta, int gr
 }
 
 constexpr int kTable = 512;  // sequences that deal() keeps in shared memory
+// Stages that a tile's queries, join and epilogue cost (0 / 2: 40 trees of up to 24 tokens 99 / 95 us, 32
+// chains with 32-bit queries 50.6 / 48.9, 100 short sequences 37.4 / 35.9; 1 and 3 within a microsecond of 2).
+constexpr int kLead = 2;
 
 // The table's entry of sequence b: tiles of all kv heads, stages of a tile.
 __device__ __forceinline__ int2 table_entry(const TreeParams& p, int b) {
@@ -268,8 +274,8 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int 
   if (__any_sync(0xffffffffu, large)) return deal_any(p, cta, grid, plan, at);
   tiles = __reduce_add_sync(0xffffffffu, tiles);
   total = __reduce_add_sync(0xffffffffu, total);
-  plan.run = 0;
-  plan.active = plan.each = plan.extra = 0;
+  plan.run = plan.lead = 0;
+  plan.active = plan.each = plan.extra = plan.origin = 0;
   if (total == 0) return 0;
   const int mean = (int)((uint32_t)(total + grid - 1) / (uint32_t)grid);
   if (tiles <= grid) {
@@ -290,38 +296,58 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int 
     } while (run_fits(run, mean));
   }
   if (plan.run == 0) {
+    plan.lead = kLead;
+    total += tiles * kLead;
     plan.active = min(grid, total);
     plan.each = (uint32_t)total / (uint32_t)plan.active;
     plan.extra = total - plan.each * plan.active;
   }
   if (cta >= plan.active) return 0;
-  const int want = plan.run > 0 ? cta : (int)plan.begin(cta);
-  int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int2 e = b0 + lane < p.batch ? table[b0 + lane] : make_int2(0, 0);
-    const int n = e.x * (plan.run > 0 ? (int)((uint32_t)(e.y + plan.run - 1) / (uint32_t)plan.run) : e.y);
-    int incl = n;
+  // a run's end, then its begin (or the piece)
+  int n_stages = 0;
+#pragma unroll 1
+  for (int k = plan.run > 0 ? 1 : 0; k < 2; k++) {
+    const int want = plan.run > 0 ? cta : (int)plan.begin(cta + 1 - k);
+    int before = 0, tiles_before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int2 e = b0 + lane < p.batch ? table[b0 + lane] : make_int2(0, 0);
+      const int n =
+          e.x * (plan.run > 0 ? (int)((uint32_t)(e.y + plan.run - 1) / (uint32_t)plan.run) : e.y + plan.lead);
+      int incl = n, incl_tiles = e.x;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
-    }
-    const int start = before + incl - n;
-    const unsigned found = __ballot_sync(0xffffffffu, want >= start && want < start + n);
-    if (found) {
-      const int src = __ffs(found) - 1;
-      const int local = want - __shfl_sync(0xffffffffu, start, src);
-      const Seq hit = seq_of(p, b0 + src);
-      if (plan.run > 0) {
-        seek_piece(p, plan.run, b0 + src, hit, (uint32_t)local, at);
-        return at.j_end - at.j;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, o), u = __shfl_up_sync(0xffffffffu, incl_tiles, o);
+        if (lane >= o) incl += t, incl_tiles += u;
       }
-      seek_stage(p, b0 + src, hit, local, at);
-      return (int)plan.begin(cta + 1) - want;
+      const int start = before + incl - n, tile0 = tiles_before + incl_tiles - e.x;
+      // (the end of the last run lies behind the last sequence)
+      const unsigned found = __ballot_sync(0xffffffffu, n > 0 && want >= start && want < start + n);
+      if (found) {
+        const int src = __ffs(found) - 1;
+        const int local = want - __shfl_sync(0xffffffffu, start, src);
+        if (plan.run > 0) {
+          seek_piece(p, plan.run, b0 + src, seq_of(p, b0 + src), (uint32_t)local, at);
+          return at.j_end - at.j;
+        }
+        const int stages = __shfl_sync(0xffffffffu, e.y, src), per = stages + plan.lead;
+        const int item = (int)((uint32_t)local / (uint32_t)per), off = local - item * per;
+        // stages before this place: all that is before it without the leads
+        const int here = want - off - (__shfl_sync(0xffffffffu, tile0, src) + item) * plan.lead + max(0, off - plan.lead);
+        if (k == 0) {
+          n_stages = here;
+        } else {
+          n_stages -= here;
+          if (n_stages > 0) seek_stage(p, b0 + src, seq_of(p, b0 + src), item * stages + max(0, off - plan.lead), at);
+          plan.origin = want - off;
+        }
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      tiles_before += __shfl_sync(0xffffffffu, incl_tiles, 31);
+      if (k == 0 && b0 + 32 >= p.batch) n_stages = before - tiles_before * plan.lead;  // all
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  return 0;
+  return n_stages;
 }
 
 // What query row r of a tile's sequence sees: prefix rows [kmin, base) and the drafted rows of

@@ -334,12 +334,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     // the tiles whose first pieces lie here and that others go on with: one that begins with this
     // CTA's stages, one at their end
     Walk w = at;
-    int done = 0;  // stages before tile w
+    int done = 0;                  // stages before tile w
+    long long base = plan.origin;  // where it begins, in the list with the leads
     for (int piece = 0; piece < 2; piece++) {
       Cut c = {};
       const int here = min(w.s.stages - w.j, n_stages - done);
       if (n_stages > 0 && w.j == 0 && here < w.s.stages && (piece == 0 || done > 0)) {
-        c.parts = plan.run > 0 ? w.chunks : (int)(plan.owner(plan.begin(cta) + done + w.s.stages - 1) - cta) + 1;
+        c.parts = plan.run > 0 ? w.chunks : (int)(plan.owner(base + plan.lead + w.s.stages - 1) - cta) + 1;
         c.stride = plan.run > 0 ? 2 * w.s.tiles : 2;
         c.rows = min(ROWS, w.s.T * p.group - w.tile * ROWS);
         c.row0 = w.s.row0;
@@ -355,6 +356,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       }
       while (done + (w.j_end - w.j) < n_stages) {
         done += w.j_end - w.j;
+        base += plan.lead + w.s.stages;
         w.next_tile(p);
       }
     }
