@@ -258,6 +258,9 @@ struct Vec<__half> {
 // 16-byte loads from the aligned address at or before the row's start; a segment that reaches over
 // either end of the row is read value by value, so nothing outside the row is read.  No thread
 // waits for another before the end of the part.
+// 384 rows of 262,144 f32 logits, capped: 81 us of the call's 87, 4.9 TB/s (0.75 of the measured copy), where
+// the issue slots of 12 instructions a logit bound it.  A few rows are bound by latency, the part's loads and the
+// join's: one row 10.6 us.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
   constexpr int VN = Vec<T>::N, NV = kEpt / VN;

@@ -7,14 +7,21 @@
 // The 128 side is always full, the work grows with the rows that exist, and at head_dim 512 the
 // accumulator of 64 rows takes 4 x 64 TMEM columns where [rows x 512] would take all 512.  TMEM
 // lane = key (scores) or head dim (output), column = query row.
-//   f16 queries: N columns are N query rows.
+//   f16 queries: a column is a query row (32 or 64 of them; of 64 columns the upper half idles at 32).
 //   f32 queries: N columns are N / 2 rows, first their high, then their low f16 terms (of Q and of
 //   P), so one MMA of N columns multiplies both; a thread adds a row's two columns itself.
 //
-// Bound.  An MMA of M 128, N 64, K 16 takes 48 cycles from shared memory (6 KB of operands at 128
-// B / cycle), so 64 columns over 128 keys at head_dim 512 take 3,072 cycles, while bringing those
-// keys' 256 KB at an SM's share of the HBM rate (about 23 B / cycle) takes 11,000: memory-bound up
-// to 3 tiles (192 columns) per kv head, tensor-bound beyond.
+// Bound.  A stage is 128 keys.  At head_dim 512 its 256 KB take 11,000 cycles at an SM's share of the HBM
+// rate (23 B / cycle).  Shared memory, 128 B / cycle, is the next limit: an MMA of M 128, N 64, K 16 reads 6
+// KB (48 cycles; 8 KB and 64 at N 128), so a stage of 64 columns moves 393 KB of operands and 256 KB of
+// copies, 5,100 cycles.  So one tile per kv head is bound by HBM and many by shared memory:
+//   8 tokens x 8 heads of 512 dims over 131,000 keys, f16: 69 us, 3.9 TB/s (0.59 of the measured copy)
+//   48 tokens, six tiles: 183 us, 564 TFLOP/s, 6,700 cycles a stage
+// Below 512 dims a stage is shorter than the softmax warps' serial chain, S -> registers -> vote -> exp2 -> P,
+// 3,600 cycles at 32 rows a warp (8 tiles of 256 dims over 32k keys: 4,900 a stage, 60 us) and about 2,400 at
+// 16.  Short calls are bound by latency: 14 us at one stage (f16), of which the start up to the first keys'
+// arrival is 5 us, a stage 3, the epilogue 1 to 2 and the join 3 to 4; a warm instruction costs less than
+// a cold one, so little code is on that path.
 //
 // Shared memory: Q [64-dim chunk][N][128 B], P [64-column chunk][128 keys][128 B], and a ring of
 // 32 KB units, each 128 keys x 128 dims of K or V as two [128 keys][128 B] chunks, all with the
@@ -23,14 +30,16 @@
 //   0-7    softmax: warp w has TMEM lanes 32 (w % 4) .. + 31 (keys) and the rows of half w / 4.
 //          A thread holds one key's scores for its rows.  The running maximum of a row is raised
 //          only when a score passes it by 2^8 (p = 2^(s - m + 7) <= 2^15 stays in f16): whether
-//          any does is one block-wide vote per stage; finding the maxima (a transposing reduction
-//          over the lanes and the four warps) and rescaling O in TMEM happens only then.
+//          any does is one vote of a half's four warps per stage; finding the maxima (a transposing
+//          reduction over the lanes and the four warps) and rescaling O in TMEM happens only then.
+//          (16 warps with half the rows each had 80 registers and no gain at 64 rows: 212 us for
+//          the six tiles above.)
 //   8-11   loads: row addresses through the page table (any page size), cp.async into the ring
 //          with zero fill for rows that are not there, and the tile's queries (f32 queries as the
 //          terms that a small kernel before this one has split them into).
-//   12     one thread issues the MMAs: S of stage i, then O of stage i - 1, so the softmax of a
-//          stage runs under the next stage's score product.
-//   13-15  hand landed units over to the MMA thread (proxy fence), V values checked on the way.
+//   12     issues the MMAs: S of stage i, then O of stage i - 1, so the softmax of a stage runs under
+//          the next stage's score product.
+//   13-15  hand landed units over to the MMA warp (proxy fence), V values checked on the way.
 // Every wait is bounded; a thread that gives up sets the abort flag and the error word, all waits
 // then end at once, and the CTA frees its TMEM and leaves.
 #include <algorithm>
@@ -942,8 +951,8 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
   static_assert(C::ROWS * (F32 ? 2 : 1) <= N, "columns");
   p.hd_pad = HD;
   const long long tiles = (tokens_rows + C::ROWS - 1) / C::ROWS;
-  const long long stages = (keys / kKeysT + p.batch) * tiles * p.nkh;
-  p.grid = (int)std::max<long long>(1, std::min<long long>(stages, std::min(ctx->num_sms, kMaxGrid)));
+  const double stages = (double)(keys / kKeysT + p.batch) * (double)tiles * p.nkh;
+  p.grid = (int)std::max(1.0, std::min(stages, (double)std::min(ctx->num_sms, kMaxGrid)));
   const size_t parts = (size_t)2 * p.grid * C::ROWS * (HD + 2) * sizeof(float);
   // workspace: the parts of cut tiles, the cuts, the queries' terms and scales (16-byte pieces)
   const size_t cuts = ((size_t)2 * p.grid * sizeof(Cut) + 15) & ~size_t(15);
@@ -982,7 +991,8 @@ g4a_status launch_tc(g4a_ctx* ctx, TreeParams& p, long long keys, long long toke
 // keys 16.4 / 18.0.  (A head of more than 256 dims has room for 64 columns only, so f32 has 32 rows.)
 g4a_status g4a_tree_tc_launch(g4a_ctx* ctx, g4a_tree::TreeParams& p, bool f32, long long keys) {
   const long long rows = (long long)p.max_tokens * p.group;
-  const bool narrow = rows <= 32 || (keys / kKeysT + p.batch) * ((rows + 31) / 32) * p.nkh <= 2 * ctx->num_sms;
+  const bool narrow =
+      rows <= 32 || (double)(keys / kKeysT + p.batch) * (double)((rows + 31) / 32) * p.nkh <= 2.0 * ctx->num_sms;
   if (p.hd > 256) {
     if (f32) return launch_tc<512, 64, true, 32>(ctx, p, keys, rows);
     return narrow ? launch_tc<512, 64, false, 32>(ctx, p, keys, rows) : launch_tc<512, 64, false, 64>(ctx, p, keys, rows);

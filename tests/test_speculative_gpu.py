@@ -602,6 +602,19 @@ def test_logprobs_reports_tokens_beyond_the_vocabulary(ctx):
 
 # -------------------------------------------------------------------------------------- compaction
 
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+def test_logprobs_of_vocabularies_of_more_than_1024_segments(ctx, fmt):
+    """More than 524,288 ids: the join goes through the segments tile by tile."""
+    rows, vocab, k = 2, 600_001, 32
+    g = torch.Generator().manual_seed(rows)
+    logits = (torch.randn((rows, vocab), generator=g) * 4).to(fmt).cuda()
+    toks = torch.randint(vocab, (rows, 3), generator=g).int().cuda()
+    for cap in (0.0, 30.0):
+        got = _run_logprobs(ctx, logits, toks, k, cap)
+        ctx.sync()
+        _check_logprobs(got, logits, toks, k, cap)
+
+
 @pytest.mark.parametrize("nkh,hd,page", [(1, 256, 64), (4, 128, 16), (2, 8, 3), (1, 512, 7)])
 def test_compact_moves_rows_as_if_read_first(ctx, nkh, hd, page):
     rnd = random.Random(hd)
