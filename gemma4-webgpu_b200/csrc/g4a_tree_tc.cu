@@ -17,11 +17,11 @@
 // copies, 5,100 cycles.  So one tile per kv head is bound by HBM and many by shared memory:
 //   8 tokens x 8 heads of 512 dims over 131,000 keys, f16: 69 us, 3.9 TB/s (0.59 of the measured copy)
 //   48 tokens, six tiles: 183 us, 564 TFLOP/s, 6,700 cycles a stage
-// Below 512 dims a stage is shorter than the softmax warps' serial chain, S -> registers -> vote -> exp2 -> P,
-// 3,600 cycles at 32 rows a warp (8 tiles of 256 dims over 32k keys: 4,900 a stage, 60 us) and about 2,400 at
-// 16.  Short calls are bound by latency: 14 us at one stage (f16), of which the start up to the first keys'
-// arrival is 5 us, a stage 3, the epilogue 1 to 2 and the join 3 to 4; a warm instruction costs less than
-// a cold one, so little code is on that path.
+// Below 512 dims the softmax warps' serial chain, S -> registers -> vote -> exp2 -> P, is longer than the
+// products: 3,600 cycles at 32 rows a warp (8 tiles of 256 dims over 32k keys: 4,900 a stage, 60 us), 1,950 at 16
+// (32 chains of up to 7 tokens x 3 heads of 128 dims, 3,000 keys: 2,830 a stage, which is the HBM share; 44 us).
+// Short calls are bound by latency: 14 us at one stage (f16), of which the start up to the first keys' arrival
+// is 5 us (3 of them to find this CTA's stages, in cold code), a stage 3, the epilogue 1 to 2, the join 3 to 4.
 //
 // Shared memory: Q [64-dim chunk][N][128 B], P [64-column chunk][128 keys][128 B], and a ring of
 // 32 KB units, each 128 keys x 128 dims of K or V as two [128 keys][128 B] chunks, all with the
