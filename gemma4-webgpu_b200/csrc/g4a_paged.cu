@@ -240,7 +240,8 @@ decltype(&paged_prep_kernel<0, QOut>) pick_prep(uint32_t hd, bool vec) {
 // 128-byte column chunk, tensor): 32 row lanes x 8 chunks of 16 bytes, at most 64 rows, so every
 // thread holds its two rows in registers across the one barrier between reads and writes.
 // Columns of different CTAs are disjoint, so nothing else has to be ordered.
-// Bound by latency, path -> page ids -> rows (1.9 us for 4 rows of 256 dims, 2.6 for 473 rows of 512 dims in 64 sequences).
+// Bound by latency, path -> page ids -> rows (1.9 us for 4 rows of 256 dims, 2.6 for 473 rows of 512 dims
+// in 64 sequences).
 constexpr int kMaxPath = 64;
 
 __global__ void __launch_bounds__(256)

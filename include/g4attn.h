@@ -69,7 +69,9 @@ const char* g4a_last_error(void);
 const char* g4a_version(void);
 
 /* Run subsequent calls on a caller-owned cudaStream_t (0 = the legacy default stream), or
- * back on the context's own non-blocking stream. */
+ * back on the context's own non-blocking stream.  Calls that use the context's workspace (split
+ * decode, tree attention, log probabilities) must not run on two streams at once: order the new
+ * stream behind the old one's work with an event, or use a context per stream. */
 g4a_status g4a_set_stream(g4a_ctx* ctx, void* cuda_stream);
 g4a_status g4a_use_own_stream(g4a_ctx* ctx);
 void* g4a_get_stream(g4a_ctx* ctx);
