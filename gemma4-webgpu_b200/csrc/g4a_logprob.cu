@@ -132,6 +132,13 @@ __device__ __forceinline__ uint64_t capped_small2(uint64_t x, uint64_t inv_cap) 
   return mul2(x, q);
 }
 
+// Largest of a warp's values, in one instruction (NaN is passed over).
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 struct Stat {
   float m, s, t;  // t in log2 units: sum (y - m) log2(e) e^(y - m)
 };
@@ -258,9 +265,10 @@ struct Vec<__half> {
 // 16-byte loads from the aligned address at or before the row's start; a segment that reaches over
 // either end of the row is read value by value, so nothing outside the row is read.  No thread
 // waits for another before the end of the part.
-// 384 rows of 262,144 f32 logits, capped: 81 us of the call's 87, 4.9 TB/s (0.75 of the measured copy), where
-// the issue slots of 12 instructions a logit bound it.  A few rows are bound by latency, the part's loads and the
-// join's: one row 10.6 us.
+// 384 rows of 262,144 f32 logits, capped, with 8 alternatives: the call takes 77 us, 5.2 TB/s (0.80 of the
+// measured copy), without the cap 68, without cap and alternatives 66 (0.93).  More registers' worth of CTAs, or
+// more and shorter parts, were slower.  A few rows are bound by latency, the part's loads and the join's chain
+// (one row 8.7 us, 37 odd f16 rows of 50,257 8.5).
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
   constexpr int VN = Vec<T>::N, NV = kEpt / VN;
@@ -310,9 +318,7 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
 #pragma unroll
     for (int e = 1; e < kEpt; e++) top = fmaxf(top, x[e]), low = fminf(low, x[e]);  // NaN is passed over
     if (seg_max != nullptr) {
-      float s = top;
-#pragma unroll
-      for (int o = 16; o >= 1; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+      const float s = warp_max(top);
       if (lane == 0) seg_max[t0 / kSeg] = s;
     }
     const float ym = CAP ? capped(top, p.cap, p.inv_cap2) : top;
@@ -419,8 +425,9 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
     }
     __syncthreads();
   };
-  // ---- the segments.  A row of up to 1024 of them: the pick-th largest of the thread maxima bounds
-  // the pick-th segment from below; what reaches it is listed and ranked.
+  // ---- the segments.  A row of up to 1024 of them: the pick-th largest of 64 maxima (of four threads'
+  // segments each) bounds the pick-th segment from below; what reaches it, mostly not twice as many as
+  // are wanted, is listed and ranked.  (Of all 256 thread maxima: a sharper bound, 2.4 us instead of 0.6.)
   bool have_segs = false;
   if (segs <= kNear * kThreadsL) {
     uint32_t o[kNear], best = 0;
@@ -429,18 +436,23 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
       o[e] = (uint32_t)(e * kThreadsL + tid) < segs ? ordered(near[e]) : 0u;
       best = max(best, o[e]);
     }
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 1));
+    best = max(best, __shfl_xor_sync(0xffffffffu, best, 2));
     uint32_t* tops = reinterpret_cast<uint32_t*>(sh.tops);
-    tops[tid] = best;
+    if ((tid & 3) == 0) tops[tid >> 2] = best;
     if (tid == 0) sh.bound = 0, sh.count = 0;
     __syncthreads();
-    int above = 0, equal = 0;
-#pragma unroll 8
-    for (int j = 0; j < kThreadsL / 4; j++) {
-      const uint4 v = reinterpret_cast<const uint4*>(tops)[j];
-      above += (v.x > best) + (v.y > best) + (v.z > best) + (v.w > best);
-      equal += (v.x == best) + (v.y == best) + (v.z == best) + (v.w == best);
+    if (tid < kThreadsL / 4) {
+      const uint32_t mine = tops[tid];
+      int above = 0, equal = 0;
+#pragma unroll
+      for (int j = 0; j < kThreadsL / 16; j++) {
+        const uint4 v = reinterpret_cast<const uint4*>(tops)[j];
+        above += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
+        equal += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
+      }
+      if (above < pick && pick <= above + equal) sh.bound = mine;
     }
-    if (above < pick && pick <= above + equal) sh.bound = best;
     __syncthreads();
     const uint32_t bound = (uint32_t)sh.bound;
 #pragma unroll
