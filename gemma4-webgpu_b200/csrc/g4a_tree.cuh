@@ -246,7 +246,7 @@ static __device__ __noinline__ int deal_any(const TreeParams& p, int cta, int gr
   return 0;
 }
 
-constexpr int kTable = 512;  // sequences that deal() keeps in shared memory
+constexpr int kTable = 512;  // sequences that deal() finds in the lanes and in shared memory
 // Stages that a tile's queries, join and epilogue cost (0 / 2: 40 trees of up to 24 tokens 99 / 95 us, 32
 // chains with 32-bit queries 50.6 / 48.9, 100 short sequences 37.4 / 35.9; 1 and 3 within a microsecond of 2).
 constexpr int kLead = 2;
@@ -257,17 +257,20 @@ __device__ __forceinline__ int2 table_entry(const TreeParams& p, int b) {
   return make_int2(p.nkh * s.tiles, s.stages);
 }
 
-// One full warp: the plan, CTA `cta`'s first stage, and their number (0: no work).  Up to kTable
-// sequences are dealt from `table` (filled by the whole CTA: one round of loads) in 32 bits and little
-// code: the kernels start cold, and every line of code on this path is fetched before the first key is.
-__device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int cta, int grid, Plan& plan, Walk& at) {
+// One full warp: the plan, CTA `cta`'s first stage, and their number (0: no work).  A lane holds the entry
+// `own` of sequence `lane`; those from 32 on, up to kTable, lie in `table` (filled by the whole CTA: one round
+// of loads).  32 bits and little code: the kernels start cold, and every line of code on this path is
+// fetched before the first key is.
+__device__ __forceinline__ int deal(const TreeParams& p, const int2 own, const int2* table, int cta, int grid, Plan& plan,
+                                    Walk& at) {
   const int lane = threadIdx.x & 31;
-  int tiles = 0, total = 0;
-  bool large = p.batch > kTable;
-  for (int b = lane; b < p.batch && !large; b += 32) {
+  int tiles = own.x, total = own.x * own.y;
+  bool large = p.batch > kTable || __umulhi((uint32_t)own.x, (uint32_t)own.y) != 0 || (uint32_t)total > 0x1fffffu;
+#pragma unroll 1
+  for (int b = lane + 32; b < p.batch && !large; b += 32) {
     const int2 e = table[b];
     const long long n = (long long)e.x * e.y;
-    large = n > 0x3fffff || total > 0x3ffffff;
+    large = n > 0x1fffff;  // (kTable of these stay below 2^30)
     tiles += e.x;
     total += (int)n;
   }
@@ -280,9 +283,11 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int 
   const int mean = (int)((uint32_t)(total + grid - 1) / (uint32_t)grid);
   if (tiles <= grid) {
     int run = mean;
+#pragma unroll 1
     do {
-      int pieces = 0;
-      for (int b = lane; b < p.batch; b += 32) {
+      int pieces = own.x * (int)((uint32_t)(own.y + run - 1) / (uint32_t)run);
+#pragma unroll 1
+      for (int b = lane + 32; b < p.batch; b += 32) {
         const int2 e = table[b];
         pieces += e.x * (int)((uint32_t)(e.y + run - 1) / (uint32_t)run);
       }
@@ -292,7 +297,7 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int 
         plan.active = pieces;
         break;
       }
-      run = max(run + 1, (int)quot((long long)run * pieces, grid));
+      run = max(run + 1, (int)((uint32_t)(run * pieces) / (uint32_t)grid));
     } while (run_fits(run, mean));
   }
   if (plan.run == 0) {
@@ -309,8 +314,9 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2* table, int 
   for (int k = plan.run > 0 ? 1 : 0; k < 2; k++) {
     const int want = plan.run > 0 ? cta : (int)plan.begin(cta + 1 - k);
     int before = 0, tiles_before = 0;
+#pragma unroll 1
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      const int2 e = b0 + lane < p.batch ? table[b0 + lane] : make_int2(0, 0);
+      const int2 e = b0 == 0 ? own : b0 + lane < p.batch ? table[b0 + lane] : make_int2(0, 0);
       const int n =
           e.x * (plan.run > 0 ? (int)((uint32_t)(e.y + plan.run - 1) / (uint32_t)plan.run) : e.y + plan.lead);
       int incl = n, incl_tiles = e.x;

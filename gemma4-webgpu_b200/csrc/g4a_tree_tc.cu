@@ -334,11 +334,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   // (the table lies where P will: P is written after every warp has read it)
   int2* table = reinterpret_cast<int2*>(smem + C::OFF_P);
   static_assert(C::P_BYTES >= kTable * (int)sizeof(int2), "table of sequences");
-  if (p.batch <= kTable) {
+  const int2 own = lane < p.batch ? table_entry(p, lane) : make_int2(0, 0);
+  if (p.batch > 32 && p.batch <= kTable) {
     for (int b = tid; b < p.batch; b += kThreadsTc) table[b] = table_entry(p, b);
     __syncthreads();
   }
-  const int n_stages = deal(p, table, cta, (int)gridDim.x, plan, at);
+  const int n_stages = deal(p, own, table, cta, (int)gridDim.x, plan, at);
   if (warp == kMmaWarp + 3) {
     // the tiles whose first pieces lie here and that others go on with: one that begins with this
     // CTA's stages, one at their end
