@@ -94,6 +94,12 @@ __device__ __forceinline__ float capped_small(float x, float inv_cap) {
   return x * q;
 }
 
+// Which of the two, by the value alone: the parts and the join have to agree, so that what a logit's own
+// rounding adds to log p cancels where it is the largest.
+__device__ __forceinline__ float capped_by(float x, float cap, float inv_cap, float inv_cap2) {
+  return fabsf(x) <= kCapRange * cap ? capped_small(x, inv_cap) : capped(x, cap, inv_cap2);
+}
+
 // Two floats in one 64-bit register: the packed multiply-add does both in one issue slot, and the
 // pass over capped logits is bound by issue slots.
 __device__ __forceinline__ uint64_t two(float a, float b) {
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
       const float s = warp_max(top);
       if (lane == 0) seg_max[t0 / kSeg] = s;
     }
-    const float ym = CAP ? capped(top, p.cap, p.inv_cap2) : top;
+    const float ym = CAP ? capped_by(top, p.cap, p.inv_cap, p.inv_cap2) : top;
     const float m = fmaxf(st.m, ym);
     if (m > st.m) {
       const float d = st.m == -INFINITY ? 0.f : (st.m - m) * kLog2eL, w = g4a::fast_exp2(d);
@@ -329,7 +335,9 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
       st.s *= w;
       st.m = m;
     }
-    const float ml = (m == -INFINITY ? 0.f : m) * kLog2eL;
+    // the exponents are y log2(e) - ml; what rounding left of m log2(e) in ml (up to 2e-6, the same for all
+    // values) is taken out of the sums: 2^-left s, 2^-left (t - left s)
+    const float mf = m == -INFINITY ? 0.f : m, ml = mf * kLog2eL, left = fmaf(mf, kLog2eL, -ml);
     float s = 0.f, t = 0.f;
     if (top <= small && low >= -small) {  // finite, and within the polynomial's range
       uint64_t s2 = 0, t2 = 0;
@@ -352,15 +360,16 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
     } else {
 #pragma unroll
       for (int e = 0; e < kEpt; e++) {
-        const float y = CAP ? capped(x[e], p.cap, p.inv_cap2) : x[e];
+        const float y = CAP ? capped_by(x[e], p.cap, p.inv_cap, p.inv_cap2) : x[e];
         const float d = fmaf(y, kLog2eL, -ml);
         const float w = g4a::fast_exp2(d);
         s += w;
         t = fmaf(fmaxf(d, -1000.f), w, t);  // -inf: -1000 * 0
       }
     }
-    st.s += s;
-    st.t += t;
+    const float f = fmaf(-kLn2L, left, 1.0f);
+    st.s = fmaf(f, s, st.s);
+    st.t = fmaf(f, fmaf(-left, s, t), st.t);
   }
   st = block_join(st, red);
   if (tid == 0) p.stats[(size_t)row * p.split + part] = make_float4(st.m, st.s, st.t, 0.f);
@@ -396,9 +405,7 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
   const float ln_s = logf(st.s);
   const float cap = p.cap;
   auto value = [&](float x) {  // log probability of a logit
-    const float y = !(cap > 0.f)                      ? x
-                    : fabsf(x) <= kCapRange * cap ? capped_small(x, p.inv_cap)
-                                                  : capped(x, cap, p.inv_cap2);
+    const float y = cap > 0.f ? capped_by(x, cap, p.inv_cap, p.inv_cap2) : x;
     return y - st.m - ln_s;
   };
   if (p.entropy && tid == 0) p.entropy[row] = ln_s - kLn2L * st.t / st.s;
