@@ -100,8 +100,8 @@ __device__ __forceinline__ float capped_by(float x, float cap, float inv_cap, fl
   return fabsf(x) <= kCapRange * cap ? capped_small(x, inv_cap) : capped(x, cap, inv_cap2);
 }
 
-// Two floats in one 64-bit register: the packed multiply-add does both in one issue slot, and the
-// pass over capped logits is bound by issue slots.
+// Two floats in one 64-bit register: the packed multiply-add does both in one issue slot (384 capped rows of
+// 262,144: 101 us with single ones, 87 so).
 __device__ __forceinline__ uint64_t two(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -271,10 +271,10 @@ struct Vec<__half> {
 // 16-byte loads from the aligned address at or before the row's start; a segment that reaches over
 // either end of the row is read value by value, so nothing outside the row is read.  No thread
 // waits for another before the end of the part.
-// 384 rows of 262,144 f32 logits, capped, with 8 alternatives: the call takes 77 us, 5.2 TB/s (0.80 of the
-// measured copy), without the cap 68, without cap and alternatives 66 (0.93).  More registers' worth of CTAs, or
-// more and shorter parts, were slower.  A few rows are bound by latency, the part's loads and the join's chain
-// (one row 8.7 us, 37 odd f16 rows of 50,257 8.5).
+// 384 rows of 262,144 f32 logits, capped, with 8 alternatives: the call takes 78 us, 5.2 TB/s (0.79 of the
+// measured copy), without the cap 68, without cap and alternatives 66 (0.93).  More CTAs to an SM (fewer
+// registers), or more and shorter parts, were slower.  A few rows are bound by latency, the part's loads and
+// the join's chain (one row 8.7 us, 37 odd f16 rows of 50,257 8.5).
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
   constexpr int VN = Vec<T>::N, NV = kEpt / VN;
@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(kThreadsL) logprob_join_kernel(const LogprobPa
   };
   // ---- the segments.  A row of up to 1024 of them: the pick-th largest of 64 maxima (of four threads'
   // segments each) bounds the pick-th segment from below; what reaches it, mostly not twice as many as
-  // are wanted, is listed and ranked.  (Of all 256 thread maxima: a sharper bound, 2.4 us instead of 0.6.)
+  // are wanted, is listed and ranked.  (Of all 256 thread maxima: a sharper bound, but 2.4 us of counting; a
+  // call of one row took 10.4 us, takes 8.7.)
   bool have_segs = false;
   if (segs <= kNear * kThreadsL) {
     uint32_t o[kNear], best = 0;

@@ -85,6 +85,7 @@ def _fmt(t, name) -> int:
 
 
 _formats_of: dict = {}
+_dtypes_of: list = []
 
 
 def _formats() -> dict:
@@ -95,8 +96,24 @@ def _formats() -> dict:
     return _formats_of
 
 
+def _dtypes() -> list:
+    """float32, float16, int32, int64 (an import statement in every call costs a tenth of a launch)."""
+    if not _dtypes_of:
+        import torch
+
+        _dtypes_of.extend((torch.float32, torch.float16, torch.int32, torch.int64))
+    return _dtypes_of
+
+
 def _rows_addr(t, name, dtype, width, device) -> tuple[int, int, int]:
     """(address, rows, row stride in elements) of a tensor whose rows are `width` packed elements."""
+    try:
+        if t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+            shape = t.shape
+            if len(shape) == 2 and shape[1] == width or len(shape) == 3 and shape[1] * shape[2] == width:
+                return t.data_ptr(), shape[0], width
+    except AttributeError:
+        pass
     import torch
 
     if not isinstance(t, torch.Tensor):
@@ -329,21 +346,19 @@ class Context:
     # ---------------------------------------------------------------- speculative step, paged cache
     def rope_table(self, positions, rope_freqs, cos_sin, *, head_dim, theta, apply_divisor=0) -> None:
         """cos and sin of the tokens' RoPE angles (g4a_rope_table), once per step for all layers."""
-        import torch
-
         dev, n = self.device, positions.numel()
-        rf = _addr(rope_freqs, "rope_freqs", torch.float16, head_dim // 2, dev) if apply_divisor else None
-        call("g4a_rope_table", self._h, _addr(positions, "positions", torch.int32, 0, dev), rf,
-             _addr(cos_sin, "cos_sin", torch.float32, n * head_dim, dev), n, head_dim, theta, apply_divisor)
+        f32, f16, i32, _ = _dtypes()
+        rf = _addr(rope_freqs, "rope_freqs", f16, head_dim // 2, dev) if apply_divisor else None
+        call("g4a_rope_table", self._h, _addr(positions, "positions", i32, 0, dev), rf,
+             _addr(cos_sin, "cos_sin", f32, n * head_dim, dev), n, head_dim, theta, apply_divisor)
 
     def _pages(self, k_pages, v_pages, page_table, num_kv_heads, head_dim, page_size):
         """Checks a page pool and its table; returns their addresses and (batch, max_pages_per_seq, num_pages)."""
-        import torch
-
         dev, size = self.device, k_pages.numel()
-        k = _addr(k_pages, "k_pages", torch.float16, 0, dev)
-        v = _addr(v_pages, "v_pages", torch.float16, size, dev)
-        t = _addr(page_table, "page_table", torch.int32, 0, dev)
+        _, f16, i32, _ = _dtypes()
+        k = _addr(k_pages, "k_pages", f16, 0, dev)
+        v = _addr(v_pages, "v_pages", f16, size, dev)
+        t = _addr(page_table, "page_table", i32, 0, dev)
         shape = page_table.shape
         if len(shape) != 2:
             raise ValueError("page_table must be [batch, max_pages_per_seq]")
@@ -357,10 +372,9 @@ class Context:
         """New tokens of a batch: q / k norm + RoPE, v norm, append to the paged cache
         (g4a_paged_qkv_prep).  q, k and v may be row-strided (columns of one projection's output);
         k = v = None computes q alone, num_q_heads = 0 stores k and v alone."""
-        import torch
-
-        dev, n, f16, f32 = self.device, token_seq.numel(), torch.float16, torch.float32
-        seq = _addr(token_seq, "token_seq", torch.int32, 0, dev)
+        dev, n = self.device, token_seq.numel()
+        f32, f16, i32, _ = _dtypes()
+        seq = _addr(token_seq, "token_seq", i32, 0, dev)
         cs = _addr(cos_sin, "cos_sin", f32, n * head_dim, dev)
         qp = qw = qo = kp = vp = kw = kpool = vpool = table = sl = None
         qs = ks = fmt = batch = max_pages = num_pages = 0
@@ -379,7 +393,7 @@ class Context:
             if ks != vs and n > 1:
                 raise ValueError(f"k and v must have one row stride, got {ks} and {vs}")
             kw = _addr(k_norm_w, "k_norm_w", f16, head_dim, dev)
-            sl = _addr(slots, "slots", torch.int32, n, dev)
+            sl = _addr(slots, "slots", i32, n, dev)
             kpool, vpool, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads,
                                                                            head_dim, page_size)
         elif page_table is not None:
@@ -394,15 +408,14 @@ class Context:
                         host_kv_lens=None) -> None:
         """Attention of drafted tokens (a tree per sequence, or a chain with tree_mask None) over the
         paged cache (g4a_tree_attn_paged).  tree_mask is int64, one word of ancestor bits per token."""
-        import torch
-
-        dev, i32 = self.device, torch.int32
+        dev = self.device
+        _, _, i32, i64 = _dtypes()
         kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
                                                                  page_size)
         fmt, n, size = _fmt(q, "q"), q.shape[0], q.numel()
         if size != n * num_q_heads * head_dim:
             raise ValueError(f"q must be [tokens, {num_q_heads}, {head_dim}], got {tuple(q.shape)}")
-        mask = None if tree_mask is None else _addr(tree_mask, "tree_mask", torch.int64, n, dev)
+        mask = None if tree_mask is None else _addr(tree_mask, "tree_mask", i64, n, dev)
         lens = None if host_kv_lens is None else _host_lens(host_kv_lens, batch)
         call("g4a_tree_attn_paged", self._h, _addr(q, "q", q.dtype, 0, dev), fmt, kp, vp, table,
              _addr(kv_lens, "kv_lens", i32, batch, dev), None if lens is None else lens.ctypes.data,
@@ -415,9 +428,8 @@ class Context:
         """Log probabilities of given tokens, entropy and top alternatives of rows of logits
         (g4a_token_logprobs).  logits [rows, vocab] f32 or f16, row-strided; tokens and logprob
         [rows, n] (both None: left out); top_logprob and top_ids [rows, k]."""
-        import torch
-
-        dev, f32 = self.device, torch.float32
+        dev = self.device
+        f32, _, i32, _ = _dtypes()
         fmt = _fmt(logits, "logits")
         if logits.dim() != 2:
             raise ValueError("logits must be [rows, vocab]")
@@ -430,7 +442,7 @@ class Context:
             if len(shape) not in (1, 2) or shape[0] != rows:
                 raise ValueError(f"tokens must be [{rows}] or [{rows}, n]")
             per_row = shape[1] if len(shape) == 2 else 1
-            tok = _addr(tokens, "tokens", torch.int32, 0, dev)
+            tok = _addr(tokens, "tokens", i32, 0, dev)
             lp = _addr(logprob, "logprob", f32, rows * per_row, dev)
         if entropy is not None:
             ent = _addr(entropy, "entropy", f32, rows, dev)
@@ -438,16 +450,15 @@ class Context:
             if top_ids is None or top_ids.dim() != 2 or top_ids.shape[0] != rows:
                 raise ValueError(f"top_ids must be [{rows}, k]")
             top_k = top_ids.shape[1]
-            ti = _addr(top_ids, "top_ids", torch.int32, 0, dev)
+            ti = _addr(top_ids, "top_ids", i32, 0, dev)
             tv = _addr(top_logprob, "top_logprob", f32, rows * top_k, dev)
         call("g4a_token_logprobs", self._h, x, fmt, tok, rows, vocab, stride, per_row, top_k, softcap, lp, ent, tv, ti)
 
     def paged_kv_compact(self, k_pages, v_pages, page_table, base_lens, path, path_lens, *, num_kv_heads, head_dim,
                          page_size) -> None:
         """Rows base + path[i] of each sequence become rows base + i (g4a_paged_kv_compact)."""
-        import torch
-
-        dev, i32 = self.device, torch.int32
+        dev = self.device
+        _, _, i32, _ = _dtypes()
         kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
                                                                  page_size)
         shape = path.shape
