@@ -746,6 +746,59 @@ def test_capture_and_replay_a_step(ctx):
         del graph
 
 
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+def test_captured_tree_attention_follows_lengths_pages_and_masks(ctx, fmt):
+    """One graph, captured while the sequences were short, replayed for longer, shorter and empty ones on
+    other pages: the partition is found from what is on the device at replay."""
+    cases = [Paged(30 + i, lens, counts, nkh=1, hd=128, page=16, spare=1) for i, (lens, counts) in enumerate(
+        [([40, 30, 20], [4, 3, 2]), ([2500, 6, 900], [5, 2, 2]), ([0, 1, 700], [0, 1, 8]), ([8, 0, 0], [8, 0, 0])])]
+    pages, width = max(c.k.shape[0] for c in cases), max(c.table.shape[1] for c in cases)
+    k = torch.zeros((pages, 16, 1, 128), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.zeros((3, width), dtype=torch.int32, device="cuda")
+    lens, indptr = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    mask = torch.zeros(9, dtype=torch.int64, device="cuda")
+    q, out = torch.zeros((9, 8, 128), dtype=fmt, device="cuda"), torch.zeros((9, 8, 128), dtype=fmt, device="cuda")
+
+    def load(case, words, x):
+        k[:case.k.shape[0]], v[:case.v.shape[0]] = case.k, case.v
+        table.zero_()
+        table[:, :case.table.shape[1]] = case.table
+        lens.copy_(case.lens_dev)
+        indptr.copy_(case.indptr)
+        mask.zero_()
+        mask[:len(words)] = mask_tensor(words)
+        q.copy_(x)
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+
+    g = torch.Generator().manual_seed(31)
+    side = torch.cuda.Stream()
+    with g4attn.Context(0) as c:
+        c.set_stream(side.cuda_stream)
+        run = lambda: c.tree_attn_paged(q, k, v, table, lens, indptr, mask, out, num_q_heads=8, num_kv_heads=1,  # noqa: E731
+                                        head_dim=128, page_size=16, max_tokens=8, scale=128 ** -0.5,
+                                        host_kv_lens=cases[0].lens)
+        graph = None
+        for case in cases:
+            words = tree_masks(case.counts, random.Random(31))
+            x = (torch.randn((9, 8, 128), generator=g) * 2).to(fmt)
+            load(case, words, x)
+            if graph is None:
+                run()
+                c.sync()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=side):
+                    run()
+            out.fill_(5.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            c.sync()
+            torch.cuda.synchronize()
+            _check_tree(out, case, x.cuda(), words)
+        del graph
+
+
 def test_speculative_step_equals_decoding_one_by_one(ctx):
     """A whole step for two sequences: prompt chunk into the pages, a drafted tree, attention of all
     its tokens at once, the accepted path moved together, and the next token decoded from the pages.
