@@ -97,6 +97,7 @@ struct Tc {
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
   static constexpr uint32_t TMEM_COLS = COL_S + 2 * N <= 256 ? 256u : 512u;
+  // (the queries are handed over after a stage's K units, so the ring has to hold those: UNITS >= MB)
   static_assert(COL_S + 2 * N <= 512 && UNITS >= 3 && UNITS >= MB && SMEM <= 232448, "tile fits");
 };
 
@@ -491,7 +492,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       rows_before = rows;
       if (++w.j == w.j_end && i + 1 < n_stages) w.next_tile(p);
     }
+    // No copy and no arrival of one may be under way when the CTA ends, also after an abort, when nobody
+    // else waits for them (all four warps issue every unit, so these waits end).
     cp_wait_all();
+    for (int u = 0; u < UNITS && u < issued; u++)
+      (void)mbar_wait_bounded(&landed[u], (uint32_t)((issued - 1 - u) / UNITS) & 1u, p.err, G4A_DEVERR_WAIT_MMA);
+    for (int u = 0; u < 4 && u <= tile_no; u++)
+      (void)mbar_wait_bounded(&qlanded[u], (uint32_t)((tile_no - u) >> 2) & 1u, p.err, G4A_DEVERR_WAIT_MMA);
   } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------------------ MMAs
     regs_down<C::REGS_MMA>();
@@ -676,6 +683,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       if (first) {
         tile_no++;
         w = pieces[tile_no & 3];
+        // (after an abort the loads run ahead and the piece may be half of another one: write nothing)
+        if (*abort_flag) w.s.T = 0;
         j_first = w.j;
       }
       const bool last = i + 1 == n_stages || w.j + 1 == w.j_end;
