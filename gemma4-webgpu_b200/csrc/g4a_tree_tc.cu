@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   Plan plan;
   Walk at = {};
   const int cta = (int)blockIdx.x;
-  // (the table lies where P will: P is written after every warp has read it)
+  // (the table lies where P will)
   int2* table = reinterpret_cast<int2*>(smem + C::OFF_P);
   static_assert(C::P_BYTES >= kTable * (int)sizeof(int2), "table of sequences");
   const int2 own = lane < p.batch ? table_entry(p, lane) : make_int2(0, 0);
@@ -341,6 +341,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     __syncthreads();
   }
   const int n_stages = deal(p, own, table, cta, (int)gridDim.x, plan, at);
+  // No warp writes P before every warp has read the table: the two softmax shares meet nowhere else before
+  // the first stage's P.
+  if (p.batch > 32 && p.batch <= kTable) __syncthreads();
   if (warp == kMmaWarp + 3) {
     // the tiles whose first pieces lie here and that others go on with: one that begins with this
     // CTA's stages, one at their end

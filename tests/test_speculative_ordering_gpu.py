@@ -1,0 +1,55 @@
+"""What several warps of a speculative-step kernel hand to one another through shared memory.
+
+Each case runs many times, behind other kernels and alone, so that warps come late in different places;
+every result has to be the first one's to the bit, and the first is held to the 64-bit definition.
+"""
+import random
+
+import pytest
+import torch
+
+from spec_ref import Paged, mask_tensor, tree_attn_ref, tree_masks, tree_tolerance
+
+pytestmark = pytest.mark.gpu
+
+
+def _tree(ctx, case, q, mask, out, window=0):
+    nqh, hd = q.shape[1], q.shape[2]
+    ctx.tree_attn_paged(q, case.k, case.v, case.table, case.lens_dev, case.indptr, mask, out, num_q_heads=nqh,
+                        num_kv_heads=case.nkh, head_dim=hd, page_size=case.page, max_tokens=max(case.counts),
+                        scale=hd ** -0.5, sliding_window=window, host_kv_lens=case.lens)
+
+
+def _same_every_time(ctx, case, q, words, repeats=200, window=0):
+    mask = mask_tensor(words)
+    first = torch.zeros_like(q)
+    _tree(ctx, case, q, mask, first, window)
+    ctx.sync()
+    ref, amp = tree_attn_ref(case, q, words, scale=q.shape[2] ** -0.5, window=window)
+    vmax = max(float(v.double().abs().max()) for _, v in case.rows if v.numel())
+    tol = tree_tolerance(amp, q.shape[2], max(case.lens), vmax, q.dtype == torch.float16)
+    assert float((first.double().cpu() - ref).abs().max()) <= tol
+    out = torch.zeros_like(q)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(repeats):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(1 + i % 3):
+            _tree(ctx, case, q, mask, out, window)
+        ctx.sync()
+        differ += (out != first).any()
+    assert int(differ) == 0
+
+
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("batch,hd,group,most", [(33, 128, 3, 6), (70, 256, 8, 4), (140, 64, 2, 2)])
+def test_tree_attn_of_33_to_512_sequences_is_the_same_every_time(ctx, fmt, batch, hd, group, most):
+    """The table of sequences shares its place with the softmax weights: all warps are done with it before the
+    first weight is written.  Short sequences, so that the first weights come early."""
+    rnd = random.Random(batch)
+    counts = [rnd.randint(1, most) for _ in range(batch)]
+    lens = [c + rnd.randint(0, 90) for c in counts]
+    case = Paged(batch, lens, counts, nkh=1, hd=hd, page=16)
+    g = torch.Generator().manual_seed(hd)
+    q = (torch.randn((sum(counts), group, hd), generator=g) * 2).to(fmt).cuda()
+    _same_every_time(ctx, case, q, tree_masks(counts, rnd))
