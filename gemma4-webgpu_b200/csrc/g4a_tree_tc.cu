@@ -87,7 +87,8 @@ struct Tc {
   static constexpr int OFF_U = OFF_SCALE + 4 * ROWS * 4;      // [softmax warps][W] m - 7 of its rows
   static constexpr int OFF_F = OFF_U + kSoftWarps * W * 4;    // [softmax warps][W] rescale factors
   static constexpr int OFF_MAX = OFF_F + kSoftWarps * W * 4;  // [shares][4 quarters][W]
-  static constexpr int OFF_OK = OFF_MAX + kSoftWarps * W * 4; // [8 stages][4] which rows are there
+  static constexpr int OFF_SUM = OFF_MAX + kSoftWarps * W * 4; // [shares][4 quarters][W]
+  static constexpr int OFF_OK = OFF_SUM + kSoftWarps * W * 4; // [8 stages][4] which rows are there
   static constexpr int OFF_BAD = OFF_OK + 128;                // [8] tile + 1 that had a V value that is not finite
   static constexpr int OFF_VOTE = OFF_BAD + 32;               // [shares][2][4 quarters]
   static constexpr int OFF_INFO = OFF_VOTE + kShares * 32;               // [4] Walk of a piece's begin
@@ -643,7 +644,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     float* su = reinterpret_cast<float*>(smem + C::OFF_U) + warp * W;
     float* sf = reinterpret_cast<float*>(smem + C::OFF_F) + warp * W;
+    // Row maxima and row sums meet in places of their own, so that a tile's first maxima may be written while
+    // a slower warp still reads the sums of the tile before (a first stage takes no vote).  Two writes of one
+    // place have a meeting between them that follows the reads of the earlier one.
     float* smax = reinterpret_cast<float*>(smem + C::OFF_MAX) + share * 4 * W;
+    float* ssum = reinterpret_cast<float*>(smem + C::OFF_SUM) + share * 4 * W;
     int* votes = reinterpret_cast<int*>(smem + C::OFF_VOTE) + share * 8;
     // The share's four warps meet (a bounded wait like every other); what they wrote before is visible
     // after.  `votes` alternates between two sets, so that nobody writes what another still reads.
@@ -829,11 +834,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         const bool later = i - (w.j - j_first) > 0;  // not the piece this CTA's stages begin with
         float* part = p.part + ((size_t)2 * cta + (later ? 1 : 0)) * ROWS * (HD + 2);
         if (live > 0) {
-          meet();  // smax is free
           const float mine = transpose_reduce<W>(l, [](float a, float c) { return a + c; });
-          if (lane < W) smax[quarter * W + lane] = mine;
+          if (lane < W) ssum[quarter * W + lane] = mine;
           meet();
-          const float lt = (smax[n_of] + smax[W + n_of]) + (smax[2 * W + n_of] + smax[3 * W + n_of]);
+          const float lt = (ssum[n_of] + ssum[W + n_of]) + (ssum[2 * W + n_of] + ssum[3 * W + n_of]);
           if (lane < W) sf[lane] = !whole ? 1.f : lt == 0.f ? 0.f : 1.f / lt;
           if (!whole && quarter == 0 && lane < W) {
             part[(size_t)ROWS * HD + share * W + lane] = m;

@@ -53,3 +53,21 @@ def test_tree_attn_of_33_to_512_sequences_is_the_same_every_time(ctx, fmt, batch
     g = torch.Generator().manual_seed(hd)
     q = (torch.randn((sum(counts), group, hd), generator=g) * 2).to(fmt).cuda()
     _same_every_time(ctx, case, q, tree_masks(counts, rnd))
+
+
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("hd,nkh,group,batch,most,longest", [
+    (64, 4, 2, 60, 8, 300),   # 16 rows to a tile, several tiles of one or two stages to a CTA
+    (256, 4, 8, 50, 8, 40),   # 64 rows, one stage to a tile
+    (512, 2, 8, 100, 4, 150),
+    (64, 1, 2, 512, 2, 90),   # as many sequences as the table holds
+])
+def test_tree_attn_of_several_tiles_to_a_cta_is_the_same_every_time(ctx, fmt, hd, nkh, group, batch, most, longest):
+    """A tile's first maxima do not reach the sums of the tile before it."""
+    rnd = random.Random(hd + batch)
+    counts = [rnd.randint(1, most) for _ in range(batch)]
+    lens = [c + rnd.randint(0, longest) for c in counts]
+    case = Paged(batch, lens, counts, nkh=nkh, hd=hd, page=16)
+    g = torch.Generator().manual_seed(hd)
+    q = (torch.randn((sum(counts), nkh * group, hd), generator=g) * 2).to(fmt).cuda()
+    _same_every_time(ctx, case, q, tree_masks(counts, rnd))
