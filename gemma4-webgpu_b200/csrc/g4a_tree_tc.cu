@@ -93,7 +93,7 @@ struct Tc {
   static constexpr int OFF_VOTE = OFF_BAD + 32;               // [shares][2][4 quarters]
   static constexpr int OFF_INFO = OFF_VOTE + kShares * 32;               // [4] Walk of a piece's begin
   static constexpr int OFF_BAR = OFF_INFO + 4 * 64;
-  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 5 + kShares;
+  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 4 + kShares + 8;
   static constexpr int OFF_END = OFF_BAR + NBARS * 8;
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
@@ -284,6 +284,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   uint64_t* ofree = pvdone + 1;         // softmax warps
   uint64_t* mend = ofree + 1;           // MMA commit
   uint64_t* meet_bar = mend + 1;        // [shares] its 4 softmax warps
+  // [8] stage & 7: the 4 loading warps, when what they have stored for the stage (okw) and for a tile that begins
+  // with it (pieces, sees, scales) is there.  The arrivals of their copies say nothing of ordinary stores.
+  uint64_t* told = meet_bar + kShares;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
 
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     mbar_init(ofree, kSoftWarps);
     mbar_init(mend, 1);
     for (int u = 0; u < kShares; u++) mbar_init(&meet_bar[u], 4);
+    for (int u = 0; u < 8; u++) mbar_init(&told[u], 4);
     *abort_flag = 0;
     for (int u = 0; u < 8; u++) badv[u] = 0;
     for (int u = 0; u < 4; u++) pieces[u] = Walk{};  // (what a role reads that had to give up a wait)
@@ -491,6 +495,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
         }
         load_units(rows, p.k);
         if (first) finish_queries();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&told[i & 7]);
       }
       if (i > 0) load_units(rows_before, p.v);
       rows_before = rows;
@@ -526,6 +532,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           if (first) {
             tile_no++;
             ok = ready(&qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+            if (ok) ok = ready(&told[i & 7], (uint32_t)(i >> 3));
             j = pieces[tile_no & 3].j;
             j_end = pieces[tile_no & 3].j_end;
           }
@@ -606,6 +613,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           if (w.j == w.j_end) {
             tile_no++;
             pass(&qlanded[tile_no & 3], &qfull[tile_no & 3], (uint32_t)(tile_no >> 2));
+            (void)warp_wait(&told[i & 7], (uint32_t)(i >> 3) & 1u, abort_flag, p.err);
             w = pieces[tile_no & 3];
           }
         }
@@ -687,6 +695,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
       const int b = i & 1;
       const bool first = w.j == w.j_end;
       (void)warp_wait(&sfull[b], (uint32_t)(i >> 1) & 1u, abort_flag, p.err);
+      (void)warp_wait(&told[i & 7], (uint32_t)(i >> 3) & 1u, abort_flag, p.err);
       tc_fence_after();
       if (first) {
         tile_no++;

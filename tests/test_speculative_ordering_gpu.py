@@ -3,11 +3,13 @@
 Each case runs many times, behind other kernels and alone, so that warps come late in different places;
 every result has to be the first one's to the bit, and the first is held to the 64-bit definition.
 """
+import math
 import random
 
 import pytest
 import torch
 
+from g4attn import G4AError
 from spec_ref import Paged, mask_tensor, tree_attn_ref, tree_masks, tree_tolerance
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +73,45 @@ def test_tree_attn_of_several_tiles_to_a_cta_is_the_same_every_time(ctx, fmt, hd
     g = torch.Generator().manual_seed(hd)
     q = (torch.randn((sum(counts), nkh * group, hd), generator=g) * 2).to(fmt).cuda()
     _same_every_time(ctx, case, q, tree_masks(counts, rnd))
+
+
+@pytest.mark.parametrize("hd,fmt", [(128, torch.float32), (256, torch.float16), (512, torch.float16)])
+def test_tree_attn_with_missing_pages_is_the_same_every_time(ctx, hd, fmt):
+    """Which rows of a stage are there, and what a tile's rows see, arrives with the stage: pages that are not there
+    in every other stage, several stages to a CTA, another mask for each tile."""
+    n_seq, group, t, n, page = 40, 4, 8, 1700, 16
+    counts, lens = [t] * n_seq, [n] * n_seq
+    case = Paged(hd, lens, counts, nkh=4, hd=hd, page=page)
+    words = tree_masks(counts, random.Random(hd))
+    gone = [[j for j in range((n - t) // page) if (j // 8 + b) % 2 == 0 and j % 3 == 0] for b in range(n_seq)]
+    for b in range(n_seq):
+        case.table[b, gone[b]] = -1
+    g = torch.Generator().manual_seed(hd)
+    q = (torch.randn((t * n_seq, 4 * group, hd), generator=g) * 2).to(fmt).cuda()
+    mask = mask_tensor(words)
+    first, out = torch.zeros_like(q), torch.zeros_like(q)
+
+    def run(into):
+        _tree(ctx, case, q, mask, into)
+        with pytest.raises(G4AError, match="page id"):
+            ctx.sync()
+
+    run(first)
+    vmax = max(float(v.double().abs().max()) for _, v in case.rows)
+    worst = amp = 0.0
+    for b in (0, 1, n_seq - 1):
+        k, v = (x.double() for x in case.rows[b])
+        keep = torch.tensor([r for r in range(n - t) if r // page not in set(gone[b])])
+        for i in range(t):
+            rows = torch.cat([keep, torch.tensor([n - t + j for j in range(t) if words[b * t + i] >> j & 1])])
+            for h in range(0, 4 * group, 3):
+                qq, kk = q[b * t + i, h].double().cpu(), k[rows, h // group]
+                amp = max(amp, float((kk.abs() @ qq.abs()).max()) * hd ** -0.5 * math.log2(math.e))
+                want = torch.softmax(kk @ qq * hd ** -0.5, 0) @ v[rows, h // group]
+                worst = max(worst, float((first[b * t + i, h].double().cpu() - want).abs().max()))
+    assert worst <= tree_tolerance(amp, hd, n, vmax, fmt == torch.float16)
+    for _ in range(100):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        run(out)
+        assert torch.equal(out, first)
