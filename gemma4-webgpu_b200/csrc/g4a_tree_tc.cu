@@ -93,7 +93,7 @@ struct Tc {
   static constexpr int OFF_VOTE = OFF_BAD + 32;               // [shares][2][4 quarters]
   static constexpr int OFF_INFO = OFF_VOTE + kShares * 32;               // [4] Walk of a piece's begin
   static constexpr int OFF_BAR = OFF_INFO + 4 * 64;
-  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 4 + kShares + 8;
+  static constexpr int NBARS = 3 * UNITS + 8 + 2 + 2 + 2 + 4 + kShares + 8 + 4;
   static constexpr int OFF_END = OFF_BAR + NBARS * 8;
   static constexpr size_t SMEM = 1024 + OFF_END + 16;
   static constexpr uint32_t COL_O = 0, COL_S = MB * N;
@@ -287,6 +287,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
   // [8] stage & 7: the 4 loading warps, when what they have stored for the stage (okw) and for a tile that begins
   // with it (pieces, sees, scales) is there.  The arrivals of their copies say nothing of ordinary stores.
   uint64_t* told = meet_bar + kShares;
+  // [4] tile & 3: the 3 handing-over warps, when badv holds what they have found in the tile's V.  (The MMA's
+  // commit, which comes later, says that products are done, not that others' stores are there.)
+  uint64_t* checked = told + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_END);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_END + 4);
 
@@ -313,6 +316,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
     mbar_init(mend, 1);
     for (int u = 0; u < kShares; u++) mbar_init(&meet_bar[u], 4);
     for (int u = 0; u < 8; u++) mbar_init(&told[u], 4);
+    for (int u = 0; u < 4; u++) mbar_init(&checked[u], 3);
     *abort_flag = 0;
     for (int u = 0; u < 8; u++) badv[u] = 0;
     for (int u = 0; u < 4; u++) pieces[u] = Walk{};  // (what a role reads that had to give up a wait)
@@ -639,6 +643,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
             }
             pass(&landed[unit % UNITS], &full[unit % UNITS], (uint32_t)(unit / UNITS));
           }
+          if ((i == n_stages || before.j + 1 == before.j_end) && lane == 0) mbar_arrive(&checked[tile_before & 3]);
         }
         before = w;
         tile_before = tile_no;
@@ -855,6 +860,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1) tree_tc_kernel(const __grid_con
           __syncwarp();
         }
         (void)warp_wait(pvdone, (uint32_t)i & 1u, abort_flag, p.err);
+        (void)warp_wait(&checked[tile_no & 3], (uint32_t)(tile_no >> 2) & 1u, abort_flag, p.err);
         tc_fence_after();
         if (live > 0) {
           const bool bad = badv[(tile_no + 1) & 7] == ((tile_no + 1) & 0xffff);

@@ -115,3 +115,33 @@ def test_tree_attn_with_missing_pages_is_the_same_every_time(ctx, hd, fmt):
         torch.cuda.synchronize()
         run(out)
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("hd,fmt", [(128, torch.float32), (256, torch.float16)])
+def test_tree_attn_of_non_finite_values_is_the_same_every_time(ctx, hd, fmt):
+    """Infinite V values of drafted rows, in some tiles of a CTA and not in others: exactly the outputs of the tokens
+    that attend to them are infinite, every time."""
+    n_seq, group, t, nkh = 90, 4, 4, 4
+    rnd = random.Random(hd)
+    counts, lens = [t] * n_seq, [t + rnd.randint(0, 100) for _ in range(n_seq)]
+    case = Paged(hd, lens, counts, nkh=nkh, hd=hd, page=16)
+    words = tree_masks(counts, rnd, "star")  # token i sees the root and itself
+    want = torch.zeros((n_seq * t, nkh * group, hd), dtype=torch.bool)
+    for b in range(0, n_seq, 3):
+        i, h, d = 1 + b % (t - 1), b % nkh, b % hd
+        row = lens[b] - t + i
+        case.v[case.table_host[b, row // 16], row % 16, h, d] = float("inf")
+        want[b * t + i, h * group:(h + 1) * group, d] = True
+    g = torch.Generator().manual_seed(hd)
+    q = (torch.randn((n_seq * t, nkh * group, hd), generator=g) * 2).to(fmt).cuda()
+    mask = mask_tensor(words)
+    first, out = torch.zeros_like(q), torch.zeros_like(q)
+    _tree(ctx, case, q, mask, first)
+    ctx.sync()
+    assert torch.equal(torch.isposinf(first).cpu(), want) and not bool(torch.isnan(first).any())
+    for _ in range(100):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        _tree(ctx, case, q, mask, out)
+        ctx.sync()
+        assert torch.equal(out, first)
