@@ -178,7 +178,8 @@ __device__ __forceinline__ Stat block_join(Stat x, Stat* red) {
 }
 
 // The k largest of n keys into kept[0, k), sorted, 0 where there are fewer; key(i) gives the i-th (0:
-// none).  All 256 threads; `low`: values below this key are known not to be among them.
+// none).  All 256 threads; `low`: values below this key are known not to be among them.  A barrier first:
+// where the count of a list that did not fit led here, every thread has read it before it is reset.
 struct alignas(16) TopShared {
   uint64_t list[kList], kept[kMaxPick], tops[kThreadsL];
   uint64_t bound;
@@ -187,6 +188,7 @@ struct alignas(16) TopShared {
 template <typename Key>
 __device__ __forceinline__ void block_top(uint64_t n, int k, uint64_t low, TopShared& sh, Key key) {
   const int tid = threadIdx.x;
+  __syncthreads();
   if (tid < kMaxPick) sh.kept[tid] = 0;
   if (tid == 0) sh.count = 0;
   int have = 0;

@@ -145,3 +145,28 @@ def test_tree_attn_of_non_finite_values_is_the_same_every_time(ctx, hd, fmt):
         _tree(ctx, case, q, mask, out)
         ctx.sync()
         assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("fmt", [torch.float32, torch.float16])
+@pytest.mark.parametrize("allowed", [0, 1, 5, 31])
+@pytest.mark.parametrize("vocab", [20_011, 262_144, 600_001])
+def test_top_k_of_equal_values_is_the_same_every_time(ctx, fmt, allowed, vocab):
+    """Fewer values than are wanted above thousands of equal ones: the short lists of the join overflow, and its threads
+    agree that they did.  Ties go to the lower id."""
+    rows, k = 64, 32
+    g = torch.Generator().manual_seed(vocab + allowed)
+    x = torch.full((rows, vocab), -3.0, dtype=fmt)
+    for r in range(rows):
+        ids = torch.randperm(vocab, generator=g)[:allowed]
+        x[r, ids] = torch.arange(allowed, dtype=fmt) * 0.25
+        if r % 2:
+            x[r][x[r] == -3.0] = -math.inf
+    x = x.cuda()
+    want = x.float().sort(dim=1, descending=True, stable=True)[1][:, :k].int().cpu()
+    val = torch.zeros((rows, k), device="cuda")
+    for _ in range(50):
+        ids = torch.full((rows, k), -9, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        ctx.token_logprobs(x, None, None, None, val, ids)
+        ctx.sync()
+        assert torch.equal(ids.cpu(), want)
