@@ -36,6 +36,9 @@ constexpr int kList = kMaxPick + kMaxPick * kEpt; // the kept values and those a
 constexpr int kMaxSplit = kThreadsL;              // parts of a row: one thread each in the join
 constexpr float kLog2eL = 1.4426950408889634f;
 constexpr float kLn2L = 0.6931471805599453f;
+// Caps up to this size bound a row's maximum so that m log2(e) is rounded by 2^-14 at most, and a first-order
+// correction of the sums leaves less than 2^-29 of that.
+constexpr float kNearCap = 1024.f;
 
 struct LogprobParams {
   const void* logits;
@@ -277,7 +280,12 @@ struct Vec<__half> {
 // measured copy), without the cap 68, without cap and alternatives 66 (0.93).  More CTAs to an SM (fewer
 // registers), or more and shorter parts, were slower.  A few rows are bound by latency, the part's loads and
 // the join's chain (one row 8.7 us, 37 odd f16 rows of 50,257 8.5).
-template <typename T, bool CAP>
+// CAP: 0 no cap, 1 a cap of at most kNearCap, 2 a larger one.  With 1 the exponents are y log2(e) - ml, one
+// multiply-add each, and what rounding left of m log2(e) in ml, the same for all values, is taken out of the
+// sums: 2^-left s, 2^-left (t - left s).  Otherwise the maximum may be huge (a row of which a thread has seen
+// tokens banned by a large negative value alone, say) and that remainder no small correction: the
+// difference y - m comes first, so that the maximum's own exponent is 0.
+template <typename T, int CAP>
 __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobParams p) {
   constexpr int VN = Vec<T>::N, NV = kEpt / VN;
   __shared__ Stat red[kThreadsL / 32];
@@ -292,7 +300,8 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
   const uint32_t lo = max(part * p.part, head);
   const uint32_t hi = min(part * p.part + p.part, p.vocab + head);
   float* seg_max = p.top_k ? p.seg_max + (size_t)row * p.segs : nullptr;
-  const float small = CAP ? kCapRange * p.cap : 3.0e38f;
+  // values that the packed sums take: within the polynomial's range, or (no cap) with finite exponents
+  const float small = CAP ? kCapRange * p.cap : 1.0e38f;
   Stat st = {-INFINITY, 0.f, 0.f};
   // the next segment's values are on their way while this one's are summed
   uint4 raw[NV];
@@ -333,21 +342,20 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
     const float m = fmaxf(st.m, ym);
     if (m > st.m) {
       const float d = st.m == -INFINITY ? 0.f : (st.m - m) * kLog2eL, w = g4a::fast_exp2(d);
-      st.t = w * (st.t + d * st.s);
+      st.t = CAP == 1 || w > 0.f ? w * (st.t + d * st.s) : 0.f;  // (without a near cap d may be -inf)
       st.s *= w;
       st.m = m;
     }
-    // the exponents are y log2(e) - ml; what rounding left of m log2(e) in ml (up to 2e-6, the same for all
-    // values) is taken out of the sums: 2^-left s, 2^-left (t - left s)
     const float mf = m == -INFINITY ? 0.f : m, ml = mf * kLog2eL, left = fmaf(mf, kLog2eL, -ml);
     float s = 0.f, t = 0.f;
-    if (top <= small && low >= -small) {  // finite, and within the polynomial's range
+    if ((CAP ? top : m) <= small && low >= -small) {
       uint64_t s2 = 0, t2 = 0;
-      const uint64_t ic = two(p.inv_cap, p.inv_cap), l2 = two(kLog2eL, kLog2eL), off = two(-ml, -ml);
+      const uint64_t ic = two(p.inv_cap, p.inv_cap), l2 = two(kLog2eL, kLog2eL);
+      const uint64_t off = CAP == 1 ? two(-ml, -ml) : two(-m, -m);
 #pragma unroll
       for (int e = 0; e < kEpt; e += 2) {
-        const uint64_t x2 = two(x[e], x[e + 1]);
-        const uint64_t d2 = fma2(CAP ? capped_small2(x2, ic) : x2, l2, off);
+        const uint64_t x2 = two(x[e], x[e + 1]), y2 = CAP ? capped_small2(x2, ic) : x2;
+        const uint64_t d2 = CAP == 1 ? fma2(y2, l2, off) : mul2(add2(y2, off), l2);
         float d0, d1;
         apart(d2, d0, d1);
         const uint64_t w2 = two(g4a::fast_exp2(d0), g4a::fast_exp2(d1));
@@ -363,15 +371,20 @@ __global__ void __launch_bounds__(kThreadsL) logprob_part_kernel(const LogprobPa
 #pragma unroll
       for (int e = 0; e < kEpt; e++) {
         const float y = CAP ? capped_by(x[e], p.cap, p.inv_cap, p.inv_cap2) : x[e];
-        const float d = fmaf(y, kLog2eL, -ml);
+        const float d = CAP == 1 ? fmaf(y, kLog2eL, -ml) : (y - mf) * kLog2eL;
         const float w = g4a::fast_exp2(d);
         s += w;
         t = fmaf(fmaxf(d, -1000.f), w, t);  // -inf: -1000 * 0
       }
     }
-    const float f = fmaf(-kLn2L, left, 1.0f);
-    st.s = fmaf(f, s, st.s);
-    st.t = fmaf(f, fmaf(-left, s, t), st.t);
+    if constexpr (CAP == 1) {
+      const float f = fmaf(-kLn2L, left, 1.0f);
+      st.s = fmaf(f, s, st.s);
+      st.t = fmaf(f, fmaf(-left, s, t), st.t);
+    } else {
+      st.s += s;
+      st.t += t;
+    }
   }
   st = block_join(st, red);
   if (tid == 0) p.stats[(size_t)row * p.split + part] = make_float4(st.m, st.s, st.t, 0.f);
@@ -563,7 +576,9 @@ g4a_status launch_logprobs(g4a_ctx* ctx, LogprobParams& p) {
   p.stats = static_cast<float4*>(ctx->workspace);
   p.seg_max = reinterpret_cast<float*>(p.stats + parts);
   g4a_prof_scope ps(ctx, G4A_PROF_TOKEN_LOGPROBS);
-  cudaError_t e = g4a_launch(p.cap > 0.f ? logprob_part_kernel<T, true> : logprob_part_kernel<T, false>,
+  cudaError_t e = g4a_launch(p.cap > kNearCap ? logprob_part_kernel<T, 2>
+                             : p.cap > 0.f    ? logprob_part_kernel<T, 1>
+                                              : logprob_part_kernel<T, 0>,
                              dim3((unsigned)parts), dim3(kThreadsL), 0, ctx->stream, true, p);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch logprob_part_kernel");
   e = g4a_launch(logprob_join_kernel<T>, dim3(p.rows), dim3(kThreadsL), 0, ctx->stream, true, p);
