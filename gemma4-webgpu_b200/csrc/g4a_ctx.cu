@@ -60,21 +60,49 @@ g4a_device_guard::~g4a_device_guard() {
 }
 
 g4a_status g4a_ensure_workspace(g4a_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->workspace_bytes) return G4A_OK;
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (bytes <= ctx->workspace_bytes) {
+    if (!ctx->captured) {
+      if (cudaStreamIsCapturing(ctx->stream, &capturing) != cudaSuccess) (void)cudaGetLastError();
+      ctx->captured = capturing != cudaStreamCaptureStatusNone;
+    }
+    return G4A_OK;
+  }
   G4A_CUDA_TRY(cudaStreamIsCapturing(ctx->stream, &capturing));
   if (capturing != cudaStreamCaptureStatusNone)
     return g4a_fail(G4A_EINVAL,
                     "the workspace has to grow to %zu bytes, which a stream capture does not allow: make one call of "
                     "this shape before capturing",
                     bytes);
-  // The old workspace is kept until the context goes: queued kernels, and graphs captured from
-  // earlier calls, still use it.  Each growth at least doubles it, so what is kept stays below
-  // the size of the last one.
-  const size_t want = std::max({bytes, (size_t)1 << 20, 2 * ctx->workspace_bytes});
+  size_t want = std::max(bytes, (size_t)1 << 20);
+  if (ctx->captured) {
+    // Graphs captured from earlier calls still use the old workspace, so it is kept until the context goes.
+    // A growth doubles it where there is memory for that, so that what is kept stays below the size of the
+    // last one.
+    want = std::max(want, 2 * ctx->workspace_bytes);
+    try {
+      ctx->old_workspaces.reserve(ctx->old_workspaces.size() + 1);
+    } catch (...) {
+      return g4a_fail(G4A_ENOMEM, "no host memory for the list of outgrown workspaces");
+    }
+  } else if (ctx->workspace) {
+    // queued kernels may still read it
+    G4A_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
+    cudaFree(ctx->workspace);
+    ctx->workspace = nullptr;
+    ctx->workspace_bytes = 0;
+  }
   void* p = nullptr;
   cudaError_t e = cudaMalloc(&p, want);
-  if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaMalloc(workspace)");
+  if (e == cudaErrorMemoryAllocation && want > bytes) {
+    (void)cudaGetLastError();
+    want = bytes;
+    e = cudaMalloc(&p, want);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();  // (later launches look at the last error)
+    return g4a_cuda_fail(e, "cudaMalloc(workspace)");
+  }
   if (ctx->workspace) ctx->old_workspaces.push_back(ctx->workspace);
   ctx->workspace = p;
   ctx->workspace_bytes = want;

@@ -52,7 +52,8 @@ struct g4a_ctx {
   // ranges.  Grown on demand by the decode entry points (or once by g4a_reserve_workspace).
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
-  std::vector<void*> old_workspaces;  // outgrown ones, which captured graphs may still use
+  bool captured = false;              // a call that uses the workspace has been captured into a graph
+  std::vector<void*> old_workspaces;  // outgrown since then: captured graphs may still use them
   // Per-token kv lengths of a prefill that runs through the decode kernels (grown on demand).
   int* seq_lens = nullptr;
   size_t seq_lens_cap = 0;

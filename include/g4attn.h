@@ -92,7 +92,8 @@ g4a_status g4a_memcpy_d2h(g4a_ctx* ctx, void* dst_host, const void* src_device, 
 g4a_status g4a_memset(g4a_ctx* ctx, void* dst_device, int value, size_t bytes);
 
 /* Pre-size the split-KV partials workspace for up to `max_batch` sequences, so that later
- * decode calls allocate nothing (needed before capturing them into a CUDA graph). */
+ * decode calls allocate nothing (needed before capturing them into a CUDA graph).  It does not size
+ * the workspace for tree attention or log probabilities: make one such call before capturing. */
 g4a_status g4a_reserve_workspace(g4a_ctx* ctx, uint32_t max_batch, uint32_t head_dim,
                                  uint32_t num_q_heads);
 
