@@ -42,6 +42,8 @@
 //   13-15  hand landed units over to the MMA warp (proxy fence), V values checked on the way.
 // Every wait is bounded; a thread that gives up sets the abort flag and the error word, all waits
 // then end at once, and the CTA frees its TMEM and leaves.
+#include <float.h>
+
 #include <algorithm>
 #include <atomic>
 
@@ -62,7 +64,7 @@ constexpr int kShares = kSoftWarps / 4;
 constexpr int kUnit = 32768;         // 128 keys x 128 dims f16
 constexpr float kPUp = 7.0f;         // p = 2^(s - m + 7)
 constexpr float kRaise = 8.0f;       // a score this far above m raises it
-constexpr float kUnseen = -1e30f;    // m of a row that has seen nothing yet (any score raises it)
+constexpr float kUnseen = -FLT_MAX;  // m of a row that has seen nothing yet (any finite score raises it)
 
 template <int HD, int N, bool F32, int R>
 struct Tc {
