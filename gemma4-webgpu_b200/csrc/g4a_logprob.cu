@@ -607,7 +607,8 @@ extern "C" g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint3
   if (tokens_per_row > 0x7fffffffu) return g4a_fail(G4A_EINVAL, "%s: tokens_per_row out of range", fn);
   if (tokens_per_row && (!tokens || !logprob)) return g4a_fail(G4A_EINVAL, "%s: null tokens or logprob", fn);
   if (top_k && (!top_logprob || !top_ids)) return g4a_fail(G4A_EINVAL, "%s: null top_logprob or top_ids", fn);
-  if (!(softcap >= 0.f) || softcap > 1e30f) return g4a_fail(G4A_EINVAL, "%s: softcap must be >= 0 and finite", fn);
+  if (softcap != 0.f && !(softcap >= 1e-30f && softcap <= 1e30f))  // (its reciprocal has to be finite)
+    return g4a_fail(G4A_EINVAL, "%s: softcap must be 0 or in [1e-30, 1e30]", fn);
   if (tokens_per_row == 0 && !entropy && top_k == 0) return G4A_OK;
   g4a_device_guard dev(ctx);
   if (dev.status != G4A_OK) return dev.status;

@@ -457,8 +457,8 @@ g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t format, con
                                uint32_t head_dim, float scale, uint32_t sliding_window, void* out);
 
 /* Log probabilities under rows of logits ([rows, vocab] f32 or f16, row_stride elements from row
- * to row, 0: packed).  softcap c > 0 first caps every logit, y = c tanh(x / c) (Gemma's final
- * logit cap; -inf stays -inf); 0 leaves y = x.  With Z = sum exp(y):
+ * to row, 0: packed).  softcap c in [1e-30, 1e30] first caps every logit, y = c tanh(x / c) (Gemma's
+ * final logit cap; +inf becomes c, -inf stays -inf); 0 leaves y = x.  With Z = sum exp(y):
  *   logprob [rows, tokens_per_row]  y[tokens[r, j]] - log Z of tokens (int32, same shape); token
  *                                   -1 (none) gives 0, another id beyond the vocabulary NaN, which
  *                                   g4a_sync reports
@@ -466,8 +466,9 @@ g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t format, con
  *   top_logprob, top_ids [rows, top_k]  the largest logits in falling order, the lower id first
  *                                   among equal ones, top_k <= 32 and <= vocab
  * logprob / tokens (tokens_per_row 0), entropy (NULL) and the top arrays (top_k 0) may each be
- * left out.  A row with a NaN or +inf, or with no finite logit, has NaN probabilities; a NaN ranks
- * below -inf.  Sums are held in f32.  One call per row count before capturing it into a graph
+ * left out.  A row with a NaN, a +inf that no cap makes finite, or nothing above -inf has NaN
+ * probabilities; a NaN ranks below -inf.  Finite logits of any size have finite results, -inf where the
+ * log probability itself is below f32's range.  Sums are held in f32.  One call per row count before capturing it into a graph
  * (the partial sums live in the context's workspace). */
 #define G4A_MAX_TOP_K 32
 g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint32_t format, const int32_t* tokens,

@@ -25,8 +25,8 @@ def _check(ctx, x, tokens, k, cap=0.0):
     """log p = (y - m) - ln S: two roundings of 2^-24 of its parts (the difference, log p), so 2^-22 |log p| at most, and
     the error of ln S, that of S relative: exponents off by 2^-24 |d| with weights e^d, of which sum |d| e^d <= S ln V,
     exp2 2^-22, f32 sums of less than 64 terms in sequence and in trees 2^-20 - together below 2^-18 for ln V <= 13.  The
-    entropy ln S - T / S has T / S <= ln V, T and S as exact as S above: 2^-18 (1 + ln V).  A cap's tanh is off by 2^-22 of
-    the cap for a value and its maximum each."""
+    entropy ln S - T / S has T / S <= ln V, T and S as exact as S above: 2^-18 (1 + ln V).  A capped
+    logit is off by 2^-22 of the largest in its row, and so is the maximum."""
     rows, vocab = x.shape
     lp = torch.full(tokens.shape, 9.0, device="cuda")
     ent = torch.full((rows,), 9.0, device="cuda")
@@ -36,13 +36,15 @@ def _check(ctx, x, tokens, k, cap=0.0):
     ctx.sync()
     rlp, rent, rtv, rti = _reference(x.cpu(), tokens.cpu(), k, cap)
     assert torch.equal(ti.cpu().long(), rti)
-    y = 2.0 ** -18 + cap * 2.0 ** -21
+    raw = x.cpu().double()
+    size = (cap * torch.tanh(raw / cap)).abs().amax(1, keepdim=True) if cap else torch.zeros((rows, 1))
+    tol = 2.0 ** -18 + size * 2.0 ** -21
     for got, want in ((lp, rlp), (tv, rtv)):
         got = got.cpu().double()
         want = want.float().double()  # (below f32's range: -inf)
         same = got == want
-        assert bool((same | ((got - want).abs() <= y + want.abs() * 2.0 ** -22)).all()), (got, want)
-    assert bool(((ent.cpu().double() - rent).abs() <= (2.0 ** -18 + cap * 2.0 ** -21) * (1 + math.log(vocab))).all()), (ent, rent)
+        assert bool((same | ((got - want).abs() <= tol + want.abs() * 2.0 ** -22)).all()), (got, want)
+    assert bool(((ent.cpu().double() - rent).abs() <= tol[:, 0] * (1 + math.log(vocab))).all()), (ent, rent)
 
 
 def _tokens(rows, vocab, ids):
@@ -97,3 +99,13 @@ def test_logprobs_under_a_large_cap(ctx, cap):
     x[2] -= cap * 3
     x[3, :29_000] = LOWEST
     _check(ctx, x.cuda(), _tokens(4, vocab, [9_999, 3, 11, 29_500]), 8, cap)
+
+
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 30.0, 1e30])
+def test_logprobs_under_the_smallest_and_largest_caps(ctx, cap):
+    """An infinite logit is the cap's value, among finite ones."""
+    vocab = 9_001
+    x = torch.randn((2, vocab), generator=torch.Generator().manual_seed(4)) * 4
+    x[1, 4_000] = math.inf
+    x[1, 5_000] = 0.0
+    _check(ctx, x.cuda(), _tokens(2, vocab, [9_000, 4_000]), 8, cap)

@@ -121,3 +121,8 @@ def test_binding_checks_without_a_gpu():
         _rows_addr(t(3, 8, dtype=torch.float16), "x", torch.float32, 8, 0)
     with pytest.raises(ValueError):
         _rows_addr(torch.zeros(3, 8), "x", torch.float32, 8, 0)
+
+
+@pytest.mark.parametrize("cap", [1e-40, 1e-31, 2e30, -1e-30])
+def test_logprob_refuses_a_cap_whose_reciprocal_is_not_finite(cap):
+    refused("g4a_token_logprobs", changed(LOGP, cap=cap), "softcap")
