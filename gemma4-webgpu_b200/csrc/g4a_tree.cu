@@ -190,8 +190,10 @@ extern "C" g4a_status g4a_tree_attn_paged(g4a_ctx* ctx, const void* q, uint32_t 
   if (head_dim == 0 || head_dim > 512 || (head_dim % 8) != 0)
     return g4a_fail(G4A_EINVAL, "%s: head_dim %u must be a multiple of 8 in [8, 512]", fn, head_dim);
   if (max_tokens == 0 || max_tokens > (uint32_t)kMaxTokens)
-    return g4a_fail(G4A_EINVAL, "%s: max_tokens %u not in [1, %d] (longer prompts: g4a_prefill_attn)", fn, max_tokens,
-                    kMaxTokens);
+    return g4a_fail(G4A_EINVAL,
+                    "%s: max_tokens %u not in [1, %d] (a longer prompt: several calls, or g4a_prefill_attn over a "
+                    "contiguous cache)",
+                    fn, max_tokens, kMaxTokens);
   if (batch == 0 || num_tokens == 0) return G4A_OK;
   if (batch > 0x00ffffffu || num_tokens > 0x7fffffffu)
     return g4a_fail(G4A_EINVAL, "%s: batch %u or num_tokens %u too large", fn, batch, num_tokens);

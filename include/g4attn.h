@@ -438,7 +438,8 @@ g4a_status g4a_paged_qkv_prep(g4a_ctx* ctx, const float* q, const float* k, cons
  * position base + (ancestors).  A token that sees nothing gets zeros.  f32 queries keep f32
  * accuracy (as g4a_decode_attn); f16 queries round the softmax weights to f16.
  * kv head of q head h is h*num_kv_heads/num_q_heads; num_q_heads must be a multiple of
- * num_kv_heads.  max_tokens (1..64) bounds T for every sequence.  q_indptr, kv_lens, page_table
+ * num_kv_heads.  max_tokens (1..64) bounds T for every sequence; a longer prompt takes several calls,
+ * each with kv_lens at the end of its chunk (rows of later chunks may be in the pages already).  q_indptr, kv_lens, page_table
  * and tree_mask are device arrays; host_kv_lens (may be NULL) is an optional host copy used only
  * to size the launch.  A sequence whose q_indptr is not increasing within [0, num_tokens], with T
  * > max_tokens, kv_lens[b] < T or kv_lens[b] beyond max_pages_per_seq*page_size is skipped (its
@@ -480,7 +481,8 @@ g4a_status g4a_token_logprobs(g4a_ctx* ctx, const void* logits, uint32_t format,
  * row base_lens[b] + path[b*max_path + i] becomes row base_lens[b] + i of k_pages and v_pages, as
  * if all rows were read before any is written.  path (device, int32 [batch, max_path]) holds
  * indices of drafted tokens, max_path <= 64.  Entries out of range are skipped and reported by
- * g4a_sync, as are sequences with path_lens[b] > max_path or a negative base. */
+ * g4a_sync, as are sequences with path_lens[b] > max_path or a negative base; an entry whose row stays
+ * where it is (path[i] = i) is not looked at. */
 g4a_status g4a_paged_kv_compact(g4a_ctx* ctx, uint16_t* k_pages, uint16_t* v_pages,
                                 const int32_t* page_table, const int32_t* base_lens, const int32_t* path,
                                 const int32_t* path_lens, uint32_t batch, uint32_t max_path,
