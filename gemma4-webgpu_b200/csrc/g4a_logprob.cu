@@ -277,7 +277,9 @@ struct Vec<__half> {
 // either end of the row is read value by value, so nothing outside the row is read.  No thread
 // waits for another before the end of the part.
 // 384 rows of 262,144 f32 logits, capped, with 8 alternatives: the call takes 78 us, 5.2 TB/s (0.79 of the
-// measured copy), without the cap 68, without cap and alternatives 66 (0.93).  More CTAs to an SM (fewer
+// measured copy), without the cap 68, without cap and alternatives 65 (0.95); f16 logits 75 and 48.  (In short runs;
+// after 10 ms of them the power limit lowers the clock to 1,715 MHz and 78 becomes 89.)  Rows with banned tokens
+// leave the packed sums where there is a cap: 120.  More CTAs to an SM (fewer
 // registers), or more and shorter parts, were slower.  A few rows are bound by latency, the part's loads and
 // the join's chain (one row 8.7 us, 37 odd f16 rows of 50,257 8.5).
 // CAP: 0 no cap, 1 a cap of at most kNearCap, 2 a larger one.  With 1 the exponents are y log2(e) - ml, one

@@ -96,8 +96,9 @@ __device__ __forceinline__ float warp_sum(float x) {
 // Bound by HBM for many tokens and by latency for few, so a warp takes two neighbouring heads of a
 // token, reads its cos / sin row once for both, and issues every load that needs no other one (both
 // heads, angles, sequence, slot) before it waits for the first; only the page id has to follow.
-// (7,490 tokens of 10 heads of 256 dims, q to f16: 25.6 us, 4.8 TB/s, 0.73 of the measured copy; one head
-// per warp that first looked at the token's sequence 36.  A decode step's token: 2.6 us.)
+// (7,491 tokens of 10 heads of 256 dims, q to f16: 25.4 us, 4.8 TB/s, 0.74 of the measured copy: a warp loads
+// once, waits and leaves, 6.3 waves of CTAs, with 62 % of the issue slots used.  One head per warp that first
+// looked at the token's sequence 36.  A decode step's token: 2.4 us.)
 // VEC > 0: hd = 64 VEC, a lane holds VEC consecutive elements of each half, in vector loads and
 // stores (16 bytes at hd >= 256).  VEC = 0: any even hd <= 512 and any alignment, elements
 // strided by 32 lanes.

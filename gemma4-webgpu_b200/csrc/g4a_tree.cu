@@ -25,11 +25,6 @@ namespace {
 using namespace g4a;
 using namespace g4a_tree;
 
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // Joins the parts of the tiles that were cut between CTAs.  The work is cut into units spread over all
 // CTAs.  A thread is a float4 column of a row and a lane over its parts, which it loads four at a time and
 // folds with a running maximum; the lanes of a row, if there are several, meet in shared memory.  What

@@ -356,6 +356,12 @@ __device__ __forceinline__ int deal(const TreeParams& p, const int2 own, const i
   return n_stages;
 }
 
+// Two floats rounded to an f16 pair.
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // What query row r of a tile's sequence sees: prefix rows [kmin, base) and the drafted rows of
 // `bits`.  Of the base + popcount(mask) rows in its list only the last W stay.
 struct Sees {

@@ -16,7 +16,9 @@
 // KB (48 cycles; 8 KB and 64 at N 128), so a stage of 64 columns moves 393 KB of operands and 256 KB of
 // copies, 5,100 cycles.  So one tile per kv head is bound by HBM and many by shared memory:
 //   8 tokens x 8 heads of 512 dims over 131,000 keys, f16: 69 us, 3.9 TB/s (0.59 of the measured copy)
-//   48 tokens, six tiles: 183 us, 564 TFLOP/s, 6,700 cycles a stage
+//   48 tokens, six tiles: 183 us, 564 TFLOP/s, 6,700 cycles a stage (201 us at the clock that the power limit
+//   leaves after some 10 ms of such calls one after another, 1,760 MHz)
+//   the same with f32 queries, 32 rows to a tile: 81 us and 336 us
 // Below 512 dims the softmax warps' serial chain, S -> registers -> vote -> exp2 -> P, is longer than the
 // products: 3,600 cycles at 32 rows a warp (8 tiles of 256 dims over 32k keys: 4,900 a stage, 60 us), 1,950 at 16
 // (32 chains of up to 7 tokens x 3 heads of 128 dims, 3,000 keys: 2,830 a stage, which is the HBM share; 44 us).
@@ -73,7 +75,8 @@ struct Tc {
   static constexpr int W = ROWS / kShares;            // rows of a softmax warp (its share)
   // Registers: 512 threads start with 128 each (65,536); the softmax warps, which hold a block of
   // scores and the row sums, take some from the others.  (Spills are dear here: shared memory leaves
-  // the L1 almost nothing, so local memory is in the L2.)
+  // the L1 almost nothing, so local memory is in the L2.  The two f32 instances of 64 rows store 36 and 40
+  // bytes a thread, the others none.)
   static constexpr int REGS_SOFT = 160, REGS_LOAD = 112, REGS_MMA = 80;
   static_assert(kSoftWarps * 32 * REGS_SOFT + 128 * REGS_LOAD + 128 * REGS_MMA <= kThreadsTc * 128, "register file");
   static constexpr int Q_BYTES = N * HD * 2;
@@ -127,10 +130,6 @@ __device__ __forceinline__ bool clear_non_finite(uint32_t& w) {
   if ((w & 0x7c000000u) == 0x7c000000u) keep &= 0x0000ffffu;
   w &= keep;
   return keep != 0xffffffffu;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 // 16 or 32 consecutive TMEM columns of this warp's 32 lanes; the registers may be used after
 // tmem_landed() has named them.
