@@ -1,0 +1,135 @@
+// Attention of a chunk of new tokens of every sequence over a paged cache (g4a_chunk_attn_paged).  No reference
+// counterpart; the semantics of one token are those of shaders/attn_score.wgsl, softmax.wgsl and
+// attn_output.wgsl over the rows that it sees, with a few first rows beside the window.
+#include <algorithm>
+#include <cmath>
+
+#include "g4a_chunk.cuh"
+
+namespace {
+
+using namespace g4a;
+using namespace g4a_chunk;
+
+// One warp per (token, q head), a lane holds up to 16 dims; one pass over the rows with a running maximum and sum.
+__global__ void __launch_bounds__(256) chunk_simple_kernel(const ChunkParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long cap = (long long)p.max_pages * p.page_size;
+  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int token = (int)(unit / p.nqh), head = (int)(unit % p.nqh);
+  if (token >= p.tokens) return;
+  for (int b = 0; b < p.batch; b++) {
+    const Seq s = seq_of(p, b, cap);
+    if (token < s.row0 || token >= s.row0 + s.T) continue;
+    const int pos = s.base() + token - s.row0, kvh = head / p.group;
+    float q[16], o[16], m = -INFINITY, l = 0.f;
+    const size_t row = (size_t)token * p.nqh + head;
+    for (int e = 0; e < 16; e++) {
+      const int d = e * 32 + lane;
+      q[e] = d < p.hd ? __half2float(p.q[row * p.hd + d]) : 0.f;
+      o[e] = 0.f;
+    }
+    const int lo = first_in_window(p, pos);
+    for (int r = 0; r <= pos; r++) {
+      if (r < lo && (uint32_t)r >= p.sinks) r = lo;
+      const long long off = row_offset(p, b, kvh, r);
+      if (off < 0) continue;
+      float x = 0.f;
+      for (int e = 0; e < 16; e++) {
+        const int d = e * 32 + lane;
+        if (d < p.hd) x = fmaf(q[e], __half2float(p.k[off + d]), x);
+      }
+      for (int w = 16; w >= 1; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+      x *= p.scale_log2;
+      const float mn = fmaxf(m, x);
+      const float f = m == mn ? 1.f : exp2f(m - mn), w = exp2f(x - mn);
+      m = mn;
+      l = l * f + w;
+      for (int e = 0; e < 16; e++) {
+        const int d = e * 32 + lane;
+        if (d < p.hd) o[e] = o[e] * f + w * __half2float(p.v[off + d]);
+      }
+    }
+    for (int e = 0; e < 16; e++) {
+      const int d = e * 32 + lane;
+      if (d < p.hd) p.out[row * p.hd + d] = __float2half_rn(l == 0.f ? 0.f : o[e] / l);
+    }
+    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2C;
+  }
+}
+
+}  // namespace
+
+g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, ChunkParams& p, const uint16_t* q, const uint16_t* k_pages,
+                            const uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                            const int32_t* q_indptr, uint32_t num_tokens, uint32_t batch, uint32_t page_size,
+                            uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_q_heads,
+                            uint32_t num_kv_heads, uint32_t head_dim, float scale, uint32_t sliding_window,
+                            uint32_t sink_tokens) {
+  if (num_q_heads == 0 || num_kv_heads == 0 || num_q_heads % num_kv_heads != 0 || num_q_heads > 65536u)
+    return g4a_fail(G4A_EINVAL, "%s: num_q_heads %u must be a multiple of num_kv_heads %u", fn, num_q_heads,
+                    num_kv_heads);
+  if (head_dim == 0 || head_dim > 512 || (head_dim % 8) != 0)
+    return g4a_fail(G4A_EINVAL, "%s: head_dim %u must be a multiple of 8 in [8, 512]", fn, head_dim);
+  if (!std::isfinite(scale)) return g4a_fail(G4A_EINVAL, "%s: scale is not finite", fn);
+  if (batch > 0x00ffffffu || num_tokens > 0x7fffffffu || (uint64_t)num_tokens * num_q_heads > 0x7fffffffu)
+    return g4a_fail(G4A_EINVAL, "%s: batch %u or num_tokens %u too large", fn, batch, num_tokens);
+  if (page_size == 0 || max_pages_per_seq == 0 || num_pages == 0 || num_pages > 0x7fffffffu)
+    return g4a_fail(G4A_EINVAL, "%s: page_size, max_pages_per_seq or num_pages out of range", fn);
+  if ((uint64_t)page_size * max_pages_per_seq > 0x7fff0000ull)
+    return g4a_fail(G4A_EINVAL, "%s: page_size * max_pages_per_seq exceeds 2^31", fn);
+  if (batch == 0 || num_tokens == 0) return G4A_OK;
+  if (!q || !k_pages || !v_pages || !page_table || !kv_lens || !q_indptr)
+    return g4a_fail(G4A_EINVAL, "%s: null pointer", fn);
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) & 15u)
+    return g4a_fail(G4A_EINVAL, "%s: q and the page pools must be 16-byte aligned", fn);
+  p.q = reinterpret_cast<const __half*>(q);
+  p.k = reinterpret_cast<const __half*>(k_pages);
+  p.v = reinterpret_cast<const __half*>(v_pages);
+  p.page_table = page_table;
+  p.kv_lens = kv_lens;
+  p.q_indptr = q_indptr;
+  p.tokens = (int)num_tokens;
+  p.batch = (int)batch;
+  p.page_size = (int)page_size;
+  p.max_pages = (int)max_pages_per_seq;
+  p.num_pages = (int)num_pages;
+  p.nqh = (int)num_q_heads;
+  p.nkh = (int)num_kv_heads;
+  p.group = (int)(num_q_heads / num_kv_heads);
+  p.hd = (int)head_dim;
+  p.scale_log2 = scale * kLog2eC;
+  p.window = sliding_window;
+  p.sinks = sink_tokens;
+  p.err = ctx->dev_err_dev;
+  return G4A_OK;
+}
+
+extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t* k_pages,
+                                           const uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                                           const int32_t* q_indptr, uint32_t num_tokens, uint32_t batch,
+                                           uint32_t page_size, uint32_t max_pages_per_seq, uint32_t num_pages,
+                                           uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                                           float scale, uint32_t sliding_window, uint32_t sink_tokens, float* lse,
+                                           uint16_t* out) {
+  G4A_CHECK_CTX(ctx);
+  const char* fn = "g4a_chunk_attn_paged";
+  ChunkParams p = {};
+  if (g4a_status s = g4a_chunk_params(fn, ctx, p, q, k_pages, v_pages, page_table, kv_lens, q_indptr, num_tokens, batch,
+                                      page_size, max_pages_per_seq, num_pages, num_q_heads, num_kv_heads, head_dim,
+                                      scale, sliding_window, sink_tokens))
+    return s;
+  if (batch == 0 || num_tokens == 0) return G4A_OK;
+  if (!out) return g4a_fail(G4A_EINVAL, "%s: null pointer", fn);
+  if ((uintptr_t)out & 15u) return g4a_fail(G4A_EINVAL, "%s: out must be 16-byte aligned", fn);
+  g4a_device_guard dev(ctx);
+  if (dev.status != G4A_OK) return dev.status;
+  p.lse = lse;
+  p.out = reinterpret_cast<__half*>(out);
+  g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
+  const long long units = (long long)num_tokens * num_q_heads;
+  const cudaError_t e =
+      g4a_launch(chunk_simple_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, ctx->stream, false, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_simple_kernel");
+  return G4A_OK;
+}

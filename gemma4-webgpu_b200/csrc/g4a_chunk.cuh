@@ -1,0 +1,72 @@
+// What the kernels of a long-context step share (g4a_chunk_attn_paged, g4a_paged_key_mass): the shapes of a call,
+// a sequence's place in them, and which rows a token sees.
+#pragma once
+
+#include "g4a_internal.cuh"
+
+namespace g4a_chunk {
+
+constexpr float kLog2eC = 1.4426950408889634f;
+constexpr float kLn2C = 0.6931471805599453f;
+
+struct ChunkParams {
+  const __half* q;  // [tokens, nqh, hd]
+  const __half *k, *v;  // page pools [num_pages, page_size, nkh, hd]
+  const int *page_table, *kv_lens, *q_indptr;
+  int tokens, batch;
+  int page_size, max_pages, num_pages;
+  int nqh, nkh, group, hd;  // group = nqh / nkh
+  float scale_log2;         // scale * log2(e)
+  uint32_t window, sinks;
+  int* err;
+  __half* out;       // attention: [tokens, nqh, hd]
+  float* lse;        // attention: written, may be null; masses: read
+  float* mass;       // masses: [batch, nkh, mass_stride]
+  long long mass_stride;
+  float decay;
+};
+
+// One sequence: T new tokens (rows row0 .. of q), which are the last of its L rows.  T = 0 and L = 0: nothing to
+// do (also for a sequence that does not fit together, which is reported).
+struct Seq {
+  int row0, T, L;
+  __device__ __forceinline__ int base() const { return L - T; }
+};
+
+__device__ __forceinline__ Seq seq_of(const ChunkParams& p, int b, long long cap) {
+  const int r0 = p.q_indptr[b], r1 = p.q_indptr[b + 1], L = p.kv_lens[b];
+  if (r0 < 0 || r1 < r0 || r1 > p.tokens || L < r1 - r0 || L > cap) {
+    atomicExch(p.err, G4A_DEVERR_TREE);
+    return Seq{0, 0, 0};
+  }
+  return Seq{r0, r1 - r0, L};
+}
+
+// The token of row `pos` sees the rows r <= pos with r >= first_in_window(pos) or r < sinks.
+__device__ __forceinline__ int first_in_window(const ChunkParams& p, int pos) {
+  return p.window != 0u && (uint32_t)pos >= p.window ? pos + 1 - (int)p.window : 0;
+}
+__device__ __forceinline__ bool sees(const ChunkParams& p, int pos, int r) {
+  return r <= pos && (r >= first_in_window(p, pos) || (uint32_t)r < p.sinks);
+}
+
+// Element offset of cache row `key` of sequence b and kv head kvh, or -1 for a bad page id.
+__device__ __forceinline__ long long row_offset(const ChunkParams& p, int b, int kvh, int key) {
+  const int j = key / p.page_size;
+  const int page = p.page_table[(size_t)b * p.max_pages + j];
+  if (page < 0 || page >= p.num_pages) {
+    atomicExch(p.err, G4A_DEVERR_PAGE);
+    return -1;
+  }
+  return (((long long)page * p.page_size + (key - j * p.page_size)) * p.nkh + kvh) * p.hd;
+}
+
+}  // namespace g4a_chunk
+
+// Checks of the arguments that the two entry points share; fills p but for what each of them adds.
+g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, g4a_chunk::ChunkParams& p, const uint16_t* q,
+                            const uint16_t* k_pages, const uint16_t* v_pages, const int32_t* page_table,
+                            const int32_t* kv_lens, const int32_t* q_indptr, uint32_t num_tokens, uint32_t batch,
+                            uint32_t page_size, uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_q_heads,
+                            uint32_t num_kv_heads, uint32_t head_dim, float scale, uint32_t sliding_window,
+                            uint32_t sink_tokens);

@@ -31,6 +31,9 @@ enum g4a_prof_label : int {
   G4A_PROF_TREE_ATTN,
   G4A_PROF_TREE_MERGE,
   G4A_PROF_TOKEN_LOGPROBS,
+  G4A_PROF_CHUNK_ATTN,
+  G4A_PROF_KEY_MASS,
+  G4A_PROF_PAGED_EVICT,
   G4A_PROF_NUM_LABELS
 };
 extern const char* const g4a_prof_names[G4A_PROF_NUM_LABELS];

@@ -468,6 +468,62 @@ class Context:
              _addr(path, "path", i32, 0, dev), _addr(path_lens, "path_lens", i32, batch, dev), batch, shape[1], page_size,
              max_pages, num_pages, num_kv_heads, head_dim)
 
+    # ---------------------------------------------------------------- long contexts, paged cache
+    def chunk_attn_paged(self, q, k_pages, v_pages, page_table, kv_lens, q_indptr, out, lse=None, *, num_q_heads,
+                         num_kv_heads, head_dim, page_size, scale=1.0, sliding_window=0, sink_tokens=0) -> None:
+        """Attention of a chunk of new tokens of every sequence over the paged cache, causal or a sliding window
+        beside the first sink_tokens rows (g4a_chunk_attn_paged).  q and out f16 [tokens, heads, dims]; lse f32
+        [tokens, heads], the log-sum-exps that paged_key_mass takes."""
+        dev = self.device
+        f32, f16, i32, _ = _dtypes()
+        kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
+                                                                 page_size)
+        n, size = q.shape[0], q.numel()
+        if size != n * num_q_heads * head_dim:
+            raise ValueError(f"q must be [tokens, {num_q_heads}, {head_dim}], got {tuple(q.shape)}")
+        call("g4a_chunk_attn_paged", self._h, _addr(q, "q", f16, 0, dev), kp, vp, table,
+             _addr(kv_lens, "kv_lens", i32, batch, dev), _addr(q_indptr, "q_indptr", i32, batch + 1, dev), n, batch,
+             page_size, max_pages, num_pages, num_q_heads, num_kv_heads, head_dim, scale, sliding_window, sink_tokens,
+             None if lse is None else _addr(lse, "lse", f32, n * num_q_heads, dev), _addr(out, "out", f16, size, dev))
+
+    def _mass(self, mass, batch, num_kv_heads):
+        """Checks the rows' weights f32 [batch, num_kv_heads, rows]; returns their address and the row count."""
+        shape = mass.shape
+        if len(shape) != 3 or shape[0] != batch or shape[1] != num_kv_heads:
+            raise ValueError(f"mass must be [{batch}, {num_kv_heads}, rows], got {tuple(shape)}")
+        return _addr(mass, "mass", _dtypes()[0], 0, self.device), shape[2]
+
+    def paged_key_mass(self, q, lse, k_pages, page_table, kv_lens, q_indptr, mass, *, num_q_heads, num_kv_heads,
+                       head_dim, page_size, scale=1.0, sliding_window=0, sink_tokens=0, decay=1.0) -> None:
+        """The attention weight that each cached row got from the chunk's tokens, added to decay * mass
+        (g4a_paged_key_mass).  q and lse as in chunk_attn_paged; mass f32 [batch, kv heads, rows]."""
+        dev = self.device
+        f32, f16, i32, _ = _dtypes()
+        kp, _, table, batch, max_pages, num_pages = self._pages(k_pages, k_pages, page_table, num_kv_heads, head_dim,
+                                                                page_size)
+        n = q.shape[0]
+        if q.numel() != n * num_q_heads * head_dim:
+            raise ValueError(f"q must be [tokens, {num_q_heads}, {head_dim}], got {tuple(q.shape)}")
+        m, stride = self._mass(mass, batch, num_kv_heads)
+        call("g4a_paged_key_mass", self._h, _addr(q, "q", f16, 0, dev), _addr(lse, "lse", f32, n * num_q_heads, dev), kp,
+             table, _addr(kv_lens, "kv_lens", i32, batch, dev), _addr(q_indptr, "q_indptr", i32, batch + 1, dev), n,
+             batch, page_size, max_pages, num_pages, num_q_heads, num_kv_heads, head_dim, scale, sliding_window,
+             sink_tokens, decay, m, stride)
+
+    def paged_kv_evict(self, k_pages, v_pages, page_table, kv_lens, mass, new_lens, kept=None, *, budget, sink_tokens=0,
+                       recent_tokens=0, num_kv_heads, head_dim, page_size) -> None:
+        """Every sequence down to `budget` rows per kv head: the first, the latest and the heaviest
+        (g4a_paged_kv_evict).  kept int32 [batch, kv heads, budget] gets the rows' old numbers."""
+        dev = self.device
+        i32 = _dtypes()[2]
+        kp, vp, table, batch, max_pages, num_pages = self._pages(k_pages, v_pages, page_table, num_kv_heads, head_dim,
+                                                                 page_size)
+        m, stride = self._mass(mass, batch, num_kv_heads)
+        call("g4a_paged_kv_evict", self._h, kp, vp, table, _addr(kv_lens, "kv_lens", i32, batch, dev), m, stride, batch,
+             budget, sink_tokens, recent_tokens, page_size, max_pages, num_pages, num_kv_heads, head_dim,
+             _addr(new_lens, "new_lens", i32, batch, dev),
+             None if kept is None else _addr(kept, "kept", i32, batch * num_kv_heads * budget, dev))
+
     # ---------------------------------------------------------------- memory and IPC
     def alloc(self, nbytes: int) -> int:
         """Device allocation through the library (cudaMalloc); returns the address."""

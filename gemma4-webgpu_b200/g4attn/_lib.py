@@ -88,6 +88,9 @@ SIGNATURES: dict[str, list] = {
     "g4a_tree_attn_paged": [_p, _p, _u32] + [_p] * 7 + [_u32] * 9 + [_f, _u32, _p],
     "g4a_token_logprobs": [_p, _p, _u32, _p, _u32, _u32, _u64, _u32, _u32, _f, _p, _p, _p, _p],
     "g4a_paged_kv_compact": [_p] * 7 + [_u32] * 7,
+    "g4a_chunk_attn_paged": [_p] * 7 + [_u32] * 8 + [_f, _u32, _u32, _p, _p],
+    "g4a_paged_key_mass": [_p] * 7 + [_u32] * 8 + [_f, _u32, _u32, _f, _p, _u64],
+    "g4a_paged_kv_evict": [_p] * 6 + [_u64] + [_u32] * 9 + [_p, _p],
     "g4a_ipc_get_handle": [_p, _p, _p],
     "g4a_ipc_open_handle": [_p, _p, POINTER(c_void_p)],
     "g4a_ipc_close_handle": [_p, _p],

@@ -489,6 +489,71 @@ g4a_status g4a_paged_kv_compact(g4a_ctx* ctx, uint16_t* k_pages, uint16_t* v_pag
                                 uint32_t page_size, uint32_t max_pages_per_seq, uint32_t num_pages,
                                 uint32_t num_kv_heads, uint32_t head_dim);
 
+/* ------------------------------------------------------------------ long contexts, paged cache */
+
+/* A prompt that comes in pieces, sliding layers that keep their first tokens in sight, and caches that are
+ * kept to a budget of rows (no reference counterpart: the reference decodes one token at a time over
+ * all of its cache).  Per step and layer:
+ *   g4a_paged_qkv_prep     (above, q to f16) the new tokens appended to the pages
+ *   g4a_chunk_attn_paged   their attention over the prefix and themselves, and its log-sum-exps
+ *   g4a_paged_key_mass     the weight that every cached row got from them, added to what it had
+ * and whenever a cache is to shrink
+ *   g4a_paged_kv_evict     the rows with the most weight kept, moved together; positions go on from where
+ *                          they were, kv_lens become new_lens (slot and position are separate arguments)
+ *
+ * Shapes of the three.  Sequence b's T new tokens are rows q_indptr[b] .. q_indptr[b+1]-1 of q (f16
+ * [num_tokens, num_q_heads, head_dim]); any T, 0 and 1 among them.  Its cache holds kv_lens[b] = L rows,
+ * the last T of which are these tokens' own.  Token i has row p = L - T + i and sees the rows r <= p
+ * with r > p - sliding_window (all where sliding_window is 0) or r < sink_tokens.  kv head of q head h is
+ * h*num_kv_heads/num_q_heads; num_q_heads must be a multiple of num_kv_heads; head_dim a multiple of
+ * 8, <= 512; any page_size.  q_indptr, kv_lens and page_table are device arrays, read when the kernels
+ * run.  A sequence whose q_indptr is not increasing within [0, num_tokens], with kv_lens[b] < T or
+ * beyond max_pages_per_seq*page_size is skipped (what it would write stays as it was) and g4a_sync
+ * reports it; so do page ids out of range, whose rows count as not there.  Partial results live in the
+ * context's workspace: before capturing a call into a graph, make one of the same shape, and do not let
+ * graphs captured from one context run at the same time. */
+
+/* out (f16, like q) = softmax(scale q K^T) V over the rows that a token sees, and lse (f32
+ * [num_tokens, num_q_heads], may be NULL) = log sum exp(scale q k) over them.  A token that sees nothing
+ * gets zeros and an lse of -inf.  Softmax weights are rounded to f16 for their product with V, sums are held in
+ * f32.  Rows of out and lse behind the last sequence stay as they were.  A value that is not finite in a
+ * row of the cache reaches only the tokens that see that row.  f32 queries: g4a_tree_attn_paged. */
+g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
+                                const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_indptr,
+                                uint32_t num_tokens, uint32_t batch, uint32_t page_size,
+                                uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_q_heads,
+                                uint32_t num_kv_heads, uint32_t head_dim, float scale, uint32_t sliding_window,
+                                uint32_t sink_tokens, float* lse, uint16_t* out);
+
+/* mass (f32, entry (b, h, r) at (b*num_kv_heads + h)*mass_stride + r) of the rows r < kv_lens[b]:
+ *   mass = decay * mass + sum over the tokens and the kv head's q heads of exp(scale q k_r - lse)
+ * over those that see r, with q and lse as in g4a_chunk_attn_paged.  The T new rows start from 0, whatever
+ * their entries held; decay 0 does the same for all rows.  0 <= decay <= 1.  mass_stride >= the largest
+ * kv_lens[b] (a longer sequence is skipped and reported); entries behind kv_lens[b] stay as they were.
+ * A q row whose lse is -inf adds nothing; a call without tokens (num_tokens 0) does nothing.  Sums are f32 in an order that does not change from run to run. */
+g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const float* lse, const uint16_t* k_pages,
+                              const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_indptr,
+                              uint32_t num_tokens, uint32_t batch, uint32_t page_size,
+                              uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_q_heads,
+                              uint32_t num_kv_heads, uint32_t head_dim, float scale, uint32_t sliding_window,
+                              uint32_t sink_tokens, float decay, float* mass, uint64_t mass_stride);
+
+/* Brings every sequence with more than `budget` rows down to it.  For each kv head by itself: the first
+ * sink_tokens and the last recent_tokens rows stay, and of those between the budget - sink_tokens -
+ * recent_tokens with the largest mass, the earlier one first among equals (a NaN ranks below all).  Kept row
+ * number i becomes row i of that kv head in k_pages, v_pages and mass, in the order that they had, as if all
+ * rows were read before any is written; what lies behind row `budget` stays as it was.  new_lens
+ * (int32 [batch], not kv_lens itself) gets min(kv_lens[b], budget); kept (int32 [batch, num_kv_heads,
+ * budget], may be NULL) the rows' old numbers, -1 behind them.  1 <= budget, sink_tokens + recent_tokens
+ * <= budget.  kv_lens[b] outside [0, min(max_pages_per_seq*page_size, mass_stride)] skips the sequence and
+ * reports it (its new_lens entry becomes kv_lens[b]); a row on a page whose id is out of range is neither read nor
+ * written, and reported.  Pages that two sequences share must not be evicted from. */
+g4a_status g4a_paged_kv_evict(g4a_ctx* ctx, uint16_t* k_pages, uint16_t* v_pages, const int32_t* page_table,
+                              const int32_t* kv_lens, float* mass, uint64_t mass_stride, uint32_t batch,
+                              uint32_t budget, uint32_t sink_tokens, uint32_t recent_tokens, uint32_t page_size,
+                              uint32_t max_pages_per_seq, uint32_t num_pages, uint32_t num_kv_heads,
+                              uint32_t head_dim, int32_t* new_lens, int32_t* kept);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif
