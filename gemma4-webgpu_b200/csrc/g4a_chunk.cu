@@ -6,59 +6,10 @@
 
 #include "g4a_chunk.cuh"
 
-namespace {
-
-using namespace g4a;
 using namespace g4a_chunk;
 
-// One warp per (token, q head), a lane holds up to 16 dims; one pass over the rows with a running maximum and sum.
-__global__ void __launch_bounds__(256) chunk_simple_kernel(const ChunkParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long cap = (long long)p.max_pages * p.page_size;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int token = (int)(unit / p.nqh), head = (int)(unit % p.nqh);
-  if (token >= p.tokens) return;
-  for (int b = 0; b < p.batch; b++) {
-    const Seq s = seq_of(p, b, cap);
-    if (token < s.row0 || token >= s.row0 + s.T) continue;
-    const int pos = s.base() + token - s.row0, kvh = head / p.group;
-    float q[16], o[16], m = -INFINITY, l = 0.f;
-    const size_t row = (size_t)token * p.nqh + head;
-    for (int e = 0; e < 16; e++) {
-      const int d = e * 32 + lane;
-      q[e] = d < p.hd ? __half2float(p.q[row * p.hd + d]) : 0.f;
-      o[e] = 0.f;
-    }
-    const int lo = first_in_window(p, pos);
-    for (int r = 0; r <= pos; r++) {
-      if (r < lo && (uint32_t)r >= p.sinks) r = lo;
-      const long long off = row_offset(p, b, kvh, r);
-      if (off < 0) continue;
-      float x = 0.f;
-      for (int e = 0; e < 16; e++) {
-        const int d = e * 32 + lane;
-        if (d < p.hd) x = fmaf(q[e], __half2float(p.k[off + d]), x);
-      }
-      for (int w = 16; w >= 1; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-      x *= p.scale_log2;
-      const float mn = fmaxf(m, x);
-      const float f = m == mn ? 1.f : exp2f(m - mn), w = exp2f(x - mn);
-      m = mn;
-      l = l * f + w;
-      for (int e = 0; e < 16; e++) {
-        const int d = e * 32 + lane;
-        if (d < p.hd) o[e] = o[e] * f + w * __half2float(p.v[off + d]);
-      }
-    }
-    for (int e = 0; e < 16; e++) {
-      const int d = e * 32 + lane;
-      if (d < p.hd) p.out[row * p.hd + d] = __float2half_rn(l == 0.f ? 0.f : o[e] / l);
-    }
-    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2C;
-  }
-}
-
-}  // namespace
+// The tensor-core kernel (g4a_chunk_tc.cu).
+g4a_status g4a_chunk_tc_launch(g4a_ctx* ctx, const ChunkParams& p);
 
 g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, ChunkParams& p, const uint16_t* q, const uint16_t* k_pages,
                             const uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
@@ -126,10 +77,5 @@ extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, cons
   if (dev.status != G4A_OK) return dev.status;
   p.lse = lse;
   p.out = reinterpret_cast<__half*>(out);
-  g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
-  const long long units = (long long)num_tokens * num_q_heads;
-  const cudaError_t e =
-      g4a_launch(chunk_simple_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, ctx->stream, false, p);
-  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_simple_kernel");
-  return G4A_OK;
+  return g4a_chunk_tc_launch(ctx, p);
 }

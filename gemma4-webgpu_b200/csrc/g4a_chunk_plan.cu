@@ -1,0 +1,280 @@
+// The planning kernel of g4a_chunk_attn_paged: one CTA reads the lengths on the device (so a captured graph follows
+// them) and deals the tiles' key blocks to the pairs of CTAs that the attention kernel runs.
+//
+// An item is a tile of one kv head (of one half of its dims, where a head has two); it has as many stages as key
+// blocks.  Two ways to deal them, the cheaper one by a count of stages is taken:
+//  - Runs: the list of all items (sequence, kv head, tile), each kLead stages longer than it is, is cut into
+//    equal runs, one for each pair.  Perfect balance; a pair has whole tiles and at most two ends of cut ones.
+//  - Chunks: every tile of a sequence is cut into the same number of chunks, and the pairs take the pieces (kv head,
+//    chunk, tile) in that order.  Neighbours read the same rows at the same time, so that of several tiles only
+//    one goes to HBM where the L2 does not hold a sequence's rows (the runs pass a row at 16 different times in 512
+//    tokens x 8 heads over 131,000 rows); and with one chunk nothing has to be joined.
+#include "g4a_chunk_plan.cuh"
+
+namespace {
+
+using namespace g4a;
+using namespace g4a_chunk;
+
+// Inclusive sums over the block's threads of N values at once; returns the totals in `all`.
+template <int N>
+__device__ __forceinline__ void block_scan(long long (&x)[N], long long (&all)[N], long long (*warp_sum)[N]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long t = __shfl_up_sync(0xffffffffu, x[i], o);
+      if (lane >= o) x[i] += t;
+    }
+    if (lane == 31) warp_sum[warp][i] = x[i];
+  }
+  __syncthreads();
+  if (warp == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      long long t = warp_sum[lane][i];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += u;
+      }
+      warp_sum[lane][i] = t;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    if (warp > 0) x[i] += warp_sum[warp - 1][i];
+    all[i] = warp_sum[kPlanThreads / 32 - 1][i];
+  }
+  __syncthreads();
+}
+
+// The last sequence b with seqs[b].x (entries) or .y (items) <= i, of n sequences.
+__device__ __forceinline__ int find_seq(const int4* seqs, int n, int i, bool items) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((items ? seqs[mid].y : seqs[mid].x) <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanParams a) {
+  __shared__ long long warp_sum[32][4];
+  __shared__ float costs[32];
+  __shared__ int cut_count, run_s;
+  const ChunkParams& p = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long cap = (long long)p.max_pages * p.page_size;
+  const int heads = p.nkh * a.halves;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (tid == 0) cut_count = 0;
+  // ---- sequences: entries (tiles of one head) and items before each, the most stages of a tile
+  int entries = 0, items = 0, longest = 0;
+  float rows_seen = 0.f;  // rows of the cache that have to be read, over the sequences (for one kv head)
+  for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    long long x[2] = {0, 0}, all[2];
+    int most = 0;
+    if (b < p.batch) {
+      const Seq s = seq_of(p, b, cap);
+      if (s.T > 0) {
+        const int tiles = tiles_of(p, s);
+        x[0] = tiles;
+        x[1] = (long long)tiles * heads;
+        most = max(blocks_of(p, s, 0, a.kb_log2).count(), blocks_of(p, s, tiles - 1, a.kb_log2).count());
+        rows_seen += (float)(s.L - first_in_window(p, s.base()));
+      }
+    }
+    const int mine = (int)x[0], mine_items = (int)x[1];
+    block_scan<2>(x, all, reinterpret_cast<long long(*)[2]>(warp_sum));
+    if (b < p.batch) a.seqs[b] = make_int4(entries + (int)x[0] - mine, items + (int)x[1] - mine_items, most, 0);
+    entries += (int)all[0];
+    items += (int)all[1];
+    longest = max(longest, most);
+  }
+  if (tid == 0) a.seqs[p.batch] = make_int4(entries, items, 0, 0);
+  {  // over the block
+    __shared__ int most_s;
+    __shared__ float seen_s;
+    if (tid == 0) most_s = 0, seen_s = 0.f;
+    __syncthreads();
+    atomicMax(&most_s, longest);
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) rows_seen += __shfl_xor_sync(0xffffffffu, rows_seen, o);
+    if (lane == 0) costs[warp] = rows_seen;
+    __syncthreads();
+    if (tid == 0)
+      for (int w = 0; w < 32; w++) seen_s += costs[w];
+    __syncthreads();
+    longest = most_s;
+    rows_seen = seen_s;
+  }
+  // ---- stages of all earlier entries
+  long long total = 0;  // of one head
+  for (int e0 = 0; e0 < entries; e0 += kPlanThreads) {
+    const int e = e0 + tid;
+    long long x[1] = {0}, all[1];
+    if (e < entries) {
+      const int b = find_seq(a.seqs, p.batch, e, false);
+      x[0] = blocks_of(p, seq_of(p, b, cap), e - a.seqs[b].x, a.kb_log2).count();
+    }
+    const long long mine = x[0];
+    block_scan<1>(x, all, reinterpret_cast<long long(*)[1]>(warp_sum));
+    if (e < entries) a.entries[e] = total + x[0] - mine;
+    total += all[0];
+  }
+  __syncthreads();
+  if (items == 0) {
+    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0;
+    for (int w = tid; w <= a.pairs; w += kPlanThreads) a.plan->first[w] = 0;
+    return;
+  }
+  // ---- which way: warp k weighs chunks of at most longest / (k + 1) stages
+  const long long stages = total * heads;
+  const float hbm = 6500.f;  // bytes per ns
+  const float once = rows_seen * (float)p.nkh * (float)p.hd * 4.f;  // bytes, K and V
+  const float floor_once = once / hbm / a.stage_ns;
+  {
+    const int run = (longest + warp) / (warp + 1);
+    long long pieces = 0, cut = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+      const int n = a.seqs[b + 1].y - a.seqs[b].y;
+      if (n == 0) continue;
+      const int parts = (a.seqs[b].z + run - 1) / run;
+      pieces += (long long)n * parts;
+      if (parts > 1) cut += (long long)n * parts;
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      pieces += __shfl_xor_sync(0xffffffffu, pieces, o);
+      cut += __shfl_xor_sync(0xffffffffu, cut, o);
+    }
+    if (lane == 0) {
+      const float waves = (float)((pieces + a.pairs - 1) / a.pairs);
+      costs[warp] = cut > a.max_slots ? 3e38f : fmaxf(waves * (float)(run + kLead), floor_once) + (cut > 0 ? kJoinCost : 0);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    const float moved = (float)stages * a.stage_bytes;
+    // (90 MB of the 126 MB L2, beside what else passes through it)
+    const float floor_runs = (once > 90e6f ? fmaxf(moved, once) : once) / hbm / a.stage_ns;
+    float best = fmaxf(((float)stages + (float)kLead * (float)items) / (float)a.pairs + kLead, floor_runs) + kJoinCost;
+    int run = 0;
+    for (int k = 0; k < 32; k++)
+      if (costs[k] < best) best = costs[k], run = (longest + k) / (k + 1);
+    run_s = run;
+  }
+  __syncthreads();
+  const int run = run_s;
+  if (run > 0) {
+    // ---- chunks: pieces before each sequence, and places of partial results (kept at its first tile)
+    int before = 0;
+    long long slots = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
+      const int b = b0 + tid;
+      long long x[2] = {0, 0}, all[2];
+      bool any = false;
+      if (b < p.batch) {
+        const int n = a.seqs[b + 1].y - a.seqs[b].y, parts = (a.seqs[b].z + run - 1) / run;
+        any = n > 0;
+        x[0] = (long long)n * parts;
+        x[1] = parts > 1 ? x[0] : 0;
+      }
+      const long long mine = x[0], mine_slots = x[1];
+      block_scan<2>(x, all, reinterpret_cast<long long(*)[2]>(warp_sum));
+      if (any) {
+        a.seqs[b].w = before + (int)(x[0] - mine);
+        a.entries[a.seqs[b].x] = slots + x[1] - mine_slots;
+      }
+      before += (int)all[0];
+      slots += all[1];
+    }
+    if (tid == 0) a.plan->step = a.pairs, a.plan->pieces = before;
+    __syncthreads();
+    for (int i = tid; i < items; i += kPlanThreads) {
+      const int b = find_seq(a.seqs, p.batch, i, true);
+      const int4 q = a.seqs[b];
+      const Seq s = seq_of(p, b, cap);
+      const int tiles = a.seqs[b + 1].x - q.x, local = i - q.y;
+      const int head = local / tiles, tile = local - head * tiles, kvh = head / a.halves, half = head - kvh * a.halves;
+      const Blocks k = blocks_of(p, s, tile, a.kb_log2);
+      const int n = k.count(), all = (q.z + run - 1) / run, parts = min(all, n);
+      const int slot = (int)a.entries[q.x] + local * all;
+      for (int c = 0; c < all; c++) {
+        Piece d;
+        d.b = b, d.head = head, d.tile = tile, d.row0 = s.row0, d.T = s.T, d.L = s.L;
+        d.j0 = c < parts ? (int)((long long)n * c / parts) : 0;
+        d.j1 = c < parts ? (int)((long long)n * (c + 1) / parts) : 0;
+        d.slot = parts > 1 ? slot + c : -1;
+        d.sinks = k.sinks, d.skip = k.window0 - k.sinks, d.pad = 0;
+        a.pieces[q.w + (kvh * all + c) * tiles * a.halves + tile * a.halves + half] = d;
+      }
+      if (parts > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{b, head, tile, slot, parts, s.row0, s.T, 0};
+    }
+    __syncthreads();
+    if (tid == 0) a.plan->cuts = cut_count;
+    return;
+  }
+  // ---- runs
+  const long long length = stages + (long long)kLead * items;
+  const int pairs = (int)min((long long)a.pairs, length);
+  auto begin = [&](int w) { return (long long)w * length / pairs; };
+  auto owner = [&](long long x) { return (int)(((x + 1) * pairs - 1) / length); };
+  long long done_pieces = 0, done_slots = 0;
+  for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    long long x[2] = {0, 0}, all[2], at = 0;
+    int b = 0, tile = 0, head = 0, n = 0, parts = 0, w0 = 0, before = -1;
+    Seq s = {0, 0, 0};
+    Blocks k = {};
+    if (i < items) {
+      b = find_seq(a.seqs, p.batch, i, true);
+      s = seq_of(p, b, cap);
+      const int e0 = a.seqs[b].x, tiles = a.seqs[b + 1].x - e0, local = i - a.seqs[b].y;
+      head = local / tiles, tile = local - head * tiles;
+      k = blocks_of(p, s, tile, a.kb_log2);
+      n = k.count();
+      const long long first = a.entries[e0], mine = (a.seqs[b + 1].x < entries ? a.entries[e0 + tiles] : total) - first;
+      at = first * heads + head * mine + (a.entries[e0 + tile] - first) + (long long)kLead * i;
+      w0 = owner(at + kLead);
+      parts = owner(at + kLead + n - 1) - w0 + 1;
+      before = i > 0 ? owner(at - 1) : -1;
+      x[0] = parts;
+      x[1] = parts > 1 ? parts : 0;
+    }
+    block_scan<2>(x, all, reinterpret_cast<long long(*)[2]>(warp_sum));
+    if (i < items) {
+      const int piece = (int)(done_pieces + x[0]) - parts, slot = (int)(done_slots + x[1]) - parts;
+      for (int w = before + 1; w <= w0; w++) a.plan->first[w] = piece;
+      for (int c = 0; c < parts; c++) {
+        Piece d;
+        d.b = b, d.head = head, d.tile = tile, d.row0 = s.row0, d.T = s.T, d.L = s.L;
+        d.j0 = (int)max(0ll, begin(w0 + c) - at - kLead);
+        d.j1 = (int)min((long long)n, begin(w0 + c + 1) - at - kLead);
+        d.slot = parts > 1 ? slot + c : -1;
+        d.sinks = k.sinks, d.skip = k.window0 - k.sinks, d.pad = 0;
+        a.pieces[piece + c] = d;
+        if (c > 0) a.plan->first[w0 + c] = piece + c;
+      }
+      if (parts > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{b, head, tile, slot, parts, s.row0, s.T, 0};
+      if (i == items - 1)
+        for (int w = w0 + parts; w <= a.pairs; w++) a.plan->first[w] = piece + parts;
+    }
+    done_pieces += all[0];
+    done_slots += all[1];
+  }
+  __syncthreads();
+  if (tid == 0) a.plan->step = 1, a.plan->pieces = (int)done_pieces, a.plan->cuts = cut_count;
+}
+
+}  // namespace
+
+cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const PlanParams& a) {
+  return g4a_launch(chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, ctx->stream, true, a);
+}

@@ -1,0 +1,79 @@
+// How the work of g4a_chunk_attn_paged is dealt out: tiles, key blocks, and the pieces that chunk_plan_kernel
+// writes for the attention kernel and the join.
+#pragma once
+
+#include "g4a_chunk.cuh"
+
+namespace g4a_chunk {
+
+constexpr int kTileRows = 256;  // query rows of a tile: (token, q head of the group), both CTAs of a pair together
+constexpr int kMaxPairs = 128;
+constexpr int kPlanThreads = 1024;
+// Stages that a piece costs besides its keys: queries, the first scores and softmax without an MMA beside them,
+// epilogue.
+constexpr int kLead = 3;
+constexpr int kJoinCost = 4;  // and the join, if any tile is cut
+
+// A run of a tile's key blocks for one pair of CTAs.
+struct Piece {
+  int b, head;      // sequence; kv head * (halves of the head dims) + half
+  int tile;         // rows tile * 256 ..
+  int j0, j1;       // its stages, of all those of the tile
+  int slot;         // where its partial result goes; -1: the whole tile, straight to the output
+  int row0, T, L;   // the sequence
+  int sinks, skip;  // stages [0, sinks) are blocks [0, sinks), stage j behind them is block j + skip
+  int pad;
+};
+
+// A tile that several pieces share.
+struct Cut {
+  int b, head, tile, slot, parts, row0, T, pad;
+};
+
+struct Plan {
+  int step;            // 1: pair w has the pieces first[w] .. first[w + 1] - 1; else w, w + step, ...
+  int pieces, cuts, pad;
+  int first[kMaxPairs + 1];
+};
+
+// What the planning kernel reads and writes besides ChunkParams.
+struct PlanParams {
+  ChunkParams c;
+  int pairs, halves, kb_log2;  // halves of the head dims; keys of a block
+  int max_slots;
+  float stage_bytes, stage_ns;  // of a block: what is loaded, about how long it takes
+  Plan* plan;
+  Piece* pieces;
+  Cut* cuts;
+  int4* seqs;       // [batch + 1]: tile entries before, items before, most stages of a tile, (mode B) pieces before
+  long long* entries;  // [tile entries]: stages of all earlier entries
+};
+
+__device__ __forceinline__ int tiles_of(const ChunkParams& p, const Seq& s) {
+  return (int)(((long long)s.T * p.group + kTileRows - 1) / kTileRows);
+}
+__device__ __forceinline__ int first_token(const ChunkParams& p, int tile) {
+  return (int)((long long)tile * kTileRows / p.group);
+}
+__device__ __forceinline__ int last_token(const ChunkParams& p, int T, int tile) {
+  return (int)min((long long)T - 1, ((long long)(tile + 1) * kTileRows - 1) / p.group);
+}
+
+// The key blocks that a tile's rows see: [0, sinks) and [window0, window1).
+struct Blocks {
+  int sinks, window0, window1;
+  __device__ __forceinline__ int count() const { return sinks + window1 - window0; }
+};
+__device__ __forceinline__ Blocks blocks_of(const ChunkParams& p, const Seq& s, int tile, int kb_log2) {
+  const int lo = first_in_window(p, s.base() + first_token(p, tile)), hi = s.base() + last_token(p, s.T, tile) + 1;
+  const int up = (1 << kb_log2) - 1;
+  Blocks r;
+  r.window0 = lo >> kb_log2;
+  r.window1 = (hi + up) >> kb_log2;
+  r.sinks = (int)((min((long long)p.sinks, (long long)lo) + up) >> kb_log2);
+  if (r.sinks >= r.window0) r.sinks = r.window0 = 0;  // they meet
+  return r;
+}
+
+}  // namespace g4a_chunk
+cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const g4a_chunk::PlanParams& a);

@@ -1,0 +1,895 @@
+// The tensor-core kernel of g4a_chunk_attn_paged (tcgen05 / TMEM on pairs of CTAs) and the join of cut tiles.
+//
+// Rows of a tile are the T tokens x G q heads that share a kv head, 256 of them: a pair of CTAs computes them
+// together with tcgen05.mma.cta_group::2 (M 256), 128 rows in each CTA, so a key that is loaded serves 256 rows and
+// each CTA holds only half of every K and V block: with 128 rows to a K and V block of its own, each SM would ask
+// the L2 for 64 bytes per cycle at the tensor cores' full rate, which is all that an SM gets.
+//   S [256 x KB]  = Q K^T    A = Q (each CTA's 128 rows), B = K block, half of its keys in each CTA
+//   O [256 x HDV] += P V     A = P from TMEM, where the scores were, B = V block, half of its dims in each CTA
+// One pass over the keys with a running row maximum m and sum l: p = 2^(s - m + 7), rounded to f16 for the product
+// with V and summed unrounded; m is raised only when a score passes it by 2^8 (p <= 2^15 stays in f16), and only
+// then O is rescaled.  KB is 128 keys.  Heads of more than 256 dims: O takes 256 TMEM columns, so the dims of V are
+// halved between two pieces of work, each with the scores of its own (3/2 of the products, but nothing to be
+// exchanged, where two CTAs that split the dims have to add each other's partial scores); 64 keys, for Q takes 128 KB.
+//
+// Warps of a CTA (12):
+//   0-3   softmax and epilogue: a thread is a row (TMEM lane).
+//   4     loads its half of the K blocks (TMA, one box of rows per page and 64 dims).
+//   5     loads its half of the V blocks.
+//   6     in the pair's first CTA: issues the MMAs of both.  S of stage i + 1 before O of stage i, so that the
+//         softmax of a stage runs under the next stage's scores and the last one's product.
+//   7     tells the first CTA that a K block has landed in this one.
+//   8-11  load the queries, and look through V blocks that not every row sees: a value that is not finite
+//         becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then they tell the first CTA.
+// Barriers that both CTAs arrive on lie in the first CTA.  Every wait is bounded; a thread that gives up sets the
+// abort flags of both CTAs and the error word, all waits then end at once, and both free their TMEM and leave.
+#include <cudaTypedefs.h>
+#include <float.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "g4a_chunk_plan.cuh"
+#include "g4a_tcgen05.cuh"
+
+namespace {
+
+using namespace g4a;
+using namespace g4a_chunk;
+
+constexpr int kThreadsC = 384;
+constexpr int kLoadK = 4, kLoadV = 5, kMma = 6, kTellK = 7, kGuard = 8;
+constexpr int kCtaRows = 128;
+constexpr float kUpC = 7.0f;          // p = 2^(s - m + 7)
+constexpr float kRaiseC = 8.0f;       // a score this far above m raises it
+constexpr float kUnseenC = -FLT_MAX;  // m of a row that has seen nothing yet (any finite score raises it)
+constexpr int kInfo = 8;              // stages whose missing rows are remembered (more than are under way)
+constexpr int kBadTags = 8;
+
+template <int HD>
+struct Cc {
+  static constexpr int HDV = HD > 256 ? 256 : HD;    // dims of O of a piece
+  static constexpr int HALVES = HD / HDV;
+  static constexpr int KB_LOG2 = HD > 256 ? 6 : 7;
+  static constexpr int KB = 1 << KB_LOG2;            // keys of a block
+  static constexpr int NCQ = HD / 64, NCV = HDV / 128;  // 64-dim chunks of Q and K, of this CTA's share of V
+  static constexpr int Q_CHUNK = kCtaRows * 128, K_CHUNK = KB / 2 * 128, V_CHUNK = KB * 128;
+  static constexpr int Q_BYTES = NCQ * Q_CHUNK, K_BYTES = NCQ * K_CHUNK, V_BYTES = NCV * V_CHUNK;
+  static constexpr int NS = HD <= 128 ? 4 : 2;       // K and V blocks in flight
+  static constexpr bool OWN_STAGING = HD <= 256;     // (else the epilogue goes through Q's place)
+  static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_V = OFF_K + NS * K_BYTES, OFF_END = OFF_V + NS * V_BYTES;
+  static constexpr int OFF_OUT = OWN_STAGING ? OFF_END : OFF_Q;  // [4 warps][32 rows][128 B]
+  static constexpr int OFF_OK = OFF_END + (OWN_STAGING ? 4 * 4096 : 0);  // [kInfo][4] which rows of a block are there
+  static constexpr int OFF_BAD = OFF_OK + kInfo * 16;                    // [kBadTags] piece + 1 with values taken out
+  static constexpr int OFF_BAR = OFF_BAD + kBadTags * 4;
+  static constexpr int NBARS = 6 * NS + kInfo + 12;
+  static constexpr size_t SMEM = 1024 + (size_t)OFF_BAR + NBARS * 8 + 16;
+  static constexpr uint32_t COL_O = 0, COL_S = HDV;  // S[b] at COL_S + KB b, P[b] in its first half
+  static constexpr uint32_t TMEM_COLS = 512;
+  static_assert(COL_S + 2 * KB <= TMEM_COLS && SMEM <= 232448, "tile fits");
+  // Registers: 384 threads start with 168; the softmax warps hold a row of scores.
+  static constexpr int REGS_SOFT = 232, REGS_REST = 104;
+  static_assert(128 * REGS_SOFT + 256 * REGS_REST <= kThreadsC * 168, "register file");
+};
+
+struct TcParams {
+  ChunkParams c;
+  const Plan* plan;
+  const Piece* pieces;
+  const Cut* cuts;
+  float* part;            // [slots] (o [HDV / 4][256][4] | m [256] | l [256])
+  int box_k, box_v;       // rows of a box
+};
+
+// ------------------------------------------------------------------------------------ pair helpers
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ bool try_wait_pair(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded wait for arrivals of both CTAs.
+__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  if (try_wait_pair(bar, parity)) return true;
+  if (*abort_flag) return false;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (try_wait_pair(bar, parity)) return true;
+    if ((++spins & 63u) == 0u) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > 2000000000ull) {
+        *abort_flag = 1;
+        if (err) atomicExch(err, G4A_DEVERR_WAIT_MMA);
+        return false;
+      }
+    }
+  }
+}
+// D (+)= A B^T on the pair: M 256, rows 128 c .. of D and A in CTA c, half of B's rows in each.
+__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on `bar` of both CTAs when the MMAs issued so far have completed.
+__device__ __forceinline__ void commit2(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__host__ __device__ constexpr uint32_t pair_idesc(int n, bool b_mn_major) {
+  return (f16_idesc(n, b_mn_major) & 0x00ffffffu) | (uint32_t)(256 >> 4) << 24;  // M 256
+}
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int head, int row, int page,
+                                         uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A piece as its roles see it.
+template <int HD>
+struct Work {
+  Piece d;
+  int kvh, half, base, first, last;  // first and last token of the tile
+  __device__ __forceinline__ Work(const ChunkParams& p, const Piece& piece) : d(piece) {
+    kvh = d.head / Cc<HD>::HALVES;
+    half = d.head - kvh * Cc<HD>::HALVES;
+    base = d.L - d.T;
+    first = first_token(p, d.tile);
+    last = last_token(p, d.T, d.tile);
+  }
+  __device__ __forceinline__ int stages() const { return d.j1 - d.j0; }
+  __device__ __forceinline__ int key0(int j) const { return (j < d.sinks ? j : j + d.skip) << Cc<HD>::KB_LOG2; }
+  // whether every row of the tile sees every key of the block at k0 (if it is there)
+  __device__ __forceinline__ bool clean(const ChunkParams& p, int k0) const {
+    const int end = k0 + Cc<HD>::KB;
+    return end <= base + first + 1 && (k0 >= first_in_window(p, base + last) || (uint32_t)end <= p.sinks);
+  }
+};
+
+// Adds to what this thread has stored for row `gr` the infinities and NaN of the V values that were taken out of
+// the piece's blocks, where the row sees their keys.
+template <int HD>
+__device__ __noinline__ void add_taken_out(const ChunkParams& p, Work<HD> w, int pos, size_t out_row, float* part, int row) {
+  using C = Cc<HD>;
+  const int d0 = w.half * C::HDV, d1 = min(p.hd, d0 + C::HDV);
+  for (int j = w.d.j0; j < w.d.j1; j++) {
+    const int k0 = w.key0(j);
+    if (w.clean(p, k0)) continue;
+    for (int key = k0; key < k0 + C::KB && key <= pos; key++) {
+      if (!sees(p, pos, key)) continue;
+      const long long off = row_offset(p, w.d.b, w.kvh, key);
+      if (off < 0) continue;
+      for (int d = d0; d < d1; d++) {
+        const float v = __half2float(p.v[off + d]);
+        if (fabsf(v) < INFINITY) continue;
+        if (part != nullptr) {
+          const int e = d - d0;
+          part[((size_t)(e >> 2) * kTileRows + row) * 4 + (e & 3)] += v;
+        } else {
+          __half* o = p.out + out_row * p.hd + d;
+          *o = __float2half_rn(__half2float(*o) + v);
+        }
+      }
+    }
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreadsC, 1)
+    chunk_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TcParams a) {
+  using C = Cc<HD>;
+  const ChunkParams& p = a.c;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* k_landed = bars;                 // [NS] this CTA's half of a K block
+  uint64_t* v_landed = k_landed + C::NS;     // [NS]
+  uint64_t* k_ready = v_landed + C::NS;      // [NS] first CTA: both halves
+  uint64_t* v_ready = k_ready + C::NS;       // [NS] first CTA: both, looked through (4 warps of each CTA)
+  uint64_t* k_free = v_ready + C::NS;        // [NS] scores done (commit)
+  uint64_t* v_free = k_free + C::NS;         // [NS] product done (commit)
+  uint64_t* info = v_free + C::NS;           // [kInfo] which rows of the block are there
+  uint64_t* q_ready = info + kInfo;          // first CTA: queries of both (4 warps of each)
+  uint64_t* q_free = q_ready + 1;            // the piece's last scores done (commit)
+  uint64_t* s_done = q_free + 1;             // [2] scores (commit)
+  uint64_t* p_ready = s_done + 2;            // [2] first CTA: weights of both (4 warps of each)
+  uint64_t* o_done = p_ready + 2;            // [2] a stage's product done (commit)
+  uint64_t* o_free = o_done + 2;             // first CTA: epilogue has read O (4 warps of each)
+  uint64_t* looked = o_free + 1;             // the piece's V blocks have been looked through (4 warps of each)
+  uint64_t* staged = looked + 1;             // the epilogue is through with the staging place (4 warps)
+  uint64_t* all_done = staged + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(C::NBARS >= 6 * C::NS + kInfo + 12, "barriers");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cta_rank();
+  const uint32_t sbase = smem_u32(smem);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::NS; s++) {
+      mbar_init(&k_landed[s], 1);
+      mbar_init(&v_landed[s], 1);
+      mbar_init(&k_ready[s], 2);
+      mbar_init(&v_ready[s], 8);
+      mbar_init(&k_free[s], 1);
+      mbar_init(&v_free[s], 1);
+    }
+    for (int s = 0; s < kInfo; s++) mbar_init(&info[s], 1);
+    mbar_init(q_ready, 8);
+    mbar_init(q_free, 1);
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&s_done[s], 1);
+      mbar_init(&p_ready[s], 8);
+      mbar_init(&o_done[s], 1);
+    }
+    mbar_init(o_free, 8);
+    mbar_init(looked, 8);
+    mbar_init(staged, 4);
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    for (int i = 0; i < kBadTags; i++) reinterpret_cast<int*>(smem + C::OFF_BAD)[i] = 0;
+    fence_mbar_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmv)) : "memory");
+  }
+  __syncwarp();
+  if (warp == kMma) {  // one CTA per SM (shared memory), so the allocation never waits
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+
+  // this pair's pieces
+  const int pair = (int)(blockIdx.x >> 1), step = a.plan->step;
+  const int begin = step == 1 ? a.plan->first[pair] : pair;
+  const int end = step == 1 ? a.plan->first[pair + 1] : a.plan->pieces;
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ softmax, epilogue
+    regs_up<C::REGS_SOFT>();
+    const int row = rank * kCtaRows + warp * 32 + lane;  // of the tile
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t p_bar0 = map_to(smem_u32(&p_ready[0]), 0), p_bar1 = map_to(smem_u32(&p_ready[1]), 0);
+    const uint32_t o_bar = map_to(smem_u32(o_free), 0);
+    const volatile int* tags = reinterpret_cast<const volatile int*>(smem + C::OFF_BAD);
+    uint32_t g = 0, done = 0;  // stages and pieces so far
+    bool ok = true;
+    for (int i = begin; ok && i < end; i += step) {
+      const Work<HD> w(p, a.pieces[i]);
+      if (w.stages() <= 0) continue;
+      const long long gr = (long long)w.d.tile * kTileRows + row;
+      const bool live = gr < (long long)w.d.T * p.group;
+      const int token = live ? (int)(gr / p.group) : w.d.T - 1;
+      const int pos = w.base + token, lo = first_in_window(p, pos);
+      float m = kUnseenC, l = 0.f;
+      for (int j = w.d.j0; j < w.d.j1; j++, g++) {
+        const uint32_t b = g & 1u;
+        const uint32_t col = lanes + C::COL_S + b * C::KB;
+        ok = warp_wait(&info[g % kInfo], (g / kInfo) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        const uint4 there = *reinterpret_cast<const uint4*>(smem + C::OFF_OK + (g % kInfo) * 16);
+        ok = warp_wait(&s_done[b], (g >> 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t s[C::KB / 32][32];
+#pragma unroll
+        for (int c = 0; c < C::KB / 32; c++) tmem_get(col + 32u * c, s[c]);
+        const int k0 = w.key0(j);
+        // from the block's first key: z the last one seen, f the first one of the window, and sinks before n
+        const int z = pos - k0, f = lo - k0;
+        const int n = (int)min((long long)p.sinks - k0, (long long)C::KB);
+        const bool full = (there.x & there.y) == 0xffffffffu && (C::KB == 64 || (there.z & there.w) == 0xffffffffu);
+        const bool plain =
+            __all_sync(0xffffffffu, z >= C::KB - 1 && (f <= 0 || n >= C::KB)) && full && p.scale_log2 > 0.f;
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < C::KB / 32; c++) tmem_landed(s[c]);
+        float by = p.scale_log2;
+        if (!plain) {
+          by = 1.f;
+#pragma unroll
+          for (int c = 0; c < C::KB / 32; c++) {
+            // bits of keys [32 c, 32 c + 32): up to z, and from f on or before n
+            const int zc = z - 32 * c, fc = f - 32 * c, nc = n - 32 * c;
+            const uint32_t upto = zc >= 31 ? 0xffffffffu : zc < 0 ? 0u : (2u << zc) - 1u;
+            const uint32_t from = fc <= 0 ? 0xffffffffu : fc > 31 ? 0u : ~((1u << fc) - 1u);
+            const uint32_t sink = nc >= 32 ? 0xffffffffu : nc <= 0 ? 0u : (1u << nc) - 1u;
+            const uint32_t bits = upto & (from | sink) & (c == 0 ? there.x : c == 1 ? there.y : c == 2 ? there.z : there.w);
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              s[c][e] = (bits >> e) & 1u ? __float_as_uint(__uint_as_float(s[c][e]) * p.scale_log2) : 0xff800000u;
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < C::KB / 32; c++)
+#pragma unroll
+          for (int e = 0; e < 32; e++) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by;
+        const bool raise = top > m + kRaiseC;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float m_new = raise ? top : m;
+          const float fall = raise ? (m == kUnseenC ? 0.f : fast_exp2(m - m_new)) : 1.f;
+          l *= fall;
+          m = m_new;
+          if (j > w.d.j0) {
+            // O holds the stages up to j - 1, whose product is the last one issued before this stage's
+            ok = warp_wait(&o_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, p.err);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < C::HDV; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(lanes + C::COL_O + c, o);
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fall);
+              tmem_st32(lanes + C::COL_O + c, o);
+            }
+          }
+        }
+        const float up = kUpC - m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < C::KB / 64; c++) {
+          uint32_t pw[32];
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const float x = fast_exp2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][(2 * e) & 31]), by, up));
+            const float y = fast_exp2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][(2 * e + 1) & 31]), by, up));
+            sum[(2 * e) & 3] += x;
+            sum[(2 * e + 1) & 3] += y;
+            pw[e] = half2_bits(x, y);
+          }
+          tmem_st32(col + 32u * c, pw);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(b ? p_bar1 : p_bar0);
+      }
+      if (!ok) break;
+      // ---- epilogue
+      ok = warp_wait(&o_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, p.err);
+      if (!ok) break;
+      ok = __all_sync(0xffffffffu, wait_pair(looked, done & 1u, abort_flag, p.err));
+      if (!ok) break;
+      const bool bad = tags[done % kBadTags] == (int)done + 1;
+      tc_fence_after();
+      const size_t out_row = live ? (size_t)(w.d.row0 + token) * p.nqh + (size_t)w.kvh * p.group + (size_t)(gr - (long long)token * p.group) : 0;
+      const unsigned lives = __ballot_sync(0xffffffffu, live);  // (the first ones)
+      float* part = w.d.slot < 0 ? nullptr : a.part + (size_t)w.d.slot * kTileRows * (C::HDV + 2);
+      if (part != nullptr) {
+#pragma unroll 1
+        for (int c = 0; c < C::HDV; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(lanes + C::COL_O + c, o);
+          if (live)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              *reinterpret_cast<uint4*>(part + ((size_t)(c / 4 + e) * kTileRows + row) * 4) =
+                  make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+        if (live) {
+          part[(size_t)C::HDV * kTileRows + row] = m;
+          part[(size_t)(C::HDV + 1) * kTileRows + row] = l;
+        }
+      } else {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        unsigned char* stage = smem + C::OFF_OUT + warp * 4096;
+#pragma unroll 1
+        for (int c = 0; c < C::HDV; c += 64) {  // 64 columns of the warp's 32 rows through shared memory
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            uint32_t o[32];
+            tmem_ld32(lanes + C::COL_O + c + 32 * h, o);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              uint4 x;
+              x.x = half2_bits(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+              x.y = half2_bits(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+              x.z = half2_bits(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+              x.w = half2_bits(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + e) ^ (lane & 7)) << 4)) = x;
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int r0 = 0; r0 < 32; r0 += 4) {
+            const int r = r0 + (lane >> 3), e = lane & 7, d = w.half * C::HDV + c + e * 8;
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((e ^ (r & 7)) << 4));
+            const size_t at = __shfl_sync(0xffffffffu, out_row, r);
+            if (((lives >> r) & 1u) && d < p.hd) *reinterpret_cast<uint4*>(p.out + at * p.hd + d) = x;
+          }
+          __syncwarp();
+        }
+        if (p.lse != nullptr && live && w.half == 0)
+          p.lse[out_row] = l == 0.f ? -INFINITY : (m - kUpC + log2f(l)) * kLn2C;
+      }
+      if (bad && live) add_taken_out<HD>(p, w, pos, out_row, part, row);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        arrive_at(o_bar);
+        if (!C::OWN_STAGING) mbar_arrive(staged);
+      }
+      done++;
+    }
+  } else {
+    regs_down<C::REGS_REST>();
+    if (warp == kLoadK || warp == kLoadV) {
+      // ---------------------------------------------------------------- loads
+      const bool kside = warp == kLoadK;
+      uint64_t* landed = kside ? k_landed : v_landed;
+      uint64_t* free_bar = kside ? k_free : v_free;
+      const CUtensorMap* map = kside ? &tmk : &tmv;
+      const int box = kside ? a.box_k : a.box_v, rows = kside ? C::KB / 2 : C::KB, chunks = kside ? C::NCQ : C::NCV;
+      const int chunk_bytes = kside ? C::K_CHUNK : C::V_CHUNK, bytes = kside ? C::K_BYTES : C::V_BYTES;
+      const int boxes = rows / box, ops = boxes * chunks;
+      const long long cap = (long long)p.max_pages * p.page_size;
+      uint32_t g = 0;
+      bool ok = true;
+      for (int i = begin; ok && i < end; i += step) {
+        const Work<HD> w(p, a.pieces[i]);
+        const int* table = p.page_table + (size_t)w.d.b * p.max_pages;
+        for (int j = w.d.j0; j < w.d.j1; j++, g++) {
+          const uint32_t s = g % C::NS;
+          if (g >= (uint32_t)C::NS) {
+            ok = warp_wait(&free_bar[s], (g / C::NS - 1) & 1u, abort_flag, p.err);
+            if (!ok) break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&landed[s], (uint32_t)bytes);
+          __syncwarp();
+          const int k0 = w.key0(j);
+          const uint32_t dst = sbase + (kside ? C::OFF_K : C::OFF_V) + s * bytes;
+          for (int o = lane; o < ops; o += 32) {
+            const int r = o / chunks, c = o - r * chunks;
+            const int key = k0 + (kside ? rank * (C::KB / 2) : 0) + r * box;
+            int page = p.num_pages, row = 0;  // a page that is not there: zeros
+            if (key < w.d.L) {
+              const int t = key / p.page_size, id = table[t];
+              row = key - t * p.page_size;
+              if (id >= 0 && id < p.num_pages) page = id;
+            }
+            const int x = kside ? 64 * c : w.half * C::HDV + rank * (C::HDV / 2) + 64 * c;
+            load_box(dst + c * chunk_bytes + r * box * 128, map, x, w.kvh, row, page, &landed[s]);
+          }
+          if (kside) {
+            // which of the block's rows are there
+            bool gone = false;
+            for (int o = lane; o < 2 * boxes; o += 32) {
+              const int key = k0 + o * box;
+              if (key >= w.d.L) continue;
+              const int id = table[key / p.page_size];
+              gone |= id < 0 || id >= p.num_pages;
+            }
+            uint32_t* to = reinterpret_cast<uint32_t*>(smem + C::OFF_OK + (g % kInfo) * 16);
+            if (!__any_sync(0xffffffffu, gone)) {
+              if (lane < 4) to[lane] = 0xffffffffu;
+            } else {
+              if (lane == 0) atomicExch(p.err, G4A_DEVERR_PAGE);
+#pragma unroll 1
+              for (int c = 0; c < 4; c++) {
+                const int key = k0 + 32 * c + lane;
+                bool here = false;
+                if (c < C::KB / 32 && key < w.d.L && key < cap) {
+                  const int id = table[key / p.page_size];
+                  here = id >= 0 && id < p.num_pages;
+                }
+                const uint32_t bits = __ballot_sync(0xffffffffu, here);
+                if (lane == 0) to[c] = bits;
+              }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&info[g % kInfo]);
+          }
+        }
+      }
+      // loads still in flight land before the CTA leaves (bounded)
+      for (uint32_t k = g > (uint32_t)C::NS ? g - C::NS : 0; k < g; k++)
+        (void)mbar_wait_bounded(&landed[k % C::NS], (k / C::NS) & 1u, p.err, G4A_DEVERR_WAIT_FULL);
+    } else if (warp == kTellK) {
+      // ---------------------------------------------------------------- K blocks landed
+      if (lane == 0) {
+        uint32_t g = 0;
+        bool ok = true;
+        for (int i = begin; ok && i < end; i += step) {
+          const int n = a.pieces[i].j1 - a.pieces[i].j0;
+          for (int j = 0; j < n; j++, g++) {
+            ok = wait_or_abort(&k_landed[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+            if (!ok) break;
+            arrive_at(map_to(smem_u32(&k_ready[g % C::NS]), 0));
+          }
+        }
+      }
+    } else if (warp == kMma) {
+      // ---------------------------------------------------------------- MMAs
+      if (rank == 0 && lane == 0) {
+        constexpr uint32_t idesc_s = pair_idesc(C::KB, false), idesc_o = pair_idesc(C::HDV, true);
+        const uint64_t dq = sw128_desc(sbase + C::OFF_Q, 16, 1024);
+        const uint64_t dk0 = sw128_desc(sbase + C::OFF_K, 16, 1024);
+        // V as the MN-major B operand: 64 dims per 128-byte row, chunks of dims V_CHUNK apart, 8-key groups 1024
+        const uint64_t dv0 = sw128_desc(sbase + C::OFF_V, (uint32_t)C::V_CHUNK, 1024);
+        uint32_t g = 0, done = 0;
+        bool ok = true;
+        auto scores = [&](uint32_t k) {
+          if (!wait_pair(&k_ready[k % C::NS], (k / C::NS) & 1u, abort_flag, p.err)) return false;
+          tc_fence_after();
+          const uint64_t dk = dk0 + (uint64_t)(((k % C::NS) * C::K_BYTES) >> 4);
+          const uint32_t d = tmem + C::COL_S + (k & 1u) * C::KB;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; kk++) {
+            const uint64_t off = (uint64_t)(((kk & 3) * 32) >> 4);
+            mma2_ss(d, dq + (uint64_t)(((kk >> 2) * C::Q_CHUNK) >> 4) + off, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
+                    idesc_s, kk > 0 ? 1u : 0u);
+          }
+          commit2(&s_done[k & 1u]);
+          commit2(&k_free[k % C::NS]);
+          return true;
+        };
+        for (int i = begin; ok && i < end; i += step) {
+          const int n = a.pieces[i].j1 - a.pieces[i].j0;
+          if (n <= 0) continue;
+          ok = wait_pair(q_ready, done & 1u, abort_flag, p.err) && scores(g);
+          if (ok && n == 1) commit2(q_free);
+          for (int j = 0; ok && j < n; j++, g++) {
+            if (j + 1 < n) {
+              ok = scores(g + 1);
+              if (!ok) break;
+              if (j + 2 == n) commit2(q_free);
+            }
+            // (the epilogue of the piece before has read O)
+            if (j == 0 && done > 0) ok = wait_pair(o_free, (done - 1) & 1u, abort_flag, p.err);
+            ok = ok && wait_pair(&v_ready[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err) &&
+                 wait_pair(&p_ready[g & 1u], (g >> 1) & 1u, abort_flag, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dv = dv0 + (uint64_t)(((g % C::NS) * C::V_BYTES) >> 4);
+            const uint32_t pa = tmem + C::COL_S + (g & 1u) * C::KB;
+#pragma unroll
+            for (int kk = 0; kk < C::KB / 16; kk++)
+              mma2_ts(tmem + C::COL_O, pa + (uint32_t)(8 * kk), dv + (uint64_t)((kk * 2048) >> 4), idesc_o,
+                      j > 0 || kk > 0 ? 1u : 0u);
+            commit2(&o_done[g & 1u]);
+            commit2(&v_free[g % C::NS]);
+          }
+          done++;
+        }
+        // no MMA may still be running when TMEM is freed, also after an abort
+        commit2(all_done);
+        (void)mbar_wait_bounded(all_done, 0, p.err, G4A_DEVERR_WAIT_MMA);
+      }
+    } else {
+      // ---------------------------------------------------------------- queries, a look through V
+      const int gw = warp - kGuard;
+      const uint32_t q_bar = map_to(smem_u32(q_ready), 0);
+      const uint32_t tags = sbase + C::OFF_BAD;
+      uint32_t g = 0, done = 0;
+      bool ok = true;
+      for (int i = begin; ok && i < end; i += step) {
+        const Work<HD> w(p, a.pieces[i]);
+        if (w.stages() <= 0) continue;
+        if (done > 0) {
+          ok = warp_wait(q_free, (done - 1) & 1u, abort_flag, p.err);
+          if (ok && !C::OWN_STAGING) ok = warp_wait(staged, (done - 1) & 1u, abort_flag, p.err);
+          if (!ok) break;
+        }
+        const long long rows = (long long)w.d.T * p.group;
+#pragma unroll 1
+        for (int r = gw; r < kCtaRows; r += 4) {
+          const long long gr = (long long)w.d.tile * kTileRows + rank * kCtaRows + r;
+          const bool live = gr < rows;
+          const int token = live ? (int)(gr / p.group) : 0;
+          const __half* from = p.q + ((size_t)(w.d.row0 + token) * p.nqh + (size_t)w.kvh * p.group +
+                                      (live ? (size_t)(gr - (long long)token * p.group) : 0)) * p.hd;
+          const uint32_t to = sbase + C::OFF_Q + r * 128;
+#pragma unroll
+          for (int e = lane; e < HD / 8; e += 32) {
+            const bool in = live && e * 8 < p.hd;
+            cp16(to + (e >> 3) * C::Q_CHUNK + (((e & 7) ^ (r & 7)) << 4), in ? from + e * 8 : p.q, in);
+          }
+        }
+        cp_wait_all();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) arrive_at(q_bar);
+        const int lo = first_in_window(p, w.base + w.first), hi = w.base + w.last + 1;
+        bool found = false;
+        for (int j = w.d.j0; j < w.d.j1; j++, g++) {
+          const uint32_t s = g % C::NS;
+          ok = warp_wait(&v_landed[s], (g / C::NS) & 1u, abort_flag, p.err);
+          if (!ok) break;
+          const int k0 = w.key0(j);
+          if (!w.clean(p, k0)) {
+            unsigned char* v = smem + C::OFF_V + s * C::V_BYTES;
+#pragma unroll 4
+            for (int e = gw * 32 + lane; e < C::V_BYTES / 16; e += 128) {
+              uint4 x = *reinterpret_cast<const uint4*>(v + e * 16);
+              const uint32_t was[4] = {x.x, x.y, x.z, x.w};
+              uint32_t now[4];
+              bool changed = false;
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                now[k] = was[k];
+                if ((now[k] & 0x7c00u) == 0x7c00u) now[k] &= 0xffff0000u;
+                if ((now[k] & 0x7c000000u) == 0x7c000000u) now[k] &= 0x0000ffffu;
+                changed |= now[k] != was[k];
+              }
+              if (changed) {
+                *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(now[0], now[1], now[2], now[3]);
+                const int key = k0 + (e >> 3) % C::KB;  // 8 pieces of 16 bytes to a row, KB rows to a chunk
+                found |= key < hi && (key >= lo || (uint32_t)key < p.sinks);
+              }
+            }
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) arrive_at(map_to(smem_u32(&v_ready[s]), 0));
+        }
+        if (!ok) break;
+        // (a CTA has half of the dims and half of the rows, so both have to know)
+#pragma unroll
+        for (uint32_t c = 0; c < 2; c++) {
+          if (found)
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(tags + (done % kBadTags) * 4, c)), "r"(done + 1) : "memory");
+          __syncwarp();
+          if (lane == 0) arrive_at(map_to(smem_u32(looked), c));
+        }
+        done++;
+      }
+    }
+  }
+  // a warp that gave up stops the partner's waits too (it leaves only through the pair's barrier)
+  __syncwarp();
+  if (lane == 0 && *abort_flag)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(smem_u32((const void*)abort_flag), (uint32_t)rank ^ 1u)),
+                 "r"(1u)
+                 : "memory");
+  __syncwarp();
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  if (warp == kMma)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+}
+
+// Joins the parts of the tiles that several pieces share.  A unit is 8 rows x 16 dims of a cut tile; the 8 warps share
+// its parts, a lane is one float4 of a row.
+constexpr int kJoinThreads = 256;
+template <int HD>
+__global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams a) {
+  using C = Cc<HD>;
+  const ChunkParams& p = a.c;
+  __shared__ float4 so[8][32];
+  __shared__ float sm[8][8], sl[8][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int r8 = lane >> 2, c4 = lane & 3;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  constexpr int kBlocks = C::HDV / 16, kUnits = kTileRows / 8 * kBlocks;
+  const long long total = (long long)a.plan->cuts * kUnits;
+  for (long long u = blockIdx.x; u < total; u += gridDim.x) {
+    const Cut cut = a.cuts[u / kUnits];
+    const int at = (int)(u % kUnits), row0 = at / kBlocks * 8, block = at % kBlocks;
+    const long long gr = (long long)cut.tile * kTileRows + row0 + r8, rows = (long long)cut.T * p.group;
+    if (gr - r8 >= rows) continue;  // (the same for the whole unit)
+    const int row = row0 + r8;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (gr < rows) {
+      constexpr int kFly = 4;
+      for (int i0 = warp; i0 < cut.parts; i0 += 8 * kFly) {
+        float mi[kFly], li[kFly];
+        float4 x[kFly];
+#pragma unroll
+        for (int f = 0; f < kFly; f++) {
+          const int i = i0 + 8 * f;
+          mi[f] = -INFINITY, li[f] = 0.f, x[f] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (i >= cut.parts) continue;
+          const float* part = a.part + (size_t)(cut.slot + i) * kTileRows * (C::HDV + 2);
+          mi[f] = __ldcg(part + (size_t)C::HDV * kTileRows + row);
+          li[f] = __ldcg(part + (size_t)(C::HDV + 1) * kTileRows + row);
+          x[f] = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)(block * 4 + c4) * kTileRows + row);
+        }
+        float mn = m;
+#pragma unroll
+        for (int f = 0; f < kFly; f++) mn = fmaxf(mn, mi[f]);
+        const float wo = m == mn ? 1.f : fast_exp2(m - mn);
+        m = mn;
+        l *= wo;
+        o.x *= wo, o.y *= wo, o.z *= wo, o.w *= wo;
+#pragma unroll
+        for (int f = 0; f < kFly; f++) {
+          const float wf = mi[f] == mn ? 1.f : fast_exp2(mi[f] - mn);
+          l = fmaf(wf, li[f], l);
+          o.x = fmaf(wf, x[f].x, o.x);
+          o.y = fmaf(wf, x[f].y, o.y);
+          o.z = fmaf(wf, x[f].z, o.z);
+          o.w = fmaf(wf, x[f].w, o.w);
+        }
+      }
+    }
+    so[warp][lane] = o;
+    if (c4 == 0) sm[warp][r8] = m, sl[warp][r8] = l;
+    __syncthreads();
+    if (warp == 0 && gr < rows) {
+      float mx = -INFINITY, lt = 0.f;
+      for (int i = 0; i < 8; i++) mx = fmaxf(mx, sm[i][r8]);
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int i = 0; i < 8; i++) {
+        const float wf = sm[i][r8] == mx ? 1.f : fast_exp2(sm[i][r8] - mx);
+        const float4 x = so[i][lane];
+        lt = fmaf(wf, sl[i][r8], lt);
+        o.x = fmaf(wf, x.x, o.x);
+        o.y = fmaf(wf, x.y, o.y);
+        o.z = fmaf(wf, x.z, o.z);
+        o.w = fmaf(wf, x.w, o.w);
+      }
+      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+      const int kvh = cut.head / C::HALVES, half = cut.head - kvh * C::HALVES, token = (int)(gr / p.group);
+      const size_t to = (size_t)(cut.row0 + token) * p.nqh + (size_t)kvh * p.group + (size_t)(gr - (long long)token * p.group);
+      const int d = half * C::HDV + block * 16 + c4 * 4;
+      if (d < p.hd)
+        *reinterpret_cast<uint2*>(p.out + to * p.hd + d) = make_uint2(half2_bits(o.x * inv, o.y * inv), half2_bits(o.z * inv, o.w * inv));
+      if (p.lse != nullptr && d == 0) p.lse[to] = lt == 0.f ? -INFINITY : (mx - kUpC + log2f(lt)) * kLn2C;
+    }
+    __syncthreads();
+  }
+}
+
+g4a_status page_map(g4a_ctx* ctx, CUtensorMap* map, const ChunkParams& p, const __half* pool, int rows, const char* what) {
+  if (!ctx->encode_tiled) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || fn == nullptr)
+      return g4a_fail(G4A_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    ctx->encode_tiled = fn;
+  }
+  auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ctx->encode_tiled);
+  const cuuint64_t row = (cuuint64_t)p.nkh * p.hd * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.nkh, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)p.hd * 2, row, row * p.page_size};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(pool), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return g4a_fail(G4A_EINVAL, "g4a_chunk_attn_paged: no tensor map for %s (%d)", what, (int)r);
+  return G4A_OK;
+}
+
+template <int HD>
+g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
+  using C = Cc<HD>;
+  const char* fn = "g4a_chunk_attn_paged";
+  static std::atomic<bool> ready[64];
+  if (ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_acquire)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(chunk_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(chunk_tc_kernel)");
+    if (ctx->device < 64) ready[ctx->device].store(true, std::memory_order_release);
+  }
+  TcParams a = {};
+  a.c = p;
+  // a box of rows lies in one page: the largest power of two that divides the page
+  const int unit = p.page_size & -p.page_size;
+  a.box_k = std::min(unit, C::KB / 2);
+  a.box_v = std::min(unit, C::KB);
+  CUtensorMap mk, mv;
+  if (g4a_status s = page_map(ctx, &mk, p, p.k, a.box_k, "the K pages")) return s;
+  if (g4a_status s = page_map(ctx, &mv, p, p.v, a.box_v, "the V pages")) return s;
+  const int pairs = std::min(ctx->num_sms / 2, kMaxPairs);
+  const long long entries = (long long)p.tokens * p.group / kTileRows + std::min(p.batch, p.tokens);
+  const long long items = entries * p.nkh * C::HALVES;
+  if (items > (1 << 24)) return g4a_fail(G4A_EINVAL, "%s: num_tokens * num_q_heads too large", fn);
+  const long long slots = 4ll * pairs, pieces = items + slots;
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  const size_t n_part = up((size_t)slots * kTileRows * (C::HDV + 2) * sizeof(float)), n_plan = up(sizeof(Plan));
+  const size_t n_piece = up((size_t)pieces * sizeof(Piece)), n_cut = up((size_t)items * sizeof(Cut));
+  const size_t n_seq = up((size_t)(p.batch + 1) * sizeof(int4)), n_entry = up((size_t)entries * sizeof(long long));
+  if (g4a_status s = g4a_ensure_workspace(ctx, n_part + n_plan + n_piece + n_cut + n_seq + n_entry)) return s;
+  char* ws = static_cast<char*>(ctx->workspace);
+  PlanParams q = {};
+  q.c = p;
+  q.pairs = pairs;
+  q.halves = C::HALVES;
+  q.kb_log2 = C::KB_LOG2;
+  q.max_slots = (int)slots;
+  q.stage_bytes = 2.f * (C::K_BYTES + C::V_BYTES);
+  q.stage_ns = C::KB * (HD + C::HDV) * (1.f / 55.f);
+  a.part = reinterpret_cast<float*>(ws);
+  q.plan = reinterpret_cast<Plan*>(ws += n_part);
+  q.pieces = reinterpret_cast<Piece*>(ws += n_plan);
+  q.cuts = reinterpret_cast<Cut*>(ws += n_piece);
+  q.seqs = reinterpret_cast<int4*>(ws += n_cut);
+  q.entries = reinterpret_cast<long long*>(ws += n_seq);
+  a.plan = q.plan;
+  a.pieces = q.pieces;
+  a.cuts = q.cuts;
+  g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
+  cudaError_t e = g4a_chunk_plan_launch(ctx, q);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_plan_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(kThreadsC);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, chunk_tc_kernel<HD>, mk, mv, a);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_tc_kernel");
+  e = g4a_launch(chunk_join_kernel<HD>, dim3(8 * ctx->num_sms), dim3(kJoinThreads), 0, ctx->stream, true, a);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_join_kernel");
+  return G4A_OK;
+}
+
+}  // namespace
+
+g4a_status g4a_chunk_tc_launch(g4a_ctx* ctx, const ChunkParams& p) {
+  if (p.hd > 256) return launch_chunk<512>(ctx, p);
+  if (p.hd > 128) return launch_chunk<256>(ctx, p);
+  return launch_chunk<128>(ctx, p);
+}
