@@ -1,10 +1,11 @@
 // Attention of a chunk of new tokens of every sequence over a paged cache (g4a_chunk_attn_paged).  No reference
 // counterpart; the semantics of one token are those of shaders/attn_score.wgsl, softmax.wgsl and
 // attn_output.wgsl over the rows that it sees, with a few first rows beside the window.
-#include <algorithm>
+#include <cudaTypedefs.h>
+
 #include <cmath>
 
-#include "g4a_chunk.cuh"
+#include "g4a_chunk_pair.cuh"
 
 using namespace g4a_chunk;
 
@@ -54,6 +55,42 @@ g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, ChunkParams& p, const 
   p.sinks = sink_tokens;
   p.err = ctx->dev_err_dev;
   return G4A_OK;
+}
+
+static g4a_status encode_map(const char* fn, g4a_ctx* ctx, CUtensorMap* map, const __half* base, const cuuint64_t (&dims)[4],
+                             const cuuint64_t (&strides)[3], const cuuint32_t (&box)[4]) {
+  if (!ctx->encode_tiled) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || f == nullptr)
+      return g4a_fail(G4A_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    ctx->encode_tiled = f;
+  }
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
+  const CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ctx->encode_tiled)(
+      map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, steps,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return g4a_fail(G4A_EINVAL, "%s: cuTensorMapEncodeTiled failed (%d)", fn, (int)r);
+  return G4A_OK;
+}
+
+g4a_status g4a_page_map(const char* fn, g4a_ctx* ctx, CUtensorMap* map, const ChunkParams& p, const __half* pool,
+                        int rows) {
+  const cuuint64_t row = (cuuint64_t)p.nkh * p.hd * 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.nkh, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)p.hd * 2, row, row * p.page_size};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
+  return encode_map(fn, ctx, map, pool, dims, strides, box);
+}
+
+g4a_status g4a_query_map(const char* fn, g4a_ctx* ctx, CUtensorMap* map, const ChunkParams& p, int heads, int tokens) {
+  const cuuint64_t head = (cuuint64_t)p.hd * 2;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.group, (cuuint64_t)p.nkh, (cuuint64_t)p.tokens};
+  const cuuint64_t strides[3] = {head, head * p.group, head * p.nqh};
+  const cuuint32_t box[4] = {64, (cuuint32_t)heads, 1, (cuuint32_t)tokens};
+  return encode_map(fn, ctx, map, p.q, dims, strides, box);
 }
 
 extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t* k_pages,

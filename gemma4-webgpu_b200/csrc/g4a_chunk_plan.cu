@@ -1,5 +1,5 @@
-// The planning kernel of g4a_chunk_attn_paged: one CTA reads the lengths on the device (so a captured graph follows
-// them) and deals the tiles' key blocks to the pairs of CTAs that the attention kernel runs.
+// The planning kernel of g4a_chunk_attn_paged and g4a_paged_key_mass: one CTA reads the lengths on the device (so a
+// captured graph follows them) and deals the work to the pairs of CTAs that the next kernel runs.
 //
 // An item is a tile of one kv head (of one half of its dims, where a head has two); it has as many stages as key
 // blocks.  Two ways to deal them, the cheaper one by a count of stages is taken:
@@ -9,6 +9,8 @@
 //    chunk, tile) in that order.  Neighbours read the same rows at the same time, so that of several tiles only
 //    one goes to HBM where the L2 does not hold a sequence's rows (the runs pass a row at 16 different times in 512
 //    tokens x 8 heads over 131,000 rows); and with one chunk nothing has to be joined.
+// The masses turn it round: a tile is 256 keys of one kv head, its stages are blocks of the query rows that see any of
+// them, and they are dealt in runs.
 #include "g4a_chunk_plan.cuh"
 
 namespace {
@@ -62,14 +64,22 @@ __device__ __forceinline__ int find_seq(const int4* seqs, int n, int i, bool ite
   return lo;
 }
 
+template <bool MASS>
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanParams a) {
   __shared__ long long warp_sum[32][4];
   __shared__ float costs[32];
   __shared__ int cut_count, run_s;
   const ChunkParams& p = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long cap = (long long)p.max_pages * p.page_size;
+  const long long cap = MASS ? min((long long)p.max_pages * p.page_size, p.mass_stride) : (long long)p.max_pages * p.page_size;
   const int heads = p.nkh * a.halves;
+  // masses: the key tile of a sequence's entry, and its row blocks
+  auto key_tile = [&](const Blocks& k, int e) { return e < k.sinks ? e : e + k.window0 - k.sinks; };
+  auto row_blocks = [&](const Seq& s, int tile, int& first) {
+    const Tokens t = tokens_of(p, s, tile << a.kb_log2, 1 << a.kb_log2);
+    first = t.first / a.block_tokens;
+    return ((t.last + a.block_tokens - 1) / a.block_tokens - first) * a.head_chunks;
+  };
   pdl_wait_primary();
   pdl_launch_dependents();
   if (tid == 0) cut_count = 0;
@@ -83,10 +93,10 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     if (b < p.batch) {
       const Seq s = seq_of(p, b, cap);
       if (s.T > 0) {
-        const int tiles = tiles_of(p, s);
+        const int tiles = MASS ? key_tiles_of(p, s, a.kb_log2).count() : tiles_of(p, s);
         x[0] = tiles;
         x[1] = (long long)tiles * heads;
-        most = max(blocks_of(p, s, 0, a.kb_log2).count(), blocks_of(p, s, tiles - 1, a.kb_log2).count());
+        if (!MASS) most = max(blocks_of(p, s, 0, a.kb_log2).count(), blocks_of(p, s, tiles - 1, a.kb_log2).count());
         rows_seen += (float)(s.L - first_in_window(p, s.base()));
       }
     }
@@ -121,7 +131,10 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     long long x[1] = {0}, all[1];
     if (e < entries) {
       const int b = find_seq(a.seqs, p.batch, e, false);
-      x[0] = blocks_of(p, seq_of(p, b, cap), e - a.seqs[b].x, a.kb_log2).count();
+      const Seq s = seq_of(p, b, cap);
+      int first;
+      x[0] = MASS ? row_blocks(s, key_tile(key_tiles_of(p, s, a.kb_log2), e - a.seqs[b].x), first)
+                  : blocks_of(p, s, e - a.seqs[b].x, a.kb_log2).count();
     }
     const long long mine = x[0];
     block_scan<1>(x, all, reinterpret_cast<long long(*)[1]>(warp_sum));
@@ -139,7 +152,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
   const float hbm = 6500.f;  // bytes per ns
   const float once = rows_seen * (float)p.nkh * (float)p.hd * 4.f;  // bytes, K and V
   const float floor_once = once / hbm / a.stage_ns;
-  {
+  if (!MASS) {
     const int run = (longest + warp) / (warp + 1);
     long long pieces = 0, cut = 0;
     for (int b = lane; b < p.batch; b += 32) {
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     const float floor_runs = (once > 90e6f ? fmaxf(moved, once) : once) / hbm / a.stage_ns;
     float best = fmaxf(((float)stages + (float)kLead * (float)items) / (float)a.pairs + kLead, floor_runs) + kJoinCost;
     int run = 0;
-    for (int k = 0; k < 32; k++)
+    for (int k = 0; k < (MASS ? 0 : 32); k++)
       if (costs[k] < best) best = costs[k], run = (longest + k) / (k + 1);
     run_s = run;
   }
@@ -238,10 +251,17 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
       s = seq_of(p, b, cap);
       const int e0 = a.seqs[b].x, tiles = a.seqs[b + 1].x - e0, local = i - a.seqs[b].y;
       head = local / tiles, tile = local - head * tiles;
-      k = blocks_of(p, s, tile, a.kb_log2);
-      n = k.count();
+      const int entry = e0 + tile;
+      if (MASS) {
+        k.sinks = 0;
+        tile = key_tile(key_tiles_of(p, s, a.kb_log2), tile);
+        n = row_blocks(s, tile, k.window0);
+      } else {
+        k = blocks_of(p, s, tile, a.kb_log2);
+        n = k.count();
+      }
       const long long first = a.entries[e0], mine = (a.seqs[b + 1].x < entries ? a.entries[e0 + tiles] : total) - first;
-      at = first * heads + head * mine + (a.entries[e0 + tile] - first) + (long long)kLead * i;
+      at = first * heads + head * mine + (a.entries[entry] - first) + (long long)kLead * i;
       w0 = owner(at + kLead);
       parts = owner(at + kLead + n - 1) - w0 + 1;
       before = i > 0 ? owner(at - 1) : -1;
@@ -262,7 +282,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
         a.pieces[piece + c] = d;
         if (c > 0) a.plan->first[w0 + c] = piece + c;
       }
-      if (parts > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{b, head, tile, slot, parts, s.row0, s.T, 0};
+      if (MASS) a.parts[i] = make_int2(slot, parts);
+      else if (parts > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{b, head, tile, slot, parts, s.row0, s.T, 0};
       if (i == items - 1)
         for (int w = w0 + parts; w <= a.pairs; w++) a.plan->first[w] = piece + parts;
     }
@@ -275,6 +296,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
 
 }  // namespace
 
-cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const PlanParams& a) {
-  return g4a_launch(chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, ctx->stream, true, a);
+cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const PlanParams& a, bool masses) {
+  return g4a_launch(masses ? chunk_plan_kernel<true> : chunk_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0,
+                    ctx->stream, true, a);
 }

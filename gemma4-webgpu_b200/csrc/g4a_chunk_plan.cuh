@@ -39,14 +39,16 @@ struct Plan {
 // What the planning kernel reads and writes besides ChunkParams.
 struct PlanParams {
   ChunkParams c;
-  int pairs, halves, kb_log2;  // halves of the head dims; keys of a block
+  int pairs, halves, kb_log2;  // halves of the head dims; keys of a block (masses: of a tile)
   int max_slots;
   float stage_bytes, stage_ns;  // of a block: what is loaded, about how long it takes
+  int block_tokens, head_chunks;  // masses: tokens of a row block, row blocks for the heads of one token
   Plan* plan;
   Piece* pieces;
   Cut* cuts;
-  int4* seqs;       // [batch + 1]: tile entries before, items before, most stages of a tile, (mode B) pieces before
+  int4* seqs;          // [batch + 1]: tile entries before, items before, most stages of a tile, (chunks) pieces before
   long long* entries;  // [tile entries]: stages of all earlier entries
+  int2* parts;         // masses: [items] place of a tile's first partial result, number of its pieces
 };
 
 __device__ __forceinline__ int tiles_of(const ChunkParams& p, const Seq& s) {
@@ -75,5 +77,27 @@ __device__ __forceinline__ Blocks blocks_of(const ChunkParams& p, const Seq& s, 
   return r;
 }
 
+// Masses: the key tiles that any token of a sequence sees, as the blocks of one tile that holds all tokens.
+__device__ __forceinline__ Blocks key_tiles_of(const ChunkParams& p, const Seq& s, int kb_log2) {
+  Blocks r = {0, 0, 0};
+  if (s.T <= 0) return r;
+  const int lo = first_in_window(p, s.base()), up = (1 << kb_log2) - 1;
+  r.window0 = lo >> kb_log2;
+  r.window1 = (int)(((long long)s.L + up) >> kb_log2);
+  r.sinks = (int)((min((long long)p.sinks, (long long)lo) + up) >> kb_log2);
+  if (r.sinks >= r.window0) r.sinks = r.window0 = 0;
+  return r;
+}
+// The tokens [first, last) that see any key of the tile at k0.
+struct Tokens {
+  int first, last;
+};
+__device__ __forceinline__ Tokens tokens_of(const ChunkParams& p, const Seq& s, int k0, int keys) {
+  Tokens t = {max(0, k0 - s.base()), s.T};
+  if (p.window != 0u && (uint32_t)k0 >= p.sinks)
+    t.last = (int)min((long long)s.T, (long long)k0 + keys - 1 + (long long)p.window - s.base());
+  return t;
+}
+
 }  // namespace g4a_chunk
-cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const g4a_chunk::PlanParams& a);
+cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const g4a_chunk::PlanParams& a, bool masses);

@@ -23,14 +23,12 @@
 //         becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then they tell the first CTA.
 // Barriers that both CTAs arrive on lie in the first CTA.  Every wait is bounded; a thread that gives up sets the
 // abort flags of both CTAs and the error word, all waits then end at once, and both free their TMEM and leave.
-#include <cudaTypedefs.h>
 #include <float.h>
 
 #include <algorithm>
 #include <atomic>
 
-#include "g4a_chunk_plan.cuh"
-#include "g4a_tcgen05.cuh"
+#include "g4a_chunk_pair.cuh"
 
 namespace {
 
@@ -81,90 +79,6 @@ struct TcParams {
   int box_k, box_v;       // rows of a box
 };
 
-// ------------------------------------------------------------------------------------ pair helpers
-__device__ __forceinline__ uint32_t cta_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void pair_sync() {
-  asm volatile(
-      "barrier.cluster.arrive.release.aligned;\n\t"
-      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-__device__ __forceinline__ bool try_wait_pair(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded wait for arrivals of both CTAs.
-__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  if (try_wait_pair(bar, parity)) return true;
-  if (*abort_flag) return false;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t spins = 0;
-  while (true) {
-    if (try_wait_pair(bar, parity)) return true;
-    if ((++spins & 63u) == 0u) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > 2000000000ull) {
-        *abort_flag = 1;
-        if (err) atomicExch(err, G4A_DEVERR_WAIT_MMA);
-        return false;
-      }
-    }
-  }
-}
-// D (+)= A B^T on the pair: M 256, rows 128 c .. of D and A in CTA c, half of B's rows in each.
-__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrive on `bar` of both CTAs when the MMAs issued so far have completed.
-__device__ __forceinline__ void commit2(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-__host__ __device__ constexpr uint32_t pair_idesc(int n, bool b_mn_major) {
-  return (f16_idesc(n, b_mn_major) & 0x00ffffffu) | (uint32_t)(256 >> 4) << 24;  // M 256
-}
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int head, int row, int page,
-                                         uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-      "[%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(head), "r"(row), "r"(page), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -792,28 +706,6 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams
   }
 }
 
-g4a_status page_map(g4a_ctx* ctx, CUtensorMap* map, const ChunkParams& p, const __half* pool, int rows, const char* what) {
-  if (!ctx->encode_tiled) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
-    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || fn == nullptr)
-      return g4a_fail(G4A_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    ctx->encode_tiled = fn;
-  }
-  auto enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ctx->encode_tiled);
-  const cuuint64_t row = (cuuint64_t)p.nkh * p.hd * 2;
-  cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.nkh, (cuuint64_t)p.page_size, (cuuint64_t)p.num_pages};
-  cuuint64_t strides[3] = {(cuuint64_t)p.hd * 2, row, row * p.page_size};
-  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(pool), dims, strides, box, estr,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return g4a_fail(G4A_EINVAL, "g4a_chunk_attn_paged: no tensor map for %s (%d)", what, (int)r);
-  return G4A_OK;
-}
-
 template <int HD>
 g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   using C = Cc<HD>;
@@ -832,8 +724,8 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   a.box_k = std::min(unit, C::KB / 2);
   a.box_v = std::min(unit, C::KB);
   CUtensorMap mk, mv;
-  if (g4a_status s = page_map(ctx, &mk, p, p.k, a.box_k, "the K pages")) return s;
-  if (g4a_status s = page_map(ctx, &mv, p, p.v, a.box_v, "the V pages")) return s;
+  if (g4a_status s = g4a_page_map(fn, ctx, &mk, p, p.k, a.box_k)) return s;
+  if (g4a_status s = g4a_page_map(fn, ctx, &mv, p, p.v, a.box_v)) return s;
   const int pairs = std::min(ctx->num_sms / 2, kMaxPairs);
   const long long entries = (long long)p.tokens * p.group / kTileRows + std::min(p.batch, p.tokens);
   const long long items = entries * p.nkh * C::HALVES;
@@ -863,7 +755,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   a.pieces = q.pieces;
   a.cuts = q.cuts;
   g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
-  cudaError_t e = g4a_chunk_plan_launch(ctx, q);
+  cudaError_t e = g4a_chunk_plan_launch(ctx, q, false);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_plan_kernel");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));

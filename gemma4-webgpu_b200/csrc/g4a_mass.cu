@@ -1,41 +1,557 @@
 // The attention weight that every cached row gets from a chunk of tokens (g4a_paged_key_mass).  No reference
-// counterpart.
+// counterpart.  With the log-sum-exps that the attention has left,
+//   mass_r = decay mass_r + sum over the query rows that see r of 2^(scale log2e q k_r - lse log2e),
+// so K is read once more and V not at all.  Two kernels:
+//  - few query rows to a sequence (decode steps): a warp has 16 keys in registers, as the A operand of mma.sync
+//    m16n8k16, 8 query rows are its B operand.  The order of the dims in a product is free, so a lane loads 16
+//    consecutive bytes of its rows and uses them as they are: no shared memory, 8 or 16 KB in flight for each warp.
+//    Bound by the HBM.
+//  - chunks: S^T [256 keys x rows] = K Q^T by pairs of CTAs (tcgen05 cta_group::2), a thread is a key and adds up its
+//    weights in a register, so nothing is reduced across lanes; the row blocks of a key tile may be cut between
+//    pairs, and a last kernel adds the parts up in a fixed order.  Bound by the tensor cores and the exp2 unit
+//    together: a block of 128 keys x 128 rows of 256 dims takes 1,024 cycles of either.
 #include <algorithm>
+#include <atomic>
 
-#include "g4a_chunk.cuh"
+#include "g4a_chunk_pair.cuh"
 
 namespace {
 
 using namespace g4a;
 using namespace g4a_chunk;
 
-// One warp per (sequence, kv head, row).
-__global__ void __launch_bounds__(256) mass_simple_kernel(const ChunkParams p) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long cap = min((long long)p.max_pages * p.page_size, p.mass_stride);
-  const int b = blockIdx.y / p.nkh, kvh = blockIdx.y % p.nkh;
-  const Seq s = seq_of(p, b, cap);
-  for (int r = blockIdx.x * 8 + warp; r < s.L; r += gridDim.x * 8) {
-    const long long off = row_offset(p, b, kvh, r);
-    if (off < 0) continue;
-    float sum = 0.f;
-    for (int t = max(0, r - s.base()); t < s.T; t++) {
-      const int pos = s.base() + t;
-      if (!sees(p, pos, r)) continue;
-      for (int h = 0; h < p.group; h++) {
-        const size_t row = (size_t)(s.row0 + t) * p.nqh + kvh * p.group + h;
-        float x = 0.f;
-        for (int d = lane; d < p.hd; d += 32) x = fmaf(__half2float(p.q[row * p.hd + d]), __half2float(p.k[off + d]), x);
-        for (int w = 16; w >= 1; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        const float lse = p.lse[row];
-        if (lse != -INFINITY) sum += exp2f(x * p.scale_log2 - lse * kLog2eC);
+// ------------------------------------------------------------------------------------ few query rows
+
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+constexpr int kFewWarps = 8;
+
+// SEG: segments of 32 dims.  Lane 4 g + t holds dims 32 s + 8 t .. + 7 of keys g and g + 8 and of query row g.
+template <int SEG>
+__global__ void __launch_bounds__(kFewWarps * 32) mass_few_kernel(const ChunkParams p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const Seq s = seq_of(p, b, min((long long)p.max_pages * p.page_size, p.mass_stride));
+  const int base = s.base();
+  const __half* q = p.q + ((size_t)s.row0 * p.nqh + (size_t)kvh * p.group) * p.hd;
+  const float* lse = p.lse + (size_t)s.row0 * p.nqh + (size_t)kvh * p.group;
+  float* mass = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride;
+  for (int k0 = ((int)blockIdx.x * kFewWarps + warp) * 16; k0 < s.L; k0 += (int)gridDim.x * kFewWarps * 16) {
+    const Tokens see = tokens_of(p, s, k0, 16);
+    const bool any = see.first < see.last;
+    if (!any && p.decay == 1.f && k0 + 16 <= base) continue;  // nothing changes
+    long long off[2] = {-1, -1};
+    float old[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
+    uint4 k[2][SEG];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int key = k0 + g + 8 * h;
+      if (key < s.L) off[h] = row_offset(p, b, kvh, key);
+      if (t == 0 && off[h] >= 0 && key < base && p.decay != 0.f) old[h] = p.decay * mass[key];
+#pragma unroll
+      for (int e = 0; e < SEG; e++) {
+        const int d = e * 32 + t * 8;
+        k[h][e] = any && off[h] >= 0 && d < p.hd ? __ldg(reinterpret_cast<const uint4*>(p.k + off[h] + d)) : make_uint4(0, 0, 0, 0);
       }
     }
-    if (lane == 0) {
-      float* at = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride + r;
-      *at = r < s.base() && p.decay != 0.f ? fmaf(p.decay, *at, sum) : sum;
+    const long long r_end = (long long)see.last * p.group;
+    for (long long r0 = any ? (long long)see.first * p.group & ~7ll : r_end; r0 < r_end; r0 += 8) {
+      const bool live = r0 + g < (long long)s.T * p.group;
+      const int token = live ? (int)((uint32_t)(r0 + g) / (uint32_t)p.group) : 0;
+      const __half* row = q + ((size_t)token * p.nqh + (live ? (size_t)(r0 + g - (long long)token * p.group) : 0)) * p.hd;
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < SEG; e++) {
+        const int d = e * 32 + t * 8;
+        const uint4 x = live && d < p.hd ? __ldg(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+        mma_16x8x16(c, k[0][e].x, k[1][e].x, k[0][e].y, k[1][e].y, x.x, x.y);
+        mma_16x8x16(c, k[0][e].z, k[1][e].z, k[0][e].w, k[1][e].w, x.z, x.w);
+      }
+#pragma unroll
+      for (int n = 0; n < 2; n++) {  // query rows r0 + 2 t + n
+        const long long r = r0 + 2 * t + n;
+        if (r >= (long long)s.T * p.group) continue;
+        const int tok = (int)((uint32_t)r / (uint32_t)p.group);
+        const float z = lse[(size_t)tok * p.nqh + (size_t)(r - (long long)tok * p.group)];
+        if (z == -INFINITY) continue;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          if (sees(p, base + tok, k0 + g + 8 * h)) sum[h] += fast_exp2(fmaf(c[2 * h + n], p.scale_log2, -z * kLog2eC));
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+      if (t == 0 && off[h] >= 0) mass[k0 + g + 8 * h] = old[h] + sum[h];
     }
   }
+}
+
+// ------------------------------------------------------------------------------------------- chunks
+
+constexpr int kThreadsM = 512;
+constexpr int kTileLog2 = 8, kCtaKeys = 128;  // keys of a tile; of a CTA
+constexpr int kWarpK = 8, kWarpQ = 9, kWarpMma = 10, kWarpLse = 11, kWarpTell = 12;
+constexpr int kScoreBufs = 4, kInfoM = 4;
+
+template <int HD>
+struct Mc {
+  static constexpr int RB = HD > 256 ? 64 : 128;  // query rows of a block, half of them loaded by each CTA
+  static constexpr int NC = HD / 64;
+  static constexpr int K_CHUNK = kCtaKeys * 128, Q_CHUNK = RB / 2 * 128;
+  static constexpr int K_BYTES = NC * K_CHUNK, Q_BYTES = NC * Q_CHUNK;
+  static constexpr int NK = HD > 256 ? 1 : 2, NQ = HD <= 128 ? 4 : 2;
+  static constexpr int OFF_Q = NK * K_BYTES;
+  static constexpr int OFF_LSE = OFF_Q + NQ * Q_BYTES;            // [kInfoM][RB] -lse log2e
+  static constexpr int OFF_VALID = OFF_LSE + kInfoM * RB * 4;     // [kInfoM][4] rows that count
+  static constexpr int OFF_SUM = OFF_VALID + kInfoM * 16;         // [2][128] sums of the second set of warps
+  static constexpr int OFF_BAR = OFF_SUM + 2 * kCtaKeys * 4;
+  static constexpr int NBARS = 3 * NK + 3 * NQ + 2 * kScoreBufs + 2 * kInfoM + 5;
+  static constexpr size_t SMEM = 1024 + (size_t)OFF_BAR + NBARS * 8 + 16;
+  static constexpr uint32_t TMEM_COLS = 512;
+  static_assert(kScoreBufs * RB <= 512 && SMEM <= 232448, "tile fits");
+};
+
+struct MassParams {
+  ChunkParams c;
+  const Plan* plan;
+  const Piece* pieces;
+  const int4* seqs;
+  const int2* parts;
+  float* part;  // [2 * pairs][256]
+  int box_k;
+  int tokens, heads, head_chunks;  // of a CTA's half block; chunks of heads for a token
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kThreadsM, 1)
+    mass_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq, const MassParams a) {
+  using C = Mc<HD>;
+  const ChunkParams& p = a.c;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* k_landed = bars;                   // [NK] this CTA's keys
+  uint64_t* k_ready = k_landed + C::NK;        // [NK] first CTA: of both
+  uint64_t* k_free = k_ready + C::NK;          // [NK] the piece's scores done (commit)
+  uint64_t* q_landed = k_free + C::NK;         // [NQ] this CTA's half of a row block
+  uint64_t* q_ready = q_landed + C::NQ;        // [NQ] first CTA: both
+  uint64_t* q_free = q_ready + C::NQ;          // [NQ] scores done (commit)
+  uint64_t* s_done = q_free + C::NQ;           // [kScoreBufs] scores (commit)
+  uint64_t* s_free = s_done + kScoreBufs;      // [kScoreBufs] first CTA: read (4 warps of each)
+  uint64_t* lse_full = s_free + kScoreBufs;    // [kInfoM] the block's log-sum-exps are here
+  uint64_t* lse_free = lse_full + kInfoM;      // [kInfoM] read (4 warps)
+  uint64_t* sum_full = lse_free + kInfoM;      // [2] sums of the second set (4 warps)
+  uint64_t* sum_free = sum_full + 2;           // [2] read (4 warps)
+  uint64_t* all_done = sum_free + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cta_rank();
+  const uint32_t sbase = smem_u32(smem);
+  const int half_rows = a.tokens * a.heads;  // rows of a half block that are loaded
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::NK; s++) {
+      mbar_init(&k_landed[s], 1);
+      mbar_init(&k_ready[s], 2);
+      mbar_init(&k_free[s], 1);
+    }
+    for (int s = 0; s < C::NQ; s++) {
+      mbar_init(&q_landed[s], 1);
+      mbar_init(&q_ready[s], 2);
+      mbar_init(&q_free[s], 1);
+    }
+    for (int s = 0; s < kScoreBufs; s++) {
+      mbar_init(&s_done[s], 1);
+      mbar_init(&s_free[s], 8);
+    }
+    for (int s = 0; s < kInfoM; s++) {
+      mbar_init(&lse_full[s], 1);
+      mbar_init(&lse_free[s], 4);
+    }
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&sum_full[s], 4);
+      mbar_init(&sum_free[s], 4);
+    }
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmq)) : "memory");
+  }
+  // rows of a half block that no load fills are zeros for good
+  if (half_rows < C::RB / 2) {
+    for (int e = threadIdx.x; e < C::NQ * C::Q_BYTES / 16; e += kThreadsM)
+      *reinterpret_cast<uint4*>(smem + C::OFF_Q + e * 16) = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
+  __syncwarp();
+  if (warp == kWarpMma) {  // one CTA per SM (shared memory), so the allocation never waits
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  __syncwarp();
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+
+  const int pair = (int)(blockIdx.x >> 1);
+  const int begin = a.plan->first[pair], end = a.plan->first[pair + 1];
+  bool ok = true;
+  uint32_t g = 0, done = 0;  // blocks and pieces so far
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ weights and their sums
+    // Warps 0-3 take the even blocks, 4-7 the odd ones; a lane is a key.
+    const uint32_t set = (uint32_t)warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int key_in = rank * kCtaKeys + (warp & 3) * 32 + lane;
+    float* sums = reinterpret_cast<float*>(smem + C::OFF_SUM);
+    for (int i = begin; ok && i < end; i++, done++) {
+      const Piece d = a.pieces[i];
+      const int key = (d.tile << kTileLog2) + key_in, base = d.L - d.T;
+      // the tokens that see the key
+      const int see0 = key - base;
+      const int see1 = p.window == 0u || (uint32_t)key < p.sinks ? 0x7fffffff : (int)min(0x7fffffffll, (long long)see0 + p.window);
+      float2 acc[4] = {};
+      for (int j = d.j0; j < d.j1; j++, g++) {
+        if ((g & 1u) != set) continue;
+        const uint32_t buf = g % kScoreBufs, inf = g % kInfoM;
+        ok = warp_wait(&lse_full[inf], (g / kInfoM) & 1u, abort_flag, p.err) &&
+             warp_wait(&s_done[buf], (g / kScoreBufs) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        tc_fence_after();
+        const float* nl = reinterpret_cast<const float*>(smem + C::OFF_LSE) + inf * C::RB;
+        const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + C::OFF_VALID + inf * 16);
+        const int t0 = (d.skip + j / a.head_chunks) * 2 * a.tokens;
+        uint32_t all = valid[0] & valid[1];
+        if (C::RB == 128) all &= valid[2] & valid[3];
+        const bool plain = __all_sync(0xffffffffu, see0 <= t0 && see1 >= t0 + 2 * a.tokens) && all == 0xffffffffu;
+#pragma unroll
+        for (int c = 0; c < C::RB / 32; c++) {
+          uint32_t s[32];
+          tmem_get(lanes + buf * C::RB + 32u * c, s);
+          tmem_wait_ld();
+          tmem_landed(s);
+          if (c == C::RB / 32 - 1) {  // the buffer may be overwritten now
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(map_to(smem_u32(&s_free[buf]), 0));
+          }
+          uint32_t bits = 0xffffffffu;
+          if (!plain) {
+            // columns of this word that see the key: those of the tokens [see0, see1)
+            constexpr int kHalfWords = C::RB / 64;
+            const int th = t0 + (c / kHalfWords) * a.tokens, w0 = (c % kHalfWords) * 32;
+            const int lo = max(0, min(see0 - th, a.tokens)) * a.heads - w0, hi = max(0, min(see1 - th, a.tokens)) * a.heads - w0;
+            const uint32_t from = lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : ~((1u << lo) - 1u);
+            const uint32_t to = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u;
+            bits = from & to & valid[c];
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 z = *reinterpret_cast<const float4*>(nl + 32 * c + e);
+            float w[4];
+            w[0] = fast_exp2(fmaf(__uint_as_float(s[e]), p.scale_log2, z.x));
+            w[1] = fast_exp2(fmaf(__uint_as_float(s[e + 1]), p.scale_log2, z.y));
+            w[2] = fast_exp2(fmaf(__uint_as_float(s[e + 2]), p.scale_log2, z.z));
+            w[3] = fast_exp2(fmaf(__uint_as_float(s[e + 3]), p.scale_log2, z.w));
+            if (!plain) {
+#pragma unroll
+              for (int k = 0; k < 4; k++)
+                if (!((bits >> (e + k)) & 1u)) w[k] = 0.f;
+            }
+            acc[(e >> 1) & 3].x += w[0];
+            acc[(e >> 1) & 3].y += w[1];
+            acc[((e >> 1) + 1) & 3].x += w[2];
+            acc[((e >> 1) + 1) & 3].y += w[3];
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&lse_free[inf]);
+      }
+      if (!ok) break;
+      const float sum = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
+      float* meet = sums + (done & 1u) * kCtaKeys + (warp & 3) * 32 + lane;
+      if (set == 1) {
+        if (done >= 2) ok = warp_wait(&sum_free[done & 1u], ((done >> 1) - 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        *meet = sum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sum_full[done & 1u]);
+      } else {
+        ok = warp_wait(&sum_full[done & 1u], (done >> 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        const float whole = sum + *meet;
+        if (d.slot >= 0) {
+          a.part[(size_t)d.slot * (2 * kCtaKeys) + key_in] = whole;
+        } else if (key < d.L && row_offset(p, d.b, d.head, key) >= 0) {
+          float* at = p.mass + ((size_t)d.b * p.nkh + d.head) * p.mass_stride + key;
+          *at = key < base && p.decay != 0.f ? fmaf(p.decay, *at, whole) : whole;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sum_free[done & 1u]);
+      }
+    }
+  } else if (warp == kWarpK) {
+    // ------------------------------------------------------------------ keys
+    const int boxes = kCtaKeys / a.box_k, ops = boxes * C::NC;
+    for (int i = begin; ok && i < end; i++, done++) {
+      const Piece d = a.pieces[i];
+      const int* table = p.page_table + (size_t)d.b * p.max_pages;
+      const uint32_t s = done % C::NK;
+      if (done >= (uint32_t)C::NK) ok = warp_wait(&k_free[s], (done / C::NK - 1) & 1u, abort_flag, p.err);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&k_landed[s], (uint32_t)C::K_BYTES);
+      __syncwarp();
+      for (int o = lane; o < ops; o += 32) {
+        const int r = o / C::NC, c = o - r * C::NC;
+        const int key = (d.tile << kTileLog2) + rank * kCtaKeys + r * a.box_k;
+        int page = p.num_pages, row = 0;  // a page that is not there: zeros
+        if (key < d.L) {
+          const int t = key / p.page_size, id = table[t];
+          row = key - t * p.page_size;
+          if (id >= 0 && id < p.num_pages) page = id;
+        }
+        load_box(sbase + s * C::K_BYTES + c * C::K_CHUNK + r * a.box_k * 128, &tmk, 64 * c, d.head, row, page, &k_landed[s]);
+      }
+    }
+    for (uint32_t k = done > (uint32_t)C::NK ? done - C::NK : 0; k < done; k++)
+      (void)mbar_wait_bounded(&k_landed[k % C::NK], (k / C::NK) & 1u, p.err, G4A_DEVERR_WAIT_FULL);
+  } else if (warp == kWarpQ) {
+    // ------------------------------------------------------------------ queries
+    for (int i = begin; ok && i < end; i++) {
+      const Piece d = a.pieces[i];
+      for (int j = d.j0; j < d.j1; j++, g++) {
+        const uint32_t s = g % C::NQ;
+        if (g >= (uint32_t)C::NQ) ok = warp_wait(&q_free[s], (g / C::NQ - 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+        const int tb = j / a.head_chunks, hc = j - tb * a.head_chunks;
+        const long long token = (long long)d.row0 + ((long long)d.skip + tb) * 2 * a.tokens + rank * a.tokens;
+        if (lane == 0) mbar_arrive_expect_tx(&q_landed[s], (uint32_t)(C::NC * half_rows * 128));
+        __syncwarp();
+        if (lane < C::NC)
+          load_box(sbase + C::OFF_Q + s * C::Q_BYTES + lane * C::Q_CHUNK, &tmq, 64 * lane, hc * a.heads, d.head,
+                   (int)min(token, (long long)p.tokens), &q_landed[s]);
+      }
+    }
+    for (uint32_t k = g > (uint32_t)C::NQ ? g - C::NQ : 0; k < g; k++)
+      (void)mbar_wait_bounded(&q_landed[k % C::NQ], (k / C::NQ) & 1u, p.err, G4A_DEVERR_WAIT_FULL);
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------------------------ MMAs of both CTAs
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = pair_idesc(C::RB, false);
+      const uint64_t dk0 = sw128_desc(sbase, 16, 1024), dq0 = sw128_desc(sbase + C::OFF_Q, 16, 1024);
+      for (int i = begin; ok && i < end; i++, done++) {
+        const int n = a.pieces[i].j1 - a.pieces[i].j0;
+        ok = wait_pair(&k_ready[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err);
+        const uint64_t dk = dk0 + (uint64_t)(((done % C::NK) * C::K_BYTES) >> 4);
+        for (int j = 0; ok && j < n; j++, g++) {
+          const uint32_t s = g % C::NQ, buf = g % kScoreBufs;
+          if (g >= (uint32_t)kScoreBufs) ok = wait_pair(&s_free[buf], (g / kScoreBufs - 1) & 1u, abort_flag, p.err);
+          ok = ok && wait_pair(&q_ready[s], (g / C::NQ) & 1u, abort_flag, p.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dq = dq0 + (uint64_t)((s * C::Q_BYTES) >> 4);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; kk++) {
+            const uint64_t off = (uint64_t)(((kk & 3) * 32) >> 4);
+            mma2_ss(tmem + buf * C::RB, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
+                    dq + (uint64_t)(((kk >> 2) * C::Q_CHUNK) >> 4) + off, idesc, kk > 0 ? 1u : 0u);
+          }
+          commit2(&s_done[buf]);
+          commit2(&q_free[s]);
+        }
+        if (ok) commit2(&k_free[done % C::NK]);
+      }
+      // no MMA may still be running when TMEM is freed, also after an abort
+      commit2(all_done);
+      (void)mbar_wait_bounded(all_done, 0, p.err, G4A_DEVERR_WAIT_MMA);
+    }
+  } else if (warp == kWarpLse) {
+    // ------------------------------------------------------------------ log-sum-exps of the row blocks
+    for (int i = begin; ok && i < end; i++) {
+      const Piece d = a.pieces[i];
+      for (int j = d.j0; j < d.j1; j++, g++) {
+        const uint32_t inf = g % kInfoM;
+        const int tb = j / a.head_chunks, hc = j - tb * a.head_chunks;
+        const int t0 = (d.skip + tb) * 2 * a.tokens;
+        float z[C::RB / 32];
+#pragma unroll
+        for (int c = 0; c < C::RB / 32; c++) {
+          constexpr int kHalfWords = C::RB / 64;
+          const int in = (c % kHalfWords) * 32 + lane, tok = t0 + (c / kHalfWords) * a.tokens + in / a.heads;
+          const int head = hc * a.heads + in % a.heads;
+          z[c] = -INFINITY;
+          if (in >= half_rows) z[c] = INFINITY;  // a column that is never anything (its query is zero): weight 0
+          else if (tok < d.T && head < p.group)
+            z[c] = p.lse[(size_t)(d.row0 + tok) * p.nqh + (size_t)d.head * p.group + head];
+        }
+        if (g >= (uint32_t)kInfoM) ok = warp_wait(&lse_free[inf], (g / kInfoM - 1) & 1u, abort_flag, p.err);
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < C::RB / 32; c++) {
+          const uint32_t bits = __ballot_sync(0xffffffffu, z[c] != -INFINITY);
+          reinterpret_cast<float*>(smem + C::OFF_LSE)[inf * C::RB + 32 * c + lane] = z[c] == -INFINITY ? 0.f : -z[c] * kLog2eC;
+          if (lane == 0) reinterpret_cast<uint32_t*>(smem + C::OFF_VALID + inf * 16)[c] = bits;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&lse_full[inf]);
+      }
+    }
+  } else if (warp == kWarpTell) {
+    // ------------------------------------------------------------------ what has landed in this CTA
+    if (lane == 0) {
+      for (int i = begin; ok && i < end; i++, done++) {
+        ok = wait_or_abort(&k_landed[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+        if (!ok) break;
+        arrive_at(map_to(smem_u32(&k_ready[done % C::NK]), 0));
+        const int n = a.pieces[i].j1 - a.pieces[i].j0;
+        for (int j = 0; j < n; j++, g++) {
+          ok = wait_or_abort(&q_landed[g % C::NQ], (g / C::NQ) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+          if (!ok) break;
+          arrive_at(map_to(smem_u32(&q_ready[g % C::NQ]), 0));
+        }
+      }
+    }
+  }
+  // a warp that gave up stops the partner's waits too (it leaves only through the pair's barrier)
+  __syncwarp();
+  if (lane == 0 && *abort_flag)
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(smem_u32((const void*)abort_flag), (uint32_t)rank ^ 1u)),
+                 "r"(1u)
+                 : "memory");
+  __syncwarp();
+  tc_fence_before();
+  pair_sync();
+  tc_fence_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+}
+
+// Adds up the parts of the tiles that were cut, and lets the rows fade that no token saw.
+__global__ void __launch_bounds__(256) mass_join_kernel(const MassParams a) {
+  const ChunkParams& p = a.c;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
+  const Seq s = seq_of(p, b, min((long long)p.max_pages * p.page_size, p.mass_stride));
+  const Blocks k = key_tiles_of(p, s, kTileLog2);
+  const int item0 = a.seqs[b].y + kvh * k.count();
+  for (int tile = (int)blockIdx.x; tile << kTileLog2 < s.L; tile += (int)gridDim.x) {
+    const int r = (tile << kTileLog2) + (int)threadIdx.x;
+    const int e = tile < k.sinks ? tile : tile >= k.window0 && tile < k.window1 ? tile - k.window0 + k.sinks : -1;
+    const int2 parts = e >= 0 ? a.parts[item0 + e] : make_int2(0, 0);
+    if (parts.y == 1 || (parts.y == 0 && p.decay == 1.f)) continue;
+    if (r >= s.L || row_offset(p, b, kvh, r) < 0) continue;
+    float sum = 0.f;
+    for (int i = 0; i < parts.y; i++) sum += a.part[(size_t)(parts.x + i) * (2 * kCtaKeys) + threadIdx.x];
+    float* at = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride + r;
+    *at = r < s.base() && p.decay != 0.f ? fmaf(p.decay, *at, sum) : sum;
+  }
+}
+
+template <int HD>
+g4a_status launch_chunk_mass(const char* fn, g4a_ctx* ctx, const ChunkParams& p) {
+  using C = Mc<HD>;
+  static std::atomic<bool> ready[64];
+  if (ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(mass_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(mass_tc_kernel)");
+    if (ctx->device < 64) ready[ctx->device].store(true, std::memory_order_release);
+  }
+  MassParams a = {};
+  a.c = p;
+  a.heads = std::min(p.group, C::RB / 2);
+  a.tokens = C::RB / 2 / a.heads;
+  a.head_chunks = (p.group + a.heads - 1) / a.heads;
+  a.box_k = std::min(p.page_size & -p.page_size, kCtaKeys);
+  CUtensorMap mk, mq;
+  if (g4a_status s = g4a_page_map(fn, ctx, &mk, p, p.k, a.box_k)) return s;
+  if (g4a_status s = g4a_query_map(fn, ctx, &mq, p, a.heads, a.tokens)) return s;
+  const int pairs = std::min(ctx->num_sms / 2, kMaxPairs);
+  // key tiles of all sequences, by the room that they have
+  const long long rows = std::min<long long>((long long)p.page_size * p.max_pages, p.mass_stride);
+  const long long entries = (long long)std::min(p.batch, p.tokens) * ((rows >> kTileLog2) + 2), items = entries * p.nkh;
+  if (items > (1 << 26)) return g4a_fail(G4A_EINVAL, "%s: batch * num_kv_heads * rows too large", fn);
+  const long long pieces = items + pairs;
+  auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
+  const size_t n_part = up((size_t)2 * pairs * 2 * kCtaKeys * sizeof(float)), n_plan = up(sizeof(Plan));
+  const size_t n_piece = up((size_t)pieces * sizeof(Piece)), n_parts = up((size_t)items * sizeof(int2));
+  const size_t n_seq = up((size_t)(p.batch + 1) * sizeof(int4)), n_entry = up((size_t)entries * sizeof(long long));
+  if (g4a_status s = g4a_ensure_workspace(ctx, n_part + n_plan + n_piece + n_parts + n_seq + n_entry)) return s;
+  char* ws = static_cast<char*>(ctx->workspace);
+  PlanParams q = {};
+  q.c = p;
+  q.pairs = pairs;
+  q.halves = 1;
+  q.kb_log2 = kTileLog2;
+  q.stage_ns = 1.f;
+  q.block_tokens = 2 * a.tokens;
+  q.head_chunks = a.head_chunks;
+  a.part = reinterpret_cast<float*>(ws);
+  q.plan = reinterpret_cast<Plan*>(ws += n_part);
+  q.pieces = reinterpret_cast<Piece*>(ws += n_plan);
+  q.parts = reinterpret_cast<int2*>(ws += n_piece);
+  q.seqs = reinterpret_cast<int4*>(ws += n_parts);
+  q.entries = reinterpret_cast<long long*>(ws += n_seq);
+  a.plan = q.plan;
+  a.pieces = q.pieces;
+  a.parts = q.parts;
+  a.seqs = q.seqs;
+  g4a_prof_scope ps(ctx, G4A_PROF_KEY_MASS);
+  cudaError_t e = g4a_chunk_plan_launch(ctx, q, true);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_plan_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(kThreadsM);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  e = cudaLaunchKernelEx(&cfg, mass_tc_kernel<HD>, mk, mq, a);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_tc_kernel");
+  const unsigned heads = (unsigned)p.batch * (unsigned)p.nkh;
+  const unsigned wide = (unsigned)std::min<long long>((rows + 255) / 256, std::max(1u, 4096u / heads));
+  e = g4a_launch(mass_join_kernel, dim3(wide, heads), dim3(256), 0, ctx->stream, true, a);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_join_kernel");
+  return G4A_OK;
+}
+
+template <int SEG>
+g4a_status launch_few(g4a_ctx* ctx, const ChunkParams& p) {
+  g4a_prof_scope ps(ctx, G4A_PROF_KEY_MASS);
+  const unsigned heads = (unsigned)p.batch * (unsigned)p.nkh;
+  const long long rows = std::min<long long>((long long)p.page_size * p.max_pages, p.mass_stride);
+  const unsigned wide = (unsigned)std::min<long long>((rows + kFewWarps * 16 - 1) / (kFewWarps * 16),
+                                                      std::max(1u, 32u * (unsigned)ctx->num_sms / heads));
+  const cudaError_t e = g4a_launch(mass_few_kernel<SEG>, dim3(wide, heads), dim3(kFewWarps * 32), 0, ctx->stream, true, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_few_kernel");
+  return G4A_OK;
 }
 
 }  // namespace
@@ -65,10 +581,11 @@ extern "C" g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const 
   p.mass = mass;
   p.mass_stride = (long long)mass_stride;
   p.decay = decay;
-  g4a_prof_scope ps(ctx, G4A_PROF_KEY_MASS);
-  const long long rows = std::min<long long>((long long)page_size * max_pages_per_seq, (long long)mass_stride);
-  const cudaError_t e = g4a_launch(mass_simple_kernel, dim3((unsigned)std::min<long long>((rows + 7) / 8, 4096), batch * num_kv_heads),
-                                   dim3(256), 0, ctx->stream, false, p);
-  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_simple_kernel");
-  return G4A_OK;
+  if ((uint64_t)batch * num_kv_heads > 65535u)
+    return g4a_fail(G4A_EINVAL, "%s: batch %u * num_kv_heads %u exceeds 65535", fn, batch, num_kv_heads);
+  // query rows of a sequence, on average
+  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 32u * (uint64_t)batch;
+  if (head_dim > 256) return few ? launch_few<16>(ctx, p) : launch_chunk_mass<512>(fn, ctx, p);
+  if (head_dim > 128) return few ? launch_few<8>(ctx, p) : launch_chunk_mass<256>(fn, ctx, p);
+  return few ? launch_few<4>(ctx, p) : launch_chunk_mass<128>(fn, ctx, p);
 }

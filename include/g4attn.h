@@ -530,7 +530,7 @@ g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t*
  * over those that see r, with q and lse as in g4a_chunk_attn_paged.  The T new rows start from 0, whatever
  * their entries held; decay 0 does the same for all rows.  0 <= decay <= 1.  mass_stride >= the largest
  * kv_lens[b] (a longer sequence is skipped and reported); entries behind kv_lens[b] stay as they were.
- * A q row whose lse is -inf adds nothing; a call without tokens (num_tokens 0) does nothing.  Sums are f32 in an order that does not change from run to run. */
+ * A q row whose lse is -inf adds nothing; a call without tokens (num_tokens 0) does nothing.  Sums are f32 in an order that does not change from run to run.  batch * num_kv_heads <= 65535. */
 g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const float* lse, const uint16_t* k_pages,
                               const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_indptr,
                               uint32_t num_tokens, uint32_t batch, uint32_t page_size,
