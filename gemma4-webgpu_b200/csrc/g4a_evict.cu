@@ -1,6 +1,7 @@
 // A paged cache brought down to a budget of rows (g4a_paged_kv_evict): for each sequence and kv head the first
 // rows, the last ones and the heaviest between stay and are moved together.  No reference counterpart.
 #include <algorithm>
+#include <atomic>
 
 #include "g4a_internal.cuh"
 
@@ -8,7 +9,11 @@ namespace {
 
 using namespace g4a;
 
-constexpr int kThreadsE = 1024;
+constexpr int kThreadsE = 1024;      // of a selecting CTA
+constexpr int kBinsE = 2048;
+constexpr int kCacheE = 40 * 1024;   // weights that a CTA keeps in shared memory
+constexpr int kMaxCluster = 8;
+constexpr int kMoveThreads = 256, kMoveFly = 4;
 
 struct EvictParams {
   __half *k, *v;
@@ -17,7 +22,13 @@ struct EvictParams {
   long long mass_stride;
   int batch, budget, sinks, recent, page_size, max_pages, num_pages, nkh, hd;
   int *new_lens, *kept;
-  int* idx;  // workspace: [batch, nkh, budget]
+  int cap;        // rows that a sequence can have
+  int rows;       // rows of a block that is moved at once
+  int blocks;     // of them in a budget
+  int* idx;       // [batch, nkh, budget] old numbers of the kept rows
+  int* rank;      // [batch, nkh, blocks + 1] kept rows before row `rows` * block
+  int* read;      // [batch, nkh, blocks] 1: the block's rows have been read
+  int* ticket;
   int* err;
 };
 
@@ -37,113 +48,232 @@ __device__ __forceinline__ long long row_at(const EvictParams& p, int b, int kvh
   return (((long long)page * p.page_size + (row - j * p.page_size)) * p.nkh + kvh) * p.hd;
 }
 
-// One CTA per (sequence, kv head): the border weight by four passes of a radix search, the kept rows' numbers in
-// order, then the rows in batches, all of a batch read before any of it is written.
-__global__ void __launch_bounds__(kThreadsE) evict_simple_kernel(const EvictParams p) {
-  __shared__ int hist[256], warp_sum[32][2], carry[2];
-  __shared__ uint32_t prefix_s;
-  __shared__ int need_s;
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_meet() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A word of CTA `rank`'s shared memory.
+__device__ __forceinline__ int peek(const int* at, uint32_t rank) {
+  uint32_t addr;
+  int x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_u32(at)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// One cluster of CTAs per (sequence, kv head), each with a slice of the rows between the first and the last ones, in
+// order.  The border weight is found digit by digit (11, 11 and 10 bits from the top): every CTA counts its slice,
+// all read each other's counts through distributed shared memory.  Then a warp knows how many rows before its own are
+// kept, and writes the numbers of its kept rows in order.  Latency: three counts and four meetings of the cluster.
+__global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictParams p) {
+  extern __shared__ uint32_t cache[];
+  __shared__ int hist[3][kBinsE], warp_sum[32], warp_gt[32], warp_tie[32], slice_gt, slice_tie, digit_s, need_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / p.nkh, kvh = blockIdx.x % p.nkh;
-  const int n = p.kv_lens[b];
-  const long long cap = min((long long)p.max_pages * p.page_size, p.mass_stride);
-  int* idx = p.idx + ((size_t)b * p.nkh + kvh) * p.budget;
-  int* kept = p.kept ? p.kept + ((size_t)b * p.nkh + kvh) * p.budget : nullptr;
-  if (kvh == 0 && tid == 0) p.new_lens[b] = n < 0 || n > cap ? n : min(n, p.budget);
-  if (n < 0 || n > cap) {
+  const uint32_t rank = cluster_rank(), ctas = cluster_size();
+  const int item = (int)(blockIdx.x / ctas), b = item / p.nkh, kvh = item % p.nkh;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (blockIdx.x == 0 && tid == 0) *p.ticket = 0;
+  const int n = p.kv_lens[b], budget = p.budget;
+  int* kept = p.kept ? p.kept + (size_t)item * budget : nullptr;
+  if (kvh == 0 && rank == 0 && tid == 0) p.new_lens[b] = n < 0 || n > p.cap ? n : min(n, budget);
+  if (n < 0 || n > p.cap) {  // (the same for the whole cluster, as the next)
     if (tid == 0) atomicExch(p.err, G4A_DEVERR_TREE);
     return;
   }
-  if (n <= p.budget) {
+  if (n <= budget) {
     if (kept)
-      for (int i = tid; i < p.budget; i += kThreadsE) kept[i] = i < n ? i : -1;
+      for (int i = (int)rank * kThreadsE + tid; i < budget; i += (int)ctas * kThreadsE) kept[i] = i < n ? i : -1;
     return;
   }
-  float* mass = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride;
-  const int first = p.sinks, end = n - p.recent, want = p.budget - p.sinks - p.recent;
-  uint32_t prefix = 0, mask = 0;
-  int need = want;
-  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kThreadsE) hist[i] = 0;
-    __syncthreads();
-    for (int i = first + tid; i < end; i += kThreadsE) {
-      const uint32_t o = order_of(mass[i]);
-      if ((o & mask) == prefix) atomicAdd(&hist[(o >> shift) & 255], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int d = 255;
-      for (; d > 0 && need > hist[d]; d--) need -= hist[d];
-      prefix_s = prefix | ((uint32_t)d << shift);
-      need_s = need;
-    }
-    __syncthreads();
-    prefix = prefix_s;
-    need = need_s;
-    mask |= 0xffu << shift;
-    __syncthreads();
-  }
-  // of the rows at the border weight `prefix` the first `need` stay
-  if (tid < 2) carry[tid] = 0;
+  int* idx = p.idx + (size_t)item * budget;
+  int* ranks = p.rank + (size_t)item * (p.blocks + 1);
+  for (int i = (int)rank * kThreadsE + tid; i < p.blocks; i += (int)ctas * kThreadsE) p.read[(size_t)item * p.blocks + i] = 0;
+  const float* mass = p.mass + (size_t)item * p.mass_stride;
+  const int first = p.sinks, end = n - p.recent, want = budget - p.sinks - p.recent, middle = end - first;
+  // slices of whole warps' rows
+  const int per_warp = ((middle + (int)ctas * 32 - 1) / ((int)ctas * 32) + 31) & ~31, slice = per_warp * 32;
+  const int at0 = first + (int)rank * slice, count = max(0, min(slice, end - at0));
+  const bool cached = count <= kCacheE;
+  for (int i = tid; i < count && cached; i += kThreadsE) cache[i] = order_of(mass[at0 + i]);
+  auto key_of = [&](int i) { return cached ? cache[i] : order_of(mass[at0 + i]); };
+  for (int i = tid; i < 3 * kBinsE; i += kThreadsE) hist[0][i] = 0;
   __syncthreads();
-  for (int i0 = 0; i0 < n; i0 += kThreadsE) {
-    const int i = i0 + tid;
-    bool sure = false, tie = false;
-    if (i < n) {
-      sure = i < first || i >= end;
-      if (!sure && want > 0) {
-        const uint32_t o = order_of(mass[i]);
-        sure = o > prefix;
-        tie = o == prefix;
-      }
+  uint32_t border = 0, mask = 0;
+  int need = want;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; pass++) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    int* h = hist[pass];
+    for (int i = tid; i < count; i += kThreadsE) {
+      const uint32_t o = key_of(i);
+      if ((o & mask) == border) atomicAdd(&h[(o >> shift) & (bins - 1)], 1);
     }
-    const unsigned ts = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) warp_sum[warp][0] = __popc(ts);
+    cluster_meet();
+    // bins from the top, two to a thread: the one in which the number of larger ones reaches `need`
+    int c[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int bin = kBinsE - 1 - (2 * tid + e);
+      if (bin < bins)
+        for (uint32_t r = 0; r < ctas; r++) c[e] += peek(&h[bin], r);
+    }
+    int incl = c[0] + c[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    int before = carry[0];
-    for (int w = 0; w < warp; w++) before += warp_sum[w][0];
-    const bool keep = sure || (tie && before + __popc(ts & ((1u << lane) - 1)) < need);
-    const unsigned ks = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) warp_sum[warp][1] = __popc(ks);
+    int before = incl - c[0] - c[1];
+    for (int w = 0; w < warp; w++) before += warp_sum[w];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      if (c[e] > 0 && before < need && before + c[e] >= need) digit_s = kBinsE - 1 - (2 * tid + e), need_s = need - before;
+      before += c[e];
+    }
     __syncthreads();
-    int at = carry[1];
-    for (int w = 0; w < warp; w++) at += warp_sum[w][1];
-    if (keep) idx[at + __popc(ks & ((1u << lane) - 1))] = i;
-    __syncthreads();
-    if (tid == 0)
-      for (int w = 0; w < 32; w++) carry[0] += warp_sum[w][0], carry[1] += warp_sum[w][1];
-    __syncthreads();
+    if (want > 0) {
+      border |= (uint32_t)digit_s << shift;
+      need = need_s;
+    }
+    mask |= (uint32_t)(bins - 1) << shift;
   }
-  const int per = p.hd / 8, rows = kThreadsE / per, sub = tid / per, col = tid - sub * per;
-  for (int i0 = 0; i0 < p.budget; i0 += rows) {
-    const int i = i0 + sub;
-    long long src = -1, dst = -1;
-    uint4 xk, xv;
-    float w = 0.f;
-    int from = -1;
-    if (sub < rows && i < p.budget) {
-      from = idx[i];
-      if (kept && col == 0) kept[i] = from;
-      if (from != i) {
-        src = row_at(p, b, kvh, from);
-        dst = row_at(p, b, kvh, i);
-        w = mass[from];
-        if (src >= 0 && dst >= 0) {
-          xk = reinterpret_cast<const uint4*>(p.k + src)[col];
-          xv = reinterpret_cast<const uint4*>(p.v + src)[col];
-        }
-      }
-    }
-    __syncthreads();
-    if (from >= 0 && from != i) {
-      if (col == 0) mass[i] = w;
-      if (src >= 0 && dst >= 0) {
-        reinterpret_cast<uint4*>(p.k + dst)[col] = xk;
-        reinterpret_cast<uint4*>(p.v + dst)[col] = xv;
-      }
-    }
-    __syncthreads();
+  // ---- of the rows at the border the first `need` stay
+  const int w0 = warp * per_warp, w1 = min(count, w0 + per_warp);
+  int gt = 0, tie = 0;
+  for (int i = w0; i < w1; i += 32) {
+    const uint32_t o = i + lane < w1 ? key_of(i + lane) : 0u;
+    const bool in = i + lane < w1 && want > 0;
+    gt += __popc(__ballot_sync(0xffffffffu, in && o > border));
+    tie += __popc(__ballot_sync(0xffffffffu, in && o == border));
   }
+  if (lane == 0) warp_gt[warp] = gt, warp_tie[warp] = tie;
+  __syncthreads();
+  if (warp == 0) {
+    const int g = __reduce_add_sync(0xffffffffu, warp_gt[lane]), t = __reduce_add_sync(0xffffffffu, warp_tie[lane]);
+    if (lane == 0) slice_gt = g, slice_tie = t;
+  }
+  cluster_meet();
+  int ties = 0, at = first;  // before this warp
+  for (uint32_t r = 0; r < rank; r++) {
+    const int t = peek(&slice_tie, r);
+    at += peek(&slice_gt, r) + max(0, min(t, need - ties));
+    ties += t;
+  }
+  for (int w = 0; w < warp; w++) {
+    at += warp_gt[w] + max(0, min(warp_tie[w], need - ties));
+    ties += warp_tie[w];
+  }
+  for (int i = w0; i < w1; i += 32) {
+    const int row = at0 + i + lane;
+    const bool in = i + lane < w1 && want > 0;
+    const uint32_t o = in ? key_of(i + lane) : 0u;
+    const unsigned tb = __ballot_sync(0xffffffffu, in && o == border), below = (1u << lane) - 1u;
+    const bool keep = in && (o > border || (o == border && ties + __popc(tb & below) < need));
+    const unsigned kb = __ballot_sync(0xffffffffu, keep);
+    const int j = at + __popc(kb & below);
+    if (keep) {
+      idx[j] = row;
+      if (kept) kept[j] = row;
+    }
+    if (i + lane < w1 && row <= p.blocks * p.rows && row % p.rows == 0) ranks[row / p.rows] = j;
+    at += __popc(kb);
+    ties += __popc(tb);
+  }
+  // the first and the last rows
+  for (int i = (int)rank * kThreadsE + tid; i < first + p.recent; i += (int)ctas * kThreadsE) {
+    const int row = i < first ? i : end + (i - first), j = i < first ? i : budget - p.recent + (i - first);
+    idx[j] = row;
+    if (kept) kept[j] = row;
+    if (row <= p.blocks * p.rows && row % p.rows == 0) ranks[row / p.rows] = j;
+  }
+  cluster_meet();  // nobody reads this CTA's counts any more
+}
+
+// Moves the rows.  Row j comes from row idx[j] >= j, and a block of rows may be written once every row that comes from its place
+// has been read; those belong to this block and two before it at most.  So a block is read into registers, says so, waits
+// for the blocks before it whose rows come from its place, and is written: each byte moves once, all SMs at work.
+// Blocks are taken by ticket, in order, and a block reads before it waits, so those that it waits for always get on; the
+// wait is bounded all the same (a block that gives up writes nothing and reports it).
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
+  __shared__ int ticket_s, ok_s;
+  const int tid = threadIdx.x;
+  pdl_wait_primary();
+  pdl_launch_dependents();
+  if (tid == 0) ticket_s = atomicAdd(p.ticket, 1), ok_s = 1;
+  __syncthreads();
+  const int item = ticket_s / p.blocks, block = ticket_s % p.blocks, b = item / p.nkh, kvh = item % p.nkh;
+  const int n = p.kv_lens[b];
+  if (n <= p.budget || n > p.cap) return;
+  const int* idx = p.idx + (size_t)item * p.budget;
+  const int j0 = block * p.rows, j1 = min(p.budget, j0 + p.rows);
+  if (idx[j1 - 1] == j1 - 1) return;  // all of them are where they were, and nobody waits for them
+  // the rows whose places lie in this block's come from rows [rank of its begin, rank of its end)
+  const int* ranks = p.rank + (size_t)item * (p.blocks + 1);
+  const int last = (block + 1) * p.rows < n ? ranks[block + 1] : p.budget;
+  const int wait0 = ranks[block] / p.rows, wait1 = min(block, (last - 1) / p.rows + 1);
+  int* read = p.read + (size_t)item * p.blocks;
+  float* mass = p.mass + (size_t)item * p.mass_stride;
+  const int per = p.hd / 8;
+  uint4 xk[kMoveFly], xv[kMoveFly];
+  long long dst[kMoveFly];
+  float w = 0.f;
+  int from = -1;
+#pragma unroll
+  for (int u = 0; u < kMoveFly; u++) {
+    const int c = tid + u * kMoveThreads, r = c / per, col = c - r * per, j = j0 + r;
+    dst[u] = -1;
+    if (r >= p.rows || j >= j1) continue;
+    const int i = idx[j];
+    if (i == j) continue;
+    const long long src = row_at(p, b, kvh, i), to = row_at(p, b, kvh, j);
+    if (src < 0 || to < 0) continue;
+    dst[u] = to + col * 8;
+    xk[u] = *reinterpret_cast<const uint4*>(p.k + src + col * 8);
+    xv[u] = *reinterpret_cast<const uint4*>(p.v + src + col * 8);
+  }
+  if (j0 + tid < j1) {
+    from = idx[j0 + tid];
+    w = mass[from];
+  }
+  __threadfence();  // each thread's reads are done
+  __syncthreads();
+  if (tid == 0) asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(read + block), "r"(1) : "memory");
+  if (wait0 + tid < wait1) {
+    const uint64_t t0 = globaltimer_ns();
+    int done = 0;
+    while (true) {
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(read + wait0 + tid) : "memory");
+      if (done) break;
+      if (globaltimer_ns() - t0 > 2000000000ull) {
+        ok_s = 0;
+        atomicExch(p.err, G4A_DEVERR_WAIT_FULL);
+        break;
+      }
+    }
+  }
+  __syncthreads();
+  if (!ok_s) return;
+#pragma unroll
+  for (int u = 0; u < kMoveFly; u++) {
+    if (dst[u] < 0) continue;
+    *reinterpret_cast<uint4*>(p.k + dst[u]) = xk[u];
+    *reinterpret_cast<uint4*>(p.v + dst[u]) = xv[u];
+  }
+  if (from >= 0) mass[j0 + tid] = w;
 }
 
 }  // namespace
@@ -199,11 +329,52 @@ extern "C" g4a_status g4a_paged_kv_evict(g4a_ctx* ctx, uint16_t* k_pages, uint16
   p.new_lens = new_lens;
   p.kept = kept;
   p.err = ctx->dev_err_dev;
-  if (g4a_status s = g4a_ensure_workspace(ctx, (size_t)batch * num_kv_heads * budget * sizeof(int))) return s;
-  p.idx = static_cast<int*>(ctx->workspace);
+  const uint64_t cap = std::min<uint64_t>((uint64_t)page_size * max_pages_per_seq, mass_stride);
+  const long long items = (long long)batch * num_kv_heads;
+  p.cap = (int)cap;
+  p.rows = std::min(kMoveThreads, kMoveThreads * kMoveFly / (p.hd / 8));
+  const bool any = budget < cap;  // whether a sequence can have more rows than the budget
+  p.blocks = any ? (p.budget + p.rows - 1) / p.rows : 1;
+  if (any && items * (p.blocks + 1ll) > 0x7fffffffll) return g4a_fail(G4A_EINVAL, "%s: batch * num_kv_heads * budget too large", fn);
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  const size_t n_idx = any ? up((size_t)items * budget * sizeof(int)) : 0, n_block = any ? up((size_t)items * (p.blocks + 1) * sizeof(int)) : 0;
+  if (g4a_status s = g4a_ensure_workspace(ctx, 256 + n_idx + 2 * n_block)) return s;
+  char* ws = static_cast<char*>(ctx->workspace);
+  p.ticket = reinterpret_cast<int*>(ws);
+  p.idx = reinterpret_cast<int*>(ws += 256);
+  p.rank = reinterpret_cast<int*>(ws += n_idx);
+  p.read = reinterpret_cast<int*>(ws += n_block);
+  static std::atomic<bool> ready[64];
+  const size_t smem = kCacheE * sizeof(uint32_t);
+  if (ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(evict_select_kernel)");
+    if (ctx->device < 64) ready[ctx->device].store(true, std::memory_order_release);
+  }
+  // CTAs of a cluster: slices of some 4,096 rows, as far as there are SMs
+  int ctas = 1;
+  while (ctas < kMaxCluster && cap > (uint64_t)ctas * 4096 && 2 * ctas * items <= ctx->num_sms) ctas *= 2;
+  if (items * ctas > 0x7fffffffll) return g4a_fail(G4A_EINVAL, "%s: batch * num_kv_heads too large", fn);
   g4a_prof_scope ps(ctx, G4A_PROF_PAGED_EVICT);
-  const cudaError_t e =
-      g4a_launch(evict_simple_kernel, dim3(batch * num_kv_heads), dim3(kThreadsE), 0, ctx->stream, false, p);
-  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch evict_simple_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * ctas));
+  cfg.blockDim = dim3(kThreadsE);
+  cfg.dynamicSmemBytes = any ? std::min(smem, (size_t)((cap / ctas + 1024 + 31) & ~31ull) * sizeof(uint32_t)) : 0;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
+  if (e != cudaSuccess) return g4a_cuda_fail(e, "launch evict_select_kernel");
+  if (any) {
+    e = g4a_launch(evict_move_kernel, dim3((unsigned)(items * p.blocks)), dim3(kMoveThreads), 0, ctx->stream, true, p);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "launch evict_move_kernel");
+  }
   return G4A_OK;
 }
