@@ -26,8 +26,14 @@ __device__ __forceinline__ void pair_sync() {
       "barrier.cluster.arrive.release.aligned;\n\t"
       "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+// Arrivals on a barrier of either CTA.  publish_at is for a thread whose stores to shared memory the other CTA's waits have
+// to see: it drains all that the thread has under way, 1,300 to 1,800 cycles.  arrive_at orders what is not stored by
+// plain stores: TMEM accesses (behind a tcgen05 fence) and copies whose arrival this thread has seen.
+__device__ __forceinline__ void publish_at(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 __device__ __forceinline__ bool try_wait_pair(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -40,17 +46,19 @@ __device__ __forceinline__ bool try_wait_pair(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded wait for arrivals of both CTAs.
-__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
-  if (try_wait_pair(bar, parity)) return true;
-  if (*abort_flag) return false;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t spins = 0;
-  while (true) {
-    if (try_wait_pair(bar, parity)) return true;
-    if ((++spins & 63u) == 0u) {
+// Bounded waits: for arrivals of both CTAs, of this one alone.  The timer is looked at only after a number of tries
+// (reading it takes longer than most waits).
+template <bool PAIR>
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  uint64_t t0 = 0;
+  for (uint32_t spins = 1;; spins++) {
+    if (PAIR ? try_wait_pair(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if ((spins & 63u) == 0u) {
       if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > 2000000000ull) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > 2000000000ull) {
         *abort_flag = 1;
         if (err) atomicExch(err, G4A_DEVERR_WAIT_MMA);
         return false;
@@ -58,29 +66,50 @@ __device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volati
     }
   }
 }
-// D (+)= A B^T on the pair: M 256, rows 128 c .. of D and A in CTA c, half of B's rows in each.
-__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ bool wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  return wait_bar<true>(bar, parity, abort_flag, err);
+}
+__device__ __forceinline__ bool wait_own(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  return wait_bar<false>(bar, parity, abort_flag, err);
+}
+__device__ __forceinline__ bool warp_wait_pair(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xffffffffu, wait_pair(bar, parity, abort_flag, err));
+}
+__device__ __forceinline__ bool warp_wait_own(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  return __all_sync(0xffffffffu, wait_own(bar, parity, abort_flag, err));
+}
+
+// D (+)= A B^T on the pair: M 256, rows 128 c .. of D and A in CTA c, half of B's rows in each.  Issued by the lane for
+// which `on` is not 0; the instructions are predicated, not branched to, so that the warp's control flow stays uniform
+// and the descriptors in uniform registers (11 cycles to issue one instead of 45, and 80 beside busy softmax warps).
+__device__ __forceinline__ void mma2_ss(uint32_t on, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(on)
       : "memory");
 }
-__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma2_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(on)
       : "memory");
 }
 // Arrive on `bar` of both CTAs when the MMAs issued so far have completed.
-__device__ __forceinline__ void commit2(uint64_t* bar) {
+__device__ __forceinline__ void commit2(uint32_t on, uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
           smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"((uint16_t)3), "r"(on)
       : "memory");
 }
 __host__ __device__ constexpr uint32_t pair_idesc(int n, bool b_mn_major) {

@@ -6,20 +6,20 @@
 // the L2 for 64 bytes per cycle at the tensor cores' full rate, which is all that an SM gets.
 //   S [256 x KB]  = Q K^T    A = Q (each CTA's 128 rows), B = K block, half of its keys in each CTA
 //   O [256 x HDV] += P V     A = P from TMEM, where the scores were, B = V block, half of its dims in each CTA
-// One pass over the keys with a running row maximum m and sum l: p = 2^(s - m + 7), rounded to f16 for the product
-// with V and summed unrounded; m is raised only when a score passes it by 2^8 (p <= 2^15 stays in f16), and only
-// then O is rescaled.  KB is 128 keys.  Heads of more than 256 dims: O takes 256 TMEM columns, so the dims of V are
+// One pass over the keys with a running row maximum m and sum l: p = 2^(s - m), rounded to f16 for the product with V
+// and summed unrounded; m follows the maximum lazily, and O is rescaled only when it is raised.  KB is 128 keys.  Heads of more than 256 dims: O takes 256 TMEM columns, so the dims of V are
 // halved between two pieces of work, each with the scores of its own (3/2 of the products, but nothing to be
 // exchanged, where two CTAs that split the dims have to add each other's partial scores); 64 keys, for Q takes 128 KB.
 //
-// Warps of a CTA (12):
-//   0-3   softmax and epilogue: a thread is a row (TMEM lane).
-//   4     loads its half of the K blocks (TMA, one box of rows per page and 64 dims).
-//   5     loads its half of the V blocks.
-//   6     in the pair's first CTA: issues the MMAs of both.  S of stage i + 1 before O of stage i, so that the
+// Warps of a CTA (16):
+//   0-7   softmax and epilogue: warps w and w + 4 have the same 32 rows (TMEM lanes), a thread is a row, and each takes
+//         half of a block's keys and of O's columns.  They exchange their maxima every stage.
+//   8     loads its half of the K blocks (TMA, one box of rows per page and 64 dims).
+//   9     loads its half of the V blocks.
+//   10    in the pair's first CTA: issues the MMAs of both.  S of stage i + 1 before O of stage i, so that the
 //         softmax of a stage runs under the next stage's scores and the last one's product.
-//   7     tells the first CTA that a K block has landed in this one.
-//   8-11  load the queries, and look through V blocks that not every row sees: a value that is not finite
+//   11    tells the first CTA that a K block has landed in this one.
+//   12-15 load the queries, and look through V blocks that not every row sees: a value that is not finite
 //         becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then they tell the first CTA.
 // Barriers that both CTAs arrive on lie in the first CTA.  Every wait is bounded; a thread that gives up sets the
 // abort flags of both CTAs and the error word, all waits then end at once, and both free their TMEM and leave.
@@ -35,13 +35,15 @@ namespace {
 using namespace g4a;
 using namespace g4a_chunk;
 
-constexpr int kThreadsC = 384;
-constexpr int kLoadK = 4, kLoadV = 5, kMma = 6, kTellK = 7, kGuard = 8;
+constexpr int kThreadsC = 512;
+constexpr int kSoft = 8, kLoadK = 8, kLoadV = 9, kMma = 10, kTellK = 11, kGuard = 12;
 constexpr int kCtaRows = 128;
-constexpr float kUpC = 7.0f;          // p = 2^(s - m + 7)
-constexpr float kRaiseC = 8.0f;       // a score this far above m raises it
+// Weights are p = 2^(s - m).  A score above m + 15 (f16 ends at 2^16) raises m: to 3 below the maximum at the row's first
+// scores, to 5 above it later on.  A raise costs the pair a stage's time (O has to be at rest to be rescaled), so later ones
+// leave room for the next 2^20: with m kept 7 below the maximum and raised at 2^8 past it, 512 tokens over 131,000 rows
+// took 604 us instead of 405.
+constexpr float kRaiseC = 15.0f, kFirstC = -3.0f, kLaterC = 5.0f;
 constexpr float kUnseenC = -FLT_MAX;  // m of a row that has seen nothing yet (any finite score raises it)
-constexpr int kInfo = 8;              // stages whose missing rows are remembered (more than are under way)
 constexpr int kBadTags = 8;
 
 template <int HD>
@@ -56,18 +58,19 @@ struct Cc {
   static constexpr int NS = HD <= 128 ? 4 : 2;       // K and V blocks in flight
   static constexpr bool OWN_STAGING = HD <= 256;     // (else the epilogue goes through Q's place)
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_V = OFF_K + NS * K_BYTES, OFF_END = OFF_V + NS * V_BYTES;
-  static constexpr int OFF_OUT = OWN_STAGING ? OFF_END : OFF_Q;  // [4 warps][32 rows][128 B]
-  static constexpr int OFF_OK = OFF_END + (OWN_STAGING ? 4 * 4096 : 0);  // [kInfo][4] which rows of a block are there
-  static constexpr int OFF_BAD = OFF_OK + kInfo * 16;                    // [kBadTags] piece + 1 with values taken out
+  static constexpr int OFF_OUT = OWN_STAGING ? OFF_END : OFF_Q;  // [8 warps][32 rows][64 B]
+  static constexpr int OFF_OK = OFF_END + (OWN_STAGING ? kSoft * 2048 : 0);  // [2 NS][4] which rows of a block are there
+  static constexpr int OFF_RED = OFF_OK + 2 * NS * 16;                       // [2][2 halves][128] maxima, sums
+  static constexpr int OFF_BAD = OFF_RED + 2 * 2 * kCtaRows * 4;             // [kBadTags] piece + 1 with values taken out
   static constexpr int OFF_BAR = OFF_BAD + kBadTags * 4;
-  static constexpr int NBARS = 6 * NS + kInfo + 12;
-  static constexpr size_t SMEM = 1024 + (size_t)OFF_BAR + NBARS * 8 + 16;
+  static constexpr int NBARS = 6 * NS + 13;
+  static constexpr size_t SMEM = (size_t)OFF_BAR + NBARS * 8 + 16;
   static constexpr uint32_t COL_O = 0, COL_S = HDV;  // S[b] at COL_S + KB b, P[b] in its first half
   static constexpr uint32_t TMEM_COLS = 512;
   static_assert(COL_S + 2 * KB <= TMEM_COLS && SMEM <= 232448, "tile fits");
-  // Registers: 384 threads start with 168; the softmax warps hold a row of scores.
-  static constexpr int REGS_SOFT = 232, REGS_REST = 104;
-  static_assert(128 * REGS_SOFT + 256 * REGS_REST <= kThreadsC * 168, "register file");
+  // Registers: 512 threads start with 128; the softmax warps hold half a row of scores.
+  static constexpr int REGS_SOFT = 160, REGS_REST = 88;
+  static_assert(256 * REGS_SOFT + 256 * REGS_REST <= kThreadsC * 128, "register file");
 };
 
 struct TcParams {
@@ -105,12 +108,12 @@ struct Work {
   }
 };
 
-// Adds to what this thread has stored for row `gr` the infinities and NaN of the V values that were taken out of
+// Adds to what this thread has stored for a row (half of its columns) the infinities and NaN of the V values that were taken out of
 // the piece's blocks, where the row sees their keys.
 template <int HD>
-__device__ __noinline__ void add_taken_out(const ChunkParams& p, Work<HD> w, int pos, size_t out_row, float* part, int row) {
+__device__ __noinline__ void add_taken_out(const ChunkParams& p, Work<HD> w, int pos, size_t out_row, float* part, int row, int half) {
   using C = Cc<HD>;
-  const int d0 = w.half * C::HDV, d1 = min(p.hd, d0 + C::HDV);
+  const int d0 = w.half * C::HDV, from = d0 + half * (C::HDV / 2), d1 = min(p.hd, from + C::HDV / 2);
   for (int j = w.d.j0; j < w.d.j1; j++) {
     const int k0 = w.key0(j);
     if (w.clean(p, k0)) continue;
@@ -118,7 +121,7 @@ __device__ __noinline__ void add_taken_out(const ChunkParams& p, Work<HD> w, int
       if (!sees(p, pos, key)) continue;
       const long long off = row_offset(p, w.d.b, w.kvh, key);
       if (off < 0) continue;
-      for (int d = d0; d < d1; d++) {
+      for (int d = from; d < d1; d++) {
         const float v = __half2float(p.v[off + d]);
         if (fabsf(v) < INFINITY) continue;
         if (part != nullptr) {
@@ -138,29 +141,27 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     chunk_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TcParams a) {
   using C = Cc<HD>;
   const ChunkParams& p = a.c;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* smem =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) unsigned char smem[];  // (at 512 dims there is no room to align it by hand)
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicExch(p.err, G4A_DEVERR_TMEM);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* k_landed = bars;                 // [NS] this CTA's half of a K block
   uint64_t* v_landed = k_landed + C::NS;     // [NS]
   uint64_t* k_ready = v_landed + C::NS;      // [NS] first CTA: both halves
-  uint64_t* v_ready = k_ready + C::NS;       // [NS] first CTA: both, looked through (4 warps of each CTA)
-  uint64_t* k_free = v_ready + C::NS;        // [NS] scores done (commit)
-  uint64_t* v_free = k_free + C::NS;         // [NS] product done (commit)
-  uint64_t* info = v_free + C::NS;           // [kInfo] which rows of the block are there
-  uint64_t* q_ready = info + kInfo;          // first CTA: queries of both (4 warps of each)
+  uint64_t* p_ready = k_ready + C::NS;       // [NS] first CTA: weights (8 warps of each) and V, looked through (4 of each)
+  uint64_t* s_done = p_ready + C::NS;        // [NS] scores (commit), and which rows of the block are there (warp 8)
+  uint64_t* o_done = s_done + C::NS;         // [NS] a stage's product done (commit)
+  uint64_t* q_ready = o_done + C::NS;        // first CTA: queries of both (4 warps of each)
   uint64_t* q_free = q_ready + 1;            // the piece's last scores done (commit)
-  uint64_t* s_done = q_free + 1;             // [2] scores (commit)
-  uint64_t* p_ready = s_done + 2;            // [2] first CTA: weights of both (4 warps of each)
-  uint64_t* o_done = p_ready + 2;            // [2] a stage's product done (commit)
-  uint64_t* o_free = o_done + 2;             // first CTA: epilogue has read O (4 warps of each)
+  uint64_t* o_free = q_free + 1;             // first CTA: epilogue has read O (8 warps of each)
   uint64_t* looked = o_free + 1;             // the piece's V blocks have been looked through (4 warps of each)
-  uint64_t* staged = looked + 1;             // the epilogue is through with the staging place (4 warps)
-  uint64_t* all_done = staged + 1;
+  uint64_t* staged = looked + 1;             // the epilogue is through with the staging place (8 warps)
+  uint64_t* swapped = staged + 1;            // [4] two warps have written what they exchange
+  uint64_t* all_done = swapped + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert(C::NBARS >= 6 * C::NS + kInfo + 12, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cta_rank();
@@ -171,21 +172,16 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       mbar_init(&k_landed[s], 1);
       mbar_init(&v_landed[s], 1);
       mbar_init(&k_ready[s], 2);
-      mbar_init(&v_ready[s], 8);
-      mbar_init(&k_free[s], 1);
-      mbar_init(&v_free[s], 1);
-    }
-    for (int s = 0; s < kInfo; s++) mbar_init(&info[s], 1);
-    mbar_init(q_ready, 8);
-    mbar_init(q_free, 1);
-    for (int s = 0; s < 2; s++) {
-      mbar_init(&s_done[s], 1);
-      mbar_init(&p_ready[s], 8);
+      mbar_init(&p_ready[s], 2 * kSoft + 8);
+      mbar_init(&s_done[s], 2);
       mbar_init(&o_done[s], 1);
     }
-    mbar_init(o_free, 8);
+    mbar_init(q_ready, 8);
+    mbar_init(q_free, 1);
+    mbar_init(o_free, 2 * kSoft);
     mbar_init(looked, 8);
-    mbar_init(staged, 4);
+    mbar_init(staged, kSoft);
+    for (int s = 0; s < 4; s++) mbar_init(&swapped[s], 2);
     mbar_init(all_done, 1);
     *abort_flag = 0;
     for (int i = 0; i < kBadTags; i++) reinterpret_cast<int*>(smem + C::OFF_BAD)[i] = 0;
@@ -213,16 +209,29 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   const int begin = step == 1 ? a.plan->first[pair] : pair;
   const int end = step == 1 ? a.plan->first[pair + 1] : a.plan->pieces;
 
-  if (warp < 4) {
+  if (warp < kSoft) {
     // ------------------------------------------------------------------ softmax, epilogue
     regs_up<C::REGS_SOFT>();
-    const int row = rank * kCtaRows + warp * 32 + lane;  // of the tile
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const uint32_t p_bar0 = map_to(smem_u32(&p_ready[0]), 0), p_bar1 = map_to(smem_u32(&p_ready[1]), 0);
-    const uint32_t o_bar = map_to(smem_u32(o_free), 0);
+    const int quarter = warp & 3, half = warp >> 2;  // rows; keys [HB half, HB half + HB) of a block
+    constexpr int HB = C::KB / 2, HO = C::HDV / 2;   // and columns [HO half, HO half + HO) of O
+    const int cta_row = quarter * 32 + lane, row = rank * kCtaRows + cta_row;  // of the CTA, of the tile
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t p_bar = map_to(smem_u32(p_ready), 0), o_bar = map_to(smem_u32(o_free), 0);
     const volatile int* tags = reinterpret_cast<const volatile int*>(smem + C::OFF_BAD);
-    uint32_t g = 0, done = 0;  // stages and pieces so far
+    float* red = reinterpret_cast<float*>(smem + C::OFF_RED);
+    uint32_t g = 0, done = 0, swaps = 0;  // stages, pieces and exchanges so far
     bool ok = true;
+    // This thread's value for the other half's thread of the row, and that one's for this.  The places alternate: a
+    // warp writes one again only after the exchange between, for which the other had to come after reading it.
+    auto swap = [&](float mine) {
+      float* at = red + (swaps & 1u) * (2 * kCtaRows) + cta_row;
+      at[half * kCtaRows] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&swapped[quarter]);
+      ok = warp_wait_own(&swapped[quarter], swaps & 1u, abort_flag, p.err);
+      swaps++;
+      return *reinterpret_cast<volatile float*>(at + (half ^ 1) * kCtaRows);
+    };
     for (int i = begin; ok && i < end; i += step) {
       const Work<HD> w(p, a.pieces[i]);
       if (w.stages() <= 0) continue;
@@ -232,38 +241,35 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       const int pos = w.base + token, lo = first_in_window(p, pos);
       float m = kUnseenC, l = 0.f;
       for (int j = w.d.j0; j < w.d.j1; j++, g++) {
-        const uint32_t b = g & 1u;
-        const uint32_t col = lanes + C::COL_S + b * C::KB;
-        ok = warp_wait(&info[g % kInfo], (g / kInfo) & 1u, abort_flag, p.err);
-        if (!ok) break;
-        const uint4 there = *reinterpret_cast<const uint4*>(smem + C::OFF_OK + (g % kInfo) * 16);
-        ok = warp_wait(&s_done[b], (g >> 1) & 1u, abort_flag, p.err);
+        const uint32_t col = lanes + C::COL_S + (g & 1u) * C::KB;
+        ok = warp_wait_own(&s_done[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err);
         if (!ok) break;
         tc_fence_after();
-        uint32_t s[C::KB / 32][32];
+        uint32_t s[HB / 32][32];
 #pragma unroll
-        for (int c = 0; c < C::KB / 32; c++) tmem_get(col + 32u * c, s[c]);
-        const int k0 = w.key0(j);
-        // from the block's first key: z the last one seen, f the first one of the window, and sinks before n
+        for (int c = 0; c < HB / 32; c++) tmem_get(col + half * HB + 32u * c, s[c]);
+        const uint32_t* there = reinterpret_cast<const uint32_t*>(smem + C::OFF_OK + (g % (2 * C::NS)) * 16) + half * (HB / 32);
+        const uint32_t there0 = there[0], there1 = HB > 32 ? there[1] : 0xffffffffu;
+        const int k0 = w.key0(j) + half * HB;
+        // from the half block's first key: z the last one seen, f the first one of the window, and sinks before n
         const int z = pos - k0, f = lo - k0;
-        const int n = (int)min((long long)p.sinks - k0, (long long)C::KB);
-        const bool full = (there.x & there.y) == 0xffffffffu && (C::KB == 64 || (there.z & there.w) == 0xffffffffu);
-        const bool plain =
-            __all_sync(0xffffffffu, z >= C::KB - 1 && (f <= 0 || n >= C::KB)) && full && p.scale_log2 > 0.f;
+        const int n = (int)max(min((long long)p.sinks - k0, (long long)HB), 0ll);
+        const bool plain = __all_sync(0xffffffffu, z >= HB - 1 && (f <= 0 || n >= HB)) && (there0 & there1) == 0xffffffffu &&
+                           p.scale_log2 > 0.f;
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < C::KB / 32; c++) tmem_landed(s[c]);
+        for (int c = 0; c < HB / 32; c++) tmem_landed(s[c]);
         float by = p.scale_log2;
         if (!plain) {
           by = 1.f;
 #pragma unroll
-          for (int c = 0; c < C::KB / 32; c++) {
+          for (int c = 0; c < HB / 32; c++) {
             // bits of keys [32 c, 32 c + 32): up to z, and from f on or before n
             const int zc = z - 32 * c, fc = f - 32 * c, nc = n - 32 * c;
             const uint32_t upto = zc >= 31 ? 0xffffffffu : zc < 0 ? 0u : (2u << zc) - 1u;
             const uint32_t from = fc <= 0 ? 0xffffffffu : fc > 31 ? 0u : ~((1u << fc) - 1u);
             const uint32_t sink = nc >= 32 ? 0xffffffffu : nc <= 0 ? 0u : (1u << nc) - 1u;
-            const uint32_t bits = upto & (from | sink) & (c == 0 ? there.x : c == 1 ? there.y : c == 2 ? there.z : there.w);
+            const uint32_t bits = upto & (from | sink) & (c == 0 ? there0 : there1);
 #pragma unroll
             for (int e = 0; e < 32; e++)
               s[c][e] = (bits >> e) & 1u ? __float_as_uint(__uint_as_float(s[c][e]) * p.scale_log2) : 0xff800000u;
@@ -271,23 +277,25 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < C::KB / 32; c++)
+        for (int c = 0; c < HB / 32; c++)
 #pragma unroll
           for (int e = 0; e < 32; e++) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by;
+        const float mine = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * by;
+        const float top = fmaxf(mine, swap(mine));
+        if (!ok) break;
         const bool raise = top > m + kRaiseC;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float m_new = raise ? top : m;
+        if (__any_sync(0xffffffffu, raise)) {  // (both halves agree)
+          const float m_new = raise ? top + (m == kUnseenC ? kFirstC : kLaterC) : m;
           const float fall = raise ? (m == kUnseenC ? 0.f : fast_exp2(m - m_new)) : 1.f;
           l *= fall;
           m = m_new;
           if (j > w.d.j0) {
             // O holds the stages up to j - 1, whose product is the last one issued before this stage's
-            ok = warp_wait(&o_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, p.err);
+            ok = warp_wait_own(&o_done[(g - 1) % C::NS], ((g - 1) / C::NS) & 1u, abort_flag, p.err);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < C::HDV; c += 32) {
+            for (int c = half * HO; c < half * HO + HO; c += 32) {
               uint32_t o[32];
               tmem_ld32(lanes + C::COL_O + c, o);
 #pragma unroll
@@ -296,30 +304,32 @@ __global__ void __launch_bounds__(kThreadsC, 1)
             }
           }
         }
-        const float up = kUpC - m;
+        const float up = -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t pw[HB / 2];
 #pragma unroll
-        for (int c = 0; c < C::KB / 64; c++) {
-          uint32_t pw[32];
-#pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const float x = fast_exp2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][(2 * e) & 31]), by, up));
-            const float y = fast_exp2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][(2 * e + 1) & 31]), by, up));
-            sum[(2 * e) & 3] += x;
-            sum[(2 * e + 1) & 3] += y;
-            pw[e] = half2_bits(x, y);
-          }
-          tmem_st32(col + 32u * c, pw);
+        for (int e = 0; e < HB / 2; e++) {
+          const float x = fast_exp2(fmaf(__uint_as_float(s[e >> 4][(2 * e) & 31]), by, up));
+          const float y = fast_exp2(fmaf(__uint_as_float(s[e >> 4][(2 * e + 1) & 31]), by, up));
+          sum[(2 * e) & 3] += x;
+          sum[(2 * e + 1) & 3] += y;
+          pw[e] = half2_bits(x, y);
         }
+        // (where the other half's scores were: it has read them, or it would not have come to the exchange)
+        if constexpr (HB == 64) tmem_st32(col + half * 32u, pw);
+        else tmem_st16(col + half * 16u, pw);
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_at(b ? p_bar1 : p_bar0);
+        if (lane == 0) arrive_at(p_bar + (g % C::NS) * 8u);
       }
       if (!ok) break;
       // ---- epilogue
-      ok = warp_wait(&o_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, abort_flag, p.err);
+      const float other = swap(l);
+      if (!ok) break;
+      l = half == 0 ? l + other : other + l;
+      ok = warp_wait_own(&o_done[(g - 1) % C::NS], ((g - 1) / C::NS) & 1u, abort_flag, p.err);
       if (!ok) break;
       ok = __all_sync(0xffffffffu, wait_pair(looked, done & 1u, abort_flag, p.err));
       if (!ok) break;
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       float* part = w.d.slot < 0 ? nullptr : a.part + (size_t)w.d.slot * kTileRows * (C::HDV + 2);
       if (part != nullptr) {
 #pragma unroll 1
-        for (int c = 0; c < C::HDV; c += 32) {
+        for (int c = half * HO; c < half * HO + HO; c += 32) {
           uint32_t o[32];
           tmem_ld32(lanes + C::COL_O + c, o);
           if (live)
@@ -339,43 +349,40 @@ __global__ void __launch_bounds__(kThreadsC, 1)
               *reinterpret_cast<uint4*>(part + ((size_t)(c / 4 + e) * kTileRows + row) * 4) =
                   make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
-        if (live) {
+        if (live && half == 0) {
           part[(size_t)C::HDV * kTileRows + row] = m;
           part[(size_t)(C::HDV + 1) * kTileRows + row] = l;
         }
       } else {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        unsigned char* stage = smem + C::OFF_OUT + warp * 4096;
+        unsigned char* stage = smem + C::OFF_OUT + warp * 2048;
 #pragma unroll 1
-        for (int c = 0; c < C::HDV; c += 64) {  // 64 columns of the warp's 32 rows through shared memory
+        for (int c = half * HO; c < half * HO + HO; c += 32) {  // 32 columns of the warp's 32 rows through shared memory
+          uint32_t o[32];
+          tmem_ld32(lanes + C::COL_O + c, o);
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            uint32_t o[32];
-            tmem_ld32(lanes + C::COL_O + c + 32 * h, o);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              uint4 x;
-              x.x = half2_bits(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
-              x.y = half2_bits(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
-              x.z = half2_bits(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
-              x.w = half2_bits(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * h + e) ^ (lane & 7)) << 4)) = x;
-            }
+          for (int e = 0; e < 4; e++) {
+            uint4 x;
+            x.x = half2_bits(__uint_as_float(o[8 * e]) * inv, __uint_as_float(o[8 * e + 1]) * inv);
+            x.y = half2_bits(__uint_as_float(o[8 * e + 2]) * inv, __uint_as_float(o[8 * e + 3]) * inv);
+            x.z = half2_bits(__uint_as_float(o[8 * e + 4]) * inv, __uint_as_float(o[8 * e + 5]) * inv);
+            x.w = half2_bits(__uint_as_float(o[8 * e + 6]) * inv, __uint_as_float(o[8 * e + 7]) * inv);
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4)) = x;
           }
           __syncwarp();
 #pragma unroll
-          for (int r0 = 0; r0 < 32; r0 += 4) {
-            const int r = r0 + (lane >> 3), e = lane & 7, d = w.half * C::HDV + c + e * 8;
-            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((e ^ (r & 7)) << 4));
+          for (int r0 = 0; r0 < 32; r0 += 8) {
+            const int r = r0 + (lane >> 2), e = lane & 3, d = w.half * C::HDV + c + e * 8;
+            const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 64 + ((e ^ ((r >> 1) & 3)) << 4));
             const size_t at = __shfl_sync(0xffffffffu, out_row, r);
             if (((lives >> r) & 1u) && d < p.hd) *reinterpret_cast<uint4*>(p.out + at * p.hd + d) = x;
           }
           __syncwarp();
         }
-        if (p.lse != nullptr && live && w.half == 0)
-          p.lse[out_row] = l == 0.f ? -INFINITY : (m - kUpC + log2f(l)) * kLn2C;
+        if (p.lse != nullptr && live && w.half == 0 && half == 0)
+          p.lse[out_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2C;
       }
-      if (bad && live) add_taken_out<HD>(p, w, pos, out_row, part, row);
+      if (bad && live) add_taken_out<HD>(p, w, pos, out_row, part, row, half);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -390,7 +397,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       // ---------------------------------------------------------------- loads
       const bool kside = warp == kLoadK;
       uint64_t* landed = kside ? k_landed : v_landed;
-      uint64_t* free_bar = kside ? k_free : v_free;
+      uint64_t* free_bar = kside ? s_done : o_done;  // (of stage g - NS)
       const CUtensorMap* map = kside ? &tmk : &tmv;
       const int box = kside ? a.box_k : a.box_v, rows = kside ? C::KB / 2 : C::KB, chunks = kside ? C::NCQ : C::NCV;
       const int chunk_bytes = kside ? C::K_CHUNK : C::V_CHUNK, bytes = kside ? C::K_BYTES : C::V_BYTES;
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         for (int j = w.d.j0; j < w.d.j1; j++, g++) {
           const uint32_t s = g % C::NS;
           if (g >= (uint32_t)C::NS) {
-            ok = warp_wait(&free_bar[s], (g / C::NS - 1) & 1u, abort_flag, p.err);
+            ok = warp_wait_own(&free_bar[s], (g / C::NS - 1) & 1u, abort_flag, p.err);
             if (!ok) break;
           }
           if (lane == 0) mbar_arrive_expect_tx(&landed[s], (uint32_t)bytes);
@@ -432,7 +439,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
               const int id = table[key / p.page_size];
               gone |= id < 0 || id >= p.num_pages;
             }
-            uint32_t* to = reinterpret_cast<uint32_t*>(smem + C::OFF_OK + (g % kInfo) * 16);
+            // (places for twice the ring: this stage's may be written while the softmax is still at stage g - NS)
+            uint32_t* to = reinterpret_cast<uint32_t*>(smem + C::OFF_OK + (g % (2 * C::NS)) * 16);
             if (!__any_sync(0xffffffffu, gone)) {
               if (lane < 4) to[lane] = 0xffffffffu;
             } else {
@@ -450,7 +458,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
               }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&info[g % kInfo]);
+            if (lane == 0) mbar_arrive(&s_done[s]);
           }
         }
       }
@@ -465,7 +473,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         for (int i = begin; ok && i < end; i += step) {
           const int n = a.pieces[i].j1 - a.pieces[i].j0;
           for (int j = 0; j < n; j++, g++) {
-            ok = wait_or_abort(&k_landed[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+            ok = wait_own(&k_landed[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err);
             if (!ok) break;
             arrive_at(map_to(smem_u32(&k_ready[g % C::NS]), 0));
           }
@@ -473,7 +481,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       }
     } else if (warp == kMma) {
       // ---------------------------------------------------------------- MMAs
-      if (rank == 0 && lane == 0) {
+      if (rank == 0) {
+        const uint32_t on = elect_one();
         constexpr uint32_t idesc_s = pair_idesc(C::KB, false), idesc_o = pair_idesc(C::HDV, true);
         const uint64_t dq = sw128_desc(sbase + C::OFF_Q, 16, 1024);
         const uint64_t dk0 = sw128_desc(sbase + C::OFF_K, 16, 1024);
@@ -482,50 +491,50 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         uint32_t g = 0, done = 0;
         bool ok = true;
         auto scores = [&](uint32_t k) {
-          if (!wait_pair(&k_ready[k % C::NS], (k / C::NS) & 1u, abort_flag, p.err)) return false;
+          if (!warp_wait_own(&k_ready[k % C::NS], (k / C::NS) & 1u, abort_flag, p.err)) return false;
           tc_fence_after();
           const uint64_t dk = dk0 + (uint64_t)(((k % C::NS) * C::K_BYTES) >> 4);
           const uint32_t d = tmem + C::COL_S + (k & 1u) * C::KB;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; kk++) {
             const uint64_t off = (uint64_t)(((kk & 3) * 32) >> 4);
-            mma2_ss(d, dq + (uint64_t)(((kk >> 2) * C::Q_CHUNK) >> 4) + off, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
+            mma2_ss(on, d, dq + (uint64_t)(((kk >> 2) * C::Q_CHUNK) >> 4) + off, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
                     idesc_s, kk > 0 ? 1u : 0u);
           }
-          commit2(&s_done[k & 1u]);
-          commit2(&k_free[k % C::NS]);
+          commit2(on, &s_done[k % C::NS]);
           return true;
         };
         for (int i = begin; ok && i < end; i += step) {
-          const int n = a.pieces[i].j1 - a.pieces[i].j0;
+          const Work<HD> w(p, a.pieces[i]);
+          const int n = w.stages();
           if (n <= 0) continue;
-          ok = wait_pair(q_ready, done & 1u, abort_flag, p.err) && scores(g);
-          if (ok && n == 1) commit2(q_free);
+          ok = warp_wait_pair(q_ready, done & 1u, abort_flag, p.err) && scores(g);
+          if (ok && n == 1) commit2(on, q_free);
           for (int j = 0; ok && j < n; j++, g++) {
             if (j + 1 < n) {
               ok = scores(g + 1);
               if (!ok) break;
-              if (j + 2 == n) commit2(q_free);
+              if (j + 2 == n) commit2(on, q_free);
             }
             // (the epilogue of the piece before has read O)
-            if (j == 0 && done > 0) ok = wait_pair(o_free, (done - 1) & 1u, abort_flag, p.err);
-            ok = ok && wait_pair(&v_ready[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err) &&
-                 wait_pair(&p_ready[g & 1u], (g >> 1) & 1u, abort_flag, p.err);
+            if (j == 0 && done > 0) ok = warp_wait_own(o_free, (done - 1) & 1u, abort_flag, p.err);
+            // (where V was looked through, there are stores of the other CTA to be seen)
+            ok = ok && (w.clean(p, w.key0(w.d.j0 + j)) ? warp_wait_own(&p_ready[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err)
+                                                       : warp_wait_pair(&p_ready[g % C::NS], (g / C::NS) & 1u, abort_flag, p.err));
             if (!ok) break;
             tc_fence_after();
             const uint64_t dv = dv0 + (uint64_t)(((g % C::NS) * C::V_BYTES) >> 4);
             const uint32_t pa = tmem + C::COL_S + (g & 1u) * C::KB;
 #pragma unroll
             for (int kk = 0; kk < C::KB / 16; kk++)
-              mma2_ts(tmem + C::COL_O, pa + (uint32_t)(8 * kk), dv + (uint64_t)((kk * 2048) >> 4), idesc_o,
+              mma2_ts(on, tmem + C::COL_O, pa + (uint32_t)(8 * kk), dv + (uint64_t)((kk * 2048) >> 4), idesc_o,
                       j > 0 || kk > 0 ? 1u : 0u);
-            commit2(&o_done[g & 1u]);
-            commit2(&v_free[g % C::NS]);
+            commit2(on, &o_done[g % C::NS]);
           }
           done++;
         }
         // no MMA may still be running when TMEM is freed, also after an abort
-        commit2(all_done);
+        commit2(on, all_done);
         (void)mbar_wait_bounded(all_done, 0, p.err, G4A_DEVERR_WAIT_MMA);
       }
     } else {
@@ -539,8 +548,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         const Work<HD> w(p, a.pieces[i]);
         if (w.stages() <= 0) continue;
         if (done > 0) {
-          ok = warp_wait(q_free, (done - 1) & 1u, abort_flag, p.err);
-          if (ok && !C::OWN_STAGING) ok = warp_wait(staged, (done - 1) & 1u, abort_flag, p.err);
+          ok = warp_wait_own(q_free, (done - 1) & 1u, abort_flag, p.err);
+          if (ok && !C::OWN_STAGING) ok = warp_wait_own(staged, (done - 1) & 1u, abort_flag, p.err);
           if (!ok) break;
         }
         const long long rows = (long long)w.d.T * p.group;
@@ -561,15 +570,16 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         cp_wait_all();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) arrive_at(q_bar);
+        if (lane == 0) publish_at(q_bar);
         const int lo = first_in_window(p, w.base + w.first), hi = w.base + w.last + 1;
         bool found = false;
         for (int j = w.d.j0; j < w.d.j1; j++, g++) {
           const uint32_t s = g % C::NS;
-          ok = warp_wait(&v_landed[s], (g / C::NS) & 1u, abort_flag, p.err);
+          ok = warp_wait_own(&v_landed[s], (g / C::NS) & 1u, abort_flag, p.err);
           if (!ok) break;
           const int k0 = w.key0(j);
-          if (!w.clean(p, k0)) {
+          const bool clean = w.clean(p, k0);
+          if (!clean) {
             unsigned char* v = smem + C::OFF_V + s * C::V_BYTES;
 #pragma unroll 4
             for (int e = gw * 32 + lane; e < C::V_BYTES / 16; e += 128) {
@@ -593,7 +603,11 @@ __global__ void __launch_bounds__(kThreadsC, 1)
             fence_proxy_async_smem();
           }
           __syncwarp();
-          if (lane == 0) arrive_at(map_to(smem_u32(&v_ready[s]), 0));
+          if (lane == 0) {
+            const uint32_t to = map_to(smem_u32(&p_ready[s]), 0);
+            if (clean) arrive_at(to);
+            else publish_at(to);
+          }
         }
         if (!ok) break;
         // (a CTA has half of the dims and half of the rows, so both have to know)
@@ -602,7 +616,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
           if (found)
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(tags + (done % kBadTags) * 4, c)), "r"(done + 1) : "memory");
           __syncwarp();
-          if (lane == 0) arrive_at(map_to(smem_u32(looked), c));
+          if (lane == 0) publish_at(map_to(smem_u32(looked), c));
         }
         done++;
       }
@@ -700,7 +714,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams
       const int d = half * C::HDV + block * 16 + c4 * 4;
       if (d < p.hd)
         *reinterpret_cast<uint2*>(p.out + to * p.hd + d) = make_uint2(half2_bits(o.x * inv, o.y * inv), half2_bits(o.z * inv, o.w * inv));
-      if (p.lse != nullptr && d == 0) p.lse[to] = lt == 0.f ? -INFINITY : (mx - kUpC + log2f(lt)) * kLn2C;
+      if (p.lse != nullptr && d == 0) p.lse[to] = lt == 0.f ? -INFINITY : (mx + log2f(lt)) * kLn2C;
     }
     __syncthreads();
   }

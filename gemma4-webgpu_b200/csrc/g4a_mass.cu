@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       for (int j = d.j0; j < d.j1; j++, g++) {
         if ((g & 1u) != set) continue;
         const uint32_t buf = g % kScoreBufs, inf = g % kInfoM;
-        ok = warp_wait(&lse_full[inf], (g / kInfoM) & 1u, abort_flag, p.err) &&
-             warp_wait(&s_done[buf], (g / kScoreBufs) & 1u, abort_flag, p.err);
+        ok = warp_wait_own(&lse_full[inf], (g / kInfoM) & 1u, abort_flag, p.err) &&
+             warp_wait_own(&s_done[buf], (g / kScoreBufs) & 1u, abort_flag, p.err);
         if (!ok) break;
         tc_fence_after();
         const float* nl = reinterpret_cast<const float*>(smem + C::OFF_LSE) + inf * C::RB;
@@ -291,13 +291,13 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       const float sum = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
       float* meet = sums + (done & 1u) * kCtaKeys + (warp & 3) * 32 + lane;
       if (set == 1) {
-        if (done >= 2) ok = warp_wait(&sum_free[done & 1u], ((done >> 1) - 1) & 1u, abort_flag, p.err);
+        if (done >= 2) ok = warp_wait_own(&sum_free[done & 1u], ((done >> 1) - 1) & 1u, abort_flag, p.err);
         if (!ok) break;
         *meet = sum;
         __syncwarp();
         if (lane == 0) mbar_arrive(&sum_full[done & 1u]);
       } else {
-        ok = warp_wait(&sum_full[done & 1u], (done >> 1) & 1u, abort_flag, p.err);
+        ok = warp_wait_own(&sum_full[done & 1u], (done >> 1) & 1u, abort_flag, p.err);
         if (!ok) break;
         const float whole = sum + *meet;
         if (d.slot >= 0) {
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       const Piece d = a.pieces[i];
       const int* table = p.page_table + (size_t)d.b * p.max_pages;
       const uint32_t s = done % C::NK;
-      if (done >= (uint32_t)C::NK) ok = warp_wait(&k_free[s], (done / C::NK - 1) & 1u, abort_flag, p.err);
+      if (done >= (uint32_t)C::NK) ok = warp_wait_own(&k_free[s], (done / C::NK - 1) & 1u, abort_flag, p.err);
       if (!ok) break;
       if (lane == 0) mbar_arrive_expect_tx(&k_landed[s], (uint32_t)C::K_BYTES);
       __syncwarp();
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       const Piece d = a.pieces[i];
       for (int j = d.j0; j < d.j1; j++, g++) {
         const uint32_t s = g % C::NQ;
-        if (g >= (uint32_t)C::NQ) ok = warp_wait(&q_free[s], (g / C::NQ - 1) & 1u, abort_flag, p.err);
+        if (g >= (uint32_t)C::NQ) ok = warp_wait_own(&q_free[s], (g / C::NQ - 1) & 1u, abort_flag, p.err);
         if (!ok) break;
         const int tb = j / a.head_chunks, hc = j - tb * a.head_chunks;
         const long long token = (long long)d.row0 + ((long long)d.skip + tb) * 2 * a.tokens + rank * a.tokens;
@@ -356,33 +356,34 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       (void)mbar_wait_bounded(&q_landed[k % C::NQ], (k / C::NQ) & 1u, p.err, G4A_DEVERR_WAIT_FULL);
   } else if (warp == kWarpMma) {
     // ------------------------------------------------------------------ MMAs of both CTAs
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
+      const uint32_t on = elect_one();
       constexpr uint32_t idesc = pair_idesc(C::RB, false);
       const uint64_t dk0 = sw128_desc(sbase, 16, 1024), dq0 = sw128_desc(sbase + C::OFF_Q, 16, 1024);
       for (int i = begin; ok && i < end; i++, done++) {
         const int n = a.pieces[i].j1 - a.pieces[i].j0;
-        ok = wait_pair(&k_ready[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err);
+        ok = warp_wait_own(&k_ready[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err);
         const uint64_t dk = dk0 + (uint64_t)(((done % C::NK) * C::K_BYTES) >> 4);
         for (int j = 0; ok && j < n; j++, g++) {
           const uint32_t s = g % C::NQ, buf = g % kScoreBufs;
-          if (g >= (uint32_t)kScoreBufs) ok = wait_pair(&s_free[buf], (g / kScoreBufs - 1) & 1u, abort_flag, p.err);
-          ok = ok && wait_pair(&q_ready[s], (g / C::NQ) & 1u, abort_flag, p.err);
+          if (g >= (uint32_t)kScoreBufs) ok = warp_wait_own(&s_free[buf], (g / kScoreBufs - 1) & 1u, abort_flag, p.err);
+          ok = ok && warp_wait_own(&q_ready[s], (g / C::NQ) & 1u, abort_flag, p.err);
           if (!ok) break;
           tc_fence_after();
           const uint64_t dq = dq0 + (uint64_t)((s * C::Q_BYTES) >> 4);
 #pragma unroll
           for (int kk = 0; kk < HD / 16; kk++) {
             const uint64_t off = (uint64_t)(((kk & 3) * 32) >> 4);
-            mma2_ss(tmem + buf * C::RB, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
+            mma2_ss(on, tmem + buf * C::RB, dk + (uint64_t)(((kk >> 2) * C::K_CHUNK) >> 4) + off,
                     dq + (uint64_t)(((kk >> 2) * C::Q_CHUNK) >> 4) + off, idesc, kk > 0 ? 1u : 0u);
           }
-          commit2(&s_done[buf]);
-          commit2(&q_free[s]);
+          commit2(on, &s_done[buf]);
+          commit2(on, &q_free[s]);
         }
-        if (ok) commit2(&k_free[done % C::NK]);
+        if (ok) commit2(on, &k_free[done % C::NK]);
       }
       // no MMA may still be running when TMEM is freed, also after an abort
-      commit2(all_done);
+      commit2(on, all_done);
       (void)mbar_wait_bounded(all_done, 0, p.err, G4A_DEVERR_WAIT_MMA);
     }
   } else if (warp == kWarpLse) {
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
           else if (tok < d.T && head < p.group)
             z[c] = p.lse[(size_t)(d.row0 + tok) * p.nqh + (size_t)d.head * p.group + head];
         }
-        if (g >= (uint32_t)kInfoM) ok = warp_wait(&lse_free[inf], (g / kInfoM - 1) & 1u, abort_flag, p.err);
+        if (g >= (uint32_t)kInfoM) ok = warp_wait_own(&lse_free[inf], (g / kInfoM - 1) & 1u, abort_flag, p.err);
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < C::RB / 32; c++) {
@@ -420,12 +421,12 @@ __global__ void __launch_bounds__(kThreadsM, 1)
     // ------------------------------------------------------------------ what has landed in this CTA
     if (lane == 0) {
       for (int i = begin; ok && i < end; i++, done++) {
-        ok = wait_or_abort(&k_landed[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+        ok = wait_own(&k_landed[done % C::NK], (done / C::NK) & 1u, abort_flag, p.err);
         if (!ok) break;
         arrive_at(map_to(smem_u32(&k_ready[done % C::NK]), 0));
         const int n = a.pieces[i].j1 - a.pieces[i].j0;
         for (int j = 0; j < n; j++, g++) {
-          ok = wait_or_abort(&q_landed[g % C::NQ], (g / C::NQ) & 1u, abort_flag, p.err, G4A_DEVERR_WAIT_FULL);
+          ok = wait_own(&q_landed[g % C::NQ], (g / C::NQ) & 1u, abort_flag, p.err);
           if (!ok) break;
           arrive_at(map_to(smem_u32(&q_ready[g % C::NQ]), 0));
         }

@@ -134,16 +134,6 @@ __device__ __forceinline__ void warp_pass(uint64_t* bar, uint32_t parity, volati
   if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) (void)warp_wait(bar, parity, abort_flag, err);
 }
 
-// 1 in one lane of a converged warp (always the same one), 0 in the others.
-__device__ __forceinline__ uint32_t elect_one() {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(r));
-  return r;
-}
 // D (+)= A B^T and the commit, by the lane for which `on` is not 0.  The instructions are predicated, not
 // branched to, so that the warp's control flow stays uniform and the descriptors in uniform registers.
 __device__ __forceinline__ void umma_if(uint32_t on, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
