@@ -25,15 +25,16 @@ struct Piece {
   int pad;
 };
 
-// A tile that several pieces share.
+// A tile that several pieces share: the first's result is in `slot`, the others' in slot1, slot1 + step, ...
 struct Cut {
-  int b, head, tile, slot, parts, row0, T, pad;
+  int b, head, tile, row0, T, parts, slot, slot1, step;
+  __device__ __forceinline__ int slot_of(int part) const { return part == 0 ? slot : slot1 + (part - 1) * step; }
 };
 
 struct Plan {
-  int step;            // 1: pair w has the pieces first[w] .. first[w + 1] - 1; else w, w + step, ...
+  int step;            // 1: pair w has the pieces first[w] .. end[w] - 1; else w, w + step, ...
   int pieces, cuts, pad;
-  int first[kMaxPairs + 1];
+  int first[kMaxPairs], end[kMaxPairs];
 };
 
 // What the planning kernel reads and writes besides ChunkParams.
@@ -48,7 +49,7 @@ struct PlanParams {
   Cut* cuts;
   int4* seqs;          // [batch + 1]: tile entries before, items before, most stages of a tile, (chunks) pieces before
   long long* entries;  // [tile entries]: stages of all earlier entries
-  int2* parts;         // masses: [items] place of a tile's first partial result, number of its pieces
+  int2* parts;         // masses: [items] the pair of a tile's first piece, number of its pieces
 };
 
 __device__ __forceinline__ int tiles_of(const ChunkParams& p, const Seq& s) {
@@ -100,4 +101,4 @@ __device__ __forceinline__ Tokens tokens_of(const ChunkParams& p, const Seq& s, 
 }
 
 }  // namespace g4a_chunk
-cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const g4a_chunk::PlanParams& a, bool masses);
+cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const g4a_chunk::PlanParams& a, bool masses, long long entries);

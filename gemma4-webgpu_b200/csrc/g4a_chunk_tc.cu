@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   // this pair's pieces
   const int pair = (int)(blockIdx.x >> 1), step = a.plan->step;
   const int begin = step == 1 ? a.plan->first[pair] : pair;
-  const int end = step == 1 ? a.plan->first[pair + 1] : a.plan->pieces;
+  const int end = step == 1 ? a.plan->end[pair] : a.plan->pieces;
 
   if (warp < kSoft) {
     // ------------------------------------------------------------------ softmax, epilogue
@@ -636,87 +636,122 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
 }
 
-// Joins the parts of the tiles that several pieces share.  A unit is 8 rows x 16 dims of a cut tile; the 8 warps share
-// its parts, a lane is one float4 of a row.
-constexpr int kJoinThreads = 256;
+// Joins the parts of the tiles that several pieces share.  A task is 8 rows x 64 dims of a cut tile for one warp, whose
+// lane has four float4 of a row; where a tile has many parts, 2, 4 or 8 warps share them and meet in shared memory.
+// All of a warp's loads of up to four parts are under way together: the kernel is one round of latency and what the
+// parts take from the L2 (32 MB of parts: 85 us with a warp for 16 dims of a row's every eighth part, 11 us so).
+constexpr int kJoinThreads = 256, kJoinX = 32, kJoinY = 37;
 template <int HD>
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams a) {
   using C = Cc<HD>;
   const ChunkParams& p = a.c;
-  __shared__ float4 so[8][32];
+  __shared__ float4 so[8][4][32];
   __shared__ float sm[8][8], sl[8][8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r8 = lane >> 2, c4 = lane & 3;
   pdl_wait_primary();
   pdl_launch_dependents();
-  constexpr int kBlocks = C::HDV / 16, kUnits = kTileRows / 8 * kBlocks;
-  const long long total = (long long)a.plan->cuts * kUnits;
-  for (long long u = blockIdx.x; u < total; u += gridDim.x) {
-    const Cut cut = a.cuts[u / kUnits];
-    const int at = (int)(u % kUnits), row0 = at / kBlocks * 8, block = at % kBlocks;
-    const long long gr = (long long)cut.tile * kTileRows + row0 + r8, rows = (long long)cut.T * p.group;
-    if (gr - r8 >= rows) continue;  // (the same for the whole unit)
-    const int row = row0 + r8;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (gr < rows) {
-      constexpr int kFly = 4;
-      for (int i0 = warp; i0 < cut.parts; i0 += 8 * kFly) {
-        float mi[kFly], li[kFly];
-        float4 x[kFly];
+  constexpr int kBlocks = C::HDV / 64;
+  const int cuts = a.plan->cuts;
+  for (int c = (int)blockIdx.y; c < cuts; c += (int)gridDim.y) {
+    const Cut cut = a.cuts[c];
+    const int share_log2 = cut.parts <= 4 ? 0 : cut.parts <= 8 ? 1 : cut.parts <= 16 ? 2 : 3;  // warps of a task
+    const long long left = (long long)cut.T * p.group - (long long)cut.tile * kTileRows;
+    const int live = (int)min(left, (long long)kTileRows);
+    const int tasks = (live + 7) / 8 * kBlocks, per = 8 >> share_log2;
+    for (int t0 = (int)blockIdx.x * per; t0 < tasks; t0 += (int)gridDim.x * per) {
+      const int task = t0 + (warp >> share_log2), part0 = warp & ((1 << share_log2) - 1), stride = 1 << share_log2;
+      const int block = task % kBlocks, row = task / kBlocks * 8 + r8;
+      const bool in = task < tasks && row < live;
+      float m = -INFINITY, l = 0.f;
+      float4 o[4];
 #pragma unroll
-        for (int f = 0; f < kFly; f++) {
-          const int i = i0 + 8 * f;
-          mi[f] = -INFINITY, li[f] = 0.f, x[f] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (i >= cut.parts) continue;
-          const float* part = a.part + (size_t)(cut.slot + i) * kTileRows * (C::HDV + 2);
-          mi[f] = __ldcg(part + (size_t)C::HDV * kTileRows + row);
-          li[f] = __ldcg(part + (size_t)(C::HDV + 1) * kTileRows + row);
-          x[f] = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)(block * 4 + c4) * kTileRows + row);
-        }
-        float mn = m;
+      for (int k = 0; k < 4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in) {
+        constexpr int kFly = 4;
+        for (int i0 = part0; i0 < cut.parts; i0 += stride * kFly) {
+          float mi[kFly], li[kFly];
+          float4 x[kFly][4];
 #pragma unroll
-        for (int f = 0; f < kFly; f++) mn = fmaxf(mn, mi[f]);
-        const float wo = m == mn ? 1.f : fast_exp2(m - mn);
-        m = mn;
-        l *= wo;
-        o.x *= wo, o.y *= wo, o.z *= wo, o.w *= wo;
+          for (int f = 0; f < kFly; f++) {
+            const int i = i0 + stride * f;
+            mi[f] = -INFINITY, li[f] = 0.f;
+            const float* part = a.part + (size_t)cut.slot_of(i) * kTileRows * (C::HDV + 2);
+            if (i < cut.parts) {
+              mi[f] = __ldcg(part + (size_t)C::HDV * kTileRows + row);
+              li[f] = __ldcg(part + (size_t)(C::HDV + 1) * kTileRows + row);
+            }
 #pragma unroll
-        for (int f = 0; f < kFly; f++) {
-          const float wf = mi[f] == mn ? 1.f : fast_exp2(mi[f] - mn);
-          l = fmaf(wf, li[f], l);
-          o.x = fmaf(wf, x[f].x, o.x);
-          o.y = fmaf(wf, x[f].y, o.y);
-          o.z = fmaf(wf, x[f].z, o.z);
-          o.w = fmaf(wf, x[f].w, o.w);
+            for (int k = 0; k < 4; k++)
+              x[f][k] = i < cut.parts ? __ldcg(reinterpret_cast<const float4*>(part) + (size_t)(block * 16 + 4 * k + c4) * kTileRows + row)
+                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          float mn = m;
+#pragma unroll
+          for (int f = 0; f < kFly; f++) mn = fmaxf(mn, mi[f]);
+          const float wo = m == mn ? 1.f : fast_exp2(m - mn);
+          m = mn;
+          l *= wo;
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[k].x *= wo, o[k].y *= wo, o[k].z *= wo, o[k].w *= wo;
+#pragma unroll
+          for (int f = 0; f < kFly; f++) {
+            // a part that saw nothing has weight 0 or sums of 0
+            const float wf = mi[f] == mn ? 1.f : fast_exp2(mi[f] - mn);
+            l = fmaf(wf, li[f], l);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              o[k].x = fmaf(wf, x[f][k].x, o[k].x);
+              o[k].y = fmaf(wf, x[f][k].y, o[k].y);
+              o[k].z = fmaf(wf, x[f][k].z, o[k].z);
+              o[k].w = fmaf(wf, x[f][k].w, o[k].w);
+            }
+          }
         }
       }
-    }
-    so[warp][lane] = o;
-    if (c4 == 0) sm[warp][r8] = m, sl[warp][r8] = l;
-    __syncthreads();
-    if (warp == 0 && gr < rows) {
-      float mx = -INFINITY, lt = 0.f;
-      for (int i = 0; i < 8; i++) mx = fmaxf(mx, sm[i][r8]);
-      o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int i = 0; i < 8; i++) {
-        const float wf = sm[i][r8] == mx ? 1.f : fast_exp2(sm[i][r8] - mx);
-        const float4 x = so[i][lane];
-        lt = fmaf(wf, sl[i][r8], lt);
-        o.x = fmaf(wf, x.x, o.x);
-        o.y = fmaf(wf, x.y, o.y);
-        o.z = fmaf(wf, x.z, o.z);
-        o.w = fmaf(wf, x.w, o.w);
+      if (share_log2 > 0) {  // (the same for the whole CTA)
+        if (c4 == 0) sm[warp][r8] = m, sl[warp][r8] = l;
+#pragma unroll
+        for (int k = 0; k < 4; k++) so[warp][k][lane] = o[k];
+        __syncthreads();
+        if (in && part0 == 0) {
+          float mx = m;
+          for (int i = 1; i < stride; i++) mx = fmaxf(mx, sm[warp + i][r8]);
+          l = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i = 0; i < stride; i++) {
+            const float wf = sm[warp + i][r8] == mx ? 1.f : fast_exp2(sm[warp + i][r8] - mx);
+            l = fmaf(wf, sl[warp + i][r8], l);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              const float4 x = so[warp + i][k][lane];
+              o[k].x = fmaf(wf, x.x, o[k].x);
+              o[k].y = fmaf(wf, x.y, o[k].y);
+              o[k].z = fmaf(wf, x.z, o[k].z);
+              o[k].w = fmaf(wf, x.w, o[k].w);
+            }
+          }
+          m = mx;
+        }
       }
-      const float inv = lt == 0.f ? 0.f : 1.f / lt;
-      const int kvh = cut.head / C::HALVES, half = cut.head - kvh * C::HALVES, token = (int)(gr / p.group);
-      const size_t to = (size_t)(cut.row0 + token) * p.nqh + (size_t)kvh * p.group + (size_t)(gr - (long long)token * p.group);
-      const int d = half * C::HDV + block * 16 + c4 * 4;
-      if (d < p.hd)
-        *reinterpret_cast<uint2*>(p.out + to * p.hd + d) = make_uint2(half2_bits(o.x * inv, o.y * inv), half2_bits(o.z * inv, o.w * inv));
-      if (p.lse != nullptr && d == 0) p.lse[to] = lt == 0.f ? -INFINITY : (mx + log2f(lt)) * kLn2C;
+      if (in && part0 == 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int kvh = cut.head / C::HALVES, half = cut.head - kvh * C::HALVES;
+        const long long gr = (long long)cut.tile * kTileRows + row;
+        const int token = (int)(gr / p.group);
+        const size_t to = (size_t)(cut.row0 + token) * p.nqh + (size_t)kvh * p.group + (size_t)(gr - (long long)token * p.group);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int d = half * C::HDV + block * 64 + k * 16 + c4 * 4;
+          if (d < p.hd)
+            *reinterpret_cast<uint2*>(p.out + to * p.hd + d) =
+                make_uint2(half2_bits(o[k].x * inv, o[k].y * inv), half2_bits(o[k].z * inv, o[k].w * inv));
+        }
+        if (p.lse != nullptr && block == 0 && half == 0 && c4 == 0) p.lse[to] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2C;
+      }
+      if (share_log2 > 0) __syncthreads();
     }
-    __syncthreads();
   }
 }
 
@@ -744,7 +779,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   const long long entries = (long long)p.tokens * p.group / kTileRows + std::min(p.batch, p.tokens);
   const long long items = entries * p.nkh * C::HALVES;
   if (items > (1 << 24)) return g4a_fail(G4A_EINVAL, "%s: num_tokens * num_q_heads too large", fn);
-  const long long slots = 4ll * pairs, pieces = items + slots;
+  const long long slots = 4ll * pairs, pieces = items + slots;  // (runs: an item's piece for pair w lies at item + w)
   auto up = [](size_t n) { return (n + 255) & ~size_t(255); };
   const size_t n_part = up((size_t)slots * kTileRows * (C::HDV + 2) * sizeof(float)), n_plan = up(sizeof(Plan));
   const size_t n_piece = up((size_t)pieces * sizeof(Piece)), n_cut = up((size_t)items * sizeof(Cut));
@@ -769,7 +804,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   a.pieces = q.pieces;
   a.cuts = q.cuts;
   g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
-  cudaError_t e = g4a_chunk_plan_launch(ctx, q, false);
+  cudaError_t e = g4a_chunk_plan_launch(ctx, q, false, entries);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_plan_kernel");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
@@ -787,7 +822,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, chunk_tc_kernel<HD>, mk, mv, a);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_tc_kernel");
-  e = g4a_launch(chunk_join_kernel<HD>, dim3(8 * ctx->num_sms), dim3(kJoinThreads), 0, ctx->stream, true, a);
+  e = g4a_launch(chunk_join_kernel<HD>, dim3(kJoinX, kJoinY), dim3(kJoinThreads), 0, ctx->stream, true, a);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_join_kernel");
   return G4A_OK;
 }

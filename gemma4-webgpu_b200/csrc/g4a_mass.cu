@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
   pdl_launch_dependents();
 
   const int pair = (int)(blockIdx.x >> 1);
-  const int begin = a.plan->first[pair], end = a.plan->first[pair + 1];
+  const int begin = a.plan->first[pair], end = a.plan->end[pair];
   bool ok = true;
   uint32_t g = 0, done = 0;  // blocks and pieces so far
 
@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const MassParams a) {
     if (parts.y == 1 || (parts.y == 0 && p.decay == 1.f)) continue;
     if (r >= s.L || row_offset(p, b, kvh, r) < 0) continue;
     float sum = 0.f;
-    for (int i = 0; i < parts.y; i++) sum += a.part[(size_t)(parts.x + i) * (2 * kCtaKeys) + threadIdx.x];
+    // (of the pair that begins the tile, in its place 2 w + 1; of the next ones, in 2 w)
+    for (int i = 0; i < parts.y; i++) sum += a.part[(size_t)(2 * (parts.x + i) + (i == 0)) * (2 * kCtaKeys) + threadIdx.x];
     float* at = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride + r;
     *at = r < s.base() && p.decay != 0.f ? fmaf(p.decay, *at, sum) : sum;
   }
@@ -518,7 +519,7 @@ g4a_status launch_chunk_mass(const char* fn, g4a_ctx* ctx, const ChunkParams& p)
   a.parts = q.parts;
   a.seqs = q.seqs;
   g4a_prof_scope ps(ctx, G4A_PROF_KEY_MASS);
-  cudaError_t e = g4a_chunk_plan_launch(ctx, q, true);
+  cudaError_t e = g4a_chunk_plan_launch(ctx, q, true, entries);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_plan_kernel");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * pairs));
