@@ -9,8 +9,9 @@
 
 using namespace g4a_chunk;
 
-// The tensor-core kernel (g4a_chunk_tc.cu).
+// Tiles of 256 query rows on the tensor cores (g4a_chunk_tc.cu), and few rows from registers (g4a_chunk_few.cu).
 g4a_status g4a_chunk_tc_launch(g4a_ctx* ctx, const ChunkParams& p);
+g4a_status g4a_chunk_few_launch(g4a_ctx* ctx, const ChunkParams& p);
 
 g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, ChunkParams& p, const uint16_t* q, const uint16_t* k_pages,
                             const uint16_t* v_pages, const int32_t* page_table, const int32_t* kv_lens,
@@ -114,5 +115,7 @@ extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, cons
   if (dev.status != G4A_OK) return dev.status;
   p.lse = lse;
   p.out = reinterpret_cast<__half*>(out);
-  return g4a_chunk_tc_launch(ctx, p);
+  // query rows of a sequence and kv head, on average
+  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 8u * (uint64_t)batch && (uint64_t)batch * num_kv_heads <= 65535u;
+  return few ? g4a_chunk_few_launch(ctx, p) : g4a_chunk_tc_launch(ctx, p);
 }

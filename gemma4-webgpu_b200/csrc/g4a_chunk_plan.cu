@@ -161,8 +161,10 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
   for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
   if (MASS && tid <= p.batch) a.seqs[tid] = make_int4(0, (tid < p.batch && tid < kPlanThreads ? entry_s[tid] : entries) * heads, 0, 0);
   __syncthreads();
-  if (items == 0) {
+  if (items == 0 || entries > a.max_entries) {
     if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0;
+    if (tid == 0 && items != 0) atomicExch(p.err, G4A_DEVERR_TREE);
+    if (MASS && tid < p.batch) a.seqs[tid] = make_int4(0, -1, 0, 0);
     return;
   }
   // ---- tiles: a thread's sequence is the last one whose entries begin at or before it (those without any share a begin)
@@ -293,6 +295,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
   pdl_launch_dependents();
   if (tid == 0) cut_count = 0;
   // ---- sequences: entries (tiles of one head) and items before each, the most stages of a tile
+  long long entries_all = 0;
   int entries = 0, items = 0, longest = 0;
   float rows_seen = 0.f;  // rows of the cache that have to be read, over the sequences (for one kv head)
   for (int b0 = 0; b0 < p.batch; b0 += kPlanThreads) {
@@ -312,6 +315,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     const int mine = (int)x[0], mine_items = (int)x[1];
     block_scan<2>(x, all, reinterpret_cast<long long(*)[2]>(warp_sum));
     if (b < p.batch) a.seqs[b] = make_int4(entries + (int)x[0] - mine, items + (int)x[1] - mine_items, most, 0);
+    entries_all += all[0];
     entries += (int)all[0];
     items += (int)all[1];
     longest = max(longest, most);
@@ -332,6 +336,12 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     __syncthreads();
     longest = most_s;
     rows_seen = seen_s;
+  }
+  if (entries_all > a.max_entries) {  // (the same for all threads)
+    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0, atomicExch(p.err, G4A_DEVERR_TREE);
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
+    for (int b = tid; MASS && b < p.batch; b += kPlanThreads) a.seqs[b] = make_int4(0, -1, 0, 0);
+    return;
   }
   // ---- stages of all earlier entries
   long long total = 0;  // of one head

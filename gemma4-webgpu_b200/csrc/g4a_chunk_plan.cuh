@@ -42,6 +42,7 @@ struct PlanParams {
   ChunkParams c;
   int pairs, halves, kb_log2;  // halves of the head dims; keys of a block (masses: of a tile)
   int max_slots;
+  long long max_entries;  // tiles that there is room for (more: the sequences' rows of q overlap)
   float stage_bytes, stage_ns;  // of a block: what is loaded, about how long it takes
   int block_tokens, head_chunks;  // masses: tokens of a row block, row blocks for the heads of one token
   Plan* plan;

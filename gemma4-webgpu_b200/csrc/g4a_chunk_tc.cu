@@ -792,6 +792,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   q.halves = C::HALVES;
   q.kb_log2 = C::KB_LOG2;
   q.max_slots = (int)slots;
+  q.max_entries = entries;
   q.stage_bytes = 2.f * (C::K_BYTES + C::V_BYTES);
   q.stage_ns = C::KB * (HD + C::HDV) * (1.f / 55.f);
   a.part = reinterpret_cast<float*>(ws);

@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const MassParams a) {
   const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
   const Seq s = seq_of(p, b, min((long long)p.max_pages * p.page_size, p.mass_stride));
   const Blocks k = key_tiles_of(p, s, kTileLog2);
+  if (a.seqs[b].y < 0) return;  // the call does not fit together
   const int item0 = a.seqs[b].y + kvh * k.count();
   for (int tile = (int)blockIdx.x; tile << kTileLog2 < s.L; tile += (int)gridDim.x) {
     const int r = (tile << kTileLog2) + (int)threadIdx.x;
@@ -506,6 +507,7 @@ g4a_status launch_chunk_mass(const char* fn, g4a_ctx* ctx, const ChunkParams& p)
   q.halves = 1;
   q.kb_log2 = kTileLog2;
   q.stage_ns = 1.f;
+  q.max_entries = entries;
   q.block_tokens = 2 * a.tokens;
   q.head_chunks = a.head_chunks;
   a.part = reinterpret_cast<float*>(ws);

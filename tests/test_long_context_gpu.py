@@ -76,6 +76,66 @@ def test_chunk_attention(ctx, counts, lens, nkh, group, hd, page, window, sinks)
     _check(ctx, case, q, window=window, sinks=sinks)
 
 
+FEW = [  # few query rows to a sequence: decode steps, some sequences idle, some with more tokens than the others
+    ([1, 0, 1], [1, 40, 500], 1, 8, 256, 64, 0, 0),
+    ([20, 0, 0], [333, 5, 9], 1, 1, 128, 16, 0, 0),
+    ([5, 1, 0, 2], [70, 1, 3, 2], 2, 3, 96, 7, 0, 0),
+    ([3, 1, 0], [120, 900, 4], 1, 4, 512, 16, 50, 5),
+    ([7, 1], [200, 1000], 1, 2, 256, 64, 33, 3),
+    ([1, 1], [17, 16], 4, 5, 64, 8, 0, 0),
+    ([8], [8], 3, 1, 8, 1, 3, 1),
+    ([1] * 9, [15 * i + 1 for i in range(9)], 1, 7, 200, 5, 0, 0),
+    ([1, 2, 1, 0], [600, 601, 602, 3], 1, 3, 384, 24, 512, 4),
+    ([6, 0], [300, 1], 1, 2, 320, 48, 100, 40),
+    ([1], [3000], 2, 8, 512, 64, 2000, 200),
+]
+
+
+@pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", FEW)
+def test_chunk_attention_of_few_rows(ctx, counts, lens, nkh, group, hd, page, window, sinks):
+    case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
+    _check(ctx, case, q, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hd,group", [(64, 1), (256, 2), (512, 1), (512, 3)])
+def test_values_that_are_not_finite_in_steps_of_few_rows(ctx, hd, group):
+    counts, lens, window, sinks = [4, 1, 0, 0], [200, 40, 5, 9], 30, 3
+    case, q = _case(hd, counts, lens, nkh=1, group=group, hd=hd, page=16)
+    clean, lse0 = _attend(ctx, case, q, window=window, sinks=sinks)
+    plant = [(0, 198, 5, float("inf")), (0, 199, hd - 1, float("nan")), (0, 1, 0, -float("inf")), (0, 168, 9, float("inf")),
+             (0, 100, 4, float("nan")), (1, 39, 3, -float("inf"))]
+    for b, r, d, x in plant:
+        case.v[case.table_host[b, r // 16], r % 16, 0, d] = x
+    out, lse = _attend(ctx, case, q, window=window, sinks=sinks)
+    want = clean.double()
+    for b, r, d, x in plant:
+        for i in range(counts[b]):
+            pos = lens[b] - counts[b] + i
+            if r <= pos and (r > pos - window or r < sinks):
+                want[case.indptr_host[b] + i, :, d] += x
+    finite = want.isfinite()
+    assert torch.equal(lse, lse0) and torch.equal(out.isfinite(), finite) and torch.equal(out[finite], clean[finite])
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want == float("inf"))
+
+
+def test_sequences_whose_rows_overlap_are_refused_where_they_do_not_fit(ctx):
+    """q_indptr that goes back and forth: each second sequence is in itself well formed, all together they are more than
+    num_tokens; nothing is written out of bounds."""
+    n, t = 40, 120
+    case, q = _case(7, [t], [300], nkh=1, group=8, hd=128, page=16)
+    table = case.table.expand(n, -1).contiguous()
+    lens = torch.full((n,), 300, dtype=torch.int32, device="cuda")
+    indptr = torch.tensor([0, t] * (n // 2) + [0], dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda")
+    mass = torch.zeros((n, 1, 300), device="cuda")
+    ctx.chunk_attn_paged(q, case.k, case.v, table, lens, indptr, out, lse, scale=0.1, **_shape(case, q))
+    with pytest.raises(G4AError, match="do not fit"):
+        ctx.sync()
+    ctx.paged_key_mass(q, lse, case.k, table, lens, indptr, mass, scale=0.1, **_shape(case, q))
+    with pytest.raises(G4AError, match="do not fit"):
+        ctx.sync()
+
+
 @pytest.mark.parametrize("hd,counts,lens,window,sinks", [
     (256, [1], [40_001], 0, 0), (512, [3], [30_000], 0, 0), (128, [20, 1], [9_000, 17_000], 0, 0),
     (256, [600], [5_003], 512, 4), (256, [900], [2_100], 0, 0), (512, [400], [3_300], 0, 0), (128, [1500], [1_900], 0, 0),
@@ -225,6 +285,66 @@ def _check_mass(ctx, case, q, *, window=0, sinks=0, decay=1.0):
 def test_key_mass(ctx, counts, lens, nkh, group, hd, page, window, sinks, decay):
     case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
     _check_mass(ctx, case, q, window=window, sinks=sinks, decay=decay)
+
+
+FEW = [  # few query rows to a sequence: decode steps, some sequences idle, some with more tokens than the others
+    ([1, 0, 1], [1, 40, 500], 1, 8, 256, 64, 0, 0),
+    ([20, 0, 0], [333, 5, 9], 1, 1, 128, 16, 0, 0),
+    ([5, 1, 0, 2], [70, 1, 3, 2], 2, 3, 96, 7, 0, 0),
+    ([3, 1, 0], [120, 900, 4], 1, 4, 512, 16, 50, 5),
+    ([7, 1], [200, 1000], 1, 2, 256, 64, 33, 3),
+    ([1, 1], [17, 16], 4, 5, 64, 8, 0, 0),
+    ([8], [8], 3, 1, 8, 1, 3, 1),
+    ([1] * 9, [15 * i + 1 for i in range(9)], 1, 7, 200, 5, 0, 0),
+    ([1, 2, 1, 0], [600, 601, 602, 3], 1, 3, 384, 24, 512, 4),
+    ([6, 0], [300, 1], 1, 2, 320, 48, 100, 40),
+    ([1], [3000], 2, 8, 512, 64, 2000, 200),
+]
+
+
+@pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", FEW)
+def test_chunk_attention_of_few_rows(ctx, counts, lens, nkh, group, hd, page, window, sinks):
+    case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
+    _check(ctx, case, q, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("hd,group", [(64, 1), (256, 2), (512, 1), (512, 3)])
+def test_values_that_are_not_finite_in_steps_of_few_rows(ctx, hd, group):
+    counts, lens, window, sinks = [4, 1, 0, 0], [200, 40, 5, 9], 30, 3
+    case, q = _case(hd, counts, lens, nkh=1, group=group, hd=hd, page=16)
+    clean, lse0 = _attend(ctx, case, q, window=window, sinks=sinks)
+    plant = [(0, 198, 5, float("inf")), (0, 199, hd - 1, float("nan")), (0, 1, 0, -float("inf")), (0, 168, 9, float("inf")),
+             (0, 100, 4, float("nan")), (1, 39, 3, -float("inf"))]
+    for b, r, d, x in plant:
+        case.v[case.table_host[b, r // 16], r % 16, 0, d] = x
+    out, lse = _attend(ctx, case, q, window=window, sinks=sinks)
+    want = clean.double()
+    for b, r, d, x in plant:
+        for i in range(counts[b]):
+            pos = lens[b] - counts[b] + i
+            if r <= pos and (r > pos - window or r < sinks):
+                want[case.indptr_host[b] + i, :, d] += x
+    finite = want.isfinite()
+    assert torch.equal(lse, lse0) and torch.equal(out.isfinite(), finite) and torch.equal(out[finite], clean[finite])
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want == float("inf"))
+
+
+def test_sequences_whose_rows_overlap_are_refused_where_they_do_not_fit(ctx):
+    """q_indptr that goes back and forth: each second sequence is in itself well formed, all together they are more than
+    num_tokens; nothing is written out of bounds."""
+    n, t = 40, 120
+    case, q = _case(7, [t], [300], nkh=1, group=8, hd=128, page=16)
+    table = case.table.expand(n, -1).contiguous()
+    lens = torch.full((n,), 300, dtype=torch.int32, device="cuda")
+    indptr = torch.tensor([0, t] * (n // 2) + [0], dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda")
+    mass = torch.zeros((n, 1, 300), device="cuda")
+    ctx.chunk_attn_paged(q, case.k, case.v, table, lens, indptr, out, lse, scale=0.1, **_shape(case, q))
+    with pytest.raises(G4AError, match="do not fit"):
+        ctx.sync()
+    ctx.paged_key_mass(q, lse, case.k, table, lens, indptr, mass, scale=0.1, **_shape(case, q))
+    with pytest.raises(G4AError, match="do not fit"):
+        ctx.sync()
 
 
 @pytest.mark.parametrize("hd,counts,lens,window,sinks", [
