@@ -61,6 +61,24 @@ __device__ __forceinline__ long long row_offset(const ChunkParams& p, int b, int
   return (((long long)page * p.page_size + (key - j * p.page_size)) * p.nkh + kvh) * p.hd;
 }
 
+// For the kernels of few query rows, whose operands come straight from global memory.
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 16 bytes that are read once (in pieces of 64 bytes a row: the L2 fetches their neighbours with them; 64 decode
+// sequences 117 -> 111 us).
+__device__ __forceinline__ uint4 load_once(const __half* at) {
+  uint4 x;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "l"(at));
+  return x;
+}
+
 }  // namespace g4a_chunk
 
 // Checks of the arguments that the two entry points share; fills p but for what each of them adds.

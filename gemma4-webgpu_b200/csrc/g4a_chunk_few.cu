@@ -26,7 +26,9 @@ namespace {
 using namespace g4a;
 using namespace g4a_chunk;
 
-constexpr int kWarps = 8, kStepKeys = 16, kTile = 8;  // warps of a CTA; keys of a step; query rows of a tile
+constexpr int kWarps = 4, kStepKeys = 16, kTile = 8;  // warps of a CTA; keys of a step; query rows of a tile
+constexpr int kNoKey = -1 - 0x7fffffff;
+constexpr long long kRounds = 3;  // of CTAs to the SMs' room (1: 135 us for 64 decode sequences, 2 to 4: 117, 6: 123)
 constexpr float kRaiseF = 15.0f, kFirstF = -3.0f, kLaterF = 5.0f, kUnseenF = -FLT_MAX;
 
 struct FewParams {
@@ -58,13 +60,6 @@ __device__ __forceinline__ size_t tile_place(const ChunkParams& p, const Seq& s,
   return (size_t)((uint32_t)((long long)s.row0 * p.group / kTile)) + (size_t)b + (size_t)tile;
 }
 
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                    uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -79,7 +74,7 @@ __device__ __forceinline__ bool clear_bad(uint32_t& w) {
 
 // SEG: 32-dim segments of a warp's share of a head; SHARE: warps that share a head's dims.
 template <int SEG, int SHARE>
-__global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewParams a) {
+__global__ void __launch_bounds__(kWarps * 32, 2) chunk_few_kernel(const FewParams a) {
   constexpr int DIMS = SEG * 32, CH = DIMS / 64, GROUPS = kWarps / SHARE;
   constexpr int PITCH = DIMS + 4;  // floats from row to row where the warps meet
   const ChunkParams& p = a.c;
@@ -124,21 +119,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
 #pragma unroll
         for (int k = 0; k < 4; k++) o[c][i][k] = 0.f;
     bool taken = false;  // values of V that are not finite
+    // The page of key g (+ 8) of a step, looked up one step ahead; -1: nobody sees the key
+    auto first_key = [&](int i) { return (i < st.sinks ? i : i - st.sinks + st.w0) * kStepKeys; };
+    auto page_of = [&](int i, int h) {
+      const int key = first_key(i) + g + 8 * h;
+      return i < i1 && key <= pos1 && (key >= lo0 || (uint32_t)key < p.sinks) ? table[(uint32_t)key / (uint32_t)p.page_size] : kNoKey;
+    };
+    int pages[2] = {page_of(i0 + group, 0), page_of(i0 + group, 1)};
     for (int i = i0 + group; i < i1; i += GROUPS) {
-      const int k0 = (i < st.sinks ? i : i - st.sinks + st.w0) * kStepKeys;
-      // where this lane's rows of K (keys g, g + 8) and V (2 t, 2 t + 1, 2 t + 8, 2 t + 9) lie; -1: nobody sees them
-      auto place = [&](int key) -> long long {
-        if (key > pos1 || !(key >= lo0 || (uint32_t)key < p.sinks)) return -1;
-        const int j = key / p.page_size, page = table[j];
-        if (page < 0 || page >= p.num_pages) {
-          atomicExch(p.err, G4A_DEVERR_PAGE);
-          return -1;
-        }
-        return (((long long)page * p.page_size + (key - j * p.page_size)) * p.nkh + kvh) * p.hd + d_warp;
-      };
+      const int k0 = first_key(i);
+      // where this lane's rows of K (keys g, g + 8) and V (2 t, 2 t + 1, 2 t + 8, 2 t + 9) lie; -1: not there
       long long at_k[2], at_v[4];
 #pragma unroll
-      for (int h = 0; h < 2; h++) at_k[h] = place(k0 + g + 8 * h);
+      for (int h = 0; h < 2; h++) {
+        const uint32_t key = (uint32_t)(k0 + g + 8 * h);
+        at_k[h] = (((long long)pages[h] * p.page_size + key % (uint32_t)p.page_size) * p.nkh + kvh) * p.hd + d_warp;
+        if (pages[h] < 0 || pages[h] >= p.num_pages) {
+          if (pages[h] != kNoKey) atomicExch(p.err, G4A_DEVERR_PAGE);
+          at_k[h] = -1;
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 4; h++)  // (a lane of the same key has looked it up: key 2 t + h is row 2 t + h of K, and so on)
         at_v[h] = __shfl_sync(0xffffffffu, h < 2 ? at_k[0] : at_k[1], (2 * t + (h & 1)) * 4);
@@ -148,15 +148,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
 #pragma unroll
         for (int e = 0; e < SEG; e++)
           k[h][e] = at_k[h] >= 0 && d_warp + e * 32 + t * 8 < p.hd
-                        ? __ldg(reinterpret_cast<const uint4*>(p.k + at_k[h] + e * 32 + t * 8))
+                        ? load_once(p.k + at_k[h] + e * 32 + t * 8)
                         : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int h = 0; h < 4; h++)
 #pragma unroll
         for (int c = 0; c < CH; c++)
           v[h][c] = at_v[h] >= 0 && d_warp + c * 64 + g * 8 < p.hd
-                        ? __ldg(reinterpret_cast<const uint4*>(p.v + at_v[h] + c * 64 + g * 8))
+                        ? load_once(p.v + at_v[h] + c * 64 + g * 8)
                         : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int h = 0; h < 2; h++) pages[h] = page_of(i + GROUPS, h);
       float x[4];  // row g, keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -164,8 +166,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
 #pragma unroll
         for (int e = 0; e < SEG; e++) {
           const uint4 q = q_s[share][e][lane];
-          mma(c, q.x, 0u, q.y, 0u, k[h][e].x, k[h][e].y);
-          mma(c, q.z, 0u, q.w, 0u, k[h][e].z, k[h][e].w);
+          mma_16x8x16(c, q.x, 0u, q.y, 0u, k[h][e].x, k[h][e].y);
+          mma_16x8x16(c, q.z, 0u, q.w, 0u, k[h][e].z, k[h][e].w);
         }
         x[2 * h] = c[0];
         x[2 * h + 1] = c[1];
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const uint32_t pick = (e & 1) ? 0x7632u : 0x5410u;  // the upper or the lower halves
-          mma(o[c][e], __byte_perm(word(0, 2 * c, e), word(1, 2 * c, e), pick),
+          mma_16x8x16(o[c][e], __byte_perm(word(0, 2 * c, e), word(1, 2 * c, e), pick),
               __byte_perm(word(0, 2 * c + 1, e), word(1, 2 * c + 1, e), pick),
               __byte_perm(word(2, 2 * c, e), word(3, 2 * c, e), pick),
               __byte_perm(word(2, 2 * c + 1, e), word(3, 2 * c + 1, e), pick), b0, b1);
@@ -251,8 +253,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
         for (int k = 0; k < 4; k++)  // row 2 t + (k & 1), dim 8 g + e of chunk 2 c + (k >> 1)
           mine[(2 * t + (k & 1)) * PITCH + (2 * c + (k >> 1)) * 64 + 8 * g + e] = o[c][e][k];
     taken = __syncthreads_or(taken);
-    {
-      const int row = warp;  // of the tile: a warp for each
+    for (int row = warp; row < kTile; row += kWarps) {  // of the tile
       float mx = kUnseenF, lt = 0.f;
 #pragma unroll
       for (int i = 0; i < GROUPS; i++) mx = fmaxf(mx, m_s[i * SHARE][row]);
@@ -282,7 +283,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) chunk_few_kernel(const FewPara
           if (taken) {  // (rare) the values that were taken out of this part's steps, for the keys that the row sees
             const int p_row = base + tok;
             for (int i = i0; i < i1; i++) {
-              const int k0 = (i < st.sinks ? i : i - st.sinks + st.w0) * kStepKeys;
+              const int k0 = first_key(i);
               if (k0 + kStepKeys <= pos0 + 1 && (k0 >= lo1 || (uint32_t)(k0 + kStepKeys) <= p.sinks)) continue;
               for (int key = k0; key < k0 + kStepKeys && key <= p_row; key++) {
                 if (!sees(p, p_row, key)) continue;
@@ -411,12 +412,12 @@ g4a_status launch(g4a_ctx* ctx, const ChunkParams& p) {
   FewParams a = {};
   a.c = p;
   const long long heads = (long long)p.batch * p.nkh;
-  // rows that a sequence can read, in CTAs with a step for every group; as many CTAs as make four rounds of the SMs
+  // rows that a sequence can read, in CTAs with a step for every group; as many CTAs as make some rounds of the SMs
   const uint64_t cap = (uint64_t)p.page_size * p.max_pages;
   uint64_t keys = cap;
   if (p.window != 0u) keys = std::min<uint64_t>(cap, (uint64_t)p.window + p.sinks + 4 * kStepKeys);
   a.splits = (int)std::max<long long>(
-      1, std::min<long long>((long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys)), (4ll * ctx->num_sms + heads - 1) / heads));
+      1, std::min<long long>((long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys)), (kRounds * 2ll * ctx->num_sms + heads - 1) / heads));
   const size_t tiles = (size_t)((long long)p.tokens * p.group / kTile) + (size_t)p.batch;
   const size_t need = tiles * p.nkh * a.splits * kTile * (p.hd + 2) * sizeof(float);
   if (g4a_status s = g4a_ensure_workspace(ctx, need)) return s;

@@ -22,44 +22,52 @@ using namespace g4a_chunk;
 
 // ------------------------------------------------------------------------------------ few query rows
 
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                            uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-constexpr int kFewWarps = 8;
+constexpr int kFewWarps = 4;
+constexpr unsigned kFewRounds = 8;  // CTAs to an SM (24 sequences of 512 dims: 4, 8, 12: 74.5, 69.9, 71.6 us)
+constexpr int kNoKey = -1 - 0x7fffffff;
 
 // SEG: segments of 32 dims.  Lane 4 g + t holds dims 32 s + 8 t .. + 7 of keys g and g + 8 and of query row g.
 template <int SEG>
-__global__ void __launch_bounds__(kFewWarps * 32) mass_few_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kernel(const ChunkParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
   pdl_wait_primary();
   pdl_launch_dependents();
   const Seq s = seq_of(p, b, min((long long)p.max_pages * p.page_size, p.mass_stride));
-  const int base = s.base();
+  const int base = s.base(), stride = (int)gridDim.x * kFewWarps * 16;
+  const int* table = p.page_table + (size_t)b * p.max_pages;
   const __half* q = p.q + ((size_t)s.row0 * p.nqh + (size_t)kvh * p.group) * p.hd;
   const float* lse = p.lse + (size_t)s.row0 * p.nqh + (size_t)kvh * p.group;
   float* mass = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride;
-  for (int k0 = ((int)blockIdx.x * kFewWarps + warp) * 16; k0 < s.L; k0 += (int)gridDim.x * kFewWarps * 16) {
+  // the pages of keys g and g + 8, looked up one step ahead
+  auto page_of = [&](long long key) { return key < s.L ? table[(uint32_t)key / (uint32_t)p.page_size] : kNoKey; };
+  int k0 = ((int)blockIdx.x * kFewWarps + warp) * 16;
+  int pages[2] = {page_of(k0 + g), page_of(k0 + g + 8)};
+  for (; k0 < s.L; k0 += stride) {
+    long long off[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint32_t key = (uint32_t)(k0 + g + 8 * h);
+      off[h] = (((long long)pages[h] * p.page_size + key % (uint32_t)p.page_size) * p.nkh + kvh) * p.hd;
+      if (pages[h] < 0 || pages[h] >= p.num_pages) {
+        if (pages[h] != kNoKey) atomicExch(p.err, G4A_DEVERR_PAGE);
+        off[h] = -1;
+      }
+      pages[h] = page_of((long long)key + stride);
+    }
     const Tokens see = tokens_of(p, s, k0, 16);
     const bool any = see.first < see.last;
     if (!any && p.decay == 1.f && k0 + 16 <= base) continue;  // nothing changes
-    long long off[2] = {-1, -1};
     float old[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
     uint4 k[2][SEG];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int key = k0 + g + 8 * h;
-      if (key < s.L) off[h] = row_offset(p, b, kvh, key);
       if (t == 0 && off[h] >= 0 && key < base && p.decay != 0.f) old[h] = p.decay * mass[key];
 #pragma unroll
       for (int e = 0; e < SEG; e++) {
         const int d = e * 32 + t * 8;
-        k[h][e] = any && off[h] >= 0 && d < p.hd ? __ldg(reinterpret_cast<const uint4*>(p.k + off[h] + d)) : make_uint4(0, 0, 0, 0);
+        k[h][e] = any && off[h] >= 0 && d < p.hd ? load_once(p.k + off[h] + d) : make_uint4(0, 0, 0, 0);
       }
     }
     const long long r_end = (long long)see.last * p.group;
@@ -101,7 +109,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) mass_few_kernel(const ChunkPar
 constexpr int kThreadsM = 512;
 constexpr int kTileLog2 = 8, kCtaKeys = 128;  // keys of a tile; of a CTA
 constexpr int kWarpK = 8, kWarpQ = 9, kWarpMma = 10, kWarpLse = 11, kWarpTell = 12;
-constexpr int kScoreBufs = 4, kInfoM = 4;
+constexpr int kScoreBufs = 4, kInfoM = 2;
 
 template <int HD>
 struct Mc {
@@ -109,14 +117,14 @@ struct Mc {
   static constexpr int NC = HD / 64;
   static constexpr int K_CHUNK = kCtaKeys * 128, Q_CHUNK = RB / 2 * 128;
   static constexpr int K_BYTES = NC * K_CHUNK, Q_BYTES = NC * Q_CHUNK;
-  static constexpr int NK = HD > 256 ? 1 : 2, NQ = HD <= 128 ? 4 : 2;
+  static constexpr int NK = HD > 256 ? 1 : 2, NQ = HD <= 128 ? 6 : 3;  // tiles of keys, row blocks in flight
   static constexpr int OFF_Q = NK * K_BYTES;
   static constexpr int OFF_LSE = OFF_Q + NQ * Q_BYTES;            // [kInfoM][RB] -lse log2e
   static constexpr int OFF_VALID = OFF_LSE + kInfoM * RB * 4;     // [kInfoM][4] rows that count
   static constexpr int OFF_SUM = OFF_VALID + kInfoM * 16;         // [2][128] sums of the second set of warps
   static constexpr int OFF_BAR = OFF_SUM + 2 * kCtaKeys * 4;
   static constexpr int NBARS = 3 * NK + 3 * NQ + 2 * kScoreBufs + 2 * kInfoM + 5;
-  static constexpr size_t SMEM = 1024 + (size_t)OFF_BAR + NBARS * 8 + 16;
+  static constexpr size_t SMEM = (size_t)OFF_BAR + NBARS * 8 + 16;
   static constexpr uint32_t TMEM_COLS = 512;
   static_assert(kScoreBufs * RB <= 512 && SMEM <= 232448, "tile fits");
 };
@@ -137,9 +145,11 @@ __global__ void __launch_bounds__(kThreadsM, 1)
     mass_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmq, const MassParams a) {
   using C = Mc<HD>;
   const ChunkParams& p = a.c;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* smem =
-      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) unsigned char smem[];  // (there is no room to align it by hand)
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicExch(p.err, G4A_DEVERR_TMEM);
+    return;
+  }
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* k_landed = bars;                   // [NK] this CTA's keys
   uint64_t* k_ready = k_landed + C::NK;        // [NK] first CTA: of both
@@ -552,7 +562,7 @@ g4a_status launch_few(g4a_ctx* ctx, const ChunkParams& p) {
   const unsigned heads = (unsigned)p.batch * (unsigned)p.nkh;
   const long long rows = std::min<long long>((long long)p.page_size * p.max_pages, p.mass_stride);
   const unsigned wide = (unsigned)std::min<long long>((rows + kFewWarps * 16 - 1) / (kFewWarps * 16),
-                                                      std::max(1u, 32u * (unsigned)ctx->num_sms / heads));
+                                                      std::max(1u, kFewRounds * (unsigned)ctx->num_sms / heads));
   const cudaError_t e = g4a_launch(mass_few_kernel<SEG>, dim3(wide, heads), dim3(kFewWarps * 32), 0, ctx->stream, true, p);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_few_kernel");
   return G4A_OK;
