@@ -304,21 +304,22 @@ __global__ void __launch_bounds__(kThreadsC, 1)
             }
           }
         }
-        const float up = -m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t by2 = f32x2(by, by), up2 = f32x2(-m, -m);
+        uint64_t sum[2] = {0, 0};
         uint32_t pw[HB / 2];
 #pragma unroll
         for (int e = 0; e < HB / 2; e++) {
-          const float x = fast_exp2(fmaf(__uint_as_float(s[e >> 4][(2 * e) & 31]), by, up));
-          const float y = fast_exp2(fmaf(__uint_as_float(s[e >> 4][(2 * e + 1) & 31]), by, up));
-          sum[(2 * e) & 3] += x;
-          sum[(2 * e + 1) & 3] += y;
-          pw[e] = half2_bits(x, y);
+          const uint64_t x = f32x2(__uint_as_float(s[e >> 4][(2 * e) & 31]), __uint_as_float(s[e >> 4][(2 * e + 1) & 31]));
+          const float2 y = f32x2_parts(fma_f32x2(x, by2, up2));
+          const float w0 = fast_exp2(y.x), w1 = fast_exp2(y.y);
+          sum[e & 1] = add_f32x2(sum[e & 1], f32x2(w0, w1));
+          pw[e] = half2_bits(w0, w1);
         }
         // (where the other half's scores were: it has read them, or it would not have come to the exchange)
         if constexpr (HB == 64) tmem_st32(col + half * 32u, pw);
         else tmem_st16(col + half * 16u, pw);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 total = f32x2_parts(add_f32x2(sum[0], sum[1]));
+        l += total.x + total.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kern
 constexpr int kThreadsM = 512;
 constexpr int kTileLog2 = 8, kCtaKeys = 128;  // keys of a tile; of a CTA
 constexpr int kWarpK = 8, kWarpQ = 9, kWarpMma = 10, kWarpLse = 11, kWarpTell = 12;
-constexpr int kScoreBufs = 4, kInfoM = 2;
+constexpr int kScoreBufs = 4, kLseBufs = 3;
 
 template <int HD>
 struct Mc {
@@ -119,11 +119,11 @@ struct Mc {
   static constexpr int K_BYTES = NC * K_CHUNK, Q_BYTES = NC * Q_CHUNK;
   static constexpr int NK = HD > 256 ? 1 : 2, NQ = HD <= 128 ? 6 : 3;  // tiles of keys, row blocks in flight
   static constexpr int OFF_Q = NK * K_BYTES;
-  static constexpr int OFF_LSE = OFF_Q + NQ * Q_BYTES;            // [kInfoM][RB] -lse log2e
-  static constexpr int OFF_VALID = OFF_LSE + kInfoM * RB * 4;     // [kInfoM][4] rows that count
-  static constexpr int OFF_SUM = OFF_VALID + kInfoM * 16;         // [2][128] sums of the second set of warps
+  static constexpr int OFF_LSE = OFF_Q + NQ * Q_BYTES;            // [kLseBufs][RB] -lse log2e
+  static constexpr int OFF_VALID = OFF_LSE + kLseBufs * RB * 4;    // [kLseBufs][4] rows that count
+  static constexpr int OFF_SUM = OFF_VALID + kLseBufs * 16;         // [2][128] sums of the second set of warps
   static constexpr int OFF_BAR = OFF_SUM + 2 * kCtaKeys * 4;
-  static constexpr int NBARS = 3 * NK + 3 * NQ + 2 * kScoreBufs + 2 * kInfoM + 5;
+  static constexpr int NBARS = 3 * NK + 3 * NQ + 3 * kScoreBufs + 5;
   static constexpr size_t SMEM = (size_t)OFF_BAR + NBARS * 8 + 16;
   static constexpr uint32_t TMEM_COLS = 512;
   static_assert(kScoreBufs * RB <= 512 && SMEM <= 232448, "tile fits");
@@ -157,11 +157,10 @@ __global__ void __launch_bounds__(kThreadsM, 1)
   uint64_t* q_landed = k_free + C::NK;         // [NQ] this CTA's half of a row block
   uint64_t* q_ready = q_landed + C::NQ;        // [NQ] first CTA: both
   uint64_t* q_free = q_ready + C::NQ;          // [NQ] scores done (commit)
-  uint64_t* s_done = q_free + C::NQ;           // [kScoreBufs] scores (commit)
+  uint64_t* s_done = q_free + C::NQ;           // [kScoreBufs] scores (commit), and the block's log-sum-exps (warp 11)
   uint64_t* s_free = s_done + kScoreBufs;      // [kScoreBufs] first CTA: read (4 warps of each)
-  uint64_t* lse_full = s_free + kScoreBufs;    // [kInfoM] the block's log-sum-exps are here
-  uint64_t* lse_free = lse_full + kInfoM;      // [kInfoM] read (4 warps)
-  uint64_t* sum_full = lse_free + kInfoM;      // [2] sums of the second set (4 warps)
+  uint64_t* lse_free = s_free + kScoreBufs;    // [kLseBufs] read (4 warps)
+  uint64_t* sum_full = lse_free + kLseBufs;    // [2] sums of the second set (4 warps)
   uint64_t* sum_free = sum_full + 2;           // [2] read (4 warps)
   uint64_t* all_done = sum_free + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBARS);
@@ -184,11 +183,8 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       mbar_init(&q_free[s], 1);
     }
     for (int s = 0; s < kScoreBufs; s++) {
-      mbar_init(&s_done[s], 1);
+      mbar_init(&s_done[s], 2);
       mbar_init(&s_free[s], 8);
-    }
-    for (int s = 0; s < kInfoM; s++) {
-      mbar_init(&lse_full[s], 1);
       mbar_init(&lse_free[s], 4);
     }
     for (int s = 0; s < 2; s++) {
@@ -240,27 +236,31 @@ __global__ void __launch_bounds__(kThreadsM, 1)
       // the tokens that see the key
       const int see0 = key - base;
       const int see1 = p.window == 0u || (uint32_t)key < p.sinks ? 0x7fffffff : (int)min(0x7fffffffll, (long long)see0 + p.window);
-      float2 acc[4] = {};
+      uint64_t acc[4] = {0, 0, 0, 0};  // pairs of sums
       for (int j = d.j0; j < d.j1; j++, g++) {
         if ((g & 1u) != set) continue;
-        const uint32_t buf = g % kScoreBufs, inf = g % kInfoM;
-        ok = warp_wait_own(&lse_full[inf], (g / kInfoM) & 1u, abort_flag, p.err) &&
-             warp_wait_own(&s_done[buf], (g / kScoreBufs) & 1u, abort_flag, p.err);
+        const uint32_t buf = g % kScoreBufs;
+        ok = warp_wait_own(&s_done[buf], (g / kScoreBufs) & 1u, abort_flag, p.err);
         if (!ok) break;
         tc_fence_after();
-        const float* nl = reinterpret_cast<const float*>(smem + C::OFF_LSE) + inf * C::RB;
-        const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + C::OFF_VALID + inf * 16);
-        const int t0 = (d.skip + j / a.head_chunks) * 2 * a.tokens;
+        constexpr int kWords = C::RB / 32, kHalfWords = C::RB / 64;
+        uint32_t s[2][32];
+        tmem_get(lanes + buf * C::RB, s[0]);
+        const float* nl = reinterpret_cast<const float*>(smem + C::OFF_LSE) + (g % kLseBufs) * C::RB;
+        const uint32_t* valid = reinterpret_cast<const uint32_t*>(smem + C::OFF_VALID + (g % kLseBufs) * 16);
+        const int t0 = (d.skip + (a.head_chunks == 1 ? j : j / a.head_chunks)) * 2 * a.tokens;
         uint32_t all = valid[0] & valid[1];
         if (C::RB == 128) all &= valid[2] & valid[3];
         const bool plain = __all_sync(0xffffffffu, see0 <= t0 && see1 >= t0 + 2 * a.tokens) && all == 0xffffffffu;
+        const uint64_t by = f32x2(p.scale_log2, p.scale_log2);
 #pragma unroll
-        for (int c = 0; c < C::RB / 32; c++) {
-          uint32_t s[32];
-          tmem_get(lanes + buf * C::RB + 32u * c, s);
+        for (int c = 0; c < kWords; c++) {
+          uint32_t(&x)[32] = s[c & 1];
           tmem_wait_ld();
-          tmem_landed(s);
-          if (c == C::RB / 32 - 1) {  // the buffer may be overwritten now
+          tmem_landed(x);
+          if (c + 1 < kWords) {  // the next word is under way while this one is worked on
+            tmem_get(lanes + buf * C::RB + 32u * (c + 1), s[(c + 1) & 1]);
+          } else {  // the buffer may be overwritten now
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(map_to(smem_u32(&s_free[buf]), 0));
@@ -268,7 +268,6 @@ __global__ void __launch_bounds__(kThreadsM, 1)
           uint32_t bits = 0xffffffffu;
           if (!plain) {
             // columns of this word that see the key: those of the tokens [see0, see1)
-            constexpr int kHalfWords = C::RB / 64;
             const int th = t0 + (c / kHalfWords) * a.tokens, w0 = (c % kHalfWords) * 32;
             const int lo = max(0, min(see0 - th, a.tokens)) * a.heads - w0, hi = max(0, min(see1 - th, a.tokens)) * a.heads - w0;
             const uint32_t from = lo <= 0 ? 0xffffffffu : lo > 31 ? 0u : ~((1u << lo) - 1u);
@@ -278,27 +277,24 @@ __global__ void __launch_bounds__(kThreadsM, 1)
 #pragma unroll
           for (int e = 0; e < 32; e += 4) {
             const float4 z = *reinterpret_cast<const float4*>(nl + 32 * c + e);
-            float w[4];
-            w[0] = fast_exp2(fmaf(__uint_as_float(s[e]), p.scale_log2, z.x));
-            w[1] = fast_exp2(fmaf(__uint_as_float(s[e + 1]), p.scale_log2, z.y));
-            w[2] = fast_exp2(fmaf(__uint_as_float(s[e + 2]), p.scale_log2, z.z));
-            w[3] = fast_exp2(fmaf(__uint_as_float(s[e + 3]), p.scale_log2, z.w));
+            const float2 u = f32x2_parts(fma_f32x2(f32x2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), by, f32x2(z.x, z.y)));
+            const float2 v = f32x2_parts(fma_f32x2(f32x2(__uint_as_float(x[e + 2]), __uint_as_float(x[e + 3])), by, f32x2(z.z, z.w)));
+            float w[4] = {fast_exp2(u.x), fast_exp2(u.y), fast_exp2(v.x), fast_exp2(v.y)};
             if (!plain) {
 #pragma unroll
               for (int k = 0; k < 4; k++)
                 if (!((bits >> (e + k)) & 1u)) w[k] = 0.f;
             }
-            acc[(e >> 1) & 3].x += w[0];
-            acc[(e >> 1) & 3].y += w[1];
-            acc[((e >> 1) + 1) & 3].x += w[2];
-            acc[((e >> 1) + 1) & 3].y += w[3];
+            acc[(e >> 1) & 3] = add_f32x2(acc[(e >> 1) & 3], f32x2(w[0], w[1]));
+            acc[((e >> 1) + 1) & 3] = add_f32x2(acc[((e >> 1) + 1) & 3], f32x2(w[2], w[3]));
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&lse_free[inf]);
+        if (lane == 0) mbar_arrive(&lse_free[g % kLseBufs]);
       }
       if (!ok) break;
-      const float sum = ((acc[0].x + acc[0].y) + (acc[1].x + acc[1].y)) + ((acc[2].x + acc[2].y) + (acc[3].x + acc[3].y));
+      const float2 pair_sum = f32x2_parts(add_f32x2(add_f32x2(acc[0], acc[1]), add_f32x2(acc[2], acc[3])));
+      const float sum = pair_sum.x + pair_sum.y;
       float* meet = sums + (done & 1u) * kCtaKeys + (warp & 3) * 32 + lane;
       if (set == 1) {
         if (done >= 2) ok = warp_wait_own(&sum_free[done & 1u], ((done >> 1) - 1) & 1u, abort_flag, p.err);
@@ -401,7 +397,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
     for (int i = begin; ok && i < end; i++) {
       const Piece d = a.pieces[i];
       for (int j = d.j0; j < d.j1; j++, g++) {
-        const uint32_t inf = g % kInfoM;
+        const uint32_t inf = g % kLseBufs;
         const int tb = j / a.head_chunks, hc = j - tb * a.head_chunks;
         const int t0 = (d.skip + tb) * 2 * a.tokens;
         float z[C::RB / 32];
@@ -415,7 +411,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
           else if (tok < d.T && head < p.group)
             z[c] = p.lse[(size_t)(d.row0 + tok) * p.nqh + (size_t)d.head * p.group + head];
         }
-        if (g >= (uint32_t)kInfoM) ok = warp_wait_own(&lse_free[inf], (g / kInfoM - 1) & 1u, abort_flag, p.err);
+        if (g >= (uint32_t)kLseBufs) ok = warp_wait_own(&lse_free[inf], (g / kLseBufs - 1) & 1u, abort_flag, p.err);
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < C::RB / 32; c++) {
@@ -424,7 +420,7 @@ __global__ void __launch_bounds__(kThreadsM, 1)
           if (lane == 0) reinterpret_cast<uint32_t*>(smem + C::OFF_VALID + inf * 16)[c] = bits;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&lse_full[inf]);
+        if (lane == 0) mbar_arrive(&s_done[g % kScoreBufs]);  // (its last use is over: block g - 3 has been read)
       }
     }
   } else if (warp == kWarpTell) {
