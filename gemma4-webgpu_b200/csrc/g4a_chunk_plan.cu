@@ -65,9 +65,10 @@ __device__ __forceinline__ int find_seq(const int4* seqs, int n, int i, bool ite
 }
 
 // Division of non-negative numbers that are nearly always below 2^32 (the 64-bit one is a long sequence of instructions).
+__device__ __noinline__ long long quot_wide(long long a, long long b) { return a / b; }
 __device__ __forceinline__ long long quot(long long a, long long b) {
   if ((((unsigned long long)a | (unsigned long long)b) >> 32) == 0) return (long long)((uint32_t)a / (uint32_t)b);
-  return a / b;
+  return quot_wide(a, b);
 }
 
 // The pieces of item i of a list that is cut into equal runs: it has n stages, and the list is `length` long, kLead for
@@ -92,8 +93,8 @@ __device__ __forceinline__ void emit_runs(const PlanParams& a, const Seq& s, int
     d.slot = parts == 1 ? -1 : c == 0 ? 2 * w + 1 : 2 * w;
     d.sinks = k.sinks, d.skip = k.window0 - k.sinks, d.pad = 0;
     a.pieces[i + w] = d;
-    if (c > 0 || before < w) a.plan->first[w] = i + w;
-    if (c < parts - 1 || after > w) a.plan->end[w] = i + w + 1;
+    if (c > 0 || before < w) a.plan->pair[w].x = i + w;
+    if (c < parts - 1 || after > w) a.plan->pair[w].y = i + w + 1;
   }
   if (MASS) a.parts[i] = make_int2(w0, parts);
   else if (parts > 1)
@@ -158,11 +159,11 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
   entry_s[tid] = scan(tiles);
   const int entries = warp_sum[32], items = entries * heads;
   if (tid == 0) entry_s[kPlanThreads] = entries;
-  for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
+  for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(0, 0, 1, 0);
   if (MASS && tid <= p.batch) a.seqs[tid] = make_int4(0, (tid < p.batch && tid < kPlanThreads ? entry_s[tid] : entries) * heads, 0, 0);
   __syncthreads();
   if (items == 0 || entries > a.max_entries) {
-    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0;
+    if (tid == 0) a.plan->cuts = 0;
     if (tid == 0 && items != 0) atomicExch(p.err, G4A_DEVERR_TREE);
     if (MASS && tid < p.batch) a.seqs[tid] = make_int4(0, -1, 0, 0);
     return;
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     __syncthreads();
     place_s[tid] = scan(parts > 1 ? tiles * heads * parts : 0);
     stage_s[tid] = pieces0;  // (the stages are not needed any more)
-    if (tid == 0) a.plan->step = a.pairs, a.plan->pieces = pieces;
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(w, pieces, a.pairs, 0);
     __syncthreads();
     if (tid < entries) {
       const int of = (b + 1 < p.batch ? entry_s[b + 1] : entries) - entry_s[b];
@@ -257,7 +258,6 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     }
   } else {
     // ---- runs
-    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0;
     const long long length = stages + (long long)kLead * items;
     const int pairs = (int)min((long long)a.pairs, length);
     if (tid < entries) {
@@ -338,8 +338,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     rows_seen = seen_s;
   }
   if (entries_all > a.max_entries) {  // (the same for all threads)
-    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0, atomicExch(p.err, G4A_DEVERR_TREE);
-    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
+    if (tid == 0) a.plan->cuts = 0, atomicExch(p.err, G4A_DEVERR_TREE);
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(0, 0, 1, 0);
     for (int b = tid; MASS && b < p.batch; b += kPlanThreads) a.seqs[b] = make_int4(0, -1, 0, 0);
     return;
   }
@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
   }
   __syncthreads();
   if (items == 0) {
-    if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = 0;
-    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
+    if (tid == 0) a.plan->cuts = 0;
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(0, 0, 1, 0);
     return;
   }
   // ---- which way: warp k weighs chunks of at most longest / (k + 1) stages
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
       before += (int)all[0];
       slots += all[1];
     }
-    if (tid == 0) a.plan->step = a.pairs, a.plan->pieces = before;
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(w, before, a.pairs, 0);
     __syncthreads();
     for (int i = tid; i < items; i += kPlanThreads) {
       const int b = find_seq(a.seqs, p.batch, i, true);
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
   // ---- runs
   const long long length = stages + (long long)kLead * items;
   const int pairs = (int)min((long long)a.pairs, length);
-  for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->first[w] = a.plan->end[w] = 0;
+  for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(0, 0, 1, 0);
   __syncthreads();
   for (int i = tid; i < items; i += kPlanThreads) {
     const int b = find_seq(a.seqs, p.batch, i, true);
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     emit_runs<MASS>(a, s, b, head, tile, k, i, items, at, n, length, pairs, &cut_count);
   }
   __syncthreads();
-  if (tid == 0) a.plan->step = 1, a.plan->pieces = 0, a.plan->cuts = cut_count;
+  if (tid == 0) a.plan->cuts = cut_count;
 }
 
 }  // namespace

@@ -32,9 +32,8 @@ struct Cut {
 };
 
 struct Plan {
-  int step;            // 1: pair w has the pieces first[w] .. end[w] - 1; else w, w + step, ...
-  int pieces, cuts, pad;
-  int first[kMaxPairs], end[kMaxPairs];
+  int cuts, pad[3];
+  int4 pair[kMaxPairs];  // x, x + z, ... below y: the pieces of each pair
 };
 
 // What the planning kernel reads and writes besides ChunkParams.
@@ -53,14 +52,15 @@ struct PlanParams {
   int2* parts;         // masses: [items] the pair of a tile's first piece, number of its pieces
 };
 
+// (num_tokens * num_q_heads is below 2^31, so rows of a kv head, and of a tile past them, are numbers of 32 bits)
 __device__ __forceinline__ int tiles_of(const ChunkParams& p, const Seq& s) {
-  return (int)(((long long)s.T * p.group + kTileRows - 1) / kTileRows);
+  return (int)(((uint32_t)s.T * (uint32_t)p.group + kTileRows - 1) / kTileRows);
 }
 __device__ __forceinline__ int first_token(const ChunkParams& p, int tile) {
-  return (int)((long long)tile * kTileRows / p.group);
+  return (int)((uint32_t)tile * kTileRows / (uint32_t)p.group);
 }
 __device__ __forceinline__ int last_token(const ChunkParams& p, int T, int tile) {
-  return (int)min((long long)T - 1, ((long long)(tile + 1) * kTileRows - 1) / p.group);
+  return (int)min((uint32_t)T - 1u, ((uint32_t)(tile + 1) * kTileRows - 1u) / (uint32_t)p.group);
 }
 
 // The key blocks that a tile's rows see: [0, sinks) and [window0, window1).

@@ -205,9 +205,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   pdl_launch_dependents();
 
   // this pair's pieces
-  const int pair = (int)(blockIdx.x >> 1), step = a.plan->step;
-  const int begin = step == 1 ? a.plan->first[pair] : pair;
-  const int end = step == 1 ? a.plan->end[pair] : a.plan->pieces;
+  const int4 mine = a.plan->pair[blockIdx.x >> 1];
+  const int begin = mine.x, end = mine.y, step = mine.z;
 
   if (warp < kSoft) {
     // ------------------------------------------------------------------ softmax, epilogue
@@ -235,9 +234,9 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     for (int i = begin; ok && i < end; i += step) {
       const Work<HD> w(p, a.pieces[i]);
       if (w.stages() <= 0) continue;
-      const long long gr = (long long)w.d.tile * kTileRows + row;
-      const bool live = gr < (long long)w.d.T * p.group;
-      const int token = live ? (int)(gr / p.group) : w.d.T - 1;
+      const uint32_t gr = (uint32_t)w.d.tile * kTileRows + (uint32_t)row;
+      const bool live = gr < (uint32_t)w.d.T * (uint32_t)p.group;
+      const int token = live ? (int)(gr / (uint32_t)p.group) : w.d.T - 1;
       const int pos = w.base + token, lo = first_in_window(p, pos);
       float m = kUnseenC, l = 0.f;
       for (int j = w.d.j0; j < w.d.j1; j++, g++) {
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       if (!ok) break;
       const bool bad = tags[done % kBadTags] == (int)done + 1;
       tc_fence_after();
-      const size_t out_row = live ? (size_t)(w.d.row0 + token) * p.nqh + (size_t)w.kvh * p.group + (size_t)(gr - (long long)token * p.group) : 0;
+      const size_t out_row = live ? (size_t)(w.d.row0 + token) * p.nqh + (size_t)(w.kvh * p.group) + (gr - (uint32_t)token * (uint32_t)p.group) : 0;
       const unsigned lives = __ballot_sync(0xffffffffu, live);  // (the first ones)
       float* part = w.d.slot < 0 ? nullptr : a.part + (size_t)w.d.slot * kTileRows * (C::HDV + 2);
       if (part != nullptr) {
@@ -553,14 +552,14 @@ __global__ void __launch_bounds__(kThreadsC, 1)
           if (ok && !C::OWN_STAGING) ok = warp_wait_own(staged, (done - 1) & 1u, abort_flag, p.err);
           if (!ok) break;
         }
-        const long long rows = (long long)w.d.T * p.group;
+        const uint32_t rows = (uint32_t)w.d.T * (uint32_t)p.group;
 #pragma unroll 1
         for (int r = gw; r < kCtaRows; r += 4) {
-          const long long gr = (long long)w.d.tile * kTileRows + rank * kCtaRows + r;
+          const uint32_t gr = (uint32_t)w.d.tile * kTileRows + (uint32_t)(rank * kCtaRows + r);
           const bool live = gr < rows;
-          const int token = live ? (int)(gr / p.group) : 0;
-          const __half* from = p.q + ((size_t)(w.d.row0 + token) * p.nqh + (size_t)w.kvh * p.group +
-                                      (live ? (size_t)(gr - (long long)token * p.group) : 0)) * p.hd;
+          const uint32_t token = live ? gr / (uint32_t)p.group : 0u;
+          const __half* from = p.q + ((size_t)(w.d.row0 + (int)token) * p.nqh + (size_t)(w.kvh * p.group) +
+                                      (live ? gr - token * (uint32_t)p.group : 0u)) * p.hd;
           const uint32_t to = sbase + C::OFF_Q + r * 128;
 #pragma unroll
           for (int e = lane; e < HD / 8; e += 32) {
@@ -657,8 +656,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams
   for (int c = (int)blockIdx.y; c < cuts; c += (int)gridDim.y) {
     const Cut cut = a.cuts[c];
     const int share_log2 = cut.parts <= 4 ? 0 : cut.parts <= 8 ? 1 : cut.parts <= 16 ? 2 : 3;  // warps of a task
-    const long long left = (long long)cut.T * p.group - (long long)cut.tile * kTileRows;
-    const int live = (int)min(left, (long long)kTileRows);
+    const int live = (int)min((uint32_t)cut.T * (uint32_t)p.group - (uint32_t)cut.tile * kTileRows, (uint32_t)kTileRows);
     const int tasks = (live + 7) / 8 * kBlocks, per = 8 >> share_log2;
     for (int t0 = (int)blockIdx.x * per; t0 < tasks; t0 += (int)gridDim.x * per) {
       const int task = t0 + (warp >> share_log2), part0 = warp & ((1 << share_log2) - 1), stride = 1 << share_log2;
@@ -739,9 +737,8 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const TcParams
       if (in && part0 == 0) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int kvh = cut.head / C::HALVES, half = cut.head - kvh * C::HALVES;
-        const long long gr = (long long)cut.tile * kTileRows + row;
-        const int token = (int)(gr / p.group);
-        const size_t to = (size_t)(cut.row0 + token) * p.nqh + (size_t)kvh * p.group + (size_t)(gr - (long long)token * p.group);
+        const uint32_t gr = (uint32_t)cut.tile * kTileRows + (uint32_t)row, token = gr / (uint32_t)p.group;
+        const size_t to = (size_t)(cut.row0 + (int)token) * p.nqh + (size_t)(kvh * p.group) + (gr - token * (uint32_t)p.group);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const int d = half * C::HDV + block * 64 + k * 16 + c4 * 4;

@@ -218,8 +218,8 @@ __global__ void __launch_bounds__(kThreadsM, 1)
   pdl_wait_primary();
   pdl_launch_dependents();
 
-  const int pair = (int)(blockIdx.x >> 1);
-  const int begin = a.plan->first[pair], end = a.plan->end[pair];
+  const int4 mine = a.plan->pair[blockIdx.x >> 1];
+  const int begin = mine.x, end = mine.y;
   bool ok = true;
   uint32_t g = 0, done = 0;  // blocks and pieces so far
 
