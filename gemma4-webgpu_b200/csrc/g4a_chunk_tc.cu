@@ -19,7 +19,7 @@
 //   10    in the pair's first CTA: issues the MMAs of both.  S of stage i + 1 before O of stage i, so that the
 //         softmax of a stage runs under the next stage's scores and the last one's product.
 //   11    tells the first CTA that a K block has landed in this one.
-//   12-15 load the queries, and look through V blocks that not every row sees: a value that is not finite
+//   12-15 load the queries (whole tokens by TMA, else row by row), and look through V blocks that not every row sees: a value that is not finite
 //         becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then they tell the first CTA.
 // Barriers that both CTAs arrive on lie in the first CTA.  Every wait is bounded; a thread that gives up sets the
 // abort flags of both CTAs and the error word, all waits then end at once, and both free their TMEM and leave.
@@ -63,7 +63,7 @@ struct Cc {
   static constexpr int OFF_RED = OFF_OK + 2 * NS * 16;                       // [2][2 halves][128] maxima, sums
   static constexpr int OFF_BAD = OFF_RED + 2 * 2 * kCtaRows * 4;             // [kBadTags] piece + 1 with values taken out
   static constexpr int OFF_BAR = OFF_BAD + kBadTags * 4;
-  static constexpr int NBARS = 6 * NS + 13;
+  static constexpr int NBARS = 6 * NS + 15;
   static constexpr size_t SMEM = (size_t)OFF_BAR + NBARS * 8 + 16;
   static constexpr uint32_t COL_O = 0, COL_S = HDV;  // S[b] at COL_S + KB b, P[b] in its first half
   static constexpr uint32_t TMEM_COLS = 512;
@@ -80,6 +80,7 @@ struct TcParams {
   const Cut* cuts;
   float* part;            // [slots] (o [HDV / 4][256][4] | m [256] | l [256])
   int box_k, box_v;       // rows of a box
+  int q_tokens;           // tokens of a CTA's queries where they are whole tokens (one box for 64 dims); 0: row by row
 };
 
 __device__ __forceinline__ uint32_t half2_bits(float a, float b) {
@@ -138,7 +139,8 @@ __device__ __noinline__ void add_taken_out(const ChunkParams& p, Work<HD> w, int
 
 template <int HD>
 __global__ void __launch_bounds__(kThreadsC, 1)
-    chunk_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TcParams a) {
+    chunk_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                    const __grid_constant__ CUtensorMap tmq, const TcParams a) {
   using C = Cc<HD>;
   const ChunkParams& p = a.c;
   extern __shared__ __align__(1024) unsigned char smem[];  // (at 512 dims there is no room to align it by hand)
@@ -156,10 +158,14 @@ __global__ void __launch_bounds__(kThreadsC, 1)
   uint64_t* q_ready = o_done + C::NS;        // first CTA: queries of both (4 warps of each)
   uint64_t* q_free = q_ready + 1;            // the piece's last scores done (commit)
   uint64_t* o_free = q_free + 1;             // first CTA: epilogue has read O (8 warps of each)
-  uint64_t* looked = o_free + 1;             // the piece's V blocks have been looked through (4 warps of each)
-  uint64_t* staged = looked + 1;             // the epilogue is through with the staging place (8 warps)
+  // [2] the piece's V blocks have been looked through (4 warps of each).  A warp may be through with a piece before
+  // another is with the one before it, so they take turns; it is not two ahead, for the scores of the piece between
+  // need every warp's word on its queries.
+  uint64_t* looked = o_free + 1;
+  uint64_t* staged = looked + 2;             // the epilogue is through with the staging place (8 warps)
   uint64_t* swapped = staged + 1;            // [4] two warps have written what they exchange
   uint64_t* all_done = swapped + 4;
+  uint64_t* q_landed = all_done + 1;         // this CTA's queries (TMA)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::NBARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -179,15 +185,18 @@ __global__ void __launch_bounds__(kThreadsC, 1)
     mbar_init(q_ready, 8);
     mbar_init(q_free, 1);
     mbar_init(o_free, 2 * kSoft);
-    mbar_init(looked, 8);
+    mbar_init(&looked[0], 8);
+    mbar_init(&looked[1], 8);
     mbar_init(staged, kSoft);
     for (int s = 0; s < 4; s++) mbar_init(&swapped[s], 2);
     mbar_init(all_done, 1);
+    mbar_init(q_landed, 1);
     *abort_flag = 0;
     for (int i = 0; i < kBadTags; i++) reinterpret_cast<int*>(smem + C::OFF_BAD)[i] = 0;
     fence_mbar_init();
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmk)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmv)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmq)) : "memory");
   }
   __syncwarp();
   if (warp == kMma) {  // one CTA per SM (shared memory), so the allocation never waits
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       l = half == 0 ? l + other : other + l;
       ok = warp_wait_own(&o_done[(g - 1) % C::NS], ((g - 1) / C::NS) & 1u, abort_flag, p.err);
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, wait_pair(looked, done & 1u, abort_flag, p.err));
+      ok = __all_sync(0xffffffffu, wait_pair(&looked[done & 1u], (done >> 1) & 1u, abort_flag, p.err));
       if (!ok) break;
       const bool bad = tags[done % kBadTags] == (int)done + 1;
       tc_fence_after();
@@ -386,8 +395,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
+        if (!C::OWN_STAGING) mbar_arrive(staged);  // (before o_free, without which no warp gets through another piece)
         arrive_at(o_bar);
-        if (!C::OWN_STAGING) mbar_arrive(staged);
       }
       done++;
     }
@@ -552,25 +561,43 @@ __global__ void __launch_bounds__(kThreadsC, 1)
           if (ok && !C::OWN_STAGING) ok = warp_wait_own(staged, (done - 1) & 1u, abort_flag, p.err);
           if (!ok) break;
         }
-        const uint32_t rows = (uint32_t)w.d.T * (uint32_t)p.group;
-#pragma unroll 1
-        for (int r = gw; r < kCtaRows; r += 4) {
-          const uint32_t gr = (uint32_t)w.d.tile * kTileRows + (uint32_t)(rank * kCtaRows + r);
-          const bool live = gr < rows;
-          const uint32_t token = live ? gr / (uint32_t)p.group : 0u;
-          const __half* from = p.q + ((size_t)(w.d.row0 + (int)token) * p.nqh + (size_t)(w.kvh * p.group) +
-                                      (live ? gr - token * (uint32_t)p.group : 0u)) * p.hd;
-          const uint32_t to = sbase + C::OFF_Q + r * 128;
-#pragma unroll
-          for (int e = lane; e < HD / 8; e += 32) {
-            const bool in = live && e * 8 < p.hd;
-            cp16(to + (e >> 3) * C::Q_CHUNK + (((e & 7) ^ (r & 7)) << 4), in ? from + e * 8 : p.q, in);
+        const uint32_t gr0 = (uint32_t)w.d.tile * kTileRows + (uint32_t)(rank * kCtaRows + gw);
+        if (a.q_tokens > 0) {
+          // (rows past the sequence's last token are another's, or zeros: what comes of them is not stored)
+          if (gw == 0) {
+            if (lane == 0) mbar_arrive_expect_tx(q_landed, (uint32_t)C::Q_BYTES);
+            __syncwarp();
+            const long long token = (long long)w.d.row0 + (long long)(w.d.tile * 2 + rank) * a.q_tokens;
+            if (lane < C::NCQ)
+              load_box(sbase + C::OFF_Q + lane * C::Q_CHUNK, &tmq, 64 * lane, 0, w.kvh, (int)min(token, (long long)p.tokens), q_landed);
+            ok = mbar_wait_bounded(q_landed, done & 1u, p.err, G4A_DEVERR_WAIT_FULL);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
           }
+          if (lane == 0) arrive_at(q_bar);
+        } else {
+          const uint32_t rows = (uint32_t)w.d.T * (uint32_t)p.group, group = (uint32_t)p.group;
+          const uint32_t up = 4u / group, over = 4u - up * group;  // four rows on: tokens, heads
+          uint32_t token = gr0 / group, head = gr0 - token * group;
+#pragma unroll 4
+          for (int r = gw; r < kCtaRows; r += 4) {
+            const bool live = gr0 + (uint32_t)(r - gw) < rows;
+            const __half* from = p.q + ((size_t)(w.d.row0 + (int)token) * p.nqh + (size_t)(w.kvh * p.group) + head) * p.hd;
+            const uint32_t to = sbase + C::OFF_Q + r * 128;
+#pragma unroll
+            for (int e = lane; e < HD / 8; e += 32) {
+              const bool in = live && e * 8 < p.hd;
+              cp16(to + (e >> 3) * C::Q_CHUNK + (((e & 7) ^ (r & 7)) << 4), in ? from + e * 8 : p.q, in);
+            }
+            token += up;
+            head += over;
+            if (head >= group) head -= group, token++;
+          }
+          cp_wait_all();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) publish_at(q_bar);
         }
-        cp_wait_all();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) publish_at(q_bar);
         const int lo = first_in_window(p, w.base + w.first), hi = w.base + w.last + 1;
         bool found = false;
         for (int j = w.d.j0; j < w.d.j1; j++, g++) {
@@ -616,7 +643,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
           if (found)
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(tags + (done % kBadTags) * 4, c)), "r"(done + 1) : "memory");
           __syncwarp();
-          if (lane == 0) publish_at(map_to(smem_u32(looked), c));
+          if (lane == 0) publish_at(map_to(smem_u32(&looked[done & 1u]), c));
         }
         done++;
       }
@@ -770,9 +797,11 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   const int unit = p.page_size & -p.page_size;
   a.box_k = std::min(unit, C::KB / 2);
   a.box_v = std::min(unit, C::KB);
-  CUtensorMap mk, mv;
+  CUtensorMap mk, mv, mq;
   if (g4a_status s = g4a_page_map(fn, ctx, &mk, p, p.k, a.box_k)) return s;
   if (g4a_status s = g4a_page_map(fn, ctx, &mv, p, p.v, a.box_v)) return s;
+  a.q_tokens = kCtaRows % p.group == 0 ? kCtaRows / p.group : 0;
+  if (g4a_status s = g4a_query_map(fn, ctx, &mq, p, a.q_tokens > 0 ? p.group : 1, std::max(a.q_tokens, 1))) return s;
   const int pairs = std::min(ctx->num_sms / 2, kMaxPairs);
   const long long entries = (long long)p.tokens * p.group / kTileRows + std::min(p.batch, p.tokens);
   const long long items = entries * p.nkh * C::HALVES;
@@ -819,7 +848,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, chunk_tc_kernel<HD>, mk, mv, a);
+  e = cudaLaunchKernelEx(&cfg, chunk_tc_kernel<HD>, mk, mv, mq, a);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_tc_kernel");
   e = g4a_launch(chunk_join_kernel<HD>, dim3(kJoinX, kJoinY), dim3(kJoinThreads), 0, ctx->stream, true, a);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_join_kernel");
