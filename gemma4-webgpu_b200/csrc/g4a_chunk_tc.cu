@@ -606,44 +606,47 @@ __global__ void __launch_bounds__(kThreadsC, 1)
           if (!ok) break;
           const int k0 = w.key0(j);
           const bool clean = w.clean(p, k0);
+          bool changed = false;
           if (!clean) {
             unsigned char* v = smem + C::OFF_V + s * C::V_BYTES;
 #pragma unroll 4
             for (int e = gw * 32 + lane; e < C::V_BYTES / 16; e += 128) {
               uint4 x = *reinterpret_cast<const uint4*>(v + e * 16);
-              const uint32_t was[4] = {x.x, x.y, x.z, x.w};
-              uint32_t now[4];
-              bool changed = false;
-#pragma unroll
-              for (int k = 0; k < 4; k++) {
-                now[k] = was[k];
-                if ((now[k] & 0x7c00u) == 0x7c00u) now[k] &= 0xffff0000u;
-                if ((now[k] & 0x7c000000u) == 0x7c000000u) now[k] &= 0x0000ffffu;
-                changed |= now[k] != was[k];
-              }
-              if (changed) {
-                *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(now[0], now[1], now[2], now[3]);
+              // an exponent of all ones and one more carry into a half's top bit
+              constexpr uint32_t kExp = 0x7c007c00u, kOne = 0x04000400u, kTop = 0x80008000u;
+              if ((((x.x & kExp) + kOne) | ((x.y & kExp) + kOne) | ((x.z & kExp) + kOne) | ((x.w & kExp) + kOne)) & kTop) {
+                auto finite = [](uint32_t w) {
+                  const uint32_t top = ((w & kExp) + kOne) & kTop;
+                  return w & ~((top >> 15) * 0xffffu);
+                };
+                *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(finite(x.x), finite(x.y), finite(x.z), finite(x.w));
+                changed = true;
                 const int key = k0 + (e >> 3) % C::KB;  // 8 pieces of 16 bytes to a row, KB rows to a chunk
                 found |= key < hi && (key >= lo || (uint32_t)key < p.sinks);
               }
             }
-            fence_proxy_async_smem();
+            if (changed) fence_proxy_async_smem();
           }
-          __syncwarp();
+          changed = __any_sync(0xffffffffu, changed);
           if (lane == 0) {
             const uint32_t to = map_to(smem_u32(&p_ready[s]), 0);
-            if (clean) arrive_at(to);
-            else publish_at(to);
+            if (changed) publish_at(to);
+            else arrive_at(to);
           }
         }
         if (!ok) break;
+        const bool any = __any_sync(0xffffffffu, found);
         // (a CTA has half of the dims and half of the rows, so both have to know)
 #pragma unroll
         for (uint32_t c = 0; c < 2; c++) {
           if (found)
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to(tags + (done % kBadTags) * 4, c)), "r"(done + 1) : "memory");
           __syncwarp();
-          if (lane == 0) publish_at(map_to(smem_u32(&looked[done & 1u]), c));
+          if (lane == 0) {
+            const uint32_t to = map_to(smem_u32(&looked[done & 1u]), c);
+            if (any) publish_at(to);
+            else arrive_at(to);
+          }
         }
         done++;
       }
