@@ -12,8 +12,8 @@ using namespace g4a;
 constexpr int kThreadsE = 1024;      // of a selecting CTA
 constexpr int kBinsE = 2048;
 constexpr int kCacheE = 40 * 1024;   // weights that a CTA keeps in shared memory
-constexpr int kMaxCluster = 8;
-constexpr int kMoveThreads = 256, kMoveFly = 4;
+constexpr int kMaxCluster = 16;
+constexpr int kRowsLog2 = 5, kRows = 1 << kRowsLog2;  // rows of a block that is moved at once, one to a lane
 
 struct EvictParams {
   __half *k, *v;
@@ -23,10 +23,9 @@ struct EvictParams {
   int batch, budget, sinks, recent, page_size, max_pages, num_pages, nkh, hd;
   int *new_lens, *kept;
   int cap;        // rows that a sequence can have
-  int rows;       // rows of a block that is moved at once
-  int blocks;     // of them in a budget
+  int blocks;     // of kRows rows in a budget
   int* idx;       // [batch, nkh, budget] old numbers of the kept rows
-  int* rank;      // [batch, nkh, blocks + 1] kept rows before row `rows` * block
+  int* rank;      // [batch, nkh, blocks + 1] kept rows before row kRows * block
   int* read;      // [batch, nkh, blocks] 1: the block's rows have been read
   int* ticket;
   int* err;
@@ -58,7 +57,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_meet() {
+__device__ __forceinline__ void cluster_meet(uint32_t ctas) {
+  if (ctas == 1) {  // (a meeting of the cluster takes 0.5 us)
+    __syncthreads();
+    return;
+  }
   asm volatile(
       "barrier.cluster.arrive.release.aligned;\n\t"
       "barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -75,10 +78,11 @@ __device__ __forceinline__ int peek(const int* at, uint32_t rank) {
 // One cluster of CTAs per (sequence, kv head), each with a slice of the rows between the first and the last ones, in
 // order.  The border weight is found digit by digit (11, 11 and 10 bits from the top): every CTA counts its slice,
 // all read each other's counts through distributed shared memory.  Then a warp knows how many rows before its own are
-// kept, and writes the numbers of its kept rows in order.  Latency: three counts and four meetings of the cluster.
+// kept, and writes the numbers of its kept rows in order.  Latency: three counts, seven meetings
+// of the cluster, and two more ways through the slice.
 __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictParams p) {
   extern __shared__ uint32_t cache[];
-  __shared__ int hist[3][kBinsE], warp_sum[32], warp_gt[32], warp_tie[32], slice_gt, slice_tie, digit_s, need_s;
+  __shared__ int hist[3][kBinsE], sums[2][kBinsE], warp_sum[32], warp_gt[32], warp_tie[32], slice_gt, slice_tie, digit_s, need_s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), ctas = cluster_size();
   const int item = (int)(blockIdx.x / ctas), b = item / p.nkh, kvh = item % p.nkh;
@@ -106,7 +110,10 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
   const int per_warp = ((middle + (int)ctas * 32 - 1) / ((int)ctas * 32) + 31) & ~31, slice = per_warp * 32;
   const int at0 = first + (int)rank * slice, count = max(0, min(slice, end - at0));
   const bool cached = count <= kCacheE;
-  for (int i = tid; i < count && cached; i += kThreadsE) cache[i] = order_of(mass[at0 + i]);
+  if (cached) {
+#pragma unroll 4
+    for (int i = tid; i < count; i += kThreadsE) cache[i] = order_of(mass[at0 + i]);
+  }
   auto key_of = [&](int i) { return cached ? cache[i] : order_of(mass[at0 + i]); };
   for (int i = tid; i < 3 * kBinsE; i += kThreadsE) hist[0][i] = 0;
   __syncthreads();
@@ -120,14 +127,25 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
       const uint32_t o = key_of(i);
       if ((o & mask) == border) atomicAdd(&h[(o >> shift) & (bins - 1)], 1);
     }
-    cluster_meet();
+    cluster_meet(ctas);
+    // every CTA adds up its share of the bins over the cluster, and then all read the sums (every CTA reading all counts
+    // took 5.5 us of a pass)
+    const int share = (bins + (int)ctas - 1) / (int)ctas, bin0 = (int)rank * share;
+    if (ctas > 1) {
+      for (int i = tid; i < share && bin0 + i < bins; i += kThreadsE) {
+        int x = 0;
+#pragma unroll 8
+        for (uint32_t r = 0; r < ctas; r++) x += peek(&h[bin0 + i], r);
+        sums[pass & 1][i] = x;  // (read by the others before they come to the next pass's first meeting)
+      }
+      cluster_meet(ctas);
+    }
     // bins from the top, two to a thread: the one in which the number of larger ones reaches `need`
     int c[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const int bin = kBinsE - 1 - (2 * tid + e);
-      if (bin < bins)
-        for (uint32_t r = 0; r < ctas; r++) c[e] += peek(&h[bin], r);
+      if (bin < bins) c[e] = ctas == 1 ? h[bin] : peek(&sums[pass & 1][bin % share], (uint32_t)(bin / share));
     }
     int incl = c[0] + c[1];
 #pragma unroll
@@ -137,8 +155,7 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
     }
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
-    int before = incl - c[0] - c[1];
-    for (int w = 0; w < warp; w++) before += warp_sum[w];
+    int before = incl - c[0] - c[1] + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       if (c[e] > 0 && before < need && before + c[e] >= need) digit_s = kBinsE - 1 - (2 * tid + e), need_s = need - before;
@@ -166,17 +183,14 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
     const int g = __reduce_add_sync(0xffffffffu, warp_gt[lane]), t = __reduce_add_sync(0xffffffffu, warp_tie[lane]);
     if (lane == 0) slice_gt = g, slice_tie = t;
   }
-  cluster_meet();
-  int ties = 0, at = first;  // before this warp
-  for (uint32_t r = 0; r < rank; r++) {
-    const int t = peek(&slice_tie, r);
-    at += peek(&slice_gt, r) + max(0, min(t, need - ties));
-    ties += t;
-  }
-  for (int w = 0; w < warp; w++) {
-    at += warp_gt[w] + max(0, min(warp_tie[w], need - ties));
-    ties += warp_tie[w];
-  }
+  cluster_meet(ctas);
+  // before this warp: larger ones, and ties (the first `need` of all stay)
+  int larger = 0, ties = 0;
+  if (lane < (int)rank) larger = peek(&slice_gt, (uint32_t)lane), ties = peek(&slice_tie, (uint32_t)lane);
+  if (lane < warp) larger += warp_gt[lane], ties += warp_tie[lane];
+  larger = __reduce_add_sync(0xffffffffu, larger);
+  ties = __reduce_add_sync(0xffffffffu, ties);
+  int at = first + larger + min(ties, need);
   for (int i = w0; i < w1; i += 32) {
     const int row = at0 + i + lane;
     const bool in = i + lane < w1 && want > 0;
@@ -189,7 +203,7 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
       idx[j] = row;
       if (kept) kept[j] = row;
     }
-    if (i + lane < w1 && row <= p.blocks * p.rows && row % p.rows == 0) ranks[row / p.rows] = j;
+    if (i + lane < w1 && (row & (kRows - 1)) == 0 && row >> kRowsLog2 <= p.blocks) ranks[row >> kRowsLog2] = j;
     at += __popc(kb);
     ties += __popc(tb);
   }
@@ -198,82 +212,98 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
     const int row = i < first ? i : end + (i - first), j = i < first ? i : budget - p.recent + (i - first);
     idx[j] = row;
     if (kept) kept[j] = row;
-    if (row <= p.blocks * p.rows && row % p.rows == 0) ranks[row / p.rows] = j;
+    if ((row & (kRows - 1)) == 0 && row >> kRowsLog2 <= p.blocks) ranks[row >> kRowsLog2] = j;
   }
-  cluster_meet();  // nobody reads this CTA's counts any more
+  cluster_meet(ctas);  // nobody reads this CTA's counts any more
 }
 
-// Moves the rows.  Row j comes from row idx[j] >= j, and a block of rows may be written once every row that comes from its place
-// has been read; those belong to this block and two before it at most.  So a block is read into registers, says so, waits
-// for the blocks before it whose rows come from its place, and is written: each byte moves once, all SMs at work.
-// Blocks are taken by ticket, in order, and a block reads before it waits, so those that it waits for always get on; the
-// wait is bounded all the same (a block that gives up writes nothing and reports it).
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictParams p) {
-  __shared__ int ticket_s, ok_s;
-  const int tid = threadIdx.x;
+// Moves the rows.  Row j comes from row idx[j] >= j, and a block of rows may be written once every row that comes from its
+// place has been read; those belong to this block and two before it at most.  So a block is read into shared memory, says
+// so, waits for the blocks before it whose rows come from its place, and is written: each byte moves once, all SMs at
+// work.  Blocks are taken by ticket, in order, and a block reads before it waits, so those that it waits for always get
+// on; the wait is bounded all the same (a block that gives up writes nothing and reports it).  A block is one warp, a lane
+// a row, and the copies are bulk ones, so an SM holds 200 KB of rows under way with next to no instructions (256 threads
+// with the rows in registers, 128 KB to an SM: 24 and 112 us instead of 22 and 76, with a cold L2, for 131,000 rows to 16,384 and for
+// 24 sequences x 4 heads).
+__global__ void __launch_bounds__(kRows) evict_move_kernel(const EvictParams p) {
+  extern __shared__ __align__(128) unsigned char rows_s[];  // [2][32][hd] f16
+  __shared__ uint64_t landed;
+  const int lane = threadIdx.x;
   pdl_wait_primary();
   pdl_launch_dependents();
-  if (tid == 0) ticket_s = atomicAdd(p.ticket, 1), ok_s = 1;
-  __syncthreads();
-  const int item = ticket_s / p.blocks, block = ticket_s % p.blocks, b = item / p.nkh, kvh = item % p.nkh;
+  int ticket = 0;
+  if (lane == 0) {
+    ticket = atomicAdd(p.ticket, 1);
+    mbar_init(&landed, 1);
+    fence_mbar_init();
+  }
+  ticket = __shfl_sync(0xffffffffu, ticket, 0);
+  const int item = ticket / p.blocks, block = ticket - item * p.blocks, b = item / p.nkh, kvh = item - b * p.nkh;
   const int n = p.kv_lens[b];
   if (n <= p.budget || n > p.cap) return;
   const int* idx = p.idx + (size_t)item * p.budget;
-  const int j0 = block * p.rows, j1 = min(p.budget, j0 + p.rows);
-  if (idx[j1 - 1] == j1 - 1) return;  // all of them are where they were, and nobody waits for them
+  const int j0 = block << kRowsLog2, j1 = min(p.budget, j0 + kRows), j = j0 + lane;
+  const int from = j < j1 ? idx[j] : j;
+  // (the last of them where it was: all are, and nobody waits for them)
+  if (__shfl_sync(0xffffffffu, from, j1 - 1 - j0) == j1 - 1) return;
   // the rows whose places lie in this block's come from rows [rank of its begin, rank of its end)
   const int* ranks = p.rank + (size_t)item * (p.blocks + 1);
-  const int last = (block + 1) * p.rows < n ? ranks[block + 1] : p.budget;
-  const int wait0 = ranks[block] / p.rows, wait1 = min(block, (last - 1) / p.rows + 1);
+  const int last = (block + 1) << kRowsLog2 < n ? ranks[block + 1] : p.budget;
+  const int wait0 = ranks[block] >> kRowsLog2, wait1 = min(block, ((last - 1) >> kRowsLog2) + 1);
   int* read = p.read + (size_t)item * p.blocks;
   float* mass = p.mass + (size_t)item * p.mass_stride;
-  const int per = p.hd / 8;
-  uint4 xk[kMoveFly], xv[kMoveFly];
-  long long dst[kMoveFly];
+  const uint32_t bytes = (uint32_t)p.hd * 2u, mine = smem_u32(rows_s) + (uint32_t)lane * bytes, of_v = kRows * bytes;
+  const bool moves = j < j1 && from != j;
+  long long src = -1, dst = -1;
   float w = 0.f;
-  int from = -1;
-#pragma unroll
-  for (int u = 0; u < kMoveFly; u++) {
-    const int c = tid + u * kMoveThreads, r = c / per, col = c - r * per, j = j0 + r;
-    dst[u] = -1;
-    if (r >= p.rows || j >= j1) continue;
-    const int i = idx[j];
-    if (i == j) continue;
-    const long long src = row_at(p, b, kvh, i), to = row_at(p, b, kvh, j);
-    if (src < 0 || to < 0) continue;
-    dst[u] = to + col * 8;
-    xk[u] = *reinterpret_cast<const uint4*>(p.k + src + col * 8);
-    xv[u] = *reinterpret_cast<const uint4*>(p.v + src + col * 8);
-  }
-  if (j0 + tid < j1) {
-    from = idx[j0 + tid];
+  if (moves) {
     w = mass[from];
+    src = row_at(p, b, kvh, from);
+    dst = row_at(p, b, kvh, j);
   }
-  __threadfence();  // each thread's reads are done
-  __syncthreads();
-  if (tid == 0) asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(read + block), "r"(1) : "memory");
-  if (wait0 + tid < wait1) {
-    const uint64_t t0 = globaltimer_ns();
-    int done = 0;
-    while (true) {
-      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(read + wait0 + tid) : "memory");
+  const bool copies = src >= 0 && dst >= 0;
+  const int copied = __popc(__ballot_sync(0xffffffffu, copies));
+  if (lane == 0) mbar_arrive_expect_tx(&landed, 2u * bytes * (uint32_t)copied);
+  __syncwarp();
+  if (copies) {
+    const uint32_t bar = smem_u32(&landed);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(mine),
+                 "l"(p.k + src), "r"(bytes), "r"(bar)
+                 : "memory");
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(mine + of_v),
+                 "l"(p.v + src), "r"(bytes), "r"(bar)
+                 : "memory");
+  }
+  bool ok = mbar_wait_bounded(&landed, 0, p.err, G4A_DEVERR_WAIT_FULL);
+  __threadfence();  // the weights have been read too
+  ok = __all_sync(0xffffffffu, ok);
+  if (lane == 0 && ok) asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(read + block), "r"(1) : "memory");
+  if (ok && wait0 + lane < wait1) {
+    uint64_t t0 = 0;
+    for (uint32_t spins = 1;; spins++) {
+      int done;
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(done) : "l"(read + wait0 + lane) : "memory");
       if (done) break;
-      if (globaltimer_ns() - t0 > 2000000000ull) {
-        ok_s = 0;
+      if ((spins & 63u) != 0u) continue;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) {
+        t0 = now;
+      } else if (now - t0 > 2000000000ull) {
+        ok = false;
         atomicExch(p.err, G4A_DEVERR_WAIT_FULL);
         break;
       }
     }
   }
-  __syncthreads();
-  if (!ok_s) return;
-#pragma unroll
-  for (int u = 0; u < kMoveFly; u++) {
-    if (dst[u] < 0) continue;
-    *reinterpret_cast<uint4*>(p.k + dst[u]) = xk[u];
-    *reinterpret_cast<uint4*>(p.v + dst[u]) = xv[u];
+  if (!__all_sync(0xffffffffu, ok)) return;
+  if (copies) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.k + dst), "r"(mine), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.v + dst), "r"(mine + of_v), "r"(bytes)
+                 : "memory");
   }
-  if (from >= 0) mass[j0 + tid] = w;
+  if (moves) mass[j] = w;
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 }  // namespace
@@ -332,9 +362,8 @@ extern "C" g4a_status g4a_paged_kv_evict(g4a_ctx* ctx, uint16_t* k_pages, uint16
   const uint64_t cap = std::min<uint64_t>((uint64_t)page_size * max_pages_per_seq, mass_stride);
   const long long items = (long long)batch * num_kv_heads;
   p.cap = (int)cap;
-  p.rows = std::min(kMoveThreads, kMoveThreads * kMoveFly / (p.hd / 8));
   const bool any = budget < cap;  // whether a sequence can have more rows than the budget
-  p.blocks = any ? (p.budget + p.rows - 1) / p.rows : 1;
+  p.blocks = any ? (int)(((long long)p.budget + kRows - 1) >> kRowsLog2) : 1;
   if (any && items * (p.blocks + 1ll) > 0x7fffffffll) return g4a_fail(G4A_EINVAL, "%s: batch * num_kv_heads * budget too large", fn);
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   const size_t n_idx = any ? up((size_t)items * budget * sizeof(int)) : 0, n_block = any ? up((size_t)items * (p.blocks + 1) * sizeof(int)) : 0;
@@ -347,8 +376,11 @@ extern "C" g4a_status g4a_paged_kv_evict(g4a_ctx* ctx, uint16_t* k_pages, uint16
   static std::atomic<bool> ready[64];
   const size_t smem = kCacheE * sizeof(uint32_t);
   if (ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(evict_select_kernel)");
+    cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)  // 64 KB: 32 rows of 512 dims, K and V
+      e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kRows * 512 * 2);
+    if (e != cudaSuccess) return g4a_cuda_fail(e, "cudaFuncSetAttribute(evict kernels)");
     if (ctx->device < 64) ready[ctx->device].store(true, std::memory_order_release);
   }
   // CTAs of a cluster: slices of some 4,096 rows, as far as there are SMs
@@ -373,7 +405,8 @@ extern "C" g4a_status g4a_paged_kv_evict(g4a_ctx* ctx, uint16_t* k_pages, uint16
   cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch evict_select_kernel");
   if (any) {
-    e = g4a_launch(evict_move_kernel, dim3((unsigned)(items * p.blocks)), dim3(kMoveThreads), 0, ctx->stream, true, p);
+    e = g4a_launch(evict_move_kernel, dim3((unsigned)(items * p.blocks)), dim3(kRows), (size_t)2 * kRows * p.hd * 2, ctx->stream,
+                   true, p);
     if (e != cudaSuccess) return g4a_cuda_fail(e, "launch evict_move_kernel");
   }
   return G4A_OK;
