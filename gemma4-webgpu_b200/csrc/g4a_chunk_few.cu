@@ -11,8 +11,8 @@
 //                               leaves in a lane (row g, keys 2 t, 2 t + 1) is the operand that the second one wants.
 // A warp has 16 KB under way (K and V of 16 keys, 256 dims), an SM 128 KB, more than the HBM's latency needs.  Heads of
 // more than 256 dims: two warps share 16 keys, half of the dims each, and add up their halves of the scores.
-// A sequence's keys are split over CTAs in equal parts; the warps of a CTA meet in shared memory, the parts of a row
-// tile in a second kernel.  Softmax as in the tcgen05 kernel: m follows the maximum lazily, p rounded to f16 for the
+// The sequences' keys are dealt to the CTAs in equal parts, as many CTAs as the SMs hold at once; the warps of a CTA meet in
+// shared memory, the parts of a row tile in a second kernel.  Softmax as in the tcgen05 kernel: m follows the maximum lazily, p rounded to f16 for the
 // product with V and summed unrounded.
 #include <float.h>
 
@@ -28,12 +28,12 @@ using namespace g4a_chunk;
 
 constexpr int kWarps = 4, kStepKeys = 16, kTile = 8;  // warps of a CTA; keys of a step; query rows of a tile
 constexpr int kNoKey = -1 - 0x7fffffff;
-constexpr long long kRounds = 3;  // of CTAs to the SMs' room (1: 135 us for 64 decode sequences, 2 to 4: 117, 6: 123)
 constexpr float kRaiseF = 15.0f, kFirstF = -3.0f, kLaterF = 5.0f, kUnseenF = -FLT_MAX;
 
 struct FewParams {
   ChunkParams c;
   int splits;   // CTAs of a sequence and kv head, at most
+  int ctas;     // CTAs to be dealt out; 0 (more sequences than threads): every sequence has `splits` of them
   float* part;  // [row tiles][nkh][splits] (o [8][hd] | m [8] | l [8])
 };
 
@@ -42,7 +42,7 @@ struct Steps {
   int sinks, w0, w1, parts;
   __device__ __forceinline__ int count() const { return sinks + w1 - w0; }
 };
-__device__ __forceinline__ Steps steps_of(const FewParams& a, const Seq& s, int tile, int groups) {
+__device__ __forceinline__ Steps steps_of(const FewParams& a, const Seq& s, int tile, int groups, int parts) {
   const ChunkParams& p = a.c;
   const int t0 = (int)((uint32_t)(tile * kTile) / (uint32_t)p.group);
   const int t1 = min(s.T - 1, (int)((uint32_t)(tile * kTile + kTile - 1) / (uint32_t)p.group));
@@ -52,8 +52,55 @@ __device__ __forceinline__ Steps steps_of(const FewParams& a, const Seq& s, int 
   r.w1 = (hi + kStepKeys - 1) / kStepKeys;
   r.sinks = (int)((min((long long)p.sinks, (long long)lo) + kStepKeys - 1) / kStepKeys);
   if (r.sinks >= r.w0) r.sinks = r.w0 = 0;
-  r.parts = min(a.splits, (r.count() + groups - 1) / groups);  // a step for each of a CTA's groups at least
+  r.parts = min(parts, (r.count() + groups - 1) / groups);  // a step for each of a CTA's groups at least
   return r;
+}
+// What CTA c does: sequence b, its parts, and kv head and part (kvh * parts + part) in `local`; b < 0: nothing.  A
+// sequence of n steps of 16 keys has n / q parts, rounded up, with the smallest q that lets all have a CTA; a thread
+// finds that for one sequence.  `own` >= 0 asks for that sequence's parts instead.
+struct Deal {
+  int b, parts, local;
+};
+template <int THREADS>
+__device__ __forceinline__ Deal deal_out(const FewParams& a, int c, int own, int groups) {
+  __shared__ int sums[THREADS / 32], counts[THREADS / 32];
+  __shared__ Deal found;
+  const ChunkParams& p = a.c;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int n = 0;
+  if (tid < p.batch) {
+    const Seq s = seq_of(p, tid, (long long)p.max_pages * p.page_size);
+    if (s.T > 0) {
+      const int lo = first_in_window(p, s.base());
+      n = (int)((min((long long)p.sinks, (long long)lo) + kStepKeys - 1) / kStepKeys) + (s.L + kStepKeys - 1) / kStepKeys - lo / kStepKeys;
+    }
+  }
+  const int total = __reduce_add_sync(0xffffffffu, n), heads = __reduce_add_sync(0xffffffffu, n > 0 ? p.nkh : 0);
+  if (lane == 0) sums[warp] = total, counts[warp] = heads;
+  if (tid == 0) found.b = -1;
+  __syncthreads();
+  long long all = 0;
+  int items = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; i++) all += sums[i], items += counts[i];
+  const long long q = max((all * p.nkh + (a.ctas - items) - 1) / (long long)(a.ctas - items), (long long)groups);
+  const int parts = n > 0 ? min((int)((n + q - 1) / q), a.splits) : 0;
+  int incl = parts * p.nkh;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; i++)
+    if (i < warp) incl += sums[i];
+  const int begin = incl - parts * p.nkh;
+  if (own >= 0 ? tid == own : c >= begin && c < incl) found = Deal{tid, parts, c - begin};
+  __syncthreads();
+  return found;
 }
 // Place of a row tile among all of the call's (a sequence has T group / 8 + 1 at most).
 __device__ __forceinline__ size_t tile_place(const ChunkParams& p, const Seq& s, int b, int tile) {
@@ -84,15 +131,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) chunk_few_kernel(const FewPara
   extern __shared__ __align__(16) float o_s[];  // [warps][8 rows][PITCH]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int share = warp % SHARE, group = warp / SHARE;
-  const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
+  int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh), split = (int)blockIdx.x, most = a.splits;
   pdl_wait_primary();
   pdl_launch_dependents();
+  if (a.ctas > 0) {
+    const Deal d = deal_out<kWarps * 32>(a, (int)blockIdx.x, -1, GROUPS);
+    if (d.b < 0) return;
+    b = d.b, kvh = d.local / d.parts, split = d.local - kvh * d.parts, most = d.parts;
+  }
   const Seq s = seq_of(p, b, (long long)p.max_pages * p.page_size);
   const int base = s.base(), rows = s.T * p.group, d_warp = share * DIMS;
   const int* table = p.page_table + (size_t)b * p.max_pages;
   for (int tile = 0; tile * kTile < rows; tile++) {
-    const Steps st = steps_of(a, s, tile, GROUPS);
-    const int split = (int)blockIdx.x;
+    const Steps st = steps_of(a, s, tile, GROUPS, most);
     if (split >= st.parts) continue;
     const int n = st.count(), i0 = (int)((long long)n * split / st.parts), i1 = (int)((long long)n * (split + 1) / st.parts);
     // row g of the tile (rows that are not there: the last token's sight, no weight in anything that is kept)
@@ -327,10 +378,11 @@ __global__ void __launch_bounds__(256) chunk_few_join_kernel(const FewParams a, 
   const int c = threadIdx.x & 7, row = (threadIdx.x >> 3) & 7, lanes = threadIdx.x >> 6, d = (int)blockIdx.x * 32 + c * 4;
   pdl_wait_primary();
   pdl_launch_dependents();
+  const int most = a.ctas > 0 ? deal_out<256>(a, 0, b, groups).parts : a.splits;
   const Seq s = seq_of(p, b, (long long)p.max_pages * p.page_size);
   const int rows = s.T * p.group;
   for (int tile = 0; tile * kTile < rows; tile++) {
-    const int parts = steps_of(a, s, tile, groups).parts;
+    const int parts = steps_of(a, s, tile, groups, most).parts;
     if (parts == 1) continue;
     const size_t pitch = (size_t)kTile * (p.hd + 2);
     const float* part = a.part + (tile_place(p, s, b, tile) * p.nkh + kvh) * a.splits * pitch;
@@ -412,18 +464,25 @@ g4a_status launch(g4a_ctx* ctx, const ChunkParams& p) {
   FewParams a = {};
   a.c = p;
   const long long heads = (long long)p.batch * p.nkh;
-  // rows that a sequence can read, in CTAs with a step for every group; as many CTAs as make some rounds of the SMs
+  // rows that a sequence can read, in CTAs with a step for every group
   const uint64_t cap = (uint64_t)p.page_size * p.max_pages;
   uint64_t keys = cap;
   if (p.window != 0u) keys = std::min<uint64_t>(cap, (uint64_t)p.window + p.sinks + 4 * kStepKeys);
-  a.splits = (int)std::max<long long>(
-      1, std::min<long long>((long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys)), (kRounds * 2ll * ctx->num_sms + heads - 1) / heads));
+  const long long most = (long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys));
+  // two CTAs to an SM, one round of them; a sequence has four times its share at most
+  const long long ctas = std::max(2ll * ctx->num_sms, 2 * heads);
+  if (p.batch <= kWarps * 32) {
+    a.ctas = (int)std::min(ctas, heads * most + heads);
+    a.splits = (int)std::min(most, 4 * ((ctas + heads - 1) / heads));
+  } else {
+    a.splits = (int)std::max<long long>(1, std::min(most, (3 * ctas + heads - 1) / heads));
+  }
   const size_t tiles = (size_t)((long long)p.tokens * p.group / kTile) + (size_t)p.batch;
   const size_t need = tiles * p.nkh * a.splits * kTile * (p.hd + 2) * sizeof(float);
   if (g4a_status s = g4a_ensure_workspace(ctx, need)) return s;
   a.part = static_cast<float*>(ctx->workspace);
   g4a_prof_scope ps(ctx, G4A_PROF_CHUNK_ATTN);
-  cudaError_t e = g4a_launch(chunk_few_kernel<SEG, SHARE>, dim3((unsigned)a.splits, (unsigned)heads), dim3(kWarps * 32), smem,
+  cudaError_t e = g4a_launch(chunk_few_kernel<SEG, SHARE>, a.ctas > 0 ? dim3((unsigned)a.ctas) : dim3((unsigned)a.splits, (unsigned)heads), dim3(kWarps * 32), smem,
                              ctx->stream, true, a);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch chunk_few_kernel");
   if (a.splits > 1) {
