@@ -71,34 +71,62 @@ __device__ __forceinline__ long long quot(long long a, long long b) {
   return quot_wide(a, b);
 }
 
-// The pieces of item i of a list that is cut into equal runs: it has n stages, and the list is `length` long, kLead for
-// each item in front of its stages; this one begins at `at`.  Run w is [w length / pairs, (w + 1) length / pairs).  A
-// piece of pair w lies at i + w in the list of pieces, so a pair's lie together (with holes between the pairs).  A pair
-// has at most one piece that goes on from the pair before (its result in place 2 w) and one that the next goes on with
-// (2 w + 1).
+// An item of a list that is cut into equal runs: it has n stages, kLead in front of them, and begins at `at`.
+struct Item {
+  int i, b, head, tile;
+  Seq s;
+  Blocks k;
+  long long at, n;
+};
+// Run w is [w length / pairs, (w + 1) length / pairs) of the list.  A piece of pair w of item i lies at i + w in the list
+// of pieces, so a pair's lie together (with holes between the pairs).  A pair has at most one piece that goes on from the
+// pair before (its result in place 2 w) and one that the next goes on with (2 w + 1).  A thread for each item writes its
+// first piece, a thread for each pair the one that goes on: one thread for all pieces of an item took 0.4 us for each.
+struct Runs {
+  long long length;
+  int pairs, items;
+  __device__ __forceinline__ long long begin(int w) const { return quot((long long)w * length, pairs); }
+  __device__ __forceinline__ int owner(long long x) const { return (int)quot((x + 1) * pairs - 1, length); }
+};
+__device__ __forceinline__ void put_piece(const PlanParams& a, const Runs& r, const Item& t, int w, long long j0, int last, bool first_of_pair) {
+  Piece d;
+  d.b = t.b, d.head = t.head, d.tile = t.tile, d.row0 = t.s.row0, d.T = t.s.T, d.L = t.s.L;
+  d.j0 = (int)j0;
+  d.j1 = w == last ? (int)t.n : (int)(r.begin(w + 1) - t.at - kLead);
+  d.slot = j0 > 0 ? 2 * w : w == last ? -1 : 2 * w + 1;
+  d.sinks = t.k.sinks, d.skip = t.k.window0 - t.k.sinks, d.pad = 0;
+  a.pieces[t.i + w] = d;
+  if (first_of_pair) a.plan->pair[w].x = t.i + w;
+  // the pair's last piece: the item goes on in the next pair, or the next item begins there
+  if (w < last || t.i + 1 == r.items || r.owner(t.at + t.n + 2 * kLead) > w) a.plan->pair[w].y = t.i + w + 1;
+}
 template <bool MASS>
-__device__ __forceinline__ void emit_runs(const PlanParams& a, const Seq& s, int b, int head, int tile, const Blocks& k,
-                                          int i, int items, long long at, long long n, long long length, int pairs,
-                                          int* cut_count) {
-  auto begin = [&](int w) { return quot((long long)w * length, pairs); };
-  auto owner = [&](long long x) { return (int)quot((x + 1) * pairs - 1, length); };
-  const int w0 = owner(at + kLead), parts = owner(at + kLead + n - 1) - w0 + 1;
-  const int before = i > 0 ? owner(at - 1) : -1, after = i + 1 < items ? owner(at + n + 2 * kLead) : pairs;
-  for (int c = 0; c < parts; c++) {
-    const int w = w0 + c;
-    Piece d;
-    d.b = b, d.head = head, d.tile = tile, d.row0 = s.row0, d.T = s.T, d.L = s.L;
-    d.j0 = c == 0 ? 0 : (int)(begin(w) - at - kLead);
-    d.j1 = c == parts - 1 ? (int)n : (int)(begin(w + 1) - at - kLead);
-    d.slot = parts == 1 ? -1 : c == 0 ? 2 * w + 1 : 2 * w;
-    d.sinks = k.sinks, d.skip = k.window0 - k.sinks, d.pad = 0;
-    a.pieces[i + w] = d;
-    if (c > 0 || before < w) a.plan->pair[w].x = i + w;
-    if (c < parts - 1 || after > w) a.plan->pair[w].y = i + w + 1;
+__device__ __forceinline__ void put_first(const PlanParams& a, const Runs& r, const Item& t, int* cut_count) {
+  const int w0 = r.owner(t.at + kLead), last = r.owner(t.at + kLead + t.n - 1);
+  put_piece(a, r, t, w0, 0, last, t.i == 0 || r.owner(t.at - 1) < w0);
+  if (MASS) a.parts[t.i] = make_int2(w0, last - w0 + 1);
+  else if (last > w0)
+    a.cuts[atomicAdd(cut_count, 1)] = Cut{t.b, t.head, t.tile, t.s.row0, t.s.T, last - w0 + 1, 2 * w0 + 1, 2 * (w0 + 1), 2};
+}
+// t: the item in which run w begins
+__device__ __forceinline__ void put_next(const PlanParams& a, const Runs& r, const Item& t, int w) {
+  const long long j0 = r.begin(w) - t.at - kLead;
+  if (j0 > 0) put_piece(a, r, t, w, j0, r.owner(t.at + kLead + t.n - 1), true);
+}
+// What joining `parts` partial results costs, in stages.
+__device__ __forceinline__ float join_cost(const PlanParams& a, float parts) {
+  return parts == 0.f ? 0.f : (kJoinNs + parts * a.part_bytes / kJoinRate) / a.stage_ns;
+}
+// The last of [0, n) for which f is not above x (f rises, f(0) <= x).
+template <typename F>
+__device__ __forceinline__ int last_not_above(int n, long long x, F f) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (f(mid) <= x) lo = mid;
+    else hi = mid - 1;
   }
-  if (MASS) a.parts[i] = make_int2(w0, parts);
-  else if (parts > 1)
-    a.cuts[atomicAdd(cut_count, 1)] = Cut{b, head, tile, s.row0, s.T, parts, 2 * w0 + 1, 2 * (w0 + 1), 2};
+  return lo;
 }
 
 // A small call: up to kPlanThreads sequences and as many tiles, one to a thread, all in shared memory.
@@ -106,7 +134,7 @@ template <bool MASS>
 __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const PlanParams a) {
   __shared__ int warp_sum[33], row0_s[kPlanThreads], T_s[kPlanThreads], L_s[kPlanThreads], entry_s[kPlanThreads + 1];
   __shared__ int most_s[kPlanThreads], stage_s[kPlanThreads + 1], place_s[kPlanThreads];
-  __shared__ float costs[32], seen_s[32];
+  __shared__ float costs[32], seen_s[32], rows_s[32];
   __shared__ int cut_count, longest_s;
   const ChunkParams& p = a.c;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -153,9 +181,13 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     }
     row0_s[tid] = mine.row0, T_s[tid] = mine.T, L_s[tid] = mine.L;
   }
+  float rows = (float)mine.T * (float)p.group;
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) seen += __shfl_xor_sync(0xffffffffu, seen, o);
-  if (lane == 0) seen_s[warp] = seen;
+  for (int o = 16; o >= 1; o >>= 1) {
+    seen += __shfl_xor_sync(0xffffffffu, seen, o);
+    rows += __shfl_xor_sync(0xffffffffu, rows, o);
+  }
+  if (lane == 0) seen_s[warp] = seen, rows_s[warp] = rows;
   entry_s[tid] = scan(tiles);
   const int entries = warp_sum[32], items = entries * heads;
   if (tid == 0) entry_s[kPlanThreads] = entries;
@@ -169,26 +201,15 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     return;
   }
   // ---- tiles: a thread's sequence is the last one whose entries begin at or before it (those without any share a begin)
-  int b = 0, e = 0, n = 0, tile = 0;
-  Seq s = {0, 0, 0};
-  Blocks k = {0, 0, 0};
+  int n = 0;
   if (tid < entries) {
-    int hi = p.batch - 1;
-    while (b < hi) {
-      const int mid = (b + hi + 1) >> 1;
-      if (entry_s[mid] <= tid) b = mid;
-      else hi = mid - 1;
-    }
-    s = Seq{row0_s[b], T_s[b], L_s[b]};
-    e = tile = tid - entry_s[b];
+    const int b = last_not_above(p.batch, tid, [&](int m) { return (long long)entry_s[m]; }), e = tid - entry_s[b];
+    const Seq s = {row0_s[b], T_s[b], L_s[b]};
     if (MASS) {
-      tile = key_tile(key_tiles_of(p, s, a.kb_log2), e);
-      const Tokens t = tokens_of(p, s, tile << a.kb_log2, 1 << a.kb_log2);
-      k.window0 = t.first / a.block_tokens;
-      n = ((t.last + a.block_tokens - 1) / a.block_tokens - k.window0) * a.head_chunks;
+      const Tokens t = tokens_of(p, s, key_tile(key_tiles_of(p, s, a.kb_log2), e) << a.kb_log2, 1 << a.kb_log2);
+      n = ((t.last + a.block_tokens - 1) / a.block_tokens - t.first / a.block_tokens) * a.head_chunks;
     } else {
-      k = blocks_of(p, s, e, a.kb_log2);
-      n = k.count();
+      n = blocks_of(p, s, e, a.kb_log2).count();
       atomicMax(&most_s[b], n);
       atomicMax(&longest_s, n);
     }
@@ -200,14 +221,21 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
   // ---- which way: warp w weighs chunks of at most longest / (w + 1) stages
   const int longest = longest_s;
   const long long stages = (long long)total * heads;
-  int run = 0;
+  int run = 0, used = a.pairs;
   if (!MASS) {
-    float rows = 0.f;
-    for (int w = 0; w < 32; w++) rows += seen_s[w];
+    float seen_all = seen_s[lane], rows_all = rows_s[lane];
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+      seen_all += __shfl_xor_sync(0xffffffffu, seen_all, o);
+      rows_all += __shfl_xor_sync(0xffffffffu, rows_all, o);
+    }
+    const float full = fminf(1.f, rows_all / ((float)entries * kTileRows));  // rows that a tile has
     constexpr float kHbm = 6500.f;  // bytes per ns
-    const float once = rows * (float)p.nkh * (float)p.hd * 4.f;  // bytes, K and V
+    const float once = seen_all * (float)p.nkh * (float)p.hd * 4.f;  // bytes, K and V
+    const float per_ns = 1.f / a.stage_ns, floor_once = once * (per_ns / kHbm);
     const int size = (longest + warp) / (warp + 1);
     int pieces = 0, cut = 0;
+#pragma unroll 1
     for (int i = lane; i < p.batch; i += 32) {
       const int m = ((i + 1 < p.batch ? entry_s[i + 1] : entries) - entry_s[i]) * heads;
       const int parts = (most_s[i] + size - 1) / size;
@@ -218,15 +246,21 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     cut = __reduce_add_sync(0xffffffffu, cut);
     if (lane == 0) {
       const float waves = (float)((pieces + a.pairs - 1) / a.pairs);
-      costs[warp] = cut > a.max_slots ? 3e38f : fmaxf(waves * (float)(size + kLead), once / kHbm / a.stage_ns) + (cut > 0 ? kJoinCost : 0);
+      costs[warp] = cut > a.max_slots ? 3e38f : fmaxf(waves * (float)(size + kLead), floor_once) + join_cost(a, (float)cut * full);
     }
     __syncthreads();
-    const float moved = (float)stages * a.stage_bytes;
+    // the cheapest chunks
+    const uint32_t mine = __float_as_uint(costs[lane]);  // (not negative: ordered as whole numbers)
+    const uint32_t least = __reduce_min_sync(0xffffffffu, mine);
+    const int k = __ffs(__ballot_sync(0xffffffffu, mine == least)) - 1;
+    // runs: fewer, longer ones where the parts would cost more than the keys (length / pairs + pairs x a part's cost is
+    // least where both are the same)
+    const float length = (float)stages + (float)kLead * (float)items;
+    used = max(1, min(a.pairs, (int)sqrtf(length * a.stage_ns * kJoinRate / (2.f * a.part_bytes * full))));
     // (90 MB of the 126 MB L2, beside what else passes through it)
-    const float floor_runs = (once > 90e6f ? fmaxf(moved, once) : once) / kHbm / a.stage_ns;
-    float best = fmaxf(((float)stages + (float)kLead * (float)items) / (float)a.pairs + kLead, floor_runs) + kJoinCost;
-    for (int w = 0; w < 32; w++)
-      if (costs[w] < best) best = costs[w], run = (longest + w) / (w + 1);
+    const float floor_runs = once > 90e6f ? fmaxf((float)stages * a.stage_bytes * (per_ns / kHbm), floor_once) : floor_once;
+    const float runs = fmaxf(length / (float)used + kLead, floor_runs) + join_cost(a, (float)(used + min(items, used)) * full);
+    if (__uint_as_float(least) < runs) run = (longest + k) / (k + 1);
   }
   if (run > 0) {
     // ---- chunks: pieces before each sequence, places of partial results
@@ -237,37 +271,68 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
     __syncthreads();
     place_s[tid] = scan(parts > 1 ? tiles * heads * parts : 0);
     stage_s[tid] = pieces0;  // (the stages are not needed any more)
-    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(w, pieces, a.pairs, 0);
     __syncthreads();
-    if (tid < entries) {
-      const int of = (b + 1 < p.batch ? entry_s[b + 1] : entries) - entry_s[b];
-      const int all = (most_s[b] + run - 1) / run, split = min(all, n);
-      for (int head = 0; head < heads; head++) {
-        const int kvh = head / a.halves, half = head - kvh * a.halves, slot = place_s[b] + (head * of + e) * all;
-        for (int c = 0; c < all; c++) {
-          Piece d;
-          d.b = b, d.head = head, d.tile = tile, d.row0 = s.row0, d.T = s.T, d.L = s.L;
-          d.j0 = c < split ? n * c / split : 0;
-          d.j1 = c < split ? n * (c + 1) / split : 0;
-          d.slot = split > 1 ? slot + c : -1;
-          d.sinks = k.sinks, d.skip = k.window0 - k.sinks, d.pad = 0;
-          a.pieces[stage_s[b] + (kvh * all + c) * of * a.halves + e * a.halves + half] = d;
-        }
-        if (split > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{b, head, tile, s.row0, s.T, split, slot, slot + 1, 1};
-      }
+    for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(w, pieces, a.pairs, 0);
+    const int most = (longest + run - 1) / run;
+    for (int x = tid; x < entries * heads * most; x += kPlanThreads) {  // (entry, head, chunk)
+      const int y = x / most, c = x - y * most, at_e = y / heads, head = y - at_e * heads;
+      const int m = last_not_above(p.batch, at_e, [&](int i) { return (long long)entry_s[i]; });
+      const int of = (m + 1 < p.batch ? entry_s[m + 1] : entries) - entry_s[m], t = at_e - entry_s[m];
+      const int all = (most_s[m] + run - 1) / run;
+      if (c >= all) continue;
+      const Seq q = {row0_s[m], T_s[m], L_s[m]};
+      const Blocks blocks = blocks_of(p, q, t, a.kb_log2);
+      const int count = blocks.count(), split = min(all, count);
+      const int kvh = head / a.halves, half = head - kvh * a.halves, slot = place_s[m] + (head * of + t) * all;
+      Piece d;
+      d.b = m, d.head = head, d.tile = t, d.row0 = q.row0, d.T = q.T, d.L = q.L;
+      d.j0 = c < split ? count * c / split : 0;
+      d.j1 = c < split ? count * (c + 1) / split : 0;
+      d.slot = split > 1 ? slot + c : -1;
+      d.sinks = blocks.sinks, d.skip = blocks.window0 - blocks.sinks, d.pad = 0;
+      a.pieces[stage_s[m] + (kvh * all + c) * of * a.halves + t * a.halves + half] = d;
+      if (c == 0 && split > 1) a.cuts[atomicAdd(&cut_count, 1)] = Cut{m, head, t, q.row0, q.T, split, slot, slot + 1, 1};
     }
   } else {
     // ---- runs
-    const long long length = stages + (long long)kLead * items;
-    const int pairs = (int)min((long long)a.pairs, length);
-    if (tid < entries) {
-      const int next = b + 1 < p.batch ? entry_s[b + 1] : entries, of = next - entry_s[b];
+    Runs r;
+    r.length = stages + (long long)kLead * items, r.items = items, r.pairs = (int)min((long long)used, r.length);
+    // tile e of head `head` of sequence b
+    auto item_of = [&](int b, int head, int e) {
+      Item t;
+      const int next = b + 1 < p.batch ? entry_s[b + 1] : entries, of = next - entry_s[b], at_e = entry_s[b] + e;
       const int first = stage_s[entry_s[b]], all = (next < entries ? stage_s[next] : total) - first;
-      for (int head = 0; head < heads; head++) {
-        const int i = entry_s[b] * heads + head * of + e;
-        const long long at = (long long)first * heads + (long long)head * all + (before - first) + (long long)kLead * i;
-        emit_runs<MASS>(a, s, b, head, tile, k, i, items, at, n, length, pairs, &cut_count);
+      t.i = entry_s[b] * heads + head * of + e, t.b = b, t.head = head;
+      t.s = Seq{row0_s[b], T_s[b], L_s[b]};
+      t.n = (at_e + 1 < entries ? stage_s[at_e + 1] : total) - stage_s[at_e];
+      t.at = (long long)first * heads + (long long)head * all + (stage_s[at_e] - first) + (long long)kLead * t.i;
+      t.k = Blocks{0, 0, 0};
+      t.tile = e;
+      if (MASS) {
+        t.tile = key_tile(key_tiles_of(p, t.s, a.kb_log2), e);
+        t.k.window0 = tokens_of(p, t.s, t.tile << a.kb_log2, 1 << a.kb_log2).first / a.block_tokens;
+      } else {
+        t.k = blocks_of(p, t.s, e, a.kb_log2);
       }
+      return t;
+    };
+    for (int x = tid; x < items; x += kPlanThreads) {  // (entry, head)
+      const int at_e = x / heads, head = x - at_e * heads;
+      const int of_b = last_not_above(p.batch, at_e, [&](int m) { return (long long)entry_s[m]; });
+      put_first<MASS>(a, r, item_of(of_b, head, at_e - entry_s[of_b]), &cut_count);
+    }
+    for (int w = tid + 1; w < r.pairs; w += kPlanThreads) {
+      const long long x = r.begin(w);
+      auto seq_at = [&](int m) {
+        return entry_s[m] < entries ? (long long)stage_s[entry_s[m]] * heads + (long long)kLead * heads * entry_s[m] : r.length;
+      };
+      const int of_b = last_not_above(p.batch, x, seq_at);
+      const int next = of_b + 1 < p.batch ? entry_s[of_b + 1] : entries, of = next - entry_s[of_b], first = stage_s[entry_s[of_b]];
+      const long long per = (next < entries ? stage_s[next] : total) - first + (long long)kLead * of, in = x - seq_at(of_b);
+      const int head = (int)quot(in, per);
+      const long long rest = in - head * per;
+      const int e = last_not_above(of, rest, [&](int m) { return (long long)(stage_s[entry_s[of_b] + m] - first) + (long long)kLead * m; });
+      put_next(a, r, item_of(of_b, head, e), w);
     }
   }
   __syncthreads();
@@ -388,7 +453,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     }
     if (lane == 0) {
       const float waves = (float)((pieces + a.pairs - 1) / a.pairs);
-      costs[warp] = cut > a.max_slots ? 3e38f : fmaxf(waves * (float)(run + kLead), floor_once) + (cut > 0 ? kJoinCost : 0);
+      costs[warp] = cut > a.max_slots ? 3e38f : fmaxf(waves * (float)(run + kLead), floor_once) + join_cost(a, (float)cut);
     }
   }
   __syncthreads();
@@ -396,7 +461,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     const float moved = (float)stages * a.stage_bytes;
     // (90 MB of the 126 MB L2, beside what else passes through it)
     const float floor_runs = (once > 90e6f ? fmaxf(moved, once) : once) / hbm / a.stage_ns;
-    float best = fmaxf(((float)stages + (float)kLead * (float)items) / (float)a.pairs + kLead, floor_runs) + kJoinCost;
+    float best = fmaxf(((float)stages + (float)kLead * (float)items) / (float)a.pairs + kLead, floor_runs) + join_cost(a, 2.f * (float)a.pairs);
     int run = 0;
     for (int k = 0; k < (MASS ? 0 : 32); k++)
       if (costs[k] < best) best = costs[k], run = (longest + k) / (k + 1);
@@ -454,27 +519,42 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
     return;
   }
   // ---- runs
-  const long long length = stages + (long long)kLead * items;
-  const int pairs = (int)min((long long)a.pairs, length);
+  Runs r;
+  r.length = stages + (long long)kLead * items, r.items = items, r.pairs = (int)min((long long)a.pairs, r.length);
   for (int w = tid; w < a.pairs; w += kPlanThreads) a.plan->pair[w] = make_int4(0, 0, 1, 0);
   __syncthreads();
-  for (int i = tid; i < items; i += kPlanThreads) {
-    const int b = find_seq(a.seqs, p.batch, i, true);
-    const Seq s = seq_of(p, b, cap);
-    const int e0 = a.seqs[b].x, tiles = a.seqs[b + 1].x - e0, local = i - a.seqs[b].y;
-    const int head = local / tiles, e = local - head * tiles;
-    const long long first = a.entries[e0], mine = (a.seqs[b + 1].x < entries ? a.entries[e0 + tiles] : total) - first;
-    const long long at = first * heads + head * mine + (a.entries[e0 + e] - first) + (long long)kLead * i;
-    int tile = e;
-    Blocks k = {0, 0, 0};
+  auto item_of = [&](int b, int head, int e) {
+    Item t;
+    const int e0 = a.seqs[b].x, next = a.seqs[b + 1].x, of = next - e0;
+    const long long first = a.entries[e0], all = (next < entries ? a.entries[next] : total) - first;
+    t.i = a.seqs[b].y + head * of + e, t.b = b, t.head = head;
+    t.s = seq_of(p, b, cap);
+    t.n = (e0 + e + 1 < entries ? a.entries[e0 + e + 1] : total) - a.entries[e0 + e];
+    t.at = first * heads + head * all + (a.entries[e0 + e] - first) + (long long)kLead * t.i;
+    t.k = Blocks{0, 0, 0};
+    t.tile = e;
     if (MASS) {
-      tile = key_tile(key_tiles_of(p, s, a.kb_log2), e);
-      row_blocks(s, tile, k.window0);
+      t.tile = key_tile(key_tiles_of(p, t.s, a.kb_log2), e);
+      (void)row_blocks(t.s, t.tile, t.k.window0);
     } else {
-      k = blocks_of(p, s, e, a.kb_log2);
+      t.k = blocks_of(p, t.s, e, a.kb_log2);
     }
-    const long long n = (e0 + e + 1 < entries ? a.entries[e0 + e + 1] : total) - a.entries[e0 + e];
-    emit_runs<MASS>(a, s, b, head, tile, k, i, items, at, n, length, pairs, &cut_count);
+    return t;
+  };
+  for (int i = tid; i < items; i += kPlanThreads) {
+    const int b = find_seq(a.seqs, p.batch, i, true), of = a.seqs[b + 1].x - a.seqs[b].x, local = i - a.seqs[b].y;
+    put_first<MASS>(a, r, item_of(b, local / of, local % of), &cut_count);
+  }
+  for (int w = tid + 1; w < r.pairs; w += kPlanThreads) {
+    const long long x = r.begin(w);
+    auto seq_at = [&](int m) {
+      return a.seqs[m].x < entries ? a.entries[a.seqs[m].x] * heads + (long long)kLead * a.seqs[m].y : r.length;
+    };
+    const int b = last_not_above(p.batch, x, seq_at), e0 = a.seqs[b].x, next = a.seqs[b + 1].x;
+    const long long first = a.entries[e0], per = (next < entries ? a.entries[next] : total) - first + (long long)kLead * (next - e0);
+    const long long in = x - seq_at(b), head = quot(in, per), rest = in - head * per;
+    const int e = last_not_above(next - e0, rest, [&](int m) { return a.entries[e0 + m] - first + (long long)kLead * m; });
+    put_next(a, r, item_of(b, (int)head, e), w);
   }
   __syncthreads();
   if (tid == 0) a.plan->cuts = cut_count;

@@ -12,7 +12,8 @@ constexpr int kPlanThreads = 1024;
 // Stages that a piece costs besides its keys: queries, the first scores and softmax without an MMA beside them,
 // epilogue.
 constexpr int kLead = 3;
-constexpr int kJoinCost = 4;  // and the join, if any tile is cut
+// And the join, if any tile is cut: ns for itself, and bytes per ns that it (and the writing) takes for the parts.
+constexpr float kJoinNs = 3500.f, kJoinRate = 2500.f;
 
 // A run of a tile's key blocks for one pair of CTAs.
 struct Piece {
@@ -43,6 +44,7 @@ struct PlanParams {
   int max_slots;
   long long max_entries;  // tiles that there is room for (more: the sequences' rows of q overlap)
   float stage_bytes, stage_ns;  // of a block: what is loaded, about how long it takes
+  float part_bytes;             // of a whole tile's partial result
   int block_tokens, head_chunks;  // masses: tokens of a row block, row blocks for the heads of one token
   Plan* plan;
   Piece* pieces;

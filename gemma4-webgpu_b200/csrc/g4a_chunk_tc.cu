@@ -824,6 +824,7 @@ g4a_status launch_chunk(g4a_ctx* ctx, const ChunkParams& p) {
   q.max_slots = (int)slots;
   q.max_entries = entries;
   q.stage_bytes = 2.f * (C::K_BYTES + C::V_BYTES);
+  q.part_bytes = (float)(kTileRows * C::HDV * sizeof(float));
   q.stage_ns = C::KB * (HD + C::HDV) * (1.f / 55.f);
   a.part = reinterpret_cast<float*>(ws);
   q.plan = reinterpret_cast<Plan*>(ws += n_part);

@@ -634,3 +634,22 @@ def test_pools_beyond_32_bits_of_elements(ctx):
     _evict(ctx, case, total, budget=100, sinks=3, recent=9)
     bits = lambda t: t.view(torch.int16)  # noqa: E731
     assert torch.equal(got, total) and torch.equal(bits(k[shift:]), bits(small_k)) and torch.equal(bits(v[shift:]), bits(small_v))
+
+
+@pytest.mark.parametrize("tokens", [1, 4])
+def test_more_sequences_than_a_small_plan_holds(ctx, tokens):
+    """More than 1,024 sequences (4 tokens of 4 heads each), and more than 128 of one token."""
+    batch = 1100 if tokens > 1 else 150
+    rnd = random.Random(tokens)
+    counts = [rnd.choice([0, tokens, tokens]) for _ in range(batch)]
+    lens = [max(1, c + rnd.randint(0, 60)) for c in counts]
+    case, q = _case(3, counts, lens, nkh=1, group=8, hd=64, page=16)
+    out, lse = _check(ctx, case, q, window=40, sinks=2)
+    _check_mass(ctx, case, q, window=40, sinks=2, decay=0.5)
+
+
+def test_many_tiles_in_one_call(ctx):
+    """More tiles than a small plan holds, several heads, whole tiles and cut ones."""
+    case, q = _case(4, [1500, 1300, 20, 900], [1500, 2000, 3500, 1000], nkh=4, group=48, hd=64, page=64)
+    _check(ctx, case, q)
+    _check_mass(ctx, case, q)
