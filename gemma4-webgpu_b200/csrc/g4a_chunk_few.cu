@@ -28,7 +28,7 @@ using namespace g4a_chunk;
 
 constexpr int kWarps = 4, kStepKeys = 16, kTile = 8;  // warps of a CTA; keys of a step; query rows of a tile
 constexpr int kNoKey = -1 - 0x7fffffff;
-constexpr float kRaiseF = 15.0f, kFirstF = -3.0f, kLaterF = 5.0f, kUnseenF = -FLT_MAX;
+constexpr float kRaiseF = 15.0f, kFirstF = -3.0f, kLaterF = 1.0f, kUnseenF = -FLT_MAX;
 
 struct FewParams {
   ChunkParams c;
@@ -469,8 +469,11 @@ g4a_status launch(g4a_ctx* ctx, const ChunkParams& p) {
   uint64_t keys = cap;
   if (p.window != 0u) keys = std::min<uint64_t>(cap, (uint64_t)p.window + p.sinks + 4 * kStepKeys);
   const long long most = (long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys));
-  // two CTAs to an SM, one round of them; a sequence has four times its share at most
-  const long long ctas = std::max(2ll * ctx->num_sms, 2 * heads);
+  // Two CTAs to an SM are one round.  While the heads are fewer than that, half a round more than the heads deals the keys
+  // evenly enough (64 sequences of up to 8,000 keys x 4 heads of 128 dims: 195 us, twice the heads 214); with more heads
+  // it takes two to a head (64 x 8 heads: 322 us, heads and half a round 351).  A sequence has four times its share at most.
+  const long long room = 2ll * ctx->num_sms;
+  const long long ctas = heads < room ? std::max(room, heads + room / 2) : 2 * heads;
   if (p.batch <= kWarps * 32) {
     a.ctas = (int)std::min(ctas, heads * most + heads);
     a.splits = (int)std::min(most, 4 * ((ctas + heads - 1) / heads));

@@ -39,10 +39,11 @@ constexpr int kThreadsC = 512;
 constexpr int kSoft = 8, kLoadK = 8, kLoadV = 9, kMma = 10, kTellK = 11, kGuard = 12;
 constexpr int kCtaRows = 128;
 // Weights are p = 2^(s - m).  A score above m + 15 (f16 ends at 2^16) raises m: to 3 below the maximum at the row's first
-// scores, to 5 above it later on.  A raise costs the pair a stage's time (O has to be at rest to be rescaled), so later ones
-// leave room for the next 2^20: with m kept 7 below the maximum and raised at 2^8 past it, 512 tokens over 131,000 rows
-// took 604 us instead of 405.
-constexpr float kRaiseC = 15.0f, kFirstC = -3.0f, kLaterC = 5.0f;
+// scores, to 1 above it later on, so the largest weight is 2^-1 at least, and f16's rounding of one is off by 2^-11 of it
+// or 2^-25.  A raise costs the pair a stage's time (O has to be at rest to be rescaled), so m does not follow the maximum
+// closely: with m kept 7 below the maximum and raised at 2^8 past it, 512 tokens over 131,000 rows took 591 us instead
+// of 447, six ragged chunks of heads of 128 dims 213 instead of 190.
+constexpr float kRaiseC = 15.0f, kFirstC = -3.0f, kLaterC = 1.0f;
 constexpr float kUnseenC = -FLT_MAX;  // m of a row that has seen nothing yet (any finite score raises it)
 constexpr int kBadTags = 8;
 

@@ -67,10 +67,10 @@ def score_error(amp, hd):
 
 def attn_tolerance(amp, hd, keys, vmax):
     """Bound of the absolute error of one f16 output: a weight is off by ln 2 times the score's error and 2^-21 for exp2
-    and its argument, twice (numerator and denominator), and by its rounding to f16, 2^-11 relative or 2^-25 (weights
-    reach 2^7 at least, so that is 2^-32 of their sum for each key); keys / 16 + 36 additions of f32; the output's rounding."""
+    and its argument, twice (numerator and denominator), and by its rounding to f16, 2^-11 relative or 2^-25 (the
+    largest weight is 2^-1 at least, so that is 2^-24 of their sum for each key); keys / 16 + 36 additions of f32; the output's rounding."""
     dp = math.log(2) * score_error(amp, hd) + 2.0 ** -21
-    return (2 * dp + 2.0 ** -11 + keys * 2.0 ** -32 + (keys / 16 + 36) * 2.0 ** -23 + 2.0 ** -11) * vmax
+    return (2 * dp + 2.0 ** -11 + keys * 2.0 ** -24 + (keys / 16 + 36) * 2.0 ** -23 + 2.0 ** -11) * vmax
 
 
 def lse_tolerance(amp, hd, keys, top):
