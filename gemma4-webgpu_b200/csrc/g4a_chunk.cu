@@ -24,7 +24,7 @@ g4a_status g4a_chunk_params(const char* fn, g4a_ctx* ctx, ChunkParams& p, const 
                     num_kv_heads);
   if (head_dim == 0 || head_dim > 512 || (head_dim % 8) != 0)
     return g4a_fail(G4A_EINVAL, "%s: head_dim %u must be a multiple of 8 in [8, 512]", fn, head_dim);
-  if (!std::isfinite(scale)) return g4a_fail(G4A_EINVAL, "%s: scale is not finite", fn);
+  if (!std::isfinite(scale * kLog2eC)) return g4a_fail(G4A_EINVAL, "%s: scale is not finite", fn);
   if (batch > 0x00ffffffu || num_tokens > 0x7fffffffu || (uint64_t)num_tokens * num_q_heads > 0x7fffffffu)
     return g4a_fail(G4A_EINVAL, "%s: batch %u or num_tokens %u too large", fn, batch, num_tokens);
   if (page_size == 0 || max_pages_per_seq == 0 || num_pages == 0 || num_pages > 0x7fffffffu)
@@ -111,11 +111,17 @@ extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, cons
   if (batch == 0 || num_tokens == 0) return G4A_OK;
   if (!out) return g4a_fail(G4A_EINVAL, "%s: null pointer", fn);
   if ((uintptr_t)out & 15u) return g4a_fail(G4A_EINVAL, "%s: out must be 16-byte aligned", fn);
+  const uint64_t size = (uint64_t)num_tokens * num_q_heads * head_dim;
+  if (out < q + size && q < out + size) return g4a_fail(G4A_EINVAL, "%s: out overlaps q", fn);
   g4a_device_guard dev(ctx);
   if (dev.status != G4A_OK) return dev.status;
   p.lse = lse;
   p.out = reinterpret_cast<__half*>(out);
-  // query rows of a sequence and kv head, on average
-  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 8u * (uint64_t)batch && (uint64_t)batch * num_kv_heads <= 65535u;
+  // By the query rows of a sequence and kv head, on average (the lengths are on the device).  Tiles of 256 rows against
+  // tiles of 8, in us: 8 rows 71, 54 (32 sequences of 8,000 rows, 256 dims), 105, 56 (16, 512 dims), 62, 35 (32, 128 dims),
+  // 23, 19 (one of 8,000), 29, 18 (32 of 1,000); 16 rows 71, 99; 107, 104; 62, 61; 23, 24; 29, 28; 32 rows 72, 188 for the
+  // first.
+  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 8u * (uint64_t)batch &&
+                   (uint64_t)batch * num_kv_heads <= 65535u;
   return few ? g4a_chunk_few_launch(ctx, p) : g4a_chunk_tc_launch(ctx, p);
 }

@@ -515,9 +515,10 @@ g4a_status g4a_paged_kv_compact(g4a_ctx* ctx, uint16_t* k_pages, uint16_t* v_pag
 
 /* out (f16, like q) = softmax(scale q K^T) V over the rows that a token sees, and lse (f32
  * [num_tokens, num_q_heads], may be NULL) = log sum exp(scale q k) over them.  A token that sees nothing
- * gets zeros and an lse of -inf.  Softmax weights are rounded to f16 for their product with V, sums are held in
- * f32.  Rows of out and lse behind the last sequence stay as they were.  A value that is not finite in a
- * row of the cache reaches only the tokens that see that row.  f32 queries: g4a_tree_attn_paged. */
+ * gets zeros and an lse of -inf.  out must not overlap q.  Softmax weights are rounded to f16 for their
+ * product with V, sums are held in f32.  Rows of out and lse behind the last sequence stay as they were.  A
+ * value that is not finite in a row of the cache reaches only the tokens that see that row.  f32 queries:
+ * g4a_tree_attn_paged. */
 g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages,
                                 const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_indptr,
                                 uint32_t num_tokens, uint32_t batch, uint32_t page_size,
@@ -530,7 +531,8 @@ g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, const uint16_t*
  * over those that see r, with q and lse as in g4a_chunk_attn_paged.  The T new rows start from 0, whatever
  * their entries held; decay 0 does the same for all rows.  0 <= decay <= 1.  mass_stride >= the largest
  * kv_lens[b] (a longer sequence is skipped and reported); entries behind kv_lens[b] stay as they were.
- * A q row whose lse is -inf adds nothing; a call without tokens (num_tokens 0) does nothing.  Sums are f32 in an order that does not change from run to run.  batch * num_kv_heads <= 65535. */
+ * A q row whose lse is -inf adds nothing; a call without tokens (num_tokens 0) does nothing.  Sums are f32 in
+ * an order that does not change from run to run.  batch * num_kv_heads <= 65535. */
 g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const float* lse, const uint16_t* k_pages,
                               const int32_t* page_table, const int32_t* kv_lens, const int32_t* q_indptr,
                               uint32_t num_tokens, uint32_t batch, uint32_t page_size,

@@ -15,7 +15,7 @@ NULL = ctypes.c_void_p(None)
 
 ATTN = (["ctx", "q", "kp", "vp", "table", "lens", "indptr", "n", "batch", "page", "max_pages", "pages", "nqh", "nkh", "hd",
          "scale", "window", "sinks", "lse", "out"],
-        [CTX, P, P, P, P, P, P, 4, 1, 16, 8, 8, 8, 1, 256, 1.0, 0, 0, P, P])
+        [CTX, P, P, P, P, P, P, 4, 1, 16, 8, 8, 8, 1, 256, 1.0, 0, 0, P, P2])
 MASS = (["ctx", "q", "lse", "kp", "table", "lens", "indptr", "n", "batch", "page", "max_pages", "pages", "nqh", "nkh", "hd",
          "scale", "window", "sinks", "decay", "mass", "stride"],
         [CTX, P, P, P, P, P, P, 4, 1, 16, 8, 8, 8, 1, 256, 1.0, 0, 0, 1.0, P, 128])
@@ -49,7 +49,8 @@ SHARED = [
 
 
 @pytest.mark.parametrize("kw,text", SHARED + [(dict(vp=NULL), "null"), (dict(vp=ODD), "aligned"), (dict(out=NULL), "null"),
-                                              (dict(out=ODD), "aligned")])
+                                              (dict(out=ODD), "aligned"), (dict(out=P), "overlaps"),
+                                              (dict(out=ctypes.c_void_p(0x10000 + 4 * 8 * 256 * 2 - 16)), "overlaps")])
 def test_chunk_refusals(kw, text):
     refused("g4a_chunk_attn_paged", changed(ATTN, **kw), text)
 
