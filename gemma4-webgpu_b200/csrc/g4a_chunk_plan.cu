@@ -563,7 +563,11 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const PlanPara
 }  // namespace
 
 cudaError_t g4a_chunk_plan_launch(g4a_ctx* ctx, const PlanParams& a, bool masses, long long entries) {
-  const bool small = a.c.batch <= kPlanThreads && entries <= kPlanThreads;
+  // (the small kernel adds up a head's stages in 32 bits)
+  const ChunkParams& p = a.c;
+  const long long rows = (long long)p.page_size * p.max_pages;
+  const long long most = masses ? ((long long)p.tokens / a.block_tokens + 2) * a.head_chunks : (rows >> a.kb_log2) + 3;
+  const bool small = p.batch <= kPlanThreads && entries <= kPlanThreads && entries * most <= 0x7fffffffll;
   return g4a_launch(small ? (masses ? chunk_plan_small_kernel<true> : chunk_plan_small_kernel<false>)
                           : (masses ? chunk_plan_kernel<true> : chunk_plan_kernel<false>),
                     dim3(1), dim3(kPlanThreads), 0, ctx->stream, true, a);

@@ -41,9 +41,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kern
   float* mass = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride;
   // the pages of keys g and g + 8, looked up one step ahead
   auto page_of = [&](long long key) { return key < s.L ? table[(uint32_t)key / (uint32_t)p.page_size] : kNoKey; };
-  int k0 = ((int)blockIdx.x * kFewWarps + warp) * 16;
-  int pages[2] = {page_of(k0 + g), page_of(k0 + g + 8)};
-  for (; k0 < s.L; k0 += stride) {
+  const int k_first = ((int)blockIdx.x * kFewWarps + warp) * 16;
+  int pages[2] = {page_of((long long)k_first + g), page_of((long long)k_first + g + 8)};
+  for (long long at = k_first; at < s.L; at += stride) {
+    const int k0 = (int)at;
     long long off[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -463,12 +464,12 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const MassParams a) {
   const Blocks k = key_tiles_of(p, s, kTileLog2);
   if (a.seqs[b].y < 0) return;  // the call does not fit together
   const int item0 = a.seqs[b].y + kvh * k.count();
-  for (int tile = (int)blockIdx.x; tile << kTileLog2 < s.L; tile += (int)gridDim.x) {
+  for (int tile = (int)blockIdx.x; (long long)tile << kTileLog2 < s.L; tile += (int)gridDim.x) {
     const int r = (tile << kTileLog2) + (int)threadIdx.x;
     const int e = tile < k.sinks ? tile : tile >= k.window0 && tile < k.window1 ? tile - k.window0 + k.sinks : -1;
     const int2 parts = e >= 0 ? a.parts[item0 + e] : make_int2(0, 0);
     if (parts.y == 1 || (parts.y == 0 && p.decay == 1.f)) continue;
-    if (r >= s.L || row_offset(p, b, kvh, r) < 0) continue;
+    if ((uint32_t)r >= (uint32_t)s.L || row_offset(p, b, kvh, r) < 0) continue;
     float sum = 0.f;
     // (of the pair that begins the tile, in its place 2 w + 1; of the next ones, in 2 w)
     for (int i = 0; i < parts.y; i++) sum += a.part[(size_t)(2 * (parts.x + i) + (i == 0)) * (2 * kCtaKeys) + threadIdx.x];
@@ -593,8 +594,10 @@ extern "C" g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const 
   p.decay = decay;
   if ((uint64_t)batch * num_kv_heads > 65535u)
     return g4a_fail(G4A_EINVAL, "%s: batch %u * num_kv_heads %u exceeds 65535", fn, batch, num_kv_heads);
-  // query rows of a sequence, on average
-  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 32u * (uint64_t)batch;
+  // By the query rows of a sequence and kv head, on average.  Tiles of 256 keys against 16 keys to a warp, in us: 16 rows
+  // 52, 38 (32 sequences of 8,000 rows, 256 dims), 48, 28 (128 dims), 45, 50 (16, 512 dims), 15, 9.7 (one of 8,000), 16.5,
+  // 9.6 (32 of 1,000); 32 rows 52, 56; 48, 42; 45, 72; 15, 9.5; 17, 10; 64 rows 52, 96; 48, 71; 45, 117; 15, 12.5; 16, 16.
+  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= (head_dim > 256 ? 16u : 32u) * (uint64_t)batch;
   if (head_dim > 256) return few ? launch_few<16>(ctx, p) : launch_chunk_mass<512>(fn, ctx, p);
   if (head_dim > 128) return few ? launch_few<8>(ctx, p) : launch_chunk_mass<256>(fn, ctx, p);
   return few ? launch_few<4>(ctx, p) : launch_chunk_mass<128>(fn, ctx, p);
