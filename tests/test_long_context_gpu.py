@@ -39,9 +39,9 @@ def _attend(ctx, case, q, *, window=0, sinks=0, scale=None, tail=3, sync=True):
     return out[:n], lse[:n]
 
 
-def _check(ctx, case, q, *, window=0, sinks=0):
+def _check(ctx, case, q, *, window=0, sinks=0, tail=3):
     hd, keys = q.shape[2], max(case.lens)
-    out, lse = _attend(ctx, case, q, window=window, sinks=sinks)
+    out, lse = _attend(ctx, case, q, window=window, sinks=sinks, tail=tail)
     want, z, amp = chunk_ref(case, q, scale=hd ** -0.5, window=window, sinks=sinks)
     vmax = max((float(v.abs().max()) for _, v in case.rows if v.numel()), default=1.0)
     assert float((out.double() - want).abs().max()) <= attn_tolerance(amp, hd, keys, vmax)
@@ -67,6 +67,11 @@ SHAPES = [  # counts, lens, nkh, group, hd, page, window, sinks
     ([257], [900], 1, 1, 128, 64, 256, 300),
     ([2, 2, 2], [512, 513, 514], 1, 8, 384, 24, 512, 4),
     ([6], [200], 1, 24, 40, 16, 0, 0),
+    # groups that do not fit into a CTA's rows, or into a tile's
+    ([5, 1], [40, 300], 1, 130, 64, 16, 0, 0),
+    ([3], [270], 1, 300, 128, 16, 20, 2),
+    ([2, 1], [400, 77], 2, 40, 256, 64, 0, 0),
+    ([4], [130], 1, 128, 512, 64, 100, 0),
 ]
 
 
@@ -88,13 +93,17 @@ FEW = [  # few query rows to a sequence: decode steps, some sequences idle, some
     ([1, 2, 1, 0], [600, 601, 602, 3], 1, 3, 384, 24, 512, 4),
     ([6, 0], [300, 1], 1, 2, 320, 48, 100, 40),
     ([1], [3000], 2, 8, 512, 64, 2000, 200),
+    ([1] * 60, [211 * i + 1 for i in range(60)], 1, 8, 512, 64, 0, 0),
+    ([1] * 60, [211 * i + 1 for i in range(60)], 6, 2, 128, 16, 0, 0),  # more heads than a round of CTAs
+    ([1] * 140, [(97 * i) % 2500 + 1 for i in range(140)], 1, 8, 256, 16, 600, 4),  # more sequences than a CTA deals out
 ]
 
 
+@pytest.mark.parametrize("tail", [0, 3])  # (rows behind the last sequence count where the kernel is chosen)
 @pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", FEW)
-def test_chunk_attention_of_few_rows(ctx, counts, lens, nkh, group, hd, page, window, sinks):
+def test_chunk_attention_of_few_rows(ctx, counts, lens, nkh, group, hd, page, window, sinks, tail):
     case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
-    _check(ctx, case, q, window=window, sinks=sinks)
+    _check(ctx, case, q, window=window, sinks=sinks, tail=tail)
 
 
 @pytest.mark.parametrize("hd,group", [(64, 1), (256, 2), (512, 1), (512, 3)])
@@ -116,6 +125,42 @@ def test_values_that_are_not_finite_in_steps_of_few_rows(ctx, hd, group):
     finite = want.isfinite()
     assert torch.equal(lse, lse0) and torch.equal(out.isfinite(), finite) and torch.equal(out[finite], clean[finite])
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want == float("inf"))
+
+
+@pytest.mark.parametrize("hd", [128, 256, 512])
+def test_steps_of_few_rows_out_of_the_ordinary(ctx, hd):
+    """Single tokens (no rows behind them): scores that grow by thousands along the rows, missing pages, a key and a
+    query that are not finite."""
+    lens = [1500, 90]
+    case, q = _case(hd, [1, 1], lens, nkh=1, group=8, hd=hd, page=16, spread=1.0)
+    k, v = case.rows[0]
+    k = (k * torch.linspace(0.02, 60.0, lens[0])[:, None, None]).half()
+    case.rows[0] = (k, v)
+    s = torch.arange(lens[0])
+    case.k[case.table_host[0].long()[s // 16], s % 16] = k.cuda()
+    _check(ctx, case, q, tail=0)
+    clean, lse0 = _attend(ctx, case, q, tail=0)
+    bad = q.clone()
+    bad[0, 3, 1] = float("inf")
+    page, row = int(case.table_host[1, 5]), 3
+    was = case.k[page, row, 0, 2].clone()
+    case.k[page, row, 0, 2] = float("nan")
+    out, lse = _attend(ctx, case, bad, tail=0)
+    assert bool(out[1].isnan().all()) and bool(lse[1].isnan().all()) and bool(out[0, 3].isnan().all())
+    others = torch.arange(8, device="cuda") != 3
+    assert torch.equal(out[0, others], clean[0, others]) and torch.equal(lse[0, others], lse0[0, others])
+    case.k[page, row, 0, 2] = was
+    there = [torch.ones(n, dtype=torch.bool) for n in lens]
+    for b, j, x in ((0, 2, -1), (0, 60, 1 << 30), (1, 0, case.k.shape[0])):
+        case.table[b, j] = x
+        there[b][j * 16:(j + 1) * 16] = False
+    out, lse = _attend(ctx, case, q, tail=0, sync=False)
+    with pytest.raises(G4AError, match="page id"):
+        ctx.sync()
+    want, z, amp = chunk_ref(case, q, scale=hd ** -0.5, there=there)
+    vmax = max(float(v.abs().max()) for _, v in case.rows)
+    assert float((out.double() - want).abs().max()) <= attn_tolerance(amp, hd, 1500, vmax)
+    assert float((lse.double() - z).abs().max()) <= lse_tolerance(amp, hd, 1500, float(z.abs().max()))
 
 
 def test_sequences_whose_rows_overlap_are_refused_where_they_do_not_fit(ctx):
@@ -281,70 +326,10 @@ def _check_mass(ctx, case, q, *, window=0, sinks=0, decay=1.0):
 
 
 @pytest.mark.parametrize("decay", [1.0, 0.9, 0.0])
-@pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", SHAPES)
+@pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", SHAPES + FEW)
 def test_key_mass(ctx, counts, lens, nkh, group, hd, page, window, sinks, decay):
     case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
     _check_mass(ctx, case, q, window=window, sinks=sinks, decay=decay)
-
-
-FEW = [  # few query rows to a sequence: decode steps, some sequences idle, some with more tokens than the others
-    ([1, 0, 1], [1, 40, 500], 1, 8, 256, 64, 0, 0),
-    ([20, 0, 0], [333, 5, 9], 1, 1, 128, 16, 0, 0),
-    ([5, 1, 0, 2], [70, 1, 3, 2], 2, 3, 96, 7, 0, 0),
-    ([3, 1, 0], [120, 900, 4], 1, 4, 512, 16, 50, 5),
-    ([7, 1], [200, 1000], 1, 2, 256, 64, 33, 3),
-    ([1, 1], [17, 16], 4, 5, 64, 8, 0, 0),
-    ([8], [8], 3, 1, 8, 1, 3, 1),
-    ([1] * 9, [15 * i + 1 for i in range(9)], 1, 7, 200, 5, 0, 0),
-    ([1, 2, 1, 0], [600, 601, 602, 3], 1, 3, 384, 24, 512, 4),
-    ([6, 0], [300, 1], 1, 2, 320, 48, 100, 40),
-    ([1], [3000], 2, 8, 512, 64, 2000, 200),
-]
-
-
-@pytest.mark.parametrize("counts,lens,nkh,group,hd,page,window,sinks", FEW)
-def test_chunk_attention_of_few_rows(ctx, counts, lens, nkh, group, hd, page, window, sinks):
-    case, q = _case(hd + sum(counts), counts, lens, nkh=nkh, group=group, hd=hd, page=page)
-    _check(ctx, case, q, window=window, sinks=sinks)
-
-
-@pytest.mark.parametrize("hd,group", [(64, 1), (256, 2), (512, 1), (512, 3)])
-def test_values_that_are_not_finite_in_steps_of_few_rows(ctx, hd, group):
-    counts, lens, window, sinks = [4, 1, 0, 0], [200, 40, 5, 9], 30, 3
-    case, q = _case(hd, counts, lens, nkh=1, group=group, hd=hd, page=16)
-    clean, lse0 = _attend(ctx, case, q, window=window, sinks=sinks)
-    plant = [(0, 198, 5, float("inf")), (0, 199, hd - 1, float("nan")), (0, 1, 0, -float("inf")), (0, 168, 9, float("inf")),
-             (0, 100, 4, float("nan")), (1, 39, 3, -float("inf"))]
-    for b, r, d, x in plant:
-        case.v[case.table_host[b, r // 16], r % 16, 0, d] = x
-    out, lse = _attend(ctx, case, q, window=window, sinks=sinks)
-    want = clean.double()
-    for b, r, d, x in plant:
-        for i in range(counts[b]):
-            pos = lens[b] - counts[b] + i
-            if r <= pos and (r > pos - window or r < sinks):
-                want[case.indptr_host[b] + i, :, d] += x
-    finite = want.isfinite()
-    assert torch.equal(lse, lse0) and torch.equal(out.isfinite(), finite) and torch.equal(out[finite], clean[finite])
-    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.isposinf(), want == float("inf"))
-
-
-def test_sequences_whose_rows_overlap_are_refused_where_they_do_not_fit(ctx):
-    """q_indptr that goes back and forth: each second sequence is in itself well formed, all together they are more than
-    num_tokens; nothing is written out of bounds."""
-    n, t = 40, 120
-    case, q = _case(7, [t], [300], nkh=1, group=8, hd=128, page=16)
-    table = case.table.expand(n, -1).contiguous()
-    lens = torch.full((n,), 300, dtype=torch.int32, device="cuda")
-    indptr = torch.tensor([0, t] * (n // 2) + [0], dtype=torch.int32, device="cuda")
-    out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda")
-    mass = torch.zeros((n, 1, 300), device="cuda")
-    ctx.chunk_attn_paged(q, case.k, case.v, table, lens, indptr, out, lse, scale=0.1, **_shape(case, q))
-    with pytest.raises(G4AError, match="do not fit"):
-        ctx.sync()
-    ctx.paged_key_mass(q, lse, case.k, table, lens, indptr, mass, scale=0.1, **_shape(case, q))
-    with pytest.raises(G4AError, match="do not fit"):
-        ctx.sync()
 
 
 @pytest.mark.parametrize("hd,counts,lens,window,sinks", [
@@ -653,3 +638,53 @@ def test_many_tiles_in_one_call(ctx):
     case, q = _case(4, [1500, 1300, 20, 900], [1500, 2000, 3500, 1000], nkh=4, group=48, hd=64, page=64)
     _check(ctx, case, q)
     _check_mass(ctx, case, q)
+
+
+@pytest.mark.parametrize("hd", [128, 256, 512])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 1.0])
+def test_scales(ctx, hd, scale):
+    """Scores that fall as the products rise, that are all alike, and that are not scaled; few rows and tiles of them."""
+    for counts, lens in (([1, 1], [300, 40]), ([70], [200])):
+        case, q = _case(hd, counts, lens, nkh=1, group=8, hd=hd, page=16, spread=0.5)
+        out, lse = _attend(ctx, case, q, scale=scale)
+        want, z, amp = chunk_ref(case, q, scale=scale)
+        vmax = max(float(v.abs().max()) for _, v in case.rows)
+        assert float((out.double() - want).abs().max()) <= attn_tolerance(amp, hd, 300, vmax)
+        assert float((lse.double() - z).abs().max()) <= lse_tolerance(amp, hd, 300, float(z.abs().max()))
+
+
+@pytest.mark.parametrize("counts,lens", [([1], [3000]), ([40], [90]), ([40], [30_000])])
+def test_log_sum_exps_may_be_left_out(ctx, counts, lens):
+    case, q = _case(1, counts, lens, nkh=1, group=8, hd=256, page=64)
+    want, _ = _attend(ctx, case, q, tail=0)  # (rows behind the last sequence may choose the other kernel)
+    out = torch.zeros_like(q)
+    ctx.chunk_attn_paged(q, case.k, case.v, case.table, case.lens_dev, case.indptr, out, scale=256 ** -0.5, **_shape(case, q))
+    ctx.sync()
+    assert torch.equal(out, want)
+
+
+def test_a_step_on_another_stream(ctx):
+    """Calls on the context's stream follow each other there, whatever the current stream does."""
+    with g4attn.Context(0) as c:
+        side = torch.cuda.Stream()
+        c.set_stream(side.cuda_stream)
+        case, q = _case(11, [50, 1], [3000, 700], nkh=2, group=4, hd=256, page=16)
+        out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda")
+        mass = torch.zeros((2, 2, 3000), device="cuda")
+        new = torch.zeros(2, dtype=torch.int32, device="cuda")
+        want, z, amp = chunk_ref(case, q, scale=256 ** -0.5)
+        torch.cuda.synchronize()
+        shape = _shape(case, q)
+        c.chunk_attn_paged(q, case.k, case.v, case.table, case.lens_dev, case.indptr, out, lse, scale=256 ** -0.5, **shape)
+        c.paged_key_mass(q, lse, case.k, case.table, case.lens_dev, case.indptr, mass, scale=256 ** -0.5, **shape)
+        got = mass_ref(case, q, z.float(), torch.zeros_like(mass), scale=256 ** -0.5)
+        c.sync()
+        assert float((out.double() - want).abs().max()) <= attn_tolerance(amp, 256, 3000, max(float(v.abs().max()) for _, v in case.rows))
+        for b, n in enumerate(case.lens):
+            # (lse is the kernel's own here: twice its error)
+            tol = mass_tolerance(amp, 256, 200, float(z.abs().max())) + 2 * lse_tolerance(amp, 256, 3000, float(z.abs().max()))
+            assert bool(((mass[b, :, :n] - got[b, :, :n]).abs() <= tol * got[b, :, :n]).all())
+        c.paged_kv_evict(case.k, case.v, case.table, case.lens_dev, mass, new, budget=500, recent_tokens=50, num_kv_heads=2,
+                         head_dim=256, page_size=16)
+        c.sync()
+        assert new.tolist() == [500, 500]
