@@ -79,6 +79,46 @@ __device__ __forceinline__ uint4 load_once(const __half* at) {
   return x;
 }
 
+// What CTA c does: sequence b, its parts, and kv head and part (kvh * parts + part) in `local`; b < 0: nothing.  A
+// sequence of n steps of keys (thread b says how many) has n / q parts, rounded up, `most` at most, with the smallest q
+// that lets all have one of the `ctas` CTAs (more than there are heads), and at least `least`.  `own` >= 0 asks for that
+// sequence's parts instead.  Up to THREADS sequences.
+struct Deal {
+  int b, parts, local;
+};
+template <int THREADS>
+__device__ __forceinline__ Deal deal_out(int n, int nkh, int ctas, int most, int least, int c, int own) {
+  __shared__ int sums[THREADS / 32], counts[THREADS / 32];
+  __shared__ Deal found;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int total = __reduce_add_sync(0xffffffffu, n), heads = __reduce_add_sync(0xffffffffu, n > 0 ? nkh : 0);
+  if (lane == 0) sums[warp] = total, counts[warp] = heads;
+  if (tid == 0) found.b = -1;
+  __syncthreads();
+  long long all = 0;
+  int items = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; i++) all += sums[i], items += counts[i];
+  const long long q = max((all * nkh + (ctas - items) - 1) / (long long)(ctas - items), (long long)least);
+  const int parts = n > 0 ? min((int)((n + q - 1) / q), most) : 0;
+  int incl = parts * nkh;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += t;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; i++)
+    if (i < warp) incl += sums[i];
+  const int begin = incl - parts * nkh;
+  if (own >= 0 ? tid == own : c >= begin && c < incl) found = Deal{tid, parts, c - begin};
+  __syncthreads();
+  return found;
+}
+
 }  // namespace g4a_chunk
 
 // Checks of the arguments that the two entry points share; fills p but for what each of them adds.

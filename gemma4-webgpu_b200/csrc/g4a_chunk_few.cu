@@ -55,52 +55,14 @@ __device__ __forceinline__ Steps steps_of(const FewParams& a, const Seq& s, int 
   r.parts = min(parts, (r.count() + groups - 1) / groups);  // a step for each of a CTA's groups at least
   return r;
 }
-// What CTA c does: sequence b, its parts, and kv head and part (kvh * parts + part) in `local`; b < 0: nothing.  A
-// sequence of n steps of 16 keys has n / q parts, rounded up, with the smallest q that lets all have a CTA; a thread
-// finds that for one sequence.  `own` >= 0 asks for that sequence's parts instead.
-struct Deal {
-  int b, parts, local;
-};
-template <int THREADS>
-__device__ __forceinline__ Deal deal_out(const FewParams& a, int c, int own, int groups) {
-  __shared__ int sums[THREADS / 32], counts[THREADS / 32];
-  __shared__ Deal found;
-  const ChunkParams& p = a.c;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int n = 0;
-  if (tid < p.batch) {
-    const Seq s = seq_of(p, tid, (long long)p.max_pages * p.page_size);
-    if (s.T > 0) {
-      const int lo = first_in_window(p, s.base());
-      n = (int)((min((long long)p.sinks, (long long)lo) + kStepKeys - 1) / kStepKeys) + (s.L + kStepKeys - 1) / kStepKeys - lo / kStepKeys;
-    }
-  }
-  const int total = __reduce_add_sync(0xffffffffu, n), heads = __reduce_add_sync(0xffffffffu, n > 0 ? p.nkh : 0);
-  if (lane == 0) sums[warp] = total, counts[warp] = heads;
-  if (tid == 0) found.b = -1;
-  __syncthreads();
-  long long all = 0;
-  int items = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; i++) all += sums[i], items += counts[i];
-  const long long q = max((all * p.nkh + (a.ctas - items) - 1) / (long long)(a.ctas - items), (long long)groups);
-  const int parts = n > 0 ? min((int)((n + q - 1) / q), a.splits) : 0;
-  int incl = parts * p.nkh;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int t = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += t;
-  }
-  __syncthreads();
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < THREADS / 32; i++)
-    if (i < warp) incl += sums[i];
-  const int begin = incl - parts * p.nkh;
-  if (own >= 0 ? tid == own : c >= begin && c < incl) found = Deal{tid, parts, c - begin};
-  __syncthreads();
-  return found;
+// The steps that thread b's sequence is dealt out by.
+__device__ __forceinline__ int steps_to_deal(const ChunkParams& p) {
+  if ((int)threadIdx.x >= p.batch) return 0;
+  const Seq s = seq_of(p, (int)threadIdx.x, (long long)p.max_pages * p.page_size);
+  if (s.T <= 0) return 0;
+  const int lo = first_in_window(p, s.base());
+  return (int)((min((long long)p.sinks, (long long)lo) + kStepKeys - 1) / kStepKeys) + (s.L + kStepKeys - 1) / kStepKeys -
+         lo / kStepKeys;
 }
 // Place of a row tile among all of the call's (a sequence has T group / 8 + 1 at most).
 __device__ __forceinline__ size_t tile_place(const ChunkParams& p, const Seq& s, int b, int tile) {
@@ -135,7 +97,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) chunk_few_kernel(const FewPara
   pdl_wait_primary();
   pdl_launch_dependents();
   if (a.ctas > 0) {
-    const Deal d = deal_out<kWarps * 32>(a, (int)blockIdx.x, -1, GROUPS);
+    const Deal d = deal_out<kWarps * 32>(steps_to_deal(p), p.nkh, a.ctas, a.splits, GROUPS, (int)blockIdx.x, -1);
     if (d.b < 0) return;
     b = d.b, kvh = d.local / d.parts, split = d.local - kvh * d.parts, most = d.parts;
   }
@@ -378,7 +340,7 @@ __global__ void __launch_bounds__(256) chunk_few_join_kernel(const FewParams a, 
   const int c = threadIdx.x & 7, row = (threadIdx.x >> 3) & 7, lanes = threadIdx.x >> 6, d = (int)blockIdx.x * 32 + c * 4;
   pdl_wait_primary();
   pdl_launch_dependents();
-  const int most = a.ctas > 0 ? deal_out<256>(a, 0, b, groups).parts : a.splits;
+  const int most = a.ctas > 0 ? deal_out<256>(steps_to_deal(p), p.nkh, a.ctas, a.splits, groups, 0, b).parts : a.splits;
   const Seq s = seq_of(p, b, (long long)p.max_pages * p.page_size);
   const int rows = s.T * p.group;
   for (int tile = 0; tile * kTile < rows; tile++) {

@@ -23,25 +23,53 @@ using namespace g4a_chunk;
 // ------------------------------------------------------------------------------------ few query rows
 
 constexpr int kFewWarps = 4;
-constexpr unsigned kFewRounds = 8;  // CTAs to an SM (24 sequences of 512 dims: 4, 8, 12: 74.5, 69.9, 71.6 us)
+constexpr int kHeld = 4;  // blocks of 8 query rows in shared memory
 constexpr int kNoKey = -1 - 0x7fffffff;
 
 // SEG: segments of 32 dims.  Lane 4 g + t holds dims 32 s + 8 t .. + 7 of keys g and g + 8 and of query row g.
+// `ctas`: CTAs to be dealt out, 0 (more sequences than threads): gridDim.x for each sequence and kv head.  A sequence's CTAs
+// take its steps in turn, so that they share the rows of a window.
 template <int SEG>
-__global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kernel(const ChunkParams p, int ctas) {
+  __shared__ __align__(16) uint4 q_s[kHeld][SEG][32];  // the first query rows as operands: [block][segment][lane]
+  __shared__ float z_s[kHeld * 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
+  int b = (int)(blockIdx.y / (unsigned)p.nkh), kvh = (int)(blockIdx.y % (unsigned)p.nkh);
+  int part = (int)blockIdx.x, parts = (int)gridDim.x;
+  const long long cap = min((long long)p.max_pages * p.page_size, p.mass_stride);
   pdl_wait_primary();
   pdl_launch_dependents();
-  const Seq s = seq_of(p, b, min((long long)p.max_pages * p.page_size, p.mass_stride));
-  const int base = s.base(), stride = (int)gridDim.x * kFewWarps * 16;
+  if (ctas > 0) {
+    const int n = (int)threadIdx.x < p.batch ? (seq_of(p, (int)threadIdx.x, cap).L + 15) / 16 : 0;
+    const Deal d = deal_out<kFewWarps * 32>(n, p.nkh, ctas, ctas, kFewWarps, (int)blockIdx.x, -1);
+    if (d.b < 0) return;
+    b = d.b, kvh = d.local / d.parts, part = d.local - kvh * d.parts, parts = d.parts;
+  }
+  const Seq s = seq_of(p, b, cap);
+  const int base = s.base(), stride = parts * kFewWarps * 16;
   const int* table = p.page_table + (size_t)b * p.max_pages;
   const __half* q = p.q + ((size_t)s.row0 * p.nqh + (size_t)kvh * p.group) * p.hd;
   const float* lse = p.lse + (size_t)s.row0 * p.nqh + (size_t)kvh * p.group;
   float* mass = p.mass + ((size_t)b * p.nkh + kvh) * p.mass_stride;
+  const long long rows = (long long)s.T * p.group;
+  // 16 bytes of dims d .. of query row r, and its log-sum-exp
+  auto query = [&](long long r, int d) {
+    if (r >= rows || d >= p.hd) return make_uint4(0, 0, 0, 0);
+    const int token = (int)((uint32_t)r / (uint32_t)p.group);
+    return __ldg(reinterpret_cast<const uint4*>(q + ((size_t)token * p.nqh + (size_t)(r - (long long)token * p.group)) * p.hd + d));
+  };
+  auto lse_of = [&](long long r) {
+    if (r >= rows) return -INFINITY;
+    const int token = (int)((uint32_t)r / (uint32_t)p.group);
+    return lse[(size_t)token * p.nqh + (size_t)(r - (long long)token * p.group)];
+  };
+  const int held = (int)min((rows + 7) / 8, (long long)kHeld);
+  for (int i = warp; i < held * SEG; i += kFewWarps) q_s[i / SEG][i % SEG][lane] = query(i / SEG * 8 + g, i % SEG * 32 + t * 8);
+  if (threadIdx.x < kHeld * 8) z_s[threadIdx.x] = lse_of(threadIdx.x);
+  __syncthreads();
   // the pages of keys g and g + 8, looked up one step ahead
   auto page_of = [&](long long key) { return key < s.L ? table[(uint32_t)key / (uint32_t)p.page_size] : kNoKey; };
-  const int k_first = ((int)blockIdx.x * kFewWarps + warp) * 16;
+  const int k_first = (part * kFewWarps + warp) * 16;
   int pages[2] = {page_of((long long)k_first + g), page_of((long long)k_first + g + 8)};
   for (long long at = k_first; at < s.L; at += stride) {
     const int k0 = (int)at;
@@ -73,27 +101,23 @@ __global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kern
     }
     const long long r_end = (long long)see.last * p.group;
     for (long long r0 = any ? (long long)see.first * p.group & ~7ll : r_end; r0 < r_end; r0 += 8) {
-      const bool live = r0 + g < (long long)s.T * p.group;
-      const int token = live ? (int)((uint32_t)(r0 + g) / (uint32_t)p.group) : 0;
-      const __half* row = q + ((size_t)token * p.nqh + (live ? (size_t)(r0 + g - (long long)token * p.group) : 0)) * p.hd;
+      const bool here = r0 < kHeld * 8;
       float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < SEG; e++) {
-        const int d = e * 32 + t * 8;
-        const uint4 x = live && d < p.hd ? __ldg(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0);
+        const uint4 x = here ? q_s[(uint32_t)r0 / 8][e][lane] : query(r0 + g, e * 32 + t * 8);
         mma_16x8x16(c, k[0][e].x, k[1][e].x, k[0][e].y, k[1][e].y, x.x, x.y);
         mma_16x8x16(c, k[0][e].z, k[1][e].z, k[0][e].w, k[1][e].w, x.z, x.w);
       }
 #pragma unroll
       for (int n = 0; n < 2; n++) {  // query rows r0 + 2 t + n
         const long long r = r0 + 2 * t + n;
-        if (r >= (long long)s.T * p.group) continue;
-        const int tok = (int)((uint32_t)r / (uint32_t)p.group);
-        const float z = lse[(size_t)tok * p.nqh + (size_t)(r - (long long)tok * p.group)];
+        const float z = here ? z_s[r] : lse_of(r);
         if (z == -INFINITY) continue;
+        const int pos = base + (int)((uint32_t)r / (uint32_t)p.group);
 #pragma unroll
         for (int h = 0; h < 2; h++)
-          if (sees(p, base + tok, k0 + g + 8 * h)) sum[h] += fast_exp2(fmaf(c[2 * h + n], p.scale_log2, -z * kLog2eC));
+          if (sees(p, pos, k0 + g + 8 * h)) sum[h] += fast_exp2(fmaf(c[2 * h + n], p.scale_log2, -z * kLog2eC));
       }
     }
 #pragma unroll
@@ -558,9 +582,16 @@ g4a_status launch_few(g4a_ctx* ctx, const ChunkParams& p) {
   g4a_prof_scope ps(ctx, G4A_PROF_KEY_MASS);
   const unsigned heads = (unsigned)p.batch * (unsigned)p.nkh;
   const long long rows = std::min<long long>((long long)p.page_size * p.max_pages, p.mass_stride);
-  const unsigned wide = (unsigned)std::min<long long>((rows + kFewWarps * 16 - 1) / (kFewWarps * 16),
-                                                      std::max(1u, kFewRounds * (unsigned)ctx->num_sms / heads));
-  const cudaError_t e = g4a_launch(mass_few_kernel<SEG>, dim3(wide, heads), dim3(kFewWarps * 32), 0, ctx->stream, true, p);
+  const long long most = (rows + kFewWarps * 16 - 1) / (kFewWarps * 16), round = (SEG > 8 ? 2ll : 4ll) * ctx->num_sms;
+  dim3 grid((unsigned)std::min(most, std::max(1ll, 2 * round / heads)), heads);
+  int ctas = 0;
+  if (p.batch <= kFewWarps * 32) {
+    // one round of CTAs, equal parts of the keys; two where the heads are many and the parts so few that one is uneven
+    // (64 sequences x 8 heads of 128 dims 123 us with one, 113 with two)
+    ctas = (int)std::min(std::max(2ll * heads > round ? 2 * round : round, heads + round / 2), heads * most + heads);
+    grid = dim3((unsigned)ctas);
+  }
+  const cudaError_t e = g4a_launch(mass_few_kernel<SEG>, grid, dim3(kFewWarps * 32), 0, ctx->stream, true, p, ctas);
   if (e != cudaSuccess) return g4a_cuda_fail(e, "launch mass_few_kernel");
   return G4A_OK;
 }
