@@ -7,9 +7,18 @@
 //   S [256 x KB]  = Q K^T    A = Q (each CTA's 128 rows), B = K block, half of its keys in each CTA
 //   O [256 x HDV] += P V     A = P from TMEM, where the scores were, B = V block, half of its dims in each CTA
 // One pass over the keys with a running row maximum m and sum l: p = 2^(s - m), rounded to f16 for the product with V
-// and summed unrounded; m follows the maximum lazily, and O is rescaled only when it is raised.  KB is 128 keys.  Heads of more than 256 dims: O takes 256 TMEM columns, so the dims of V are
-// halved between two pieces of work, each with the scores of its own (3/2 of the products, but nothing to be
-// exchanged, where two CTAs that split the dims have to add each other's partial scores); 64 keys, for Q takes 128 KB.
+// and summed unrounded; m follows the maximum lazily, and O is rescaled only when it is raised.  KB is 128 keys.
+// Heads of more than 256 dims: O takes 256 TMEM columns, so the dims of V are halved between two pieces of work, each
+// with the scores of its own (3/2 of the products, but nothing to be exchanged, where two CTAs that split the dims
+// have to add each other's partial scores); 64 keys, for Q takes 128 KB.
+//
+// What bounds it.  256 dims: the power limit (512 tokens x 8 heads over 131,000 rows: 450 us, 1.2 PFLOP/s).  512 dims: Q
+// comes from shared memory for every 64 keys (1,536 cycles for 1,024 of products), beside the half of the
+// scores that is computed twice (1,001 tokens x 8 heads over 20,003 rows: 450 us, 0.71 PFLOP/s, tensor pipe 64 % busy).
+// 128 dims: the softmax of a stage, 2,400 cycles for 1,024 of MMAs (six ragged pieces: 197 us, 0.66 PFLOP/s, 39 %): the
+// exp2 unit's 1,024, and waits, scores from TMEM, maxima and their exchange, which nothing overlaps.  Two sets of
+// warps that take whole stages in turn (237 us), or the next stage's maxima ahead of this one's weights (226), read the
+// scores twice and were slower.
 //
 // Warps of a CTA (16):
 //   0-7   softmax and epilogue: warps w and w + 4 have the same 32 rows (TMEM lanes), a thread is a row, and each takes
@@ -19,8 +28,9 @@
 //   10    in the pair's first CTA: issues the MMAs of both.  S of stage i + 1 before O of stage i, so that the
 //         softmax of a stage runs under the next stage's scores and the last one's product.
 //   11    tells the first CTA that a K block has landed in this one.
-//   12-15 load the queries (whole tokens by TMA, else row by row), and look through V blocks that not every row sees: a value that is not finite
-//         becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then they tell the first CTA.
+//   12-15 load the queries (whole tokens by TMA, else row by row), and look through V blocks that not every row sees: a
+//         value that is not finite becomes 0 (0 x inf is NaN), and the rows that see it get it in the epilogue.  Then
+//         they tell the first CTA.
 // Barriers that both CTAs arrive on lie in the first CTA.  Every wait is bounded; a thread that gives up sets the
 // abort flags of both CTAs and the error word, all waits then end at once, and both free their TMEM and leave.
 #include <float.h>

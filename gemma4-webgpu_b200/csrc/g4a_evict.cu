@@ -1,5 +1,7 @@
 // A paged cache brought down to a budget of rows (g4a_paged_kv_evict): for each sequence and kv head the first
 // rows, the last ones and the heaviest between stay and are moved together.  No reference counterpart.
+// Two kernels, the choice and the move.  One sequence of 131,000 rows of 512 dims to 16,384: 33 us, the latency of the choice
+// (24 us by itself with a cold L2) and then the move; 24 sequences x 4 heads of up to 9,000 rows to 4,097: 50 us, 6.2 TB/s.
 #include <algorithm>
 #include <atomic>
 
@@ -78,8 +80,8 @@ __device__ __forceinline__ int peek(const int* at, uint32_t rank) {
 // One cluster of CTAs per (sequence, kv head), each with a slice of the rows between the first and the last ones, in
 // order.  The border weight is found digit by digit (11, 11 and 10 bits from the top): every CTA counts its slice,
 // all read each other's counts through distributed shared memory.  Then a warp knows how many rows before its own are
-// kept, and writes the numbers of its kept rows in order.  Latency: three counts, seven meetings
-// of the cluster, and two more ways through the slice.
+// kept, and writes the numbers of its kept rows in order.  Latency: three counts, seven meetings of the cluster, and two
+// more ways through the slice.
 __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictParams p) {
   extern __shared__ uint32_t cache[];
   __shared__ int hist[3][kBinsE], sums[2][kBinsE], warp_sum[32], warp_gt[32], warp_tie[32], slice_gt, slice_tie, digit_s, need_s;
@@ -223,8 +225,8 @@ __global__ void __launch_bounds__(kThreadsE) evict_select_kernel(const EvictPara
 // work.  Blocks are taken by ticket, in order, and a block reads before it waits, so those that it waits for always get
 // on; the wait is bounded all the same (a block that gives up writes nothing and reports it).  A block is one warp, a lane
 // a row, and the copies are bulk ones, so an SM holds 200 KB of rows under way with next to no instructions (256 threads
-// with the rows in registers, 128 KB to an SM: 24 and 112 us instead of 22 and 76, with a cold L2, for 131,000 rows to 16,384 and for
-// 24 sequences x 4 heads).
+// with the rows in registers, 128 KB to an SM: 24 and 112 us instead of 22 and 76, with a cold L2, for 131,000 rows to
+// 16,384 and for 24 sequences x 4 heads).
 __global__ void __launch_bounds__(kRows) evict_move_kernel(const EvictParams p) {
   extern __shared__ __align__(128) unsigned char rows_s[];  // [2][32][hd] f16
   __shared__ uint64_t landed;

@@ -4,12 +4,16 @@
 // so K is read once more and V not at all.  Two kernels:
 //  - few query rows to a sequence (decode steps): a warp has 16 keys in registers, as the A operand of mma.sync
 //    m16n8k16, 8 query rows are its B operand.  The order of the dims in a product is free, so a lane loads 16
-//    consecutive bytes of its rows and uses them as they are: no shared memory, 8 or 16 KB in flight for each warp.
-//    Bound by the HBM.
+//    consecutive bytes of its rows and uses them as they are: no shared memory for K, 8 or 16 KB in flight for each
+//    warp.  The keys of all sequences are dealt in equal parts to one round of CTAs.  Bound by the HBM and by the ends
+//    of a step, when a warp multiplies and has nothing under way (24 ragged sequences of up to 16,000 rows of 512 dims:
+//    61 us, 4.5 TB/s).  Loading the next step's rows into registers as they are used, or by bulk copies into rings in
+//    shared memory, took 129 and 108 us.
 //  - chunks: S^T [256 keys x rows] = K Q^T by pairs of CTAs (tcgen05 cta_group::2), a thread is a key and adds up its
 //    weights in a register, so nothing is reduced across lanes; the row blocks of a key tile may be cut between
 //    pairs, and a last kernel adds the parts up in a fixed order.  Bound by the tensor cores and the exp2 unit
-//    together: a block of 128 keys x 128 rows of 256 dims takes 1,024 cycles of either.
+//    together: a block of 128 keys x 128 rows of 256 dims takes 1,024 cycles of either (515 tokens x 8 heads over
+//    32,000 rows: 74 us, 0.9 PFLOP/s, with 13 us of planning, start and join).
 #include <algorithm>
 #include <atomic>
 
@@ -103,11 +107,22 @@ __global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kern
     for (long long r0 = any ? (long long)see.first * p.group & ~7ll : r_end; r0 < r_end; r0 += 8) {
       const bool here = r0 < kHeld * 8;
       float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int e = 0; e < SEG; e++) {
-        const uint4 x = here ? q_s[(uint32_t)r0 / 8][e][lane] : query(r0 + g, e * 32 + t * 8);
+      auto product = [&](int e, const uint4& x) {
         mma_16x8x16(c, k[0][e].x, k[1][e].x, k[0][e].y, k[1][e].y, x.x, x.y);
         mma_16x8x16(c, k[0][e].z, k[1][e].z, k[0][e].w, k[1][e].w, x.z, x.w);
+      };
+      if (here) {
+#pragma unroll
+        for (int e = 0; e < SEG; e++) product(e, q_s[(uint32_t)r0 / 8][e][lane]);
+      } else {
+        const bool live = r0 + g < rows;
+        const int token = live ? (int)((uint32_t)(r0 + g) / (uint32_t)p.group) : 0;
+        const __half* row = q + ((size_t)token * p.nqh + (live ? (size_t)(r0 + g - (long long)token * p.group) : 0)) * p.hd;
+#pragma unroll
+        for (int e = 0; e < SEG; e++) {
+          const int d = e * 32 + t * 8;
+          product(e, live && d < p.hd ? __ldg(reinterpret_cast<const uint4*>(row + d)) : make_uint4(0, 0, 0, 0));
+        }
       }
 #pragma unroll
       for (int n = 0; n < 2; n++) {  // query rows r0 + 2 t + n
@@ -625,9 +640,11 @@ extern "C" g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const 
   p.decay = decay;
   if ((uint64_t)batch * num_kv_heads > 65535u)
     return g4a_fail(G4A_EINVAL, "%s: batch %u * num_kv_heads %u exceeds 65535", fn, batch, num_kv_heads);
-  // By the query rows of a sequence and kv head, on average.  Tiles of 256 keys against 16 keys to a warp, in us: 16 rows
-  // 52, 38 (32 sequences of 8,000 rows, 256 dims), 48, 28 (128 dims), 45, 50 (16, 512 dims), 15, 9.7 (one of 8,000), 16.5,
-  // 9.6 (32 of 1,000); 32 rows 52, 56; 48, 42; 45, 72; 15, 9.5; 17, 10; 64 rows 52, 96; 48, 71; 45, 117; 15, 12.5; 16, 16.
+  // By the query rows of a sequence and kv head, on average.  Tiles of 256 keys against 16 keys to a warp, in us:
+  //            32 sequences of 8,000 rows, 256 dims    128 dims    16, 512 dims    one of 8,000    32 of 1,000, 256 dims
+  //  16 rows   54, 31                                  49, 24      46, 41          14, 8.9         17, 9.1
+  //  32 rows   53, 44                                  49, 34      46, 55          14, 9.9         18, 12
+  //  64 rows   54, 101                                 49, 68      46, 109         14, 17          18, 20
   const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= (head_dim > 256 ? 16u : 32u) * (uint64_t)batch;
   if (head_dim > 256) return few ? launch_few<16>(ctx, p) : launch_chunk_mass<512>(fn, ctx, p);
   if (head_dim > 128) return few ? launch_few<8>(ctx, p) : launch_chunk_mass<256>(fn, ctx, p);
