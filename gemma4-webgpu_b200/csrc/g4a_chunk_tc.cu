@@ -15,7 +15,7 @@
 // What bounds it.  256 dims: the power limit (512 tokens x 8 heads over 131,000 rows: 450 us, 1.2 PFLOP/s).  512 dims: Q
 // comes from shared memory for every 64 keys (1,536 cycles for 1,024 of products), beside the half of the
 // scores that is computed twice (1,001 tokens x 8 heads over 20,003 rows: 450 us, 0.71 PFLOP/s, tensor pipe 64 % busy).
-// 128 dims: the softmax of a stage, 2,400 cycles for 1,024 of MMAs (six ragged pieces: 197 us, 0.66 PFLOP/s, 39 %): the
+// 128 dims: the softmax of a stage, about 2,500 cycles for 1,024 of MMAs (six ragged pieces: 197 us, 0.66 PFLOP/s, 39 %): the
 // exp2 unit's 1,024, and waits, scores from TMEM, maxima and their exchange, which nothing overlaps.  Two sets of
 // warps that take whole stages in turn (237 us), or the next stage's maxima ahead of this one's weights (226), read the
 // scores twice and were slower.

@@ -13,7 +13,7 @@
 //    weights in a register, so nothing is reduced across lanes; the row blocks of a key tile may be cut between
 //    pairs, and a last kernel adds the parts up in a fixed order.  Bound by the tensor cores and the exp2 unit
 //    together: a block of 128 keys x 128 rows of 256 dims takes 1,024 cycles of either (515 tokens x 8 heads over
-//    32,000 rows: 74 us, 0.9 PFLOP/s, with 13 us of planning, start and join).
+//    32,000 rows: 75 us, 0.9 PFLOP/s, the plan and the join with it; tensor pipe 51 % busy).
 #include <algorithm>
 #include <atomic>
 
