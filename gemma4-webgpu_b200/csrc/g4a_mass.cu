@@ -7,8 +7,8 @@
 //    consecutive bytes of its rows and uses them as they are: no shared memory for K, 8 or 16 KB in flight for each
 //    warp.  The keys of all sequences are dealt in equal parts to one round of CTAs.  Bound by the HBM and by the ends
 //    of a step, when a warp multiplies and has nothing under way (24 ragged sequences of up to 16,000 rows of 512 dims:
-//    61 us, 4.5 TB/s).  Loading the next step's rows into registers as they are used, or by bulk copies into rings in
-//    shared memory, took 129 and 108 us.
+//    50 us, 5.5 TB/s).  Loading the next step's rows into registers as they are used, or by bulk copies into rings in
+//    shared memory, took 129 and 108 us (of 67 then).
 //  - chunks: S^T [256 keys x rows] = K Q^T by pairs of CTAs (tcgen05 cta_group::2), a thread is a key and adds up its
 //    weights in a register, so nothing is reduced across lanes; the row blocks of a key tile may be cut between
 //    pairs, and a last kernel adds the parts up in a fixed order.  Bound by the tensor cores and the exp2 unit
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, SEG > 8 ? 2 : 4) mass_few_kern
 #pragma unroll
       for (int e = 0; e < SEG; e++) {
         const int d = e * 32 + t * 8;
-        k[h][e] = any && off[h] >= 0 && d < p.hd ? load_once(p.k + off[h] + d) : make_uint4(0, 0, 0, 0);
+        k[h][e] = load_once_if(p.k + off[h] + d, any && off[h] >= 0 && d < p.hd);
       }
     }
     const long long r_end = (long long)see.last * p.group;
