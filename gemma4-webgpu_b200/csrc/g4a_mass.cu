@@ -642,10 +642,10 @@ extern "C" g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const 
     return g4a_fail(G4A_EINVAL, "%s: batch %u * num_kv_heads %u exceeds 65535", fn, batch, num_kv_heads);
   // By the query rows of a sequence and kv head, on average.  Tiles of 256 keys against 16 keys to a warp, in us:
   //            32 sequences of 8,000 rows, 256 dims    128 dims    16, 512 dims    one of 8,000    32 of 1,000, 256 dims
-  //  16 rows   54, 31                                  49, 24      46, 41          14, 8.9         17, 9.1
-  //  32 rows   53, 44                                  49, 34      46, 55          14, 9.9         18, 12
-  //  64 rows   54, 101                                 49, 68      46, 109         14, 17          18, 20
-  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= (head_dim > 256 ? 16u : 32u) * (uint64_t)batch;
+  //  16 rows   54, 31                                  50, 24      46, 34          14, 8.6         17, 9.0
+  //  32 rows   54, 44                                  49, 34      46, 49          14, 10          17, 12
+  //  64 rows   54, 111                                 50, 68      46, 104         14, 18          17, 21
+  const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 32u * (uint64_t)batch;
   if (head_dim > 256) return few ? launch_few<16>(ctx, p) : launch_chunk_mass<512>(fn, ctx, p);
   if (head_dim > 128) return few ? launch_few<8>(ctx, p) : launch_chunk_mass<256>(fn, ctx, p);
   return few ? launch_few<4>(ctx, p) : launch_chunk_mass<128>(fn, ctx, p);
