@@ -651,6 +651,14 @@ def test_scales(ctx, hd, scale):
         vmax = max(float(v.abs().max()) for _, v in case.rows)
         assert float((out.double() - want).abs().max()) <= attn_tolerance(amp, hd, 300, vmax)
         assert float((lse.double() - z).abs().max()) <= lse_tolerance(amp, hd, 300, float(z.abs().max()))
+        before = torch.zeros((len(lens), 1, max(lens)), device="cuda")
+        got = before.clone()
+        torch.cuda.synchronize()
+        ctx.paged_key_mass(q, z.float(), case.k, case.table, case.lens_dev, case.indptr, got, scale=scale, **_shape(case, q))
+        ctx.sync()
+        want = mass_ref(case, q, z.float(), before, scale=scale)
+        tol = mass_tolerance(amp, hd, max(counts) * 8, float(z.abs().max()))
+        assert bool(((got.double() - want).abs() <= tol * want + 1e-37).all())
 
 
 @pytest.mark.parametrize("counts,lens", [([1], [3000]), ([40], [90]), ([40], [30_000])])
@@ -688,3 +696,45 @@ def test_a_step_on_another_stream(ctx):
                          head_dim=256, page_size=16)
         c.sync()
         assert new.tolist() == [500, 500]
+
+
+def test_two_contexts_at_once(ctx):
+    """Steps of two contexts on streams of their own, in flight together, give what each gives alone."""
+    jobs = []
+    for seed, hd, counts, lens in ((1, 128, [300, 1, 40], [2000, 900, 333]), (2, 512, [90], [5000]), (3, 256, [1] * 12, [800] * 12)):
+        case, q = _case(seed, counts, lens, nkh=2, group=4, hd=hd, page=16)
+        weights = torch.rand((len(lens), 2, max(lens)), generator=torch.Generator().manual_seed(seed)).cuda()
+        jobs.append((case, q, weights))
+
+    def step(c, case, q, weights):
+        out, lse, mass = torch.zeros_like(q), torch.zeros(q.shape[:2], device="cuda"), weights.clone()
+        k, v, new = case.k.clone(), case.v.clone(), torch.zeros(len(case.lens), dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        shape = _shape(case, q)
+
+        def run():
+            c.chunk_attn_paged(q, k, v, case.table, case.lens_dev, case.indptr, out, lse, scale=0.1, **shape)
+            c.paged_key_mass(q, lse, k, case.table, case.lens_dev, case.indptr, mass, scale=0.1, **shape)
+            c.paged_kv_evict(k, v, case.table, case.lens_dev, mass, new, budget=200, recent_tokens=20, num_kv_heads=2,
+                             head_dim=q.shape[2], page_size=16)
+        return run, (out, lse, mass, k, v, new)
+
+    with g4attn.Context(0) as a, g4attn.Context(0) as b:
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for c, s in zip((a, b), streams):
+            c.set_stream(s.cuda_stream)
+        for one in jobs:
+            for other in jobs:
+                alone = [step(ctx, *one), step(ctx, *other)]
+                for run, _ in alone:
+                    run()
+                    ctx.sync()
+                both = [step(a, *one), step(b, *other)]
+                for run, _ in both:
+                    run()
+                a.sync()
+                b.sync()
+                for (_, want), (_, got) in zip(alone, both):
+                    for x, y, name in zip(want, got, ("out", "lse", "mass", "k", "v", "new")):
+                        kind = torch.int16 if x.dtype == torch.float16 else torch.int32  # (unused rows of the pools are NaN)
+                        assert torch.equal(x.view(kind), y.view(kind)), name
