@@ -83,9 +83,10 @@ __device__ __forceinline__ bool clear_bad(uint32_t& w) {
   return w != was;
 }
 
-// SEG: 32-dim segments of a warp's share of a head; SHARE: warps that share a head's dims.
+// SEG: 32-dim segments of a warp's share of a head; SHARE: warps that share a head's dims.  Three CTAs to an SM where the
+// registers allow (64 ragged sequences of 128 dims 54 us, with two 63; with four, which spill, 66).
 template <int SEG, int SHARE>
-__global__ void __launch_bounds__(kWarps * 32, 2) chunk_few_kernel(const FewParams a) {
+__global__ void __launch_bounds__(kWarps * 32, SEG > 4 ? 2 : 3) chunk_few_kernel(const FewParams a) {
   constexpr int DIMS = SEG * 32, CH = DIMS / 64, GROUPS = kWarps / SHARE;
   constexpr int PITCH = DIMS + 4;  // floats from row to row where the warps meet
   const ChunkParams& p = a.c;
@@ -433,11 +434,16 @@ g4a_status launch(g4a_ctx* ctx, const ChunkParams& p) {
   uint64_t keys = cap;
   if (p.window != 0u) keys = std::min<uint64_t>(cap, (uint64_t)p.window + p.sinks + 4 * kStepKeys);
   const long long most = (long long)((keys + groups * kStepKeys - 1) / (groups * kStepKeys));
-  // Two CTAs to an SM are one round.  While the heads are fewer than that, half a round more than the heads deals the keys
-  // evenly enough (64 sequences of up to 8,000 keys x 4 heads of 128 dims: 195 us, twice the heads 214); with more heads
-  // it takes two to a head (64 x 8 heads: 322 us, heads and half a round 351).  A sequence has four times its share at most.
-  const long long room = 2ll * ctx->num_sms;
-  const long long ctas = heads < room ? std::max(room, heads + room / 2) : 2 * heads;
+  // One round of CTAs, equal parts, while the heads are few: half a round more than the heads at least, or the parts are
+  // too uneven.  With more heads there have to be more parts than CTAs at once:
+  //  - up to 128 dims four to a head from half a round on (64 ragged sequences x 4 heads 155 us, one round 181; x 8
+  //    heads 269, two to a head 286; as many equal ones 103 and 121, 198 and 237);
+  //  - above, two to a head from a round on (64 ragged sequences x 8 heads 322 us, one round 351), not before (x 4 heads
+  //    324 us, two to a head 355, though 50 x 4 heads 303 and 289).
+  // A sequence has four times its share at most.
+  const long long room = (SEG > 4 ? 2ll : 3ll) * ctx->num_sms;
+  const bool many = SEG > 4 ? heads >= room : 2 * heads >= room;
+  const long long ctas = many ? (SEG > 4 ? 2 : 4) * heads : std::max(room, heads + room / 2);
   if (p.batch <= kWarps * 32) {
     a.ctas = (int)std::min(ctas, heads * most + heads);
     a.splits = (int)std::min(most, 4 * ((ctas + heads - 1) / heads));
