@@ -118,9 +118,11 @@ extern "C" g4a_status g4a_chunk_attn_paged(g4a_ctx* ctx, const uint16_t* q, cons
   p.lse = lse;
   p.out = reinterpret_cast<__half*>(out);
   // By the query rows of a sequence and kv head, on average (the lengths are on the device).  Tiles of 256 rows against
-  // tiles of 8, in us: 8 rows 71, 54 (32 sequences of 8,000 rows, 256 dims), 105, 56 (16, 512 dims), 62, 35 (32, 128 dims),
-  // 23, 19 (one of 8,000), 29, 18 (32 of 1,000); 16 rows 71, 99; 107, 104; 62, 61; 23, 24; 29, 28; 32 rows 72, 188 for the
-  // first.
+  // tiles of 8, in us:
+  //            32 sequences of 8,000 rows, 256 dims    128 dims    16, 512 dims    one of 8,000    32 of 1,000, 256 dims
+  //   8 rows   70, 54                                  62, 33      105, 56         24, 15          28, 18
+  //  16 rows   71, 99                                  62, 58      105, 104        24, 24          27, 28
+  //  32 rows   73, 190                                 60, 105     107, 197        24, 42          28, 47
   const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 8u * (uint64_t)batch &&
                    (uint64_t)batch * num_kv_heads <= 65535u;
   return few ? g4a_chunk_few_launch(ctx, p) : g4a_chunk_tc_launch(ctx, p);
