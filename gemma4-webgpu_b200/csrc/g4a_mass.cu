@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kThreadsM, 1)
     for (int s = 0; s < kScoreBufs; s++) {
       mbar_init(&s_done[s], 2);
       mbar_init(&s_free[s], 8);
-      mbar_init(&lse_free[s], 4);
     }
+    for (int s = 0; s < kLseBufs; s++) mbar_init(&lse_free[s], 4);
     for (int s = 0; s < 2; s++) {
       mbar_init(&sum_full[s], 4);
       mbar_init(&sum_free[s], 4);
