@@ -404,6 +404,8 @@ __global__ void __launch_bounds__(kThreadsC, 1)
       }
       if (bad && live) add_taken_out<HD>(p, w, pos, out_row, part, row, half);
       tc_fence_before();
+      // the next queries are copied by TMA to where this output has been
+      if (!C::OWN_STAGING) fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
         if (!C::OWN_STAGING) mbar_arrive(staged);  // (before o_free, without which no warp gets through another piece)
