@@ -199,8 +199,10 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_small_kernel(const Pl
   __syncthreads();
   if (items == 0 || entries > a.max_entries) {
     if (tid == 0) a.plan->cuts = 0;
-    if (tid == 0 && items != 0) atomicExch(p.err, G4A_DEVERR_TREE);
-    if (MASS && tid < p.batch) a.seqs[tid] = make_int4(0, -1, 0, 0);
+    if (items != 0) {  // (no items: the masses' rows fade all the same)
+      if (tid == 0) atomicExch(p.err, G4A_DEVERR_TREE);
+      if (MASS && tid < p.batch) a.seqs[tid] = make_int4(0, -1, 0, 0);
+    }
     return;
   }
   // ---- tiles: a thread's sequence is the last one whose entries begin at or before it (those without any share a begin)
