@@ -30,7 +30,7 @@ using namespace g4a_chunk;
 
 constexpr int kWarps = 4, kStepKeys = 16, kTile = 8;  // warps of a CTA; keys of a step; query rows of a tile
 constexpr int kNoKey = -1 - 0x7fffffff;
-constexpr float kRaiseF = 15.0f, kFirstF = -3.0f, kLaterF = 1.0f, kUnseenF = -FLT_MAX;
+constexpr float kRaiseF = 15.0f, kBelowF = 3.0f, kUnseenF = -FLT_MAX;  // (of m, as in the tcgen05 kernel)
 
 struct FewParams {
   ChunkParams c;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kWarps * 32, SEG > 4 ? 2 : 3) chunk_few_kernel
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const bool raise = top > m + kRaiseF;
       if (__any_sync(0xffffffffu, raise)) {
-        const float m_new = raise ? top + (m == kUnseenF ? kFirstF : kLaterF) : m;
+        const float m_new = raise ? top - kBelowF : m;
         const float fall = raise ? (m == kUnseenF ? 0.f : fast_exp2(m - m_new)) : 1.f;
         l *= fall;
         m = m_new;

@@ -48,12 +48,13 @@ using namespace g4a_chunk;
 constexpr int kThreadsC = 512;
 constexpr int kSoft = 8, kLoadK = 8, kLoadV = 9, kMma = 10, kTellK = 11, kGuard = 12;
 constexpr int kCtaRows = 128;
-// Weights are p = 2^(s - m).  A score above m + 15 (f16 ends at 2^16) raises m: to 3 below the maximum at the row's first
-// scores, to 1 above it later on, so the largest weight is 2^-1 at least, and f16's rounding of one is off by 2^-11 of it
-// or 2^-25.  A raise costs the pair a stage's time (O has to be at rest to be rescaled), so m does not follow the maximum
-// closely: with m kept 7 below the maximum and raised at 2^8 past it, 512 tokens over 131,000 rows took 591 us instead
-// of 447, six ragged chunks of heads of 128 dims 213 instead of 190.
-constexpr float kRaiseC = 15.0f, kFirstC = -3.0f, kLaterC = 1.0f;
+// Weights are p = 2^(s - m).  A score above m + 15 (f16 ends at 2^16) raises m to 3 below it, so the largest weight is 2^3 at
+// least, and f16's rounding of one is off by 2^-11 of it or, below 2^-14, by 2^-25, which is 2^-28 of the largest.  A raise costs
+// the pair a stage's time (O has to be at rest to be rescaled), so m does not follow the maximum closely: with m kept 7 below
+// the maximum and raised at 2^8 past it, 512 tokens over 131,000 rows took 591 us instead of 447, six ragged chunks of
+// heads of 128 dims 213 instead of 190.  With later raises to 1 above the maximum, which leave the most room, both took
+// the same time as now, and one row found late left 131,000 rows at 2^-24.2 of it no weight at all.
+constexpr float kRaiseC = 15.0f, kBelowC = 3.0f;
 constexpr float kUnseenC = -FLT_MAX;  // m of a row that has seen nothing yet (any finite score raises it)
 constexpr int kBadTags = 8;
 
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kThreadsC, 1)
         if (!ok) break;
         const bool raise = top > m + kRaiseC;
         if (__any_sync(0xffffffffu, raise)) {  // (both halves agree)
-          const float m_new = raise ? top + (m == kUnseenC ? kFirstC : kLaterC) : m;
+          const float m_new = raise ? top - kBelowC : m;
           const float fall = raise ? (m == kUnseenC ? 0.f : fast_exp2(m - m_new)) : 1.f;
           l *= fall;
           m = m_new;
