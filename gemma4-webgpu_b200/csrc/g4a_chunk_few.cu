@@ -11,8 +11,10 @@
 //                               leaves in a lane (row g, keys 2 t, 2 t + 1) is the operand that the second one wants.
 // A warp has 16 KB under way (K and V of 16 keys, 256 dims), an SM 128 KB, more than the HBM's latency needs.  Heads of
 // more than 256 dims: two warps share 16 keys, half of the dims each, and add up their halves of the scores.
-// The sequences' keys are dealt to the CTAs in equal parts, as many CTAs as the SMs hold at once; the warps of a CTA
-// meet in shared memory, the parts of a row tile in a second kernel.  Softmax as in the tcgen05 kernel: m follows the
+// The sequences' keys are dealt to the CTAs in equal parts, as many CTAs as the SMs hold at once, but no sequence gets more
+// than four times its share of the CTAs (the partial results have places by that; one sequence of 131,000 rows takes 46 us,
+// with 63 of 500 beside it, which leave it 20 CTAs, 232); the warps of a CTA meet in shared memory, the parts of a row tile
+// in a second kernel.  Softmax as in the tcgen05 kernel: m follows the
 // maximum lazily, p rounded to f16 for the product with V and summed unrounded.
 // 64 decode sequences of up to 12,000 rows of 256 dims: 106 us, 5.0 TB/s; one token over 512 rows of a window: 10.6 us,
 // the two kernels' latency.  Fetching the next step into the L2 ahead made the first 309 us.

@@ -12,7 +12,8 @@
 // with the scores of its own (3/2 of the products, but nothing to be exchanged, where two CTAs that split the dims
 // have to add each other's partial scores); 64 keys, for Q takes 128 KB.
 //
-// What bounds it.  256 dims: the power limit (512 tokens x 8 heads over 131,000 rows: 450 us, 1.2 PFLOP/s).  512 dims: Q
+// What bounds it.  256 dims: the clock that the power limit leaves (512 tokens x 8 heads over 131,000 rows: 594,000 cycles with
+// the tensor pipe 79 % busy; 458 us, 1.2 PFLOP/s, in calls for seconds on end at 1,000 W, 388 in short bursts).  512 dims: Q
 // comes from shared memory for every 64 keys (1,536 cycles for 1,024 of products), beside the half of the
 // scores that is computed twice (1,001 tokens x 8 heads over 20,003 rows: 450 us, 0.71 PFLOP/s, tensor pipe 64 % busy).
 // 128 dims: the softmax of a stage, about 2,500 cycles for 1,024 of MMAs (six ragged pieces: 197 us, 0.66 PFLOP/s, 39 %): the

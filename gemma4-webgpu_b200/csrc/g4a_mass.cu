@@ -651,6 +651,8 @@ extern "C" g4a_status g4a_paged_key_mass(g4a_ctx* ctx, const uint16_t* q, const 
   //  16 rows   54, 31                                  50, 24      46, 34          14, 8.6         17, 9.0
   //  32 rows   54, 44                                  49, 34      46, 49          14, 10          17, 12
   //  64 rows   54, 111                                 50, 68      46, 104         14, 18          17, 21
+  // It is a mean, and the keys are dealt without a look at how many rows read them: 63 sequences with one token and one with 190,
+  // 32,000 rows of 256 dims, 8 heads, take 18.9 ms in one call, 164 and 38 us in two.
   const bool few = (uint64_t)num_tokens * (uint64_t)p.group <= 32u * (uint64_t)batch;
   if (head_dim > 256) return few ? launch_few<16>(ctx, p) : launch_chunk_mass<512>(fn, ctx, p);
   if (head_dim > 128) return few ? launch_few<8>(ctx, p) : launch_chunk_mass<256>(fn, ctx, p);
