@@ -122,8 +122,11 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag, err, G4A_DEVERR_WAIT_MMA));
 }
 
-// 16 or 32 consecutive TMEM columns of this warp's 32 lanes; the registers may be used after
+// 1, 16 or 32 consecutive TMEM columns of this warp's 32 lanes; the registers may be used after
 // tmem_landed() has named them.
+__device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void tmem_get(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -152,6 +155,7 @@ __device__ __forceinline__ void tmem_landed(uint32_t (&r)[W]) {
 #pragma unroll
   for (int n = 0; n < W; n++) asm volatile("" : "+r"(r[n]));
 }
+__device__ __forceinline__ void tmem_landed(uint32_t& r) { asm volatile("" : "+r"(r)); }
 // Registers of a warpgroup's threads, up or down to R.
 template <int R>
 __device__ __forceinline__ void regs_up() {
