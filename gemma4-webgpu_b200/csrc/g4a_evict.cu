@@ -1,8 +1,8 @@
 // A paged cache brought down to a budget of rows (g4a_paged_kv_evict): for each sequence and kv head the first
 // rows, the last ones and the heaviest between stay and are moved together.  No reference counterpart.
 // Two kernels, the choice and the move.  One sequence of 131,000 rows of 512 dims to 16,384: 33 us, the latency of the choice
-// (24 us by itself with a cold L2) and then the move; 24 sequences x 4 heads of up to 9,000 rows to 4,097: 49 to 51 us,
-// 6.1 TB/s, and 61 once on another card.
+// (24 us by itself with a cold L2) and then the move; 24 sequences x 4 heads of up to 9,000 rows to 4,097: 49 to 52 us,
+// 6.0 TB/s, and 61 once on another card.
 #include <algorithm>
 #include <atomic>
 

@@ -7,7 +7,7 @@
 //    consecutive bytes of its rows and uses them as they are: no shared memory for K, 8 or 16 KB in flight for each
 //    warp.  The keys of all sequences are dealt in equal parts to one round of CTAs.  Bound by the HBM and by the ends
 //    of a step, when a warp multiplies and has nothing under way (24 ragged sequences of up to 16,000 rows of 512 dims:
-//    50 us, 5.5 TB/s).  Loading the next step's rows into registers as they are used, or by bulk copies into rings in
+//    51 us, 5.4 TB/s).  Loading the next step's rows into registers as they are used, or by bulk copies into rings in
 //    shared memory, took 129 and 108 us (of 67 then).
 //  - chunks: S^T [256 keys x rows] = K Q^T by pairs of CTAs (tcgen05 cta_group::2), a thread is a key and adds up its
 //    weights in a register, so nothing is reduced across lanes; the row blocks of a key tile may be cut between
